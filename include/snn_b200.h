@@ -384,6 +384,112 @@ int snn_propagate_static(const int32_t* post, const float* w, int64_t n_pre, int
                          const uint8_t* spikes, int32_t* acc, int64_t n_post, int32_t frac_bits,
                          void* stream);
 
+/* ---- token drive and leaky scans ---------------------------------------
+ * Operators on device tensors for models that are trained beside, or read out
+ * from, a spiking network: the drive rows of a token stream, and leaky
+ * (gated) integration along whole sequences.  No counterpart in the
+ * reference, which drives its neurons one-hot (src/stage2e/input_encoding.cu:
+ * 192-203) and advances its leaky potentials and traces a step at a time.
+ * All pointers are device pointers of the current device; the calls are
+ * asynchronous on `stream` (a cudaStream_t, NULL = legacy default stream),
+ * allocate nothing, keep nothing between calls and may be captured into CUDA
+ * graphs.  The tensors of concurrent calls are only read by both, or differ.
+ * Errors: SNN_ERR_* codes with the message in snn_last_error(NULL). */
+
+/* element types */
+#define SNN_F32 0
+#define SNN_BF16 1
+#define SNN_F16 2
+/* token types */
+#define SNN_U8 8
+#define SNN_I32 9
+#define SNN_I64 10
+
+/* out[i, :] = scale * table[tokens[i], :] for i < n: the product in f32,
+ * rounded once to out_type.  table is [vocab, dim], out [n, dim], both with
+ * unit column stride and the given row strides in elements (< 2^32; of what is
+ * written >= dim).  A token
+ * outside [0, vocab) gives a row of zeros.  n <= 2^30, vocab < 2^31. */
+int snn_embed(const void* tokens, int32_t tok_type, int64_t n, const void* table,
+              int32_t table_type, int64_t vocab, int64_t dim, int64_t table_stride, float scale,
+              void* out, int32_t out_type, int64_t out_stride, void* stream);
+
+/* The gradient of snn_embed for the table:
+ *   dtable[v, :] = scale * sum of dy[i, :] over the i with tokens[i] == v
+ * (added to what dtable holds when accumulate is non-zero; rows that do not
+ * occur are then not touched, otherwise they become zero).  Tokens outside
+ * [0, vocab) contribute nothing.  The positions are sorted by token and summed in
+ * f32 in an order that depends on the tokens, n and dim alone, so equal calls give
+ * equal bits; rounded once to dtable_type.  work: work_bytes bytes of device
+ * memory, 256-byte aligned, at least what snn_embed_grad_workspace says for
+ * the same n, vocab and dim; it is free again when the call's work on `stream`
+ * is done.  n <= 2^30, vocab < 2^31. */
+int snn_embed_grad_workspace(int64_t n, int64_t vocab, int64_t dim, int64_t* bytes);
+int snn_embed_grad(const void* tokens, int32_t tok_type, int64_t n, const void* dy,
+                   int32_t dy_type, int64_t dim, int64_t dy_stride, float scale, void* dtable,
+                   int32_t dtable_type, int64_t vocab, int64_t dtable_stride, int32_t accumulate,
+                   void* work, int64_t work_bytes, void* stream);
+
+/* Leaky scan: along every sequence, for every channel,
+ *   h_t = a_t h_{t-1} + u_t,   y_t = h_t,   u_t = x_t, or (1 - a_t) x_t with SNN_SCAN_LEAKY
+ * with a_t the gate, or 1 / (1 + exp(-gate)) with SNN_SCAN_LOGIT.  The state
+ * is f32; y is rounded once.
+ * Layout: dense (offsets NULL): n_seq sequences of n_steps steps; packed
+ * (offsets set): n_steps rows in all, sequence s the rows
+ * [offsets[s], offsets[s + 1]) of every tensor (int64[n_seq + 1] in device
+ * memory, ascending within [0, n_steps]; entries are clamped to that).  Rows
+ * of no sequence are not read and not written.  A sequence may be empty: its
+ * final state is its initial one.
+ * Strides are any of which rows that are written do not overlap (time-major
+ * rows too); what is only read may be broadcast by a stride of 0.  Outputs
+ * must not overlap inputs, but for h and dh0 below.
+ * x, y, gate are [.., channels] rows of element type `type`, unit channel
+ * stride; with SNN_SCAN_RASTER x is the packed spike raster of snn_run
+ * (uint32 words, bit c % 32 of word c / 32) and strides are in words; with
+ * SNN_SCAN_CHANNEL the gate is one f32 per channel. */
+#define SNN_SCAN_LOGIT 1
+#define SNN_SCAN_LEAKY 2
+#define SNN_SCAN_CHANNEL 4
+#define SNN_SCAN_RASTER 8
+typedef struct snn_scan {
+    int32_t type;            /* SNN_F32 / SNN_BF16 / SNN_F16                     */
+    int32_t flags;           /* SNN_SCAN_*                                       */
+    int64_t n_seq;
+    int64_t n_steps;         /* dense: steps of a sequence; packed: rows in all  */
+    int64_t n_channels;
+    const int64_t* offsets;  /* NULL = dense                                     */
+} snn_scan;
+typedef struct snn_rows {    /* one tensor of rows                               */
+    void* data;
+    int64_t seq_stride;      /* elements between sequences (dense)               */
+    int64_t step_stride;     /* elements between steps (rows)                    */
+} snn_rows;
+
+/* h0 (nullable: zeros) and h (nullable) are f32 [n_seq, n_channels]; h may be
+ * h0 itself, so that one state is carried from call to call.  saved (nullable)
+ * receives the states that snn_leaky_scan_grad starts its blocks of steps from:
+ * snn_leaky_scan_saved(desc) floats. */
+int snn_leaky_scan_saved(const snn_scan* desc, int64_t* floats);
+int snn_leaky_scan(const snn_scan* desc, const snn_rows* gate, const snn_rows* x, const float* h0,
+                   const snn_rows* y, float* h, float* saved, void* stream);
+
+/* Gradients of snn_leaky_scan, from the gradients dy of y (nullable) and dh
+ * of the final state (nullable; not both NULL):
+ *   g_t = dy_t + a_{t+1} g_{t+1}  (the last step: dy_t + dh)
+ *   dx_t = g_t, or (1 - a_t) g_t;   da_t = g_t h_{t-1}, or g_t (h_{t-1} - x_t);
+ *   dgate = da, or da a (1 - a) with SNN_SCAN_LOGIT;   dh0 = a_1 g_1.
+ * dgate (nullable) has the gate's form: rows, or with SNN_SCAN_CHANNEL f32
+ * [n_channels], the sum over all steps of all sequences in an order that
+ * depends on the sizes alone.  dx (nullable, NULL with SNN_SCAN_RASTER) and dh0
+ * (nullable, f32 [n_seq, n_channels], may be dh itself) as their inputs; rows of no sequence are
+ * not written.  saved is what the forward call wrote.  work: as for
+ * snn_embed_grad, of the size that snn_leaky_scan_grad_workspace says. */
+int snn_leaky_scan_grad_workspace(const snn_scan* desc, int64_t* bytes);
+int snn_leaky_scan_grad(const snn_scan* desc, const snn_rows* gate, const snn_rows* x,
+                        const float* saved, const snn_rows* dy, const float* dh,
+                        const snn_rows* dgate, const snn_rows* dx, float* dh0, void* work,
+                        int64_t work_bytes, void* stream);
+
 /* Seeded synthetic UTF-8 byte stream: a fraction p_cjk of characters are
  * CJK code points U+4E00..U+9FFF drawn Zipf(zipf_s) by rank (rank -> code
  * point through a seeded permutation), 3 bytes each; the rest are ASCII

@@ -36,6 +36,25 @@ int guard(snn_ctx* ctx, F&& f) {
     }
 }
 
+// the entry points without a context: the message goes to snn_last_error(NULL)
+template <typename F>
+int guard_op(F&& f) {
+    try {
+        f();
+        g_create_err.clear();
+        return SNN_OK;
+    } catch (const snnb::Error& e) {
+        g_create_err = e.what();
+        return e.code;
+    } catch (const std::bad_alloc&) {
+        g_create_err = "host allocation failed";
+        return SNN_ERR_OOM;
+    } catch (const std::exception& e) {
+        g_create_err = e.what();
+        return SNN_ERR_STATE;
+    }
+}
+
 snn_topology_spec reference_columns(int32_t n_columns) {
     snn_topology_spec s;
     memset(&s, 0, sizeof(s));
@@ -373,6 +392,60 @@ int snn_propagate_static(const int32_t* post, const float* w, int64_t n_pre, int
         g_create_err = e.what();
         return SNN_ERR_STATE;
     }
+}
+
+int snn_embed(const void* tokens, int32_t tok_type, int64_t n, const void* table,
+              int32_t table_type, int64_t vocab, int64_t dim, int64_t table_stride, float scale,
+              void* out, int32_t out_type, int64_t out_stride, void* stream) {
+    return guard_op([&] {
+        snnb::embed(tokens, tok_type, n, table, table_type, vocab, dim, table_stride, scale, out, out_type,
+                    out_stride, (cudaStream_t)stream);
+    });
+}
+
+int snn_embed_grad_workspace(int64_t n, int64_t vocab, int64_t dim, int64_t* bytes) {
+    return guard_op([&] {
+        SNN_REQUIRE(bytes, SNN_ERR_ARG, "null result");
+        *bytes = snnb::embed_grad_workspace(n, vocab, dim);
+    });
+}
+
+int snn_embed_grad(const void* tokens, int32_t tok_type, int64_t n, const void* dy,
+                   int32_t dy_type, int64_t dim, int64_t dy_stride, float scale, void* dtable,
+                   int32_t dtable_type, int64_t vocab, int64_t dtable_stride, int32_t accumulate,
+                   void* work, int64_t work_bytes, void* stream) {
+    return guard_op([&] {
+        snnb::embed_grad(tokens, tok_type, n, dy, dy_type, dim, dy_stride, scale, dtable, dtable_type, vocab,
+                         dtable_stride, accumulate, work, work_bytes, (cudaStream_t)stream);
+    });
+}
+
+int snn_leaky_scan_saved(const snn_scan* desc, int64_t* floats) {
+    return guard_op([&] {
+        SNN_REQUIRE(floats, SNN_ERR_ARG, "null result");
+        *floats = snnb::leaky_scan_saved(desc);
+    });
+}
+
+int snn_leaky_scan(const snn_scan* desc, const snn_rows* gate, const snn_rows* x, const float* h0,
+                   const snn_rows* y, float* h, float* saved, void* stream) {
+    return guard_op([&] { snnb::leaky_scan(desc, gate, x, h0, y, h, saved, (cudaStream_t)stream); });
+}
+
+int snn_leaky_scan_grad_workspace(const snn_scan* desc, int64_t* bytes) {
+    return guard_op([&] {
+        SNN_REQUIRE(bytes, SNN_ERR_ARG, "null result");
+        *bytes = snnb::leaky_scan_grad_workspace(desc);
+    });
+}
+
+int snn_leaky_scan_grad(const snn_scan* desc, const snn_rows* gate, const snn_rows* x,
+                        const float* saved, const snn_rows* dy, const float* dh,
+                        const snn_rows* dgate, const snn_rows* dx, float* dh0, void* work,
+                        int64_t work_bytes, void* stream) {
+    return guard_op([&] {
+        snnb::leaky_scan_grad(desc, gate, x, saved, dy, dh, dgate, dx, dh0, work, work_bytes, (cudaStream_t)stream);
+    });
 }
 
 }  // extern "C"

@@ -113,5 +113,19 @@ void propagate(const int32_t* post, const float* w, int64_t n_pre, int32_t fanou
 void propagate_static(const int32_t* post, const float* w, int64_t n_pre, int32_t fanout,
                       const uint8_t* spikes, int32_t* acc, int64_t n_post, int32_t frac_bits,
                       cudaStream_t stream);
+void embed(const void* tokens, int32_t tok_type, int64_t n, const void* table, int32_t table_type, int64_t vocab,
+           int64_t dim, int64_t table_stride, float scale, void* out, int32_t out_type, int64_t out_stride,
+           cudaStream_t stream);
+int64_t embed_grad_workspace(int64_t n, int64_t vocab, int64_t dim);
+void embed_grad(const void* tokens, int32_t tok_type, int64_t n, const void* dy, int32_t dy_type, int64_t dim,
+                int64_t dy_stride, float scale, void* dtable, int32_t dtable_type, int64_t vocab,
+                int64_t dtable_stride, int32_t accumulate, void* work, int64_t work_bytes, cudaStream_t stream);
+int64_t leaky_scan_saved(const snn_scan* desc);
+int64_t leaky_scan_grad_workspace(const snn_scan* desc);
+void leaky_scan(const snn_scan* desc, const snn_rows* gate, const snn_rows* x, const float* h0, const snn_rows* y,
+                float* h, float* saved, cudaStream_t stream);
+void leaky_scan_grad(const snn_scan* desc, const snn_rows* gate, const snn_rows* x, const float* saved,
+                     const snn_rows* dy, const float* dh, const snn_rows* dgate, const snn_rows* dx, float* dh0,
+                     void* work, int64_t work_bytes, cudaStream_t stream);
 
 }  // namespace snnb

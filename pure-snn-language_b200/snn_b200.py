@@ -29,6 +29,7 @@ MODEL_STAGE2E, MODEL_STAGE0, MODEL_PROP = 0, 1, 2
 PROP_PLAIN, PROP_STDP, PROP_STP = 0, 1, 2
 PRESET_REF, PRESET_BASELINE = 0, 1
 CORPUS_TEXT_FILTER = 1
+SCAN_LOGIT, SCAN_LEAKY, SCAN_CHANNEL, SCAN_RASTER = 1, 2, 4, 8
 FMT_NATIVE, FMT_SNN2_V1, FMT_SCKP_V2, FMT_RAW_F32 = 0, 1, 2, 3
 
 STATE = {
@@ -117,13 +118,24 @@ class Profile(C.Structure):
                             for i in range(k)}}
 
 
+class Scan(C.Structure):
+    _fields_ = [("type", C.c_int32), ("flags", C.c_int32), ("n_seq", C.c_int64),
+                ("n_steps", C.c_int64), ("n_channels", C.c_int64), ("offsets", C.c_void_p)]
+
+
+class Rows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("seq_stride", C.c_int64), ("step_stride", C.c_int64)]
+
+
 EXPORTS = ["snn_config_init", "snn_topology_init", "snn_create", "snn_destroy",
            "snn_last_error", "snn_version", "snn_build_columns", "snn_set_corpus", "snn_step",
            "snn_run", "snn_synchronize", "snn_get_spikes", "snn_get_state", "snn_get_counters",
            "snn_set_dopamine", "snn_set_e0", "snn_save", "snn_load", "snn_stream_generate",
            "snn_set_profiling", "snn_get_profile", "snn_propagate", "snn_propagate_static",
            "snn_nccl_unique_id", "snn_set_shard", "snn_shard_plan", "snn_semantic_eval",
-           "snn_set_corpus_ex", "snn_load_text_corpus", "snn_byte_classes"]
+           "snn_set_corpus_ex", "snn_load_text_corpus", "snn_byte_classes", "snn_embed",
+           "snn_embed_grad", "snn_embed_grad_workspace", "snn_leaky_scan", "snn_leaky_scan_saved",
+           "snn_leaky_scan_grad", "snn_leaky_scan_grad_workspace"]
 
 _lib = None
 _lib_refmath = None
@@ -178,6 +190,16 @@ def _load(path):
     L.snn_propagate_static.argtypes = L.snn_propagate.argtypes
     L.snn_nccl_unique_id.argtypes = [vp, C.c_int64]
     L.snn_set_shard.argtypes = [vp, C.c_int32, C.c_int32, vp, C.c_int64]
+    i32, i64 = C.c_int32, C.c_int64
+    L.snn_embed.argtypes = [vp, i32, i64, vp, i32, i64, i64, i64, C.c_float, vp, i32, i64, vp]
+    L.snn_embed_grad_workspace.argtypes = [i64, i64, i64, vp]
+    L.snn_embed_grad.argtypes = [vp, i32, i64, vp, i32, i64, i64, C.c_float, vp, i32, i64, i64,
+                                 i32, vp, i64, vp]
+    ps, pr = C.POINTER(Scan), C.POINTER(Rows)
+    L.snn_leaky_scan_saved.argtypes = [ps, vp]
+    L.snn_leaky_scan.argtypes = [ps, pr, pr, vp, pr, vp, vp, vp]
+    L.snn_leaky_scan_grad_workspace.argtypes = [ps, vp]
+    L.snn_leaky_scan_grad.argtypes = [ps, pr, pr, vp, pr, vp, pr, pr, vp, vp, i64, vp]
     L.snn_shard_plan.argtypes = [C.POINTER(TopologySpec), C.c_int32, C.c_int32, vp, C.c_int32]
     return L
 
@@ -197,6 +219,283 @@ def propagate(post, w, fanout, spikes, acc, frac_bits=24, stream=None, static=Fa
             acc.data_ptr(), acc.numel(), frac_bits, st.cuda_stream)
     if rc:
         raise SnnError(rc, lib().snn_last_error(None).decode())
+
+
+def _elem(t):
+    """SNN_F32 / SNN_BF16 / SNN_F16 of a torch dtype."""
+    global _elem
+    import torch
+    codes = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+    def _elem(t):
+        c = codes.get(t)
+        if c is None:
+            raise SnnError(1, f"element type must be float32, bfloat16 or float16, not {t}")
+        return c
+    return _elem(t)
+
+
+def _token(t):
+    """SNN_U8 / SNN_I32 / SNN_I64 of a torch dtype."""
+    global _token
+    import torch
+    codes = {torch.uint8: 8, torch.int32: 9, torch.int64: 10}
+
+    def _token(t):
+        c = codes.get(t)
+        if c is None:
+            raise SnnError(1, f"tokens must be uint8, int32 or int64, not {t}")
+        return c
+    return _token(t)
+
+
+def _require(ok, msg):
+    if not ok:
+        raise SnnError(1, msg)
+
+
+def _on_device(dev, stream, fn, *args):
+    """Call fn(*args, stream) with `dev` current, on `stream` (default: the
+    device's current stream)."""
+    import torch
+    if stream is not None:
+        _require(stream.device == dev, f"the stream is on {stream.device}, the tensors on {dev}")
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, (stream or torch.cuda.current_stream(dev)).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, (stream or torch.cuda.current_stream(dev)).cuda_stream)
+    if rc:
+        raise SnnError(rc, lib().snn_last_error(None).decode())
+
+
+def _new(dev, stream, shape, dtype):
+    """torch.empty of memory that belongs to `stream` (the one it is used on)."""
+    import torch
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=dev)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=dev)
+
+
+def _same_device(dev, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise SnnError(1, f"{name} must be a CUDA tensor on {dev}, not on {t.device}")
+
+
+def _matrix(t, name):
+    """t as [rows, dim] with unit column stride and one row stride (no copy)."""
+    dim = t.shape[-1]
+    if t.is_contiguous():
+        return t.numel() // max(dim, 1), dim, dim
+    _require(t.dim() == 2 and (dim == 1 or t.stride(1) == 1), f"{name} wants unit column stride and, "
+             "unless it is contiguous, two dimensions")
+    return t.shape[0], dim, t.stride(0)
+
+
+def embed(tokens, table, scale=1.0, dtype=None, out=None, stream=None):
+    """The drive rows of a token stream (snn_embed): scale * table[tokens].
+
+    tokens: contiguous uint8 / int32 / int64 CUDA tensor of any shape; table
+    [vocab, dim] in float32 / bfloat16 / float16, unit column stride.  Returns
+    tokens.shape + (dim,) in `dtype` (default: the table's), or `out`.  A
+    token outside [0, vocab) gives zeros.  Runs on `stream` (default: the
+    current stream of the tensors' device), on which new results are made."""
+    dev = tokens.device
+    _require(tokens.is_cuda and tokens.is_contiguous(), "tokens must be a contiguous CUDA tensor")
+    _same_device(dev, table=table, out=out)
+    _require(table.dim() == 2, "table must be [vocab, dim]")
+    vocab, dim = table.shape
+    _require(vocab >= 1 and dim >= 1, "table must not be empty")
+    _, _, stride = _matrix(table, "table")
+    if out is None:
+        out = _new(dev, stream, tokens.shape + (dim,), dtype or table.dtype)
+        ostride = dim
+    else:
+        _require(out.shape == tokens.shape + (dim,) and (dtype is None or dtype == out.dtype),
+                 "out must be tokens.shape + (dim,) of the wanted dtype")
+        _, _, ostride = _matrix(out, "out")
+    _on_device(dev, stream, lib().snn_embed, tokens.data_ptr(), _token(tokens.dtype), tokens.numel(),
+               table.data_ptr(), _elem(table.dtype), vocab, dim, stride, scale, out.data_ptr(),
+               _elem(out.dtype), ostride)
+    return out
+
+
+def embed_grad(tokens, dy, vocab=None, scale=1.0, dtype=None, out=None, accumulate=False, stream=None):
+    """Gradient of `embed` for its table (snn_embed_grad): [vocab, dim] with
+    scale * the sum of dy over the positions of each token, in f32 over the
+    positions sorted by token (equal calls give equal bits), rounded once.
+
+    tokens as for `embed`; dy tokens.shape + (dim,).  Returns a new tensor of
+    `dtype` (default float32), or `out`; with accumulate=True the sum is added
+    to `out` and rows that do not occur are not touched."""
+    import torch
+    dev = tokens.device
+    _require(tokens.is_cuda and tokens.is_contiguous(), "tokens must be a contiguous CUDA tensor")
+    _same_device(dev, dy=dy, out=out)
+    n = tokens.numel()
+    _require(dy.dim() >= 1 and dy.shape[:-1] == tokens.shape and dy.shape[-1] >= 1,
+             "dy must be tokens.shape + (dim,)")
+    _, dim, dstride = _matrix(dy, "dy")
+    if out is None:
+        _require(vocab is not None and not accumulate, "give vocab, or out (accumulate wants out)")
+        _require(vocab >= 1, "vocab must be positive")
+        out = _new(dev, stream, (vocab, dim), dtype or torch.float32)
+        ostride = dim
+    else:
+        _require(out.dim() == 2 and out.shape[1] == dim and out.shape[0] >= 1
+                 and vocab in (None, out.shape[0]) and (dtype is None or dtype == out.dtype),
+                 "out must be [vocab, dim] of the wanted dtype")
+        vocab = out.shape[0]
+        _, _, ostride = _matrix(out, "out")
+    size = C.c_int64(0)
+    rc = lib().snn_embed_grad_workspace(n, vocab, dim, C.byref(size))
+    if rc:
+        raise SnnError(rc, lib().snn_last_error(None).decode())
+    work = _new(dev, stream, (size.value,), torch.uint8)
+    _on_device(dev, stream, lib().snn_embed_grad, tokens.data_ptr(), _token(tokens.dtype), n,
+               dy.data_ptr(), _elem(dy.dtype), dim, dstride, scale, out.data_ptr(),
+               _elem(out.dtype), vocab, ostride, int(accumulate), work.data_ptr(), size.value)
+    return out
+
+
+def _scan_rows(t, name, shape, dtype):
+    """snn_rows of a tensor [steps, c] (packed) or [sequences, steps, c]."""
+    _require(t.shape == shape and t.dtype == dtype, f"{name} must be {tuple(shape)} in {dtype}, "
+             f"not {tuple(t.shape)} in {t.dtype}")
+    st = t.stride()
+    _require(shape[-1] == 1 or st[-1] == 1, f"{name} wants unit channel stride")
+    return Rows(t.data_ptr(), st[0] if len(shape) == 3 else 0, st[-2])
+
+
+def _scan_args(gate, x, logit, leaky, offsets, dtype):
+    """(description, gate rows, x rows, type, shape of y, shape of the state)"""
+    import torch
+    dev = x.device
+    _require(x.is_cuda, "x must be a CUDA tensor")
+    raster = not x.dtype.is_floating_point
+    if raster:
+        _require(x.dtype in (torch.int32, torch.uint32), "a raster x must be int32 or uint32 words")
+        dtype = dtype or torch.float32
+    else:
+        _require(dtype in (None, x.dtype), "y has x's dtype")
+        dtype = x.dtype
+    _require(x.dim() == (3 if offsets is None else 2),
+             "x must be [sequences, steps, channels], or [rows, channels] with offsets")
+    lead = x.shape[:-1]
+    channel = gate.dim() == 1
+    d = gate.shape[-1] if raster else x.shape[-1]
+    _require(d >= 1, "no channels")
+    _same_device(dev, gate=gate, offsets=offsets)
+    if offsets is not None:
+        _require(offsets.dtype == torch.int64 and offsets.dim() == 1 and offsets.is_contiguous()
+                 and offsets.numel() >= 1, "offsets must be contiguous int64 [sequences + 1]")
+        n_seq, n_steps = offsets.numel() - 1, lead[0]
+    else:
+        n_seq, n_steps = lead
+    if channel:
+        _require(gate.shape == (d,) and gate.dtype == torch.float32 and gate.is_contiguous(),
+                 "a gate per channel must be contiguous float32 [channels]")
+        g = Rows(gate.data_ptr(), 0, 0)
+    else:
+        g = _scan_rows(gate, "gate", lead + (d,), dtype)
+    xr = _scan_rows(x, "x", lead + ((d + 31) // 32,) if raster else lead + (d,), x.dtype)
+    flags = (SCAN_LOGIT if logit else 0) | (SCAN_LEAKY if leaky else 0) | \
+        (SCAN_CHANNEL if channel else 0) | (SCAN_RASTER if raster else 0)
+    desc = Scan(_elem(dtype), flags, n_seq, n_steps, d, offsets.data_ptr() if offsets is not None else None)
+    return desc, g, xr, dtype, lead + (d,), (n_seq, d)
+
+
+def _state(t, name, shape, dev):
+    import torch
+    if t is None:
+        return None
+    _same_device(dev, **{name: t})
+    _require(t.shape == shape and t.dtype == torch.float32 and t.is_contiguous(),
+             f"{name} must be contiguous float32 {tuple(shape)}")
+    return t.data_ptr()
+
+
+def leaky_scan(gate, x, h0=None, logit=False, leaky=False, offsets=None, dtype=None, out=None,
+               h_out=None, save=False, stream=None):
+    """Leaky integration along whole sequences (snn_leaky_scan):
+    h_t = a_t h_{t-1} + u_t with a = gate, or 1 / (1 + exp(-gate)) (logit),
+    and u = x, or (1 - a) x (leaky).
+
+    x: [sequences, steps, channels] or, with offsets (int64 [sequences + 1]),
+    packed [rows, channels] in float32 / bfloat16 / float16; or the spike
+    raster of Network.run (int32 / uint32 words, y in `dtype`, default
+    float32).  gate: x's form and dtype, or float32 [channels].  h0: float32
+    [sequences, channels] (default zeros).  Returns (y, h), h the float32
+    states after the last steps; with save=True also what leaky_scan_grad
+    needs.  `out` takes y; `h_out` takes h and may be h0, so that a stream of
+    single steps keeps its state in place.  Rows of no sequence are not
+    written: in a new y they hold what the memory held."""
+    import torch
+    desc, g, xr, dtype, shape, state = _scan_args(gate, x, logit, leaky, offsets, dtype)
+    dev = x.device
+    if out is None:
+        out = _new(dev, stream, shape, dtype)
+    else:
+        _same_device(dev, out=out)
+    if h_out is None:
+        h_out = _new(dev, stream, state, torch.float32)
+    saved = None
+    if save:
+        size = C.c_int64(0)
+        rc = lib().snn_leaky_scan_saved(C.byref(desc), C.byref(size))
+        if rc:
+            raise SnnError(rc, lib().snn_last_error(None).decode())
+        saved = _new(dev, stream, (size.value,), torch.float32)
+    _on_device(dev, stream, lib().snn_leaky_scan, C.byref(desc), C.byref(g), C.byref(xr),
+               _state(h0, "h0", state, dev), C.byref(_scan_rows(out, "out", shape, dtype)),
+               _state(h_out, "h_out", state, dev), saved.data_ptr() if save else None)
+    return (out, h_out, saved) if save else (out, h_out)
+
+
+def leaky_scan_grad(gate, x, dy, saved, dh=None, logit=False, leaky=False, offsets=None,
+                    need_gate=True, need_x=True, need_h0=True, stream=None):
+    """Gradients of leaky_scan (snn_leaky_scan_grad) from those of y (dy, None
+    for none) and of the final states (dh): returns (dgate, dx, dh0), each
+    None where it is not needed (dx of a raster never is).  gate, x, logit,
+    leaky and offsets as in the forward call with save=True, `saved` its
+    result.  dgate has gate's shape and dtype (a gate per channel: the sum over
+    all steps), dx x's, dh0 is float32 [sequences, channels]."""
+    import torch
+    raster = not x.dtype.is_floating_point
+    desc, g, xr, dtype, shape, state = _scan_args(
+        gate, x, logit, leaky, offsets, (dy.dtype if dy is not None else None) if raster else None)
+    dev = x.device
+    _require(dy is not None or dh is not None, "neither dy nor dh is given")
+    _same_device(dev, dy=dy, saved=saved)
+    size = C.c_int64(0)
+    rc = lib().snn_leaky_scan_saved(C.byref(desc), C.byref(size))
+    if rc:
+        raise SnnError(rc, lib().snn_last_error(None).decode())
+    _require(saved.dtype == torch.float32 and saved.numel() == size.value and saved.is_contiguous(),
+             "saved is not what the forward call of these sizes gives")
+    dyr = C.byref(_scan_rows(dy, "dy", shape, dtype)) if dy is not None else None
+    dgate = dgr = dx = dxr = dh0 = work = None
+    if need_gate:
+        dgate = _new(dev, stream, gate.shape, gate.dtype)
+        dgr = C.byref(Rows(dgate.data_ptr(), 0, 0) if gate.dim() == 1
+                      else _scan_rows(dgate, "dgate", shape, dtype))
+        rc = lib().snn_leaky_scan_grad_workspace(C.byref(desc), C.byref(size))
+        if rc:
+            raise SnnError(rc, lib().snn_last_error(None).decode())
+        if size.value:
+            work = _new(dev, stream, (size.value,), torch.uint8)
+    if need_x and not raster:
+        dx = _new(dev, stream, shape, dtype)
+        dxr = C.byref(_scan_rows(dx, "dx", shape, dtype))
+    if need_h0:
+        dh0 = _new(dev, stream, state, torch.float32)
+    _on_device(dev, stream, lib().snn_leaky_scan_grad, C.byref(desc), C.byref(g), C.byref(xr),
+               saved.data_ptr(), dyr, _state(dh, "dh", state, dev), dgr, dxr,
+               dh0.data_ptr() if need_h0 else None, work.data_ptr() if work is not None else None,
+               work.numel() if work is not None else 0)
+    return dgate, dx, dh0
 
 
 def nccl_unique_id():
