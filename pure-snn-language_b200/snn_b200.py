@@ -13,6 +13,7 @@ a CUDA device, raises instead of falling back to anything else.
 """
 import ctypes as C
 import os
+import struct
 
 import numpy as np
 
@@ -118,15 +119,6 @@ class Profile(C.Structure):
                             for i in range(k)}}
 
 
-class Scan(C.Structure):
-    _fields_ = [("type", C.c_int32), ("flags", C.c_int32), ("n_seq", C.c_int64),
-                ("n_steps", C.c_int64), ("n_channels", C.c_int64), ("offsets", C.c_void_p)]
-
-
-class Rows(C.Structure):
-    _fields_ = [("data", C.c_void_p), ("seq_stride", C.c_int64), ("step_stride", C.c_int64)]
-
-
 EXPORTS = ["snn_config_init", "snn_topology_init", "snn_create", "snn_destroy",
            "snn_last_error", "snn_version", "snn_build_columns", "snn_set_corpus", "snn_step",
            "snn_run", "snn_synchronize", "snn_get_spikes", "snn_get_state", "snn_get_counters",
@@ -195,7 +187,7 @@ def _load(path):
     L.snn_embed_grad_workspace.argtypes = [i64, i64, i64, vp]
     L.snn_embed_grad.argtypes = [vp, i32, i64, vp, i32, i64, i64, C.c_float, vp, i32, i64, i64,
                                  i32, vp, i64, vp]
-    ps, pr = C.POINTER(Scan), C.POINTER(Rows)
+    ps = pr = C.c_char_p  # snn_scan, snn_rows: packed bytes
     L.snn_leaky_scan_saved.argtypes = [ps, vp]
     L.snn_leaky_scan.argtypes = [ps, pr, pr, vp, pr, vp, vp, vp]
     L.snn_leaky_scan_grad_workspace.argtypes = [ps, vp]
@@ -221,32 +213,24 @@ def propagate(post, w, fanout, spikes, acc, frac_bits=24, stream=None, static=Fa
         raise SnnError(rc, lib().snn_last_error(None).decode())
 
 
-def _elem(t):
+_T = None  # torch, from the first call of an operator on
+
+
+def _torch():
+    global _T, _ELEM, _TOKEN
+    import torch
+    _ELEM = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    _TOKEN = {torch.uint8: 8, torch.int32: 9, torch.int64: 10}
+    _T = torch
+    return torch
+
+
+def _elem(dtype):
     """SNN_F32 / SNN_BF16 / SNN_F16 of a torch dtype."""
-    global _elem
-    import torch
-    codes = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-
-    def _elem(t):
-        c = codes.get(t)
-        if c is None:
-            raise SnnError(1, f"element type must be float32, bfloat16 or float16, not {t}")
-        return c
-    return _elem(t)
-
-
-def _token(t):
-    """SNN_U8 / SNN_I32 / SNN_I64 of a torch dtype."""
-    global _token
-    import torch
-    codes = {torch.uint8: 8, torch.int32: 9, torch.int64: 10}
-
-    def _token(t):
-        c = codes.get(t)
-        if c is None:
-            raise SnnError(1, f"tokens must be uint8, int32 or int64, not {t}")
-        return c
-    return _token(t)
+    c = _ELEM.get(dtype)
+    if c is None:
+        raise SnnError(1, f"element type must be float32, bfloat16 or float16, not {dtype}")
+    return c
 
 
 def _require(ok, msg):
@@ -254,44 +238,58 @@ def _require(ok, msg):
         raise SnnError(1, msg)
 
 
-def _on_device(dev, stream, fn, *args):
-    """Call fn(*args, stream) with `dev` current, on `stream` (default: the
+def _check(rc):
+    if rc:
+        raise SnnError(rc, lib().snn_last_error(None).decode())
+
+
+def _call(fn, dev, stream, *args):
+    """fn(*args, stream) with `dev` current, on `stream` (default: the
     device's current stream)."""
-    import torch
-    if stream is not None:
-        _require(stream.device == dev, f"the stream is on {stream.device}, the tensors on {dev}")
-    if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, (stream or torch.cuda.current_stream(dev)).cuda_stream)
+    if stream is None:
+        raw = _T._C._cuda_getCurrentRawStream(dev.index)
     else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, (stream or torch.cuda.current_stream(dev)).cuda_stream)
+        _require(stream.device == dev, f"the stream is on {stream.device}, the tensors on {dev}")
+        raw = stream.cuda_stream
+    if _T._C._cuda_getDevice() == dev.index:
+        rc = fn(*args, raw)
+    else:
+        with _T.cuda.device(dev):
+            rc = fn(*args, raw)
     if rc:
         raise SnnError(rc, lib().snn_last_error(None).decode())
 
 
 def _new(dev, stream, shape, dtype):
     """torch.empty of memory that belongs to `stream` (the one it is used on)."""
-    import torch
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=dev)
-    with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=dev)
+        return _T.empty(shape, dtype=dtype, device=dev)
+    with _T.cuda.stream(stream):
+        return _T.empty(shape, dtype=dtype, device=dev)
 
 
-def _same_device(dev, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise SnnError(1, f"{name} must be a CUDA tensor on {dev}, not on {t.device}")
+def _cuda(t, name, dev):
+    if t.device != dev:
+        raise SnnError(1, f"{name} must be a CUDA tensor on {dev}, not on {t.device}")
 
 
-def _matrix(t, name):
-    """t as [rows, dim] with unit column stride and one row stride (no copy)."""
-    dim = t.shape[-1]
+def _tokens(tokens):
+    """(device, type code) of a token tensor."""
+    if not (tokens.is_cuda and tokens.is_contiguous()):
+        raise SnnError(1, "tokens must be a contiguous CUDA tensor")
+    code = _TOKEN.get(tokens.dtype)
+    if code is None:
+        raise SnnError(1, f"tokens must be uint8, int32 or int64, not {tokens.dtype}")
+    return tokens.device, code
+
+
+def _row_stride(t, name):
+    """The stride of t's rows (its last dimension, of unit stride)."""
     if t.is_contiguous():
-        return t.numel() // max(dim, 1), dim, dim
-    _require(t.dim() == 2 and (dim == 1 or t.stride(1) == 1), f"{name} wants unit column stride and, "
-             "unless it is contiguous, two dimensions")
-    return t.shape[0], dim, t.stride(0)
+        return t.shape[-1]
+    _require(t.dim() == 2 and (t.shape[1] == 1 or t.stride(1) == 1), f"{name} wants unit column "
+             "stride and, unless it is contiguous, two dimensions")
+    return t.stride(0)
 
 
 def embed(tokens, table, scale=1.0, dtype=None, out=None, stream=None):
@@ -302,23 +300,25 @@ def embed(tokens, table, scale=1.0, dtype=None, out=None, stream=None):
     tokens.shape + (dim,) in `dtype` (default: the table's), or `out`.  A
     token outside [0, vocab) gives zeros.  Runs on `stream` (default: the
     current stream of the tensors' device), on which new results are made."""
-    dev = tokens.device
-    _require(tokens.is_cuda and tokens.is_contiguous(), "tokens must be a contiguous CUDA tensor")
-    _same_device(dev, table=table, out=out)
-    _require(table.dim() == 2, "table must be [vocab, dim]")
+    if _T is None:
+        _torch()
+    dev, tok = _tokens(tokens)
+    _cuda(table, "table", dev)
+    if table.dim() != 2 or table.numel() == 0:
+        raise SnnError(1, "table must be [vocab, dim] and not empty")
     vocab, dim = table.shape
-    _require(vocab >= 1 and dim >= 1, "table must not be empty")
-    _, _, stride = _matrix(table, "table")
+    shape = (*tokens.shape, dim)
     if out is None:
-        out = _new(dev, stream, tokens.shape + (dim,), dtype or table.dtype)
+        out = _new(dev, stream, shape, dtype or table.dtype)
         ostride = dim
     else:
-        _require(out.shape == tokens.shape + (dim,) and (dtype is None or dtype == out.dtype),
+        _cuda(out, "out", dev)
+        _require(out.shape == shape and (dtype is None or dtype == out.dtype),
                  "out must be tokens.shape + (dim,) of the wanted dtype")
-        _, _, ostride = _matrix(out, "out")
-    _on_device(dev, stream, lib().snn_embed, tokens.data_ptr(), _token(tokens.dtype), tokens.numel(),
-               table.data_ptr(), _elem(table.dtype), vocab, dim, stride, scale, out.data_ptr(),
-               _elem(out.dtype), ostride)
+        ostride = _row_stride(out, "out")
+    _call(lib().snn_embed, dev, stream, tokens.data_ptr(), tok, tokens.numel(), table.data_ptr(),
+          _elem(table.dtype), vocab, dim, _row_stride(table, "table"), scale, out.data_ptr(),
+          _elem(out.dtype), ostride)
     return out
 
 
@@ -330,91 +330,109 @@ def embed_grad(tokens, dy, vocab=None, scale=1.0, dtype=None, out=None, accumula
     tokens as for `embed`; dy tokens.shape + (dim,).  Returns a new tensor of
     `dtype` (default float32), or `out`; with accumulate=True the sum is added
     to `out` and rows that do not occur are not touched."""
-    import torch
-    dev = tokens.device
-    _require(tokens.is_cuda and tokens.is_contiguous(), "tokens must be a contiguous CUDA tensor")
-    _same_device(dev, dy=dy, out=out)
+    if _T is None:
+        _torch()
+    dev, tok = _tokens(tokens)
+    _cuda(dy, "dy", dev)
     n = tokens.numel()
-    _require(dy.dim() >= 1 and dy.shape[:-1] == tokens.shape and dy.shape[-1] >= 1,
-             "dy must be tokens.shape + (dim,)")
-    _, dim, dstride = _matrix(dy, "dy")
+    if dy.dim() < 1 or dy.shape[:-1] != tokens.shape or dy.shape[-1] < 1:
+        raise SnnError(1, "dy must be tokens.shape + (dim,)")
+    dim = dy.shape[-1]
     if out is None:
-        _require(vocab is not None and not accumulate, "give vocab, or out (accumulate wants out)")
-        _require(vocab >= 1, "vocab must be positive")
-        out = _new(dev, stream, (vocab, dim), dtype or torch.float32)
+        _require(vocab is not None and vocab >= 1 and not accumulate,
+                 "give a positive vocab, or out (accumulate wants out)")
+        out = _new(dev, stream, (vocab, dim), dtype or _T.float32)
         ostride = dim
     else:
+        _cuda(out, "out", dev)
         _require(out.dim() == 2 and out.shape[1] == dim and out.shape[0] >= 1
                  and vocab in (None, out.shape[0]) and (dtype is None or dtype == out.dtype),
                  "out must be [vocab, dim] of the wanted dtype")
         vocab = out.shape[0]
-        _, _, ostride = _matrix(out, "out")
-    size = C.c_int64(0)
-    rc = lib().snn_embed_grad_workspace(n, vocab, dim, C.byref(size))
-    if rc:
-        raise SnnError(rc, lib().snn_last_error(None).decode())
-    work = _new(dev, stream, (size.value,), torch.uint8)
-    _on_device(dev, stream, lib().snn_embed_grad, tokens.data_ptr(), _token(tokens.dtype), n,
-               dy.data_ptr(), _elem(dy.dtype), dim, dstride, scale, out.data_ptr(),
-               _elem(out.dtype), vocab, ostride, int(accumulate), work.data_ptr(), size.value)
+        ostride = _row_stride(out, "out")
+    L = lib()
+    size = C.c_int64()
+    _check(L.snn_embed_grad_workspace(n, vocab, dim, C.byref(size)))
+    work = _new(dev, stream, (size.value,), _T.uint8)
+    _call(L.snn_embed_grad, dev, stream, tokens.data_ptr(), tok, n, dy.data_ptr(), _elem(dy.dtype),
+          dim, _row_stride(dy, "dy"), scale, out.data_ptr(), _elem(out.dtype), vocab, ostride,
+          1 if accumulate else 0, work.data_ptr(), size.value)
     return out
+
+
+_SCAN = struct.Struct("=iiqqqQ")  # snn_scan
+_ROWS = struct.Struct("=Qqq")     # snn_rows
 
 
 def _scan_rows(t, name, shape, dtype):
     """snn_rows of a tensor [steps, c] (packed) or [sequences, steps, c]."""
-    _require(t.shape == shape and t.dtype == dtype, f"{name} must be {tuple(shape)} in {dtype}, "
-             f"not {tuple(t.shape)} in {t.dtype}")
+    if t.shape != shape or t.dtype != dtype:
+        raise SnnError(1, f"{name} must be {tuple(shape)} in {dtype}, not {tuple(t.shape)} in {t.dtype}")
     st = t.stride()
-    _require(shape[-1] == 1 or st[-1] == 1, f"{name} wants unit channel stride")
-    return Rows(t.data_ptr(), st[0] if len(shape) == 3 else 0, st[-2])
+    if st[-1] != 1 and shape[-1] != 1:
+        raise SnnError(1, f"{name} wants unit channel stride")
+    return _ROWS.pack(t.data_ptr(), st[0], st[-2])
 
 
 def _scan_args(gate, x, logit, leaky, offsets, dtype):
-    """(description, gate rows, x rows, type, shape of y, shape of the state)"""
-    import torch
-    dev = x.device
-    _require(x.is_cuda, "x must be a CUDA tensor")
-    raster = not x.dtype.is_floating_point
-    if raster:
-        _require(x.dtype in (torch.int32, torch.uint32), "a raster x must be int32 or uint32 words")
-        dtype = dtype or torch.float32
-    else:
-        _require(dtype in (None, x.dtype), "y has x's dtype")
+    """(snn_scan, gate rows, x rows, dtype of y, its shape, the states' shape)"""
+    if _T is None:
+        _torch()
+    if not x.is_cuda:
+        raise SnnError(1, "x must be a CUDA tensor")
+    _cuda(gate, "gate", x.device)
+    flags = (SCAN_LOGIT if logit else 0) | (SCAN_LEAKY if leaky else 0)
+    shape = x.shape
+    if x.dtype.is_floating_point:
+        if dtype is not None and dtype != x.dtype:
+            raise SnnError(1, "y has x's dtype")
         dtype = x.dtype
-    _require(x.dim() == (3 if offsets is None else 2),
-             "x must be [sequences, steps, channels], or [rows, channels] with offsets")
-    lead = x.shape[:-1]
-    channel = gate.dim() == 1
-    d = gate.shape[-1] if raster else x.shape[-1]
-    _require(d >= 1, "no channels")
-    _same_device(dev, gate=gate, offsets=offsets)
-    if offsets is not None:
-        _require(offsets.dtype == torch.int64 and offsets.dim() == 1 and offsets.is_contiguous()
+    else:
+        _require(x.dtype in (_T.int32, _T.uint32), "a raster x must be int32 or uint32 words")
+        dtype = dtype or _T.float32
+        flags |= SCAN_RASTER
+    if x.dim() != (3 if offsets is None else 2):
+        raise SnnError(1, "x must be [sequences, steps, channels], or [rows, channels] with offsets")
+    if flags & SCAN_RASTER:
+        d = gate.shape[-1]
+        xr = _scan_rows(x, "x", (*shape[:-1], (d + 31) // 32), x.dtype)
+        shape = (*shape[:-1], d)
+    else:
+        d = shape[-1]
+        xr = _scan_rows(x, "x", shape, dtype)
+    if d < 1:
+        raise SnnError(1, "no channels")
+    if offsets is None:
+        n_seq, off = shape[0], 0
+    else:
+        _cuda(offsets, "offsets", x.device)
+        _require(offsets.dtype == _T.int64 and offsets.dim() == 1 and offsets.is_contiguous()
                  and offsets.numel() >= 1, "offsets must be contiguous int64 [sequences + 1]")
-        n_seq, n_steps = offsets.numel() - 1, lead[0]
-    else:
-        n_seq, n_steps = lead
-    if channel:
-        _require(gate.shape == (d,) and gate.dtype == torch.float32 and gate.is_contiguous(),
+        n_seq, off = offsets.numel() - 1, offsets.data_ptr()
+    if gate.dim() == 1:
+        _require(gate.shape[0] == d and gate.dtype == _T.float32 and gate.is_contiguous(),
                  "a gate per channel must be contiguous float32 [channels]")
-        g = Rows(gate.data_ptr(), 0, 0)
+        g = _ROWS.pack(gate.data_ptr(), 0, 0)
+        flags |= SCAN_CHANNEL
     else:
-        g = _scan_rows(gate, "gate", lead + (d,), dtype)
-    xr = _scan_rows(x, "x", lead + ((d + 31) // 32,) if raster else lead + (d,), x.dtype)
-    flags = (SCAN_LOGIT if logit else 0) | (SCAN_LEAKY if leaky else 0) | \
-        (SCAN_CHANNEL if channel else 0) | (SCAN_RASTER if raster else 0)
-    desc = Scan(_elem(dtype), flags, n_seq, n_steps, d, offsets.data_ptr() if offsets is not None else None)
-    return desc, g, xr, dtype, lead + (d,), (n_seq, d)
+        g = _scan_rows(gate, "gate", shape, dtype)
+    return _SCAN.pack(_elem(dtype), flags, n_seq, shape[-2], d, off), g, xr, dtype, shape, (n_seq, d)
 
 
 def _state(t, name, shape, dev):
-    import torch
+    """Address of a float32 state tensor, or None."""
     if t is None:
         return None
-    _same_device(dev, **{name: t})
-    _require(t.shape == shape and t.dtype == torch.float32 and t.is_contiguous(),
-             f"{name} must be contiguous float32 {tuple(shape)}")
+    _cuda(t, name, dev)
+    if t.shape != shape or t.dtype != _T.float32 or not t.is_contiguous():
+        raise SnnError(1, f"{name} must be contiguous float32 {tuple(shape)}")
     return t.data_ptr()
+
+
+def _saved_floats(desc):
+    size = C.c_int64()
+    _check(lib().snn_leaky_scan_saved(desc, C.byref(size)))
+    return size.value
 
 
 def leaky_scan(gate, x, h0=None, logit=False, leaky=False, offsets=None, dtype=None, out=None,
@@ -432,25 +450,18 @@ def leaky_scan(gate, x, h0=None, logit=False, leaky=False, offsets=None, dtype=N
     needs.  `out` takes y; `h_out` takes h and may be h0, so that a stream of
     single steps keeps its state in place.  Rows of no sequence are not
     written: in a new y they hold what the memory held."""
-    import torch
     desc, g, xr, dtype, shape, state = _scan_args(gate, x, logit, leaky, offsets, dtype)
     dev = x.device
     if out is None:
         out = _new(dev, stream, shape, dtype)
     else:
-        _same_device(dev, out=out)
+        _cuda(out, "out", dev)
     if h_out is None:
-        h_out = _new(dev, stream, state, torch.float32)
-    saved = None
-    if save:
-        size = C.c_int64(0)
-        rc = lib().snn_leaky_scan_saved(C.byref(desc), C.byref(size))
-        if rc:
-            raise SnnError(rc, lib().snn_last_error(None).decode())
-        saved = _new(dev, stream, (size.value,), torch.float32)
-    _on_device(dev, stream, lib().snn_leaky_scan, C.byref(desc), C.byref(g), C.byref(xr),
-               _state(h0, "h0", state, dev), C.byref(_scan_rows(out, "out", shape, dtype)),
-               _state(h_out, "h_out", state, dev), saved.data_ptr() if save else None)
+        h_out = _new(dev, stream, state, _T.float32)
+    saved = _new(dev, stream, (_saved_floats(desc),), _T.float32) if save else None
+    _call(lib().snn_leaky_scan, dev, stream, desc, g, xr, _state(h0, "h0", state, dev),
+          _scan_rows(out, "out", shape, dtype), _state(h_out, "h_out", state, dev),
+          saved.data_ptr() if save else None)
     return (out, h_out, saved) if save else (out, h_out)
 
 
@@ -462,39 +473,36 @@ def leaky_scan_grad(gate, x, dy, saved, dh=None, logit=False, leaky=False, offse
     leaky and offsets as in the forward call with save=True, `saved` its
     result.  dgate has gate's shape and dtype (a gate per channel: the sum over
     all steps), dx x's, dh0 is float32 [sequences, channels]."""
-    import torch
     raster = not x.dtype.is_floating_point
     desc, g, xr, dtype, shape, state = _scan_args(
-        gate, x, logit, leaky, offsets, (dy.dtype if dy is not None else None) if raster else None)
+        gate, x, logit, leaky, offsets, dy.dtype if raster and dy is not None else None)
     dev = x.device
-    _require(dy is not None or dh is not None, "neither dy nor dh is given")
-    _same_device(dev, dy=dy, saved=saved)
-    size = C.c_int64(0)
-    rc = lib().snn_leaky_scan_saved(C.byref(desc), C.byref(size))
-    if rc:
-        raise SnnError(rc, lib().snn_last_error(None).decode())
-    _require(saved.dtype == torch.float32 and saved.numel() == size.value and saved.is_contiguous(),
-             "saved is not what the forward call of these sizes gives")
-    dyr = C.byref(_scan_rows(dy, "dy", shape, dtype)) if dy is not None else None
-    dgate = dgr = dx = dxr = dh0 = work = None
+    if dy is None and dh is None:
+        raise SnnError(1, "neither dy nor dh is given")
+    _cuda(saved, "saved", dev)
+    if saved.dtype != _T.float32 or saved.numel() != _saved_floats(desc) or not saved.is_contiguous():
+        raise SnnError(1, "saved is not what the forward call of these sizes gives")
+    dyr = dgate = dgr = dx = dxr = dh0 = work = None
+    size = C.c_int64()
+    if dy is not None:
+        _cuda(dy, "dy", dev)
+        dyr = _scan_rows(dy, "dy", shape, dtype)
     if need_gate:
         dgate = _new(dev, stream, gate.shape, gate.dtype)
-        dgr = C.byref(Rows(dgate.data_ptr(), 0, 0) if gate.dim() == 1
-                      else _scan_rows(dgate, "dgate", shape, dtype))
-        rc = lib().snn_leaky_scan_grad_workspace(C.byref(desc), C.byref(size))
-        if rc:
-            raise SnnError(rc, lib().snn_last_error(None).decode())
-        if size.value:
-            work = _new(dev, stream, (size.value,), torch.uint8)
+        if gate.dim() == 1:
+            dgr = _ROWS.pack(dgate.data_ptr(), 0, 0)
+            _check(lib().snn_leaky_scan_grad_workspace(desc, C.byref(size)))
+            work = _new(dev, stream, (size.value,), _T.uint8)
+        else:
+            dgr = _scan_rows(dgate, "dgate", shape, dtype)
     if need_x and not raster:
         dx = _new(dev, stream, shape, dtype)
-        dxr = C.byref(_scan_rows(dx, "dx", shape, dtype))
+        dxr = _scan_rows(dx, "dx", shape, dtype)
     if need_h0:
-        dh0 = _new(dev, stream, state, torch.float32)
-    _on_device(dev, stream, lib().snn_leaky_scan_grad, C.byref(desc), C.byref(g), C.byref(xr),
-               saved.data_ptr(), dyr, _state(dh, "dh", state, dev), dgr, dxr,
-               dh0.data_ptr() if need_h0 else None, work.data_ptr() if work is not None else None,
-               work.numel() if work is not None else 0)
+        dh0 = _new(dev, stream, state, _T.float32)
+    _call(lib().snn_leaky_scan_grad, dev, stream, desc, g, xr, saved.data_ptr(), dyr,
+          _state(dh, "dh", state, dev), dgr, dxr, dh0.data_ptr() if need_h0 else None,
+          work.data_ptr() if work is not None else None, size.value)
     return dgate, dx, dh0
 
 

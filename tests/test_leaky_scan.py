@@ -74,8 +74,8 @@ def call(grad=False, desc=(), **over):
     a = dict(h0=None, h=None, saved=1 << 20, dh=None, dh0=None, work=None, bytes=0)
     for k, v in over.items():
         (r if k in r else a)[k] = v
-    ro = {k: C.byref(snn.Rows(*v)) if v else None for k, v in r.items()}
-    de = C.byref(snn.Scan(*d.values()))
+    ro = {k: snn._ROWS.pack(v[0] or 0, *v[1:]) if v else None for k, v in r.items()}
+    de = snn._SCAN.pack(*(v or 0 for v in d.values()))
     L = snn.lib()
     if grad:
         return L.snn_leaky_scan_grad(de, ro["gate"], ro["x"], a["saved"], ro["y"], a["dh"], ro["dgate"], ro["dx"],
@@ -106,10 +106,10 @@ def test_null_descriptions():
     n = C.c_int64()
     assert snn.lib().snn_leaky_scan(None, None, None, None, None, None, None, None) == 1
     assert snn.lib().snn_leaky_scan_saved(None, C.byref(n)) == 1
-    d = snn.Scan(0, 0, 3, 100, 7, None)
-    assert snn.lib().snn_leaky_scan_saved(C.byref(d), None) == 1
+    d = snn._SCAN.pack(0, 0, 3, 100, 7, 0)
+    assert snn.lib().snn_leaky_scan_saved(d, None) == 1
     # a state for every block of every sequence, whatever the lengths
-    assert snn.lib().snn_leaky_scan_saved(C.byref(d), C.byref(n)) == 0 and n.value >= 3 * 2 * 7
+    assert snn.lib().snn_leaky_scan_saved(d, C.byref(n)) == 0 and n.value >= 3 * 2 * 7
 
 
 # ---- GPU ------------------------------------------------------------------------------
