@@ -13,7 +13,10 @@ using snnb::to_f32;
 // of y, and the states stay f32.
 constexpr int BLOCK = 64;
 
-enum { GATE_VALUE = 0, GATE_LOGIT = 1, GATE_CHANNEL = 2 };
+// how the decays are given: per step, as they are or as logits; per channel
+enum { GATE_VALUE = 0, GATE_LOGIT = 1, GATE_CHANNEL = 2, GATE_CHANNEL_LOGIT = 3 };
+template <int GM> constexpr bool per_channel = GM >= GATE_CHANNEL;
+template <int GM> constexpr bool is_logit = (GM & 1) != 0;
 
 struct Rows {
     void* p;
@@ -61,70 +64,241 @@ __device__ __forceinline__ long long row_at(const ScanArgs& A, const Rows& r, lo
     return A.off ? (sp.begin + t) * r.st : s * r.ss + t * r.st;
 }
 
-// A decay in the form the recurrence needs it: a = m, or a = 1 + m where
-// `keep` is all ones.  The logistic decay of a large gate is 1 - s with a
-// small s; kept as -s it has s's relative precision, which is what a state
-// with a long memory (1/s steps) is proportional to, while 1 - s rounded to
-// f32 is off by 2^-25 / s of it.
-struct Decay {
-    float m;
-    unsigned keep;
-    __device__ __forceinline__ float step(float h, float u) const {
-        return fmaf(m, h, __uint_as_float(__float_as_uint(h) & keep) + u);
-    }
-    __device__ __forceinline__ float times(float h) const {
-        return fmaf(m, h, __uint_as_float(__float_as_uint(h) & keep));
-    }
-    __device__ __forceinline__ float rest() const { return keep ? -m : 1.0f - m; }  // 1 - a
-    __device__ __forceinline__ float slope() const {                                // a (1 - a) of a logistic decay
-        const float s = fabsf(m);
-        return s * (1.0f - s);
-    }
+// V values side by side; pairs go through the packed f32 instructions
+template <int V>
+struct Vec {
+    float v[V];
 };
-__device__ __forceinline__ Decay decay_value(float a) { return {a, 0u}; }
-__device__ __forceinline__ Decay decay_logit(float z) {
-    const float e = expf(-fabsf(z));
-    const float s = __fdiv_rn(e, 1.0f + e);
-    Decay d;
-    d.keep = (__float_as_uint(z) >> 31) - 1u;  // z >= 0: all ones
-    d.m = d.keep ? -s : s;
+template <int V>
+__device__ __forceinline__ Vec<V> splat(float x) {
+    Vec<V> r;
+#pragma unroll
+    for (int k = 0; k < V; ++k) r.v[k] = x;
+    return r;
+}
+__device__ __forceinline__ Vec<1> vfma(Vec<1> a, Vec<1> b, Vec<1> c) { return {fmaf(a.v[0], b.v[0], c.v[0])}; }
+__device__ __forceinline__ Vec<1> vmul(Vec<1> a, Vec<1> b) { return {a.v[0] * b.v[0]}; }
+__device__ __forceinline__ Vec<1> vadd(Vec<1> a, Vec<1> b) { return {a.v[0] + b.v[0]}; }
+__device__ __forceinline__ Vec<2> vfma(Vec<2> a, Vec<2> b, Vec<2> c) {
+    Vec<2> d;
+    asm("{.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;}"
+        : "=f"(d.v[0]), "=f"(d.v[1])
+        : "f"(a.v[0]), "f"(a.v[1]), "f"(b.v[0]), "f"(b.v[1]), "f"(c.v[0]), "f"(c.v[1]));
+    return d;
+}
+__device__ __forceinline__ Vec<2> vmul(Vec<2> a, Vec<2> b) {
+    Vec<2> d;
+    asm("{.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;}"
+        : "=f"(d.v[0]), "=f"(d.v[1])
+        : "f"(a.v[0]), "f"(a.v[1]), "f"(b.v[0]), "f"(b.v[1]));
+    return d;
+}
+__device__ __forceinline__ Vec<2> vadd(Vec<2> a, Vec<2> b) {
+    Vec<2> d;
+    asm("{.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;}"
+        : "=f"(d.v[0]), "=f"(d.v[1])
+        : "f"(a.v[0]), "f"(a.v[1]), "f"(b.v[0]), "f"(b.v[1]));
     return d;
 }
 
+// The decays of V channels.  A logistic decay near 1 is 1 - s with a small s.
+// Rounded to f32 it is off by up to 2^-25, which a memory of 1 / s steps adds
+// up to 2^-25 / s of the state where the gate stays the same.  Per-channel
+// gates and f32 gates therefore keep what the rounding lost as `lo` (one more
+// FMA a step); 16-bit gates, whose own rounding is 2^-9 and up of the exponent
+// and differs from step to step, do not.  (An infinite state times lo may be
+// NaN: infinities do not survive, they end as infinities or NaN.)
+template <int V, bool LO>
+struct Decay {
+    Vec<V> a;
+    __device__ __forceinline__ Vec<V> step(Vec<V> h, Vec<V> u) const { return vfma(a, h, u); }
+    __device__ __forceinline__ Vec<V> times(Vec<V> h) const { return vmul(a, h); }
+    __device__ __forceinline__ void set_lo(int, float) {}
+};
+template <int V>
+struct Decay<V, true> {
+    Vec<V> a, lo;
+    __device__ __forceinline__ Vec<V> step(Vec<V> h, Vec<V> u) const { return vfma(a, h, vfma(lo, h, u)); }
+    __device__ __forceinline__ Vec<V> times(Vec<V> h) const { return vfma(a, h, vmul(lo, h)); }
+    __device__ __forceinline__ void set_lo(int k, float x) { lo.v[k] = x; }
+};
 template <typename T, int GM>
-__device__ __forceinline__ Decay decay_at(const ScanArgs& A, long long row, int c, const Decay& fixed) {
-    if (GM == GATE_CHANNEL) return fixed;
-    const float v = to_f32(reinterpret_cast<const T*>(A.gate.p)[row + c]);
-    return GM == GATE_LOGIT ? decay_logit(v) : decay_value(v);
+constexpr bool keeps_lo = GM == GATE_CHANNEL_LOGIT || (GM == GATE_LOGIT && sizeof(T) == 4);
+
+// decay a = 1 / (1 + exp(-z)) and its rest 1 - a, each with its own relative
+// precision: from e = exp(-|z|) the larger is 1 / (1 + e), the smaller e times that
+__device__ __forceinline__ void logistic(float z, float& a, float& lo, float& rest) {
+    const float e = expf(-fabsf(z));
+    const float big = __frcp_rn(1.0f + e), s = e * big;
+    const bool up = z >= 0.0f;
+    const float near1 = 1.0f - s;
+    a = up ? near1 : s;
+    lo = up ? (1.0f - near1) - s : 0.0f;
+    rest = up ? s : big;
+    if (z != z) a = rest = z;
 }
-__device__ __forceinline__ Decay decay_channel(const ScanArgs& A, int c) {
-    const float v = reinterpret_cast<const float*>(A.gate.p)[c];
-    return A.logit ? decay_logit(v) : decay_value(v);
-}
-template <typename T, bool RASTER>
-__device__ __forceinline__ float input_at(const ScanArgs& A, long long row, int c) {
-    if (RASTER) return (float)((reinterpret_cast<const unsigned*>(A.x.p)[row + (c >> 5)] >> (c & 31)) & 1u);
-    return to_f32(reinterpret_cast<const T*>(A.x.p)[row + c]);
+// the same by the short instructions (2 ulp each, the argument rounded once)
+__device__ __forceinline__ void logistic_fast(float z, float& a, float& rest) {
+    float e, big;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fabsf(z) * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(big) : "f"(1.0f + e));
+    const float s = e * big;
+    const bool up = z >= 0.0f;
+    a = up ? big : s;
+    rest = up ? s : big;
 }
 
-// One thread per sequence and channel, a step at a time.
-template <typename T, int GM, bool RASTER>
-__global__ void __launch_bounds__(128) k_scan_seq(const ScanArgs A) {
-    const int c = (int)(blockIdx.x * 128 + threadIdx.x);
+// decay and rest of V gates
+template <typename T, int GM, int V>
+__device__ __forceinline__ void decays(const Vec<V>& z, Decay<V, keeps_lo<T, GM>>& d, Vec<V>& rest) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const float v = z.v[k];
+        float a = v, lo = 0.0f, r = 1.0f - v;
+        if (GM == GATE_LOGIT) {
+            if (sizeof(T) == 4) logistic(v, a, lo, r);
+            else logistic_fast(v, a, r);
+        }
+        d.a.v[k] = a;
+        d.set_lo(k, lo);
+        rest.v[k] = r;
+    }
+}
+// those of the per-channel gates c .. c + V
+template <typename T, int GM, int V>
+__device__ __forceinline__ void channel_decays(const ScanArgs& A, int c, bool live, Decay<V, keeps_lo<T, GM>>& d,
+                                               Vec<V>& rest) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const float v = live ? reinterpret_cast<const float*>(A.gate.p)[c + k] : 0.0f;
+        float a = v, lo = 0.0f, r = 1.0f - v;
+        if (is_logit<GM>) logistic(v, a, lo, r);
+        d.a.v[k] = a;
+        d.set_lo(k, lo);
+        rest.v[k] = r;
+    }
+}
+
+// V elements of type T as the one register (or pair) that a load fills: they
+// are unpacked where they are used, not where they are loaded, so that loads
+// stay in flight
+template <int BYTES>
+struct Raw;
+template <>
+struct Raw<2> {
+    using type = unsigned short;
+};
+template <>
+struct Raw<4> {
+    using type = unsigned;
+};
+template <>
+struct Raw<8> {
+    using type = uint2;
+};
+template <typename T, int V>
+using Word = typename Raw<sizeof(T) * V>::type;
+// what a lane reads of an input row: V elements, or the raster word they lie in
+template <typename T, int V, bool RASTER>
+using InWord = std::conditional_t<RASTER, unsigned, Word<T, V>>;
+
+template <typename T>
+struct Unpack;
+template <>
+struct Unpack<float> {
+    static __device__ __forceinline__ Vec<1> get(unsigned w) { return {__uint_as_float(w)}; }
+    static __device__ __forceinline__ Vec<2> get(uint2 w) { return {__uint_as_float(w.x), __uint_as_float(w.y)}; }
+    static __device__ __forceinline__ unsigned put(Vec<1> x) { return __float_as_uint(x.v[0]); }
+    static __device__ __forceinline__ uint2 put(Vec<2> x) { return {__float_as_uint(x.v[0]), __float_as_uint(x.v[1])}; }
+};
+template <>
+struct Unpack<__nv_bfloat16> {
+    static __device__ __forceinline__ Vec<1> get(unsigned short w) { return {__uint_as_float((unsigned)w << 16)}; }
+    static __device__ __forceinline__ Vec<2> get(unsigned w) {
+        return {__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
+    }
+    static __device__ __forceinline__ unsigned short put(Vec<1> x) {
+        return __bfloat16_as_ushort(__float2bfloat16_rn(x.v[0]));
+    }
+    static __device__ __forceinline__ unsigned put(Vec<2> x) {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(x.v[0], x.v[1]);
+        unsigned r;
+        memcpy(&r, &p, 4);
+        return r;
+    }
+};
+template <>
+struct Unpack<__half> {
+    static __device__ __forceinline__ Vec<1> get(unsigned short w) { return {__half2float(__ushort_as_half(w))}; }
+    static __device__ __forceinline__ Vec<2> get(unsigned w) {
+        __half2 p;
+        memcpy(&p, &w, 4);
+        const float2 f = __half22float2(p);
+        return {f.x, f.y};
+    }
+    static __device__ __forceinline__ unsigned short put(Vec<1> x) { return __half_as_ushort(__float2half_rn(x.v[0])); }
+    static __device__ __forceinline__ unsigned put(Vec<2> x) {
+        const __half2 p = __floats2half2_rn(x.v[0], x.v[1]);
+        unsigned r;
+        memcpy(&r, &p, 4);
+        return r;
+    }
+};
+template <typename T, int V, bool RASTER>
+__device__ __forceinline__ Vec<V> in_values(InWord<T, V, RASTER> w, int c) {
+    if constexpr (RASTER) {
+        Vec<V> r;
+#pragma unroll
+        for (int k = 0; k < V; ++k) r.v[k] = (w >> ((c + k) & 31)) & 1u ? 1.0f : 0.0f;
+        return r;
+    } else {
+        return Unpack<T>::get(w);
+    }
+}
+template <int V>
+__device__ __forceinline__ Vec<V> load_f32(const float* p, bool live) {
+    Vec<V> r;
+#pragma unroll
+    for (int k = 0; k < V; ++k) r.v[k] = live ? p[k] : 0.0f;
+    return r;
+}
+template <int V>
+__device__ __forceinline__ void store_f32(float* p, const Vec<V>& x) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) p[k] = x.v[k];
+}
+
+// ---- short sequences: a thread per sequence and V channels, a step at a time ----
+template <typename T, int GM, bool RASTER, int V>
+__global__ void __launch_bounds__(128) k_scan_steps(const ScanArgs A) {
+    using X = InWord<T, V, RASTER>;
+    const int c = (int)(blockIdx.x * 128 + threadIdx.x) * V;
     if (c >= A.D) return;
     for (long long s = blockIdx.y; s < A.n_seq; s += gridDim.y) {
         const Span sp = span_of(A, s);
-        const Decay fixed = GM == GATE_CHANNEL ? decay_channel(A, c) : Decay();
-        float h = A.h0 ? A.h0[s * A.D + c] : 0.0f;
+        Decay<V, keeps_lo<T, GM>> d;
+        Vec<V> rest;
+        if (per_channel<GM>) channel_decays<T, GM, V>(A, c, true, d, rest);
+        Vec<V> h = load_f32<V>(A.h0 + s * A.D + c, A.h0 != nullptr);
         for (long long t = 0; t < sp.len; ++t) {
-            if (A.saved && t % BLOCK == 0) A.saved[(sp.block0 + t / BLOCK) * A.D + c] = h;
-            const Decay d = decay_at<T, GM>(A, row_at(A, A.gate, s, sp, t), c, fixed);
-            float u = input_at<T, RASTER>(A, row_at(A, A.x, s, sp, t), c);
-            if (A.leaky) u = d.rest() * u;
+            if (A.saved && t % BLOCK == 0) store_f32<V>(A.saved + (sp.block0 + t / BLOCK) * A.D + c, h);
+            if (!per_channel<GM>) {
+                const Word<T, V> g = *reinterpret_cast<const Word<T, V>*>(
+                    reinterpret_cast<const T*>(A.gate.p) + row_at(A, A.gate, s, sp, t) + c);
+                decays<T, GM, V>(Unpack<T>::get(g), d, rest);
+            }
+            const long long xr = row_at(A, A.x, s, sp, t);
+            const X xw = RASTER ? *reinterpret_cast<const X*>(reinterpret_cast<const unsigned*>(A.x.p) + xr + (c >> 5))
+                                : *reinterpret_cast<const X*>(reinterpret_cast<const T*>(A.x.p) + xr + c);
+            Vec<V> u = in_values<T, V, RASTER>(xw, c);
+            if (A.leaky) u = vmul(rest, u);
             h = d.step(h, u);
-            reinterpret_cast<T*>(A.y.p)[row_at(A, A.y, s, sp, t) + c] = from_f32<T>(h);
+            *reinterpret_cast<Word<T, V>*>(reinterpret_cast<T*>(A.y.p) + row_at(A, A.y, s, sp, t) + c) = Unpack<T>::put(h);
         }
-        if (A.h) A.h[s * A.D + c] = h;
+        if (A.h) store_f32<V>(A.h + s * A.D + c, h);
     }
 }
 
@@ -139,221 +313,154 @@ __global__ void __launch_bounds__(128) k_scan_seq(const ScanArgs A) {
 // tiles is carried in registers to its next round.
 constexpr int W = 8;
 constexpr int TILE_THREADS = 32 * W;
-constexpr int L_FWD = 16, L_BWD = 8;
+template <typename T>
+constexpr int fwd_steps = sizeof(T) == 4 ? 8 : 16;
+constexpr int L_BWD = 8;
 constexpr int MAX_CLUSTER = 8;
-static_assert((W * L_BWD) == BLOCK && (W * L_FWD) % BLOCK == 0 && BLOCK % L_FWD == 0, "blocks start at a warp's steps");
-
-template <typename T, int V>
-struct alignas(sizeof(T) * V) Word {
-    T v[V];
-};
-template <typename T, int V>
-__device__ __forceinline__ Word<T, V> zero_word() {
-    Word<T, V> r;
-#pragma unroll
-    for (int k = 0; k < V; ++k) r.v[k] = from_f32<T>(0.0f);
-    return r;
-}
-// what a lane reads of an input row: V elements, or the raster word they lie in
-template <typename T, int V, bool RASTER>
-struct InWord {
-    using type = Word<T, V>;
-};
-template <typename T, int V>
-struct InWord<T, V, true> {
-    using type = unsigned;
-};
-template <int V, typename T>
-__device__ __forceinline__ float in_value(const Word<T, V>& w, int k, int) {
-    return to_f32(w.v[k]);
-}
-template <int V>
-__device__ __forceinline__ float in_value(unsigned w, int k, int c) {
-    return (float)((w >> ((c + k) & 31)) & 1u);
-}
-
-// The decay of a gate as one float.  GATE_LOGIT: the sign says the form (m, or
-// 1 + m for a set sign, -0 included).  16-bit gates use the short exponential
-// and reciprocal: off by some 2^-20 relative, their own rounding by 2^-9.
-template <typename T, int GM>
-__device__ __forceinline__ float gate_m(float z) {
-    if (GM != GATE_LOGIT) return z;
-    float s;
-    if (sizeof(T) == 4) {
-        const float e = expf(-fabsf(z));
-        s = __fdiv_rn(e, 1.0f + e);
-    } else {
-        const float e = __expf(-fabsf(z));
-        s = __fdividef(e, 1.0f + e);
-    }
-    return __uint_as_float((__float_as_uint(s) & 0x7fffffffu) | (~__float_as_uint(z) & 0x80000000u));
-}
-template <int GM>
-__device__ __forceinline__ Decay decay_m(float m, unsigned keep) {
-    Decay d;
-    d.m = m;
-    d.keep = GM == GATE_VALUE ? 0u : GM == GATE_LOGIT ? (unsigned)(__float_as_int(m) >> 31) : keep;
-    return d;
-}
+static_assert(W * L_BWD == BLOCK && BLOCK % (2 * L_BWD) == 0, "blocks start at a warp's steps");
 
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // store to the same shared-memory variable of CTA `rank` of the cluster
-__device__ __forceinline__ void store_peer(float* p, int rank, float v) {
-    unsigned a = (unsigned)__cvta_generic_to_shared(p), r;
+template <int V>
+__device__ __forceinline__ void store_peer(Vec<V>* p, int rank, const Vec<V>& x) {
+    const unsigned a = (unsigned)__cvta_generic_to_shared(p);
+    unsigned r;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(r), "f"(v) : "memory");
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(r + 4 * k), "f"(x.v[k]) : "memory");
 }
 
 template <int V>
 struct ClusterMaps {  // the tiles' maps of a round, by rank; two rounds
-    float a[2][MAX_CLUSTER][32 * V], h[2][MAX_CLUSTER][32 * V];
+    Vec<V> a[2][MAX_CLUSTER][32], h[2][MAX_CLUSTER][32];
 };
 
 template <typename T, int GM, bool RASTER, int V>
 __global__ void __launch_bounds__(TILE_THREADS, 2) k_scan_tile(const ScanArgs A) {
-    constexpr int L = L_FWD, TT = W * L;
+    constexpr int L = fwd_steps<T>, TT = W * L;
+    constexpr bool LO = keeps_lo<T, GM>;
     using G = Word<T, V>;
-    using X = typename InWord<T, V, RASTER>::type;
-    __shared__ float sa[2][W][32 * V], sh[2][W][32 * V];
+    using X = InWord<T, V, RASTER>;
+    using XE = std::conditional_t<RASTER, unsigned, T>;
+    __shared__ Vec<V> sa[2][W][32], sh[2][W][32];
     __shared__ ClusterMaps<V> cm;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int CL = A.cluster, rank = blockIdx.x % CL, item = blockIdx.x / CL;
     const int c = (item % A.ctiles * 32 + lane) * V;
     const bool live = c < A.D;
-    float fm[V];
-    unsigned fk[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-        fm[k] = 0.0f;
-        fk[k] = 0u;
-        if (GM == GATE_CHANNEL && live) {
-            const Decay d = decay_channel(A, c + k);
-            fm[k] = d.m;
-            fk[k] = d.keep;
-        }
+    Decay<V, LO> fixed;
+    Vec<V> factor = splat<V>(1.0f);
+    if (per_channel<GM>) {
+        channel_decays<T, GM, V>(A, c, live, fixed, factor);
+        if (!A.leaky) factor = splat<V>(1.0f);
     }
     int par = 0;
     for (long long s = item / A.ctiles; s < A.n_seq; s += A.workers) {
         const Span sp = span_of(A, s);
-        float carry[V];
-#pragma unroll
-        for (int k = 0; k < V; ++k) carry[k] = A.h0 && live ? A.h0[s * A.D + c + k] : 0.0f;
+        Vec<V> carry = load_f32<V>(A.h0 + s * A.D + c, A.h0 && live);
         if (sp.len == 0) {
-            if (A.h && live && rank == 0 && w == 0)
-#pragma unroll
-                for (int k = 0; k < V; ++k) A.h[s * A.D + c + k] = carry[k];
+            if (A.h && live && rank == 0 && w == 0) store_f32<V>(A.h + s * A.D + c, carry);
             continue;
         }
         const T* pg = reinterpret_cast<const T*>(A.gate.p) + row_at(A, A.gate, s, sp, 0) + c;
-        const char* px = RASTER ? (const char*)(reinterpret_cast<const unsigned*>(A.x.p) + row_at(A, A.x, s, sp, 0) + (c >> 5))
-                                : (const char*)(reinterpret_cast<const T*>(A.x.p) + row_at(A, A.x, s, sp, 0) + c);
+        const XE* px = reinterpret_cast<const XE*>(A.x.p) + row_at(A, A.x, s, sp, 0) + (RASTER ? c >> 5 : c);
         T* py = reinterpret_cast<T*>(A.y.p) + row_at(A, A.y, s, sp, 0) + c;
-        constexpr int XS = RASTER ? 4 : sizeof(T);
         G rg[L];
         X rx[L];
         auto fetch = [&](long long t0) {
             const T* qg = pg + t0 * A.gate.st;
-            const char* qx = px + t0 * A.x.st * XS;
+            const XE* qx = px + t0 * A.x.st;
+            const int n = live ? (int)min((long long)L, sp.len - t0) : 0;
+            if (n == L) {
 #pragma unroll
-            for (int i = 0; i < L; ++i) {
-                if (live && t0 + i < sp.len) {
-                    if (GM != GATE_CHANNEL) rg[i] = *reinterpret_cast<const G*>(qg + i * A.gate.st);
-                    rx[i] = *reinterpret_cast<const X*>(qx + i * A.x.st * XS);
+                for (int i = 0; i < L; ++i) {
+                    if (!per_channel<GM>) rg[i] = *reinterpret_cast<const G*>(qg + i * A.gate.st);
+                    rx[i] = *reinterpret_cast<const X*>(qx + i * A.x.st);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < L; ++i) {
+                    if (i >= n) continue;
+                    if (!per_channel<GM>) rg[i] = *reinterpret_cast<const G*>(qg + i * A.gate.st);
+                    rx[i] = *reinterpret_cast<const X*>(qx + i * A.x.st);
                 }
             }
         };
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-            rg[i] = zero_word<T, V>();
+            memset(&rg[i], 0, sizeof(G));
             memset(&rx[i], 0, sizeof(X));
         }
         const long long round = (long long)CL * TT;
         fetch((long long)rank * TT + w * L);
         for (long long b = 0; b < sp.len; b += round) {
             const long long t0 = b + (long long)rank * TT + w * L;
-            float m[L][V], u[L][V], a[V], h[V];
+            Decay<V, LO> d[per_channel<GM> ? 1 : L];
+            Vec<V> u[L];
 #pragma unroll
-            for (int i = 0; i < L; ++i)
-#pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    m[i][k] = GM == GATE_CHANNEL ? fm[k] : gate_m<T, GM>(to_f32(rg[i].v[k]));
-                    u[i][k] = in_value<V>(rx[i], k, c);
-                    if (A.leaky) u[i][k] *= decay_m<GM>(m[i][k], fk[k]).rest();
+            for (int i = 0; i < L; ++i) {
+                Vec<V> f = factor;
+                if (!per_channel<GM>) {
+                    decays<T, GM, V>(Unpack<T>::get(rg[i]), d[i], f);
+                    if (!A.leaky) f = splat<V>(1.0f);
                 }
+                u[i] = vmul(f, in_values<T, V, RASTER>(rx[i], c));
+            }
+            if (per_channel<GM>) d[0] = fixed;
             if (b + round < sp.len) fetch(t0 + round);
+            Vec<V> a = splat<V>(1.0f), h = splat<V>(0.0f);
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                a[k] = 1.0f;
-                h[k] = 0.0f;
+            for (int i = 0; i < L; ++i) {
+                const Decay<V, LO>& q = d[per_channel<GM> ? 0 : i];
+                h = q.step(h, u[i]);
+                a = q.times(a);
             }
-#pragma unroll
-            for (int i = 0; i < L; ++i)
-#pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    const Decay d = decay_m<GM>(m[i][k], fk[k]);
-                    h[k] = d.step(h[k], u[i][k]);
-                    a[k] = d.times(a[k]);
-                }
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                sa[par][w][lane * V + k] = a[k];
-                sh[par][w][lane * V + k] = h[k];
-            }
+            sa[par][w][lane] = a;
+            sh[par][w][lane] = h;
             __syncthreads();
             if (CL > 1) {
                 if (w == 0) {
+                    Vec<V> ta = splat<V>(1.0f), th = splat<V>(0.0f);
 #pragma unroll
-                    for (int k = 0; k < V; ++k) {
-                        float ta = 1.0f, th = 0.0f;
-                        for (int j = 0; j < W; ++j) {
-                            th = fmaf(sa[par][j][lane * V + k], th, sh[par][j][lane * V + k]);
-                            ta *= sa[par][j][lane * V + k];
-                        }
-                        for (int r = 0; r < CL; ++r) {
-                            store_peer(&cm.a[par][rank][lane * V + k], r, ta);
-                            store_peer(&cm.h[par][rank][lane * V + k], r, th);
-                        }
+                    for (int j = 0; j < W; ++j) {
+                        th = vfma(sa[par][j][lane], th, sh[par][j][lane]);
+                        ta = vmul(sa[par][j][lane], ta);
+                    }
+                    for (int r = 0; r < CL; ++r) {
+                        store_peer<V>(&cm.a[par][rank][lane], r, ta);
+                        store_peer<V>(&cm.h[par][rank][lane], r, th);
                     }
                 }
                 cluster_sync();
             }
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                float hk = carry[k];
-                if (CL > 1) {
-                    for (int r = 0; r < rank; ++r) hk = fmaf(cm.a[par][r][lane * V + k], hk, cm.h[par][r][lane * V + k]);
-                    float next = hk;
-                    for (int r = rank; r < CL; ++r) next = fmaf(cm.a[par][r][lane * V + k], next, cm.h[par][r][lane * V + k]);
-                    carry[k] = next;
-                }
-                for (int j = 0; j < w; ++j) hk = fmaf(sa[par][j][lane * V + k], hk, sh[par][j][lane * V + k]);
-                h[k] = hk;
-                if (CL == 1) {
-                    for (int j = w; j < W; ++j) hk = fmaf(sa[par][j][lane * V + k], hk, sh[par][j][lane * V + k]);
-                    carry[k] = hk;
-                }
+            h = carry;
+            if (CL > 1) {
+                for (int r = 0; r < rank; ++r) h = vfma(cm.a[par][r][lane], h, cm.h[par][r][lane]);
+                carry = h;
+                for (int r = rank; r < CL; ++r) carry = vfma(cm.a[par][r][lane], carry, cm.h[par][r][lane]);
+            }
+            for (int j = 0; j < w; ++j) h = vfma(sa[par][j][lane], h, sh[par][j][lane]);
+            if (CL == 1) {
+                carry = h;
+                for (int j = w; j < W; ++j) carry = vfma(sa[par][j][lane], carry, sh[par][j][lane]);
             }
             par ^= 1;
-            if (A.saved && live && t0 % BLOCK == 0 && t0 < sp.len)
-#pragma unroll
-                for (int k = 0; k < V; ++k) A.saved[(sp.block0 + t0 / BLOCK) * A.D + c + k] = h[k];
+            if (!live || t0 >= sp.len) continue;
+            if (A.saved && t0 % BLOCK == 0) store_f32<V>(A.saved + (sp.block0 + t0 / BLOCK) * A.D + c, h);
             T* qy = py + t0 * A.y.st;
+            const int n = (int)min((long long)L, sp.len - t0);
 #pragma unroll
             for (int i = 0; i < L; ++i) {
-                if (t0 + i >= sp.len) break;
-                G o;
-#pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    h[k] = decay_m<GM>(m[i][k], fk[k]).step(h[k], u[i][k]);
-                    o.v[k] = from_f32<T>(h[k]);
+                if (i < n) {
+                    h = d[per_channel<GM> ? 0 : i].step(h, u[i]);
+                    *reinterpret_cast<G*>(qy) = Unpack<T>::put(h);
                 }
-                if (live) *reinterpret_cast<G*>(qy + i * A.y.st) = o;
-                if (t0 + i == sp.len - 1 && A.h && live)
-#pragma unroll
-                    for (int k = 0; k < V; ++k) A.h[s * A.D + c + k] = h[k];
+                qy += A.y.st;
             }
+            if (A.h && t0 + n == sp.len) store_f32<V>(A.h + s * A.D + c, h);
         }
     }
 }
@@ -364,193 +471,171 @@ __global__ void __launch_bounds__(TILE_THREADS, 2) k_scan_tile(const ScanArgs A)
 template <typename T, int GM, bool RASTER, int V>
 __global__ void __launch_bounds__(TILE_THREADS, 2) k_scan_grad_tile(const ScanArgs A) {
     constexpr int L = L_BWD, TT = W * L;
+    constexpr bool LO = keeps_lo<T, GM>, PC = per_channel<GM>;
     using G = Word<T, V>;
-    using X = typename InWord<T, V, RASTER>::type;
-    __shared__ float sa[2][W][32 * V], sh[2][W][32 * V], sr[2][W][32 * V];
+    using X = InWord<T, V, RASTER>;
+    using XE = std::conditional_t<RASTER, unsigned, T>;
+    __shared__ Vec<V> sa[2][W][32], sh[2][W][32], sr[2][W][32];
     __shared__ ClusterMaps<V> cm;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int CL = A.cluster, rank = blockIdx.x % CL, item = blockIdx.x / CL;
     const int c = (item % A.ctiles * 32 + lane) * V;
     const bool live = c < A.D;
-    float fm[V], sum[V];
-    unsigned fk[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-        fm[k] = sum[k] = 0.0f;
-        fk[k] = 0u;
-        if (GM == GATE_CHANNEL && live) {
-            const Decay d = decay_channel(A, c + k);
-            fm[k] = d.m;
-            fk[k] = d.keep;
-        }
+    const Vec<V> one = splat<V>(1.0f), minus = splat<V>(A.leaky ? -1.0f : 0.0f);
+    Decay<V, LO> fixed;
+    Vec<V> factor = one, sum = splat<V>(0.0f);
+    if (PC) {
+        channel_decays<T, GM, V>(A, c, live, fixed, factor);
+        if (!A.leaky) factor = one;
     }
     int par = 0;
     for (long long s = item / A.ctiles; s < A.n_seq; s += A.workers) {
         const Span sp = span_of(A, s);
-        float carry[V];
-#pragma unroll
-        for (int k = 0; k < V; ++k) carry[k] = 0.0f;
+        Vec<V> carry = splat<V>(0.0f);
         if (sp.len == 0) {
             if (A.dh0 && live && rank == 0 && w == 0)
-#pragma unroll
-                for (int k = 0; k < V; ++k) A.dh0[s * A.D + c + k] = A.dh ? A.dh[s * A.D + c + k] : 0.0f;
+                store_f32<V>(A.dh0 + s * A.D + c, load_f32<V>(A.dh + s * A.D + c, A.dh != nullptr));
             continue;
         }
         const T* pg = reinterpret_cast<const T*>(A.gate.p) + row_at(A, A.gate, s, sp, 0) + c;
-        const char* px = RASTER ? (const char*)(reinterpret_cast<const unsigned*>(A.x.p) + row_at(A, A.x, s, sp, 0) + (c >> 5))
-                                : (const char*)(reinterpret_cast<const T*>(A.x.p) + row_at(A, A.x, s, sp, 0) + c);
-        const T* pd = A.y.p ? reinterpret_cast<const T*>(A.y.p) + row_at(A, A.y, s, sp, 0) + c : nullptr;
-        T* pdg = GM != GATE_CHANNEL && A.dgate.p ? reinterpret_cast<T*>(A.dgate.p) + row_at(A, A.dgate, s, sp, 0) + c : nullptr;
-        T* pdx = A.dx.p ? reinterpret_cast<T*>(A.dx.p) + row_at(A, A.dx, s, sp, 0) + c : nullptr;
-        constexpr int XS = RASTER ? 4 : sizeof(T);
+        const XE* px = reinterpret_cast<const XE*>(A.x.p) + row_at(A, A.x, s, sp, 0) + (RASTER ? c >> 5 : c);
+        const T* pd = reinterpret_cast<const T*>(A.y.p) + row_at(A, A.y, s, sp, 0) + c;
+        T* pdg = reinterpret_cast<T*>(A.dgate.p) + (PC ? 0 : row_at(A, A.dgate, s, sp, 0) + c);
+        T* pdx = reinterpret_cast<T*>(A.dx.p) + row_at(A, A.dx, s, sp, 0) + c;
         G rg[L], rd[L];
         X rx[L];
-        float rs[V];
+        Vec<V> rs = splat<V>(0.0f);
         auto fetch = [&](long long t0) {
-            if (!live || t0 < 0) return;
+            if (t0 < 0) return;
             const T* qg = pg + t0 * A.gate.st;
             const T* qd = pd + t0 * A.y.st;
-            const char* qx = px + t0 * A.x.st * XS;
+            const XE* qx = px + t0 * A.x.st;
+            const int n = live ? (int)min((long long)L, sp.len - t0) : 0;
+            if (n == L && A.y.p) {
 #pragma unroll
-            for (int i = 0; i < L; ++i) {
-                if (t0 + i < sp.len) {
-                    if (GM != GATE_CHANNEL) rg[i] = *reinterpret_cast<const G*>(qg + i * A.gate.st);
-                    rx[i] = *reinterpret_cast<const X*>(qx + i * A.x.st * XS);
-                    if (pd) rd[i] = *reinterpret_cast<const G*>(qd + i * A.y.st);
-                } else {
-                    rd[i] = zero_word<T, V>();
+                for (int i = 0; i < L; ++i) {
+                    if (!PC) rg[i] = *reinterpret_cast<const G*>(qg + i * A.gate.st);
+                    rx[i] = *reinterpret_cast<const X*>(qx + i * A.x.st);
+                    rd[i] = *reinterpret_cast<const G*>(qd + i * A.y.st);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < L; ++i) {
+                    if (i >= n) continue;
+                    if (!PC) rg[i] = *reinterpret_cast<const G*>(qg + i * A.gate.st);
+                    rx[i] = *reinterpret_cast<const X*>(qx + i * A.x.st);
+                    if (A.y.p) rd[i] = *reinterpret_cast<const G*>(qd + i * A.y.st);
                 }
             }
-#pragma unroll
-            for (int k = 0; k < V; ++k) rs[k] = A.saved[(sp.block0 + t0 / BLOCK) * A.D + c + k];
+            rs = load_f32<V>(A.saved + (sp.block0 + t0 / BLOCK) * A.D + c, live);
         };
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-            rg[i] = rd[i] = zero_word<T, V>();
+            memset(&rg[i], 0, sizeof(G));
+            memset(&rd[i], 0, sizeof(G));
             memset(&rx[i], 0, sizeof(X));
         }
-#pragma unroll
-        for (int k = 0; k < V; ++k) rs[k] = 0.0f;
         const long long tiles = (sp.len + TT - 1) / TT;
         fetch((tiles - 1 - rank) * TT + w * L);
         for (long long b = 0; b < tiles; b += CL) {
             const long long t0 = (tiles - 1 - b - rank) * TT + w * L;  // negative: no tile left for this CTA
-            float m[L][V], xv[L][V], o[L][V], a[V], h[V], r[V], h0[V];
+            Decay<V, LO> d[PC ? 1 : L];
+            Vec<V> rest[PC ? 1 : L], x[L], o[L];
 #pragma unroll
-            for (int i = 0; i < L; ++i)
-#pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    m[i][k] = GM == GATE_CHANNEL ? fm[k] : gate_m<T, GM>(to_f32(rg[i].v[k]));
-                    xv[i][k] = in_value<V>(rx[i], k, c);
-                    o[i][k] = to_f32(rd[i].v[k]);
-                    if (t0 + i == sp.len - 1 && A.dh && live) o[i][k] += A.dh[s * A.D + c + k];
-                }
-#pragma unroll
-            for (int k = 0; k < V; ++k) h0[k] = rs[k];
+            for (int i = 0; i < L; ++i) {
+                if (!PC) decays<T, GM, V>(Unpack<T>::get(rg[i]), d[i], rest[i]);
+                x[i] = in_values<T, V, RASTER>(rx[i], c);
+                o[i] = Unpack<T>::get(rd[i]);
+                if (t0 + i == sp.len - 1) o[i] = vadd(o[i], load_f32<V>(A.dh + s * A.D + c, A.dh && live));
+            }
+            if (PC) d[0] = fixed;
+            const Vec<V> h0 = rs;
             if (b + CL < tiles) fetch(t0 - (long long)CL * TT);
+            Vec<V> a = one, h = splat<V>(0.0f), r = h;
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                a[k] = 1.0f;
-                h[k] = r[k] = 0.0f;
+            for (int i = 0; i < L; ++i) {
+                const Decay<V, LO>& q = d[PC ? 0 : i];
+                const Vec<V> f = PC ? factor : A.leaky ? rest[PC ? 0 : i] : one;
+                h = q.step(h, vmul(f, x[i]));
+                a = q.times(a);
+                r = d[PC ? 0 : L - 1 - i].times(vadd(o[L - 1 - i], r));
             }
-#pragma unroll
-            for (int i = 0; i < L; ++i)
-#pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    const Decay d = decay_m<GM>(m[i][k], fk[k]);
-                    h[k] = d.step(h[k], A.leaky ? d.rest() * xv[i][k] : xv[i][k]);
-                    a[k] = d.times(a[k]);
-                    const Decay e = decay_m<GM>(m[L - 1 - i][k], fk[k]);
-                    r[k] = e.times(o[L - 1 - i][k] + r[k]);
-                }
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                sa[par][w][lane * V + k] = a[k];
-                sh[par][w][lane * V + k] = h[k];
-                sr[par][w][lane * V + k] = r[k];
-            }
+            sa[par][w][lane] = a;
+            sh[par][w][lane] = h;
+            sr[par][w][lane] = r;
             __syncthreads();
             if (CL > 1) {
                 if (w == 0) {
+                    Vec<V> ta = one, tr = splat<V>(0.0f);
 #pragma unroll
-                    for (int k = 0; k < V; ++k) {
-                        float ta = 1.0f, tr = 0.0f;
-                        for (int j = W - 1; j >= 0; --j) {
-                            tr = fmaf(sa[par][j][lane * V + k], tr, sr[par][j][lane * V + k]);
-                            ta *= sa[par][j][lane * V + k];
-                        }
-                        for (int q = 0; q < CL; ++q) {
-                            store_peer(&cm.a[par][rank][lane * V + k], q, ta);
-                            store_peer(&cm.h[par][rank][lane * V + k], q, tr);
-                        }
+                    for (int j = W - 1; j >= 0; --j) {
+                        tr = vfma(sa[par][j][lane], tr, sr[par][j][lane]);
+                        ta = vmul(sa[par][j][lane], ta);
+                    }
+                    for (int q = 0; q < CL; ++q) {
+                        store_peer<V>(&cm.a[par][rank][lane], q, ta);
+                        store_peer<V>(&cm.h[par][rank][lane], q, tr);
                     }
                 }
                 cluster_sync();
             }
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                float hk = h0[k];
-                for (int j = 0; j < w; ++j) hk = fmaf(sa[par][j][lane * V + k], hk, sh[par][j][lane * V + k]);
-                h[k] = hk;
-                float rk = carry[k];
-                if (CL > 1) {
-                    for (int q = 0; q < rank; ++q) rk = fmaf(cm.a[par][q][lane * V + k], rk, cm.h[par][q][lane * V + k]);
-                    float next = rk;
-                    for (int q = rank; q < CL; ++q) next = fmaf(cm.a[par][q][lane * V + k], next, cm.h[par][q][lane * V + k]);
-                    carry[k] = next;
-                }
-                for (int j = W - 1; j > w; --j) rk = fmaf(sa[par][j][lane * V + k], rk, sr[par][j][lane * V + k]);
-                r[k] = rk;
-                if (CL == 1) {
-                    for (int j = w; j >= 0; --j) rk = fmaf(sa[par][j][lane * V + k], rk, sr[par][j][lane * V + k]);
-                    carry[k] = rk;
-                }
+            h = h0;
+            for (int j = 0; j < w; ++j) h = vfma(sa[par][j][lane], h, sh[par][j][lane]);
+            r = carry;
+            if (CL > 1) {
+                for (int q = 0; q < rank; ++q) r = vfma(cm.a[par][q][lane], r, cm.h[par][q][lane]);
+                carry = r;
+                for (int q = rank; q < CL; ++q) carry = vfma(cm.a[par][q][lane], carry, cm.h[par][q][lane]);
+            }
+            for (int j = W - 1; j > w; --j) r = vfma(sa[par][j][lane], r, sr[par][j][lane]);
+            if (CL == 1) {
+                carry = r;
+                for (int j = w; j >= 0; --j) carry = vfma(sa[par][j][lane], carry, sr[par][j][lane]);
             }
             par ^= 1;
-            if (t0 < 0) continue;
-            // xv becomes the derivative of h_t in a_t: h_{t-1}, or h_{t-1} - x_t
+            if (!live || t0 < 0 || t0 >= sp.len) continue;
+            // x becomes the derivative of h_t in a_t: h_{t-1}, or h_{t-1} - x_t
 #pragma unroll
-            for (int i = 0; i < L; ++i)
-#pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    const Decay d = decay_m<GM>(m[i][k], fk[k]);
-                    const float before = h[k], x = xv[i][k];
-                    h[k] = d.step(before, A.leaky ? d.rest() * x : x);
-                    xv[i][k] = A.leaky ? before - x : before;
-                }
+            for (int i = 0; i < L; ++i) {
+                const Vec<V> f = PC ? factor : A.leaky ? rest[PC ? 0 : i] : one;
+                const Vec<V> before = h, xi = x[i];
+                h = d[PC ? 0 : i].step(h, vmul(f, xi));
+                x[i] = A.leaky ? vfma(minus, xi, before) : before;
+            }
+            const int n = (int)min((long long)L, sp.len - t0);
+            T* qg = pdg + (t0 + L - 1) * A.dgate.st;
+            T* qx = pdx + (t0 + L - 1) * A.dx.st;
 #pragma unroll
             for (int i = L - 1; i >= 0; --i) {
-                if (t0 + i >= sp.len) continue;
-                G og, ox;
-#pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    const Decay d = decay_m<GM>(m[i][k], fk[k]);
-                    const float g = o[i][k] + r[k], da = g * xv[i][k];
-                    if (GM == GATE_CHANNEL) sum[k] += da;
-                    og.v[k] = from_f32<T>(GM == GATE_LOGIT ? da * d.slope() : da);
-                    ox.v[k] = from_f32<T>(A.leaky ? d.rest() * g : g);
-                    r[k] = d.times(g);
+                if (i < n) {
+                    const Decay<V, LO>& q = d[PC ? 0 : i];
+                    const Vec<V> f = PC ? factor : A.leaky ? rest[PC ? 0 : i] : one;
+                    const Vec<V> g = vadd(o[i], r);
+                    if (PC) {
+                        sum = vfma(g, x[i], sum);
+                    } else if (A.dgate.p) {
+                        Vec<V> da = vmul(g, x[i]);
+                        if (GM == GATE_LOGIT) da = vmul(da, vmul(q.a, rest[PC ? 0 : i]));
+                        *reinterpret_cast<G*>(qg) = Unpack<T>::put(da);
+                    }
+                    if (A.dx.p) *reinterpret_cast<G*>(qx) = Unpack<T>::put(vmul(f, g));
+                    r = q.times(g);
                 }
-                if (live && pdg) *reinterpret_cast<G*>(pdg + (t0 + i) * A.dgate.st) = og;
-                if (live && pdx) *reinterpret_cast<G*>(pdx + (t0 + i) * A.dx.st) = ox;
+                qg -= A.dgate.st;
+                qx -= A.dx.st;
             }
-            if (t0 == 0 && A.dh0 && live)
-#pragma unroll
-                for (int k = 0; k < V; ++k) A.dh0[s * A.D + c + k] = r[k];
+            if (t0 == 0 && A.dh0) store_f32<V>(A.dh0 + s * A.D + c, r);
         }
     }
-    if (GM == GATE_CHANNEL && A.part) {
+    if (PC && A.part) {
         __syncthreads();
-#pragma unroll
-        for (int k = 0; k < V; ++k) sa[0][w][lane * V + k] = sum[k];
+        sa[0][w][lane] = sum;
         __syncthreads();
-        if (w == 0 && live)
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                float t = 0.0f;
-                for (int j = 0; j < W; ++j) t += sa[0][j][lane * V + k];
-                A.part[((long long)(item / A.ctiles) * CL + rank) * A.D + c + k] = t;
-            }
+        if (w == 0 && live) {
+            Vec<V> t = splat<V>(0.0f);
+            for (int j = 0; j < W; ++j) t = vadd(t, sa[0][j][lane]);
+            store_f32<V>(A.part + ((long long)(item / A.ctiles) * CL + rank) * A.D + c, t);
+        }
     }
 }
 
@@ -566,7 +651,11 @@ __global__ void __launch_bounds__(256) k_scan_gate_sum(const ScanArgs A, int row
     __syncthreads();
     if (grp != 0 || c >= A.D) return;
     for (int g = 1; g < 8; ++g) sum += s[g][lane];
-    if (A.logit) sum *= decay_channel(A, c).slope();
+    if (A.logit) {
+        float a, lo, rest;
+        logistic(reinterpret_cast<const float*>(A.gate.p)[c], a, lo, rest);
+        sum *= a * rest;
+    }
     reinterpret_cast<float*>(A.dgate.p)[c] = sum;
 }
 
@@ -632,11 +721,11 @@ using Const = std::integral_constant<int, V>;
 template <typename F>
 void dispatch(const snn_scan* d, F&& f) {
     snnb::with_elem(d->type, [&](auto t) {
-        const bool raster = (d->flags & SNN_SCAN_RASTER) != 0;
-        const int gm = d->flags & SNN_SCAN_CHANNEL ? GATE_CHANNEL : d->flags & SNN_SCAN_LOGIT ? GATE_LOGIT : GATE_VALUE;
-        if (gm == GATE_CHANNEL) raster ? f(t, Const<GATE_CHANNEL>(), Const<1>()) : f(t, Const<GATE_CHANNEL>(), Const<0>());
-        else if (gm == GATE_LOGIT) raster ? f(t, Const<GATE_LOGIT>(), Const<1>()) : f(t, Const<GATE_LOGIT>(), Const<0>());
-        else raster ? f(t, Const<GATE_VALUE>(), Const<1>()) : f(t, Const<GATE_VALUE>(), Const<0>());
+        auto with_gate = [&](auto gm) { d->flags & SNN_SCAN_RASTER ? f(t, gm, Const<1>()) : f(t, gm, Const<0>()); };
+        if (d->flags & SNN_SCAN_CHANNEL)
+            d->flags & SNN_SCAN_LOGIT ? with_gate(Const<GATE_CHANNEL_LOGIT>()) : with_gate(Const<GATE_CHANNEL>());
+        else
+            d->flags & SNN_SCAN_LOGIT ? with_gate(Const<GATE_LOGIT>()) : with_gate(Const<GATE_VALUE>());
     });
 }
 
@@ -713,25 +802,30 @@ void leaky_scan(const snn_scan* d, const snn_rows* gate, const snn_rows* x, cons
     A.h0 = h0;
     A.h = h;
     A.saved = saved;
+    const int size = elem_size(d->type);
+    const bool raster_x = (d->flags & SNN_SCAN_RASTER) != 0, channel = (d->flags & SNN_SCAN_CHANNEL) != 0;
+    const bool two = d->n_channels % 2 == 0 && (channel || fits_vec(A.gate, size, 2)) &&
+                     (raster_x || fits_vec(A.x, size, 2)) && fits_vec(A.y, size, 2);
     if (mean_steps(d) <= 8) {
-        const dim3 grid((unsigned)((d->n_channels + 127) / 128), (unsigned)std::min<int64_t>(d->n_seq, 65535));
+        const int vec = two ? 2 : 1;
+        const dim3 grid((unsigned)((d->n_channels + 128 * vec - 1) / (128 * vec)),
+                        (unsigned)std::min<int64_t>(d->n_seq, 65535));
         dispatch(d, [&](auto t, auto gm, auto raster) {
-            k_scan_seq<decltype(t), decltype(gm)::value, decltype(raster)::value != 0><<<grid, 128, 0, st>>>(A);
+            using T = decltype(t);
+            constexpr int GM = decltype(gm)::value;
+            constexpr bool RA = decltype(raster)::value != 0;
+            if (two) k_scan_steps<T, GM, RA, 2><<<grid, 128, 0, st>>>(A);
+            else k_scan_steps<T, GM, RA, 1><<<grid, 128, 0, st>>>(A);
         });
         SNN_CUDA(cudaGetLastError());
         return;
     }
-    const int size = elem_size(d->type);
-    const bool raster_x = (d->flags & SNN_SCAN_RASTER) != 0, channel = (d->flags & SNN_SCAN_CHANNEL) != 0;
-    const bool two = size == 2 && d->n_channels % 2 == 0 && (channel || fits_vec(A.gate, size, 2)) &&
-                     (raster_x || fits_vec(A.x, size, 2)) && fits_vec(A.y, size, 2);
-    const Plan p = plan_of(d, two ? 2 : 1, W * L_FWD);
+    const Plan p = plan_of(d, two ? 2 : 1, W * (size == 4 ? fwd_steps<float> : fwd_steps<__half>));
     dispatch(d, [&](auto t, auto gm, auto raster) {
         using T = decltype(t);
         constexpr int GM = decltype(gm)::value;
         constexpr bool RA = decltype(raster)::value != 0;
-        if constexpr (sizeof(T) == 2)
-            if (two) return launch((const void*)k_scan_tile<T, GM, RA, 2>, p, A, st);
+        if (two) return launch((const void*)k_scan_tile<T, GM, RA, 2>, p, A, st);
         launch((const void*)k_scan_tile<T, GM, RA, 1>, p, A, st);
     });
 }
@@ -765,7 +859,7 @@ void leaky_scan_grad(const snn_scan* d, const snn_rows* gate, const snn_rows* x,
     } else if (dgate) {
         A.dgate = rows_of(d, dgate, "dgate", d->n_channels, size, true);
     }
-    const bool two = size == 2 && d->n_channels % 2 == 0 && (channel || fits_vec(A.gate, size, 2)) &&
+    const bool two = d->n_channels % 2 == 0 && (channel || fits_vec(A.gate, size, 2)) &&
                      ((d->flags & SNN_SCAN_RASTER) || fits_vec(A.x, size, 2)) && fits_vec(A.y, size, 2) &&
                      fits_vec(A.dx, size, 2) && (channel || fits_vec(A.dgate, size, 2));
     const Plan p = plan_of(d, two ? 2 : 1, W * L_BWD);
@@ -773,8 +867,7 @@ void leaky_scan_grad(const snn_scan* d, const snn_rows* gate, const snn_rows* x,
         using T = decltype(t);
         constexpr int GM = decltype(gm)::value;
         constexpr bool RA = decltype(raster)::value != 0;
-        if constexpr (sizeof(T) == 2)
-            if (two) return launch((const void*)k_scan_grad_tile<T, GM, RA, 2>, p, A, st);
+        if (two) return launch((const void*)k_scan_grad_tile<T, GM, RA, 2>, p, A, st);
         launch((const void*)k_scan_grad_tile<T, GM, RA, 1>, p, A, st);
     });
     if (A.part) {
