@@ -129,10 +129,20 @@ template <typename T, int GM>
 constexpr bool keeps_lo = GM == GATE_CHANNEL_LOGIT || (GM == GATE_LOGIT && sizeof(T) == 4);
 
 // decay a = 1 / (1 + exp(-z)) and its rest 1 - a, each with its own relative
-// precision: from e = exp(-|z|) the larger is 1 / (1 + e), the smaller e times that
+// precision: from e = exp(-|z|) the larger is 1 / (1 + e), the smaller e times
+// that.  exp(-|z|) = 2^p (1 + q ln 2) with p the rounded product -|z| log2(e)
+// and q what its rounding and log2(e)'s own lost: within 2 ulp, as the
+// exponential instruction is, where the product alone would be off by |z|
+// 2^-24.  Beyond |z| = 150 e is 0.
 __device__ __forceinline__ void logistic(float z, float& a, float& lo, float& rest) {
-    const float e = expf(-fabsf(z));
-    const float big = __frcp_rn(1.0f + e), s = e * big;
+    const float m = fminf(fabsf(z), 150.0f);
+    const float p = m * -1.44269502f;  // log2(e) = 1.44269502 + 1.9259630e-8
+    const float q = fmaf(m, -1.92596303e-8f, fmaf(m, -1.44269502f, -p));
+    float e, big;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(p));
+    e = fmaf(e, q * 0.693147182f, e);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(big) : "f"(1.0f + e));
+    const float s = e * big;
     const bool up = z >= 0.0f;
     const float near1 = 1.0f - s;
     a = up ? near1 : s;
@@ -169,11 +179,11 @@ __device__ __forceinline__ void decays(const Vec<V>& z, Decay<V, keeps_lo<T, GM>
 }
 // those of the per-channel gates c .. c + V
 template <typename T, int GM, int V>
-__device__ __forceinline__ void channel_decays(const ScanArgs& A, int c, bool live, Decay<V, keeps_lo<T, GM>>& d,
+__device__ __forceinline__ void channel_decays(const ScanArgs& A, int c, int nl, Decay<V, keeps_lo<T, GM>>& d,
                                                Vec<V>& rest) {
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-        const float v = live ? reinterpret_cast<const float*>(A.gate.p)[c + k] : 0.0f;
+        const float v = k < nl ? reinterpret_cast<const float*>(A.gate.p)[c + k] : 0.0f;
         float a = v, lo = 0.0f, r = 1.0f - v;
         if (is_logit<GM>) logistic(v, a, lo, r);
         d.a.v[k] = a;
@@ -281,7 +291,7 @@ __global__ void __launch_bounds__(128) k_scan_steps(const ScanArgs A) {
         const Span sp = span_of(A, s);
         Decay<V, keeps_lo<T, GM>> d;
         Vec<V> rest;
-        if (per_channel<GM>) channel_decays<T, GM, V>(A, c, true, d, rest);
+        if (per_channel<GM>) channel_decays<T, GM, V>(A, c, V, d, rest);
         Vec<V> h = load_f32<V>(A.h0 + s * A.D + c, A.h0 != nullptr);
         for (long long t = 0; t < sp.len; ++t) {
             if (A.saved && t % BLOCK == 0) store_f32<V>(A.saved + (sp.block0 + t / BLOCK) * A.D + c, h);
@@ -304,20 +314,21 @@ __global__ void __launch_bounds__(128) k_scan_steps(const ScanArgs A) {
 
 // ---- tiles ---------------------------------------------------------------------
 // A CTA of W warps takes W * L consecutive steps of 32 * V channels at a time:
-// a warp L steps, a lane V channels, all in registers.  Over its L steps a
-// warp's map of the state is h -> A h + H (A the product of the decays, H the
-// end state from zero); the CTA joins its warps' maps in shared memory, so
-// each warp learns the state it starts from and runs its steps once more with
-// it.  With few channels a cluster of CTAs takes consecutive tiles and joins
-// their maps through distributed shared memory; the state after the cluster's
-// tiles is carried in registers to its next round.
+// a warp L steps, a lane V channels (one 4-byte word of a row).  Over its L
+// steps a warp's map of the state is h -> A h + H (A the product of the
+// decays, H the end state from zero); the CTA joins its warps' maps in shared
+// memory, so each warp learns the state it starts from and runs its steps once
+// more with it, from registers.  With few channels a cluster of CTAs takes
+// consecutive tiles and joins their maps through distributed shared memory;
+// the state after the cluster's tiles is carried in registers to its next round.
 constexpr int W = 8;
 constexpr int TILE_THREADS = 32 * W;
-template <typename T>
-constexpr int fwd_steps = sizeof(T) == 4 ? 8 : 16;
-constexpr int L_BWD = 8;
+constexpr int L_FWD = 16, L_BWD = 8;
+constexpr int S_FWD = 2, S_BWD = 3;  // stages of rows in flight per warp
 constexpr int MAX_CLUSTER = 8;
-static_assert(W * L_BWD == BLOCK && BLOCK % (2 * L_BWD) == 0, "blocks start at a warp's steps");
+static_assert(W * L_BWD == BLOCK && BLOCK % L_FWD == 0, "blocks start at a warp's steps");
+template <typename T>
+constexpr int lane_channels = 4 / (int)sizeof(T);
 
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -338,269 +349,406 @@ struct ClusterMaps {  // the tiles' maps of a round, by rank; two rounds
     Vec<V> a[2][MAX_CLUSTER][32], h[2][MAX_CLUSTER][32];
 };
 
-template <typename T, int GM, bool RASTER, int V>
+// Rows are staged in shared memory by asynchronous copies, each warp its own
+// rows, so that they need no barrier and no registers while in flight.  COPY is
+// the words that all rows allow: 16 bytes, 4 bytes, or (16-bit types, odd row
+// strides or offsets) the aligned 4-byte words that cover a row, 33 for 32.
+// Of a word at a row's end that reaches past the tile only the lower half is
+// read; one at a row's begin may hold the element before, which lies in the
+// same allocation (allocations begin aligned).
+template <int COPY>
+constexpr int row_bytes = COPY == 2 ? 132 : 128;
+
+__device__ __forceinline__ void copy_async(unsigned dst, const void* src, int bytes, int words16) {
+    if (words16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// rows 0 .. n of L (the rest zero) of a tile of nc channels, row 0 at p, to dst
+template <typename T, int COPY, int L>
+__device__ __forceinline__ void stage_rows(unsigned dst, const T* p, long long st, int n, int nc, int lane) {
+    constexpr int E = (int)sizeof(T);
+    if constexpr (COPY == 16) {
+        const int ch = lane & 7, r0 = lane >> 3;
+        const int most = ch * 16 < nc * E ? n : 0;
+        const char* q = reinterpret_cast<const char*>(p) + (r0 * st * E + ch * 16);
+#pragma unroll
+        for (int i = 0; i < L; i += 4)
+            copy_async(dst + (r0 + i) * 128 + ch * 16, r0 + i < most ? q + (long long)i * E * st : (const char*)p,
+                       r0 + i < most ? 16 : 0, 1);
+    } else if constexpr (COPY == 4) {
+        const int most = lane * 4 < nc * E ? n : 0;
+        const char* q = reinterpret_cast<const char*>(p) + lane * 4;
+#pragma unroll
+        for (int i = 0; i < L; ++i)
+            copy_async(dst + i * 128 + lane * 4, i < most ? q + (long long)i * E * st : (const char*)((uintptr_t)p & ~3ull),
+                       i < most ? 4 : 0, 0);
+    } else {
+        const uintptr_t any = (uintptr_t)p & ~(uintptr_t)3;
+        auto half = [&](int e) { return e + 1 < nc ? 4 : e >= 0 && e < nc ? 2 : 0; };  // bytes of the word at element e
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            const uintptr_t q = (uintptr_t)(p + i * st);
+            const int b = i < n ? half(2 * lane - (int)((q >> 1) & 1)) : 0;
+            copy_async(dst + i * 132 + lane * 4, (const void*)(b ? (q & ~(uintptr_t)3) + lane * 4 : any), b, 0);
+        }
+        if (lane < L) {
+            const uintptr_t q = (uintptr_t)(p + lane * st);
+            const int b = lane < n && ((q >> 1) & 1) && 63 < nc ? 2 : 0;
+            copy_async(dst + lane * 132 + 128, (const void*)(b ? (q & ~(uintptr_t)3) + 128 : any), b, 0);
+        }
+    }
+}
+// the lane's word of row i; odd: the row begins in the upper half of its first word
+template <int COPY>
+__device__ __forceinline__ unsigned staged(const char* rows, int i, int lane, unsigned odd) {
+    const unsigned* r = reinterpret_cast<const unsigned*>(rows + i * row_bytes<COPY>) + lane;
+    if constexpr (COPY == 2) return __funnelshift_r(r[0], r[1], odd * 16);
+    return r[0];
+}
+template <int COPY, typename T>
+__device__ __forceinline__ unsigned odd_row(const T* p, long long st, int i) {
+    return COPY == 2 ? (unsigned)(((uintptr_t)p >> 1) + (uintptr_t)(i * st)) & 1u : 0u;
+}
+// the lane's channels of a written row
+template <typename T, int COPY>
+__device__ __forceinline__ void write_row(T* p, const Vec<lane_channels<T>>& x, int nl) {
+    const unsigned w = Unpack<T>::put(x);
+    if constexpr (COPY == 2) {
+        reinterpret_cast<unsigned short*>(p)[0] = (unsigned short)w;
+        if (nl > 1) reinterpret_cast<unsigned short*>(p)[1] = (unsigned short)(w >> 16);
+    } else {
+        *reinterpret_cast<unsigned*>(p) = w;
+    }
+}
+template <int V>
+__device__ __forceinline__ Vec<V> load_n(const float* p, int nl) {
+    Vec<V> r;
+#pragma unroll
+    for (int k = 0; k < V; ++k) r.v[k] = k < nl ? p[k] : 0.0f;
+    return r;
+}
+template <int V>
+__device__ __forceinline__ void store_n(float* p, const Vec<V>& x, int nl) {
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+        if (k < nl) p[k] = x.v[k];
+}
+
+// A raster's words of L rows of a tile: lane (row, word) holds one (V words a row)
+template <int V, int L>
+__device__ __forceinline__ unsigned raster_word(const unsigned* p, long long st, int n, int words, int lane) {
+    const int r = lane / V, k = lane % V;
+    return r < L && r < n && k < words ? p[r * st + k] : 0u;
+}
+template <int V>
+__device__ __forceinline__ Vec<V> raster_values(unsigned held, int i, int lane) {
+    const unsigned w = __shfl_sync(~0u, held, i * V + lane * V / 32);
+    Vec<V> r;
+#pragma unroll
+    for (int k = 0; k < V; ++k) r.v[k] = (w >> ((lane * V + k) & 31)) & 1u ? 1.0f : 0.0f;
+    return r;
+}
+
+template <typename T, int GM, bool RASTER, int COPY>
+struct FwdStage {  // a warp's staged rows
+    static constexpr int gate = 0, x = per_channel<GM> ? 0 : L_FWD * row_bytes<COPY>;
+    static constexpr int bytes = x + (RASTER ? 0 : L_FWD * row_bytes<COPY>);
+};
+template <typename T, int GM, bool RASTER, int COPY>
+struct BwdStage {
+    static constexpr int gate = 0, x = per_channel<GM> ? 0 : L_BWD * row_bytes<COPY>;
+    static constexpr int dy = x + (RASTER ? 0 : L_BWD * row_bytes<COPY>), bytes = dy + L_BWD * row_bytes<COPY>;
+};
+
+template <typename T, int GM, bool RASTER, bool LEAKY, int COPY>
 __global__ void __launch_bounds__(TILE_THREADS, 2) k_scan_tile(const ScanArgs A) {
-    constexpr int L = fwd_steps<T>, TT = W * L;
-    constexpr bool LO = keeps_lo<T, GM>;
-    using G = Word<T, V>;
-    using X = InWord<T, V, RASTER>;
-    using XE = std::conditional_t<RASTER, unsigned, T>;
+    constexpr int L = L_FWD, TT = W * L, V = lane_channels<T>, S = S_FWD;
+    constexpr bool LO = keeps_lo<T, GM>, PC = per_channel<GM>;
+    using Stage = FwdStage<T, GM, RASTER, COPY>;
+    extern __shared__ __align__(16) char rows[];
     __shared__ Vec<V> sa[2][W][32], sh[2][W][32];
     __shared__ ClusterMaps<V> cm;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int CL = A.cluster, rank = blockIdx.x % CL, item = blockIdx.x / CL;
-    const int c = (item % A.ctiles * 32 + lane) * V;
-    const bool live = c < A.D;
+    const int c0 = item % A.ctiles * 32 * V, c = c0 + lane * V;
+    const int nc = min(32 * V, A.D - c0), nl = min(V, A.D - c);  // channels of the tile, of the lane (<= 0: none)
+    char* const mine = rows + w * S * Stage::bytes;
+    const unsigned mine_s = (unsigned)__cvta_generic_to_shared(mine);
     Decay<V, LO> fixed;
     Vec<V> factor = splat<V>(1.0f);
-    if (per_channel<GM>) {
-        channel_decays<T, GM, V>(A, c, live, fixed, factor);
-        if (!A.leaky) factor = splat<V>(1.0f);
-    }
+    if (PC) channel_decays<T, GM, V>(A, c, nl, fixed, factor);
     int par = 0;
     for (long long s = item / A.ctiles; s < A.n_seq; s += A.workers) {
         const Span sp = span_of(A, s);
-        Vec<V> carry = load_f32<V>(A.h0 + s * A.D + c, A.h0 && live);
+        Vec<V> carry = load_n<V>(A.h0 + s * A.D + c, A.h0 ? nl : 0);
         if (sp.len == 0) {
-            if (A.h && live && rank == 0 && w == 0) store_f32<V>(A.h + s * A.D + c, carry);
+            if (A.h && rank == 0 && w == 0) store_n<V>(A.h + s * A.D + c, carry, nl);
             continue;
         }
-        const T* pg = reinterpret_cast<const T*>(A.gate.p) + row_at(A, A.gate, s, sp, 0) + c;
-        const XE* px = reinterpret_cast<const XE*>(A.x.p) + row_at(A, A.x, s, sp, 0) + (RASTER ? c >> 5 : c);
+        const T* pg = reinterpret_cast<const T*>(A.gate.p) + row_at(A, A.gate, s, sp, 0) + c0;
+        const T* px = reinterpret_cast<const T*>(A.x.p) + row_at(A, A.x, s, sp, 0) + c0;
+        const unsigned* pw = reinterpret_cast<const unsigned*>(A.x.p) + row_at(A, A.x, s, sp, 0) + (c0 >> 5);
         T* py = reinterpret_cast<T*>(A.y.p) + row_at(A, A.y, s, sp, 0) + c;
-        G rg[L];
-        X rx[L];
-        auto fetch = [&](long long t0) {
-            const T* qg = pg + t0 * A.gate.st;
-            const XE* qx = px + t0 * A.x.st;
-            const int n = live ? (int)min((long long)L, sp.len - t0) : 0;
-            if (n == L) {
-#pragma unroll
-                for (int i = 0; i < L; ++i) {
-                    if (!per_channel<GM>) rg[i] = *reinterpret_cast<const G*>(qg + i * A.gate.st);
-                    rx[i] = *reinterpret_cast<const X*>(qx + i * A.x.st);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < L; ++i) {
-                    if (i >= n) continue;
-                    if (!per_channel<GM>) rg[i] = *reinterpret_cast<const G*>(qg + i * A.gate.st);
-                    rx[i] = *reinterpret_cast<const X*>(qx + i * A.x.st);
-                }
-            }
-        };
-#pragma unroll
-        for (int i = 0; i < L; ++i) {
-            memset(&rg[i], 0, sizeof(G));
-            memset(&rx[i], 0, sizeof(X));
-        }
         const long long round = (long long)CL * TT;
-        fetch((long long)rank * TT + w * L);
+        unsigned words = 0;
+        auto fetch = [&](long long t, int slot) {  // this warp's steps from t on
+            const int n = (int)max(0ll, min((long long)L, sp.len - t));
+            const unsigned dst = mine_s + slot * Stage::bytes;
+            if (n > 0) {
+                if (!PC) stage_rows<T, COPY, L>(dst + Stage::gate, pg + t * A.gate.st, A.gate.st, n, nc, lane);
+                if (!RASTER) stage_rows<T, COPY, L>(dst + Stage::x, px + t * A.x.st, A.x.st, n, nc, lane);
+            }
+            copy_commit();
+        };
+        auto fetch_words = [&](long long t) {
+            if (RASTER)
+                words = t < sp.len ? raster_word<V, L>(pw + t * A.x.st, A.x.st, (int)min((long long)L, sp.len - t),
+                                                       (nc + 31) >> 5, lane)
+                                   : 0u;
+        };
+        const long long t1 = (long long)rank * TT + w * L;
+        for (int k = 0; k < S; ++k) fetch(t1 + k * round, k);
+        fetch_words(t1);
+        int slot = 0;
         for (long long b = 0; b < sp.len; b += round) {
-            const long long t0 = b + (long long)rank * TT + w * L;
-            Decay<V, LO> d[per_channel<GM> ? 1 : L];
+            const long long t0 = b + t1;
+            Decay<V, LO> d[PC ? 1 : L];
             Vec<V> u[L];
+            copy_wait<S - 1>();
+            __syncwarp();
+            const char* from = mine + slot * Stage::bytes;
+            const unsigned held = words;
 #pragma unroll
             for (int i = 0; i < L; ++i) {
                 Vec<V> f = factor;
-                if (!per_channel<GM>) {
-                    decays<T, GM, V>(Unpack<T>::get(rg[i]), d[i], f);
-                    if (!A.leaky) f = splat<V>(1.0f);
-                }
-                u[i] = vmul(f, in_values<T, V, RASTER>(rx[i], c));
+                if (!PC)
+                    decays<T, GM, V>(Unpack<T>::get(staged<COPY>(from + Stage::gate, i, lane,
+                                                                 odd_row<COPY>(pg + t0 * A.gate.st, A.gate.st, i))),
+                                     d[i], f);
+                if constexpr (RASTER) u[i] = raster_values<V>(held, i, lane);
+                else u[i] = Unpack<T>::get(staged<COPY>(from + Stage::x, i, lane, odd_row<COPY>(px + t0 * A.x.st, A.x.st, i)));
+                if (LEAKY) u[i] = vmul(f, u[i]);
             }
-            if (per_channel<GM>) d[0] = fixed;
-            if (b + round < sp.len) fetch(t0 + round);
+            if (PC) d[0] = fixed;
+            __syncwarp();
+            fetch(t0 + S * round, slot);
+            fetch_words(t0 + round);
+            slot = slot + 1 == S ? 0 : slot + 1;
             Vec<V> a = splat<V>(1.0f), h = splat<V>(0.0f);
 #pragma unroll
             for (int i = 0; i < L; ++i) {
-                const Decay<V, LO>& q = d[per_channel<GM> ? 0 : i];
+                const Decay<V, LO>& q = d[PC ? 0 : i];
                 h = q.step(h, u[i]);
                 a = q.times(a);
             }
             sa[par][w][lane] = a;
             sh[par][w][lane] = h;
             __syncthreads();
-            if (CL > 1) {
-                if (w == 0) {
-                    Vec<V> ta = splat<V>(1.0f), th = splat<V>(0.0f);
+            // the maps of the warps before this one (a, h) and of the whole tile (ta, th)
+            Vec<V> ta = splat<V>(1.0f), th = CL > 1 ? splat<V>(0.0f) : carry;
 #pragma unroll
-                    for (int j = 0; j < W; ++j) {
-                        th = vfma(sa[par][j][lane], th, sh[par][j][lane]);
-                        ta = vmul(sa[par][j][lane], ta);
-                    }
-                    for (int r = 0; r < CL; ++r) {
-                        store_peer<V>(&cm.a[par][rank][lane], r, ta);
-                        store_peer<V>(&cm.h[par][rank][lane], r, th);
-                    }
+            for (int j = 0; j < W; ++j) {
+                if (j == w) {
+                    a = ta;
+                    h = th;
+                }
+                const Vec<V> ja = sa[par][j][lane];
+                th = vfma(ja, th, sh[par][j][lane]);
+                ta = vmul(ja, ta);
+            }
+            if (CL > 1) {
+                for (int r = w; r < CL; r += W) {
+                    store_peer<V>(&cm.a[par][rank][lane], r, ta);
+                    store_peer<V>(&cm.h[par][rank][lane], r, th);
                 }
                 cluster_sync();
-            }
-            h = carry;
-            if (CL > 1) {
-                for (int r = 0; r < rank; ++r) h = vfma(cm.a[par][r][lane], h, cm.h[par][r][lane]);
-                carry = h;
-                for (int r = rank; r < CL; ++r) carry = vfma(cm.a[par][r][lane], carry, cm.h[par][r][lane]);
-            }
-            for (int j = 0; j < w; ++j) h = vfma(sa[par][j][lane], h, sh[par][j][lane]);
-            if (CL == 1) {
-                carry = h;
-                for (int j = w; j < W; ++j) carry = vfma(sa[par][j][lane], carry, sh[par][j][lane]);
+                Vec<V> in = carry;
+                for (int r = 0; r < CL; ++r) {
+                    if (r == rank) in = carry;
+                    carry = vfma(cm.a[par][r][lane], carry, cm.h[par][r][lane]);
+                }
+                h = vfma(a, in, h);
+            } else {
+                carry = th;
             }
             par ^= 1;
-            if (!live || t0 >= sp.len) continue;
-            if (A.saved && t0 % BLOCK == 0) store_f32<V>(A.saved + (sp.block0 + t0 / BLOCK) * A.D + c, h);
+            if (nl <= 0 || t0 >= sp.len) continue;
+            if (A.saved && t0 % BLOCK == 0) store_n<V>(A.saved + (sp.block0 + t0 / BLOCK) * A.D + c, h, nl);
             T* qy = py + t0 * A.y.st;
             const int n = (int)min((long long)L, sp.len - t0);
 #pragma unroll
             for (int i = 0; i < L; ++i) {
                 if (i < n) {
-                    h = d[per_channel<GM> ? 0 : i].step(h, u[i]);
-                    *reinterpret_cast<G*>(qy) = Unpack<T>::put(h);
+                    h = d[PC ? 0 : i].step(h, u[i]);
+                    write_row<T, COPY>(qy, h, nl);
                 }
                 qy += A.y.st;
             }
-            if (A.h && t0 + n == sp.len) store_f32<V>(A.h + s * A.D + c, h);
+            if (A.h && t0 + n == sp.len) store_n<V>(A.h + s * A.D + c, h, nl);
         }
+        copy_wait<0>();
+        __syncwarp();
     }
 }
 
 // The gradient runs from the last tile to the first.  With r the gradient that
 // reaches a step from later ones, g = o + r and r' = a g: the map of a tile is
 // r -> A r + R.  The states inside the tile come from its saved first state.
-template <typename T, int GM, bool RASTER, int V>
+template <typename T, int GM, bool RASTER, bool LEAKY, int COPY>
 __global__ void __launch_bounds__(TILE_THREADS, 2) k_scan_grad_tile(const ScanArgs A) {
-    constexpr int L = L_BWD, TT = W * L;
+    constexpr int L = L_BWD, TT = W * L, V = lane_channels<T>, S = S_BWD;
     constexpr bool LO = keeps_lo<T, GM>, PC = per_channel<GM>;
-    using G = Word<T, V>;
-    using X = InWord<T, V, RASTER>;
-    using XE = std::conditional_t<RASTER, unsigned, T>;
+    using Stage = BwdStage<T, GM, RASTER, COPY>;
+    extern __shared__ __align__(16) char rows[];
     __shared__ Vec<V> sa[2][W][32], sh[2][W][32], sr[2][W][32];
     __shared__ ClusterMaps<V> cm;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int CL = A.cluster, rank = blockIdx.x % CL, item = blockIdx.x / CL;
-    const int c = (item % A.ctiles * 32 + lane) * V;
-    const bool live = c < A.D;
-    const Vec<V> one = splat<V>(1.0f), minus = splat<V>(A.leaky ? -1.0f : 0.0f);
+    const int c0 = item % A.ctiles * 32 * V, c = c0 + lane * V;
+    const int nc = min(32 * V, A.D - c0), nl = min(V, A.D - c);
+    char* const mine = rows + w * S * Stage::bytes;
+    const unsigned mine_s = (unsigned)__cvta_generic_to_shared(mine);
+    const Vec<V> one = splat<V>(1.0f), minus = splat<V>(-1.0f);
     Decay<V, LO> fixed;
     Vec<V> factor = one, sum = splat<V>(0.0f);
-    if (PC) {
-        channel_decays<T, GM, V>(A, c, live, fixed, factor);
-        if (!A.leaky) factor = one;
-    }
+    if (PC) channel_decays<T, GM, V>(A, c, nl, fixed, factor);
     int par = 0;
     for (long long s = item / A.ctiles; s < A.n_seq; s += A.workers) {
         const Span sp = span_of(A, s);
         Vec<V> carry = splat<V>(0.0f);
         if (sp.len == 0) {
-            if (A.dh0 && live && rank == 0 && w == 0)
-                store_f32<V>(A.dh0 + s * A.D + c, load_f32<V>(A.dh + s * A.D + c, A.dh != nullptr));
+            if (A.dh0 && rank == 0 && w == 0)
+                store_n<V>(A.dh0 + s * A.D + c, load_n<V>(A.dh + s * A.D + c, A.dh ? nl : 0), nl);
             continue;
         }
-        const T* pg = reinterpret_cast<const T*>(A.gate.p) + row_at(A, A.gate, s, sp, 0) + c;
-        const XE* px = reinterpret_cast<const XE*>(A.x.p) + row_at(A, A.x, s, sp, 0) + (RASTER ? c >> 5 : c);
-        const T* pd = reinterpret_cast<const T*>(A.y.p) + row_at(A, A.y, s, sp, 0) + c;
+        const T* pg = reinterpret_cast<const T*>(A.gate.p) + row_at(A, A.gate, s, sp, 0) + c0;
+        const T* px = reinterpret_cast<const T*>(A.x.p) + row_at(A, A.x, s, sp, 0) + c0;
+        const unsigned* pw = reinterpret_cast<const unsigned*>(A.x.p) + row_at(A, A.x, s, sp, 0) + (c0 >> 5);
+        const T* pd = reinterpret_cast<const T*>(A.y.p) + row_at(A, A.y, s, sp, 0) + c0;
         T* pdg = reinterpret_cast<T*>(A.dgate.p) + (PC ? 0 : row_at(A, A.dgate, s, sp, 0) + c);
         T* pdx = reinterpret_cast<T*>(A.dx.p) + row_at(A, A.dx, s, sp, 0) + c;
-        G rg[L], rd[L];
-        X rx[L];
-        Vec<V> rs = splat<V>(0.0f);
-        auto fetch = [&](long long t0) {
-            if (t0 < 0) return;
-            const T* qg = pg + t0 * A.gate.st;
-            const T* qd = pd + t0 * A.y.st;
-            const XE* qx = px + t0 * A.x.st;
-            const int n = live ? (int)min((long long)L, sp.len - t0) : 0;
-            if (n == L && A.y.p) {
-#pragma unroll
-                for (int i = 0; i < L; ++i) {
-                    if (!PC) rg[i] = *reinterpret_cast<const G*>(qg + i * A.gate.st);
-                    rx[i] = *reinterpret_cast<const X*>(qx + i * A.x.st);
-                    rd[i] = *reinterpret_cast<const G*>(qd + i * A.y.st);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < L; ++i) {
-                    if (i >= n) continue;
-                    if (!PC) rg[i] = *reinterpret_cast<const G*>(qg + i * A.gate.st);
-                    rx[i] = *reinterpret_cast<const X*>(qx + i * A.x.st);
-                    if (A.y.p) rd[i] = *reinterpret_cast<const G*>(qd + i * A.y.st);
-                }
+        Vec<V> first = splat<V>(0.0f);
+        unsigned words = 0;
+        auto fetch = [&](long long t, int slot) {
+            if (t >= 0 && t < sp.len) {
+                const int n = (int)min((long long)L, sp.len - t);
+                const unsigned dst = mine_s + slot * Stage::bytes;
+                if (!PC) stage_rows<T, COPY, L>(dst + Stage::gate, pg + t * A.gate.st, A.gate.st, n, nc, lane);
+                if (!RASTER) stage_rows<T, COPY, L>(dst + Stage::x, px + t * A.x.st, A.x.st, n, nc, lane);
+                if (A.y.p) stage_rows<T, COPY, L>(dst + Stage::dy, pd + t * A.y.st, A.y.st, n, nc, lane);
             }
-            rs = load_f32<V>(A.saved + (sp.block0 + t0 / BLOCK) * A.D + c, live);
+            copy_commit();
         };
-#pragma unroll
-        for (int i = 0; i < L; ++i) {
-            memset(&rg[i], 0, sizeof(G));
-            memset(&rd[i], 0, sizeof(G));
-            memset(&rx[i], 0, sizeof(X));
-        }
-        const long long tiles = (sp.len + TT - 1) / TT;
-        fetch((tiles - 1 - rank) * TT + w * L);
+        auto fetch_words = [&](long long t) {
+            if (t >= 0) first = load_n<V>(A.saved + (sp.block0 + t / BLOCK) * A.D + c, nl);
+            if (RASTER)
+                words = t >= 0 && t < sp.len ? raster_word<V, L>(pw + t * A.x.st, A.x.st, (int)min((long long)L, sp.len - t),
+                                                                 (nc + 31) >> 5, lane)
+                                             : 0u;
+        };
+        const long long tiles = (sp.len + TT - 1) / TT, round = (long long)CL * TT;
+        const long long t1 = (tiles - 1 - rank) * TT + w * L;
+        for (int k = 0; k < S; ++k) fetch(t1 - k * round, k);
+        fetch_words(t1);
+        int slot = 0;
         for (long long b = 0; b < tiles; b += CL) {
-            const long long t0 = (tiles - 1 - b - rank) * TT + w * L;  // negative: no tile left for this CTA
+            const long long t0 = t1 - b * TT;  // negative: no tile left for this CTA
+            const bool some = t0 >= 0 && t0 < sp.len;
             Decay<V, LO> d[PC ? 1 : L];
             Vec<V> rest[PC ? 1 : L], x[L], o[L];
+            copy_wait<S - 1>();
+            __syncwarp();
+            const char* from = mine + slot * Stage::bytes;
+            const unsigned held = words;
+            const Vec<V> h0 = first;
 #pragma unroll
             for (int i = 0; i < L; ++i) {
-                if (!PC) decays<T, GM, V>(Unpack<T>::get(rg[i]), d[i], rest[i]);
-                x[i] = in_values<T, V, RASTER>(rx[i], c);
-                o[i] = Unpack<T>::get(rd[i]);
-                if (t0 + i == sp.len - 1) o[i] = vadd(o[i], load_f32<V>(A.dh + s * A.D + c, A.dh && live));
+                if (!PC)
+                    decays<T, GM, V>(Unpack<T>::get(staged<COPY>(from + Stage::gate, i, lane,
+                                                                 odd_row<COPY>(pg + t0 * A.gate.st, A.gate.st, i))),
+                                     d[i], rest[i]);
+                if constexpr (RASTER) x[i] = raster_values<V>(held, i, lane);
+                else x[i] = Unpack<T>::get(staged<COPY>(from + Stage::x, i, lane, odd_row<COPY>(px + t0 * A.x.st, A.x.st, i)));
+                o[i] = splat<V>(0.0f);
+                if (A.y.p && some)
+                    o[i] = Unpack<T>::get(staged<COPY>(from + Stage::dy, i, lane, odd_row<COPY>(pd + t0 * A.y.st, A.y.st, i)));
+            }
+            if (A.dh && some && t0 + L >= sp.len) {  // the last step
+                const Vec<V> dh = load_n<V>(A.dh + s * A.D + c, nl);
+#pragma unroll
+                for (int i = 0; i < L; ++i)
+                    if (t0 + i == sp.len - 1) o[i] = vadd(o[i], dh);
             }
             if (PC) d[0] = fixed;
-            const Vec<V> h0 = rs;
-            if (b + CL < tiles) fetch(t0 - (long long)CL * TT);
+            __syncwarp();
+            fetch(t0 - S * round, slot);
+            fetch_words(t0 - round);
+            slot = slot + 1 == S ? 0 : slot + 1;
             Vec<V> a = one, h = splat<V>(0.0f), r = h;
 #pragma unroll
             for (int i = 0; i < L; ++i) {
                 const Decay<V, LO>& q = d[PC ? 0 : i];
-                const Vec<V> f = PC ? factor : A.leaky ? rest[PC ? 0 : i] : one;
-                h = q.step(h, vmul(f, x[i]));
+                h = q.step(h, LEAKY ? vmul(PC ? factor : rest[PC ? 0 : i], x[i]) : x[i]);
                 a = q.times(a);
                 r = d[PC ? 0 : L - 1 - i].times(vadd(o[L - 1 - i], r));
+            }
+            if (!some) {  // steps behind the end, whose rows were not read: r passes unchanged
+                a = one;
+                r = splat<V>(0.0f);
             }
             sa[par][w][lane] = a;
             sh[par][w][lane] = h;
             sr[par][w][lane] = r;
             __syncthreads();
-            if (CL > 1) {
-                if (w == 0) {
-                    Vec<V> ta = one, tr = splat<V>(0.0f);
+            Vec<V> hw = h0;
 #pragma unroll
-                    for (int j = W - 1; j >= 0; --j) {
-                        tr = vfma(sa[par][j][lane], tr, sr[par][j][lane]);
-                        ta = vmul(sa[par][j][lane], ta);
-                    }
-                    for (int q = 0; q < CL; ++q) {
-                        store_peer<V>(&cm.a[par][rank][lane], q, ta);
-                        store_peer<V>(&cm.h[par][rank][lane], q, tr);
-                    }
+            for (int j = 0; j < W; ++j) {
+                if (j == w) h = hw;
+                if (j < W - 1) hw = vfma(sa[par][j][lane], hw, sh[par][j][lane]);
+            }
+            // the maps of the warps behind this one (a, r) and of the whole tile (ta, tr)
+            Vec<V> ta = one, tr = CL > 1 ? splat<V>(0.0f) : carry;
+#pragma unroll
+            for (int j = W - 1; j >= 0; --j) {
+                if (j == w) {
+                    a = ta;
+                    r = tr;
+                }
+                const Vec<V> ja = sa[par][j][lane];
+                tr = vfma(ja, tr, sr[par][j][lane]);
+                ta = vmul(ja, ta);
+            }
+            if (CL > 1) {
+                for (int q = w; q < CL; q += W) {
+                    store_peer<V>(&cm.a[par][rank][lane], q, ta);
+                    store_peer<V>(&cm.h[par][rank][lane], q, tr);
                 }
                 cluster_sync();
-            }
-            h = h0;
-            for (int j = 0; j < w; ++j) h = vfma(sa[par][j][lane], h, sh[par][j][lane]);
-            r = carry;
-            if (CL > 1) {
-                for (int q = 0; q < rank; ++q) r = vfma(cm.a[par][q][lane], r, cm.h[par][q][lane]);
-                carry = r;
-                for (int q = rank; q < CL; ++q) carry = vfma(cm.a[par][q][lane], carry, cm.h[par][q][lane]);
-            }
-            for (int j = W - 1; j > w; --j) r = vfma(sa[par][j][lane], r, sr[par][j][lane]);
-            if (CL == 1) {
-                carry = r;
-                for (int j = w; j >= 0; --j) carry = vfma(sa[par][j][lane], carry, sr[par][j][lane]);
+                Vec<V> in = carry;
+                for (int q = 0; q < CL; ++q) {
+                    if (q == rank) in = carry;
+                    carry = vfma(cm.a[par][q][lane], carry, cm.h[par][q][lane]);
+                }
+                r = vfma(a, in, r);
+            } else {
+                carry = tr;
             }
             par ^= 1;
-            if (!live || t0 < 0 || t0 >= sp.len) continue;
+            if (nl <= 0 || !some) continue;
             // x becomes the derivative of h_t in a_t: h_{t-1}, or h_{t-1} - x_t
 #pragma unroll
             for (int i = 0; i < L; ++i) {
-                const Vec<V> f = PC ? factor : A.leaky ? rest[PC ? 0 : i] : one;
                 const Vec<V> before = h, xi = x[i];
-                h = d[PC ? 0 : i].step(h, vmul(f, xi));
-                x[i] = A.leaky ? vfma(minus, xi, before) : before;
+                h = d[PC ? 0 : i].step(h, LEAKY ? vmul(PC ? factor : rest[PC ? 0 : i], xi) : xi);
+                x[i] = LEAKY ? vfma(minus, xi, before) : before;
             }
             const int n = (int)min((long long)L, sp.len - t0);
             T* qg = pdg + (t0 + L - 1) * A.dgate.st;
@@ -609,32 +757,33 @@ __global__ void __launch_bounds__(TILE_THREADS, 2) k_scan_grad_tile(const ScanAr
             for (int i = L - 1; i >= 0; --i) {
                 if (i < n) {
                     const Decay<V, LO>& q = d[PC ? 0 : i];
-                    const Vec<V> f = PC ? factor : A.leaky ? rest[PC ? 0 : i] : one;
                     const Vec<V> g = vadd(o[i], r);
                     if (PC) {
                         sum = vfma(g, x[i], sum);
                     } else if (A.dgate.p) {
                         Vec<V> da = vmul(g, x[i]);
                         if (GM == GATE_LOGIT) da = vmul(da, vmul(q.a, rest[PC ? 0 : i]));
-                        *reinterpret_cast<G*>(qg) = Unpack<T>::put(da);
+                        write_row<T, COPY>(qg, da, nl);
                     }
-                    if (A.dx.p) *reinterpret_cast<G*>(qx) = Unpack<T>::put(vmul(f, g));
+                    if (A.dx.p) write_row<T, COPY>(qx, LEAKY ? vmul(PC ? factor : rest[PC ? 0 : i], g) : g, nl);
                     r = q.times(g);
                 }
                 qg -= A.dgate.st;
                 qx -= A.dx.st;
             }
-            if (t0 == 0 && A.dh0) store_f32<V>(A.dh0 + s * A.D + c, r);
+            if (t0 == 0 && A.dh0) store_n<V>(A.dh0 + s * A.D + c, r, nl);
         }
+        copy_wait<0>();
+        __syncwarp();
     }
     if (PC && A.part) {
         __syncthreads();
         sa[0][w][lane] = sum;
         __syncthreads();
-        if (w == 0 && live) {
+        if (w == 0 && nl > 0) {
             Vec<V> t = splat<V>(0.0f);
             for (int j = 0; j < W; ++j) t = vadd(t, sa[0][j][lane]);
-            store_f32<V>(A.part + ((long long)(item / A.ctiles) * CL + rank) * A.D + c, t);
+            store_n<V>(A.part + ((long long)(item / A.ctiles) * CL + rank) * A.D + c, t, nl);
         }
     }
 }
@@ -735,16 +884,13 @@ void dispatch(const snn_scan* d, F&& f) {
 // that leaves SMs empty, a cluster of up to MAX_CLUSTER CTAs along the steps.
 constexpr int SMS = 148;
 struct Plan {
-    int vec, ctiles, workers, cluster;
+    int ctiles, workers, cluster;
 };
-bool fits_vec(const Rows& r, int size, int vec) {
-    return (uintptr_t)r.p % (size * vec) == 0 && r.ss % vec == 0 && r.st % vec == 0;
-}
 int64_t mean_steps(const snn_scan* d) { return d->offsets ? d->n_steps / std::max<int64_t>(d->n_seq, 1) : d->n_steps; }
-Plan plan_of(const snn_scan* d, int vec, int tile) {
+Plan plan_of(const snn_scan* d, int tile) {
+    const int width = 128 / snnb::elem_size(d->type);
     Plan p;
-    p.vec = vec;
-    p.ctiles = (int)((d->n_channels + 32 * vec - 1) / (32 * vec));
+    p.ctiles = (int)((d->n_channels + width - 1) / width);
     p.workers = (int)std::min<int64_t>(d->n_seq, std::max(32, 32 * SMS / p.ctiles));
     p.cluster = 1;
     while (p.cluster < MAX_CLUSTER && (int64_t)p.ctiles * p.workers * p.cluster < 2 * SMS &&
@@ -753,7 +899,23 @@ Plan plan_of(const snn_scan* d, int vec, int tile) {
     return p;
 }
 
-void launch(const void* kernel, const Plan& p, ScanArgs& A, cudaStream_t st) {
+// whether r's rows are words of `bytes` from the first element on
+bool fits(const Rows& r, int size, int bytes) {
+    return (uintptr_t)r.p % bytes == 0 && r.ss * size % bytes == 0 && r.st * size % bytes == 0;
+}
+// The words that rows are staged in (see stage_rows); written rows go in 4-byte
+// words, or in the third form an element at a time.
+int copy_words(const snn_scan* d, std::initializer_list<Rows> in, std::initializer_list<Rows> out) {
+    const int size = snnb::elem_size(d->type);
+    auto all = [&](std::initializer_list<Rows> rows, int bytes) {
+        return d->n_channels * size % bytes == 0 &&
+               std::all_of(rows.begin(), rows.end(), [&](const Rows& r) { return !r.p || fits(r, size, bytes); });
+    };
+    if (!all(in, 4) || !all(out, 4)) return 2;
+    return all(in, 16) ? 16 : 4;
+}
+
+void launch(const void* kernel, int smem, const Plan& p, ScanArgs& A, cudaStream_t st) {
     A.ctiles = p.ctiles;
     A.workers = p.workers;
     A.cluster = p.cluster;
@@ -762,6 +924,7 @@ void launch(const void* kernel, const Plan& p, ScanArgs& A, cudaStream_t st) {
     SNN_REQUIRE((int64_t)p.ctiles * p.workers * p.cluster < (1ll << 31), SNN_ERR_ARG, "scan: too many tiles");
     cfg.gridDim = dim3((unsigned)(p.ctiles * p.workers * p.cluster));
     cfg.blockDim = dim3(TILE_THREADS);
+    cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = st;
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeClusterDimension;
@@ -769,8 +932,23 @@ void launch(const void* kernel, const Plan& p, ScanArgs& A, cudaStream_t st) {
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = p.cluster > 1 ? 1 : 0;
+    SNN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     void* args[] = {&A};
     SNN_CUDA(cudaLaunchKernelExC(&cfg, kernel, args));
+}
+
+template <typename T, int GM, bool RASTER, int COPY>
+void launch_fwd(const Plan& p, ScanArgs& A, cudaStream_t st) {
+    const int smem = W * S_FWD * FwdStage<T, GM, RASTER, COPY>::bytes;
+    launch(A.leaky ? (const void*)k_scan_tile<T, GM, RASTER, true, COPY> : (const void*)k_scan_tile<T, GM, RASTER, false, COPY>,
+           smem, p, A, st);
+}
+template <typename T, int GM, bool RASTER, int COPY>
+void launch_bwd(const Plan& p, ScanArgs& A, cudaStream_t st) {
+    const int smem = W * S_BWD * BwdStage<T, GM, RASTER, COPY>::bytes;
+    launch(A.leaky ? (const void*)k_scan_grad_tile<T, GM, RASTER, true, COPY>
+                   : (const void*)k_scan_grad_tile<T, GM, RASTER, false, COPY>,
+           smem, p, A, st);
 }
 
 }  // namespace
@@ -785,12 +963,8 @@ int64_t leaky_scan_saved(const snn_scan* d) {
 int64_t leaky_scan_grad_workspace(const snn_scan* d) {
     check_desc(d);
     if (!(d->flags & SNN_SCAN_CHANNEL)) return 0;
-    int64_t most = 0;  // of the words that the alignment may choose
-    for (int vec = 1; vec <= 2; ++vec) {
-        const Plan p = plan_of(d, vec, W * L_BWD);
-        most = std::max(most, (int64_t)p.workers * p.cluster * d->n_channels * 4);
-    }
-    return most;
+    const Plan p = plan_of(d, W * L_BWD);
+    return (int64_t)p.workers * p.cluster * d->n_channels * 4;
 }
 
 void leaky_scan(const snn_scan* d, const snn_rows* gate, const snn_rows* x, const float* h0,
@@ -802,31 +976,32 @@ void leaky_scan(const snn_scan* d, const snn_rows* gate, const snn_rows* x, cons
     A.h0 = h0;
     A.h = h;
     A.saved = saved;
-    const int size = elem_size(d->type);
     const bool raster_x = (d->flags & SNN_SCAN_RASTER) != 0, channel = (d->flags & SNN_SCAN_CHANNEL) != 0;
-    const bool two = d->n_channels % 2 == 0 && (channel || fits_vec(A.gate, size, 2)) &&
-                     (raster_x || fits_vec(A.x, size, 2)) && fits_vec(A.y, size, 2);
+    const Rows none = {nullptr, 0, 0};
+    const int words = copy_words(d, {channel ? none : A.gate, raster_x ? none : A.x}, {A.y});
     if (mean_steps(d) <= 8) {
-        const int vec = two ? 2 : 1;
+        const int vec = d->type != SNN_F32 && words > 2 ? 2 : 1;
         const dim3 grid((unsigned)((d->n_channels + 128 * vec - 1) / (128 * vec)),
                         (unsigned)std::min<int64_t>(d->n_seq, 65535));
         dispatch(d, [&](auto t, auto gm, auto raster) {
             using T = decltype(t);
             constexpr int GM = decltype(gm)::value;
             constexpr bool RA = decltype(raster)::value != 0;
-            if (two) k_scan_steps<T, GM, RA, 2><<<grid, 128, 0, st>>>(A);
+            if (vec == 2) k_scan_steps<T, GM, RA, 2><<<grid, 128, 0, st>>>(A);
             else k_scan_steps<T, GM, RA, 1><<<grid, 128, 0, st>>>(A);
         });
         SNN_CUDA(cudaGetLastError());
         return;
     }
-    const Plan p = plan_of(d, two ? 2 : 1, W * (size == 4 ? fwd_steps<float> : fwd_steps<__half>));
+    const Plan p = plan_of(d, W * L_FWD);
     dispatch(d, [&](auto t, auto gm, auto raster) {
         using T = decltype(t);
         constexpr int GM = decltype(gm)::value;
         constexpr bool RA = decltype(raster)::value != 0;
-        if (two) return launch((const void*)k_scan_tile<T, GM, RA, 2>, p, A, st);
-        launch((const void*)k_scan_tile<T, GM, RA, 1>, p, A, st);
+        if (words == 16) return launch_fwd<T, GM, RA, 16>(p, A, st);
+        if constexpr (sizeof(T) == 2)
+            if (words == 2) return launch_fwd<T, GM, RA, 2>(p, A, st);
+        launch_fwd<T, GM, RA, 4>(p, A, st);
     });
 }
 
@@ -859,16 +1034,18 @@ void leaky_scan_grad(const snn_scan* d, const snn_rows* gate, const snn_rows* x,
     } else if (dgate) {
         A.dgate = rows_of(d, dgate, "dgate", d->n_channels, size, true);
     }
-    const bool two = d->n_channels % 2 == 0 && (channel || fits_vec(A.gate, size, 2)) &&
-                     ((d->flags & SNN_SCAN_RASTER) || fits_vec(A.x, size, 2)) && fits_vec(A.y, size, 2) &&
-                     fits_vec(A.dx, size, 2) && (channel || fits_vec(A.dgate, size, 2));
-    const Plan p = plan_of(d, two ? 2 : 1, W * L_BWD);
+    const Rows none = {nullptr, 0, 0};
+    const int words = copy_words(d, {channel ? none : A.gate, d->flags & SNN_SCAN_RASTER ? none : A.x, A.y},
+                                 {channel ? none : A.dgate, A.dx});
+    const Plan p = plan_of(d, W * L_BWD);
     dispatch(d, [&](auto t, auto gm, auto raster) {
         using T = decltype(t);
         constexpr int GM = decltype(gm)::value;
         constexpr bool RA = decltype(raster)::value != 0;
-        if (two) return launch((const void*)k_scan_grad_tile<T, GM, RA, 2>, p, A, st);
-        launch((const void*)k_scan_grad_tile<T, GM, RA, 1>, p, A, st);
+        if (words == 16) return launch_bwd<T, GM, RA, 16>(p, A, st);
+        if constexpr (sizeof(T) == 2)
+            if (words == 2) return launch_bwd<T, GM, RA, 2>(p, A, st);
+        launch_bwd<T, GM, RA, 4>(p, A, st);
     });
     if (A.part) {
         k_scan_gate_sum<<<(unsigned)((d->n_channels + 31) / 32), 256, 0, st>>>(A, p.workers * p.cluster);
