@@ -1,0 +1,5 @@
+// scan_bwd_f32.cu - the leaky scan's gradient tile kernels for f32
+#define SNN_SCAN_TILE_LAUNCH
+#include "scan_tile.h"
+
+template void snnb_scan::launch_tiles<true, float>(int, bool, int, const Plan&, ScanArgs&, cudaStream_t);

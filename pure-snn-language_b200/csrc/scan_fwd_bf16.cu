@@ -1,0 +1,5 @@
+// scan_fwd_bf16.cu - the leaky scan's forward tile kernels for bf16
+#define SNN_SCAN_TILE_LAUNCH
+#include "scan_tile.h"
+
+template void snnb_scan::launch_tiles<false, __nv_bfloat16>(int, bool, int, const Plan&, ScanArgs&, cudaStream_t);

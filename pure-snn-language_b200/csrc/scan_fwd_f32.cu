@@ -1,0 +1,5 @@
+// scan_fwd_f32.cu - the leaky scan's forward tile kernels for f32
+#define SNN_SCAN_TILE_LAUNCH
+#include "scan_tile.h"
+
+template void snnb_scan::launch_tiles<false, float>(int, bool, int, const Plan&, ScanArgs&, cudaStream_t);

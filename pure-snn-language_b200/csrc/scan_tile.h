@@ -1,0 +1,870 @@
+// scan_tile.h - the leaky scan's kernels over tiles of steps and channels
+// (k_scan_tile, k_scan_grad_tile) and what they share with scan.cu.  Each
+// element type and direction is compiled by a file of its own (scan_*.cu).
+#pragma once
+#include <algorithm>
+#include "elem.h"
+
+namespace snnb_scan {
+using snnb::from_f32;
+using snnb::to_f32;
+
+// Steps between two states that the forward pass keeps for the backward pass.
+// The backward pass recomputes the states inside a block from the inputs that
+// it reads anyway: 4 bytes per 32 steps and channel instead of a second read
+// of y, and the states stay f32.
+constexpr int BLOCK = 32;
+
+// how the decays are given: per step, as they are or as logits; per channel
+enum { GATE_VALUE = 0, GATE_LOGIT = 1, GATE_CHANNEL = 2, GATE_CHANNEL_LOGIT = 3 };
+template <int GM> constexpr bool per_channel = GM >= GATE_CHANNEL;
+template <int GM> constexpr bool is_logit = (GM & 1) != 0;
+
+struct Rows {
+    void* p;
+    long long ss, st;
+};
+
+struct ScanArgs {
+    const int64_t* off;
+    long long n_seq;
+    int n_steps, D, logit, leaky;
+    Rows gate, x, y, dgate, dx;
+    const float* h0;
+    float* h;
+    float* saved;
+    const float* dh;
+    float* dh0;
+    float* part;   // per-CTA sums of a channel gate's gradient
+    int ctiles, workers, cluster;
+};
+
+// rows of sequence s: [begin, begin + len) of the flat row index (packed), or
+// of the sequence itself (dense)
+struct Span {
+    long long begin, block0;
+    int len;
+};
+__device__ __forceinline__ Span span_of(const ScanArgs& A, long long s) {
+    Span r;
+    long long flat;
+    if (A.off) {
+        const long long b = min(max((long long)A.off[s], 0ll), (long long)A.n_steps);
+        const long long e = min(max((long long)A.off[s + 1], b), (long long)A.n_steps);
+        r.begin = flat = b;
+        r.len = (int)(e - b);
+    } else {
+        flat = s * A.n_steps;
+        r.begin = 0;
+        r.len = A.n_steps;
+    }
+    // first block of the sequence among the saved states: floor(flat / BLOCK) + s
+    // leaves room for ceil(len / BLOCK) blocks in every sequence, whatever the lengths
+    r.block0 = flat / BLOCK + s;
+    return r;
+}
+__device__ __forceinline__ long long row_at(const ScanArgs& A, const Rows& r, long long s, const Span& sp, long long t) {
+    return A.off ? (sp.begin + t) * r.st : s * r.ss + t * r.st;
+}
+
+// V values side by side; pairs go through the packed f32 instructions
+template <int V>
+struct Vec {
+    float v[V];
+};
+template <int V>
+__device__ __forceinline__ Vec<V> splat(float x) {
+    Vec<V> r;
+#pragma unroll
+    for (int k = 0; k < V; ++k) r.v[k] = x;
+    return r;
+}
+__device__ __forceinline__ Vec<1> vfma(Vec<1> a, Vec<1> b, Vec<1> c) { return {fmaf(a.v[0], b.v[0], c.v[0])}; }
+__device__ __forceinline__ Vec<1> vmul(Vec<1> a, Vec<1> b) { return {a.v[0] * b.v[0]}; }
+__device__ __forceinline__ Vec<1> vadd(Vec<1> a, Vec<1> b) { return {a.v[0] + b.v[0]}; }
+__device__ __forceinline__ Vec<2> vfma(Vec<2> a, Vec<2> b, Vec<2> c) {
+    Vec<2> d;
+    asm("{.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;}"
+        : "=f"(d.v[0]), "=f"(d.v[1])
+        : "f"(a.v[0]), "f"(a.v[1]), "f"(b.v[0]), "f"(b.v[1]), "f"(c.v[0]), "f"(c.v[1]));
+    return d;
+}
+__device__ __forceinline__ Vec<2> vmul(Vec<2> a, Vec<2> b) {
+    Vec<2> d;
+    asm("{.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;}"
+        : "=f"(d.v[0]), "=f"(d.v[1])
+        : "f"(a.v[0]), "f"(a.v[1]), "f"(b.v[0]), "f"(b.v[1]));
+    return d;
+}
+__device__ __forceinline__ Vec<2> vadd(Vec<2> a, Vec<2> b) {
+    Vec<2> d;
+    asm("{.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;}"
+        : "=f"(d.v[0]), "=f"(d.v[1])
+        : "f"(a.v[0]), "f"(a.v[1]), "f"(b.v[0]), "f"(b.v[1]));
+    return d;
+}
+
+// The decays of V channels.  A logistic decay near 1 is 1 - s with a small s.
+// Rounded to f32 it is off by up to 2^-25, which a memory of 1 / s steps adds
+// up to 2^-25 / s of the state where the gate stays the same.  Per-channel
+// gates and f32 gates therefore keep what the rounding lost as `lo` (one more
+// FMA a step); 16-bit gates, whose own rounding is 2^-9 and up of the exponent
+// and differs from step to step, do not.  (An infinite state times lo may be
+// NaN: infinities do not survive, they end as infinities or NaN.)
+template <int V, bool LO>
+struct Decay {
+    Vec<V> a;
+    __device__ __forceinline__ Vec<V> step(Vec<V> h, Vec<V> u) const { return vfma(a, h, u); }
+    __device__ __forceinline__ Vec<V> times(Vec<V> h) const { return vmul(a, h); }
+    __device__ __forceinline__ void set_lo(int, float) {}
+};
+template <int V>
+struct Decay<V, true> {
+    Vec<V> a, lo;
+    __device__ __forceinline__ Vec<V> step(Vec<V> h, Vec<V> u) const { return vfma(a, h, vfma(lo, h, u)); }
+    __device__ __forceinline__ Vec<V> times(Vec<V> h) const { return vfma(a, h, vmul(lo, h)); }
+    __device__ __forceinline__ void set_lo(int k, float x) { lo.v[k] = x; }
+};
+template <typename T, int GM>
+constexpr bool keeps_lo = GM == GATE_CHANNEL_LOGIT || (GM == GATE_LOGIT && sizeof(T) == 4);
+
+// decay a = 1 / (1 + exp(-z)) and its rest 1 - a, each with its own relative
+// precision: from e = exp(-|z|) the larger is 1 / (1 + e), the smaller e times
+// that.  exp(-|z|) = 2^p (1 + q ln 2) with p the rounded product -|z| log2(e)
+// and q what its rounding and log2(e)'s own lost: within 2 ulp, as the
+// exponential instruction is, where the product alone would be off by |z|
+// 2^-24.  Beyond |z| = 150 e is 0.
+__device__ __forceinline__ void logistic(float z, float& a, float& lo, float& rest) {
+    const float m = fminf(fabsf(z), 150.0f);
+    const float p = m * -1.44269502f;  // log2(e) = 1.44269502 + 1.9259630e-8
+    const float q = fmaf(m, -1.92596303e-8f, fmaf(m, -1.44269502f, -p));
+    float e, big;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(p));
+    e = fmaf(e, q * 0.693147182f, e);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(big) : "f"(1.0f + e));
+    const float s = e * big;
+    const bool up = z >= 0.0f;
+    const float near1 = 1.0f - s;
+    a = up ? near1 : s;
+    lo = up ? (1.0f - near1) - s : 0.0f;
+    rest = up ? s : big;
+    if (z != z) a = rest = z;
+}
+// the same by the short instructions (2 ulp each, the argument rounded once)
+__device__ __forceinline__ void logistic_fast(float z, float& a, float& rest) {
+    float e, big;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fabsf(z) * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(big) : "f"(1.0f + e));
+    const float s = e * big;
+    const bool up = z >= 0.0f;
+    a = up ? big : s;
+    rest = up ? s : big;
+}
+
+// decay and rest of V gates
+template <typename T, int GM, int V>
+__device__ __forceinline__ void decays(const Vec<V>& z, Decay<V, keeps_lo<T, GM>>& d, Vec<V>& rest) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const float v = z.v[k];
+        float a = v, lo = 0.0f, r = 1.0f - v;
+        if (GM == GATE_LOGIT) {
+            if (sizeof(T) == 4) logistic(v, a, lo, r);
+            else logistic_fast(v, a, r);
+        }
+        d.a.v[k] = a;
+        d.set_lo(k, lo);
+        rest.v[k] = r;
+    }
+}
+// those of the per-channel gates c .. c + V
+template <typename T, int GM, int V>
+__device__ __forceinline__ void channel_decays(const ScanArgs& A, int c, int nl, Decay<V, keeps_lo<T, GM>>& d,
+                                               Vec<V>& rest) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const float v = k < nl ? reinterpret_cast<const float*>(A.gate.p)[c + k] : 0.0f;
+        float a = v, lo = 0.0f, r = 1.0f - v;
+        if (is_logit<GM>) logistic(v, a, lo, r);
+        d.a.v[k] = a;
+        d.set_lo(k, lo);
+        rest.v[k] = r;
+    }
+}
+
+// V elements of type T as the one register (or pair) that a load fills: they
+// are unpacked where they are used, not where they are loaded, so that loads
+// stay in flight
+template <int BYTES>
+struct Raw;
+template <>
+struct Raw<2> {
+    using type = unsigned short;
+};
+template <>
+struct Raw<4> {
+    using type = unsigned;
+};
+template <>
+struct Raw<8> {
+    using type = uint2;
+};
+template <typename T, int V>
+using Word = typename Raw<sizeof(T) * V>::type;
+// what a lane reads of an input row: V elements, or the raster word they lie in
+template <typename T, int V, bool RASTER>
+using InWord = std::conditional_t<RASTER, unsigned, Word<T, V>>;
+
+template <typename T>
+struct Unpack;
+template <>
+struct Unpack<float> {
+    static __device__ __forceinline__ Vec<1> get(unsigned w) { return {__uint_as_float(w)}; }
+    static __device__ __forceinline__ Vec<2> get(uint2 w) { return {__uint_as_float(w.x), __uint_as_float(w.y)}; }
+    static __device__ __forceinline__ unsigned put(Vec<1> x) { return __float_as_uint(x.v[0]); }
+    static __device__ __forceinline__ uint2 put(Vec<2> x) { return {__float_as_uint(x.v[0]), __float_as_uint(x.v[1])}; }
+};
+template <>
+struct Unpack<__nv_bfloat16> {
+    static __device__ __forceinline__ Vec<1> get(unsigned short w) { return {__uint_as_float((unsigned)w << 16)}; }
+    static __device__ __forceinline__ Vec<2> get(unsigned w) {
+        return {__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
+    }
+    static __device__ __forceinline__ unsigned short put(Vec<1> x) {
+        return __bfloat16_as_ushort(__float2bfloat16_rn(x.v[0]));
+    }
+    static __device__ __forceinline__ unsigned put(Vec<2> x) {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(x.v[0], x.v[1]);
+        unsigned r;
+        memcpy(&r, &p, 4);
+        return r;
+    }
+};
+template <>
+struct Unpack<__half> {
+    static __device__ __forceinline__ Vec<1> get(unsigned short w) { return {__half2float(__ushort_as_half(w))}; }
+    static __device__ __forceinline__ Vec<2> get(unsigned w) {
+        __half2 p;
+        memcpy(&p, &w, 4);
+        const float2 f = __half22float2(p);
+        return {f.x, f.y};
+    }
+    static __device__ __forceinline__ unsigned short put(Vec<1> x) { return __half_as_ushort(__float2half_rn(x.v[0])); }
+    static __device__ __forceinline__ unsigned put(Vec<2> x) {
+        const __half2 p = __floats2half2_rn(x.v[0], x.v[1]);
+        unsigned r;
+        memcpy(&r, &p, 4);
+        return r;
+    }
+};
+template <typename T, int V, bool RASTER>
+__device__ __forceinline__ Vec<V> in_values(InWord<T, V, RASTER> w, int c) {
+    if constexpr (RASTER) {
+        Vec<V> r;
+#pragma unroll
+        for (int k = 0; k < V; ++k) r.v[k] = (w >> ((c + k) & 31)) & 1u ? 1.0f : 0.0f;
+        return r;
+    } else {
+        return Unpack<T>::get(w);
+    }
+}
+template <int V>
+__device__ __forceinline__ Vec<V> load_f32(const float* p, bool live) {
+    Vec<V> r;
+#pragma unroll
+    for (int k = 0; k < V; ++k) r.v[k] = live ? p[k] : 0.0f;
+    return r;
+}
+template <int V>
+__device__ __forceinline__ void store_f32(float* p, const Vec<V>& x) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) p[k] = x.v[k];
+}
+
+// ---- tiles ---------------------------------------------------------------------
+// A CTA of W warps takes W * L consecutive steps of 32 * V channels at a time:
+// a warp L steps, a lane V channels (one 4-byte word of a row).  Over its L
+// steps a warp's map of the state is h -> A h + H (A the product of the
+// decays, H the end state from zero); the CTA joins its warps' maps in shared
+// memory, so each warp learns the state it starts from and runs its steps once
+// more with it, from registers.  With few channels a cluster of CTAs takes
+// consecutive tiles and joins their maps through distributed shared memory;
+// the state after the cluster's tiles is carried in registers to its next round.
+template <int W_, int L_, int S_, int CTAS_>
+struct Shape {
+    static constexpr int W = W_, L = L_, TT = W_ * L_, threads = 32 * W_;
+    static constexpr int S = S_;        // stages of rows in flight per warp
+    static constexpr int CTAS = CTAS_;  // CTAs an SM is to hold
+};
+using Fwd = Shape<8, 16, 2, 2>;
+using Bwd = Shape<8, 8, 3, 2>;
+using BwdMany = Shape<4, 8, 3, 4>;  // where channels and sequences alone fill the SMs
+constexpr int MAX_CLUSTER = 8;
+static_assert(Bwd::TT % BLOCK == 0 && BwdMany::TT % BLOCK == 0 && BLOCK % Fwd::L == 0,
+              "a gradient tile begins with a saved state, a block with a warp's steps");
+template <typename T>
+constexpr int lane_channels = 4 / (int)sizeof(T);
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// store to the same shared-memory variable of CTA `rank` of the cluster
+template <int V>
+__device__ __forceinline__ void store_peer(Vec<V>* p, int rank, const Vec<V>& x) {
+    const unsigned a = (unsigned)__cvta_generic_to_shared(p);
+    unsigned r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(r + 4 * k), "f"(x.v[k]) : "memory");
+}
+
+template <int V>
+struct ClusterMaps {  // the tiles' maps of a round, by rank; two rounds
+    Vec<V> a[2][MAX_CLUSTER][32], h[2][MAX_CLUSTER][32];
+};
+
+// Rows are staged in shared memory by asynchronous copies, each warp its own
+// rows, so that they need no barrier and no registers while in flight.  COPY is
+// the words that all rows allow: 16 bytes, 4 bytes, or (16-bit types, odd row
+// strides or offsets) the aligned 4-byte words that cover a row, 33 for 32.
+// Of a word at a row's end that reaches past the tile only the lower half is
+// read; one at a row's begin may hold the element before, which lies in the
+// same allocation (allocations begin aligned).
+template <int COPY>
+constexpr int row_bytes = COPY == 2 ? 132 : 128;
+
+template <int WORD>
+__device__ __forceinline__ void copy_async(unsigned dst, const void* src, int bytes) {
+    if constexpr (WORD == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// A stream of rows: where the warp's next rows begin and how they are staged
+template <typename T, int COPY, int L>
+struct Rower {
+    const char* p;       // element 0 of the tile in the warp's next first row
+    long long st, jump;  // bytes between rows, between a warp's first rows
+    __device__ __forceinline__ void start(const T* first, long long stride, long long steps) {
+        p = reinterpret_cast<const char*>(first);
+        st = stride * (int)sizeof(T);
+        jump = st * steps;
+    }
+    // rows 0 .. n (<= L) of nc channels to dst; zeros for the rest
+    __device__ __forceinline__ void fetch(unsigned dst, int n, int nc, int lane) const {
+        constexpr int E = (int)sizeof(T), FULL = 128 / E;
+        if constexpr (COPY == 16) {
+            const int ch = lane & 7, r0 = lane >> 3;
+            const int most = ch * 16 < nc * E ? n : 0;
+            const char* q = p + r0 * st + ch * 16;
+            dst += r0 * 128 + ch * 16;
+#pragma unroll
+            for (int i = 0; i < L; i += 4) {
+                copy_async<16>(dst + i * 128, r0 + i < most ? q : p, r0 + i < most ? 16 : 0);
+                q += 4 * st;
+            }
+        } else if constexpr (COPY == 4) {
+            const int most = lane * 4 < nc * E ? n : 0;
+            const char* q = p + lane * 4;
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                copy_async<4>(dst + i * 128 + lane * 4, i < most ? q : p, i < most ? 4 : 0);
+                q += st;
+            }
+        } else {
+            const char* q = p + lane * 4;
+            if (n == L && nc == FULL) {
+#pragma unroll
+                for (int i = 0; i < L; ++i) {
+                    copy_async<4>(dst + i * 132 + lane * 4, (const void*)((uintptr_t)q & ~(uintptr_t)3), 4);
+                    q += st;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < L; ++i) {
+                    const int e = 2 * lane - (int)(((uintptr_t)q >> 1) & 1);  // the word's lower element
+                    const int b = i >= n ? 0 : e + 1 < nc ? 4 : e >= 0 && e < nc ? 2 : 0;
+                    copy_async<4>(dst + i * 132 + lane * 4, (const void*)((uintptr_t)(b ? q : p) & ~(uintptr_t)3), b);
+                    q += st;
+                }
+            }
+            if (lane < L) {  // the 33rd words of all rows
+                q = p + lane * st + 128;
+                const int b = lane < n && nc == FULL && (((uintptr_t)q >> 1) & 1) ? 2 : 0;
+                copy_async<4>(dst + lane * 132 + 128, (const void*)((uintptr_t)(b ? q : p) & ~(uintptr_t)3), b);
+            }
+        }
+    }
+    // for rows at q: by how many bits row i begins in its first word, by i's parity
+    __device__ __forceinline__ unsigned shift(const char* q, int i) const {
+        return COPY == 2 ? (unsigned)(((uintptr_t)q + (i & 1 ? st : 0)) & 2) * 8 : 0u;
+    }
+};
+// the lane's word of a staged row
+template <int COPY>
+__device__ __forceinline__ unsigned staged(const char* rows, int i, int lane, unsigned shift) {
+    const unsigned* r = reinterpret_cast<const unsigned*>(rows + i * row_bytes<COPY>) + lane;
+    if constexpr (COPY == 2) return __funnelshift_r(r[0], r[1], shift);
+    return r[0];
+}
+// the lane's channels of a written row
+template <typename T, int COPY>
+__device__ __forceinline__ void write_row(T* p, const Vec<lane_channels<T>>& x, int nl) {
+    const auto w = Unpack<T>::put(x);
+    if constexpr (COPY == 2 && sizeof(T) == 2) {
+        reinterpret_cast<unsigned short*>(p)[0] = (unsigned short)w;
+        if (nl > 1) reinterpret_cast<unsigned short*>(p)[1] = (unsigned short)(w >> 16);
+    } else {
+        *reinterpret_cast<unsigned*>(p) = w;
+    }
+}
+template <int V>
+__device__ __forceinline__ Vec<V> load_n(const float* p, int nl) {
+    Vec<V> r;
+#pragma unroll
+    for (int k = 0; k < V; ++k) r.v[k] = k < nl ? p[k] : 0.0f;
+    return r;
+}
+template <int V>
+__device__ __forceinline__ void store_n(float* p, const Vec<V>& x, int nl) {
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+        if (k < nl) p[k] = x.v[k];
+}
+
+// A raster's words of L rows of a tile: lane (row, word) holds one (V words a row)
+template <int V, int L>
+__device__ __forceinline__ unsigned raster_word(const unsigned* p, long long st, int n, int words, int lane) {
+    const int r = lane / V, k = lane % V;
+    return r < L && r < n && k < words ? p[r * st + k] : 0u;
+}
+template <int V>
+__device__ __forceinline__ Vec<V> raster_values(unsigned held, int i, int lane) {
+    const unsigned w = __shfl_sync(~0u, held, i * V + lane * V / 32);
+    Vec<V> r;
+#pragma unroll
+    for (int k = 0; k < V; ++k) r.v[k] = (w >> ((lane * V + k) & 31)) & 1u ? 1.0f : 0.0f;
+    return r;
+}
+
+// a warp's stage of rows: gate, x, dy, where they are staged
+template <int GM, bool RASTER, int COPY, int L, bool GRAD>
+struct Stage {
+    static constexpr int rows = L * row_bytes<COPY>;
+    static constexpr int gate = 0, x = per_channel<GM> ? 0 : rows;
+    static constexpr int dy = x + (RASTER ? 0 : rows), bytes = dy + (GRAD ? rows : 0);
+};
+
+template <typename SH, typename T, int GM, bool RASTER, bool LEAKY, int COPY>
+__global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanArgs A) {
+    constexpr int W = SH::W, L = SH::L, TT = SH::TT, S = SH::S, V = lane_channels<T>;
+    constexpr bool LO = keeps_lo<T, GM>, PC = per_channel<GM>;
+    using St = Stage<GM, RASTER, COPY, L, false>;
+    static_assert(L * V <= 32, "a lane holds one raster word");
+    extern __shared__ __align__(16) char rows[];
+    __shared__ Vec<V> sa[2][W][32], sh[2][W][32];
+    __shared__ ClusterMaps<V> cm;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int CL = A.cluster, rank = blockIdx.x % CL, item = blockIdx.x / CL;
+    const int c0 = item % A.ctiles * 32 * V, c = c0 + lane * V;
+    const int nc = min(32 * V, A.D - c0), nl = min(V, A.D - c);  // channels of the tile, of the lane (<= 0: none)
+    const int round = CL * TT;
+    char* const mine = rows + w * S * St::bytes;
+    const unsigned mine_s = (unsigned)__cvta_generic_to_shared(mine);
+    Decay<V, LO> fixed;
+    Vec<V> factor = splat<V>(1.0f);
+    if (PC) channel_decays<T, GM, V>(A, c, nl, fixed, factor);
+    int par = 0;
+    for (long long s = item / A.ctiles; s < A.n_seq; s += A.workers) {
+        const Span sp = span_of(A, s);
+        Vec<V> carry = load_n<V>(A.h0 + s * A.D + c, A.h0 ? nl : 0);
+        if (sp.len == 0) {
+            if (A.h && rank == 0 && w == 0) store_n<V>(A.h + s * A.D + c, carry, nl);
+            continue;
+        }
+        const int t1 = rank * TT + w * L;  // the warp's first step
+        Rower<T, COPY, L> rg, rx;
+        rg.start(reinterpret_cast<const T*>(A.gate.p) + row_at(A, A.gate, s, sp, t1) + c0, A.gate.st, round);
+        rx.start(reinterpret_cast<const T*>(A.x.p) + row_at(A, A.x, s, sp, t1) + c0, A.x.st, round);
+        const unsigned* pw = reinterpret_cast<const unsigned*>(A.x.p) + row_at(A, A.x, s, sp, t1) + (c0 >> 5);
+        T* py = reinterpret_cast<T*>(A.y.p) + row_at(A, A.y, s, sp, t1) + c;
+        const long long yjump = A.y.st * round;
+        const unsigned g0 = rg.shift(rg.p, 0), g1 = rg.shift(rg.p, 1), x0 = rx.shift(rx.p, 0), x1 = rx.shift(rx.p, 1);
+        unsigned words = 0;
+        auto fetch = [&](int t, int slot) {  // this warp's steps from t on
+            const int n = min(L, sp.len - t);
+            const unsigned dst = mine_s + slot * St::bytes;
+            if (n > 0) {
+                if (!PC) rg.fetch(dst + St::gate, n, nc, lane);
+                if (!RASTER) rx.fetch(dst + St::x, n, nc, lane);
+            }
+            rg.p += rg.jump;
+            rx.p += rx.jump;
+            copy_commit();
+        };
+        auto fetch_words = [&](int t) {
+            if (RASTER) {
+                words = t < sp.len ? raster_word<V, L>(pw, A.x.st, min(L, sp.len - t), (nc + 31) >> 5, lane) : 0u;
+                pw += A.x.st * round;
+            }
+        };
+#pragma unroll
+        for (int k = 0; k < S; ++k) fetch(t1 + k * round, k);
+        fetch_words(t1);
+        int slot = 0;
+        for (int t0 = t1; t0 - t1 < sp.len; t0 += round) {
+            Decay<V, LO> d[PC ? 1 : L];
+            Vec<V> u[L];
+            copy_wait<S - 1>();
+            __syncwarp();
+            const char* from = mine + slot * St::bytes;
+            const unsigned held = words;
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                Vec<V> f = factor;
+                if (!PC)
+                    decays<T, GM, V>(Unpack<T>::get(staged<COPY>(from + St::gate, i, lane, i & 1 ? g1 : g0)), d[i], f);
+                if constexpr (RASTER) u[i] = raster_values<V>(held, i, lane);
+                else u[i] = Unpack<T>::get(staged<COPY>(from + St::x, i, lane, i & 1 ? x1 : x0));
+                if (LEAKY) u[i] = vmul(f, u[i]);
+            }
+            if (PC) d[0] = fixed;
+            __syncwarp();
+            fetch(t0 + S * round, slot);
+            fetch_words(t0 + round);
+            slot = slot + 1 == S ? 0 : slot + 1;
+            Vec<V> a = splat<V>(1.0f), h = splat<V>(0.0f);
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                const Decay<V, LO>& q = d[PC ? 0 : i];
+                h = q.step(h, u[i]);
+                a = q.times(a);
+            }
+            sa[par][w][lane] = a;
+            sh[par][w][lane] = h;
+            __syncthreads();
+            // the maps of the warps before this one (a, h) and of the whole tile (ta, th)
+            Vec<V> ta = splat<V>(1.0f), th = CL > 1 ? splat<V>(0.0f) : carry;
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                if (j == w) {
+                    a = ta;
+                    h = th;
+                }
+                const Vec<V> ja = sa[par][j][lane];
+                th = vfma(ja, th, sh[par][j][lane]);
+                ta = vmul(ja, ta);
+            }
+            if (CL > 1) {
+                for (int r = w; r < CL; r += W) {
+                    store_peer<V>(&cm.a[par][rank][lane], r, ta);
+                    store_peer<V>(&cm.h[par][rank][lane], r, th);
+                }
+                cluster_sync();
+                Vec<V> in = carry;
+                for (int r = 0; r < CL; ++r) {
+                    if (r == rank) in = carry;
+                    carry = vfma(cm.a[par][r][lane], carry, cm.h[par][r][lane]);
+                }
+                h = vfma(a, in, h);
+            } else {
+                carry = th;
+            }
+            par ^= 1;
+            const int n = min(L, sp.len - t0);
+            if (nl > 0 && n > 0) {
+                if (A.saved && t0 % BLOCK == 0) store_n<V>(A.saved + (sp.block0 + t0 / BLOCK) * A.D + c, h, nl);
+                T* qy = py;
+#pragma unroll
+                for (int i = 0; i < L; ++i) {
+                    if (i < n) {
+                        h = d[PC ? 0 : i].step(h, u[i]);
+                        write_row<T, COPY>(qy, h, nl);
+                    }
+                    qy += A.y.st;
+                }
+                if (A.h && t0 + n == sp.len) store_n<V>(A.h + s * A.D + c, h, nl);
+            }
+            py += yjump;
+        }
+        copy_wait<0>();
+        __syncwarp();
+    }
+}
+
+// The gradient runs from the last tile to the first.  With r the gradient that
+// reaches a step from later ones, g = o + r and r' = a g: the map of a tile is
+// r -> A r + R.  The states inside the tile come from its saved first state.
+template <typename SH, typename T, int GM, bool RASTER, bool LEAKY, int COPY>
+__global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const ScanArgs A) {
+    constexpr int W = SH::W, L = SH::L, TT = SH::TT, S = SH::S, V = lane_channels<T>;
+    constexpr bool LO = keeps_lo<T, GM>, PC = per_channel<GM>;
+    using St = Stage<GM, RASTER, COPY, L, true>;
+    extern __shared__ __align__(16) char rows[];
+    __shared__ Vec<V> sa[2][W][32], sh[2][W][32], sr[2][W][32];
+    __shared__ ClusterMaps<V> cm;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int CL = A.cluster, rank = blockIdx.x % CL, item = blockIdx.x / CL;
+    const int c0 = item % A.ctiles * 32 * V, c = c0 + lane * V;
+    const int nc = min(32 * V, A.D - c0), nl = min(V, A.D - c);
+    const int round = CL * TT;
+    char* const mine = rows + w * S * St::bytes;
+    const unsigned mine_s = (unsigned)__cvta_generic_to_shared(mine);
+    const Vec<V> one = splat<V>(1.0f), minus = splat<V>(-1.0f);
+    Decay<V, LO> fixed;
+    Vec<V> factor = one, sum = splat<V>(0.0f);
+    if (PC) channel_decays<T, GM, V>(A, c, nl, fixed, factor);
+    int par = 0;
+    for (long long s = item / A.ctiles; s < A.n_seq; s += A.workers) {
+        const Span sp = span_of(A, s);
+        Vec<V> carry = splat<V>(0.0f);
+        if (sp.len == 0) {
+            if (A.dh0 && rank == 0 && w == 0)
+                store_n<V>(A.dh0 + s * A.D + c, load_n<V>(A.dh + s * A.D + c, A.dh ? nl : 0), nl);
+            continue;
+        }
+        const int tiles = (sp.len + TT - 1) / TT;
+        const int t1 = (tiles - 1 - rank) * TT + w * L;  // the warp's first (latest) steps; may be negative
+        Rower<T, COPY, L> rg, rx, rd;
+        rg.start(reinterpret_cast<const T*>(A.gate.p) + row_at(A, A.gate, s, sp, t1) + c0, A.gate.st, -round);
+        rx.start(reinterpret_cast<const T*>(A.x.p) + row_at(A, A.x, s, sp, t1) + c0, A.x.st, -round);
+        rd.start(reinterpret_cast<const T*>(A.y.p) + row_at(A, A.y, s, sp, t1) + c0, A.y.st, -round);
+        const unsigned* pw = reinterpret_cast<const unsigned*>(A.x.p) + row_at(A, A.x, s, sp, t1) + (c0 >> 5);
+        T* pdg = reinterpret_cast<T*>(A.dgate.p) + (PC ? 0 : row_at(A, A.dgate, s, sp, t1 + L - 1) + c);
+        T* pdx = reinterpret_cast<T*>(A.dx.p) + row_at(A, A.dx, s, sp, t1 + L - 1) + c;
+        const long long gjump = A.dgate.st * round, xjump = A.dx.st * round;
+        const unsigned g0 = rg.shift(rg.p, 0), g1 = rg.shift(rg.p, 1), x0 = rx.shift(rx.p, 0), x1 = rx.shift(rx.p, 1);
+        const unsigned d0 = rd.shift(rd.p, 0), d1 = rd.shift(rd.p, 1);
+        Vec<V> first = splat<V>(0.0f);
+        unsigned words = 0;
+        auto fetch = [&](int t, int slot) {
+            if (t >= 0 && t < sp.len) {
+                const int n = min(L, sp.len - t);
+                const unsigned dst = mine_s + slot * St::bytes;
+                if (!PC) rg.fetch(dst + St::gate, n, nc, lane);
+                if (!RASTER) rx.fetch(dst + St::x, n, nc, lane);
+                if (A.y.p) rd.fetch(dst + St::dy, n, nc, lane);
+            }
+            rg.p += rg.jump;
+            rx.p += rx.jump;
+            rd.p += rd.jump;
+            copy_commit();
+        };
+        auto fetch_words = [&](int t) {
+            if (t >= 0) first = load_n<V>(A.saved + (sp.block0 + (t - w * L) / BLOCK) * A.D + c, nl);
+            if (RASTER) {
+                words = t >= 0 && t < sp.len ? raster_word<V, L>(pw, A.x.st, min(L, sp.len - t), (nc + 31) >> 5, lane) : 0u;
+                pw -= A.x.st * round;
+            }
+        };
+#pragma unroll
+        for (int k = 0; k < S; ++k) fetch(t1 - k * round, k);
+        fetch_words(t1);
+        int slot = 0, t0 = t1;
+        for (int b = 0; b < tiles; b += CL, t0 -= round) {  // t0 negative: no tile left for this CTA
+            const bool some = t0 >= 0 && t0 < sp.len;
+            Decay<V, LO> d[PC ? 1 : L];
+            Vec<V> rest[PC ? 1 : L], x[L], o[L];
+            copy_wait<S - 1>();
+            __syncwarp();
+            const char* from = mine + slot * St::bytes;
+            const unsigned held = words;
+            const Vec<V> h0 = first;
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                if (!PC)
+                    decays<T, GM, V>(Unpack<T>::get(staged<COPY>(from + St::gate, i, lane, i & 1 ? g1 : g0)), d[i], rest[i]);
+                if constexpr (RASTER) x[i] = raster_values<V>(held, i, lane);
+                else x[i] = Unpack<T>::get(staged<COPY>(from + St::x, i, lane, i & 1 ? x1 : x0));
+                o[i] = splat<V>(0.0f);
+                if (A.y.p) o[i] = Unpack<T>::get(staged<COPY>(from + St::dy, i, lane, i & 1 ? d1 : d0));
+            }
+            if (A.dh && some && t0 + L >= sp.len) {  // the last step
+                const Vec<V> dh = load_n<V>(A.dh + s * A.D + c, nl);
+#pragma unroll
+                for (int i = 0; i < L; ++i)
+                    if (t0 + i == sp.len - 1) o[i] = vadd(o[i], dh);
+            }
+            if (PC) d[0] = fixed;
+            __syncwarp();
+            fetch(t0 - S * round, slot);
+            fetch_words(t0 - round);
+            slot = slot + 1 == S ? 0 : slot + 1;
+            Vec<V> a = one, h = splat<V>(0.0f), r = h;
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                const Decay<V, LO>& q = d[PC ? 0 : i];
+                h = q.step(h, LEAKY ? vmul(PC ? factor : rest[PC ? 0 : i], x[i]) : x[i]);
+                a = q.times(a);
+                r = d[PC ? 0 : L - 1 - i].times(vadd(o[L - 1 - i], r));
+            }
+            if (!some) {  // steps behind the end, whose rows were not read: r passes unchanged
+                a = one;
+                r = splat<V>(0.0f);
+            }
+            sa[par][w][lane] = a;
+            sh[par][w][lane] = h;
+            sr[par][w][lane] = r;
+            __syncthreads();
+            Vec<V> hw = h0;
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                if (j == w) h = hw;
+                if (j < W - 1) hw = vfma(sa[par][j][lane], hw, sh[par][j][lane]);
+            }
+            // the maps of the warps behind this one (a, r) and of the whole tile (ta, tr)
+            Vec<V> ta = one, tr = CL > 1 ? splat<V>(0.0f) : carry;
+#pragma unroll
+            for (int j = W - 1; j >= 0; --j) {
+                if (j == w) {
+                    a = ta;
+                    r = tr;
+                }
+                const Vec<V> ja = sa[par][j][lane];
+                tr = vfma(ja, tr, sr[par][j][lane]);
+                ta = vmul(ja, ta);
+            }
+            if (CL > 1) {
+                for (int q = w; q < CL; q += W) {
+                    store_peer<V>(&cm.a[par][rank][lane], q, ta);
+                    store_peer<V>(&cm.h[par][rank][lane], q, tr);
+                }
+                cluster_sync();
+                Vec<V> in = carry;
+                for (int q = 0; q < CL; ++q) {
+                    if (q == rank) in = carry;
+                    carry = vfma(cm.a[par][q][lane], carry, cm.h[par][q][lane]);
+                }
+                r = vfma(a, in, r);
+            } else {
+                carry = tr;
+            }
+            par ^= 1;
+            if (nl > 0 && some) {
+                // x becomes the derivative of h_t in a_t: h_{t-1}, or h_{t-1} - x_t
+#pragma unroll
+                for (int i = 0; i < L; ++i) {
+                    const Vec<V> before = h, xi = x[i];
+                    h = d[PC ? 0 : i].step(h, LEAKY ? vmul(PC ? factor : rest[PC ? 0 : i], xi) : xi);
+                    x[i] = LEAKY ? vfma(minus, xi, before) : before;
+                }
+                const int n = min(L, sp.len - t0);
+                T *qg = pdg, *qx = pdx;
+#pragma unroll
+                for (int i = L - 1; i >= 0; --i) {
+                    if (i < n) {
+                        const Decay<V, LO>& q = d[PC ? 0 : i];
+                        const Vec<V> g = vadd(o[i], r);
+                        if (PC) {
+                            sum = vfma(g, x[i], sum);
+                        } else if (A.dgate.p) {
+                            Vec<V> da = vmul(g, x[i]);
+                            if (GM == GATE_LOGIT) da = vmul(da, vmul(q.a, rest[PC ? 0 : i]));
+                            write_row<T, COPY>(qg, da, nl);
+                        }
+                        if (A.dx.p) write_row<T, COPY>(qx, LEAKY ? vmul(PC ? factor : rest[PC ? 0 : i], g) : g, nl);
+                        r = q.times(g);
+                    }
+                    qg -= A.dgate.st;
+                    qx -= A.dx.st;
+                }
+                if (t0 == 0 && A.dh0) store_n<V>(A.dh0 + s * A.D + c, r, nl);
+            }
+            pdg -= gjump;
+            pdx -= xjump;
+        }
+        copy_wait<0>();
+        __syncwarp();
+    }
+    if (PC && A.part) {
+        __syncthreads();
+        sa[0][w][lane] = sum;
+        __syncthreads();
+        if (w == 0 && nl > 0) {
+            Vec<V> t = splat<V>(0.0f);
+            for (int j = 0; j < W; ++j) t = vadd(t, sa[0][j][lane]);
+            store_n<V>(A.part + ((long long)(item / A.ctiles) * CL + rank) * A.D + c, t, nl);
+        }
+    }
+}
+
+struct Plan {
+    int ctiles, workers, cluster;
+    bool many;
+};
+
+// the forward (GRAD = false) or gradient kernel of element type T
+template <bool GRAD, typename T>
+void launch_tiles(int gate_mode, bool raster, int words, const Plan& p, ScanArgs& A, cudaStream_t st);
+
+#ifdef SNN_SCAN_TILE_LAUNCH
+inline void launch(const void* kernel, int threads, int smem, const Plan& p, ScanArgs& A, cudaStream_t st) {
+    A.ctiles = p.ctiles;
+    A.workers = p.workers;
+    A.cluster = p.cluster;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    SNN_REQUIRE((int64_t)p.ctiles * p.workers * p.cluster < (1ll << 31), SNN_ERR_ARG, "scan: too many tiles");
+    cfg.gridDim = dim3((unsigned)(p.ctiles * p.workers * p.cluster));
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = (unsigned)p.cluster;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = p.cluster > 1 ? 1 : 0;
+    SNN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    void* args[] = {&A};
+    SNN_CUDA(cudaLaunchKernelExC(&cfg, kernel, args));
+}
+
+template <bool GRAD, typename SH, typename T, int GM, bool RASTER, int COPY>
+void launch_shape(const Plan& p, ScanArgs& A, cudaStream_t st) {
+    const int smem = SH::W * SH::S * Stage<GM, RASTER, COPY, SH::L, GRAD>::bytes;
+    const void* k;
+    if constexpr (GRAD)
+        k = A.leaky ? (const void*)k_scan_grad_tile<SH, T, GM, RASTER, true, COPY>
+                    : (const void*)k_scan_grad_tile<SH, T, GM, RASTER, false, COPY>;
+    else
+        k = A.leaky ? (const void*)k_scan_tile<SH, T, GM, RASTER, true, COPY>
+                    : (const void*)k_scan_tile<SH, T, GM, RASTER, false, COPY>;
+    launch(k, SH::threads, smem, p, A, st);
+}
+template <bool GRAD, typename T, int GM, bool RASTER, int COPY>
+void launch_copy(const Plan& p, ScanArgs& A, cudaStream_t st) {
+    if constexpr (!GRAD) launch_shape<false, Fwd, T, GM, RASTER, COPY>(p, A, st);
+    else if constexpr (RASTER) launch_shape<true, Bwd, T, GM, true, COPY>(p, A, st);
+    else if (p.many) launch_shape<true, BwdMany, T, GM, false, COPY>(p, A, st);
+    else launch_shape<true, Bwd, T, GM, false, COPY>(p, A, st);
+}
+template <bool GRAD, typename T, int GM>
+void launch_gate(bool raster, int words, const Plan& p, ScanArgs& A, cudaStream_t st) {
+    if constexpr (sizeof(T) == 2)
+        if (words == 2)
+            return raster ? launch_copy<GRAD, T, GM, true, 2>(p, A, st) : launch_copy<GRAD, T, GM, false, 2>(p, A, st);
+    if (raster) launch_copy<GRAD, T, GM, true, 4>(p, A, st);
+    else if (words == 16) launch_copy<GRAD, T, GM, false, 16>(p, A, st);
+    else launch_copy<GRAD, T, GM, false, 4>(p, A, st);
+}
+template <bool GRAD, typename T>
+void launch_tiles(int gate_mode, bool raster, int words, const Plan& p, ScanArgs& A, cudaStream_t st) {
+    if (gate_mode == GATE_VALUE) launch_gate<GRAD, T, GATE_VALUE>(raster, words, p, A, st);
+    else if (gate_mode == GATE_LOGIT) launch_gate<GRAD, T, GATE_LOGIT>(raster, words, p, A, st);
+    else if (gate_mode == GATE_CHANNEL) launch_gate<GRAD, T, GATE_CHANNEL>(raster, words, p, A, st);
+    else launch_gate<GRAD, T, GATE_CHANNEL_LOGIT>(raster, words, p, A, st);
+}
+#endif
+
+}  // namespace snnb_scan
