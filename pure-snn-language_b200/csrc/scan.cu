@@ -135,10 +135,11 @@ Plan plan_of(const snn_scan* d, int tile) {
     p.cluster = 1;
     while (p.cluster < MAX_CLUSTER && items * p.cluster < wanted && (int64_t)tile * p.cluster < mean_steps(d))
         p.cluster *= 2;
-    // the gradient by smaller CTAs, twice as many on an SM: 16 x 4,096 x 2,048 in
-    // bf16 332 -> 305 us; with clusters they lose (one sequence of 50,021 steps by
-    // 1,000 channels in f32: 301 -> 447 us)
-    p.many = p.cluster == 1 && items >= 3 * SMS;
+    // Without clusters: 16 x 4,096 x 2,048 in bf16 (512 items) gradient 332 us by
+    // tiles, 299 by the smaller ones, 375 by single warps (forward 158 / - / 178);
+    // a raster of 1,000 x 55,000 (1,719 items) forward 69 / - / 49, gradient 134 /
+    // - / 79.
+    p.shape = p.cluster > 1 || items < 3 * SMS ? 0 : items < 8 * SMS ? 1 : 2;
     return p;
 }
 

@@ -11,9 +11,9 @@ using snnb::to_f32;
 
 // Steps between two states that the forward pass keeps for the backward pass.
 // The backward pass recomputes the states inside a block from the inputs that
-// it reads anyway: 4 bytes per 32 steps and channel instead of a second read
+// it reads anyway: 4 bytes per 16 steps and channel instead of a second read
 // of y, and the states stay f32.
-constexpr int BLOCK = 32;
+constexpr int BLOCK = 16;
 
 // how the decays are given: per step, as they are or as logits; per channel
 enum { GATE_VALUE = 0, GATE_LOGIT = 1, GATE_CHANNEL = 2, GATE_CHANNEL_LOGIT = 3 };
@@ -301,10 +301,15 @@ struct Shape {
 };
 using Fwd = Shape<8, 16, 2, 2>;
 using Bwd = Shape<8, 8, 3, 2>;
-using BwdMany = Shape<4, 8, 3, 4>;  // where channels and sequences alone fill the SMs
+// Without clusters the gradient takes smaller CTAs, twice as many on an SM.
+using BwdMany = Shape<4, 8, 3, 4>;
+// Where channels and sequences alone fill the SMs with warps: a warp by itself,
+// which has its state at hand and needs no maps.
+using FwdSeq = Shape<1, 16, 4, 12>;
+using BwdSeq = Shape<1, 16, 3, 8>;
 constexpr int MAX_CLUSTER = 8;
-static_assert(Bwd::TT % BLOCK == 0 && BwdMany::TT % BLOCK == 0 && BLOCK % Fwd::L == 0,
-              "a gradient tile begins with a saved state, a block with a warp's steps");
+static_assert(Bwd::TT % BLOCK == 0 && BwdMany::TT % BLOCK == 0 && BwdSeq::TT % BLOCK == 0 && FwdSeq::L % BLOCK == 0 && Fwd::L % BLOCK == 0,
+              "a gradient tile and a warp's forward steps begin with a saved state");
 template <typename T>
 constexpr int lane_channels = 4 / (int)sizeof(T);
 
@@ -442,34 +447,37 @@ __device__ __forceinline__ void store_n(float* p, const Vec<V>& x, int nl) {
         if (k < nl) p[k] = x.v[k];
 }
 
-// A raster's words of L rows of a tile: lane (row, word) holds one (V words a row)
+// rows 0 .. n (<= L) of a tile's raster words (V a row) to dst, a word a lane
 template <int V, int L>
-__device__ __forceinline__ unsigned raster_word(const unsigned* p, long long st, int n, int words, int lane) {
+__device__ __forceinline__ void fetch_raster(unsigned dst, const unsigned* p, long long st, int n, int words, int lane) {
     const int r = lane / V, k = lane % V;
-    return r < L && r < n && k < words ? p[r * st + k] : 0u;
+    const bool in = r < L && r < n && k < words;
+    copy_async<4>(dst + lane * 4, in ? p + r * st + k : p, in ? 4 : 0);
 }
 template <int V>
-__device__ __forceinline__ Vec<V> raster_values(unsigned held, int i, int lane) {
-    const unsigned w = __shfl_sync(~0u, held, i * V + lane * V / 32);
+__device__ __forceinline__ Vec<V> raster_values(const char* words, int i, int lane) {
+    const unsigned w = reinterpret_cast<const unsigned*>(words)[i * V + lane * V / 32];
     Vec<V> r;
 #pragma unroll
     for (int k = 0; k < V; ++k) r.v[k] = (w >> ((lane * V + k) & 31)) & 1u ? 1.0f : 0.0f;
     return r;
 }
 
-// a warp's stage of rows: gate, x, dy, where they are staged
-template <int GM, bool RASTER, int COPY, int L, bool GRAD>
+// a warp's stage of rows: gate, x (or raster words), dy and the block's first
+// state, where they are staged
+template <int GM, bool RASTER, int COPY, int L, int V, bool GRAD>
 struct Stage {
     static constexpr int rows = L * row_bytes<COPY>;
     static constexpr int gate = 0, x = per_channel<GM> ? 0 : rows;
-    static constexpr int dy = x + (RASTER ? 0 : rows), bytes = dy + (GRAD ? rows : 0);
+    static constexpr int dy = x + (RASTER ? 128 : rows), state = dy + (GRAD ? rows : 0);
+    static constexpr int bytes = state + (GRAD ? 128 * V : 0);
 };
 
 template <typename SH, typename T, int GM, bool RASTER, bool LEAKY, int COPY>
 __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanArgs A) {
     constexpr int W = SH::W, L = SH::L, TT = SH::TT, S = SH::S, V = lane_channels<T>;
     constexpr bool LO = keeps_lo<T, GM>, PC = per_channel<GM>;
-    using St = Stage<GM, RASTER, COPY, L, false>;
+    using St = Stage<GM, RASTER, COPY, L, V, false>;
     static_assert(L * V <= 32, "a lane holds one raster word");
     extern __shared__ __align__(16) char rows[];
     __shared__ Vec<V> sa[2][W][32], sh[2][W][32];
@@ -500,27 +508,21 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
         T* py = reinterpret_cast<T*>(A.y.p) + row_at(A, A.y, s, sp, t1) + c;
         const long long yjump = A.y.st * round;
         const unsigned g0 = rg.shift(rg.p, 0), g1 = rg.shift(rg.p, 1), x0 = rx.shift(rx.p, 0), x1 = rx.shift(rx.p, 1);
-        unsigned words = 0;
         auto fetch = [&](int t, int slot) {  // this warp's steps from t on
             const int n = min(L, sp.len - t);
             const unsigned dst = mine_s + slot * St::bytes;
             if (n > 0) {
                 if (!PC) rg.fetch(dst + St::gate, n, nc, lane);
-                if (!RASTER) rx.fetch(dst + St::x, n, nc, lane);
+                if (RASTER) fetch_raster<V, L>(dst + St::x, pw, A.x.st, n, (nc + 31) >> 5, lane);
+                else rx.fetch(dst + St::x, n, nc, lane);
             }
             rg.p += rg.jump;
             rx.p += rx.jump;
+            pw += A.x.st * round;
             copy_commit();
-        };
-        auto fetch_words = [&](int t) {
-            if (RASTER) {
-                words = t < sp.len ? raster_word<V, L>(pw, A.x.st, min(L, sp.len - t), (nc + 31) >> 5, lane) : 0u;
-                pw += A.x.st * round;
-            }
         };
 #pragma unroll
         for (int k = 0; k < S; ++k) fetch(t1 + k * round, k);
-        fetch_words(t1);
         int slot = 0;
         for (int t0 = t1; t0 - t1 < sp.len; t0 += round) {
             Decay<V, LO> d[PC ? 1 : L];
@@ -528,62 +530,64 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
             copy_wait<S - 1>();
             __syncwarp();
             const char* from = mine + slot * St::bytes;
-            const unsigned held = words;
 #pragma unroll
             for (int i = 0; i < L; ++i) {
                 Vec<V> f = factor;
                 if (!PC)
                     decays<T, GM, V>(Unpack<T>::get(staged<COPY>(from + St::gate, i, lane, i & 1 ? g1 : g0)), d[i], f);
-                if constexpr (RASTER) u[i] = raster_values<V>(held, i, lane);
+                if constexpr (RASTER) u[i] = raster_values<V>(from + St::x, i, lane);
                 else u[i] = Unpack<T>::get(staged<COPY>(from + St::x, i, lane, i & 1 ? x1 : x0));
                 if (LEAKY) u[i] = vmul(f, u[i]);
             }
             if (PC) d[0] = fixed;
             __syncwarp();
             fetch(t0 + S * round, slot);
-            fetch_words(t0 + round);
             slot = slot + 1 == S ? 0 : slot + 1;
-            Vec<V> a = splat<V>(1.0f), h = splat<V>(0.0f);
+            Vec<V> h = carry;
+            if constexpr (W > 1) {
+                Vec<V> a = splat<V>(1.0f);
+                h = splat<V>(0.0f);
 #pragma unroll
-            for (int i = 0; i < L; ++i) {
-                const Decay<V, LO>& q = d[PC ? 0 : i];
-                h = q.step(h, u[i]);
-                a = q.times(a);
-            }
-            sa[par][w][lane] = a;
-            sh[par][w][lane] = h;
-            __syncthreads();
-            // the maps of the warps before this one (a, h) and of the whole tile (ta, th)
-            Vec<V> ta = splat<V>(1.0f), th = CL > 1 ? splat<V>(0.0f) : carry;
+                for (int i = 0; i < L; ++i) {
+                    const Decay<V, LO>& q = d[PC ? 0 : i];
+                    h = q.step(h, u[i]);
+                    a = q.times(a);
+                }
+                sa[par][w][lane] = a;
+                sh[par][w][lane] = h;
+                __syncthreads();
+                // the maps of the warps before this one (a, h) and of the whole tile (ta, th)
+                Vec<V> ta = splat<V>(1.0f), th = CL > 1 ? splat<V>(0.0f) : carry;
 #pragma unroll
-            for (int j = 0; j < W; ++j) {
-                if (j == w) {
-                    a = ta;
-                    h = th;
+                for (int j = 0; j < W; ++j) {
+                    if (j == w) {
+                        a = ta;
+                        h = th;
+                    }
+                    const Vec<V> ja = sa[par][j][lane];
+                    th = vfma(ja, th, sh[par][j][lane]);
+                    ta = vmul(ja, ta);
                 }
-                const Vec<V> ja = sa[par][j][lane];
-                th = vfma(ja, th, sh[par][j][lane]);
-                ta = vmul(ja, ta);
+                if (CL > 1) {
+                    for (int r = w; r < CL; r += W) {
+                        store_peer<V>(&cm.a[par][rank][lane], r, ta);
+                        store_peer<V>(&cm.h[par][rank][lane], r, th);
+                    }
+                    cluster_sync();
+                    Vec<V> in = carry;
+                    for (int r = 0; r < CL; ++r) {
+                        if (r == rank) in = carry;
+                        carry = vfma(cm.a[par][r][lane], carry, cm.h[par][r][lane]);
+                    }
+                    h = vfma(a, in, h);
+                } else {
+                    carry = th;
+                }
+                par ^= 1;
             }
-            if (CL > 1) {
-                for (int r = w; r < CL; r += W) {
-                    store_peer<V>(&cm.a[par][rank][lane], r, ta);
-                    store_peer<V>(&cm.h[par][rank][lane], r, th);
-                }
-                cluster_sync();
-                Vec<V> in = carry;
-                for (int r = 0; r < CL; ++r) {
-                    if (r == rank) in = carry;
-                    carry = vfma(cm.a[par][r][lane], carry, cm.h[par][r][lane]);
-                }
-                h = vfma(a, in, h);
-            } else {
-                carry = th;
-            }
-            par ^= 1;
             const int n = min(L, sp.len - t0);
             if (nl > 0 && n > 0) {
-                if (A.saved && t0 % BLOCK == 0) store_n<V>(A.saved + (sp.block0 + t0 / BLOCK) * A.D + c, h, nl);
+                if (A.saved) store_n<V>(A.saved + (sp.block0 + t0 / BLOCK) * A.D + c, h, nl);
                 T* qy = py;
 #pragma unroll
                 for (int i = 0; i < L; ++i) {
@@ -594,6 +598,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
                     qy += A.y.st;
                 }
                 if (A.h && t0 + n == sp.len) store_n<V>(A.h + s * A.D + c, h, nl);
+                if (W == 1) carry = h;
             }
             py += yjump;
         }
@@ -609,7 +614,7 @@ template <typename SH, typename T, int GM, bool RASTER, bool LEAKY, int COPY>
 __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const ScanArgs A) {
     constexpr int W = SH::W, L = SH::L, TT = SH::TT, S = SH::S, V = lane_channels<T>;
     constexpr bool LO = keeps_lo<T, GM>, PC = per_channel<GM>;
-    using St = Stage<GM, RASTER, COPY, L, true>;
+    using St = Stage<GM, RASTER, COPY, L, V, true>;
     extern __shared__ __align__(16) char rows[];
     __shared__ Vec<V> sa[2][W][32], sh[2][W][32], sr[2][W][32];
     __shared__ ClusterMaps<V> cm;
@@ -645,31 +650,30 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
         const long long gjump = A.dgate.st * round, xjump = A.dx.st * round;
         const unsigned g0 = rg.shift(rg.p, 0), g1 = rg.shift(rg.p, 1), x0 = rx.shift(rx.p, 0), x1 = rx.shift(rx.p, 1);
         const unsigned d0 = rd.shift(rd.p, 0), d1 = rd.shift(rd.p, 1);
-        Vec<V> first = splat<V>(0.0f);
-        unsigned words = 0;
         auto fetch = [&](int t, int slot) {
             if (t >= 0 && t < sp.len) {
                 const int n = min(L, sp.len - t);
                 const unsigned dst = mine_s + slot * St::bytes;
                 if (!PC) rg.fetch(dst + St::gate, n, nc, lane);
-                if (!RASTER) rx.fetch(dst + St::x, n, nc, lane);
+                if (RASTER) fetch_raster<V, L>(dst + St::x, pw, A.x.st, n, (nc + 31) >> 5, lane);
+                else rx.fetch(dst + St::x, n, nc, lane);
                 if (A.y.p) rd.fetch(dst + St::dy, n, nc, lane);
+            }
+            if (t >= 0) {  // the tile's first state, where t lies behind the end too
+                const float* q = A.saved + (sp.block0 + (t - w * L) / BLOCK) * A.D + c;
+#pragma unroll
+                for (int k = 0; k < V; ++k)
+                    copy_async<4>(mine_s + slot * St::bytes + St::state + (lane * V + k) * 4, k < nl ? q + k : A.saved,
+                                  k < nl ? 4 : 0);
             }
             rg.p += rg.jump;
             rx.p += rx.jump;
             rd.p += rd.jump;
+            pw -= A.x.st * round;
             copy_commit();
-        };
-        auto fetch_words = [&](int t) {
-            if (t >= 0) first = load_n<V>(A.saved + (sp.block0 + (t - w * L) / BLOCK) * A.D + c, nl);
-            if (RASTER) {
-                words = t >= 0 && t < sp.len ? raster_word<V, L>(pw, A.x.st, min(L, sp.len - t), (nc + 31) >> 5, lane) : 0u;
-                pw -= A.x.st * round;
-            }
         };
 #pragma unroll
         for (int k = 0; k < S; ++k) fetch(t1 - k * round, k);
-        fetch_words(t1);
         int slot = 0, t0 = t1;
         for (int b = 0; b < tiles; b += CL, t0 -= round) {  // t0 negative: no tile left for this CTA
             const bool some = t0 >= 0 && t0 < sp.len;
@@ -678,13 +682,12 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
             copy_wait<S - 1>();
             __syncwarp();
             const char* from = mine + slot * St::bytes;
-            const unsigned held = words;
-            const Vec<V> h0 = first;
+            const Vec<V> h0 = reinterpret_cast<const Vec<V>*>(from + St::state)[lane];
 #pragma unroll
             for (int i = 0; i < L; ++i) {
                 if (!PC)
                     decays<T, GM, V>(Unpack<T>::get(staged<COPY>(from + St::gate, i, lane, i & 1 ? g1 : g0)), d[i], rest[i]);
-                if constexpr (RASTER) x[i] = raster_values<V>(held, i, lane);
+                if constexpr (RASTER) x[i] = raster_values<V>(from + St::x, i, lane);
                 else x[i] = Unpack<T>::get(staged<COPY>(from + St::x, i, lane, i & 1 ? x1 : x0));
                 o[i] = splat<V>(0.0f);
                 if (A.y.p) o[i] = Unpack<T>::get(staged<COPY>(from + St::dy, i, lane, i & 1 ? d1 : d0));
@@ -698,58 +701,61 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
             if (PC) d[0] = fixed;
             __syncwarp();
             fetch(t0 - S * round, slot);
-            fetch_words(t0 - round);
             slot = slot + 1 == S ? 0 : slot + 1;
-            Vec<V> a = one, h = splat<V>(0.0f), r = h;
+            Vec<V> h = h0, r = carry;
+            if constexpr (W > 1) {
+                Vec<V> a = one;
+                h = r = splat<V>(0.0f);
 #pragma unroll
-            for (int i = 0; i < L; ++i) {
-                const Decay<V, LO>& q = d[PC ? 0 : i];
-                h = q.step(h, LEAKY ? vmul(PC ? factor : rest[PC ? 0 : i], x[i]) : x[i]);
-                a = q.times(a);
-                r = d[PC ? 0 : L - 1 - i].times(vadd(o[L - 1 - i], r));
-            }
-            if (!some) {  // steps behind the end, whose rows were not read: r passes unchanged
-                a = one;
-                r = splat<V>(0.0f);
-            }
-            sa[par][w][lane] = a;
-            sh[par][w][lane] = h;
-            sr[par][w][lane] = r;
-            __syncthreads();
-            Vec<V> hw = h0;
+                for (int i = 0; i < L; ++i) {
+                    const Decay<V, LO>& q = d[PC ? 0 : i];
+                    h = q.step(h, LEAKY ? vmul(PC ? factor : rest[PC ? 0 : i], x[i]) : x[i]);
+                    a = q.times(a);
+                    r = d[PC ? 0 : L - 1 - i].times(vadd(o[L - 1 - i], r));
+                }
+                if (!some) {  // steps behind the end, whose rows were not read: r passes unchanged
+                    a = one;
+                    r = splat<V>(0.0f);
+                }
+                sa[par][w][lane] = a;
+                sh[par][w][lane] = h;
+                sr[par][w][lane] = r;
+                __syncthreads();
+                Vec<V> hw = h0;
 #pragma unroll
-            for (int j = 0; j < W; ++j) {
-                if (j == w) h = hw;
-                if (j < W - 1) hw = vfma(sa[par][j][lane], hw, sh[par][j][lane]);
-            }
-            // the maps of the warps behind this one (a, r) and of the whole tile (ta, tr)
-            Vec<V> ta = one, tr = CL > 1 ? splat<V>(0.0f) : carry;
+                for (int j = 0; j < W; ++j) {
+                    if (j == w) h = hw;
+                    if (j < W - 1) hw = vfma(sa[par][j][lane], hw, sh[par][j][lane]);
+                }
+                // the maps of the warps behind this one (a, r) and of the whole tile (ta, tr)
+                Vec<V> ta = one, tr = CL > 1 ? splat<V>(0.0f) : carry;
 #pragma unroll
-            for (int j = W - 1; j >= 0; --j) {
-                if (j == w) {
-                    a = ta;
-                    r = tr;
+                for (int j = W - 1; j >= 0; --j) {
+                    if (j == w) {
+                        a = ta;
+                        r = tr;
+                    }
+                    const Vec<V> ja = sa[par][j][lane];
+                    tr = vfma(ja, tr, sr[par][j][lane]);
+                    ta = vmul(ja, ta);
                 }
-                const Vec<V> ja = sa[par][j][lane];
-                tr = vfma(ja, tr, sr[par][j][lane]);
-                ta = vmul(ja, ta);
+                if (CL > 1) {
+                    for (int q = w; q < CL; q += W) {
+                        store_peer<V>(&cm.a[par][rank][lane], q, ta);
+                        store_peer<V>(&cm.h[par][rank][lane], q, tr);
+                    }
+                    cluster_sync();
+                    Vec<V> in = carry;
+                    for (int q = 0; q < CL; ++q) {
+                        if (q == rank) in = carry;
+                        carry = vfma(cm.a[par][q][lane], carry, cm.h[par][q][lane]);
+                    }
+                    r = vfma(a, in, r);
+                } else {
+                    carry = tr;
+                }
+                par ^= 1;
             }
-            if (CL > 1) {
-                for (int q = w; q < CL; q += W) {
-                    store_peer<V>(&cm.a[par][rank][lane], q, ta);
-                    store_peer<V>(&cm.h[par][rank][lane], q, tr);
-                }
-                cluster_sync();
-                Vec<V> in = carry;
-                for (int q = 0; q < CL; ++q) {
-                    if (q == rank) in = carry;
-                    carry = vfma(cm.a[par][q][lane], carry, cm.h[par][q][lane]);
-                }
-                r = vfma(a, in, r);
-            } else {
-                carry = tr;
-            }
-            par ^= 1;
             if (nl > 0 && some) {
                 // x becomes the derivative of h_t in a_t: h_{t-1}, or h_{t-1} - x_t
 #pragma unroll
@@ -779,6 +785,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
                     qx -= A.dx.st;
                 }
                 if (t0 == 0 && A.dh0) store_n<V>(A.dh0 + s * A.D + c, r, nl);
+                if (W == 1) carry = r;
             }
             pdg -= gjump;
             pdx -= xjump;
@@ -800,7 +807,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
 
 struct Plan {
     int ctiles, workers, cluster;
-    bool many;
+    int shape;  // 0 tiles, 1 smaller tiles (gradient), 2 a warp by itself
 };
 
 // the forward (GRAD = false) or gradient kernel of element type T
@@ -832,7 +839,7 @@ inline void launch(const void* kernel, int threads, int smem, const Plan& p, Sca
 
 template <bool GRAD, typename SH, typename T, int GM, bool RASTER, int COPY>
 void launch_shape(const Plan& p, ScanArgs& A, cudaStream_t st) {
-    const int smem = SH::W * SH::S * Stage<GM, RASTER, COPY, SH::L, GRAD>::bytes;
+    const int smem = SH::W * SH::S * Stage<GM, RASTER, COPY, SH::L, lane_channels<T>, GRAD>::bytes;
     const void* k;
     if constexpr (GRAD)
         k = A.leaky ? (const void*)k_scan_grad_tile<SH, T, GM, RASTER, true, COPY>
@@ -844,10 +851,13 @@ void launch_shape(const Plan& p, ScanArgs& A, cudaStream_t st) {
 }
 template <bool GRAD, typename T, int GM, bool RASTER, int COPY>
 void launch_copy(const Plan& p, ScanArgs& A, cudaStream_t st) {
-    if constexpr (!GRAD) launch_shape<false, Fwd, T, GM, RASTER, COPY>(p, A, st);
-    else if constexpr (RASTER) launch_shape<true, Bwd, T, GM, true, COPY>(p, A, st);
-    else if (p.many) launch_shape<true, BwdMany, T, GM, false, COPY>(p, A, st);
-    else launch_shape<true, Bwd, T, GM, false, COPY>(p, A, st);
+    if (p.shape == 2) return launch_shape<GRAD, std::conditional_t<GRAD, BwdSeq, FwdSeq>, T, GM, RASTER, COPY>(p, A, st);
+    if constexpr (GRAD) {
+        if (p.shape == 1) return launch_shape<true, BwdMany, T, GM, RASTER, COPY>(p, A, st);
+        launch_shape<true, Bwd, T, GM, RASTER, COPY>(p, A, st);
+    } else {
+        launch_shape<false, Fwd, T, GM, RASTER, COPY>(p, A, st);
+    }
 }
 template <bool GRAD, typename T, int GM>
 void launch_gate(bool raster, int words, const Plan& p, ScanArgs& A, cudaStream_t st) {
