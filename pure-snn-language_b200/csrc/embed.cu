@@ -51,23 +51,76 @@ __global__ void __launch_bounds__(E_THREADS) k_embed(const TOK* tok, long long n
     }
 }
 
+// A kernel launched as the dependent of the one before (launch_next) starts
+// while that one still runs: it must call after_previous() before it touches
+// what earlier kernels write.  let_next() allows the next kernel to start; it
+// comes after after_previous(), so that what ran before the previous kernel is
+// complete for the next one's start.
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <typename... P, typename... Q>
+void launch_next(void (*kernel)(P...), dim3 grid, dim3 block, cudaStream_t st, Q&&... args) {
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    SNN_CUDA(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
+}
+
 // ---- the positions sorted by token -------------------------------------------
 // Least significant digit first, up to 9 bits a pass (vocabularies of up to 511
 // tokens take one pass, up to 2^18 - 1 two).  A pass counts the digits of every
 // tile and scatters in input order, so positions of one token stay in
-// ascending order; a tile's offsets are sums over the counts (digit, tile),
-// taken by every scattering CTA itself where there are few tiles, else by a
-// scan between the two.
+// ascending order.  Launches are what a short sort costs: up to S_OWN items
+// every scattering CTA counts them all itself (one launch a pass), beyond there
+// are three: counts by tile, their sums by digit, the scatter.
 constexpr int S_THREADS = 512;
-constexpr int S_PER = 8;
+constexpr int S_PER = 4, S_OWN_PER = 2;  // items a thread
+constexpr int S_OWN = 32768;
 constexpr int S_TILE = S_THREADS * S_PER;
 constexpr int S_BINS = 512;
-constexpr int S_FEW = 96;  // tiles up to which a CTA sums the counts itself (192 KB of them)
 static_assert(S_BINS == S_THREADS, "a thread per digit");
 
 struct Pair {
     unsigned key, pos;
 };
+
+// The gradient's rows set to zero by CTAs of the first sorting kernel, most of
+// whose SMs are idle: rows that do not occur stay zero, the others are written
+// again by the sums.
+struct Clear {
+    char* p;
+    long long rows, row_bytes, stride;  // contiguous rows count as one
+    int word;                           // 16, 4 or 2 bytes a store
+    int ctas;                           // 0: nothing to clear
+};
+__device__ __forceinline__ void clear_rows(const Clear& C, int cta) {
+    const long long step = (long long)C.ctas * blockDim.x, t = (long long)cta * blockDim.x + threadIdx.x;
+    if (C.word == 16) {
+        const long long per = C.row_bytes / 16;
+        if (C.rows == 1) {
+            for (long long i = t; i < per; i += step) reinterpret_cast<uint4*>(C.p)[i] = make_uint4(0, 0, 0, 0);
+            for (long long i = per * 16 + t * 2; i < C.row_bytes; i += step * 2) *reinterpret_cast<unsigned short*>(C.p + i) = 0;
+        } else {
+            for (long long r = cta; r < C.rows; r += C.ctas)
+                for (long long i = threadIdx.x; i < per; i += blockDim.x)
+                    reinterpret_cast<uint4*>(C.p + r * C.stride)[i] = make_uint4(0, 0, 0, 0);
+        }
+    } else {
+        const long long per = C.row_bytes / C.word;
+        for (long long r = cta; r < C.rows; r += C.ctas)
+            for (long long i = threadIdx.x; i < per; i += blockDim.x) {
+                if (C.word == 4) reinterpret_cast<unsigned*>(C.p + r * C.stride)[i] = 0;
+                else reinterpret_cast<unsigned short*>(C.p + r * C.stride)[i] = 0;
+            }
+    }
+}
 
 template <typename TOK>
 struct FromTokens {
@@ -79,6 +132,8 @@ struct FromPairs {
     const Pair* p;
     __device__ Pair operator()(long long i) const { return p[i]; }
 };
+
+__global__ void __launch_bounds__(S_THREADS) k_clear(Clear clear) { clear_rows(clear, blockIdx.x); }
 
 // exclusive sum of one value a thread over the CTA (1,024 threads at most)
 __device__ __forceinline__ unsigned block_scan(unsigned v, unsigned* ws, unsigned& total) {
@@ -105,86 +160,89 @@ __device__ __forceinline__ unsigned block_scan(unsigned v, unsigned* ws, unsigne
     return r;
 }
 
-template <typename SRC>
+template <typename SRC, int PER>
 __global__ void __launch_bounds__(S_THREADS) k_sort_count(SRC src, long long n, int shift, int bins, unsigned* counts,
-                                                          uint8_t* present) {
+                                                          int tiles, Clear clear) {
     __shared__ unsigned h[S_BINS];
+    after_previous();
+    let_next();
+    if ((int)blockIdx.x >= tiles) return clear_rows(clear, blockIdx.x - tiles);
     h[threadIdx.x] = 0;
     __syncthreads();
-    const long long b = (long long)blockIdx.x * S_TILE;
-    Pair p[S_PER];
+    const long long b = (long long)blockIdx.x * (S_THREADS * PER);
+    Pair p[PER];
 #pragma unroll
-    for (int u = 0; u < S_PER; ++u) {
+    for (int u = 0; u < PER; ++u) {
         const long long i = b + u * S_THREADS + threadIdx.x;
         if (i < n) p[u] = src(i);
     }
 #pragma unroll
-    for (int u = 0; u < S_PER; ++u) {
-        if (b + u * S_THREADS + threadIdx.x < n) {
-            atomicAdd(&h[(p[u].key >> shift) & (bins - 1)], 1u);
-            if (present) present[p[u].key] = 1;
-        }
+    for (int u = 0; u < PER; ++u) {
+        if (b + u * S_THREADS + threadIdx.x < n) atomicAdd(&h[(p[u].key >> shift) & (bins - 1)], 1u);
     }
     __syncthreads();
-    if ((int)threadIdx.x < bins) counts[(size_t)threadIdx.x * gridDim.x + blockIdx.x] = h[threadIdx.x];
+    if ((int)threadIdx.x < bins)
+        counts[(size_t)threadIdx.x * tiles + blockIdx.x] = h[threadIdx.x];
 }
 
-// exclusive sum of m counts, one CTA
-__global__ void __launch_bounds__(1024) k_sort_scan(unsigned* c, int m) {
+// per digit: exclusive sums of the tiles' counts, and the digit's total
+__global__ void __launch_bounds__(256) k_sort_scan(unsigned* counts, int tiles, unsigned* totals) {
     __shared__ unsigned ws[32];
+    after_previous();
+    let_next();
+    unsigned* c = counts + (size_t)blockIdx.x * tiles;
     unsigned base = 0;
-    for (int b = 0; b < m; b += 4096) {
-        unsigned v[4], sum = 0, total;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int i = b + threadIdx.x * 4 + k;
-            v[k] = i < m ? c[i] : 0u;
-            sum += v[k];
-        }
-        unsigned at = base + block_scan(sum, ws, total);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int i = b + threadIdx.x * 4 + k;
-            if (i < m) c[i] = at;
-            at += v[k];
-        }
+    for (int b = 0; b < tiles; b += 256) {
+        const int i = b + threadIdx.x;
+        const unsigned v = i < tiles ? c[i] : 0u;
+        unsigned total;
+        const unsigned at = block_scan(v, ws, total);
+        if (i < tiles) c[i] = base + at;
         base += total;
     }
+    if (threadIdx.x == 0) totals[blockIdx.x] = base;
 }
 
-// FEW: counts are as counted; otherwise summed already
-template <typename SRC, bool FEW>
+// OWN: the CTA counts all n items itself; else counts and totals are from the scan
+template <typename SRC, bool OWN, int PER>
 __global__ void __launch_bounds__(S_THREADS) k_sort_scatter(SRC src, long long n, int shift, int bins,
-                                                            const unsigned* counts, Pair* out) {
+                                                            const unsigned* counts, const unsigned* totals, Pair* out,
+                                                            int tiles, Clear clear) {
     constexpr int W = S_THREADS / 32;
     __shared__ unsigned wc[W][S_BINS];
     __shared__ unsigned ws[32];
+    after_previous();
+    let_next();
+    if ((int)blockIdx.x >= tiles) return clear_rows(clear, blockIdx.x - tiles);
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    // a warp's S_PER * 32 items are consecutive
-    const long long b = (long long)blockIdx.x * S_TILE + w * (S_PER * 32) + lane;
-    Pair p[S_PER];
+    // a warp's PER * 32 items are consecutive
+    const long long tile = (long long)blockIdx.x * (S_THREADS * PER), b = tile + w * (PER * 32) + lane;
+    Pair p[PER];
 #pragma unroll
-    for (int u = 0; u < S_PER; ++u)
+    for (int u = 0; u < PER; ++u)
         if (b + u * 32 < n) p[u] = src(b + u * 32);
-    unsigned run = 0;  // of this thread's digit: items of smaller digits and of earlier tiles
-    if (FEW) {
-        unsigned before = 0, all = 0;
-        if ((int)threadIdx.x < bins)
-            for (int t = 0; t < (int)gridDim.x; ++t) {
-                const unsigned v = counts[(size_t)threadIdx.x * gridDim.x + t];
-                if (t < (int)blockIdx.x) before += v;
-                all += v;
-            }
-        unsigned total;
-        run = block_scan(all, ws, total) + before;
-    } else if ((int)threadIdx.x < bins) {
-        run = counts[(size_t)threadIdx.x * gridDim.x + blockIdx.x];
+    unsigned run = 0, total;  // of this thread's digit: items of smaller digits and of earlier tiles
+    if (OWN) {
+        wc[0][threadIdx.x] = wc[1][threadIdx.x] = 0;
+        __syncthreads();
+#pragma unroll 8
+        for (int i = threadIdx.x; i < (int)n; i += S_THREADS) {
+            const unsigned d = (src(i).key >> shift) & (bins - 1);
+            atomicAdd(&wc[i < (int)tile ? 0 : 1][d], 1u);
+        }
+        __syncthreads();
+        const unsigned before = wc[0][threadIdx.x];
+        run = block_scan(before + wc[1][threadIdx.x], ws, total) + before;
+    } else {
+        const bool in = (int)threadIdx.x < bins;
+        const unsigned before = in ? counts[(size_t)threadIdx.x * tiles + blockIdx.x] : 0u;
+        run = block_scan(in ? totals[threadIdx.x] : 0u, ws, total) + before;
     }
     for (int i = threadIdx.x; i < W * S_BINS; i += S_THREADS) (&wc[0][0])[i] = 0;
     __syncthreads();
-    unsigned rank[S_PER];
+    unsigned rank[PER];
 #pragma unroll
-    for (int u = 0; u < S_PER; ++u) {
+    for (int u = 0; u < PER; ++u) {
         const bool in = b + u * 32 < n;
         const unsigned live = __ballot_sync(~0u, in);
         if (in) {
@@ -206,7 +264,7 @@ __global__ void __launch_bounds__(S_THREADS) k_sort_scatter(SRC src, long long n
     }
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < S_PER; ++u)
+    for (int u = 0; u < PER; ++u)
         if (b + u * 32 < n) out[wc[w][(p[u].key >> shift) & (bins - 1)] + rank[u]] = p[u];
 }
 
@@ -286,7 +344,6 @@ struct GradArgs {
     void* out;
     long long ostride;
     float* part;
-    const uint8_t* present;
 };
 
 // The sorted positions are cut into pieces of `per`; blockDim.x threads sum one
@@ -300,19 +357,13 @@ constexpr int G_UNROLL = 8;
 constexpr int G_SHARED = 2048;  // positions a CTA holds, all its pieces together
 
 template <typename DT, typename OT, int V>
-__global__ void __launch_bounds__(G_THREADS) k_grad_pieces(const GradArgs A, int ctas) {
+__global__ void __launch_bounds__(G_THREADS, 8) k_grad_pieces(const GradArgs A) {
     using R = typename Raw<sizeof(DT) * V>::type;
     const int c = ((int)blockIdx.y * blockDim.x + threadIdx.x) * V;
     OT* const out = reinterpret_cast<OT*>(A.out);
-    if ((int)blockIdx.x >= ctas) {
-        if (c >= A.dim) return;
-        const float zero[V] = {};
-        for (unsigned v = (blockIdx.x - ctas) * blockDim.y + threadIdx.y; v < A.vocab;
-             v += (gridDim.x - ctas) * blockDim.y)
-            if (!A.present[v]) put_row<OT, V>(out + (long long)v * A.ostride + c, zero, 1.0f, 0, A.words);
-        return;
-    }
     __shared__ Pair held[G_SHARED];
+    after_previous();
+    let_next();
     const int first = blockIdx.x * blockDim.y * A.per;  // of the CTA's positions
     const int all = min(A.per * (int)blockDim.y, A.n - first);
     for (int i = threadIdx.y * blockDim.x + threadIdx.x; i < all; i += blockDim.x * blockDim.y)
@@ -371,8 +422,8 @@ __global__ void __launch_bounds__(G_THREADS) k_grad_pieces(const GradArgs A, int
     flush(cur == next);
 }
 
-// The runs that cross pieces: the CTA of the piece a run starts in sums the
-// run's parts, every J_GROUPS-th piece by one warp, the warps' sums in order.
+// The runs that cross pieces: the CTA of the piece a run starts in (found from
+// the sorted tokens while the pieces are still summed) sums the run's parts, every J_GROUPS-th piece by one warp, the warps' sums in order.
 constexpr int J_GROUPS = 8;
 constexpr int J_COLS = 4;
 template <typename OT>
@@ -384,13 +435,23 @@ __global__ void __launch_bounds__(32 * J_GROUPS) k_grad_join(const GradArgs A) {
     const unsigned before = b > 0 ? A.pair[b - 1].key : ~0u;
     if (key >= A.vocab || after != key) return;
     if (at == key && before == key) return;  // started earlier
-    int lo = piece + 1, hi = A.pieces;  // pieces (piece, end) begin with this key
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (A.pair[(long long)mid * A.per].key == key) lo = mid + 1;
-        else hi = mid;
-    }
     const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
+    int lo = piece + 1;  // becomes the end of the pieces that begin with this key
+    for (bool more = true; more; lo += 128) {
+        unsigned in[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const long long q = lo + k * 32 + lane;
+            in[k] = __ballot_sync(~0u, q < A.pieces && A.pair[q * A.per].key == key);
+        }
+        int run = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (run == k * 32) run += in[k] == ~0u ? 32 : __ffs(~in[k]) - 1;
+        more = run == 128;
+        if (!more) lo += run - 128;
+    }
+    after_previous();  // the pieces' sums
     __shared__ float s[J_GROUPS][J_COLS][32];
     const int c0 = blockIdx.y * (32 * J_COLS) + lane;
     float acc[J_COLS] = {};
@@ -413,11 +474,130 @@ __global__ void __launch_bounds__(32 * J_GROUPS) k_grad_join(const GradArgs A) {
     put_row<OT, 1>(reinterpret_cast<OT*>(A.out) + (long long)key * A.ostride + c, sum, A.scale, A.accumulate, 0);
 }
 
-// rows of a gradient without positions
-template <typename OT>
-__global__ void __launch_bounds__(256) k_grad_clear(unsigned vocab, int dim, OT* out, long long ostride) {
-    for (unsigned v = blockIdx.x; v < vocab; v += gridDim.x)
-        for (int c = threadIdx.x; c < dim; c += 256) out[(long long)v * ostride + c] = from_f32<OT>(0.0f);
+// Short calls in one launch: a CTA sorts all n tokens in shared memory (a
+// bitonic network over token * 2048 + position, so equal tokens keep their
+// order) and sums for 8 * V columns; groups of 8 threads take consecutive parts
+// of the sorted positions, and the group a run starts in joins its parts.
+// 512 bytes by 500 columns in f32: 29 us by the kernels above, 11 by this one.
+constexpr int T_THREADS = 512, T_COLS = 8, T_GROUPS = T_THREADS / T_COLS;
+constexpr int T_N = 2048, T_VOCAB = 4096;
+
+template <typename TOK, typename DT, typename OT, int V>
+__global__ void __launch_bounds__(T_THREADS) k_grad_small(const TOK* tok, const GradArgs A) {
+    using R = typename Raw<sizeof(DT) * V>::type;
+    __shared__ unsigned key[T_N];
+    __shared__ unsigned seen[T_VOCAB / 32 + 1];
+    __shared__ float part[T_GROUPS][2][T_COLS * V];
+    // element e * T_THREADS + thread: partners within a thread, a warp, or the CTA
+    constexpr int E = T_N / T_THREADS;
+    unsigned v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int i = e * T_THREADS + threadIdx.x;
+        v[e] = i < A.n ? token_at(tok, i, A.vocab) << 11 | i : ~0u;
+    }
+    for (int i = threadIdx.x; i < T_VOCAB / 32 + 1; i += T_THREADS) seen[i] = 0;
+    const int held = A.n <= T_THREADS ? 1 : E;
+    const int size = held * T_THREADS;
+    for (int k = 2; k <= size; k *= 2)
+        for (int j = k / 2; j > 0; j /= 2) {
+            if (j >= T_THREADS) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const int o = e ^ (j / T_THREADS);
+                    if (o > e && o < E) {
+                        const unsigned lo = min(v[e], v[o]), hi = max(v[e], v[o]);
+                        const bool up = ((e * T_THREADS) & k) == 0;
+                        v[e] = up ? lo : hi;
+                        v[o] = up ? hi : lo;
+                    }
+                }
+                continue;
+            }
+            if (j >= 32) {
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (e < held) key[e * T_THREADS + threadIdx.x] = v[e];
+                __syncthreads();
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                if (e >= held) continue;
+                const int i = e * T_THREADS + threadIdx.x;
+                const unsigned o = j >= 32 ? key[i ^ j] : __shfl_xor_sync(~0u, v[e], j);
+                v[e] = ((i & j) == 0) == ((i & k) == 0) ? min(v[e], o) : max(v[e], o);
+            }
+        }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (e < held) key[e * T_THREADS + threadIdx.x] = v[e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < A.n; i += T_THREADS) atomicOr(&seen[key[i] >> 16], 1u << (key[i] >> 11 & 31));
+    __syncthreads();
+    const int x = threadIdx.x % T_COLS, g = threadIdx.x / T_COLS;
+    const int c = (blockIdx.x * T_COLS + x) * V;
+    const bool live = c < A.dim;
+    const int per = (A.n + T_GROUPS - 1) / T_GROUPS, b = g * per, m = min(per, A.n - b);
+    OT* const out = reinterpret_cast<OT*>(A.out) + c;
+    float acc[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) acc[k] = 0.0f;
+    if (live && m > 0) {
+        const char* dy = reinterpret_cast<const char*>(reinterpret_cast<const DT*>(A.dy) + c);
+        const long long ds = A.dstride * (int)sizeof(DT);
+        unsigned cur = key[b] >> 11;
+        bool head = b > 0 && key[b - 1] >> 11 == cur;
+        for (int i0 = 0; i0 <= m; i0 += G_UNROLL) {
+            R in[G_UNROLL];
+#pragma unroll
+            for (int u = 0; u < G_UNROLL; ++u)
+                if (i0 < m) in[u] = *reinterpret_cast<const R*>(dy + (long long)(key[b + min(i0 + u, m - 1)] & (T_N - 1)) * ds);
+#pragma unroll
+            for (int u = 0; u < G_UNROLL; ++u) {
+                const int i = i0 + u;
+                if (i > m) break;
+                // i == m: the position behind the part, which ends its last run
+                const unsigned t = b + i < A.n ? key[b + i] >> 11 : ~0u;
+                if (t != cur || i == m) {
+                    const bool tail = i == m && t == cur;
+                    if (cur < A.vocab) {
+                        if (head || tail) {
+#pragma unroll
+                            for (int k = 0; k < V; ++k) part[g][head ? 0 : 1][x * V + k] = acc[k];
+                        } else {
+                            put_row<OT, V>(out + (long long)cur * A.ostride, acc, A.scale, A.accumulate, A.words);
+                        }
+                    }
+                    head = false;
+                    cur = t;
+#pragma unroll
+                    for (int k = 0; k < V; ++k) acc[k] = 0.0f;
+                }
+                if (i < m && t < A.vocab) add_raw(acc, in[u], DT());
+            }
+        }
+    }
+    __syncthreads();
+    if (!live) return;
+    if (m > 0 && b + m < A.n) {
+        const unsigned last = key[b + m - 1] >> 11;
+        const bool started = key[b] >> 11 != last || b == 0 || key[b - 1] >> 11 != last;
+        if (last < A.vocab && key[b + m] >> 11 == last && started) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) acc[k] = part[g][1][x * V + k];
+            for (int q = g + 1; q < T_GROUPS && q * per < A.n && key[q * per] >> 11 == last; ++q)
+#pragma unroll
+                for (int k = 0; k < V; ++k) acc[k] += part[q][0][x * V + k];
+            put_row<OT, V>(out + (long long)last * A.ostride, acc, A.scale, A.accumulate, A.words);
+        }
+    }
+    if (A.accumulate) return;
+#pragma unroll
+    for (int k = 0; k < V; ++k) acc[k] = 0.0f;
+    for (unsigned v = g; v < A.vocab; v += T_GROUPS)
+        if (!(seen[v >> 5] >> (v & 31) & 1u)) put_row<OT, V>(out + (long long)v * A.ostride, acc, 1.0f, 0, A.words);
 }
 
 // How the columns and positions are cut.  The order of the sums follows `per`,
@@ -430,14 +610,17 @@ int pieces_per(int64_t n, int64_t dim) {
 }
 
 struct GradWork {
-    int64_t pairs_a, pairs_b, counts, present, part, bytes;
+    int64_t pairs_a, pairs_b, counts, totals, part, bytes;
     int per, pieces, tiles;
+    bool small;
 };
 GradWork grad_work(int64_t n, int64_t vocab, int64_t dim) {
     GradWork w;
     w.per = pieces_per(n, dim);
     w.pieces = (int)((n + w.per - 1) / w.per);
     w.tiles = (int)((n + S_TILE - 1) / S_TILE);
+    w.small = n <= T_N && vocab <= T_VOCAB;
+    if (w.small) n = w.pieces = w.tiles = 0;
     int64_t at = 0;
     auto take = [&](int64_t b) {
         const int64_t p = at;
@@ -447,7 +630,7 @@ GradWork grad_work(int64_t n, int64_t vocab, int64_t dim) {
     w.pairs_a = take(n * 8);
     w.pairs_b = take(n * 8);
     w.counts = take((int64_t)S_BINS * w.tiles * 4);
-    w.present = take(vocab + 1);
+    w.totals = take(S_BINS * 4);
     w.part = take((int64_t)2 * w.pieces * dim * 4);
     w.bytes = std::max<int64_t>(at, 256);
     return w;
@@ -548,77 +731,109 @@ void embed_grad(const void* tokens, int32_t tok_type, int64_t n, const void* dy,
     char* w = (char*)work;
     Pair* a = (Pair*)(w + L.pairs_a);
     Pair* b = (Pair*)(w + L.pairs_b);
-    unsigned* counts = (unsigned*)(w + L.counts);
-    uint8_t* present = accumulate ? nullptr : (uint8_t*)(w + L.present);
-    float* part = (float*)(w + L.part);
-    if (n == 0) {
-        if (present)
-            with_elem(dtable_type, [&](auto ot) {
-                using OT = decltype(ot);
-                k_grad_clear<OT><<<(unsigned)std::min<int64_t>(vocab, SMS * 8), 256, 0, st>>>(
-                    (unsigned)vocab, (int)dim, (OT*)dtable, dtable_stride);
-            });
-        SNN_CUDA(cudaGetLastError());
-        return;
-    }
-    if (present) SNN_CUDA(cudaMemsetAsync(present, 0, (size_t)vocab + 1, st));
-    int bits = 1;
-    while ((vocab >> bits) != 0) ++bits;  // keys 0 .. vocab
-    const int passes = (bits + 8) / 9, digit = (bits + passes - 1) / passes, bins = 1 << digit;
-    auto pass = [&](auto src, int shift, Pair* dst, uint8_t* mark) {
-        using SRC = decltype(src);
-        k_sort_count<<<L.tiles, S_THREADS, 0, st>>>(src, (long long)n, shift, bins, counts, mark);
-        if (L.tiles <= S_FEW) {
-            k_sort_scatter<SRC, true><<<L.tiles, S_THREADS, 0, st>>>(src, (long long)n, shift, bins, counts, dst);
-        } else {
-            k_sort_scan<<<1, 1024, 0, st>>>(counts, bins * L.tiles);
-            k_sort_scatter<SRC, false><<<L.tiles, S_THREADS, 0, st>>>(src, (long long)n, shift, bins, counts, dst);
-        }
-    };
-    with_token(tok_type, tokens, [&](auto tok) {
-        using TOK = std::remove_const_t<std::remove_pointer_t<decltype(tok)>>;
-        pass(FromTokens<TOK>{tok, (unsigned)vocab}, 0, a, present);
-    });
-    for (int k = 1; k < passes; ++k) {
-        pass(FromPairs{a}, k * digit, b, (uint8_t*)nullptr);
-        std::swap(a, b);
-    }
+    unsigned *counts = (unsigned*)(w + L.counts), *totals = (unsigned*)(w + L.totals);
     GradArgs A;
-    A.pair = a;
+    A.pair = nullptr;
     A.n = (int)n;
     A.per = L.per;
     A.pieces = L.pieces;
     A.dim = (int)dim;
     A.accumulate = accumulate != 0;
+    A.words = 0;
     A.vocab = (unsigned)vocab;
     A.dy = dy;
     A.dstride = dy_stride;
     A.scale = scale;
     A.out = dtable;
     A.ostride = dtable_stride;
-    A.part = part;
-    A.present = present;
-    with_elem(dy_type, [&](auto dt) {
-        with_elem(dtable_type, [&](auto ot) {
-            using DT = decltype(dt);
-            using OT = decltype(ot);
-            auto go = [&](auto vc) {
-                constexpr int V = decltype(vc)::value;
-                A.words = fits(dtable, dtable_type, dim, dtable_stride, V);
-                int tx = 1;  // threads a row of a piece, a power of two
-                while (tx < G_THREADS && (int64_t)tx * V < dim) tx *= 2;
-                const int ty = std::min(G_THREADS / tx, G_SHARED / L.per);
-                const unsigned ctas = (unsigned)((L.pieces + ty - 1) / ty);
-                const unsigned clear = present ? (unsigned)std::min<int64_t>((vocab + ty - 1) / ty, SMS * 4) : 0u;
-                const unsigned cols = (unsigned)((dim + (int64_t)tx * V - 1) / ((int64_t)tx * V));
-                k_grad_pieces<DT, OT, V><<<dim3(ctas + clear, cols), dim3(tx, ty), 0, st>>>(A, (int)ctas);
-            };
-            constexpr int V16 = 16 / (int)sizeof(DT);
-            if (fits(dy, dy_type, dim, dy_stride, V16)) go(std::integral_constant<int, V16>());
-            else go(std::integral_constant<int, 1>());
-            k_grad_join<OT><<<dim3((unsigned)L.pieces, (unsigned)((dim + 32 * J_COLS - 1) / (32 * J_COLS))),
-                              32 * J_GROUPS, 0, st>>>(A);
+    A.part = (float*)(w + L.part);
+    // f(DT(), OT(), V): the types and the columns a thread takes
+    auto typed = [&](auto&& f) {
+        with_elem(dy_type, [&](auto dt) {
+            with_elem(dtable_type, [&](auto ot) {
+                constexpr int V16 = 16 / (int)sizeof(dt);
+                if (n > 0 && fits(dy, dy_type, dim, dy_stride, V16)) {
+                    A.words = fits(dtable, dtable_type, dim, dtable_stride, V16);
+                    f(dt, ot, std::integral_constant<int, V16>());
+                } else {
+                    A.words = 1;
+                    f(dt, ot, std::integral_constant<int, 1>());
+                }
+            });
         });
+    };
+    if (L.small) {
+        with_token(tok_type, tokens, [&](auto tok) {
+            using TOK = std::remove_const_t<std::remove_pointer_t<decltype(tok)>>;
+            typed([&](auto dt, auto ot, auto vc) {
+                constexpr int V = decltype(vc)::value;
+                const unsigned ctas = (unsigned)((dim + T_COLS * V - 1) / (T_COLS * V));
+                k_grad_small<TOK, decltype(dt), decltype(ot), V><<<ctas, T_THREADS, 0, st>>>(tok, A);
+            });
+        });
+        SNN_CUDA(cudaGetLastError());
+        return;
+    }
+    const int size = elem_size(dtable_type);
+    Clear clear = {(char*)dtable, vocab, dim * size, dtable_stride * size, 0, 0};
+    if (!accumulate) {
+        if (clear.stride == clear.row_bytes) {
+            clear.row_bytes *= vocab;
+            clear.rows = 1;
+        }
+        const bool wide = (uintptr_t)dtable % 16 == 0 &&
+                          (clear.rows == 1 || (clear.row_bytes % 16 == 0 && clear.stride % 16 == 0));
+        clear.word = wide ? 16 : size;
+        clear.ctas = (int)std::min<int64_t>(SMS * 3, (clear.rows * clear.row_bytes + (1 << 14) - 1) >> 14);
+    }
+    if (n == 0) {
+        if (clear.ctas) k_clear<<<(unsigned)clear.ctas, S_THREADS, 0, st>>>(clear);
+        SNN_CUDA(cudaGetLastError());
+        return;
+    }
+    const Clear nothing = {nullptr, 0, 0, 0, 0, 0};
+    int bits = 1;
+    while ((vocab >> bits) != 0) ++bits;  // keys 0 .. vocab
+    const int passes = (bits + 8) / 9, digit = (bits + passes - 1) / passes, bins = 1 << digit;
+    bool later = false;  // the first kernel waits for all work before the call
+    auto pass = [&](auto src, int shift, Pair* dst, const Clear& C) {
+        using SRC = decltype(src);
+        auto start = [&](auto kernel, int ctas, auto... args) {
+            if (later) launch_next(kernel, dim3(ctas), dim3(S_THREADS), st, args...);
+            else kernel<<<ctas, S_THREADS, 0, st>>>(args...);
+            later = true;
+        };
+        if (n <= S_OWN) {
+            const int tiles = (int)((n + S_THREADS * S_OWN_PER - 1) / (S_THREADS * S_OWN_PER));
+            start(k_sort_scatter<SRC, true, S_OWN_PER>, tiles + C.ctas, src, (long long)n, shift, bins, counts, totals,
+                  dst, tiles, C);
+            return;
+        }
+        start(k_sort_count<SRC, S_PER>, L.tiles + C.ctas, src, (long long)n, shift, bins, counts, L.tiles, C);
+        launch_next(k_sort_scan, dim3(bins), dim3(256), st, counts, L.tiles, totals);
+        launch_next(k_sort_scatter<SRC, false, S_PER>, dim3(L.tiles), dim3(S_THREADS), st, src, (long long)n, shift, bins,
+                    counts, totals, dst, L.tiles, nothing);
+    };
+    with_token(tok_type, tokens, [&](auto tok) {
+        using TOK = std::remove_const_t<std::remove_pointer_t<decltype(tok)>>;
+        pass(FromTokens<TOK>{tok, (unsigned)vocab}, 0, a, clear);
+    });
+    for (int k = 1; k < passes; ++k) {
+        pass(FromPairs{a}, k * digit, b, nothing);
+        std::swap(a, b);
+    }
+    A.pair = a;
+    typed([&](auto dt, auto ot, auto vc) {
+        using OT = decltype(ot);
+        constexpr int V = decltype(vc)::value;
+        int tx = 1;  // threads a row of a piece, a power of two
+        while (tx < G_THREADS && (int64_t)tx * V < dim) tx *= 2;
+        const int ty = std::min(G_THREADS / tx, G_SHARED / L.per);
+        const unsigned ctas = (unsigned)((L.pieces + ty - 1) / ty);
+        const unsigned cols = (unsigned)((dim + (int64_t)tx * V - 1) / ((int64_t)tx * V));
+        launch_next(k_grad_pieces<decltype(dt), OT, V>, dim3(ctas, cols), dim3(tx, ty), st, A);
+        launch_next(k_grad_join<OT>, dim3((unsigned)L.pieces, (unsigned)((dim + 32 * J_COLS - 1) / (32 * J_COLS))),
+                    dim3(32 * J_GROUPS), st, A);
     });
     SNN_CUDA(cudaGetLastError());
 }
