@@ -138,7 +138,8 @@ constexpr bool keeps_lo = GM == GATE_CHANNEL_LOGIT || (GM == GATE_LOGIT && sizeo
 // exponential instruction is, where the product alone would be off by |z|
 // 2^-24.  Beyond |z| = 150 e is 0.
 __device__ __forceinline__ void logistic(float z, float& a, float& lo, float& rest) {
-    const float m = fminf(fabsf(z), 150.0f);
+    float m;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(fabsf(z)), "f"(150.0f));
     const float p = m * -1.44269502f;  // log2(e) = 1.44269502 + 1.9259630e-8
     const float q = fmaf(m, -1.92596303e-8f, fmaf(m, -1.44269502f, -p));
     float e, big;
@@ -151,7 +152,6 @@ __device__ __forceinline__ void logistic(float z, float& a, float& lo, float& re
     a = up ? near1 : s;
     lo = up ? (1.0f - near1) - s : 0.0f;
     rest = up ? s : big;
-    if (z != z) a = rest = z;
 }
 // the same by the short instructions (2 ulp each, the argument rounded once)
 __device__ __forceinline__ void logistic_fast(float z, float& a, float& rest) {
@@ -301,6 +301,9 @@ struct Shape {
 };
 using Fwd = Shape<8, 16, 2, 2>;
 using Bwd = Shape<8, 8, 3, 2>;
+// Decays per channel leave the forward pass registers for a third CTA (the
+// gradient spills and loses by one: documents 171 -> 187 us).
+using FwdChannel = Shape<8, 16, 2, 3>;
 // Without clusters the gradient takes smaller CTAs, twice as many on an SM.
 using BwdMany = Shape<4, 8, 3, 4>;
 // Where channels and sequences alone fill the SMs with warps: a warp by itself,
@@ -815,7 +818,8 @@ template <bool GRAD, typename T>
 void launch_tiles(int gate_mode, bool raster, int words, const Plan& p, ScanArgs& A, cudaStream_t st);
 
 #ifdef SNN_SCAN_TILE_LAUNCH
-inline void launch(const void* kernel, int threads, int smem, const Plan& p, ScanArgs& A, cudaStream_t st) {
+inline void launch(const void* kernel, std::atomic<uint64_t>& ready, int threads, int smem, const Plan& p, ScanArgs& A,
+                   cudaStream_t st) {
     A.ctiles = p.ctiles;
     A.workers = p.workers;
     A.cluster = p.cluster;
@@ -832,7 +836,15 @@ inline void launch(const void* kernel, int threads, int smem, const Plan& p, Sca
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = p.cluster > 1 ? 1 : 0;
-    SNN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (smem > 0) {  // more than the default needs asking, once on a device
+        int dev = 0;
+        SNN_CUDA(cudaGetDevice(&dev));
+        SNN_REQUIRE(dev >= 0 && dev < 64, SNN_ERR_ARG, "device ordinal above 63");
+        if (!(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+            SNN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+            ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+        }
+    }
     void* args[] = {&A};
     SNN_CUDA(cudaLaunchKernelExC(&cfg, kernel, args));
 }
@@ -847,7 +859,8 @@ void launch_shape(const Plan& p, ScanArgs& A, cudaStream_t st) {
     else
         k = A.leaky ? (const void*)k_scan_tile<SH, T, GM, RASTER, true, COPY>
                     : (const void*)k_scan_tile<SH, T, GM, RASTER, false, COPY>;
-    launch(k, SH::threads, smem, p, A, st);
+    static std::atomic<uint64_t> ready[2];  // by device, of the two kernels
+    launch(k, ready[A.leaky ? 1 : 0], SH::threads, smem, p, A, st);
 }
 template <bool GRAD, typename T, int GM, bool RASTER, int COPY>
 void launch_copy(const Plan& p, ScanArgs& A, cudaStream_t st) {
@@ -856,7 +869,7 @@ void launch_copy(const Plan& p, ScanArgs& A, cudaStream_t st) {
         if (p.shape == 1) return launch_shape<true, BwdMany, T, GM, RASTER, COPY>(p, A, st);
         launch_shape<true, Bwd, T, GM, RASTER, COPY>(p, A, st);
     } else {
-        launch_shape<false, Fwd, T, GM, RASTER, COPY>(p, A, st);
+        launch_shape<false, std::conditional_t<per_channel<GM>, FwdChannel, Fwd>, T, GM, RASTER, COPY>(p, A, st);
     }
 }
 template <bool GRAD, typename T, int GM>
