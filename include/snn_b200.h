@@ -409,7 +409,7 @@ int snn_propagate_static(const int32_t* post, const float* w, int64_t n_pre, int
  * rounded once to out_type.  table is [vocab, dim], out [n, dim], both with
  * unit column stride and the given row strides in elements (< 2^32; of what is
  * written >= dim).  A token
- * outside [0, vocab) gives a row of zeros.  n <= 2^30, vocab < 2^31. */
+ * outside [0, vocab) gives a row of zeros.  n <= 2^30, vocab < 2^31, dim <= 2^22. */
 int snn_embed(const void* tokens, int32_t tok_type, int64_t n, const void* table,
               int32_t table_type, int64_t vocab, int64_t dim, int64_t table_stride, float scale,
               void* out, int32_t out_type, int64_t out_stride, void* stream);
@@ -419,11 +419,11 @@ int snn_embed(const void* tokens, int32_t tok_type, int64_t n, const void* table
  * (added to what dtable holds when accumulate is non-zero; rows that do not
  * occur are then not touched, otherwise they become zero).  Tokens outside
  * [0, vocab) contribute nothing.  The positions are sorted by token and summed in
- * f32 in an order that depends on the tokens, n and dim alone, so equal calls give
- * equal bits; rounded once to dtable_type.  work: work_bytes bytes of device
+ * f32 in an order that depends on the tokens, sizes and alignment alone, so equal
+ * calls give equal bits; rounded once to dtable_type.  work: work_bytes bytes of device
  * memory, 256-byte aligned, at least what snn_embed_grad_workspace says for
  * the same n, vocab and dim; it is free again when the call's work on `stream`
- * is done.  n <= 2^30, vocab < 2^31. */
+ * is done.  Limits as above. */
 int snn_embed_grad_workspace(int64_t n, int64_t vocab, int64_t dim, int64_t* bytes);
 int snn_embed_grad(const void* tokens, int32_t tok_type, int64_t n, const void* dy,
                    int32_t dy_type, int64_t dim, int64_t dy_stride, float scale, void* dtable,
@@ -433,7 +433,8 @@ int snn_embed_grad(const void* tokens, int32_t tok_type, int64_t n, const void* 
 /* Leaky scan: along every sequence, for every channel,
  *   h_t = a_t h_{t-1} + u_t,   y_t = h_t,   u_t = x_t, or (1 - a_t) x_t with SNN_SCAN_LEAKY
  * with a_t the gate, or 1 / (1 + exp(-gate)) with SNN_SCAN_LOGIT.  The state
- * is f32; y is rounded once.
+ * is f32; y is rounded once.  n_steps <= 2^30, n_channels < 2^30.  A state that
+ * has become infinite stays infinite or turns NaN.
  * Layout: dense (offsets NULL): n_seq sequences of n_steps steps; packed
  * (offsets set): n_steps rows in all, sequence s the rows
  * [offsets[s], offsets[s + 1]) of every tensor (int64[n_seq + 1] in device
@@ -442,7 +443,7 @@ int snn_embed_grad(const void* tokens, int32_t tok_type, int64_t n, const void* 
  * final state is its initial one.
  * Strides are any of which rows that are written do not overlap (time-major
  * rows too); what is only read may be broadcast by a stride of 0.  Outputs
- * must not overlap inputs, but for h and dh0 below.
+ * must not overlap inputs, but for h below.
  * x, y, gate are [.., channels] rows of element type `type`, unit channel
  * stride; with SNN_SCAN_RASTER x is the packed spike raster of snn_run
  * (uint32 words, bit c % 32 of word c / 32) and strides are in words; with
@@ -481,7 +482,7 @@ int snn_leaky_scan(const snn_scan* desc, const snn_rows* gate, const snn_rows* x
  * dgate (nullable) has the gate's form: rows, or with SNN_SCAN_CHANNEL f32
  * [n_channels], the sum over all steps of all sequences in an order that
  * depends on the sizes alone.  dx (nullable, NULL with SNN_SCAN_RASTER) and dh0
- * (nullable, f32 [n_seq, n_channels], may be dh itself) as their inputs; rows of no sequence are
+ * (nullable, f32 [n_seq, n_channels]) as their inputs; rows of no sequence are
  * not written.  saved is what the forward call wrote.  work: as for
  * snn_embed_grad, of the size that snn_leaky_scan_grad_workspace says. */
 int snn_leaky_scan_grad_workspace(const snn_scan* desc, int64_t* bytes);

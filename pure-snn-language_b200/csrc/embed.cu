@@ -4,6 +4,7 @@
 #include "elem.h"
 
 namespace {
+constexpr int SMS = 148;  // multiprocessors of a B200
 using snnb::from_f32;
 using snnb::to_f32;
 
@@ -603,7 +604,6 @@ __global__ void __launch_bounds__(T_THREADS) k_grad_small(const TOK* tok, const 
 // How the columns and positions are cut.  The order of the sums follows `per`,
 // so it goes by n and dim alone: pieces such that SMS * 8 CTAs' worth of threads
 // have one each, of 32 to 1,024 positions.
-constexpr int SMS = 148;
 int pieces_per(int64_t n, int64_t dim) {
     const int64_t cols = (dim + 1023) / 1024, wanted = std::max<int64_t>(1, SMS * 8 / cols);
     return (int)std::min<int64_t>(1024, std::max<int64_t>(32, (n + wanted - 1) / wanted));
@@ -662,7 +662,7 @@ void check_rows(const void* p, int32_t type, int64_t dim, int64_t stride, const 
 void check_sizes(int64_t n, int64_t vocab, int64_t dim) {
     SNN_REQUIRE(n >= 0 && n <= (1ll << 30), SNN_ERR_ARG, "embed: n must lie in [0, 2^30]");
     SNN_REQUIRE(vocab >= 1 && vocab < (1ll << 31), SNN_ERR_ARG, "embed: vocab must lie in [1, 2^31)");
-    SNN_REQUIRE(dim >= 1 && dim < (1ll << 24), SNN_ERR_ARG, "embed: dim must lie in [1, 2^24)");
+    SNN_REQUIRE(dim >= 1 && dim <= (1ll << 22), SNN_ERR_ARG, "embed: dim must lie in [1, 2^22]");
 }
 
 // whether rows at p, `stride` elements apart, can be accessed in words of v elements

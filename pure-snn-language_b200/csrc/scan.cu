@@ -18,20 +18,32 @@ __global__ void __launch_bounds__(128) k_scan_steps(const ScanArgs A) {
         Vec<V> rest;
         if (per_channel<GM>) channel_decays<T, GM, V>(A, c, V, d, rest);
         Vec<V> h = load_f32<V>(A.h0 + s * A.D + c, A.h0 != nullptr);
-        for (int t = 0; t < sp.len; ++t) {
-            if (A.saved && t % BLOCK == 0) store_f32<V>(A.saved + (sp.block0 + t / BLOCK) * A.D + c, h);
-            if (!per_channel<GM>) {
-                const Word<T, V> g = *reinterpret_cast<const Word<T, V>*>(
-                    reinterpret_cast<const T*>(A.gate.p) + row_at(A, A.gate, s, sp, t) + c);
-                decays<T, GM, V>(Unpack<T>::get(g), d, rest);
+        constexpr int U = 4;  // steps whose rows are loaded before the first is used
+        for (int t0 = 0; t0 < sp.len; t0 += U) {
+            Word<T, V> g[U];
+            X xw[U];
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const int t = min(t0 + i, sp.len - 1);
+                if (!per_channel<GM>)
+                    g[i] = *reinterpret_cast<const Word<T, V>*>(reinterpret_cast<const T*>(A.gate.p) +
+                                                                row_at(A, A.gate, s, sp, t) + c);
+                const long long xr = row_at(A, A.x, s, sp, t);
+                xw[i] = RASTER ? *reinterpret_cast<const X*>(reinterpret_cast<const unsigned*>(A.x.p) + xr + (c >> 5))
+                               : *reinterpret_cast<const X*>(reinterpret_cast<const T*>(A.x.p) + xr + c);
             }
-            const long long xr = row_at(A, A.x, s, sp, t);
-            const X xw = RASTER ? *reinterpret_cast<const X*>(reinterpret_cast<const unsigned*>(A.x.p) + xr + (c >> 5))
-                                : *reinterpret_cast<const X*>(reinterpret_cast<const T*>(A.x.p) + xr + c);
-            Vec<V> u = in_values<T, V, RASTER>(xw, c);
-            if (A.leaky) u = vmul(rest, u);
-            h = d.step(h, u);
-            *reinterpret_cast<Word<T, V>*>(reinterpret_cast<T*>(A.y.p) + row_at(A, A.y, s, sp, t) + c) = Unpack<T>::put(h);
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const int t = t0 + i;
+                if (t >= sp.len) break;
+                if (A.saved && t % BLOCK == 0) store_f32<V>(A.saved + (sp.block0 + t / BLOCK) * A.D + c, h);
+                if (!per_channel<GM>) decays<T, GM, V>(Unpack<T>::get(g[i]), d, rest);
+                Vec<V> u = in_values<T, V, RASTER>(xw[i], c);
+                if (A.leaky) u = vmul(rest, u);
+                h = d.step(h, u);
+                *reinterpret_cast<Word<T, V>*>(reinterpret_cast<T*>(A.y.p) + row_at(A, A.y, s, sp, t) + c) =
+                    Unpack<T>::put(h);
+            }
         }
         if (A.h) store_f32<V>(A.h + s * A.D + c, h);
     }
@@ -91,7 +103,12 @@ Rows rows_of(const snn_scan* d, const snn_rows* r, const char* name, int64_t wid
     return {r->data, ss, st};
 }
 
+void check_states(std::initializer_list<const void*> p) {
+    for (const void* q : p) SNN_REQUIRE((uintptr_t)q % 4 == 0, SNN_ERR_ARG, "scan: misaligned states");
+}
+
 ScanArgs base_args(const snn_scan* d, const snn_rows* gate, const snn_rows* x) {
+    SNN_REQUIRE((uintptr_t)d->offsets % 8 == 0, SNN_ERR_ARG, "scan: misaligned offsets");
     ScanArgs A;
     memset(&A, 0, sizeof(A));
     A.off = d->offsets;
@@ -181,6 +198,7 @@ void leaky_scan(const snn_scan* d, const snn_rows* gate, const snn_rows* x, cons
     if (d->n_seq == 0) return;
     ScanArgs A = base_args(d, gate, x);
     A.y = rows_of(d, y, "y", d->n_channels, elem_size(d->type), true);
+    check_states({h0, h, saved});
     A.h0 = h0;
     A.h = h;
     A.saved = saved;
@@ -230,6 +248,7 @@ void leaky_scan_grad(const snn_scan* d, const snn_rows* gate, const snn_rows* x,
     SNN_REQUIRE(saved, SNN_ERR_ARG, "scan: null saved");
     ScanArgs A = base_args(d, gate, x);
     const int size = elem_size(d->type);
+    check_states({saved, dh, dh0});
     A.saved = const_cast<float*>(saved);
     A.dh = dh;
     A.dh0 = dh0;

@@ -306,7 +306,8 @@ def embed(tokens, table, scale=1.0, dtype=None, out=None, stream=None):
     [vocab, dim] in float32 / bfloat16 / float16, unit column stride.  Returns
     tokens.shape + (dim,) in `dtype` (default: the table's), or `out`.  A
     token outside [0, vocab) gives zeros.  Runs on `stream` (default: the
-    current stream of the tensors' device), on which new results are made."""
+    current stream of the tensors' device), on which new results are made.
+    autograd does not see these operators: embed_grad is the gradient."""
     if _T is None:
         _torch()
     dev, tok = _tokens(tokens)

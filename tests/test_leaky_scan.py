@@ -89,13 +89,13 @@ BAD = [dict(desc=dict(type=3)), dict(desc=dict(flags=16)), dict(desc=dict(n_seq=
        dict(desc=dict(flags=4), gate=(8194, 0, 0))]
 
 
-@pytest.mark.parametrize("over", BAD + [dict(y=None), dict(y=(8192, 40, 7)), dict(y=(8192, 39, 8)), dict(y=(8192, 0, 8))])
+@pytest.mark.parametrize("over", BAD + [dict(h0=1026), dict(h=1026), dict(saved=(1 << 20) + 2), dict(desc=dict(offsets=4100)), dict(y=None), dict(y=(8192, 40, 7)), dict(y=(8192, 39, 8)), dict(y=(8192, 0, 8))])
 def test_scan_refuses(over):
     assert call(**over) == 1 and b"scan" in snn.lib().snn_last_error(None)
 
 
 @pytest.mark.parametrize("over", BAD + [
-    dict(y=None), dict(saved=None), dict(dx=(8192, 40, 7)), dict(dgate=(8192, 39, 8)), dict(desc=dict(flags=8)),
+    dict(y=None), dict(saved=None), dict(dh=1026), dict(dh0=1026), dict(dx=(8192, 40, 7)), dict(dgate=(8192, 39, 8)), dict(desc=dict(flags=8)),
     dict(desc=dict(flags=4)), dict(desc=dict(flags=4), work=1 << 21, bytes=8),
     dict(desc=dict(flags=4), work=(1 << 21) + 4, bytes=1 << 30)])
 def test_scan_grad_refuses(over):

@@ -45,7 +45,7 @@ def embed_args(**over):
 
 @pytest.mark.parametrize("over", [
     dict(tokens=None), dict(tok=3), dict(tok=9, tokens=4098), dict(n=-1), dict(n=(1 << 30) + 1),
-    dict(table=None), dict(table=8194), dict(ttype=3), dict(vocab=0), dict(vocab=1 << 31), dict(dim=0),
+    dict(table=None), dict(table=8194), dict(ttype=3), dict(vocab=0), dict(vocab=1 << 31), dict(dim=0), dict(dim=(1 << 22) + 1, tstride=1 << 23, ostride=1 << 23),
     dict(tstride=-1), dict(out=None), dict(otype=7), dict(otype=1, out=16385), dict(ostride=7)])
 def test_embed_refuses(over):
     assert snn.lib().snn_embed(*embed_args(**over)) == 1
@@ -177,6 +177,23 @@ def test_embed_grad_accumulates(n, vocab, dim, ok):
     want, bound = ref.embed_grad(t.cpu().numpy(), host(dy), vocab, 1.0, base=host(before[:, :dim]))
     ref.close(host(got), want, bound, ok)
     assert torch.equal(out[:, dim:], before[:, dim:]) and torch.equal(out[vocab // 2:], before[vocab // 2:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ok", ["f32", "bf16"])
+@pytest.mark.parametrize("n,vocab,dim,width", [(0, 5000, 24, 40), (300, 50, 9, 12), (3000, 50, 33, 40), (3000, 6000, 24, 32),
+                                               (50000, 700, 17, 18), (40000, 20, 256, 264)])
+def test_embed_grad_into_wider_rows(n, vocab, dim, width, ok):
+    """Rows of `out` inside wider ones: all of its own are written, what lies beside them stays."""
+    import torch
+    rng = np.random.default_rng(n + dim)
+    t = torch.from_numpy(rng.integers(0, max(vocab // 2, 1), n).astype(np.int32)).cuda()
+    dy = make(rng, (n, dim), "bf16")
+    wide = torch.full((vocab, width), 7.0, dtype=dt(ok), device="cuda")
+    got = snn.embed_grad(t, dy, out=wide[:, width - dim:])
+    want, bound = ref.embed_grad(t.cpu().numpy(), host(dy), vocab, 1.0)
+    ref.close(host(got), want, bound, ok)
+    assert (wide[:, :width - dim] == 7).all()
 
 
 @pytest.mark.gpu
