@@ -469,10 +469,14 @@ typedef struct snn_rows {    /* one tensor of rows                              
 /* h0 (nullable: zeros) and h (nullable) are f32 [n_seq, n_channels]; h may be
  * h0 itself, so that one state is carried from call to call.  saved (nullable)
  * receives the states that snn_leaky_scan_grad starts its blocks of steps from:
- * snn_leaky_scan_saved(desc) floats. */
+ * snn_leaky_scan_saved(desc) floats.  work: as for snn_embed_grad, of
+ * the size that snn_leaky_scan_workspace says for the same description (it may
+ * be 0). */
 int snn_leaky_scan_saved(const snn_scan* desc, int64_t* floats);
+int snn_leaky_scan_workspace(const snn_scan* desc, int64_t* bytes);
 int snn_leaky_scan(const snn_scan* desc, const snn_rows* gate, const snn_rows* x, const float* h0,
-                   const snn_rows* y, float* h, float* saved, void* stream);
+                   const snn_rows* y, float* h, float* saved, void* work, int64_t work_bytes,
+                   void* stream);
 
 /* Gradients of snn_leaky_scan, from the gradients dy of y (nullable) and dh
  * of the final state (nullable; not both NULL):

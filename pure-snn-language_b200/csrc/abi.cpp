@@ -428,14 +428,22 @@ int snn_leaky_scan_saved(const snn_scan* desc, int64_t* floats) {
 }
 
 int snn_leaky_scan(const snn_scan* desc, const snn_rows* gate, const snn_rows* x, const float* h0,
-                   const snn_rows* y, float* h, float* saved, void* stream) {
-    return guard_op([&] { snnb::leaky_scan(desc, gate, x, h0, y, h, saved, (cudaStream_t)stream); });
+                   const snn_rows* y, float* h, float* saved, void* work, int64_t work_bytes, void* stream) {
+    return guard_op(
+        [&] { snnb::leaky_scan(desc, gate, x, h0, y, h, saved, work, work_bytes, (cudaStream_t)stream); });
+}
+
+int snn_leaky_scan_workspace(const snn_scan* desc, int64_t* bytes) {
+    return guard_op([&] {
+        SNN_REQUIRE(bytes, SNN_ERR_ARG, "null result");
+        *bytes = snnb::leaky_scan_workspace(desc, false);
+    });
 }
 
 int snn_leaky_scan_grad_workspace(const snn_scan* desc, int64_t* bytes) {
     return guard_op([&] {
         SNN_REQUIRE(bytes, SNN_ERR_ARG, "null result");
-        *bytes = snnb::leaky_scan_grad_workspace(desc);
+        *bytes = snnb::leaky_scan_workspace(desc, true);
     });
 }
 

@@ -121,9 +121,9 @@ void embed_grad(const void* tokens, int32_t tok_type, int64_t n, const void* dy,
                 int64_t dy_stride, float scale, void* dtable, int32_t dtable_type, int64_t vocab,
                 int64_t dtable_stride, int32_t accumulate, void* work, int64_t work_bytes, cudaStream_t stream);
 int64_t leaky_scan_saved(const snn_scan* desc);
-int64_t leaky_scan_grad_workspace(const snn_scan* desc);
+int64_t leaky_scan_workspace(const snn_scan* desc, bool grad);
 void leaky_scan(const snn_scan* desc, const snn_rows* gate, const snn_rows* x, const float* h0, const snn_rows* y,
-                float* h, float* saved, cudaStream_t stream);
+                float* h, float* saved, void* work, int64_t work_bytes, cudaStream_t stream);
 void leaky_scan_grad(const snn_scan* desc, const snn_rows* gate, const snn_rows* x, const float* saved,
                      const snn_rows* dy, const float* dh, const snn_rows* dgate, const snn_rows* dx, float* dh0,
                      void* work, int64_t work_bytes, cudaStream_t stream);

@@ -69,6 +69,47 @@ __global__ void __launch_bounds__(256) k_scan_gate_sum(const ScanArgs A, int row
     reinterpret_cast<float*>(A.dgate.p)[c] = sum;
 }
 
+// The states (GRAD: r) that the chunks of a sequence start from, from their
+// maps; in place of map_h.  A warp per consecutive part of the chunks joins its
+// maps, the parts' maps give each its first state.
+template <bool GRAD>
+__global__ void k_scan_join(const ScanArgs A) {
+    __shared__ float sa[32][32], sh[32][32];
+    const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, groups = blockDim.x >> 5;
+    const int c = (int)blockIdx.x * 32 + lane;
+    for (long long s = blockIdx.y; s < A.n_seq; s += gridDim.y) {
+        const Span sp = span_of(A, s);
+        const int n = max(1, (sp.len + A.chunk - 1) / A.chunk);
+        const long long j0 = chunk0_of(A, s);
+        // position p of the chain: chunk j0 + p, or from the last one back
+        auto at = [&](int p) { return (j0 + (GRAD ? n - 1 - p : p)) * A.D + c; };
+        const int per = (n + groups - 1) / groups, lo = min(n, g * per), hi = min(n, lo + per);
+        float a = 1.0f, h = 0.0f;
+        if (c < A.D)
+#pragma unroll 8
+            for (int p = lo; p < min(hi, n - 1); ++p) {
+                const float ma = A.map_a[at(p)];
+                h = fmaf(ma, h, A.map_h[at(p)]);
+                a *= ma;
+            }
+        sa[g][lane] = a;
+        sh[g][lane] = h;
+        __syncthreads();
+        if (c < A.D) {
+            h = !GRAD && A.h0 ? A.h0[s * A.D + c] : 0.0f;
+            for (int k = 0; k < g; ++k) h = fmaf(sa[k][lane], h, sh[k][lane]);
+#pragma unroll 8
+            for (int p = lo; p < hi; ++p) {
+                const bool map = p < n - 1;
+                const float ma = map ? A.map_a[at(p)] : 0.0f, mh = map ? A.map_h[at(p)] : 0.0f;
+                A.map_h[at(p)] = h;
+                h = fmaf(ma, h, mh);
+            }
+        }
+        __syncthreads();
+    }
+}
+
 void check_desc(const snn_scan* d) {
     SNN_REQUIRE(d, SNN_ERR_ARG, "null scan description");
     SNN_REQUIRE(snnb::elem_type_ok(d->type), SNN_ERR_ARG, "scan: type must be SNN_F32, SNN_BF16 or SNN_F16");
@@ -136,28 +177,84 @@ int gate_mode(const snn_scan* d) {
 constexpr int SMS = 148;
 int64_t mean_steps(const snn_scan* d) { return d->offsets ? d->n_steps / std::max<int64_t>(d->n_seq, 1) : d->n_steps; }
 
-// Grid of the tile kernels.  The sizes alone decide (the sums of a channel
-// gate's gradient follow the grid): a cluster per (tile of channels, worker), a
-// worker for each sequence up to 32 CTAs an SM, the rest taken in turn; where
-// that leaves SMs empty, a cluster of up to MAX_CLUSTER CTAs along the steps.
-// Packed sequences may differ in length and end at different times: four times
-// the CTAs, so that the longest is split too (24 sequences of 40,003 rows by
-// 1,001 channels: forward 117 -> 94 us, gradient 249 -> 169 us).
-Plan plan_of(const snn_scan* d, int tile) {
-    const int width = 128 / snnb::elem_size(d->type);
+// Grid of the kernels.  The sizes alone decide (the sums of a channel gate's
+// gradient follow the grid).  A cluster per (tile of channels, worker), a worker
+// for each sequence up to 32 CTAs an SM, the rest taken in turn; where that
+// leaves SMs empty, a cluster of up to MAX_CLUSTER CTAs along the steps.  Packed
+// sequences may differ in length and end at different times: four times the
+// CTAs, so that the longest is split too (24 sequences of 40,003 rows by 1,001
+// channels: forward 117 -> 94 us, gradient 249 -> 169 us).
+// Where even clusters leave most SMs empty for long, the sequences are cut into
+// chunks: a first kernel reads them for their maps, a second joins the maps,
+// and the chunks run as sequences of their own.  That reads the inputs twice and
+// costs 22 us (gradient 28) however little there is, so it takes long
+// sequences of few (tile, sequence) items, by clusters / by chunks in us:
+//   1 x 50,000 x 64 f32 (2 items)           forward 102 / 32   gradient 214 / 39
+//   39 packed, 1,997,736 rows x 33 (39)               692 / 307          1406 / 588
+//   1 x 50,021 x 1,000 f32 (32)                       163 / 197           292 / 236
+//   2 packed, 20,106 x 59 f32 (4)                      34 / 32             65 / 42
+//   3 packed, 30,000 x 2,000 bf16 (96)                132 / 150           243 / 277
+//   1 x 2,000 x 512 bf16 (8)                           12 / 26             18 / 32
+Plan plan_of(const snn_scan* d, bool grad) {
+    const int width = 128 / snnb::elem_size(d->type), tile = grad ? Bwd::TT : Fwd::TT;
     Plan p;
     p.ctiles = (int)((d->n_channels + width - 1) / width);
     p.workers = (int)std::min<int64_t>(d->n_seq, std::max(32, 32 * SMS / p.ctiles));
-    const int64_t items = (int64_t)p.ctiles * p.workers, wanted = (d->offsets ? 8 : 2) * SMS;
     p.cluster = 1;
-    while (p.cluster < MAX_CLUSTER && items * p.cluster < wanted && (int64_t)tile * p.cluster < mean_steps(d))
+    p.chunk = 0;
+    p.n_chunks = 0;
+    const int64_t rows = d->offsets ? d->n_steps : d->n_seq * d->n_steps, items = (int64_t)p.ctiles * d->n_seq;
+    if (mean_steps(d) >= (grad ? 6144 : 12288) && items <= (d->offsets ? 48 : grad ? 36 : 16)) {
+        const int64_t warps = SMS * (grad ? 8 : 12) * (d->flags & SNN_SCAN_CHANNEL ? 2 : 1);
+        const int64_t c = (rows * p.ctiles + warps - 1) / warps;
+        p.chunk = (int)std::max<int64_t>(128, (c + 15) / 16 * 16);
+        p.n_chunks = rows / p.chunk + d->n_seq;
+        p.workers = (int)std::min<int64_t>(p.n_chunks, std::max(32, 32 * SMS / p.ctiles));
+        p.shape = 2;
+        return p;
+    }
+    const int64_t wanted = (d->offsets ? 8 : 2) * SMS, ctas = (int64_t)p.ctiles * p.workers;
+    while (p.cluster < MAX_CLUSTER && ctas * p.cluster < wanted && (int64_t)tile * p.cluster < mean_steps(d))
         p.cluster *= 2;
     // Without clusters: 16 x 4,096 x 2,048 in bf16 (512 items) gradient 332 us by
     // tiles, 299 by the smaller ones, 375 by single warps (forward 158 / - / 178);
     // a raster of 1,000 x 55,000 (1,719 items) forward 69 / - / 49, gradient 134 /
     // - / 79.
-    p.shape = p.cluster > 1 || items < 3 * SMS ? 0 : items < 8 * SMS ? 1 : 2;
+    p.shape = p.cluster > 1 || ctas < 3 * SMS ? 0 : ctas < 8 * SMS ? 1 : 2;
     return p;
+}
+// workspace: the maps of the chunks, then a channel gate's sums
+int64_t map_floats(const snn_scan* d, const Plan& p) { return (p.n_chunks * d->n_channels + 63) / 64 * 64; }
+int64_t work_bytes_of(const snn_scan* d, const Plan& p, bool grad) {
+    const int64_t sums = grad && (d->flags & SNN_SCAN_CHANNEL) ? (int64_t)p.workers * p.cluster * d->n_channels : 0;
+    return (2 * map_floats(d, p) + sums) * 4;
+}
+void check_work(const void* work, int64_t bytes, int64_t needed) {
+    SNN_REQUIRE(needed == 0 || (work && (uintptr_t)work % 256 == 0 && bytes >= needed), SNN_ERR_ARG,
+                "scan: workspace null, misaligned or too small");
+}
+
+// the kernels of a plan
+template <bool GRAD>
+void run_plan(const snn_scan* d, int words, const Plan& p, void* work, ScanArgs& A, cudaStream_t st) {
+    A.chunk = p.chunk;
+    A.n_chunks = p.n_chunks;
+    A.map_a = (float*)work;
+    A.map_h = (float*)work + map_floats(d, p);
+    const int gm = gate_mode(d);
+    const bool raster = (d->flags & SNN_SCAN_RASTER) != 0;
+    snnb::with_elem(d->type, [&](auto t) {
+        using T = decltype(t);
+        if (p.chunk) {
+            launch_tiles<GRAD, T>(gm, raster, words, true, p, A, st);
+            const int64_t mean = p.n_chunks / d->n_seq;
+            int groups = 1;
+            while (groups < 32 && groups * 4 < mean) groups *= 2;
+            k_scan_join<GRAD><<<dim3((unsigned)((d->n_channels + 31) / 32), (unsigned)std::min<int64_t>(d->n_seq, 65535)),
+                                32 * groups, 0, st>>>(A);
+        }
+        launch_tiles<GRAD, T>(gm, raster, words, false, p, A, st);
+    });
 }
 
 // whether r's rows are words of `bytes` from the first element on
@@ -185,15 +282,13 @@ int64_t leaky_scan_saved(const snn_scan* d) {
     return saved_floats(d);
 }
 
-int64_t leaky_scan_grad_workspace(const snn_scan* d) {
+int64_t leaky_scan_workspace(const snn_scan* d, bool grad) {
     check_desc(d);
-    if (!(d->flags & SNN_SCAN_CHANNEL)) return 0;
-    const Plan p = plan_of(d, Bwd::TT);
-    return (int64_t)p.workers * p.cluster * d->n_channels * 4;
+    return d->n_seq ? work_bytes_of(d, plan_of(d, grad), grad) : 0;
 }
 
 void leaky_scan(const snn_scan* d, const snn_rows* gate, const snn_rows* x, const float* h0,
-                const snn_rows* y, float* h, float* saved, cudaStream_t st) {
+                const snn_rows* y, float* h, float* saved, void* work, int64_t work_bytes, cudaStream_t st) {
     check_desc(d);
     if (d->n_seq == 0) return;
     ScanArgs A = base_args(d, gate, x);
@@ -229,8 +324,9 @@ void leaky_scan(const snn_scan* d, const snn_rows* gate, const snn_rows* x, cons
         SNN_CUDA(cudaGetLastError());
         return;
     }
-    const Plan p = plan_of(d, Fwd::TT);
-    with_elem(d->type, [&](auto t) { launch_tiles<false, decltype(t)>(gate_mode(d), raster_x, words, p, A, st); });
+    const Plan p = plan_of(d, false);
+    check_work(work, work_bytes, work_bytes_of(d, p, false));
+    run_plan<false>(d, words, p, work, A, st);
 }
 
 void leaky_scan_grad(const snn_scan* d, const snn_rows* gate, const snn_rows* x, const float* saved,
@@ -256,20 +352,17 @@ void leaky_scan_grad(const snn_scan* d, const snn_rows* gate, const snn_rows* x,
     if (dx) A.dx = rows_of(d, dx, "dx", d->n_channels, size, true);
     if (dgate && channel) {
         SNN_REQUIRE(dgate->data && (uintptr_t)dgate->data % 4 == 0, SNN_ERR_ARG, "scan: null or misaligned dgate");
-        SNN_REQUIRE(work && (uintptr_t)work % 256 == 0 && work_bytes >= leaky_scan_grad_workspace(d), SNN_ERR_ARG,
-                    "scan: workspace null, misaligned or too small");
         A.dgate = {dgate->data, 0, 0};
-        A.part = (float*)work;
     } else if (dgate) {
         A.dgate = rows_of(d, dgate, "dgate", d->n_channels, size, true);
     }
     const Rows none = {nullptr, 0, 0};
     const int words = copy_words(d, {channel ? none : A.gate, d->flags & SNN_SCAN_RASTER ? none : A.x, A.y},
                                  {channel ? none : A.dgate, A.dx});
-    const Plan p = plan_of(d, Bwd::TT);
-    with_elem(d->type, [&](auto t) {
-        launch_tiles<true, decltype(t)>(gate_mode(d), (d->flags & SNN_SCAN_RASTER) != 0, words, p, A, st);
-    });
+    const Plan p = plan_of(d, true);
+    check_work(work, work_bytes, work_bytes_of(d, p, true));
+    if (channel && dgate) A.part = (float*)work + 2 * map_floats(d, p);
+    run_plan<true>(d, words, p, work, A, st);
     if (A.part) {
         k_scan_gate_sum<<<(unsigned)((d->n_channels + 31) / 32), 256, 0, st>>>(A, p.workers * p.cluster);
         SNN_CUDA(cudaGetLastError());

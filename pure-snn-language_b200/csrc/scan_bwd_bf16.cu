@@ -2,4 +2,4 @@
 #define SNN_SCAN_TILE_LAUNCH
 #include "scan_tile.h"
 
-template void snnb_scan::launch_tiles<true, __nv_bfloat16>(int, bool, int, const Plan&, ScanArgs&, cudaStream_t);
+template void snnb_scan::launch_tiles<true, __nv_bfloat16>(int, bool, int, bool, const Plan&, ScanArgs&, cudaStream_t);

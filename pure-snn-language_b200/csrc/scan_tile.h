@@ -37,6 +37,11 @@ struct ScanArgs {
     float* dh0;
     float* part;   // per-CTA sums of a channel gate's gradient
     int ctiles, workers, cluster;
+    // sequences cut into chunks of `chunk` steps (0: whole): the chunks' maps,
+    // then in map_h the states (gradient: r) that they start from
+    int chunk;
+    long long n_chunks;
+    float *map_a, *map_h;
 };
 
 // rows of sequence s: [begin, begin + len) of the flat row index (packed), or
@@ -62,6 +67,31 @@ __device__ __forceinline__ Span span_of(const ScanArgs& A, long long s) {
     // leaves room for ceil(len / BLOCK) blocks in every sequence, whatever the lengths
     r.block0 = flat / BLOCK + s;
     return r;
+}
+// Chunk j of the launch: steps [from, to) of sequence s.  Sequence s has the
+// chunks from floor(flat / chunk) + s on, as with the blocks; the others hold
+// nothing (from = to = 1).  An empty sequence has one chunk (from = to = 0).
+__device__ __forceinline__ long long chunk0_of(const ScanArgs& A, long long s) {
+    const long long flat = A.off ? min(max((long long)A.off[s], 0ll), (long long)A.n_steps) : s * A.n_steps;
+    return flat / A.chunk + s;
+}
+__device__ __forceinline__ Span chunk_at(const ScanArgs& A, long long j, long long& s, int& from, int& to) {
+    long long lo = 0, hi = A.n_seq;
+    while (hi - lo > 1) {
+        const long long mid = (lo + hi) >> 1;
+        if (chunk0_of(A, mid) <= j) lo = mid;
+        else hi = mid;
+    }
+    s = lo;
+    const Span sp = span_of(A, s);
+    const long long at = (j - chunk0_of(A, s)) * A.chunk;
+    if (at < 0 || (at > 0 && at >= sp.len)) {
+        from = to = 1;  // nothing
+    } else {
+        from = (int)at;
+        to = (int)min(at + A.chunk, (long long)sp.len);
+    }
+    return sp;
 }
 __device__ __forceinline__ long long row_at(const ScanArgs& A, const Rows& r, long long s, const Span& sp, long long t) {
     return A.off ? (sp.begin + t) * r.st : s * r.ss + t * r.st;
@@ -310,6 +340,8 @@ using BwdMany = Shape<4, 8, 3, 4>;
 // which has its state at hand and needs no maps.
 using FwdSeq = Shape<1, 16, 4, 12>;
 using BwdSeq = Shape<1, 16, 3, 8>;
+using FwdSeqChannel = Shape<1, 16, 4, 24>;
+using BwdSeqChannel = Shape<1, 16, 3, 16>;
 constexpr int MAX_CLUSTER = 8;
 static_assert(Bwd::TT % BLOCK == 0 && BwdMany::TT % BLOCK == 0 && BwdSeq::TT % BLOCK == 0 && FwdSeq::L % BLOCK == 0 && Fwd::L % BLOCK == 0,
               "a gradient tile and a warp's forward steps begin with a saved state");
@@ -483,8 +515,6 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
     using St = Stage<GM, RASTER, COPY, L, V, false>;
     static_assert(L * V <= 32, "a lane holds one raster word");
     extern __shared__ __align__(16) char rows[];
-    __shared__ Vec<V> sa[2][W][32], sh[2][W][32];
-    __shared__ ClusterMaps<V> cm;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int CL = A.cluster, rank = blockIdx.x % CL, item = blockIdx.x / CL;
     const int c0 = item % A.ctiles * 32 * V, c = c0 + lane * V;
@@ -496,14 +526,23 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
     Vec<V> factor = splat<V>(1.0f);
     if (PC) channel_decays<T, GM, V>(A, c, nl, fixed, factor);
     int par = 0;
-    for (long long s = item / A.ctiles; s < A.n_seq; s += A.workers) {
-        const Span sp = span_of(A, s);
-        Vec<V> carry = load_n<V>(A.h0 + s * A.D + c, A.h0 ? nl : 0);
-        if (sp.len == 0) {
-            if (A.h && rank == 0 && w == 0) store_n<V>(A.h + s * A.D + c, carry, nl);
+    const bool split = W == 1 && A.chunk > 0;
+    for (long long j = item / A.ctiles; j < (split ? A.n_chunks : A.n_seq); j += A.workers) {
+        long long s = j;
+        int from_t = 0, to_t;
+        Span sp;
+        if (split) {
+            sp = chunk_at(A, j, s, from_t, to_t);
+        } else {
+            sp = span_of(A, s);
+            to_t = sp.len;
+        }
+        Vec<V> carry = split ? load_n<V>(A.map_h + j * A.D + c, nl) : load_n<V>(A.h0 + s * A.D + c, A.h0 ? nl : 0);
+        if (to_t == from_t) {
+            if (A.h && to_t == 0 && rank == 0 && w == 0) store_n<V>(A.h + s * A.D + c, carry, nl);
             continue;
         }
-        const int t1 = rank * TT + w * L;  // the warp's first step
+        const int t1 = from_t + rank * TT + w * L;  // the warp's first step
         Rower<T, COPY, L> rg, rx;
         rg.start(reinterpret_cast<const T*>(A.gate.p) + row_at(A, A.gate, s, sp, t1) + c0, A.gate.st, round);
         rx.start(reinterpret_cast<const T*>(A.x.p) + row_at(A, A.x, s, sp, t1) + c0, A.x.st, round);
@@ -512,7 +551,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
         const long long yjump = A.y.st * round;
         const unsigned g0 = rg.shift(rg.p, 0), g1 = rg.shift(rg.p, 1), x0 = rx.shift(rx.p, 0), x1 = rx.shift(rx.p, 1);
         auto fetch = [&](int t, int slot) {  // this warp's steps from t on
-            const int n = min(L, sp.len - t);
+            const int n = min(L, to_t - t);
             const unsigned dst = mine_s + slot * St::bytes;
             if (n > 0) {
                 if (!PC) rg.fetch(dst + St::gate, n, nc, lane);
@@ -527,7 +566,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
 #pragma unroll
         for (int k = 0; k < S; ++k) fetch(t1 + k * round, k);
         int slot = 0;
-        for (int t0 = t1; t0 - t1 < sp.len; t0 += round) {
+        for (int t0 = t1; t0 - t1 < to_t - from_t; t0 += round) {
             Decay<V, LO> d[PC ? 1 : L];
             Vec<V> u[L];
             copy_wait<S - 1>();
@@ -548,6 +587,8 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
             slot = slot + 1 == S ? 0 : slot + 1;
             Vec<V> h = carry;
             if constexpr (W > 1) {
+                __shared__ Vec<V> sa[2][W][32], sh[2][W][32];
+                __shared__ ClusterMaps<V> cm;
                 Vec<V> a = splat<V>(1.0f);
                 h = splat<V>(0.0f);
 #pragma unroll
@@ -588,7 +629,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
                 }
                 par ^= 1;
             }
-            const int n = min(L, sp.len - t0);
+            const int n = min(L, to_t - t0);
             if (nl > 0 && n > 0) {
                 if (A.saved) store_n<V>(A.saved + (sp.block0 + t0 / BLOCK) * A.D + c, h, nl);
                 T* qy = py;
@@ -619,8 +660,6 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
     constexpr bool LO = keeps_lo<T, GM>, PC = per_channel<GM>;
     using St = Stage<GM, RASTER, COPY, L, V, true>;
     extern __shared__ __align__(16) char rows[];
-    __shared__ Vec<V> sa[2][W][32], sh[2][W][32], sr[2][W][32];
-    __shared__ ClusterMaps<V> cm;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int CL = A.cluster, rank = blockIdx.x % CL, item = blockIdx.x / CL;
     const int c0 = item % A.ctiles * 32 * V, c = c0 + lane * V;
@@ -633,16 +672,26 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
     Vec<V> factor = one, sum = splat<V>(0.0f);
     if (PC) channel_decays<T, GM, V>(A, c, nl, fixed, factor);
     int par = 0;
-    for (long long s = item / A.ctiles; s < A.n_seq; s += A.workers) {
-        const Span sp = span_of(A, s);
-        Vec<V> carry = splat<V>(0.0f);
-        if (sp.len == 0) {
-            if (A.dh0 && rank == 0 && w == 0)
+    const bool split = W == 1 && A.chunk > 0;
+    for (long long j = item / A.ctiles; j < (split ? A.n_chunks : A.n_seq); j += A.workers) {
+        long long s = j;
+        int from_t = 0, to_t;
+        Span sp;
+        if (split) {
+            sp = chunk_at(A, j, s, from_t, to_t);
+        } else {
+            sp = span_of(A, s);
+            to_t = sp.len;
+        }
+        Vec<V> carry = load_n<V>(A.map_h + j * A.D + c, split ? nl : 0);
+        if (to_t == from_t) {
+            if (A.dh0 && to_t == 0 && rank == 0 && w == 0)
                 store_n<V>(A.dh0 + s * A.D + c, load_n<V>(A.dh + s * A.D + c, A.dh ? nl : 0), nl);
             continue;
         }
-        const int tiles = (sp.len + TT - 1) / TT;
-        const int t1 = (tiles - 1 - rank) * TT + w * L;  // the warp's first (latest) steps; may be negative
+        const int tiles = (to_t - from_t + TT - 1) / TT;
+        // the warp's first (latest) steps; before from_t where the CTA has no tile
+        const int t1 = from_t + (tiles - 1 - rank) * TT + w * L;
         Rower<T, COPY, L> rg, rx, rd;
         rg.start(reinterpret_cast<const T*>(A.gate.p) + row_at(A, A.gate, s, sp, t1) + c0, A.gate.st, -round);
         rx.start(reinterpret_cast<const T*>(A.x.p) + row_at(A, A.x, s, sp, t1) + c0, A.x.st, -round);
@@ -654,15 +703,15 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
         const unsigned g0 = rg.shift(rg.p, 0), g1 = rg.shift(rg.p, 1), x0 = rx.shift(rx.p, 0), x1 = rx.shift(rx.p, 1);
         const unsigned d0 = rd.shift(rd.p, 0), d1 = rd.shift(rd.p, 1);
         auto fetch = [&](int t, int slot) {
-            if (t >= 0 && t < sp.len) {
-                const int n = min(L, sp.len - t);
+            if (t >= from_t && t < to_t) {
+                const int n = min(L, to_t - t);
                 const unsigned dst = mine_s + slot * St::bytes;
                 if (!PC) rg.fetch(dst + St::gate, n, nc, lane);
                 if (RASTER) fetch_raster<V, L>(dst + St::x, pw, A.x.st, n, (nc + 31) >> 5, lane);
                 else rx.fetch(dst + St::x, n, nc, lane);
                 if (A.y.p) rd.fetch(dst + St::dy, n, nc, lane);
             }
-            if (t >= 0) {  // the tile's first state, where t lies behind the end too
+            if (t >= from_t) {  // the tile's first state, where t lies behind the end too
                 const float* q = A.saved + (sp.block0 + (t - w * L) / BLOCK) * A.D + c;
 #pragma unroll
                 for (int k = 0; k < V; ++k)
@@ -678,8 +727,8 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
 #pragma unroll
         for (int k = 0; k < S; ++k) fetch(t1 - k * round, k);
         int slot = 0, t0 = t1;
-        for (int b = 0; b < tiles; b += CL, t0 -= round) {  // t0 negative: no tile left for this CTA
-            const bool some = t0 >= 0 && t0 < sp.len;
+        for (int b = 0; b < tiles; b += CL, t0 -= round) {  // t0 before from_t: no tile left for this CTA
+            const bool some = t0 >= from_t && t0 < to_t;
             Decay<V, LO> d[PC ? 1 : L];
             Vec<V> rest[PC ? 1 : L], x[L], o[L];
             copy_wait<S - 1>();
@@ -707,6 +756,8 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
             slot = slot + 1 == S ? 0 : slot + 1;
             Vec<V> h = h0, r = carry;
             if constexpr (W > 1) {
+                __shared__ Vec<V> sa[2][W][32], sh[2][W][32], sr[2][W][32];
+                __shared__ ClusterMaps<V> cm;
                 Vec<V> a = one;
                 h = r = splat<V>(0.0f);
 #pragma unroll
@@ -767,7 +818,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
                     h = d[PC ? 0 : i].step(h, LEAKY ? vmul(PC ? factor : rest[PC ? 0 : i], xi) : xi);
                     x[i] = LEAKY ? vfma(minus, xi, before) : before;
                 }
-                const int n = min(L, sp.len - t0);
+                const int n = min(L, to_t - t0);
                 T *qg = pdg, *qx = pdx;
 #pragma unroll
                 for (int i = L - 1; i >= 0; --i) {
@@ -797,25 +848,127 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
         __syncwarp();
     }
     if (PC && A.part) {
-        __syncthreads();
-        sa[0][w][lane] = sum;
-        __syncthreads();
-        if (w == 0 && nl > 0) {
-            Vec<V> t = splat<V>(0.0f);
-            for (int j = 0; j < W; ++j) t = vadd(t, sa[0][j][lane]);
-            store_n<V>(A.part + ((long long)(item / A.ctiles) * CL + rank) * A.D + c, t, nl);
+        Vec<V> t = sum;
+        if constexpr (W > 1) {
+            __shared__ Vec<V> sums[W][32];
+            sums[w][lane] = sum;
+            __syncthreads();
+            t = splat<V>(0.0f);
+            for (int k = 0; k < W; ++k) t = vadd(t, sums[k][lane]);
         }
+        if (w == 0) store_n<V>(A.part + ((long long)(item / A.ctiles) * CL + rank) * A.D + c, t, nl);
+    }
+}
+
+// The map of a chunk of steps, a warp for each (chunk, tile of channels): the
+// decays' product and the end state from zero (GRAD: r at its first step).
+// The last chunk of a sequence (GRAD: the first) needs none.
+template <typename SH, typename T, int GM, bool RASTER, bool LEAKY, int COPY, bool GRAD>
+__global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_map(const ScanArgs A) {
+    constexpr int L = SH::L, S = SH::S, V = lane_channels<T>;
+    constexpr bool LO = keeps_lo<T, GM>, PC = per_channel<GM>;
+    using St = Stage<GM, RASTER, COPY, L, V, false>;  // its x is dy for the gradient
+    static_assert(SH::W == 1, "a warp by itself");
+    extern __shared__ __align__(16) char rows[];
+    const int lane = threadIdx.x;
+    const int item = blockIdx.x;
+    const int c0 = item % A.ctiles * 32 * V, c = c0 + lane * V;
+    const int nc = min(32 * V, A.D - c0), nl = min(V, A.D - c);
+    const unsigned rows_s = (unsigned)__cvta_generic_to_shared(rows);
+    for (long long j = item / A.ctiles; j < A.n_chunks; j += A.workers) {
+        long long s;
+        int from_t, to_t;
+        const Span sp = chunk_at(A, j, s, from_t, to_t);
+        if (from_t == to_t || (GRAD ? from_t == 0 : to_t == sp.len)) continue;
+        const int tiles = (to_t - from_t + L - 1) / L;
+        const int step = GRAD ? -L : L, t1 = GRAD ? from_t + (tiles - 1) * L : from_t;
+        const Rows& in = GRAD ? A.y : A.x;
+        Rower<T, COPY, L> rg, rx;
+        rg.start(reinterpret_cast<const T*>(A.gate.p) + row_at(A, A.gate, s, sp, t1) + c0, A.gate.st, step);
+        rx.start(reinterpret_cast<const T*>(in.p) + row_at(A, in, s, sp, t1) + c0, in.st, step);
+        const unsigned* pw = reinterpret_cast<const unsigned*>(A.x.p) + row_at(A, A.x, s, sp, t1) + (c0 >> 5);
+        const unsigned g0 = rg.shift(rg.p, 0), g1 = rg.shift(rg.p, 1), x0 = rx.shift(rx.p, 0), x1 = rx.shift(rx.p, 1);
+        auto fetch = [&](int t, int slot) {
+            const int n = min(L, to_t - t);
+            const unsigned dst = rows_s + slot * St::bytes;
+            if (t >= from_t && n > 0) {
+                if (!PC) rg.fetch(dst + St::gate, n, nc, lane);
+                if (RASTER) fetch_raster<V, L>(dst + St::x, pw, A.x.st, n, (nc + 31) >> 5, lane);
+                else if (in.p) rx.fetch(dst + St::x, n, nc, lane);
+            }
+            rg.p += rg.jump;
+            rx.p += rx.jump;
+            pw += A.x.st * step;
+            copy_commit();
+        };
+#pragma unroll
+        for (int k = 0; k < S; ++k) fetch(t1 + k * step, k);
+        Decay<V, LO> fixed;
+        Vec<V> factor = splat<V>(1.0f);
+        if (PC) channel_decays<T, GM, V>(A, c, nl, fixed, factor);
+        Vec<V> a = splat<V>(1.0f), h = splat<V>(0.0f);
+        int slot = 0, t0 = t1;
+        for (int b = 0; b < tiles; ++b, t0 += step) {
+            Decay<V, LO> d[PC ? 1 : L];
+            Vec<V> u[L];
+            copy_wait<S - 1>();
+            __syncwarp();
+            const char* from = rows + slot * St::bytes;
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                Vec<V> f = factor;
+                if (!PC)
+                    decays<T, GM, V>(Unpack<T>::get(staged<COPY>(from + St::gate, i, lane, i & 1 ? g1 : g0)), d[i], f);
+                if constexpr (RASTER) u[i] = raster_values<V>(from + St::x, i, lane);
+                else u[i] = Unpack<T>::get(staged<COPY>(from + St::x, i, lane, i & 1 ? x1 : x0));
+                if (!in.p) u[i] = splat<V>(0.0f);
+                if (LEAKY && !GRAD) u[i] = vmul(f, u[i]);
+            }
+            if (PC) d[0] = fixed;
+            __syncwarp();
+            fetch(t0 + S * step, slot);
+            slot = slot + 1 == S ? 0 : slot + 1;
+            const int n = min(L, to_t - t0);
+            if (GRAD) {
+                if (A.dh && t0 + n == sp.len) {
+                    const Vec<V> dh = load_n<V>(A.dh + s * A.D + c, nl);
+#pragma unroll
+                    for (int i = 0; i < L; ++i)
+                        if (i == n - 1) u[i] = vadd(u[i], dh);
+                }
+#pragma unroll
+                for (int i = L - 1; i >= 0; --i)
+                    if (i < n) {
+                        h = d[PC ? 0 : i].times(vadd(u[i], h));
+                        a = d[PC ? 0 : i].times(a);
+                    }
+            } else {
+#pragma unroll
+                for (int i = 0; i < L; ++i)
+                    if (i < n) {
+                        h = d[PC ? 0 : i].step(h, u[i]);
+                        a = d[PC ? 0 : i].times(a);
+                    }
+            }
+        }
+        copy_wait<0>();
+        __syncwarp();
+        store_n<V>(A.map_a + j * A.D + c, a, nl);
+        store_n<V>(A.map_h + j * A.D + c, h, nl);
     }
 }
 
 struct Plan {
     int ctiles, workers, cluster;
     int shape;  // 0 tiles, 1 smaller tiles (gradient), 2 a warp by itself
+    int chunk;  // 2: the sequences are cut into chunks of so many steps (0: not)
+    int64_t n_chunks;
 };
 
-// the forward (GRAD = false) or gradient kernel of element type T
+// the forward (GRAD = false) or gradient kernel of element type T; map: that of
+// the chunks' maps
 template <bool GRAD, typename T>
-void launch_tiles(int gate_mode, bool raster, int words, const Plan& p, ScanArgs& A, cudaStream_t st);
+void launch_tiles(int gate_mode, bool raster, int words, bool map, const Plan& p, ScanArgs& A, cudaStream_t st);
 
 #ifdef SNN_SCAN_TILE_LAUNCH
 inline void launch(const void* kernel, std::atomic<uint64_t>& ready, int threads, int smem, const Plan& p, ScanArgs& A,
@@ -863,8 +1016,26 @@ void launch_shape(const Plan& p, ScanArgs& A, cudaStream_t st) {
     launch(k, ready[A.leaky ? 1 : 0], SH::threads, smem, p, A, st);
 }
 template <bool GRAD, typename T, int GM, bool RASTER, int COPY>
-void launch_copy(const Plan& p, ScanArgs& A, cudaStream_t st) {
-    if (p.shape == 2) return launch_shape<GRAD, std::conditional_t<GRAD, BwdSeq, FwdSeq>, T, GM, RASTER, COPY>(p, A, st);
+void launch_map(const Plan& p, ScanArgs& A, cudaStream_t st) {
+    // the gradient's maps read the gate and dy alone
+    constexpr bool RA = RASTER && !GRAD;
+    using SH = std::conditional_t<per_channel<GM>, FwdSeqChannel, FwdSeq>;
+    const int smem = SH::S * Stage<GM, RA, COPY, SH::L, lane_channels<T>, false>::bytes;
+    const bool leaky = A.leaky && !GRAD;
+    const void* k;
+    if constexpr (GRAD) k = (const void*)k_scan_map<SH, T, GM, false, false, COPY, true>;
+    else
+        k = leaky ? (const void*)k_scan_map<SH, T, GM, RASTER, true, COPY, false>
+                  : (const void*)k_scan_map<SH, T, GM, RASTER, false, COPY, false>;
+    static std::atomic<uint64_t> ready[2];
+    launch(k, ready[leaky ? 1 : 0], 32, smem, p, A, st);
+}
+template <bool GRAD, typename T, int GM, bool RASTER, int COPY>
+void launch_copy(bool map, const Plan& p, ScanArgs& A, cudaStream_t st) {
+    if (map) return launch_map<GRAD, T, GM, RASTER, COPY>(p, A, st);
+    using Seq = std::conditional_t<GRAD, std::conditional_t<per_channel<GM>, BwdSeqChannel, BwdSeq>,
+                                   std::conditional_t<per_channel<GM>, FwdSeqChannel, FwdSeq>>;
+    if (p.shape == 2) return launch_shape<GRAD, Seq, T, GM, RASTER, COPY>(p, A, st);
     if constexpr (GRAD) {
         if (p.shape == 1) return launch_shape<true, BwdMany, T, GM, RASTER, COPY>(p, A, st);
         launch_shape<true, Bwd, T, GM, RASTER, COPY>(p, A, st);
@@ -873,20 +1044,20 @@ void launch_copy(const Plan& p, ScanArgs& A, cudaStream_t st) {
     }
 }
 template <bool GRAD, typename T, int GM>
-void launch_gate(bool raster, int words, const Plan& p, ScanArgs& A, cudaStream_t st) {
+void launch_gate(bool raster, int words, bool map, const Plan& p, ScanArgs& A, cudaStream_t st) {
     if constexpr (sizeof(T) == 2)
         if (words == 2)
-            return raster ? launch_copy<GRAD, T, GM, true, 2>(p, A, st) : launch_copy<GRAD, T, GM, false, 2>(p, A, st);
-    if (raster) launch_copy<GRAD, T, GM, true, 4>(p, A, st);
-    else if (words == 16) launch_copy<GRAD, T, GM, false, 16>(p, A, st);
-    else launch_copy<GRAD, T, GM, false, 4>(p, A, st);
+            return raster ? launch_copy<GRAD, T, GM, true, 2>(map, p, A, st) : launch_copy<GRAD, T, GM, false, 2>(map, p, A, st);
+    if (raster) launch_copy<GRAD, T, GM, true, 4>(map, p, A, st);
+    else if (words == 16) launch_copy<GRAD, T, GM, false, 16>(map, p, A, st);
+    else launch_copy<GRAD, T, GM, false, 4>(map, p, A, st);
 }
 template <bool GRAD, typename T>
-void launch_tiles(int gate_mode, bool raster, int words, const Plan& p, ScanArgs& A, cudaStream_t st) {
-    if (gate_mode == GATE_VALUE) launch_gate<GRAD, T, GATE_VALUE>(raster, words, p, A, st);
-    else if (gate_mode == GATE_LOGIT) launch_gate<GRAD, T, GATE_LOGIT>(raster, words, p, A, st);
-    else if (gate_mode == GATE_CHANNEL) launch_gate<GRAD, T, GATE_CHANNEL>(raster, words, p, A, st);
-    else launch_gate<GRAD, T, GATE_CHANNEL_LOGIT>(raster, words, p, A, st);
+void launch_tiles(int gate_mode, bool raster, int words, bool map, const Plan& p, ScanArgs& A, cudaStream_t st) {
+    if (gate_mode == GATE_VALUE) launch_gate<GRAD, T, GATE_VALUE>(raster, words, map, p, A, st);
+    else if (gate_mode == GATE_LOGIT) launch_gate<GRAD, T, GATE_LOGIT>(raster, words, map, p, A, st);
+    else if (gate_mode == GATE_CHANNEL) launch_gate<GRAD, T, GATE_CHANNEL>(raster, words, map, p, A, st);
+    else launch_gate<GRAD, T, GATE_CHANNEL_LOGIT>(raster, words, map, p, A, st);
 }
 #endif
 

@@ -126,7 +126,7 @@ EXPORTS = ["snn_config_init", "snn_topology_init", "snn_create", "snn_destroy",
            "snn_set_profiling", "snn_get_profile", "snn_propagate", "snn_propagate_static",
            "snn_nccl_unique_id", "snn_set_shard", "snn_shard_plan", "snn_semantic_eval",
            "snn_set_corpus_ex", "snn_load_text_corpus", "snn_byte_classes", "snn_embed",
-           "snn_embed_grad", "snn_embed_grad_workspace", "snn_leaky_scan", "snn_leaky_scan_saved",
+           "snn_embed_grad", "snn_embed_grad_workspace", "snn_leaky_scan", "snn_leaky_scan_saved", "snn_leaky_scan_workspace",
            "snn_leaky_scan_grad", "snn_leaky_scan_grad_workspace"]
 
 _lib = None
@@ -189,7 +189,8 @@ def _load(path):
                                  i32, vp, i64, vp]
     ps = pr = C.c_char_p  # snn_scan, snn_rows: packed bytes
     L.snn_leaky_scan_saved.argtypes = [ps, vp]
-    L.snn_leaky_scan.argtypes = [ps, pr, pr, vp, pr, vp, vp, vp]
+    L.snn_leaky_scan.argtypes = [ps, pr, pr, vp, pr, vp, vp, vp, i64, vp]
+    L.snn_leaky_scan_workspace.argtypes = [ps, vp]
     L.snn_leaky_scan_grad_workspace.argtypes = [ps, vp]
     L.snn_leaky_scan_grad.argtypes = [ps, pr, pr, vp, pr, vp, pr, pr, vp, vp, i64, vp]
     L.snn_shard_plan.argtypes = [C.POINTER(TopologySpec), C.c_int32, C.c_int32, vp, C.c_int32]
@@ -445,6 +446,16 @@ def _saved_floats(desc):
     return size.value
 
 
+def _scan_work(fn, desc, dev, stream):
+    """(workspace or None, its address, its bytes)"""
+    size = C.c_int64()
+    _check(fn(desc, C.byref(size)))
+    if not size.value:
+        return None, None, 0
+    work = _new(dev, stream, (size.value,), _T.uint8)
+    return work, work.data_ptr(), size.value
+
+
 def leaky_scan(gate, x, h0=None, logit=False, leaky=False, offsets=None, dtype=None, out=None,
                h_out=None, save=False, stream=None):
     """Leaky integration along whole sequences (snn_leaky_scan):
@@ -478,8 +489,10 @@ def leaky_scan(gate, x, h0=None, logit=False, leaky=False, offsets=None, dtype=N
     if save:
         saved = _new(dev, stream, (_saved_floats(desc),), _T.float32)
         sp = saved.data_ptr()
-    _call(lib().snn_leaky_scan, dev, stream, desc, g, xr,
-          None if h0 is None else _state(h0, "h0", state, dev), yr, hp, sp)
+    L = lib()
+    work, wp, wn = _scan_work(L.snn_leaky_scan_workspace, desc, dev, stream)
+    _call(L.snn_leaky_scan, dev, stream, desc, g, xr,
+          None if h0 is None else _state(h0, "h0", state, dev), yr, hp, sp, wp, wn)
     return (out, h_out, saved) if save else (out, h_out)
 
 
@@ -500,27 +513,24 @@ def leaky_scan_grad(gate, x, dy, saved, dh=None, logit=False, leaky=False, offse
     _cuda(saved, "saved", dev)
     if saved.dtype != _T.float32 or saved.numel() != _saved_floats(desc) or not saved.is_contiguous():
         raise SnnError(1, "saved is not what the forward call of these sizes gives")
-    dyr = dgate = dgr = dx = dxr = dh0 = hp = work = wp = None
+    dyr = dgate = dgr = dx = dxr = dh0 = hp = None
     d = shape[-1]
     if dy is not None:
         _cuda(dy, "dy", dev)
         dyr = _scan_rows(dy, "dy", shape, dtype)
-    size = C.c_int64()
     if need_gate:
         dgate = _new(dev, stream, gate.shape, gate.dtype)
         dgr = _ROWS.pack(dgate.data_ptr(), shape[-2] * d, d)
-        if gate.dim() == 1:
-            _check(lib().snn_leaky_scan_grad_workspace(desc, C.byref(size)))
-            work = _new(dev, stream, (size.value,), _T.uint8)
-            wp = work.data_ptr()
     if need_x and not raster:
         dx = _new(dev, stream, shape, dtype)
         dxr = _ROWS.pack(dx.data_ptr(), shape[-2] * d, d)
     if need_h0:
         dh0 = _new(dev, stream, state, _T.float32)
         hp = dh0.data_ptr()
-    _call(lib().snn_leaky_scan_grad, dev, stream, desc, g, xr, saved.data_ptr(), dyr,
-          None if dh is None else _state(dh, "dh", state, dev), dgr, dxr, hp, wp, size.value)
+    L = lib()
+    work, wp, wn = _scan_work(L.snn_leaky_scan_grad_workspace, desc, dev, stream)
+    _call(L.snn_leaky_scan_grad, dev, stream, desc, g, xr, saved.data_ptr(), dyr,
+          None if dh is None else _state(dh, "dh", state, dev), dgr, dxr, hp, wp, wn)
     return dgate, dx, dh0
 
 
