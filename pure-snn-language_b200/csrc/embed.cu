@@ -8,11 +8,59 @@ constexpr int SMS = 148;  // multiprocessors of a B200
 using snnb::from_f32;
 using snnb::to_f32;
 
-// V elements that are loaded and stored as one word of at most 16 bytes
+// V elements that are stored as one word of at most 16 bytes
 template <typename T, int V>
 struct alignas(sizeof(T) * V > 16 ? 16 : sizeof(T) * V) Pack {
     T v[V];
 };
+// N bytes in registers, as one load (32: two) brings them; unpacked where they
+// are used, so that loads stay in flight
+struct Raw32 {
+    uint4 lo, hi;
+};
+template <int N> struct Raw;
+template <> struct Raw<2> { using type = unsigned short; };
+template <> struct Raw<4> { using type = unsigned; };
+template <> struct Raw<8> { using type = uint2; };
+template <> struct Raw<16> { using type = uint4; };
+template <> struct Raw<32> { using type = Raw32; };
+
+__device__ __forceinline__ void unpack(float* o, unsigned w, float) { o[0] = __uint_as_float(w); }
+__device__ __forceinline__ void unpack(float* o, unsigned w, __nv_bfloat16) {
+    o[0] = __uint_as_float(w << 16);
+    o[1] = __uint_as_float(w & 0xffff0000u);
+}
+__device__ __forceinline__ void unpack(float* o, unsigned w, __half) {
+    __half2 p;
+    memcpy(&p, &w, 4);
+    const float2 f = __half22float2(p);
+    o[0] = f.x;
+    o[1] = f.y;
+}
+__device__ __forceinline__ void unpack(float* o, unsigned short w, __nv_bfloat16) {
+    o[0] = __uint_as_float((unsigned)w << 16);
+}
+__device__ __forceinline__ void unpack(float* o, unsigned short w, __half) { o[0] = __half2float(__ushort_as_half(w)); }
+template <typename T>
+__device__ __forceinline__ void unpack(float* o, const uint2& w, T t) {
+    constexpr int E = 4 / (int)sizeof(T);
+    unpack(o, w.x, t);
+    unpack(o + E, w.y, t);
+}
+template <typename T>
+__device__ __forceinline__ void unpack(float* o, const uint4& w, T t) {
+    constexpr int E = 4 / (int)sizeof(T);
+    unpack(o, w.x, t);
+    unpack(o + E, w.y, t);
+    unpack(o + 2 * E, w.z, t);
+    unpack(o + 3 * E, w.w, t);
+}
+template <typename T>
+__device__ __forceinline__ void unpack(float* o, const Raw32& w, T t) {
+    constexpr int E = 16 / (int)sizeof(T);
+    unpack(o, w.lo, t);
+    unpack(o + E, w.hi, t);
+}
 
 template <typename TOK>
 __device__ __forceinline__ unsigned token_at(const TOK* tok, long long i, unsigned vocab) {
@@ -22,31 +70,37 @@ __device__ __forceinline__ unsigned token_at(const TOK* tok, long long i, unsign
 }
 
 // ---- out[i] = scale * table[tok[i]] -----------------------------------------
-// A warp per segment of SEG vectors of a row.
+// A warp takes up to 32 * e_unroll words of a row, all in flight at once.  Bound by the writes of the
+// rows (and their reads, where the table is large).
 constexpr int E_THREADS = 256;
-constexpr int E_UNROLL = 4;
+template <int V>
+constexpr int e_unroll = V >= 4 ? 4 : V == 2 ? 8 : 16;
 template <typename TOK, typename TT, typename OT, int V>
 __global__ void __launch_bounds__(E_THREADS) k_embed(const TOK* tok, long long n, const TT* table, unsigned vocab,
                                                      int dv, long long tstride, float scale, OT* out,
                                                      long long ostride, int segs) {
+    using R = typename Raw<sizeof(TT) * V>::type;
+    constexpr int E_UNROLL = e_unroll<V>;
     const int lane = threadIdx.x & 31;
     const long long nw = (long long)gridDim.x * (E_THREADS / 32);
     for (long long w = (long long)blockIdx.x * (E_THREADS / 32) + (threadIdx.x >> 5); w < n * segs; w += nw) {
-        const long long i = w / segs;
+        const long long i = segs == 1 ? w : w / segs;
         const int c0 = (int)(w - i * segs) * (32 * E_UNROLL) + lane;
         const unsigned t = token_at(tok, i, vocab);
-        const Pack<TT, V>* src = reinterpret_cast<const Pack<TT, V>*>(table + (long long)t * tstride);
+        // a token outside the vocabulary reads row 0 and writes zeros
+        const R* src = reinterpret_cast<const R*>(table + (long long)(t < vocab ? t : 0u) * tstride);
         Pack<OT, V>* dst = reinterpret_cast<Pack<OT, V>*>(out + i * ostride);
-        Pack<TT, V> in[E_UNROLL];
+        R in[E_UNROLL];
 #pragma unroll
-        for (int u = 0; u < E_UNROLL; ++u)
-            if (t < vocab && c0 + u * 32 < dv) in[u] = src[c0 + u * 32];
+        for (int u = 0; u < E_UNROLL; ++u) in[u] = src[min(c0 + u * 32, dv - 1)];
 #pragma unroll
         for (int u = 0; u < E_UNROLL; ++u) {
-            if (c0 + u * 32 >= dv) continue;
+            if (c0 + u * 32 >= dv) break;
+            float f[V];
+            unpack(f, in[u], TT());
             Pack<OT, V> o;
 #pragma unroll
-            for (int k = 0; k < V; ++k) o.v[k] = from_f32<OT>(t < vocab ? scale * to_f32(in[u].v[k]) : 0.0f);
+            for (int k = 0; k < V; ++k) o.v[k] = from_f32<OT>(t < vocab ? scale * f[k] : 0.0f);
             dst[c0 + u * 32] = o;
         }
     }
@@ -270,52 +324,12 @@ __global__ void __launch_bounds__(S_THREADS) k_sort_scatter(SRC src, long long n
 }
 
 // ---- sums over runs of one token ----------------------------------------------
-// N bytes in registers, as one load brings them (unpacked where they are used)
-template <int N>
-struct Raw;
-template <>
-struct Raw<2> {
-    using type = unsigned short;
-};
-template <>
-struct Raw<4> {
-    using type = unsigned;
-};
-template <>
-struct Raw<16> {
-    using type = uint4;
-};
-__device__ __forceinline__ void add_raw(float (&acc)[4], const uint4& w, float) {
-    acc[0] += __uint_as_float(w.x);
-    acc[1] += __uint_as_float(w.y);
-    acc[2] += __uint_as_float(w.z);
-    acc[3] += __uint_as_float(w.w);
-}
-__device__ __forceinline__ void add_raw(float (&acc)[1], unsigned w, float) { acc[0] += __uint_as_float(w); }
-__device__ __forceinline__ void add_raw(float (&acc)[8], const uint4& w, __nv_bfloat16) {
-    const unsigned v[4] = {w.x, w.y, w.z, w.w};
+template <int V, typename R, typename T>
+__device__ __forceinline__ void add_raw(float (&acc)[V], const R& w, T t) {
+    float f[V];
+    unpack(f, w, t);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        acc[2 * k] += __uint_as_float(v[k] << 16);
-        acc[2 * k + 1] += __uint_as_float(v[k] & 0xffff0000u);
-    }
-}
-__device__ __forceinline__ void add_raw(float (&acc)[8], const uint4& w, __half) {
-    const unsigned v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        __half2 p;
-        memcpy(&p, &v[k], 4);
-        const float2 f = __half22float2(p);
-        acc[2 * k] += f.x;
-        acc[2 * k + 1] += f.y;
-    }
-}
-__device__ __forceinline__ void add_raw(float (&acc)[1], unsigned short w, __nv_bfloat16) {
-    acc[0] += __uint_as_float((unsigned)w << 16);
-}
-__device__ __forceinline__ void add_raw(float (&acc)[1], unsigned short w, __half) {
-    acc[0] += __half2float(__ushort_as_half(w));
+    for (int k = 0; k < V; ++k) acc[k] += f[k];
 }
 
 // V columns of a row of the gradient: stored, or added to what is there
@@ -354,12 +368,14 @@ struct GradArgs {
 // run: part[2 piece] only).  The CTAs behind the pieces clear the rows of
 // tokens that do not occur.
 constexpr int G_THREADS = 128;
-constexpr int G_UNROLL = 8;
+template <typename R>
+constexpr int g_unroll = sizeof(R) >= 8 ? 8 : 16;  // rows in flight a thread
 constexpr int G_SHARED = 2048;  // positions a CTA holds, all its pieces together
 
 template <typename DT, typename OT, int V>
 __global__ void __launch_bounds__(G_THREADS, 8) k_grad_pieces(const GradArgs A) {
     using R = typename Raw<sizeof(DT) * V>::type;
+    constexpr int G_UNROLL = g_unroll<R>;
     const int c = ((int)blockIdx.y * blockDim.x + threadIdx.x) * V;
     OT* const out = reinterpret_cast<OT*>(A.out);
     __shared__ Pair held[G_SHARED];
@@ -486,6 +502,7 @@ constexpr int T_N = 2048, T_VOCAB = 4096;
 template <typename TOK, typename DT, typename OT, int V>
 __global__ void __launch_bounds__(T_THREADS) k_grad_small(const TOK* tok, const GradArgs A) {
     using R = typename Raw<sizeof(DT) * V>::type;
+    constexpr int G_UNROLL = 8;
     __shared__ unsigned key[T_N];
     __shared__ unsigned seen[T_VOCAB / 32 + 1];
     __shared__ float part[T_GROUPS][2][T_COLS * V];
@@ -693,7 +710,7 @@ void embed(const void* tokens, int32_t tok_type, int64_t n, const void* table, i
                 auto go = [&](auto vc) {
                     constexpr int V = decltype(vc)::value;
                     const int dv = (int)(dim / V);
-                    const int segs = (dv + 32 * E_UNROLL - 1) / (32 * E_UNROLL);
+                    const int segs = (dv + 32 * e_unroll<V> - 1) / (32 * e_unroll<V>);
                     const int64_t ctas = std::min<int64_t>((n * segs + E_THREADS / 32 - 1) / (E_THREADS / 32),
                                                            (int64_t)sms * 32);
                     k_embed<TOK, TT, OT, V><<<(unsigned)ctas, E_THREADS, 0, st>>>(
@@ -704,6 +721,7 @@ void embed(const void* tokens, int32_t tok_type, int64_t n, const void* table, i
                 };
                 if (ok(8)) go(std::integral_constant<int, 8>());
                 else if (ok(4)) go(std::integral_constant<int, 4>());
+                else if (ok(2)) go(std::integral_constant<int, 2>());
                 else go(std::integral_constant<int, 1>());
             });
         });
@@ -751,14 +769,16 @@ void embed_grad(const void* tokens, int32_t tok_type, int64_t n, const void* dy,
     auto typed = [&](auto&& f) {
         with_elem(dy_type, [&](auto dt) {
             with_elem(dtable_type, [&](auto ot) {
-                constexpr int V16 = 16 / (int)sizeof(dt);
-                if (n > 0 && fits(dy, dy_type, dim, dy_stride, V16)) {
-                    A.words = fits(dtable, dtable_type, dim, dtable_stride, V16);
-                    f(dt, ot, std::integral_constant<int, V16>());
-                } else {
-                    A.words = 1;
-                    f(dt, ot, std::integral_constant<int, 1>());
-                }
+                constexpr int V4 = 4 / (int)sizeof(dt);
+                auto ok = [&](int v) { return n > 0 && fits(dy, dy_type, dim, dy_stride, v); };
+                auto go = [&](auto vc) {
+                    A.words = fits(dtable, dtable_type, dim, dtable_stride, decltype(vc)::value);
+                    f(dt, ot, vc);
+                };
+                if (ok(4 * V4)) go(std::integral_constant<int, 4 * V4>());
+                else if (ok(2 * V4)) go(std::integral_constant<int, 2 * V4>());
+                else if (V4 > 1 && ok(V4)) go(std::integral_constant<int, V4>());
+                else go(std::integral_constant<int, 1>());
             });
         });
     };
