@@ -110,7 +110,8 @@ __global__ void __launch_bounds__(E_THREADS) k_embed(const TOK* tok, long long n
 // while that one still runs: it must call after_previous() before it touches
 // what earlier kernels write.  let_next() allows the next kernel to start; it
 // comes after after_previous(), so that what ran before the previous kernel is
-// complete for the next one's start.
+// complete for the next one's start.  In every kernel at least one CTA waits, so
+// that what follows the call on the stream finds all of its kernels done.
 __device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 template <typename... P, typename... Q>
@@ -447,11 +448,13 @@ template <typename OT>
 __global__ void __launch_bounds__(32 * J_GROUPS) k_grad_join(const GradArgs A) {
     const int piece = blockIdx.x;
     const int b = piece * A.per, e = min(b + A.per, A.n);
-    if (e >= A.n) return;
-    const unsigned key = A.pair[e - 1].key, after = A.pair[e].key, at = A.pair[b].key;
+    const unsigned key = A.pair[e - 1].key, after = e < A.n ? A.pair[e].key : ~0u, at = A.pair[b].key;
     const unsigned before = b > 0 ? A.pair[b - 1].key : ~0u;
-    if (key >= A.vocab || after != key) return;
-    if (at == key && before == key) return;  // started earlier
+    if (key >= A.vocab || after != key || (at == key && before == key)) {  // no run begins here and goes on
+        // one CTA waits in any case: this kernel does not end before the one it depends on
+        if (blockIdx.x == 0 && blockIdx.y == 0) after_previous();
+        return;
+    }
     const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
     int lo = piece + 1;  // becomes the end of the pieces that begin with this key
     for (bool more = true; more; lo += 128) {

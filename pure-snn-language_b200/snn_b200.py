@@ -12,6 +12,7 @@ module on a machine without the built library, or creating a network without
 a CUDA device, raises instead of falling back to anything else.
 """
 import ctypes as C
+import functools
 import os
 import struct
 
@@ -335,6 +336,14 @@ def embed(tokens, table, scale=1.0, dtype=None, out=None, stream=None):
     return out
 
 
+@functools.lru_cache(maxsize=1024)
+def _embed_work(n, vocab, dim):
+    """Workspace bytes of embed_grad's sizes."""
+    size = C.c_int64()
+    _check(lib().snn_embed_grad_workspace(n, vocab, dim, C.byref(size)))
+    return size.value
+
+
 def embed_grad(tokens, dy, vocab=None, scale=1.0, dtype=None, out=None, accumulate=False, stream=None):
     """Gradient of `embed` for its table (snn_embed_grad): [vocab, dim] with
     scale * the sum of dy over the positions of each token, in f32 over the
@@ -363,13 +372,11 @@ def embed_grad(tokens, dy, vocab=None, scale=1.0, dtype=None, out=None, accumula
                  "out must be [vocab, dim] of the wanted dtype")
         vocab = out.shape[0]
         ostride = _row_stride(out, "out")
-    L = lib()
-    size = C.c_int64()
-    _check(L.snn_embed_grad_workspace(n, vocab, dim, C.byref(size)))
-    work = _new(dev, stream, (size.value,), _T.uint8)
-    _call(L.snn_embed_grad, dev, stream, tokens.data_ptr(), tok, n, dy.data_ptr(), _elem(dy.dtype),
+    size = _embed_work(n, vocab, dim)
+    work = _new(dev, stream, (size,), _T.uint8)
+    _call(lib().snn_embed_grad, dev, stream, tokens.data_ptr(), tok, n, dy.data_ptr(), _elem(dy.dtype),
           dim, _row_stride(dy, "dy"), scale, out.data_ptr(), _elem(out.dtype), vocab, ostride,
-          1 if accumulate else 0, work.data_ptr(), size.value)
+          1 if accumulate else 0, work.data_ptr(), size)
     return out
 
 
@@ -388,7 +395,7 @@ def _scan_rows(t, name, shape, dtype):
 
 
 def _scan_args(gate, x, logit, leaky, offsets, dtype):
-    """(snn_scan, gate rows, x rows, dtype of y, its shape, the states' shape)"""
+    """(snn_scan, gate rows, x rows, dtype of y, its shape, the states' shape, _scan_sizes)"""
     if _T is None:
         _torch()
     dev, xt, shape = x.device, x.dtype, x.shape
@@ -427,7 +434,9 @@ def _scan_args(gate, x, logit, leaky, offsets, dtype):
         flags |= SCAN_CHANNEL
     else:
         g = _scan_rows(gate, "gate", shape, dtype)
-    return _SCAN.pack(_elem(dtype), flags, n_seq, shape[-2], d, off), g, xr, dtype, shape, (n_seq, d)
+    kind = _elem(dtype)
+    return (_SCAN.pack(kind, flags, n_seq, shape[-2], d, off), g, xr, dtype, shape, (n_seq, d),
+            _scan_sizes(kind, flags, n_seq, shape[-2], d, offsets is not None))
 
 
 def _state(t, name, shape, dev):
@@ -440,20 +449,14 @@ def _state(t, name, shape, dev):
     return t.data_ptr()
 
 
-def _saved_floats(desc):
-    size = C.c_int64()
-    _check(lib().snn_leaky_scan_saved(desc, C.byref(size)))
-    return size.value
-
-
-def _scan_work(fn, desc, dev, stream):
-    """(workspace or None, its address, its bytes)"""
-    size = C.c_int64()
-    _check(fn(desc, C.byref(size)))
-    if not size.value:
-        return None, None, 0
-    work = _new(dev, stream, (size.value,), _T.uint8)
-    return work, work.data_ptr(), size.value
+@functools.lru_cache(maxsize=1024)
+def _scan_sizes(kind, flags, n_seq, n_steps, channels, packed):
+    """(floats of saved, workspace bytes forward, gradient) of a scan's sizes."""
+    desc, size, L, out = _SCAN.pack(kind, flags, n_seq, n_steps, channels, 8 if packed else 0), C.c_int64(), lib(), []
+    for fn in (L.snn_leaky_scan_saved, L.snn_leaky_scan_workspace, L.snn_leaky_scan_grad_workspace):
+        _check(fn(desc, C.byref(size)))
+        out.append(size.value)
+    return tuple(out)
 
 
 def leaky_scan(gate, x, h0=None, logit=False, leaky=False, offsets=None, dtype=None, out=None,
@@ -471,7 +474,7 @@ def leaky_scan(gate, x, h0=None, logit=False, leaky=False, offsets=None, dtype=N
     needs.  `out` takes y; `h_out` takes h and may be h0, so that a stream of
     single steps keeps its state in place.  Rows of no sequence are not
     written: in a new y they hold what the memory held."""
-    desc, g, xr, dtype, shape, state = _scan_args(gate, x, logit, leaky, offsets, dtype)
+    desc, g, xr, dtype, shape, state, sizes = _scan_args(gate, x, logit, leaky, offsets, dtype)
     dev = x.device
     if out is None:
         out = _new(dev, stream, shape, dtype)
@@ -485,14 +488,15 @@ def leaky_scan(gate, x, h0=None, logit=False, leaky=False, offsets=None, dtype=N
         hp = h_out.data_ptr()
     else:
         hp = _state(h_out, "h_out", state, dev)
-    saved = sp = None
+    saved = sp = wp = None
     if save:
-        saved = _new(dev, stream, (_saved_floats(desc),), _T.float32)
+        saved = _new(dev, stream, (sizes[0],), _T.float32)
         sp = saved.data_ptr()
-    L = lib()
-    work, wp, wn = _scan_work(L.snn_leaky_scan_workspace, desc, dev, stream)
-    _call(L.snn_leaky_scan, dev, stream, desc, g, xr,
-          None if h0 is None else _state(h0, "h0", state, dev), yr, hp, sp, wp, wn)
+    if sizes[1]:
+        work = _new(dev, stream, (sizes[1],), _T.uint8)
+        wp = work.data_ptr()
+    _call(lib().snn_leaky_scan, dev, stream, desc, g, xr,
+          None if h0 is None else _state(h0, "h0", state, dev), yr, hp, sp, wp, sizes[1])
     return (out, h_out, saved) if save else (out, h_out)
 
 
@@ -505,15 +509,15 @@ def leaky_scan_grad(gate, x, dy, saved, dh=None, logit=False, leaky=False, offse
     result.  dgate has gate's shape and dtype (a gate per channel: the sum over
     all steps), dx x's, dh0 is float32 [sequences, channels]."""
     raster = not x.dtype.is_floating_point
-    desc, g, xr, dtype, shape, state = _scan_args(
+    desc, g, xr, dtype, shape, state, sizes = _scan_args(
         gate, x, logit, leaky, offsets, dy.dtype if raster and dy is not None else None)
     dev = x.device
     if dy is None and dh is None:
         raise SnnError(1, "neither dy nor dh is given")
     _cuda(saved, "saved", dev)
-    if saved.dtype != _T.float32 or saved.numel() != _saved_floats(desc) or not saved.is_contiguous():
+    if saved.dtype != _T.float32 or saved.numel() != sizes[0] or not saved.is_contiguous():
         raise SnnError(1, "saved is not what the forward call of these sizes gives")
-    dyr = dgate = dgr = dx = dxr = dh0 = hp = None
+    dyr = dgate = dgr = dx = dxr = dh0 = hp = wp = None
     d = shape[-1]
     if dy is not None:
         _cuda(dy, "dy", dev)
@@ -527,10 +531,11 @@ def leaky_scan_grad(gate, x, dy, saved, dh=None, logit=False, leaky=False, offse
     if need_h0:
         dh0 = _new(dev, stream, state, _T.float32)
         hp = dh0.data_ptr()
-    L = lib()
-    work, wp, wn = _scan_work(L.snn_leaky_scan_grad_workspace, desc, dev, stream)
-    _call(L.snn_leaky_scan_grad, dev, stream, desc, g, xr, saved.data_ptr(), dyr,
-          None if dh is None else _state(dh, "dh", state, dev), dgr, dxr, hp, wp, wn)
+    if sizes[2]:
+        work = _new(dev, stream, (sizes[2],), _T.uint8)
+        wp = work.data_ptr()
+    _call(lib().snn_leaky_scan_grad, dev, stream, desc, g, xr, saved.data_ptr(), dyr,
+          None if dh is None else _state(dh, "dh", state, dev), dgr, dxr, hp, wp, sizes[2])
     return dgate, dx, dh0
 
 

@@ -258,6 +258,50 @@ def test_two_graphs_streams_and_eager_calls():
 
 
 @pytest.mark.gpu
+def test_two_host_threads():
+    """Calls of two threads, each on its own stream, and of both on one stream."""
+    import threading
+    import torch
+    rng = np.random.default_rng(13)
+    sets = []
+    for n, vocab, dim in ((9000, 256, 96), (7000, 5000, 40)):
+        t, dy = tokens_of(rng, n, vocab, "int32"), make(rng, (n, dim), "f32")
+        sets.append((t, dy, vocab, snn.embed_grad(t, dy, vocab), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    one = torch.cuda.Stream()
+    for shared in (False, True):
+        wrong = []
+
+        def work(t, dy, vocab, want, stream):
+            for _ in range(40):
+                got = snn.embed_grad(t, dy, vocab, stream=one if shared else stream)
+                (one if shared else stream).synchronize()
+                if not torch.equal(got, want):
+                    wrong.append(vocab)
+
+        threads = [threading.Thread(target=work, args=s) for s in sets]
+        for th in threads:
+            th.start()
+        for th in threads:
+            th.join()
+        assert not wrong
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [50000, 200000])
+def test_result_is_ready_for_the_next_kernel(vocab):
+    """Runs that never cross pieces (each token once): what follows on the stream sees every row."""
+    import torch
+    n, dim = 40000, 256
+    t = torch.randperm(vocab, device="cuda")[:n]
+    dy = torch.randn(n, dim, device="cuda")
+    want = torch.zeros(vocab, dim, device="cuda")
+    want[t] = dy
+    for _ in range(20):
+        assert torch.equal(snn.embed_grad(t, dy, vocab), want)
+
+
+@pytest.mark.gpu
 def test_rows_past_32_bit_offsets():
     """A table of more than 2^31 elements (2^32 bytes in bf16), its last rows read and written."""
     import torch
