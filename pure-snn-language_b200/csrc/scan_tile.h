@@ -363,6 +363,10 @@ __device__ __forceinline__ void store_peer(Vec<V>* p, int rank, const Vec<V>& x)
 }
 
 template <int V>
+struct alignas(8 * V) Map {  // h -> a h + h0, one word of shared memory
+    Vec<V> a, h;
+};
+template <int V>
 struct ClusterMaps {  // the tiles' maps of a round, by rank; two rounds
     Vec<V> a[2][MAX_CLUSTER][32], h[2][MAX_CLUSTER][32];
 };
@@ -525,6 +529,9 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
     Decay<V, LO> fixed;
     Vec<V> factor = splat<V>(1.0f);
     if (PC) channel_decays<T, GM, V>(A, c, nl, fixed, factor);
+    Vec<V> whole = splat<V>(1.0f);  // L decays per channel
+    if (PC && W > 1)
+        for (int i = 0; i < L; ++i) whole = fixed.times(whole);
     int par = 0;
     const bool split = W == 1 && A.chunk > 0;
     for (long long j = item / A.ctiles; j < (split ? A.n_chunks : A.n_seq); j += A.workers) {
@@ -587,18 +594,18 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
             slot = slot + 1 == S ? 0 : slot + 1;
             Vec<V> h = carry;
             if constexpr (W > 1) {
-                __shared__ Vec<V> sa[2][W][32], sh[2][W][32];
+                __shared__ Map<V> maps[2][W][32];
                 __shared__ ClusterMaps<V> cm;
-                Vec<V> a = splat<V>(1.0f);
+                // decays per channel: every warp's product is the same, whole
+                Vec<V> a = PC ? whole : splat<V>(1.0f);
                 h = splat<V>(0.0f);
 #pragma unroll
                 for (int i = 0; i < L; ++i) {
                     const Decay<V, LO>& q = d[PC ? 0 : i];
                     h = q.step(h, u[i]);
-                    a = q.times(a);
+                    if (!PC) a = q.times(a);
                 }
-                sa[par][w][lane] = a;
-                sh[par][w][lane] = h;
+                maps[par][w][lane] = {a, h};
                 __syncthreads();
                 // the maps of the warps before this one (a, h) and of the whole tile (ta, th)
                 Vec<V> ta = splat<V>(1.0f), th = CL > 1 ? splat<V>(0.0f) : carry;
@@ -608,8 +615,8 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
                         a = ta;
                         h = th;
                     }
-                    const Vec<V> ja = sa[par][j][lane];
-                    th = vfma(ja, th, sh[par][j][lane]);
+                    const Vec<V> jh = maps[par][j][lane].h, ja = PC ? whole : maps[par][j][lane].a;
+                    th = vfma(ja, th, jh);
                     ta = vmul(ja, ta);
                 }
                 if (CL > 1) {
@@ -671,6 +678,9 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
     Decay<V, LO> fixed;
     Vec<V> factor = one, sum = splat<V>(0.0f);
     if (PC) channel_decays<T, GM, V>(A, c, nl, fixed, factor);
+    Vec<V> whole = splat<V>(1.0f);  // L decays per channel
+    if (PC && W > 1)
+        for (int i = 0; i < L; ++i) whole = fixed.times(whole);
     int par = 0;
     const bool split = W == 1 && A.chunk > 0;
     for (long long j = item / A.ctiles; j < (split ? A.n_chunks : A.n_seq); j += A.workers) {
@@ -756,31 +766,34 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
             slot = slot + 1 == S ? 0 : slot + 1;
             Vec<V> h = h0, r = carry;
             if constexpr (W > 1) {
-                __shared__ Vec<V> sa[2][W][32], sh[2][W][32], sr[2][W][32];
+                __shared__ Map<V> maps[2][W][32];
+                __shared__ Vec<V> sr[2][W][32];
                 __shared__ ClusterMaps<V> cm;
-                Vec<V> a = one;
+                Vec<V> a = PC ? whole : one;
                 h = r = splat<V>(0.0f);
 #pragma unroll
                 for (int i = 0; i < L; ++i) {
                     const Decay<V, LO>& q = d[PC ? 0 : i];
                     h = q.step(h, LEAKY ? vmul(PC ? factor : rest[PC ? 0 : i], x[i]) : x[i]);
-                    a = q.times(a);
+                    if (!PC) a = q.times(a);
                     r = d[PC ? 0 : L - 1 - i].times(vadd(o[L - 1 - i], r));
                 }
-                if (!some) {  // steps behind the end, whose rows were not read: r passes unchanged
+                if (!some) {  // steps behind the end, whose rows were not read: there r is 0 and stays so
                     a = one;
                     r = splat<V>(0.0f);
                 }
-                sa[par][w][lane] = a;
-                sh[par][w][lane] = h;
+                maps[par][w][lane] = {a, h};
                 sr[par][w][lane] = r;
                 __syncthreads();
-                Vec<V> hw = h0;
+                Vec<V> hw = h0, ja[PC ? 1 : W];
 #pragma unroll
                 for (int j = 0; j < W; ++j) {
                     if (j == w) h = hw;
-                    if (j < W - 1) hw = vfma(sa[par][j][lane], hw, sh[par][j][lane]);
+                    const Map<V> m = maps[par][j][lane];
+                    if (!PC) ja[PC ? 0 : j] = m.a;
+                    if (j < W - 1) hw = vfma(PC ? whole : m.a, hw, m.h);
                 }
+                if (PC) ja[0] = whole;
                 // the maps of the warps behind this one (a, r) and of the whole tile (ta, tr)
                 Vec<V> ta = one, tr = CL > 1 ? splat<V>(0.0f) : carry;
 #pragma unroll
@@ -789,9 +802,8 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
                         a = ta;
                         r = tr;
                     }
-                    const Vec<V> ja = sa[par][j][lane];
-                    tr = vfma(ja, tr, sr[par][j][lane]);
-                    ta = vmul(ja, ta);
+                    tr = vfma(ja[PC ? 0 : j], tr, sr[par][j][lane]);
+                    ta = vmul(ja[PC ? 0 : j], ta);
                 }
                 if (CL > 1) {
                     for (int q = w; q < CL; q += W) {
