@@ -24,11 +24,12 @@ VOCAB = 20999  # code points the synthetic stream draws from: U+4E00..U+9FFF and
 
 
 def _own():
-    pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "pure-snn-language_b200")
-    if pkg not in sys.path:
-        sys.path.insert(0, pkg)
-    import snn_b200
-    return snn_b200
+    if "snn_b200" not in sys.modules:
+        pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "pure-snn-language_b200")
+        if pkg not in sys.path:
+            sys.path.insert(0, pkg)
+        import snn_b200  # noqa: F401
+    return sys.modules["snn_b200"]
 
 
 def listed():
