@@ -533,6 +533,8 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
     if (PC && W > 1)
         for (int i = 0; i < L; ++i) whole = fixed.times(whole);
     int par = 0;
+    // a peer's shared memory may be written once the peer runs
+    if (W > 1 && CL > 1) cluster_sync();
     const bool split = W == 1 && A.chunk > 0;
     for (long long j = item / A.ctiles; j < (split ? A.n_chunks : A.n_seq); j += A.workers) {
         long long s = j;
@@ -682,6 +684,8 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
     if (PC && W > 1)
         for (int i = 0; i < L; ++i) whole = fixed.times(whole);
     int par = 0;
+    // a peer's shared memory may be written once the peer runs
+    if (W > 1 && CL > 1) cluster_sync();
     const bool split = W == 1 && A.chunk > 0;
     for (long long j = item / A.ctiles; j < (split ? A.n_chunks : A.n_seq); j += A.workers) {
         long long s = j;
