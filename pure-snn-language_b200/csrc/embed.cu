@@ -800,14 +800,15 @@ void embed_grad(const void* tokens, int32_t tok_type, int64_t n, const void* dy,
     const int size = elem_size(dtable_type);
     Clear clear = {(char*)dtable, vocab, dim * size, dtable_stride * size, 0, 0};
     if (!accumulate) {
-        if (clear.stride == clear.row_bytes) {
-            clear.row_bytes *= vocab;
+        const bool aligned = (uintptr_t)dtable % 16 == 0;
+        const int64_t all = clear.rows * clear.row_bytes;
+        clear.word = aligned && clear.row_bytes % 16 == 0 && clear.stride % 16 == 0 ? 16 : size;
+        if (aligned && clear.stride == clear.row_bytes) {  // one stretch of memory
             clear.rows = 1;
+            clear.row_bytes = all;
+            clear.word = 16;
         }
-        const bool wide = (uintptr_t)dtable % 16 == 0 &&
-                          (clear.rows == 1 || (clear.row_bytes % 16 == 0 && clear.stride % 16 == 0));
-        clear.word = wide ? 16 : size;
-        clear.ctas = (int)std::min<int64_t>(SMS * 3, (clear.rows * clear.row_bytes + (1 << 14) - 1) >> 14);
+        clear.ctas = (int)std::min<int64_t>(SMS * 3, (all + (1 << 14) - 1) >> 14);
     }
     if (n == 0) {
         if (clear.ctas) k_clear<<<(unsigned)clear.ctas, S_THREADS, 0, st>>>(clear);

@@ -197,6 +197,22 @@ def test_embed_grad_into_wider_rows(n, vocab, dim, width, ok):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,vocab,dim", [(500, 300, 24), (4000, 9000, 25), (40000, 6000, 40), (0, 7000, 8)])
+def test_embed_grad_at_an_odd_element(n, vocab, dim):
+    """A gradient, dy and table that begin at an odd element of a buffer."""
+    import torch
+    rng = np.random.default_rng(n)
+    t = torch.from_numpy(rng.integers(0, vocab, n)).cuda()
+    dy = make(rng, (n * dim + 1,), "bf16")[1:].view(n, dim)
+    flat = torch.full((vocab * dim + 2,), 7.0, dtype=torch.bfloat16, device="cuda")
+    got = snn.embed_grad(t, dy, out=flat[1:-1].view(vocab, dim))
+    want, bound = ref.embed_grad(t.cpu().numpy(), host(dy), vocab, 1.0)
+    ref.close(host(got), want, bound, "bf16")
+    assert flat[0] == 7 and flat[-1] == 7
+    assert torch.equal(snn.embed(t, got), got[t])
+
+
+@pytest.mark.gpu
 def test_embed_grad_of_no_valid_token():
     import torch
     t = torch.full((3000,), -1, dtype=torch.int32, device="cuda")
