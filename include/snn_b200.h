@@ -485,7 +485,7 @@ int snn_leaky_scan(const snn_scan* desc, const snn_rows* gate, const snn_rows* x
  *   dgate = da, or da a (1 - a) with SNN_SCAN_LOGIT;   dh0 = a_1 g_1.
  * dgate (nullable) has the gate's form: rows, or with SNN_SCAN_CHANNEL f32
  * [n_channels], the sum over all steps of all sequences in an order that
- * depends on the sizes alone.  dx (nullable, NULL with SNN_SCAN_RASTER) and dh0
+ * depends on the sizes and lengths alone.  dx (nullable, NULL with SNN_SCAN_RASTER) and dh0
  * (nullable, f32 [n_seq, n_channels]) as their inputs; rows of no sequence are
  * not written.  saved is what the forward call wrote.  work: as for
  * snn_embed_grad, of the size that snn_leaky_scan_grad_workspace says. */

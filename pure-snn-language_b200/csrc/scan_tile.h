@@ -68,6 +68,22 @@ __device__ __forceinline__ Span span_of(const ScanArgs& A, long long s) {
     r.block0 = flat / BLOCK + s;
     return r;
 }
+// The k-th longest of up to 64 packed sequences: they are taken in that order, so
+// that the longest do not start last.  All lanes of a warp call it.
+constexpr int MAX_SORTED = 64;
+__device__ __forceinline__ int by_length(const ScanArgs& A, int k) {
+    const int lane = threadIdx.x & 31, n = (int)A.n_seq;
+    const int a = lane < n ? span_of(A, lane).len : -1, b = lane + 32 < n ? span_of(A, lane + 32).len : -1;
+    int ra = 0, rb = 0;
+#pragma unroll 8
+    for (int q = 0; q < 32; ++q) {
+        const int x = __shfl_sync(~0u, a, q), y = __shfl_sync(~0u, b, q);
+        ra += (x > a || (x == a && q < lane)) + (y > a);
+        rb += (x >= b) + (y > b || (y == b && q < lane));
+    }
+    const unsigned ma = __ballot_sync(~0u, a >= 0 && ra == k), mb = __ballot_sync(~0u, b >= 0 && rb == k);
+    return ma ? __ffs(ma) - 1 : 31 + __ffs(mb);
+}
 // Chunk j of the launch: steps [from, to) of sequence s.  Sequence s has the
 // chunks from floor(flat / chunk) + s on, as with the blocks; the others hold
 // nothing (from = to = 1).  An empty sequence has one chunk (from = to = 0).
@@ -543,6 +559,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
         if (split) {
             sp = chunk_at(A, j, s, from_t, to_t);
         } else {
+            if (A.off && A.n_seq <= MAX_SORTED) s = by_length(A, (int)j);
             sp = span_of(A, s);
             to_t = sp.len;
         }
@@ -694,6 +711,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
         if (split) {
             sp = chunk_at(A, j, s, from_t, to_t);
         } else {
+            if (A.off && A.n_seq <= MAX_SORTED) s = by_length(A, (int)j);
             sp = span_of(A, s);
             to_t = sp.len;
         }
