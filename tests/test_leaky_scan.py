@@ -84,7 +84,8 @@ def call(grad=False, desc=(), **over):
 
 
 BAD = [dict(desc=dict(type=3)), dict(desc=dict(flags=16)), dict(desc=dict(n_seq=-1)), dict(desc=dict(n_steps=-1)),
-       dict(desc=dict(n_channels=0)), dict(desc=dict(n_channels=1 << 30)), dict(gate=None), dict(x=None),
+       dict(desc=dict(n_channels=0)), dict(desc=dict(n_channels=1 << 30)),
+       dict(desc=dict(n_seq=1 << 20, n_steps=1 << 20, n_channels=1 << 10)), dict(gate=None), dict(x=None),
        dict(gate=(None, 40, 8)), dict(x=(8193, 40, 8)), dict(x=(8192, -40, 8)), dict(x=(8192, 40, -8)),
        dict(desc=dict(flags=4), gate=(8194, 0, 0))]
 
