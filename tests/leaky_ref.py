@@ -50,6 +50,7 @@ def decay(z, logit):
         return 1 / (1 + np.exp(-z)), 1 / (1 + np.exp(z))
 
 
+@np.errstate(over="ignore", invalid="ignore")  # gates beyond 1 in magnitude may overflow; see close()
 def scan(gate, x, h0, dy=None, dh=None, logit=False, leaky=False, kind="f32"):
     """One sequence batch [b, t, d] in 64 bits: dict of name -> (value, bound).
     gate [b, t, d] or [d]; dy, dh None for zeros."""
