@@ -196,6 +196,8 @@ int64_t mean_steps(const snn_scan* d) { return d->offsets ? d->n_steps / std::ma
 //   39 packed, 1,997,736 rows x 33 (39)               692 / 307          1406 / 588
 //   1 x 50,021 x 1,000 f32 (32)                       163 / 197           292 / 236
 //   2 packed, 20,106 x 59 f32 (4)                      34 / 32             65 / 42
+//   100 packed, 2,000,000 x 30, per channel (100)     465 / 169           972 / 372
+//   120 packed, 2,400,000 x 20 f32 (120)              391 / 292           793 / 529
 //   3 packed, 30,000 x 2,000 bf16 (96)                132 / 150           243 / 277
 //   1 x 2,000 x 512 bf16 (8)                           12 / 26             18 / 32
 Plan plan_of(const snn_scan* d, bool grad) {
@@ -207,7 +209,7 @@ Plan plan_of(const snn_scan* d, bool grad) {
     p.chunk = 0;
     p.n_chunks = 0;
     const int64_t rows = d->offsets ? d->n_steps : d->n_seq * d->n_steps, items = (int64_t)p.ctiles * d->n_seq;
-    if (mean_steps(d) >= (grad ? 6144 : 12288) && items <= (d->offsets ? 48 : grad ? 36 : 16)) {
+    if (mean_steps(d) >= (grad ? 6144 : 12288) && items <= (d->offsets ? (p.ctiles <= 8 ? 160 : 48) : grad ? 36 : 16)) {
         const int64_t warps = SMS * (grad ? 8 : 12) * (d->flags & SNN_SCAN_CHANNEL ? 2 : 1);
         const int64_t c = (rows * p.ctiles + warps - 1) / warps;
         p.chunk = (int)std::max<int64_t>(128, (c + 15) / 16 * 16);

@@ -171,7 +171,8 @@ def test_scan_long(b, t, d, kind, channel, logit, leaky):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("lengths", [[0, 30000, 0, 1, 17000, 0], [0, 0, 40000], [16, 25001, 129], [12300, 12300]])
+@pytest.mark.parametrize("lengths", [[0, 30000, 0, 1, 17000, 0], [0, 0, 40000], [16, 25001, 129], [12300, 12300],
+                                     [6500] * 30 + [0, 3, 70000] + [1] * 3])
 @pytest.mark.parametrize("channel", [False, True])
 def test_packed_long(lengths, channel):
     """The same of packed sequences, with empty ones among them and rows of no sequence around them."""
