@@ -257,6 +257,7 @@ void run_plan(const snn_scan* d, int words, const Plan& p, void* work, ScanArgs&
             while (groups < 32 && groups * 4 < mean) groups *= 2;
             k_scan_join<GRAD><<<dim3((unsigned)((d->n_channels + 31) / 32), (unsigned)std::min<int64_t>(d->n_seq, 65535)),
                                 32 * groups, 0, st>>>(A);
+            SNN_CUDA(cudaGetLastError());  // the launch after it does not report this one
         }
         launch_tiles<GRAD, T>(gm, raster, words, false, p, A, st);
     });
