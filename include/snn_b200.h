@@ -434,7 +434,11 @@ int snn_embed_grad(const void* tokens, int32_t tok_type, int64_t n, const void* 
  *   h_t = a_t h_{t-1} + u_t,   y_t = h_t,   u_t = x_t, or (1 - a_t) x_t with SNN_SCAN_LEAKY
  * with a_t the gate, or 1 / (1 + exp(-gate)) with SNN_SCAN_LOGIT.  The state
  * is f32; y is rounded once.  n_steps <= 2^30, n_channels < 2^30.  A state that
- * has become infinite stays infinite or turns NaN.
+ * has become infinite stays infinite or turns NaN.  The gate may be any number.
+ * Spans of steps (up to a whole sequence) are joined by the products of their
+ * decays: where decays beyond 1 take such a product past f32, a state of 0 stays
+ * what the steps make of it, any other may turn infinite or NaN even if step by
+ * step it would not.  The same holds for the gradients.
  * Layout: dense (offsets NULL): n_seq sequences of n_steps steps; packed
  * (offsets set): n_steps rows in all, sequence s the rows
  * [offsets[s], offsets[s + 1]) of every tensor (int64[n_seq + 1] in device

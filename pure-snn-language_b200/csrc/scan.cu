@@ -77,6 +77,8 @@ __global__ void k_scan_join(const ScanArgs A) {
     __shared__ float sa[32][32], sh[32][32];
     const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, groups = blockDim.x >> 5;
     const int c = (int)blockIdx.x * 32 + lane;
+    // a product that overflowed leaves a state of 0 where it was (see mapped)
+    auto apply = [](float ma, float h, float mh) { return h == 0.0f ? mh : fmaf(ma, h, mh); };
     for (long long s = blockIdx.y; s < A.n_seq; s += gridDim.y) {
         const Span sp = span_of(A, s);
         const int n = max(1, (sp.len + A.chunk - 1) / A.chunk);
@@ -89,7 +91,7 @@ __global__ void k_scan_join(const ScanArgs A) {
 #pragma unroll 8
             for (int p = lo; p < min(hi, n - 1); ++p) {
                 const float ma = A.map_a[at(p)];
-                h = fmaf(ma, h, A.map_h[at(p)]);
+                h = apply(ma, h, A.map_h[at(p)]);
                 a *= ma;
             }
         sa[g][lane] = a;
@@ -97,13 +99,13 @@ __global__ void k_scan_join(const ScanArgs A) {
         __syncthreads();
         if (c < A.D) {
             h = !GRAD && A.h0 ? A.h0[s * A.D + c] : 0.0f;
-            for (int k = 0; k < g; ++k) h = fmaf(sa[k][lane], h, sh[k][lane]);
+            for (int k = 0; k < g; ++k) h = apply(sa[k][lane], h, sh[k][lane]);
 #pragma unroll 8
             for (int p = lo; p < hi; ++p) {
                 const bool map = p < n - 1;
                 const float ma = map ? A.map_a[at(p)] : 0.0f, mh = map ? A.map_h[at(p)] : 0.0f;
                 A.map_h[at(p)] = h;
-                h = fmaf(ma, h, mh);
+                h = apply(ma, h, mh);
             }
         }
         __syncthreads();

@@ -382,6 +382,37 @@ template <int V>
 struct alignas(8 * V) Map {  // h -> a h + h0, one word of shared memory
     Vec<V> a, h;
 };
+// A span's map applied to a state: a h + b.  The product a of decays beyond 1
+// may overflow over a span in which the state is 0: then a h is NaN where the
+// states stay 0.  The joins of a tile use the plain form and, where that left a
+// NaN, the spans once more by join_spans (one test a tile instead of two
+// instructions a map; the kernels are bound by instruction issue).
+template <int V>
+__device__ __forceinline__ Vec<V> mapped(const Vec<V>& a, const Vec<V>& h, const Vec<V>& b) {
+    Vec<V> r;
+#pragma unroll
+    for (int k = 0; k < V; ++k) r.v[k] = h.v[k] == 0.0f ? b.v[k] : fmaf(a.v[k], h.v[k], b.v[k]);
+    return r;
+}
+template <int V>
+__device__ __forceinline__ bool any_nan(const Vec<V>& x) {
+    bool r = false;
+#pragma unroll
+    for (int k = 0; k < V; ++k) r |= x.v[k] != x.v[k];
+    return r;
+}
+// n spans from state x: x the state behind them, own the one before span `at`;
+// map(j, a, b) gives the j-th span's map.  Not unrolled: it keeps few registers.
+template <int V, typename F>
+__device__ __forceinline__ void join_spans(int n, int at, Vec<V>& x, Vec<V>& own, F map) {
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+        if (j == at) own = x;
+        Vec<V> a, b;
+        map(j, a, b);
+        x = mapped(a, x, b);
+    }
+}
 template <int V>
 struct ClusterMaps {  // the tiles' maps of a round, by rank; two rounds
     Vec<V> a[2][MAX_CLUSTER][32], h[2][MAX_CLUSTER][32];
@@ -638,18 +669,33 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
                     th = vfma(ja, th, jh);
                     ta = vmul(ja, ta);
                 }
+                if (any_nan(th)) {
+                    th = CL > 1 ? splat<V>(0.0f) : carry;
+                    join_spans(W, w, th, h, [&](int j, Vec<V>& ja, Vec<V>& jh) {
+                        ja = PC ? whole : maps[par][j][lane].a;
+                        jh = maps[par][j][lane].h;
+                    });
+                }
                 if (CL > 1) {
                     for (int r = w; r < CL; r += W) {
                         store_peer<V>(&cm.a[par][rank][lane], r, ta);
                         store_peer<V>(&cm.h[par][rank][lane], r, th);
                     }
                     cluster_sync();
+                    const Vec<V> was = carry;
                     Vec<V> in = carry;
                     for (int r = 0; r < CL; ++r) {
                         if (r == rank) in = carry;
                         carry = vfma(cm.a[par][r][lane], carry, cm.h[par][r][lane]);
                     }
-                    h = vfma(a, in, h);
+                    if (any_nan(carry)) {
+                        carry = was;
+                        join_spans(CL, rank, carry, in, [&](int r, Vec<V>& ra, Vec<V>& rh) {
+                            ra = cm.a[par][r][lane];
+                            rh = cm.h[par][r][lane];
+                        });
+                    }
+                    h = mapped(a, in, h);
                 } else {
                     carry = th;
                 }
@@ -827,18 +873,40 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
                     tr = vfma(ja[PC ? 0 : j], tr, sr[par][j][lane]);
                     ta = vmul(ja[PC ? 0 : j], ta);
                 }
+                if (any_nan(h)) {
+                    hw = h0;
+                    join_spans(W, w, hw, h, [&](int j, Vec<V>& ma, Vec<V>& mh) {
+                        ma = PC ? whole : maps[par][j][lane].a;
+                        mh = maps[par][j][lane].h;
+                    });
+                }
+                if (any_nan(tr)) {
+                    tr = CL > 1 ? splat<V>(0.0f) : carry;
+                    join_spans(W, W - 1 - w, tr, r, [&](int j, Vec<V>& ma, Vec<V>& mr) {
+                        ma = PC ? whole : maps[par][W - 1 - j][lane].a;
+                        mr = sr[par][W - 1 - j][lane];
+                    });
+                }
                 if (CL > 1) {
                     for (int q = w; q < CL; q += W) {
                         store_peer<V>(&cm.a[par][rank][lane], q, ta);
                         store_peer<V>(&cm.h[par][rank][lane], q, tr);
                     }
                     cluster_sync();
+                    const Vec<V> was = carry;
                     Vec<V> in = carry;
                     for (int q = 0; q < CL; ++q) {
                         if (q == rank) in = carry;
                         carry = vfma(cm.a[par][q][lane], carry, cm.h[par][q][lane]);
                     }
-                    r = vfma(a, in, r);
+                    if (any_nan(carry)) {
+                        carry = was;
+                        join_spans(CL, rank, carry, in, [&](int q, Vec<V>& qa, Vec<V>& qr) {
+                            qa = cm.a[par][q][lane];
+                            qr = cm.h[par][q][lane];
+                        });
+                    }
+                    r = mapped(a, in, r);
                 } else {
                     carry = tr;
                 }
