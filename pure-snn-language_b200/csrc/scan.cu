@@ -14,9 +14,10 @@ __global__ void __launch_bounds__(128) k_scan_steps(const ScanArgs A) {
     if (c >= A.D) return;
     for (long long s = blockIdx.y; s < A.n_seq; s += gridDim.y) {
         const Span sp = span_of(A, s);
-        Decay<V, keeps_lo<T, GM>> d;
+        constexpr bool LO = is_logit<GM>;
+        Decay<V, LO> d;
         Vec<V> rest;
-        if (per_channel<GM>) channel_decays<T, GM, V>(A, c, V, d, rest);
+        if (per_channel<GM>) channel_decays<GM>(A, c, V, d, rest);
         Vec<V> h = load_f32<V>(A.h0 + s * A.D + c, A.h0 != nullptr);
         constexpr int U = 4;  // steps whose rows are loaded before the first is used
         for (int t0 = 0; t0 < sp.len; t0 += U) {
@@ -37,10 +38,16 @@ __global__ void __launch_bounds__(128) k_scan_steps(const ScanArgs A) {
                 const int t = t0 + i;
                 if (t >= sp.len) break;
                 if (A.saved && t % BLOCK == 0) store_f32<V>(A.saved + (sp.block0 + t / BLOCK) * A.D + c, h);
-                if (!per_channel<GM>) decays<T, GM, V>(Unpack<T>::get(g[i]), d, rest);
+                if (!per_channel<GM>) decays<T, GM>(Unpack<T>::get(g[i]), d, rest);
                 Vec<V> u = in_values<T, V, RASTER>(xw[i], c);
                 if (A.leaky) u = vmul(rest, u);
+                const Vec<V> before = h;
                 h = d.step(h, u);
+                if constexpr (short_logit<T, GM>) {  // an infinite state stays so
+#pragma unroll
+                    for (int k = 0; k < V; ++k)
+                        if (fabsf(before.v[k]) > FLT_MAX) h.v[k] = fmaf(d.a.v[k], before.v[k], u.v[k]);
+                }
                 *reinterpret_cast<Word<T, V>*>(reinterpret_cast<T*>(A.y.p) + row_at(A, A.y, s, sp, t) + c) =
                     Unpack<T>::put(h);
             }
@@ -72,13 +79,11 @@ __global__ void __launch_bounds__(256) k_scan_gate_sum(const ScanArgs A, int row
 // The states (GRAD: r) that the chunks of a sequence start from, from their
 // maps; in place of map_h.  A warp per consecutive part of the chunks joins its
 // maps, the parts' maps give each its first state.
-template <bool GRAD>
+template <bool GRAD, bool KEEP>
 __global__ void k_scan_join(const ScanArgs A) {
-    __shared__ float sa[32][32], sh[32][32];
+    __shared__ Vec<1> sa[32][32], sl[32][32], sh[32][32];
     const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, groups = blockDim.x >> 5;
     const int c = (int)blockIdx.x * 32 + lane;
-    // a product that overflowed leaves a state of 0 where it was (see mapped)
-    auto apply = [](float ma, float h, float mh) { return h == 0.0f ? mh : fmaf(ma, h, mh); };
     for (long long s = blockIdx.y; s < A.n_seq; s += gridDim.y) {
         const Span sp = span_of(A, s);
         const int n = max(1, (sp.len + A.chunk - 1) / A.chunk);
@@ -86,26 +91,29 @@ __global__ void k_scan_join(const ScanArgs A) {
         // position p of the chain: chunk j0 + p, or from the last one back
         auto at = [&](int p) { return (j0 + (GRAD ? n - 1 - p : p)) * A.D + c; };
         const int per = (n + groups - 1) / groups, lo = min(n, g * per), hi = min(n, lo + per);
-        float a = 1.0f, h = 0.0f;
+        Vec<1> a = {1.0f}, l = {0.0f}, h = {0.0f};
         if (c < A.D)
 #pragma unroll 8
             for (int p = lo; p < min(hi, n - 1); ++p) {
-                const float ma = A.map_a[at(p)];
-                h = apply(ma, h, A.map_h[at(p)]);
-                a *= ma;
+                const Vec<1> ma = {A.map_a[at(p)]}, ml = {KEEP ? A.map_l[at(p)] : 0.0f}, mh = {A.map_h[at(p)]};
+                h = mapped<KEEP>(ma, ml, h, mh);
+                if (KEEP) span_times(ma, ml, a, l);
+                else a = vmul(ma, a);
             }
         sa[g][lane] = a;
+        sl[g][lane] = l;
         sh[g][lane] = h;
         __syncthreads();
         if (c < A.D) {
-            h = !GRAD && A.h0 ? A.h0[s * A.D + c] : 0.0f;
-            for (int k = 0; k < g; ++k) h = apply(sa[k][lane], h, sh[k][lane]);
+            h.v[0] = !GRAD && A.h0 ? A.h0[s * A.D + c] : 0.0f;
+            for (int k = 0; k < g; ++k) h = mapped<KEEP>(sa[k][lane], sl[k][lane], h, sh[k][lane]);
 #pragma unroll 8
             for (int p = lo; p < hi; ++p) {
                 const bool map = p < n - 1;
-                const float ma = map ? A.map_a[at(p)] : 0.0f, mh = map ? A.map_h[at(p)] : 0.0f;
-                A.map_h[at(p)] = h;
-                h = apply(ma, h, mh);
+                const Vec<1> ma = {map ? A.map_a[at(p)] : 0.0f}, ml = {map && KEEP ? A.map_l[at(p)] : 0.0f};
+                const Vec<1> mh = {map ? A.map_h[at(p)] : 0.0f};
+                A.map_h[at(p)] = h.v[0];
+                h = mapped<KEEP>(ma, ml, h, mh);
             }
         }
         __syncthreads();
@@ -234,7 +242,7 @@ Plan plan_of(const snn_scan* d, bool grad) {
 int64_t map_floats(const snn_scan* d, const Plan& p) { return (p.n_chunks * d->n_channels + 63) / 64 * 64; }
 int64_t work_bytes_of(const snn_scan* d, const Plan& p, bool grad) {
     const int64_t sums = grad && (d->flags & SNN_SCAN_CHANNEL) ? (int64_t)p.workers * p.cluster * d->n_channels : 0;
-    return (2 * map_floats(d, p) + sums) * 4;
+    return (3 * map_floats(d, p) + sums) * 4;
 }
 void check_work(const void* work, int64_t bytes, int64_t needed) {
     SNN_REQUIRE(needed == 0 || (work && (uintptr_t)work % 256 == 0 && bytes >= needed), SNN_ERR_ARG,
@@ -247,7 +255,8 @@ void run_plan(const snn_scan* d, int words, const Plan& p, void* work, ScanArgs&
     A.chunk = p.chunk;
     A.n_chunks = p.n_chunks;
     A.map_a = (float*)work;
-    A.map_h = (float*)work + map_floats(d, p);
+    A.map_l = (float*)work + map_floats(d, p);
+    A.map_h = (float*)work + 2 * map_floats(d, p);
     const int gm = gate_mode(d);
     const bool raster = (d->flags & SNN_SCAN_RASTER) != 0;
     snnb::with_elem(d->type, [&](auto t) {
@@ -257,8 +266,9 @@ void run_plan(const snn_scan* d, int words, const Plan& p, void* work, ScanArgs&
             const int64_t mean = p.n_chunks / d->n_seq;
             int groups = 1;
             while (groups < 32 && groups * 4 < mean) groups *= 2;
-            k_scan_join<GRAD><<<dim3((unsigned)((d->n_channels + 31) / 32), (unsigned)std::min<int64_t>(d->n_seq, 65535)),
-                                32 * groups, 0, st>>>(A);
+            const dim3 grid((unsigned)((d->n_channels + 31) / 32), (unsigned)std::min<int64_t>(d->n_seq, 65535));
+            if (A.logit) k_scan_join<GRAD, true><<<grid, 32 * groups, 0, st>>>(A);
+            else k_scan_join<GRAD, false><<<grid, 32 * groups, 0, st>>>(A);
             SNN_CUDA(cudaGetLastError());  // the launch after it does not report this one
         }
         launch_tiles<GRAD, T>(gm, raster, words, false, p, A, st);
@@ -369,7 +379,7 @@ void leaky_scan_grad(const snn_scan* d, const snn_rows* gate, const snn_rows* x,
                                  {channel ? none : A.dgate, A.dx});
     const Plan p = plan_of(d, true);
     check_work(work, work_bytes, work_bytes_of(d, p, true));
-    if (channel && dgate) A.part = (float*)work + 2 * map_floats(d, p);
+    if (channel && dgate) A.part = (float*)work + 3 * map_floats(d, p);
     run_plan<true>(d, words, p, work, A, st);
     if (A.part) {
         k_scan_gate_sum<<<(unsigned)((d->n_channels + 31) / 32), 256, 0, st>>>(A, p.workers * p.cluster);

@@ -3,6 +3,7 @@
 // element type and direction is compiled by a file of its own (scan_*.cu).
 #pragma once
 #include <algorithm>
+#include <cfloat>
 #include "elem.h"
 
 namespace snnb_scan {
@@ -41,7 +42,7 @@ struct ScanArgs {
     // then in map_h the states (gradient: r) that they start from
     int chunk;
     long long n_chunks;
-    float *map_a, *map_h;
+    float *map_a, *map_l, *map_h;  // product of decays, what it lost, end state
 };
 
 // rows of sequence s: [begin, begin + len) of the flat row index (packed), or
@@ -155,11 +156,17 @@ __device__ __forceinline__ Vec<2> vadd(Vec<2> a, Vec<2> b) {
 
 // The decays of V channels.  A logistic decay near 1 is 1 - s with a small s.
 // Rounded to f32 it is off by up to 2^-25, which a memory of 1 / s steps adds
-// up to 2^-25 / s of the state where the gate stays the same.  Per-channel
-// gates and f32 gates therefore keep what the rounding lost as `lo` (one more
-// FMA a step); 16-bit gates, whose own rounding is 2^-9 and up of the exponent
-// and differs from step to step, do not.  (An infinite state times lo may be
-// NaN: infinities do not survive, they end as infinities or NaN.)
+// up to 2^-25 / s of the state where the gate stays the same.  What the rounding
+// lost is therefore kept wherever a state is carried on:
+//  - per-channel and f32 gates keep it as `lo` (one more FMA a step), and so do
+//    single steps;
+//  - a warp by itself with 16-bit gates takes it into the next step's decay
+//    (decays_on): no registers, and no more than one rounding is ever open;
+//  - tiles of warps with 16-bit gates do without inside a warp's 16 (gradient
+//    8) steps, since the state goes from warp to warp by their maps, whose
+//    products keep it (span_lo).
+// (An infinite state times lo, or times what a product keeps, may be NaN:
+// infinities do not survive, they end as infinities or NaN.)
 template <int V, bool LO>
 struct Decay {
     Vec<V> a;
@@ -176,7 +183,24 @@ struct Decay<V, true> {
 };
 template <typename T, int GM>
 constexpr bool keeps_lo = GM == GATE_CHANNEL_LOGIT || (GM == GATE_LOGIT && sizeof(T) == 4);
+// 16-bit logits
+template <typename T, int GM>
+constexpr bool short_logit = GM == GATE_LOGIT && sizeof(T) == 2;
 
+// The map of a span of steps, h -> (a + l) h + b: a the rounded product of its
+// decays, l what that product is off by.  Where states come a long way a is near
+// 1, and 1 - a is known better than a: as r = the sum over the steps of (1 -
+// decay) times the product before it, each 1 - decay with its own relative
+// precision.  So l = (1 - a) - r where 1 - a is exact; where a span halves the
+// state, roundings of its own add up over few spans only, and l is 0.  Kept for
+// logits (KEEP); decays that are given are multiplied as they are.
+template <int V>
+__device__ __forceinline__ Vec<V> span_lo(const Vec<V>& a, const Vec<V>& r) {
+    Vec<V> l;
+#pragma unroll
+    for (int k = 0; k < V; ++k) l.v[k] = a.v[k] >= 0.5f ? (1.0f - a.v[k]) - r.v[k] : 0.0f;
+    return l;
+}
 // decay a = 1 / (1 + exp(-z)) and its rest 1 - a, each with its own relative
 // precision: from e = exp(-|z|) the larger is 1 / (1 + e), the smaller e times
 // that.  exp(-|z|) = 2^p (1 + q ln 2) with p the rounded product -|z| log2(e)
@@ -199,37 +223,62 @@ __device__ __forceinline__ void logistic(float z, float& a, float& lo, float& re
     lo = up ? (1.0f - near1) - s : 0.0f;
     rest = up ? s : big;
 }
-// the same by the short instructions (2 ulp each, the argument rounded once)
-__device__ __forceinline__ void logistic_fast(float z, float& a, float& rest) {
-    float e, big;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fabsf(z) * -1.4426950408889634f));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(big) : "f"(1.0f + e));
-    const float s = e * big;
-    const bool up = z >= 0.0f;
-    a = up ? big : s;
-    rest = up ? s : big;
+// The same of V logits by the short instructions (2 ulp each, the argument
+// rounded once): a = 1 / (1 + t) and rest = t a with t = exp(-z), each with its
+// own relative precision on both sides of 0, so that nothing is selected.  t ends
+// at 2^126, where the subtraction leaves a = 0.
+template <int V>
+__device__ __forceinline__ void logistic_fast(const Vec<V>& z, Vec<V>& a, Vec<V>& rest) {
+    Vec<V> t = vmul(z, splat<V>(-1.4426950408889634f));
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        asm("min.NaN.f32 %0, %0, %1;" : "+f"(t.v[k]) : "f"(126.0f));
+        asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(t.v[k]));
+    }
+    a = vadd(t, splat<V>(1.0f));
+#pragma unroll
+    for (int k = 0; k < V; ++k) asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a.v[k]));
+    rest = vmul(t, a);
+    a = vadd(a, splat<V>(-1.17549435e-38f));
 }
 
 // decay and rest of V gates
-template <typename T, int GM, int V>
-__device__ __forceinline__ void decays(const Vec<V>& z, Decay<V, keeps_lo<T, GM>>& d, Vec<V>& rest) {
+template <typename T, int GM, int V, bool LO>
+__device__ __forceinline__ void decays(const Vec<V>& z, Decay<V, LO>& d, Vec<V>& rest) {
+    if constexpr (short_logit<T, GM>) {
+        logistic_fast(z, d.a, rest);
+        const Vec<V> lo = span_lo(d.a, rest);
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        const float v = z.v[k];
-        float a = v, lo = 0.0f, r = 1.0f - v;
-        if (GM == GATE_LOGIT) {
-            if (sizeof(T) == 4) logistic(v, a, lo, r);
-            else logistic_fast(v, a, r);
+        for (int k = 0; k < V; ++k) d.set_lo(k, lo.v[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const float v = z.v[k];
+            float a = v, lo = 0.0f, r = 1.0f - v;
+            if (GM == GATE_LOGIT) logistic(v, a, lo, r);
+            d.a.v[k] = a;
+            d.set_lo(k, lo);
+            rest.v[k] = r;
         }
-        d.a.v[k] = a;
-        d.set_lo(k, lo);
-        rest.v[k] = r;
     }
 }
+// The same for 16-bit logits in the order of a recurrence: `left` is what the
+// steps before still have to lose, by which the decays' product over any number
+// of steps stays within one rounding.  After a NaN it is NaN, as the recurrence
+// is from there on; a decay below 1/2 drops it.
+template <int V>
+__device__ __forceinline__ void decays_on(const Vec<V>& z, Decay<V, false>& d, Vec<V>& rest, Vec<V>& left) {
+    const Vec<V> one = splat<V>(1.0f), minus = splat<V>(-1.0f);
+    logistic_fast(z, d.a, rest);
+    const Vec<V> t = vadd(rest, left), a = vfma(minus, t, one);
+    left = vfma(minus, vfma(minus, a, one), t);
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+        if (d.a.v[k] >= 0.5f) d.a.v[k] = a.v[k];
+}
 // those of the per-channel gates c .. c + V
-template <typename T, int GM, int V>
-__device__ __forceinline__ void channel_decays(const ScanArgs& A, int c, int nl, Decay<V, keeps_lo<T, GM>>& d,
-                                               Vec<V>& rest) {
+template <int GM, int V, bool LO>
+__device__ __forceinline__ void channel_decays(const ScanArgs& A, int c, int nl, Decay<V, LO>& d, Vec<V>& rest) {
 #pragma unroll
     for (int k = 0; k < V; ++k) {
         const float v = k < nl ? reinterpret_cast<const float*>(A.gate.p)[c + k] : 0.0f;
@@ -344,11 +393,13 @@ struct Shape {
     static constexpr int W = W_, L = L_, TT = W_ * L_, threads = 32 * W_;
     static constexpr int S = S_;        // stages of rows in flight per warp
     static constexpr int CTAS = CTAS_;  // CTAs an SM is to hold
+    static constexpr bool clusters = W_ == 8;
 };
 using Fwd = Shape<8, 16, 2, 2>;
 using Bwd = Shape<8, 8, 3, 2>;
-// Decays per channel leave the forward pass registers for a third CTA (the
-// gradient spills and loses by one: documents 171 -> 187 us).
+// Decays per channel leave the forward pass registers for a third CTA: 80 a
+// thread, of which 16-bit forms spill 8 - 24 bytes (the gradient spills more and
+// loses by one: documents 171 -> 187 us).
 using FwdChannel = Shape<8, 16, 2, 3>;
 // Without clusters the gradient takes smaller CTAs, twice as many on an SM.
 using BwdMany = Shape<4, 8, 3, 4>;
@@ -378,20 +429,41 @@ __device__ __forceinline__ void store_peer(Vec<V>* p, int rank, const Vec<V>& x)
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(r + 4 * k), "f"(x.v[k]) : "memory");
 }
 
+// the product (a, l) of spans times one more, each with what it is off by
 template <int V>
-struct alignas(8 * V) Map {  // h -> a h + h0, one word of shared memory
-    Vec<V> a, h;
+__device__ __forceinline__ void span_times(const Vec<V>& sa, const Vec<V>& sl, Vec<V>& a, Vec<V>& l) {
+    const Vec<V> n = vmul(sa, a);
+    l = vfma(sa, l, vfma(sl, a, vfma(sa, a, vmul(splat<V>(-1.0f), n))));
+    a = n;
+}
+template <int V>
+struct alignas(8 * V) Pair {  // one word of shared memory
+    Vec<V> a, b;
 };
-// A span's map applied to a state: a h + b.  The product a of decays beyond 1
-// may overflow over a span in which the state is 0: then a h is NaN where the
-// states stay 0.  The joins of a tile use the plain form and, where that left a
-// NaN, the spans once more by join_spans (one test a tile instead of two
-// instructions a map; the kernels are bound by instruction issue).
-template <int V>
-__device__ __forceinline__ Vec<V> mapped(const Vec<V>& a, const Vec<V>& h, const Vec<V>& b) {
-    Vec<V> r;
+// A map applied to a state.  The product of decays beyond 1 (given ones, not
+// logits') may overflow over a span in which the state is 0: then a h is NaN
+// where the states stay 0.  The warps of a tile learn at their barrier whether a
+// product among them did, and take the spans by join_spans then.  This is
+// compiled for given decays alone: in the gradient of 16 x 4,096 x 2,048 bf16
+// logits it would take 20 of 315 us (a test for NaN behind the joins 26).
+template <bool KEEP, int V>
+__device__ __forceinline__ Vec<V> plain(const Vec<V>& a, const Vec<V>& l, const Vec<V>& h, const Vec<V>& b) {
+    return vfma(a, h, KEEP ? vfma(l, h, b) : b);
+}
+// the same with 0 as it is: equal wherever the plain form gives a number
+template <bool KEEP, int V>
+__device__ __forceinline__ Vec<V> mapped(const Vec<V>& a, const Vec<V>& l, const Vec<V>& h, const Vec<V>& b) {
+    const Vec<V> r = plain<KEEP>(a, l, h, b);
+    Vec<V> q;
 #pragma unroll
-    for (int k = 0; k < V; ++k) r.v[k] = h.v[k] == 0.0f ? b.v[k] : fmaf(a.v[k], h.v[k], b.v[k]);
+    for (int k = 0; k < V; ++k) q.v[k] = h.v[k] == 0.0f ? b.v[k] : r.v[k];
+    return q;
+}
+template <int V>
+__device__ __forceinline__ bool overflowed(const Vec<V>& x) {  // infinite or NaN
+    bool r = false;
+#pragma unroll
+    for (int k = 0; k < V; ++k) r |= !(fabsf(x.v[k]) <= FLT_MAX);
     return r;
 }
 template <int V>
@@ -402,20 +474,39 @@ __device__ __forceinline__ bool any_nan(const Vec<V>& x) {
     return r;
 }
 // n spans from state x: x the state behind them, own the one before span `at`;
-// map(j, a, b) gives the j-th span's map.  Not unrolled: it keeps few registers.
-template <int V, typename F>
+// map(j, a, l, b) gives the j-th span's map.  Not unrolled: it keeps few registers.
+template <bool KEEP, int V, typename F>
 __device__ __forceinline__ void join_spans(int n, int at, Vec<V>& x, Vec<V>& own, F map) {
 #pragma unroll 1
     for (int j = 0; j < n; ++j) {
         if (j == at) own = x;
-        Vec<V> a, b;
-        map(j, a, b);
-        x = mapped(a, x, b);
+        Vec<V> a, l, b;
+        map(j, a, l, b);
+        x = mapped<KEEP>(a, l, x, b);
     }
+}
+// Decays per channel: every warp's product is the same.  In shared memory, by
+// lane: the products of 0 .. W warps.  Says whether one warp's overflows.
+template <int V, int W>
+struct Powers {
+    Pair<V> p[W + 1][32];
+};
+template <int V, int W, bool LO>
+__device__ __forceinline__ bool powers(Powers<V, W>& P, const Decay<V, LO>& d, const Vec<V>& rest, int steps, int w, int lane) {
+    Vec<V> a = splat<V>(1.0f), r = splat<V>(0.0f), pa = a, pl = r;
+    for (int i = 0; i < steps; ++i) {
+        if (LO) r = vfma(rest, a, r);
+        a = vmul(d.a, a);
+    }
+    const Vec<V> l = LO ? span_lo(a, r) : r;
+    if (w == 0) P.p[0][lane] = {pa, pl};
+    for (int j = 0; j <= w; ++j) span_times(a, l, pa, pl);
+    P.p[w + 1][lane] = {pa, LO ? pl : r};
+    return __syncthreads_or(!LO && overflowed(a));
 }
 template <int V>
 struct ClusterMaps {  // the tiles' maps of a round, by rank; two rounds
-    Vec<V> a[2][MAX_CLUSTER][32], h[2][MAX_CLUSTER][32];
+    Vec<V> a[2][MAX_CLUSTER][32], l[2][MAX_CLUSTER][32], h[2][MAX_CLUSTER][32];
 };
 
 // Rows are staged in shared memory by asynchronous copies, each warp its own
@@ -562,7 +653,7 @@ struct Stage {
 template <typename SH, typename T, int GM, bool RASTER, bool LEAKY, int COPY>
 __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanArgs A) {
     constexpr int W = SH::W, L = SH::L, TT = SH::TT, S = SH::S, V = lane_channels<T>;
-    constexpr bool LO = keeps_lo<T, GM>, PC = per_channel<GM>;
+    constexpr bool LO = keeps_lo<T, GM>, PC = per_channel<GM>, KEEP = is_logit<GM>;
     using St = Stage<GM, RASTER, COPY, L, V, false>;
     static_assert(L * V <= 32, "a lane holds one raster word");
     extern __shared__ __align__(16) char rows[];
@@ -573,12 +664,13 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
     const int round = CL * TT;
     char* const mine = rows + w * S * St::bytes;
     const unsigned mine_s = (unsigned)__cvta_generic_to_shared(mine);
+    const Vec<V> one = splat<V>(1.0f), zero = splat<V>(0.0f);
     Decay<V, LO> fixed;
-    Vec<V> factor = splat<V>(1.0f);
-    if (PC) channel_decays<T, GM, V>(A, c, nl, fixed, factor);
-    Vec<V> whole = splat<V>(1.0f);  // L decays per channel
-    if (PC && W > 1)
-        for (int i = 0; i < L; ++i) whole = fixed.times(whole);
+    Vec<V> factor = one;
+    if (PC) channel_decays<GM>(A, c, nl, fixed, factor);
+    __shared__ std::conditional_t<PC && (W > 1), Powers<V, W>, char> pw_s;
+    bool over = false;  // a product of a warp's decays overflows
+    if constexpr (PC && W > 1) over = powers<V, W>(pw_s, fixed, factor, L, w, lane);
     int par = 0;
     // a peer's shared memory may be written once the peer runs
     if (W > 1 && CL > 1) cluster_sync();
@@ -623,17 +715,25 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
 #pragma unroll
         for (int k = 0; k < S; ++k) fetch(t1 + k * round, k);
         int slot = 0;
+        Vec<V> left = zero;
         for (int t0 = t1; t0 - t1 < to_t - from_t; t0 += round) {
             Decay<V, LO> d[PC ? 1 : L];
-            Vec<V> u[L];
+            Vec<V> u[L], a = one, ar = zero;  // the product of the decays and 1 - it
             copy_wait<S - 1>();
             __syncwarp();
             const char* from = mine + slot * St::bytes;
 #pragma unroll
             for (int i = 0; i < L; ++i) {
                 Vec<V> f = factor;
-                if (!PC)
-                    decays<T, GM, V>(Unpack<T>::get(staged<COPY>(from + St::gate, i, lane, i & 1 ? g1 : g0)), d[i], f);
+                if constexpr (!PC) {
+                    const Vec<V> z = Unpack<T>::get(staged<COPY>(from + St::gate, i, lane, i & 1 ? g1 : g0));
+                    if constexpr (W == 1 && short_logit<T, GM>) decays_on(z, d[i], f, left);
+                    else decays<T, GM>(z, d[i], f);
+                    if (W > 1) {
+                        if (KEEP) ar = vfma(f, a, ar);
+                        a = vmul(d[i].a, a);
+                    }
+                }
                 if constexpr (RASTER) u[i] = raster_values<V>(from + St::x, i, lane);
                 else u[i] = Unpack<T>::get(staged<COPY>(from + St::x, i, lane, i & 1 ? x1 : x0));
                 if (LEAKY) u[i] = vmul(f, u[i]);
@@ -644,60 +744,102 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
             slot = slot + 1 == S ? 0 : slot + 1;
             Vec<V> h = carry;
             if constexpr (W > 1) {
-                __shared__ Map<V> maps[2][W][32];
+                // (a, h) and (l, 1 - a) of the warps' maps; h alone where the products are fixed
+                __shared__ Pair<V> maps[PC ? 1 : 2][PC ? 1 : W][32], prods[PC ? 1 : 2][PC ? 1 : W][32];
+                __shared__ Vec<V> ends[PC ? 2 : 1][PC ? W : 1][32];
                 __shared__ ClusterMaps<V> cm;
-                // decays per channel: every warp's product is the same, whole
-                Vec<V> a = PC ? whole : splat<V>(1.0f);
-                h = splat<V>(0.0f);
+                h = zero;
 #pragma unroll
-                for (int i = 0; i < L; ++i) {
-                    const Decay<V, LO>& q = d[PC ? 0 : i];
-                    h = q.step(h, u[i]);
-                    if (!PC) a = q.times(a);
+                for (int i = 0; i < L; ++i) h = d[PC ? 0 : i].step(h, u[i]);
+                if (t0 >= to_t) {  // steps behind the end, whose rows were not read
+                    a = one;
+                    ar = h = zero;
                 }
-                maps[par][w][lane] = {a, h};
-                __syncthreads();
-                // the maps of the warps before this one (a, h) and of the whole tile (ta, th)
-                Vec<V> ta = splat<V>(1.0f), th = CL > 1 ? splat<V>(0.0f) : carry;
-#pragma unroll
-                for (int j = 0; j < W; ++j) {
-                    if (j == w) {
-                        a = ta;
-                        h = th;
+                if constexpr (PC) {
+                    ends[par][w][lane] = h;
+                    __syncthreads();
+                } else {
+                    maps[par][w][lane] = {a, h};
+                    if (KEEP) prods[par][w][lane] = {span_lo(a, ar), ar};
+                    if (KEEP) __syncthreads();
+                    else over = __syncthreads_or(overflowed(a));
+                }
+                auto map = [&](int j, Vec<V>& ja, Vec<V>& jl, Vec<V>& jh) {
+                    if constexpr (PC) {
+                        ja = pw_s.p[1][lane].a;
+                        jl = pw_s.p[1][lane].b;
+                        jh = ends[par][j][lane];
+                    } else {
+                        ja = maps[par][j][lane].a;
+                        jh = maps[par][j][lane].b;
+                        jl = KEEP ? prods[par][j][lane].a : zero;
                     }
-                    const Vec<V> jh = maps[par][j][lane].h, ja = PC ? whole : maps[par][j][lane].a;
-                    th = vfma(ja, th, jh);
-                    ta = vmul(ja, ta);
-                }
-                if (any_nan(th)) {
-                    th = CL > 1 ? splat<V>(0.0f) : carry;
-                    join_spans(W, w, th, h, [&](int j, Vec<V>& ja, Vec<V>& jh) {
-                        ja = PC ? whole : maps[par][j][lane].a;
-                        jh = maps[par][j][lane].h;
-                    });
-                }
+                };
+                // the state before this warp (h) and behind the tile (th); with a cluster those from zero
                 if (CL > 1) {
+                    Vec<V> th = zero, al, ta = one, tl = zero;  // the products of the warps before this one, of the tile
+#pragma unroll
+                    for (int j = 0; j < W; ++j) {
+                        if (j == w) {
+                            h = th;
+                            a = ta;
+                            ar = tl;
+                        }
+                        Vec<V> ja, jl, jh;
+                        map(j, ja, jl, jh);
+                        th = plain<KEEP>(ja, jl, th, jh);
+                        if constexpr (!PC) {
+                            if (KEEP) tl = vfma(prods[par][j][lane].b, ta, tl);
+                            ta = vmul(ja, ta);
+                        }
+                    }
+                    if (!KEEP && over) {
+                        th = zero;
+                        join_spans<KEEP>(W, w, th, h, map);
+                    }
+                    if constexpr (PC) {
+                        a = pw_s.p[w][lane].a;
+                        al = pw_s.p[w][lane].b;
+                        ta = pw_s.p[W][lane].a;
+                        tl = pw_s.p[W][lane].b;
+                    } else {
+                        al = KEEP ? span_lo(a, ar) : zero;
+                        if (KEEP) tl = span_lo(ta, tl);
+                    }
                     for (int r = w; r < CL; r += W) {
-                        store_peer<V>(&cm.a[par][rank][lane], r, ta);
+                        if (!PC) store_peer<V>(&cm.a[par][rank][lane], r, ta);
+                        if (!PC && KEEP) store_peer<V>(&cm.l[par][rank][lane], r, tl);
                         store_peer<V>(&cm.h[par][rank][lane], r, th);
                     }
                     cluster_sync();
+                    auto tile_map = [&](int r, Vec<V>& ra, Vec<V>& rl, Vec<V>& rh) {
+                        ra = PC ? ta : cm.a[par][r][lane];
+                        rl = PC || !KEEP ? tl : cm.l[par][r][lane];
+                        rh = cm.h[par][r][lane];
+                    };
                     const Vec<V> was = carry;
                     Vec<V> in = carry;
                     for (int r = 0; r < CL; ++r) {
                         if (r == rank) in = carry;
-                        carry = vfma(cm.a[par][r][lane], carry, cm.h[par][r][lane]);
+                        Vec<V> ra, rl, rh;
+                        tile_map(r, ra, rl, rh);
+                        carry = plain<KEEP>(ra, rl, carry, rh);
                     }
-                    if (any_nan(carry)) {
+                    if (!KEEP && any_nan(carry)) {
                         carry = was;
-                        join_spans(CL, rank, carry, in, [&](int r, Vec<V>& ra, Vec<V>& rh) {
-                            ra = cm.a[par][r][lane];
-                            rh = cm.h[par][r][lane];
-                        });
+                        join_spans<KEEP>(CL, rank, carry, in, tile_map);
                     }
-                    h = mapped(a, in, h);
+                    h = KEEP ? plain<KEEP>(a, al, in, h) : mapped<KEEP>(a, al, in, h);
+                } else if (!KEEP && over) {
+                    join_spans<KEEP>(W, w, carry, h, map);
                 } else {
-                    carry = th;
+#pragma unroll
+                    for (int j = 0; j < W; ++j) {
+                        if (j == w) h = carry;
+                        Vec<V> ja, jl, jh;
+                        map(j, ja, jl, jh);
+                        carry = plain<KEEP>(ja, jl, carry, jh);
+                    }
                 }
                 par ^= 1;
             }
@@ -729,7 +871,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
 template <typename SH, typename T, int GM, bool RASTER, bool LEAKY, int COPY>
 __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const ScanArgs A) {
     constexpr int W = SH::W, L = SH::L, TT = SH::TT, S = SH::S, V = lane_channels<T>;
-    constexpr bool LO = keeps_lo<T, GM>, PC = per_channel<GM>;
+    constexpr bool LO = keeps_lo<T, GM>, PC = per_channel<GM>, KEEP = is_logit<GM>;
     using St = Stage<GM, RASTER, COPY, L, V, true>;
     extern __shared__ __align__(16) char rows[];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -739,13 +881,13 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
     const int round = CL * TT;
     char* const mine = rows + w * S * St::bytes;
     const unsigned mine_s = (unsigned)__cvta_generic_to_shared(mine);
-    const Vec<V> one = splat<V>(1.0f), minus = splat<V>(-1.0f);
+    const Vec<V> one = splat<V>(1.0f), zero = splat<V>(0.0f), minus = splat<V>(-1.0f);
     Decay<V, LO> fixed;
-    Vec<V> factor = one, sum = splat<V>(0.0f);
-    if (PC) channel_decays<T, GM, V>(A, c, nl, fixed, factor);
-    Vec<V> whole = splat<V>(1.0f);  // L decays per channel
-    if (PC && W > 1)
-        for (int i = 0; i < L; ++i) whole = fixed.times(whole);
+    Vec<V> factor = one, sum = zero;
+    if (PC) channel_decays<GM>(A, c, nl, fixed, factor);
+    __shared__ std::conditional_t<PC && (W > 1), Powers<V, W>, char> pw_s;
+    bool over = false;  // a product of a warp's decays overflows
+    if constexpr (PC && W > 1) over = powers<V, W>(pw_s, fixed, factor, L, w, lane);
     int par = 0;
     // a peer's shared memory may be written once the peer runs
     if (W > 1 && CL > 1) cluster_sync();
@@ -805,18 +947,26 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
 #pragma unroll
         for (int k = 0; k < S; ++k) fetch(t1 - k * round, k);
         int slot = 0, t0 = t1;
+        Vec<V> left = zero;
         for (int b = 0; b < tiles; b += CL, t0 -= round) {  // t0 before from_t: no tile left for this CTA
             const bool some = t0 >= from_t && t0 < to_t;
             Decay<V, LO> d[PC ? 1 : L];
-            Vec<V> rest[PC ? 1 : L], x[L], o[L];
+            Vec<V> rest[PC ? 1 : L], x[L], o[L], a = one, ar = zero;
             copy_wait<S - 1>();
             __syncwarp();
             const char* from = mine + slot * St::bytes;
             const Vec<V> h0 = reinterpret_cast<const Vec<V>*>(from + St::state)[lane];
 #pragma unroll
-            for (int i = 0; i < L; ++i) {
-                if (!PC)
-                    decays<T, GM, V>(Unpack<T>::get(staged<COPY>(from + St::gate, i, lane, i & 1 ? g1 : g0)), d[i], rest[i]);
+            for (int i = L - 1; i >= 0; --i) {
+                if constexpr (!PC) {
+                    const Vec<V> z = Unpack<T>::get(staged<COPY>(from + St::gate, i, lane, i & 1 ? g1 : g0));
+                    if constexpr (W == 1 && short_logit<T, GM>) decays_on(z, d[i], rest[i], left);
+                    else decays<T, GM>(z, d[i], rest[i]);
+                    if (W > 1) {
+                        if (KEEP) ar = vfma(rest[i], a, ar);
+                        a = vmul(d[i].a, a);
+                    }
+                }
                 if constexpr (RASTER) x[i] = raster_values<V>(from + St::x, i, lane);
                 else x[i] = Unpack<T>::get(staged<COPY>(from + St::x, i, lane, i & 1 ? x1 : x0));
                 o[i] = splat<V>(0.0f);
@@ -834,82 +984,119 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
             slot = slot + 1 == S ? 0 : slot + 1;
             Vec<V> h = h0, r = carry;
             if constexpr (W > 1) {
-                __shared__ Map<V> maps[2][W][32];
-                __shared__ Vec<V> sr[2][W][32];
-                __shared__ ClusterMaps<V> cm;
-                Vec<V> a = PC ? whole : one;
-                h = r = splat<V>(0.0f);
+                // (a, h), (r, l) and 1 - a of the warps' maps; h and r where the products are fixed
+                constexpr bool RESTS = !PC && KEEP && SH::clusters;
+                __shared__ Pair<V> maps[PC ? 1 : 2][PC ? 1 : W][32], back[2][W][32];
+                __shared__ Vec<V> ends[PC ? 2 : 1][PC ? W : 1][32], rests[RESTS ? 2 : 1][RESTS ? W : 1][32];
+                h = r = zero;
 #pragma unroll
                 for (int i = 0; i < L; ++i) {
-                    const Decay<V, LO>& q = d[PC ? 0 : i];
-                    h = q.step(h, LEAKY ? vmul(PC ? factor : rest[PC ? 0 : i], x[i]) : x[i]);
-                    if (!PC) a = q.times(a);
+                    h = d[PC ? 0 : i].step(h, LEAKY ? vmul(PC ? factor : rest[PC ? 0 : i], x[i]) : x[i]);
                     r = d[PC ? 0 : L - 1 - i].times(vadd(o[L - 1 - i], r));
                 }
                 if (!some) {  // steps behind the end, whose rows were not read: there r is 0 and stays so
                     a = one;
-                    r = splat<V>(0.0f);
+                    ar = r = zero;
                 }
-                maps[par][w][lane] = {a, h};
-                sr[par][w][lane] = r;
-                __syncthreads();
-                Vec<V> hw = h0, ja[PC ? 1 : W];
+                if constexpr (PC) {
+                    ends[par][w][lane] = h;
+                    back[par][w][lane].a = r;
+                    __syncthreads();
+                } else {
+                    maps[par][w][lane] = {a, h};
+                    back[par][w][lane] = {r, KEEP ? span_lo(a, ar) : zero};
+                    if constexpr (RESTS) rests[par][w][lane] = ar;
+                    if (KEEP) __syncthreads();
+                    else over = __syncthreads_or(overflowed(a));
+                }
+                // The states start anew in every tile: they do without l.
+                auto map = [&](int j, Vec<V>& ja, Vec<V>& jl, Vec<V>& jh) {
+                    jl = zero;
+                    if constexpr (PC) {
+                        ja = pw_s.p[1][lane].a;
+                        jh = ends[par][j][lane];
+                    } else {
+                        ja = maps[par][j][lane].a;
+                        jh = maps[par][j][lane].b;
+                    }
+                };
+                auto map_back = [&](int j, Vec<V>& ja, Vec<V>& jl, Vec<V>& jr) {
+                    jr = back[par][W - 1 - j][lane].a;
+                    if constexpr (PC) {
+                        ja = pw_s.p[1][lane].a;
+                        jl = pw_s.p[1][lane].b;
+                    } else {
+                        ja = maps[par][W - 1 - j][lane].a;
+                        jl = back[par][W - 1 - j][lane].b;
+                    }
+                };
+                Vec<V> hw = h0, ja[W], jl, jh;
 #pragma unroll
                 for (int j = 0; j < W; ++j) {
                     if (j == w) h = hw;
-                    const Map<V> m = maps[par][j][lane];
-                    if (!PC) ja[PC ? 0 : j] = m.a;
-                    if (j < W - 1) hw = vfma(PC ? whole : m.a, hw, m.h);
+                    map(j, ja[j], jl, jh);
+                    if (j < W - 1) hw = vfma(ja[j], hw, jh);
                 }
-                if (PC) ja[0] = whole;
-                // the maps of the warps behind this one (a, r) and of the whole tile (ta, tr)
-                Vec<V> ta = one, tr = CL > 1 ? splat<V>(0.0f) : carry;
+                // r behind this warp's steps (r) and before the tile's (tr); with a cluster those from zero
+                Vec<V> tr = CL > 1 ? zero : carry, al, ta = one, tl = zero;
 #pragma unroll
-                for (int j = W - 1; j >= 0; --j) {
-                    if (j == w) {
-                        a = ta;
+                for (int j = 0; j < W; ++j) {
+                    if (W - 1 - j == w) {
                         r = tr;
+                        a = ta;
+                        ar = tl;
                     }
-                    tr = vfma(ja[PC ? 0 : j], tr, sr[par][j][lane]);
-                    ta = vmul(ja[PC ? 0 : j], ta);
+                    Vec<V> jr, unused;
+                    map_back(j, unused, jl, jr);
+                    tr = plain<KEEP>(ja[W - 1 - j], jl, tr, jr);
+                    if constexpr (!PC && SH::clusters) {  // the products of the warps behind this one, of the tile
+                        if constexpr (RESTS) tl = vfma(rests[par][W - 1 - j][lane], ta, tl);
+                        ta = vmul(ja[W - 1 - j], ta);
+                    }
                 }
-                if (any_nan(h)) {
+                if (!KEEP && over) {
                     hw = h0;
-                    join_spans(W, w, hw, h, [&](int j, Vec<V>& ma, Vec<V>& mh) {
-                        ma = PC ? whole : maps[par][j][lane].a;
-                        mh = maps[par][j][lane].h;
-                    });
+                    join_spans<KEEP>(W, w, hw, h, map);
+                    tr = CL > 1 ? zero : carry;
+                    join_spans<KEEP>(W, W - 1 - w, tr, r, map_back);
                 }
-                if (any_nan(tr)) {
-                    tr = CL > 1 ? splat<V>(0.0f) : carry;
-                    join_spans(W, W - 1 - w, tr, r, [&](int j, Vec<V>& ma, Vec<V>& mr) {
-                        ma = PC ? whole : maps[par][W - 1 - j][lane].a;
-                        mr = sr[par][W - 1 - j][lane];
-                    });
-                }
-                if (CL > 1) {
+                if constexpr (SH::clusters) if (CL > 1) {
+                    __shared__ ClusterMaps<V> cm;
+                    if constexpr (PC) {
+                        a = pw_s.p[W - 1 - w][lane].a;
+                        al = pw_s.p[W - 1 - w][lane].b;
+                        ta = pw_s.p[W][lane].a;
+                        tl = pw_s.p[W][lane].b;
+                    } else {
+                        al = KEEP ? span_lo(a, ar) : zero;
+                        if (KEEP) tl = span_lo(ta, tl);
+                    }
                     for (int q = w; q < CL; q += W) {
-                        store_peer<V>(&cm.a[par][rank][lane], q, ta);
+                        if (!PC) store_peer<V>(&cm.a[par][rank][lane], q, ta);
+                        if (!PC && KEEP) store_peer<V>(&cm.l[par][rank][lane], q, tl);
                         store_peer<V>(&cm.h[par][rank][lane], q, tr);
                     }
                     cluster_sync();
+                    auto tile_map = [&](int q, Vec<V>& qa, Vec<V>& ql, Vec<V>& qr) {
+                        qa = PC ? ta : cm.a[par][q][lane];
+                        ql = PC || !KEEP ? tl : cm.l[par][q][lane];
+                        qr = cm.h[par][q][lane];
+                    };
                     const Vec<V> was = carry;
                     Vec<V> in = carry;
                     for (int q = 0; q < CL; ++q) {
                         if (q == rank) in = carry;
-                        carry = vfma(cm.a[par][q][lane], carry, cm.h[par][q][lane]);
+                        Vec<V> qa, ql, qr;
+                        tile_map(q, qa, ql, qr);
+                        carry = plain<KEEP>(qa, ql, carry, qr);
                     }
-                    if (any_nan(carry)) {
+                    if (!KEEP && any_nan(carry)) {
                         carry = was;
-                        join_spans(CL, rank, carry, in, [&](int q, Vec<V>& qa, Vec<V>& qr) {
-                            qa = cm.a[par][q][lane];
-                            qr = cm.h[par][q][lane];
-                        });
+                        join_spans<KEEP>(CL, rank, carry, in, tile_map);
                     }
-                    r = mapped(a, in, r);
-                } else {
-                    carry = tr;
+                    r = KEEP ? plain<KEEP>(a, al, in, r) : mapped<KEEP>(a, al, in, r);
                 }
+                if (CL == 1) carry = tr;
                 par ^= 1;
             }
             if (nl > 0 && some) {
@@ -968,7 +1155,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
 template <typename SH, typename T, int GM, bool RASTER, bool LEAKY, int COPY, bool GRAD>
 __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_map(const ScanArgs A) {
     constexpr int L = SH::L, S = SH::S, V = lane_channels<T>;
-    constexpr bool LO = keeps_lo<T, GM>, PC = per_channel<GM>;
+    constexpr bool LO = keeps_lo<T, GM>, PC = per_channel<GM>, KEEP = is_logit<GM>;
     using St = Stage<GM, RASTER, COPY, L, V, false>;  // its x is dy for the gradient
     static_assert(SH::W == 1, "a warp by itself");
     extern __shared__ __align__(16) char rows[];
@@ -1007,30 +1194,41 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_map(const ScanAr
         for (int k = 0; k < S; ++k) fetch(t1 + k * step, k);
         Decay<V, LO> fixed;
         Vec<V> factor = splat<V>(1.0f);
-        if (PC) channel_decays<T, GM, V>(A, c, nl, fixed, factor);
-        Vec<V> a = splat<V>(1.0f), h = splat<V>(0.0f);
+        if (PC) channel_decays<GM>(A, c, nl, fixed, factor);
+        const Vec<V> one = splat<V>(1.0f), zero = splat<V>(0.0f);
+        Vec<V> a = one, l = zero, h = zero, left = zero;
         int slot = 0, t0 = t1;
         for (int b = 0; b < tiles; ++b, t0 += step) {
             Decay<V, LO> d[PC ? 1 : L];
-            Vec<V> u[L];
+            Vec<V> u[L], ra = one, rr = zero;  // these steps' product of decays and 1 - it
             copy_wait<S - 1>();
             __syncwarp();
             const char* from = rows + slot * St::bytes;
+            const int n = min(L, to_t - t0);
 #pragma unroll
-            for (int i = 0; i < L; ++i) {
+            for (int k = 0; k < L; ++k) {
+                const int i = GRAD ? L - 1 - k : k;
                 Vec<V> f = factor;
-                if (!PC)
-                    decays<T, GM, V>(Unpack<T>::get(staged<COPY>(from + St::gate, i, lane, i & 1 ? g1 : g0)), d[i], f);
+                if constexpr (!PC) {
+                    const Vec<V> z = Unpack<T>::get(staged<COPY>(from + St::gate, i, lane, i & 1 ? g1 : g0));
+                    if constexpr (short_logit<T, GM>) decays_on(z, d[i], f, left);
+                    else decays<T, GM>(z, d[i], f);
+                }
                 if constexpr (RASTER) u[i] = raster_values<V>(from + St::x, i, lane);
                 else u[i] = Unpack<T>::get(staged<COPY>(from + St::x, i, lane, i & 1 ? x1 : x0));
-                if (!in.p) u[i] = splat<V>(0.0f);
+                if (!in.p) u[i] = zero;
                 if (LEAKY && !GRAD) u[i] = vmul(f, u[i]);
+                if (i < n) {
+                    if (KEEP) rr = vfma(f, ra, rr);
+                    ra = vmul(PC ? fixed.a : d[PC ? 0 : i].a, ra);
+                }
             }
             if (PC) d[0] = fixed;
             __syncwarp();
             fetch(t0 + S * step, slot);
             slot = slot + 1 == S ? 0 : slot + 1;
-            const int n = min(L, to_t - t0);
+            if (KEEP) span_times(ra, span_lo(ra, rr), a, l);
+            else a = vmul(ra, a);
             if (GRAD) {
                 if (A.dh && t0 + n == sp.len) {
                     const Vec<V> dh = load_n<V>(A.dh + s * A.D + c, nl);
@@ -1040,22 +1238,17 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_map(const ScanAr
                 }
 #pragma unroll
                 for (int i = L - 1; i >= 0; --i)
-                    if (i < n) {
-                        h = d[PC ? 0 : i].times(vadd(u[i], h));
-                        a = d[PC ? 0 : i].times(a);
-                    }
+                    if (i < n) h = d[PC ? 0 : i].times(vadd(u[i], h));
             } else {
 #pragma unroll
                 for (int i = 0; i < L; ++i)
-                    if (i < n) {
-                        h = d[PC ? 0 : i].step(h, u[i]);
-                        a = d[PC ? 0 : i].times(a);
-                    }
+                    if (i < n) h = d[PC ? 0 : i].step(h, u[i]);
             }
         }
         copy_wait<0>();
         __syncwarp();
         store_n<V>(A.map_a + j * A.D + c, a, nl);
+        if (KEEP) store_n<V>(A.map_l + j * A.D + c, l, nl);
         store_n<V>(A.map_h + j * A.D + c, h, nl);
     }
 }

@@ -1,8 +1,10 @@
 """Leaky scans at the edges of what their arguments allow, each through the kernels that the sizes choose."""
+import numpy as np
 import pytest
 
+import leaky_ref as ref
 import snn_b200 as snn
-from test_leaky_scan import dt
+from test_leaky_scan import dt, host
 
 SMS = 148
 
@@ -52,3 +54,52 @@ def test_silent_channels_stay_silent(fwd, bwd, b, t, d, kind, channel):
     dgate, dx, dh0 = snn.leaky_scan_grad(gate, x, dy, saved)
     assert (dx[:, 0] == 2).all() and (dx[:, 1:] == 0).all() and (dgate == 0).all()
     assert torch.equal(dh0, (2 * row).expand(b, d))
+
+
+# ---- logits that stay the same -----------------------------------------------------
+KEPT = [("cluster", "cluster", 1, 16384, 8192), ("warps", "warps", 10, 4096, 8192), ("chunks", "chunks", 1, 50000, 512),
+        ("tiles", "small", 500, 1000, 64)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fwd,bwd,b,t,d", KEPT)
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("z", [7.25, 8.5, 10.0, 11.375])
+def test_constant_logits_keep_their_memory(fwd, bwd, b, t, d, kind, z):
+    """A logit that is the same at every step (a row broadcast over the steps; each z is exact in bf16): over t steps
+    the state shrinks by a^t, and the decay's own rounding would take it off by up to t U, the same in every channel.
+    Here the mean over the n = b d channels is compared: a step rounds the state by at most U of it, differently from
+    channel to channel (the first states are random), and so do the joins; by Hoeffding's bound the mean of those n t
+    errors passes U sqrt(2 t ln(2 / p) / n) with probability p = 1e-12 at most, twice that with the joins.  What
+    remains is in proportion to the small side s = 1 - a: 25 U of it a step from exponential and reciprocal, and its
+    sum over a span rounded at every step and every join, 25 U again; and 64 U for the last steps, up to 16 of them
+    with decays each rounded (4 U) on its own."""
+    import torch
+    assert (plan(b, t, d, kind, False), plan(b, t, d, kind, True)) == (fwd, bwd)
+    n, s = b * d, 1 / (1 + np.exp(z))
+    bound = ref.U * (2 * np.sqrt(2 * t * np.log(2e12) / n) + 50 * s * t + 64)
+    rng = np.random.default_rng(int(z * 8))
+    first = torch.from_numpy(rng.uniform(1, 2, (b, d)).astype(np.float32)).cuda()
+    gate = torch.full((d,), z, dtype=dt(kind), device="cuda").expand(b, t, d)
+    x = torch.zeros((d,), dtype=dt(kind), device="cuda").expand(b, t, d)
+    want = host(first) * np.exp(-t * np.log1p(np.exp(-z)))
+    y, h, saved = snn.leaky_scan(gate, x, first, logit=True, leaky=True, save=True)
+    assert abs((host(h) / want - 1).mean()) <= bound
+    _, _, dh0 = snn.leaky_scan_grad(gate, x, None, saved, dh=first, logit=True, leaky=True, need_gate=False, need_x=False)
+    assert abs((host(dh0) / want - 1).mean()) <= bound
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+def test_constant_logits_step_by_step(kind):
+    """The same a step a call, the state carried in place; 4,096 channels, 3,000 calls."""
+    import torch
+    z, b, t, d = 9.5, 4, 3000, 1024
+    bound = ref.U * (2 * np.sqrt(2 * t * np.log(2e12) / (b * d)) + 50 * t / (1 + np.exp(z)) + 64)
+    first = torch.rand(b, d, device="cuda", generator=torch.Generator("cuda").manual_seed(1)) + 1
+    gate, x = torch.full((b, 1, d), z, dtype=dt(kind), device="cuda"), torch.zeros(b, 1, d, dtype=dt(kind), device="cuda")
+    state, out = first.clone(), torch.empty_like(x)
+    for _ in range(t):
+        snn.leaky_scan(gate, x, state, logit=True, leaky=True, out=out, h_out=state)
+    want = host(first) * np.exp(-t * np.log1p(np.exp(-z)))
+    assert abs((host(state) / want - 1).mean()) <= bound
