@@ -445,8 +445,9 @@ int snn_embed_grad(const void* tokens, int32_t tok_type, int64_t n, const void* 
  * (offsets set): n_steps rows in all, sequence s the rows
  * [offsets[s], offsets[s + 1]) of every tensor (int64[n_seq + 1] in device
  * memory, ascending within [0, n_steps]; entries are clamped to that).  Rows
- * of no sequence are not read and not written.  A sequence may be empty: its
- * final state is its initial one.
+ * of no sequence, before the first one and behind the last, are not read, and
+ * not written either unless SNN_SCAN_ZERO asks for zeros there.  A sequence may
+ * be empty: its final state is its initial one.
  * Strides are any of which rows that are written do not overlap (time-major
  * rows too); what is only read may be broadcast by a stride of 0.  Outputs
  * must not overlap inputs, but for h below.
@@ -458,6 +459,7 @@ int snn_embed_grad(const void* tokens, int32_t tok_type, int64_t n, const void* 
 #define SNN_SCAN_LEAKY 2
 #define SNN_SCAN_CHANNEL 4
 #define SNN_SCAN_RASTER 8
+#define SNN_SCAN_ZERO 32 /* packed: rows of no sequence become zero in y, dgate and dx */
 typedef struct snn_scan {
     int32_t type;            /* SNN_F32 / SNN_BF16 / SNN_F16                     */
     int32_t flags;           /* SNN_SCAN_*                                       */
@@ -493,7 +495,7 @@ int snn_leaky_scan(const snn_scan* desc, const snn_rows* gate, const snn_rows* x
  * [n_channels], the sum over all steps of all sequences in an order that
  * depends on the sizes and lengths alone.  dx (nullable, NULL with SNN_SCAN_RASTER) and dh0
  * (nullable, f32 [n_seq, n_channels]) as their inputs; rows of no sequence are
- * not written.  saved is what the forward call wrote.  work: as for
+ * not written, or zero with SNN_SCAN_ZERO.  saved is what the forward call wrote.  work: as for
  * snn_embed_grad, of the size that snn_leaky_scan_grad_workspace says. */
 int snn_leaky_scan_grad_workspace(const snn_scan* desc, int64_t* bytes);
 int snn_leaky_scan_grad(const snn_scan* desc, const snn_rows* gate, const snn_rows* x,

@@ -11,8 +11,7 @@ template <typename T, int GM, bool RASTER, int V>
 __global__ void __launch_bounds__(128) k_scan_steps(const ScanArgs A) {
     using X = InWord<T, V, RASTER>;
     const int c = (int)(blockIdx.x * 128 + threadIdx.x) * V;
-    if (c >= A.D) return;
-    for (long long s = blockIdx.y; s < A.n_seq; s += gridDim.y) {
+    for (long long s = blockIdx.y; s < A.n_seq && c < A.D; s += gridDim.y) {
         const Span sp = span_of(A, s);
         constexpr bool LO = is_logit<GM>;
         Decay<V, LO> d;
@@ -54,6 +53,13 @@ __global__ void __launch_bounds__(128) k_scan_steps(const ScanArgs A) {
         }
         if (A.h) store_f32<V>(A.h + s * A.D + c, h);
     }
+    if (A.zero) zero_rest<T>(A, A.y, (long long)blockIdx.y * gridDim.x + blockIdx.x, (long long)gridDim.x * gridDim.y);
+}
+
+// the same rows where there is no sequence at all
+template <typename T>
+__global__ void __launch_bounds__(128) k_scan_zero(const ScanArgs A, Rows r) {
+    zero_rest<T>(A, r, blockIdx.x, gridDim.x);
 }
 
 // dgate of a channel gate: the CTAs' sums, every eighth by one warp
@@ -123,7 +129,7 @@ __global__ void k_scan_join(const ScanArgs A) {
 void check_desc(const snn_scan* d) {
     SNN_REQUIRE(d, SNN_ERR_ARG, "null scan description");
     SNN_REQUIRE(snnb::elem_type_ok(d->type), SNN_ERR_ARG, "scan: type must be SNN_F32, SNN_BF16 or SNN_F16");
-    SNN_REQUIRE((d->flags & ~(SNN_SCAN_LOGIT | SNN_SCAN_LEAKY | SNN_SCAN_CHANNEL | SNN_SCAN_RASTER)) == 0,
+    SNN_REQUIRE((d->flags & ~(SNN_SCAN_LOGIT | SNN_SCAN_LEAKY | SNN_SCAN_CHANNEL | SNN_SCAN_RASTER | SNN_SCAN_ZERO)) == 0,
                 SNN_ERR_ARG, "scan: unknown flags");
     SNN_REQUIRE(d->n_seq >= 0 && d->n_seq < (1ll << 31), SNN_ERR_ARG, "scan: n_seq must lie in [0, 2^31)");
     SNN_REQUIRE(d->n_channels >= 1 && d->n_channels < (1ll << 30), SNN_ERR_ARG,
@@ -170,6 +176,7 @@ ScanArgs base_args(const snn_scan* d, const snn_rows* gate, const snn_rows* x) {
     A.D = (int)d->n_channels;
     A.logit = (d->flags & SNN_SCAN_LOGIT) != 0;
     A.leaky = (d->flags & SNN_SCAN_LEAKY) != 0;
+    A.zero = d->offsets && (d->flags & SNN_SCAN_ZERO) != 0;
     const int size = snnb::elem_size(d->type);
     if (d->flags & SNN_SCAN_CHANNEL) {
         SNN_REQUIRE(gate && gate->data && (uintptr_t)gate->data % 4 == 0, SNN_ERR_ARG, "scan: null or misaligned gate");
@@ -275,6 +282,15 @@ void run_plan(const snn_scan* d, int words, const Plan& p, void* work, ScanArgs&
     });
 }
 
+// no sequence: all rows of r are rows of no sequence
+void zero_rows(const snn_scan* d, const ScanArgs& A, const Rows& r, cudaStream_t st) {
+    if (!A.zero || !r.p || d->n_steps == 0) return;
+    snnb::with_elem(d->type, [&](auto t) {
+        k_scan_zero<decltype(t)><<<(unsigned)std::min<int64_t>(d->n_steps, 8 * SMS), 128, 0, st>>>(A, r);
+    });
+    SNN_CUDA(cudaGetLastError());
+}
+
 // whether r's rows are words of `bytes` from the first element on
 bool fits(const Rows& r, int size, int bytes) {
     return (uintptr_t)r.p % bytes == 0 && r.ss * size % bytes == 0 && r.st * size % bytes == 0;
@@ -308,9 +324,10 @@ int64_t leaky_scan_workspace(const snn_scan* d, bool grad) {
 void leaky_scan(const snn_scan* d, const snn_rows* gate, const snn_rows* x, const float* h0,
                 const snn_rows* y, float* h, float* saved, void* work, int64_t work_bytes, cudaStream_t st) {
     check_desc(d);
-    if (d->n_seq == 0) return;
+    if (d->n_seq == 0 && !(d->offsets && (d->flags & SNN_SCAN_ZERO))) return;
     ScanArgs A = base_args(d, gate, x);
     A.y = rows_of(d, y, "y", d->n_channels, elem_size(d->type), true);
+    if (d->n_seq == 0) return zero_rows(d, A, A.y, st);
     check_states({h0, h, saved});
     A.h0 = h0;
     A.h = h;
@@ -357,11 +374,11 @@ void leaky_scan_grad(const snn_scan* d, const snn_rows* gate, const snn_rows* x,
     if (d->n_seq == 0) {
         if (channel && dgate && dgate->data)
             SNN_CUDA(cudaMemsetAsync(dgate->data, 0, (size_t)d->n_channels * 4, st));
-        return;
+        if (!(d->offsets && (d->flags & SNN_SCAN_ZERO))) return;
     }
-    SNN_REQUIRE(saved, SNN_ERR_ARG, "scan: null saved");
-    ScanArgs A = base_args(d, gate, x);
     const int size = elem_size(d->type);
+    SNN_REQUIRE(saved || d->n_seq == 0, SNN_ERR_ARG, "scan: null saved");
+    ScanArgs A = base_args(d, gate, x);
     check_states({saved, dh, dh0});
     A.saved = const_cast<float*>(saved);
     A.dh = dh;
@@ -373,6 +390,11 @@ void leaky_scan_grad(const snn_scan* d, const snn_rows* gate, const snn_rows* x,
         A.dgate = {dgate->data, 0, 0};
     } else if (dgate) {
         A.dgate = rows_of(d, dgate, "dgate", d->n_channels, size, true);
+    }
+    if (d->n_seq == 0) {
+        zero_rows(d, A, A.dx, st);
+        if (!channel) zero_rows(d, A, A.dgate, st);
+        return;
     }
     const Rows none = {nullptr, 0, 0};
     const int words = copy_words(d, {channel ? none : A.gate, d->flags & SNN_SCAN_RASTER ? none : A.x, A.y},

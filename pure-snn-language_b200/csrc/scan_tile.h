@@ -30,6 +30,7 @@ struct ScanArgs {
     const int64_t* off;
     long long n_seq;
     int n_steps, D, logit, leaky;
+    int zero;  // rows of no sequence become zero in what is written
     Rows gate, x, y, dgate, dx;
     const float* h0;
     float* h;
@@ -112,6 +113,19 @@ __device__ __forceinline__ Span chunk_at(const ScanArgs& A, long long j, long lo
 }
 __device__ __forceinline__ long long row_at(const ScanArgs& A, const Rows& r, long long s, const Span& sp, long long t) {
     return A.off ? (sp.begin + t) * r.st : s * r.ss + t * r.st;
+}
+
+// Rows of no sequence (before the first one, behind the last) of what a call
+// writes, one CTA of n a row: zero.  The kernels do it behind their steps, where
+// without such rows it costs two loads (a launch of its own 2 us).
+template <typename T>
+__device__ __forceinline__ void zero_rest(const ScanArgs& A, const Rows& r, long long cta, long long n) {
+    const long long b = min(max((long long)A.off[0], 0ll), (long long)A.n_steps);
+    const long long e = min(max((long long)A.off[A.n_seq], b), (long long)A.n_steps);
+    for (long long i = cta; i < b + A.n_steps - e; i += n) {
+        T* p = reinterpret_cast<T*>(r.p) + (i < b ? i : e + i - b) * r.st;
+        for (int c = threadIdx.x; c < A.D; c += blockDim.x) p[c] = from_f32<T>(0.0f);
+    }
 }
 
 // V values side by side; pairs go through the packed f32 instructions
@@ -863,6 +877,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
         copy_wait<0>();
         __syncwarp();
     }
+    if (A.zero) zero_rest<T>(A, A.y, blockIdx.x, gridDim.x);
 }
 
 // The gradient runs from the last tile to the first.  With r the gradient that
@@ -1135,6 +1150,10 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
         }
         copy_wait<0>();
         __syncwarp();
+    }
+    if (A.zero) {
+        if (A.dx.p) zero_rest<T>(A, A.dx, blockIdx.x, gridDim.x);
+        if (!PC && A.dgate.p) zero_rest<T>(A, A.dgate, blockIdx.x, gridDim.x);
     }
     if (PC && A.part) {
         Vec<V> t = sum;

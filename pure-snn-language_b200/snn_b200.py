@@ -31,7 +31,7 @@ MODEL_STAGE2E, MODEL_STAGE0, MODEL_PROP = 0, 1, 2
 PROP_PLAIN, PROP_STDP, PROP_STP = 0, 1, 2
 PRESET_REF, PRESET_BASELINE = 0, 1
 CORPUS_TEXT_FILTER = 1
-SCAN_LOGIT, SCAN_LEAKY, SCAN_CHANNEL, SCAN_RASTER = 1, 2, 4, 8
+SCAN_LOGIT, SCAN_LEAKY, SCAN_CHANNEL, SCAN_RASTER, SCAN_ZERO = 1, 2, 4, 8, 32
 FMT_NATIVE, FMT_SNN2_V1, FMT_SCKP_V2, FMT_RAW_F32 = 0, 1, 2, 3
 
 STATE = {
@@ -394,8 +394,9 @@ def _scan_rows(t, name, shape, dtype):
     return _ROWS.pack(t.data_ptr(), st[0], st[-2])
 
 
-def _scan_args(gate, x, logit, leaky, offsets, dtype):
-    """(snn_scan, gate rows, x rows, dtype of y, its shape, the states' shape, _scan_sizes)"""
+def _scan_args(gate, x, logit, leaky, offsets, dtype, zero):
+    """(snn_scan, gate rows, x rows, dtype of y, its shape, the states' shape, _scan_sizes); zero: rows of no
+    sequence become zero in what the call writes"""
     if _T is None:
         _torch()
     dev, xt, shape = x.device, x.dtype, x.shape
@@ -427,6 +428,8 @@ def _scan_args(gate, x, logit, leaky, offsets, dtype):
         _require(offsets.dtype == _T.int64 and offsets.dim() == 1 and offsets.is_contiguous()
                  and offsets.numel() >= 1, "offsets must be contiguous int64 [sequences + 1]")
         n_seq, off = offsets.numel() - 1, offsets.data_ptr()
+        if zero:
+            flags |= SCAN_ZERO
     if gate.dim() == 1:
         _require(gate.shape[0] == d and gate.dtype == _T.float32 and gate.is_contiguous(),
                  "a gate per channel must be contiguous float32 [channels]")
@@ -472,9 +475,10 @@ def leaky_scan(gate, x, h0=None, logit=False, leaky=False, offsets=None, dtype=N
     [sequences, channels] (default zeros).  Returns (y, h), h the float32
     states after the last steps; with save=True also what leaky_scan_grad
     needs.  `out` takes y; `h_out` takes h and may be h0, so that a stream of
-    single steps keeps its state in place.  Rows of no sequence are not
-    written: in a new y they hold what the memory held."""
-    desc, g, xr, dtype, shape, state, sizes = _scan_args(gate, x, logit, leaky, offsets, dtype)
+    single steps keeps its state in place.  Rows of no sequence (before
+    offsets[0], from offsets[-1] on) are zero in a new y and not written in
+    `out`.  autograd does not see this call: leaky_scan_grad is the gradient."""
+    desc, g, xr, dtype, shape, state, sizes = _scan_args(gate, x, logit, leaky, offsets, dtype, out is None)
     dev = x.device
     if out is None:
         out = _new(dev, stream, shape, dtype)
@@ -507,10 +511,11 @@ def leaky_scan_grad(gate, x, dy, saved, dh=None, logit=False, leaky=False, offse
     None where it is not needed (dx of a raster never is).  gate, x, logit,
     leaky and offsets as in the forward call with save=True, `saved` its
     result.  dgate has gate's shape and dtype (a gate per channel: the sum over
-    all steps), dx x's, dh0 is float32 [sequences, channels]."""
+    all steps), dx x's, dh0 is float32 [sequences, channels].  Rows of no
+    sequence have the gradient 0."""
     raster = not x.dtype.is_floating_point
     desc, g, xr, dtype, shape, state, sizes = _scan_args(
-        gate, x, logit, leaky, offsets, dy.dtype if raster and dy is not None else None)
+        gate, x, logit, leaky, offsets, dy.dtype if raster and dy is not None else None, True)
     dev = x.device
     if dy is None and dh is None:
         raise SnnError(1, "neither dy nor dh is given")

@@ -4,7 +4,7 @@ import pytest
 
 import leaky_ref as ref
 import snn_b200 as snn
-from test_leaky_scan import dt, host
+from test_leaky_scan import dt, gate_of, host, make
 
 SMS = 148
 
@@ -103,3 +103,59 @@ def test_constant_logits_step_by_step(kind):
         snn.leaky_scan(gate, x, state, logit=True, leaky=True, out=out, h_out=state)
     want = host(first) * np.exp(-t * np.log1p(np.exp(-z)))
     assert abs((host(state) / want - 1).mean()) <= bound
+
+
+# ---- rows of no sequence -----------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("d", [1, 33, 64])
+@pytest.mark.parametrize("channel", [False, True])
+@pytest.mark.parametrize("lengths,before,behind", [
+    ([5, 0, 70], 0, 40), ([200], 7, 0), ([0, 0], 3, 20), ([], 0, 30), ([300, 1, 40], 33, 1000), ([1] * 40, 5, 2),
+    ([13000, 14000], 9, 500)])
+def test_rows_of_no_sequence_have_no_gradient(kind, d, channel, lengths, before, behind, monkeypatch):
+    """New results are made in memory that holds NaN: what no sequence covers is zero in them."""
+    import torch
+    new = snn._new
+
+    def dirty(*a):
+        v = new(*a)
+        return v.fill_(float("nan")) if v.dtype.is_floating_point else v
+
+    rng = np.random.default_rng(len(lengths))
+    off = np.cumsum([before] + lengths)
+    rows, b = int(off[-1]) + behind, len(lengths)
+    gate = gate_of(rng, (d,), "f32", True) if channel else gate_of(rng, (rows, d), kind, True)
+    x, dy = make(rng, (rows, d), kind), make(rng, (rows, d), kind)
+    out = torch.full_like(x, 7.0)
+    how = dict(logit=True, leaky=True, offsets=torch.from_numpy(off).cuda())
+    end = rows - behind
+    torch.cuda.synchronize()
+    monkeypatch.setattr(snn, "_new", dirty)
+    y, h, saved = snn.leaky_scan(gate, x, save=True, **how)
+    dgate, dx, dh0 = snn.leaky_scan_grad(gate, x, dy, saved, **how)
+    for v in (y, dx) if channel else (y, dx, dgate):
+        assert (v[:before] == 0).all() and (v[end:] == 0).all() and torch.isfinite(v).all()
+    assert torch.isfinite(dgate).all() and torch.isfinite(dh0).all()
+    y2, _ = snn.leaky_scan(gate, x, out=out, **how)  # a given one keeps them
+    assert torch.equal(y2[before:end], y[before:end]) and (out[:before] == 7).all() and (out[end:] == 7).all()
+
+
+@pytest.mark.gpu
+def test_padded_rows_into_the_embedding_gradient(monkeypatch):
+    """A padded packed batch through drive and scan: the padding adds nothing to the table's gradient."""
+    import torch
+    rng = np.random.default_rng(3)
+    tok = torch.from_numpy(rng.integers(0, 256, 500).astype(np.uint8)).cuda()
+    table, dy = make(rng, (256, 40), "f32"), make(rng, (500, 40), "f32")
+    off, tau = torch.tensor([0, 100, 380], device="cuda"), make(rng, (40,), "f32", 1.0, 2.0)
+    x = snn.embed(tok, table)
+    new, how = snn._new, dict(logit=True, leaky=True, offsets=off)
+    _, _, saved = snn.leaky_scan(tau, x, save=True, **how)
+    monkeypatch.setattr(snn, "_new", lambda *a: new(*a).fill_(7))
+    _, dx, _ = snn.leaky_scan_grad(tau, x, dy, saved, **how)
+    got = snn.embed_grad(tok, dx, 256)
+    dx[380:] = 0  # the order of the sums goes by the sizes: the same call without what lies in the padding
+    assert torch.equal(got, snn.embed_grad(tok, dx, 256))
+    want, bound = ref.embed_grad(tok.cpu().numpy()[:380], host(dx[:380]), 256, 1.0)
+    ref.close(host(got), want, bound, "f32")
