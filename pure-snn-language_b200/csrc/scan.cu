@@ -102,7 +102,7 @@ __global__ void k_scan_join(const ScanArgs A) {
 #pragma unroll 8
             for (int p = lo; p < min(hi, n - 1); ++p) {
                 const Vec<1> ma = {A.map_a[at(p)]}, ml = {KEEP ? A.map_l[at(p)] : 0.0f}, mh = {A.map_h[at(p)]};
-                h = mapped<KEEP>(ma, ml, h, mh);
+                h = KEEP ? plain<KEEP>(ma, ml, h, mh) : mapped<KEEP>(ma, ml, h, mh);
                 if (KEEP) span_times(ma, ml, a, l);
                 else a = vmul(ma, a);
             }
@@ -112,14 +112,14 @@ __global__ void k_scan_join(const ScanArgs A) {
         __syncthreads();
         if (c < A.D) {
             h.v[0] = !GRAD && A.h0 ? A.h0[s * A.D + c] : 0.0f;
-            for (int k = 0; k < g; ++k) h = mapped<KEEP>(sa[k][lane], sl[k][lane], h, sh[k][lane]);
+            for (int k = 0; k < g; ++k) h = KEEP ? plain<KEEP>(sa[k][lane], sl[k][lane], h, sh[k][lane]) : mapped<KEEP>(sa[k][lane], sl[k][lane], h, sh[k][lane]);
 #pragma unroll 8
             for (int p = lo; p < hi; ++p) {
                 const bool map = p < n - 1;
                 const Vec<1> ma = {map ? A.map_a[at(p)] : 0.0f}, ml = {map && KEEP ? A.map_l[at(p)] : 0.0f};
                 const Vec<1> mh = {map ? A.map_h[at(p)] : 0.0f};
                 A.map_h[at(p)] = h.v[0];
-                h = mapped<KEEP>(ma, ml, h, mh);
+                h = KEEP ? plain<KEEP>(ma, ml, h, mh) : mapped<KEEP>(ma, ml, h, mh);
             }
         }
         __syncthreads();
@@ -229,7 +229,7 @@ Plan plan_of(const snn_scan* d, bool grad) {
     if (mean_steps(d) >= (grad ? 6144 : 12288) && items <= (d->offsets ? (p.ctiles <= 8 ? 160 : 48) : grad ? 36 : 16)) {
         const int64_t warps = SMS * (grad ? 8 : 12) * (d->flags & SNN_SCAN_CHANNEL ? 2 : 1);
         const int64_t c = (rows * p.ctiles + warps - 1) / warps;
-        p.chunk = (int)std::max<int64_t>(128, (c + 15) / 16 * 16);
+        p.chunk = (int)std::max<int64_t>(96, (c + 15) / 16 * 16);
         p.n_chunks = rows / p.chunk + d->n_seq;
         p.workers = (int)std::min<int64_t>(p.n_chunks, std::max(32, 32 * SMS / p.ctiles));
         p.shape = 2;

@@ -172,13 +172,10 @@ __device__ __forceinline__ Vec<2> vadd(Vec<2> a, Vec<2> b) {
 // Rounded to f32 it is off by up to 2^-25, which a memory of 1 / s steps adds
 // up to 2^-25 / s of the state where the gate stays the same.  What the rounding
 // lost is therefore kept wherever a state is carried on:
-//  - per-channel and f32 gates keep it as `lo` (one more FMA a step), and so do
-//    single steps;
-//  - a warp by itself with 16-bit gates takes it into the next step's decay
-//    (decays_on): no registers, and no more than one rounding is ever open;
-//  - tiles of warps with 16-bit gates do without inside a warp's 16 (gradient
-//    8) steps, since the state goes from warp to warp by their maps, whose
-//    products keep it (span_lo).
+//  - as `lo` of the step (one more FMA) by per-channel and f32 gates, and by
+//    16-bit ones in single steps;
+//  - with 16-bit gates tiles do without inside a warp's 16 (gradient 8) steps:
+//    the state goes on by the map of these steps, whose product keeps it (span_lo).
 // (An infinite state times lo, or times what a product keeps, may be NaN:
 // infinities do not survive, they end as infinities or NaN.)
 template <int V, bool LO>
@@ -275,20 +272,6 @@ __device__ __forceinline__ void decays(const Vec<V>& z, Decay<V, LO>& d, Vec<V>&
             rest.v[k] = r;
         }
     }
-}
-// The same for 16-bit logits in the order of a recurrence: `left` is what the
-// steps before still have to lose, by which the decays' product over any number
-// of steps stays within one rounding.  After a NaN it is NaN, as the recurrence
-// is from there on; a decay below 1/2 drops it.
-template <int V>
-__device__ __forceinline__ void decays_on(const Vec<V>& z, Decay<V, false>& d, Vec<V>& rest, Vec<V>& left) {
-    const Vec<V> one = splat<V>(1.0f), minus = splat<V>(-1.0f);
-    logistic_fast(z, d.a, rest);
-    const Vec<V> t = vadd(rest, left), a = vfma(minus, t, one);
-    left = vfma(minus, vfma(minus, a, one), t);
-#pragma unroll
-    for (int k = 0; k < V; ++k)
-        if (d.a.v[k] >= 0.5f) d.a.v[k] = a.v[k];
 }
 // those of the per-channel gates c .. c + V
 template <int GM, int V, bool LO>
@@ -433,14 +416,19 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // store to the same shared-memory variable of CTA `rank` of the cluster
-template <int V>
-__device__ __forceinline__ void store_peer(Vec<V>* p, int rank, const Vec<V>& x) {
+template <typename T>
+__device__ __forceinline__ void store_peer(T* p, int rank, const T& x) {
     const unsigned a = (unsigned)__cvta_generic_to_shared(p);
     unsigned r;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
-#pragma unroll
-    for (int k = 0; k < V; ++k)
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(r + 4 * k), "f"(x.v[k]) : "memory");
+    float f[sizeof(T) / 4];
+    memcpy(f, &x, sizeof(T));
+    if constexpr (sizeof(T) == 16)
+        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(r), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]) : "memory");
+    else if constexpr (sizeof(T) == 8)
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(r), "f"(f[0]), "f"(f[1]) : "memory");
+    else
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(r), "f"(f[0]) : "memory");
 }
 
 // the product (a, l) of spans times one more, each with what it is off by
@@ -519,8 +507,9 @@ __device__ __forceinline__ bool powers(Powers<V, W>& P, const Decay<V, LO>& d, c
     return __syncthreads_or(!LO && overflowed(a));
 }
 template <int V>
-struct ClusterMaps {  // the tiles' maps of a round, by rank; two rounds
-    Vec<V> a[2][MAX_CLUSTER][32], l[2][MAX_CLUSTER][32], h[2][MAX_CLUSTER][32];
+struct ClusterMaps {  // the tiles' maps of a round, by rank: (a, l) and the end state; two rounds
+    Pair<V> p[2][MAX_CLUSTER][32];
+    alignas(4 * V) Vec<V> h[2][MAX_CLUSTER][32];
 };
 
 // Rows are staged in shared memory by asynchronous copies, each warp its own
@@ -729,7 +718,6 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
 #pragma unroll
         for (int k = 0; k < S; ++k) fetch(t1 + k * round, k);
         int slot = 0;
-        Vec<V> left = zero;
         for (int t0 = t1; t0 - t1 < to_t - from_t; t0 += round) {
             Decay<V, LO> d[PC ? 1 : L];
             Vec<V> u[L], a = one, ar = zero;  // the product of the decays and 1 - it
@@ -741,9 +729,8 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
                 Vec<V> f = factor;
                 if constexpr (!PC) {
                     const Vec<V> z = Unpack<T>::get(staged<COPY>(from + St::gate, i, lane, i & 1 ? g1 : g0));
-                    if constexpr (W == 1 && short_logit<T, GM>) decays_on(z, d[i], f, left);
-                    else decays<T, GM>(z, d[i], f);
-                    if (W > 1) {
+                    decays<T, GM>(z, d[i], f);
+                    if (W > 1 || short_logit<T, GM>) {
                         if (KEEP) ar = vfma(f, a, ar);
                         a = vmul(d[i].a, a);
                     }
@@ -789,46 +776,52 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
                         jl = KEEP ? prods[par][j][lane].a : zero;
                     }
                 };
-                // the state before this warp (h) and behind the tile (th); with a cluster those from zero
                 if (CL > 1) {
-                    Vec<V> th = zero, al, ta = one, tl = zero;  // the products of the warps before this one, of the tile
+                    // The warps before this one as one map: state from zero ht, product ta and 1 - it.  The last
+                    // warp, whose own steps end the tile, sends the tile's map to all.
+                    Vec<V> ht = zero, ta = one, tr = zero, tl = zero;
+                    if (!KEEP && over) {
+                        Vec<V> end = zero;
+                        join_spans<KEEP>(W, w, end, ht, map);
+                    }
 #pragma unroll
-                    for (int j = 0; j < W; ++j) {
-                        if (j == w) {
-                            h = th;
-                            a = ta;
-                            ar = tl;
-                        }
+                    for (int j = 0; j < W - 1; ++j) {
+                        if (j == w) break;
                         Vec<V> ja, jl, jh;
                         map(j, ja, jl, jh);
-                        th = plain<KEEP>(ja, jl, th, jh);
+                        if (KEEP || !over) ht = plain<KEEP>(ja, jl, ht, jh);
                         if constexpr (!PC) {
-                            if (KEEP) tl = vfma(prods[par][j][lane].b, ta, tl);
+                            if (KEEP) tr = vfma(prods[par][j][lane].b, ta, tr);
                             ta = vmul(ja, ta);
                         }
                     }
-                    if (!KEEP && over) {
-                        th = zero;
-                        join_spans<KEEP>(W, w, th, h, map);
-                    }
                     if constexpr (PC) {
-                        a = pw_s.p[w][lane].a;
-                        al = pw_s.p[w][lane].b;
-                        ta = pw_s.p[W][lane].a;
-                        tl = pw_s.p[W][lane].b;
+                        ta = pw_s.p[w][lane].a;
+                        tl = pw_s.p[w][lane].b;
                     } else {
-                        al = KEEP ? span_lo(a, ar) : zero;
-                        if (KEEP) tl = span_lo(ta, tl);
+                        if (KEEP) tl = span_lo(ta, tr);
                     }
-                    for (int r = w; r < CL; r += W) {
-                        if (!PC) store_peer<V>(&cm.a[par][rank][lane], r, ta);
-                        if (!PC && KEEP) store_peer<V>(&cm.l[par][rank][lane], r, tl);
-                        store_peer<V>(&cm.h[par][rank][lane], r, th);
+                    if (w == W - 1) {
+                        Vec<V> ja, jl, jh;
+                        map(w, ja, jl, jh);
+                        jh = KEEP ? plain<KEEP>(ja, jl, ht, jh) : mapped<KEEP>(ja, jl, ht, jh);
+                        if constexpr (!PC) {
+                            if (KEEP) tr = vfma(ar, ta, tr);
+                            ja = vmul(a, ta);
+                            jl = KEEP ? span_lo(ja, tr) : zero;
+                        }
+                        for (int r = 0; r < CL; ++r) {
+                            if (!PC) store_peer(&cm.p[par][rank][lane], r, Pair<V>{ja, jl});
+                            store_peer(&cm.h[par][rank][lane], r, jh);
+                        }
                     }
                     cluster_sync();
                     auto tile_map = [&](int r, Vec<V>& ra, Vec<V>& rl, Vec<V>& rh) {
-                        ra = PC ? ta : cm.a[par][r][lane];
-                        rl = PC || !KEEP ? tl : cm.l[par][r][lane];
+                        Pair<V> p;
+                        if constexpr (PC) p = pw_s.p[W][lane];
+                        else p = cm.p[par][r][lane];
+                        ra = p.a;
+                        rl = p.b;
                         rh = cm.h[par][r][lane];
                     };
                     const Vec<V> was = carry;
@@ -843,8 +836,8 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
                         carry = was;
                         join_spans<KEEP>(CL, rank, carry, in, tile_map);
                     }
-                    h = KEEP ? plain<KEEP>(a, al, in, h) : mapped<KEEP>(a, al, in, h);
-                } else if (!KEEP && over) {
+                    h = KEEP ? plain<KEEP>(ta, tl, in, ht) : mapped<KEEP>(ta, tl, in, ht);
+                } else if (!KEEP && over) {  // the state before this warp (h) and behind the tile (carry)
                     join_spans<KEEP>(W, w, carry, h, map);
                 } else {
 #pragma unroll
@@ -856,6 +849,12 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
                     }
                 }
                 par ^= 1;
+            }
+            if constexpr (W == 1 && short_logit<T, GM>) {
+                Vec<V> end = zero;
+#pragma unroll
+                for (int i = 0; i < L; ++i) end = d[i].step(end, u[i]);
+                carry = plain<KEEP>(a, span_lo(a, ar), carry, end);
             }
             const int n = min(L, to_t - t0);
             if (nl > 0 && n > 0) {
@@ -870,7 +869,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
                     qy += A.y.st;
                 }
                 if (A.h && t0 + n == sp.len) store_n<V>(A.h + s * A.D + c, h, nl);
-                if (W == 1) carry = h;
+                if (W == 1 && !short_logit<T, GM>) carry = h;
             }
             py += yjump;
         }
@@ -962,7 +961,6 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
 #pragma unroll
         for (int k = 0; k < S; ++k) fetch(t1 - k * round, k);
         int slot = 0, t0 = t1;
-        Vec<V> left = zero;
         for (int b = 0; b < tiles; b += CL, t0 -= round) {  // t0 before from_t: no tile left for this CTA
             const bool some = t0 >= from_t && t0 < to_t;
             Decay<V, LO> d[PC ? 1 : L];
@@ -972,12 +970,11 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
             const char* from = mine + slot * St::bytes;
             const Vec<V> h0 = reinterpret_cast<const Vec<V>*>(from + St::state)[lane];
 #pragma unroll
-            for (int i = L - 1; i >= 0; --i) {
+            for (int i = 0; i < L; ++i) {
                 if constexpr (!PC) {
                     const Vec<V> z = Unpack<T>::get(staged<COPY>(from + St::gate, i, lane, i & 1 ? g1 : g0));
-                    if constexpr (W == 1 && short_logit<T, GM>) decays_on(z, d[i], rest[i], left);
-                    else decays<T, GM>(z, d[i], rest[i]);
-                    if (W > 1) {
+                    decays<T, GM>(z, d[i], rest[i]);
+                    if (W > 1 || short_logit<T, GM>) {
                         if (KEEP) ar = vfma(rest[i], a, ar);
                         a = vmul(d[i].a, a);
                     }
@@ -1045,56 +1042,66 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
                         jl = back[par][W - 1 - j][lane].b;
                     }
                 };
-                Vec<V> hw = h0, ja[W], jl, jh;
-#pragma unroll
-                for (int j = 0; j < W; ++j) {
-                    if (j == w) h = hw;
-                    map(j, ja[j], jl, jh);
-                    if (j < W - 1) hw = vfma(ja[j], hw, jh);
-                }
-                // r behind this warp's steps (r) and before the tile's (tr); with a cluster those from zero
-                Vec<V> tr = CL > 1 ? zero : carry, al, ta = one, tl = zero;
-#pragma unroll
-                for (int j = 0; j < W; ++j) {
-                    if (W - 1 - j == w) {
-                        r = tr;
-                        a = ta;
-                        ar = tl;
-                    }
-                    Vec<V> jr, unused;
-                    map_back(j, unused, jl, jr);
-                    tr = plain<KEEP>(ja[W - 1 - j], jl, tr, jr);
-                    if constexpr (!PC && SH::clusters) {  // the products of the warps behind this one, of the tile
-                        if constexpr (RESTS) tl = vfma(rests[par][W - 1 - j][lane], ta, tl);
-                        ta = vmul(ja[W - 1 - j], ta);
-                    }
-                }
                 if (!KEEP && over) {
-                    hw = h0;
-                    join_spans<KEEP>(W, w, hw, h, map);
-                    tr = CL > 1 ? zero : carry;
-                    join_spans<KEEP>(W, W - 1 - w, tr, r, map_back);
+                    Vec<V> end = h0;
+                    join_spans<KEEP>(W, w, end, h, map);
+                } else {
+                    h = h0;
+#pragma unroll
+                    for (int j = 0; j < W - 1; ++j) {
+                        if (j == w) break;
+                        Vec<V> ja, jl, jh;
+                        map(j, ja, jl, jh);
+                        h = vfma(ja, h, jh);
+                    }
                 }
+                bool joined = false;
                 if constexpr (SH::clusters) if (CL > 1) {
                     __shared__ ClusterMaps<V> cm;
-                    if constexpr (PC) {
-                        a = pw_s.p[W - 1 - w][lane].a;
-                        al = pw_s.p[W - 1 - w][lane].b;
-                        ta = pw_s.p[W][lane].a;
-                        tl = pw_s.p[W][lane].b;
-                    } else {
-                        al = KEEP ? span_lo(a, ar) : zero;
-                        if (KEEP) tl = span_lo(ta, tl);
+                    // as in the forward pass, from the last warp to the first
+                    Vec<V> rt = zero, ta = one, tr = zero, tl = zero;
+                    if (!KEEP && over) {
+                        Vec<V> end = zero;
+                        join_spans<KEEP>(W, W - 1 - w, end, rt, map_back);
                     }
-                    for (int q = w; q < CL; q += W) {
-                        if (!PC) store_peer<V>(&cm.a[par][rank][lane], q, ta);
-                        if (!PC && KEEP) store_peer<V>(&cm.l[par][rank][lane], q, tl);
-                        store_peer<V>(&cm.h[par][rank][lane], q, tr);
+#pragma unroll
+                    for (int j = 0; j < W - 1; ++j) {
+                        if (W - 1 - j == w) break;
+                        Vec<V> ja, jl, jr;
+                        map_back(j, ja, jl, jr);
+                        if (KEEP || !over) rt = plain<KEEP>(ja, jl, rt, jr);
+                        if constexpr (!PC) {
+                            if constexpr (RESTS) tr = vfma(rests[par][W - 1 - j][lane], ta, tr);
+                            ta = vmul(ja, ta);
+                        }
+                    }
+                    if constexpr (PC) {
+                        ta = pw_s.p[W - 1 - w][lane].a;
+                        tl = pw_s.p[W - 1 - w][lane].b;
+                    } else {
+                        if (KEEP) tl = span_lo(ta, tr);
+                    }
+                    if (w == 0) {
+                        Vec<V> ja, jl, jr;
+                        map_back(W - 1, ja, jl, jr);
+                        jr = KEEP ? plain<KEEP>(ja, jl, rt, jr) : mapped<KEEP>(ja, jl, rt, jr);
+                        if constexpr (!PC) {
+                            if (KEEP) tr = vfma(ar, ta, tr);
+                            ja = vmul(a, ta);
+                            jl = KEEP ? span_lo(ja, tr) : zero;
+                        }
+                        for (int q = 0; q < CL; ++q) {
+                            if (!PC) store_peer(&cm.p[par][rank][lane], q, Pair<V>{ja, jl});
+                            store_peer(&cm.h[par][rank][lane], q, jr);
+                        }
                     }
                     cluster_sync();
                     auto tile_map = [&](int q, Vec<V>& qa, Vec<V>& ql, Vec<V>& qr) {
-                        qa = PC ? ta : cm.a[par][q][lane];
-                        ql = PC || !KEEP ? tl : cm.l[par][q][lane];
+                        Pair<V> p;
+                        if constexpr (PC) p = pw_s.p[W][lane];
+                        else p = cm.p[par][q][lane];
+                        qa = p.a;
+                        ql = p.b;
                         qr = cm.h[par][q][lane];
                     };
                     const Vec<V> was = carry;
@@ -1109,10 +1116,28 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
                         carry = was;
                         join_spans<KEEP>(CL, rank, carry, in, tile_map);
                     }
-                    r = KEEP ? plain<KEEP>(a, al, in, r) : mapped<KEEP>(a, al, in, r);
+                    r = KEEP ? plain<KEEP>(ta, tl, in, rt) : mapped<KEEP>(ta, tl, in, rt);
+                    joined = true;
                 }
-                if (CL == 1) carry = tr;
+                if (joined) {
+                } else if (!KEEP && over) {  // r behind this warp's steps (r) and before the tile's (carry)
+                    join_spans<KEEP>(W, W - 1 - w, carry, r, map_back);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < W; ++j) {
+                        if (W - 1 - j == w) r = carry;
+                        Vec<V> ja, jl, jr;
+                        map_back(j, ja, jl, jr);
+                        carry = plain<KEEP>(ja, jl, carry, jr);
+                    }
+                }
                 par ^= 1;
+            }
+            if constexpr (W == 1 && short_logit<T, GM>) {
+                Vec<V> end = zero;
+#pragma unroll
+                for (int i = L - 1; i >= 0; --i) end = d[i].times(vadd(o[i], end));
+                carry = plain<KEEP>(a, span_lo(a, ar), carry, end);
             }
             if (nl > 0 && some) {
                 // x becomes the derivative of h_t in a_t: h_{t-1}, or h_{t-1} - x_t
@@ -1143,7 +1168,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
                     qx -= A.dx.st;
                 }
                 if (t0 == 0 && A.dh0) store_n<V>(A.dh0 + s * A.D + c, r, nl);
-                if (W == 1) carry = r;
+                if (W == 1 && !short_logit<T, GM>) carry = r;
             }
             pdg -= gjump;
             pdx -= xjump;
@@ -1215,7 +1240,18 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_map(const ScanAr
         Vec<V> factor = splat<V>(1.0f);
         if (PC) channel_decays<GM>(A, c, nl, fixed, factor);
         const Vec<V> one = splat<V>(1.0f), zero = splat<V>(0.0f);
-        Vec<V> a = one, l = zero, h = zero, left = zero;
+        Vec<V> a = one, l = zero, h = zero;
+        auto product = [&](int n, Vec<V>& pa, Vec<V>& pr) {  // of n decays per channel, and 1 - it
+            pa = one;
+            pr = zero;
+#pragma unroll 1
+            for (int i = 0; i < n; ++i) {
+                if (KEEP) pr = vfma(factor, pa, pr);
+                pa = vmul(fixed.a, pa);
+            }
+        };
+        Vec<V> all_a, all_r;
+        if (PC) product(L, all_a, all_r);
         int slot = 0, t0 = t1;
         for (int b = 0; b < tiles; ++b, t0 += step) {
             Decay<V, LO> d[PC ? 1 : L];
@@ -1225,29 +1261,37 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_map(const ScanAr
             const char* from = rows + slot * St::bytes;
             const int n = min(L, to_t - t0);
 #pragma unroll
-            for (int k = 0; k < L; ++k) {
-                const int i = GRAD ? L - 1 - k : k;
+            for (int i = 0; i < L; ++i) {
                 Vec<V> f = factor;
                 if constexpr (!PC) {
                     const Vec<V> z = Unpack<T>::get(staged<COPY>(from + St::gate, i, lane, i & 1 ? g1 : g0));
-                    if constexpr (short_logit<T, GM>) decays_on(z, d[i], f, left);
-                    else decays<T, GM>(z, d[i], f);
+                    decays<T, GM>(z, d[i], f);
                 }
                 if constexpr (RASTER) u[i] = raster_values<V>(from + St::x, i, lane);
                 else u[i] = Unpack<T>::get(staged<COPY>(from + St::x, i, lane, i & 1 ? x1 : x0));
                 if (!in.p) u[i] = zero;
                 if (LEAKY && !GRAD) u[i] = vmul(f, u[i]);
-                if (i < n) {
+                if (!PC && i < n) {
                     if (KEEP) rr = vfma(f, ra, rr);
-                    ra = vmul(PC ? fixed.a : d[PC ? 0 : i].a, ra);
+                    ra = vmul(d[PC ? 0 : i].a, ra);
                 }
             }
             if (PC) d[0] = fixed;
             __syncwarp();
             fetch(t0 + S * step, slot);
             slot = slot + 1 == S ? 0 : slot + 1;
+            if (PC) {
+                if (n == L) {
+                    ra = all_a;
+                    rr = all_r;
+                } else {
+                    product(n, ra, rr);
+                }
+            }
             if (KEEP) span_times(ra, span_lo(ra, rr), a, l);
             else a = vmul(ra, a);
+            const Vec<V> before = h;
+            if (short_logit<T, GM>) h = zero;
             if (GRAD) {
                 if (A.dh && t0 + n == sp.len) {
                     const Vec<V> dh = load_n<V>(A.dh + s * A.D + c, nl);
@@ -1263,6 +1307,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_map(const ScanAr
                 for (int i = 0; i < L; ++i)
                     if (i < n) h = d[PC ? 0 : i].step(h, u[i]);
             }
+            if (short_logit<T, GM>) h = plain<KEEP>(ra, span_lo(ra, rr), before, h);
         }
         copy_wait<0>();
         __syncwarp();
