@@ -514,8 +514,10 @@ def leaky_scan_grad(gate, x, dy, saved, dh=None, logit=False, leaky=False, offse
     all steps), dx x's, dh0 is float32 [sequences, channels].  Rows of no
     sequence have the gradient 0."""
     raster = not x.dtype.is_floating_point
-    desc, g, xr, dtype, shape, state, sizes = _scan_args(
-        gate, x, logit, leaky, offsets, dy.dtype if raster and dy is not None else None, True)
+    kind = None  # a raster's gradients have dy's type, without dy that of a gate per step
+    if raster:
+        kind = dy.dtype if dy is not None else gate.dtype if gate.dim() > 1 else None
+    desc, g, xr, dtype, shape, state, sizes = _scan_args(gate, x, logit, leaky, offsets, kind, True)
     dev = x.device
     if dy is None and dh is None:
         raise SnnError(1, "neither dy nor dh is given")

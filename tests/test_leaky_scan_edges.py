@@ -159,3 +159,18 @@ def test_padded_rows_into_the_embedding_gradient(monkeypatch):
     assert torch.equal(got, snn.embed_grad(tok, dx, 256))
     want, bound = ref.embed_grad(tok.cpu().numpy()[:380], host(dx[:380]), 256, 1.0)
     ref.close(host(got), want, bound, "f32")
+
+
+# ---- rasters -----------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+def test_raster_gradient_of_the_last_state_alone(kind):
+    """Without dy the gradients' type is the gate's."""
+    import torch
+    rng = np.random.default_rng(2)
+    words = torch.from_numpy(rng.integers(-2 ** 31, 2 ** 31, (2, 50, 2)).astype(np.int32)).cuda()
+    gate, dh = gate_of(rng, (2, 50, 40), kind, False), make(rng, (2, 40), "f32")
+    _, _, saved = snn.leaky_scan(gate, words, dtype=dt(kind), save=True)
+    got = snn.leaky_scan_grad(gate, words, None, saved, dh=dh)
+    want = snn.leaky_scan_grad(gate, words, torch.zeros_like(gate), saved, dh=dh)
+    assert got[1] is None and torch.equal(got[0], want[0]) and torch.equal(got[2], want[2])
