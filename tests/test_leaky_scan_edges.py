@@ -4,7 +4,7 @@ import pytest
 
 import leaky_ref as ref
 import snn_b200 as snn
-from test_leaky_scan import dt, gate_of, host, make
+from test_leaky_scan import check, dt, gate_of, host, make, test_packed as packed_case
 
 SMS = 148
 
@@ -174,3 +174,74 @@ def test_raster_gradient_of_the_last_state_alone(kind):
     got = snn.leaky_scan_grad(gate, words, None, saved, dh=dh)
     want = snn.leaky_scan_grad(gate, words, torch.zeros_like(gate), saved, dh=dh)
     assert got[1] is None and torch.equal(got[0], want[0]) and torch.equal(got[2], want[2])
+
+
+# ---- every kernel, over several tiles and sequences ---------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("fwd,bwd,b,t", [("tiles", "tiles", 350, 300), ("tiles", "small", 600, 300),
+                                         ("warps", "warps", 1200, 40)])
+@pytest.mark.parametrize("kind,d", [("f32", 16), ("f32", 17), ("bf16", 16), ("bf16", 18), ("bf16", 31), ("f16", 16),
+                                    ("f16", 18), ("f16", 17)])
+@pytest.mark.parametrize("channel", [False, True])
+def test_several_tiles_a_cta(fwd, bwd, b, t, kind, d, channel):
+    """CTAs without a cluster that take several tiles and a part of one, from rows of 16-byte, 4-byte and odd words."""
+    assert (plan(b, t, d, kind, False), plan(b, t, d, kind, True)) == (fwd, bwd)
+    check(kind, b, t, d, channel)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,b,d", [("f32", 200, 2048), ("bf16", 170, 4096 - 31)])
+@pytest.mark.parametrize("channel", [False, True])
+def test_several_sequences_a_cta(kind, b, d, channel):
+    """More sequences than CTAs to take them (74 a tile of channels)."""
+    ctiles = -(-d // (32 if kind == "f32" else 64))
+    assert plan(b, 18, d, kind, False) == plan(b, 18, d, kind, True) == "warps" and 32 * SMS // ctiles < b
+    check(kind, b, 18, d, channel)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("channel", [False, True])
+@pytest.mark.parametrize("d", [33, 64])
+@pytest.mark.parametrize("b,long,fwd,bwd", [(100, 500, "cluster", "cluster"), (500, 140, "tiles", "small")])
+def test_many_packed_sequences_of_mixed_lengths(kind, channel, d, b, long, fwd, bwd):
+    """More packed sequences than are sorted by length."""
+    rng = np.random.default_rng(b)
+    lengths = (rng.integers(0, long, b) * (rng.random(b) < 0.8)).tolist()
+    lengths[7] = 2 * long
+    rows = sum(lengths) + 9
+    assert (plan(b, rows, d, kind, False, True), plan(b, rows, d, kind, True, True)) == (fwd, bwd)
+    packed_case(kind, channel, d, lengths)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fwd,bwd,b,t,d", SILENT)
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+def test_holding_resetting_and_nan_logits(fwd, bwd, b, t, d, kind):
+    """Logits of +inf hold a state exactly and give x no gradient, those of -inf pass x and its gradient; one -inf
+    forgets a state of 1e30; what a NaN spoils lies in its channel, in the outputs from its step on and in the
+    gradients up to it."""
+    import torch
+    assert (plan(b, t, d, kind, False), plan(b, t, d, kind, True)) == (fwd, bwd)
+    rng = np.random.default_rng(t)
+    gate, x, dy = (make(rng, (b, t, d), kind) for _ in range(3))
+    h0, dh = make(rng, (b, d), "f32"), make(rng, (b, d), "f32")
+    inf, at = float("inf"), t // 2
+    gate[:, :, 0], gate[:, :, 1] = inf, -inf
+    h0[:, 2] = 1e30
+    gate[:, at, 2] = -inf
+    gate[:, :at, 2] = 60.0
+    gate[b - 1, at, 3] = float("nan")
+    y, h, saved = snn.leaky_scan(gate, x, h0, logit=True, leaky=True, save=True)
+    assert torch.equal(h[:, 0], h0[:, 0]) and torch.equal(y[:, :, 0], h0[:, :1].to(dt(kind)).expand(b, t))
+    assert torch.equal(y[:, :, 1], x[:, :, 1]) and torch.equal(y[:, at, 2], x[:, at, 2])
+    assert torch.equal(torch.isfinite(y[:, at:, 2]), torch.ones_like(y[:, at:, 2], dtype=torch.bool))
+    spoilt = torch.isnan(y)
+    assert spoilt[b - 1, at:, 3].all() and spoilt.sum() == t - at
+    dgate, dx, dh0 = snn.leaky_scan_grad(gate, x, dy, saved, dh=dh, logit=True, leaky=True)
+    assert (dx[:, :, 0] == 0).all() and (dgate[:, :, :2] == 0).all() and (dh0[:, 1] == 0).all()
+    assert torch.equal(dx[:, :-1, 1], dy[:, :-1, 1])
+    spoilt = torch.isnan(dx)
+    assert spoilt[b - 1, :at + 1, 3].all() and spoilt.sum() == at + 1
+    spoilt = torch.isnan(dh0)
+    assert spoilt[b - 1, 3] and spoilt.sum() == 1

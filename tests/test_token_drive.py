@@ -137,6 +137,18 @@ def test_embed_strides(dim, width, at):
         snn.embed(t, table, dtype=torch.float32, out=out[:, at:at + dim])
 
 
+@pytest.mark.gpu
+def test_embed_into_an_output_of_another_type():
+    """`out` sets the type where dtype is not given; a given one has to be out's."""
+    import torch
+    rng = np.random.default_rng(12)
+    t, table = tokens_of(rng, 70, 300, "int32"), make(rng, (300, 24), "bf16")
+    out = torch.full((70, 24), 7.0, device="cuda")
+    assert snn.embed(t, table, out=out) is out and torch.equal(out, table[t.long()].float())
+    with pytest.raises(snn.SnnError):
+        snn.embed(t, table, dtype=torch.bfloat16, out=out)
+
+
 # ---- gradient --------------------------------------------------------------------
 GRAD = [
     (1, 1, 1, "uint8", "zipf"), (2, 256, 8, "uint8", "one"), (31, 2, 33, "int32", "each"),
