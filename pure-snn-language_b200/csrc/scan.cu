@@ -203,20 +203,23 @@ int64_t mean_steps(const snn_scan* d) { return d->offsets ? d->n_steps / std::ma
 // sequences may differ in length and end at different times: four times the
 // CTAs, so that the longest is split too (24 sequences of 40,003 rows by 1,001
 // channels, us by 2 / 4 / 8 CTAs an SM: forward 117 / 101 / 88, gradient 249 /
-// 177 / 160).
+// 177 / 160 before the last changes of the joins; by 8 now 87 / 156).  The mean
+// length stands for the longest: one sequence of 30,000 rows beside 255 of one
+// row, by 2,048 channels in bf16, goes to single warps and takes 1.2 ms forward,
+// where 16 of equal lengths take 0.14.
 // Where even clusters leave most SMs empty for long, the sequences are cut into
 // chunks: a first kernel reads them for their maps, a second joins the maps,
 // and the chunks run as sequences of their own.  That reads the inputs twice and
-// costs 22 us (gradient 28) however little there is, so it takes long
+// costs 20 us (gradient 27) however little there is, so it takes long
 // sequences of few (tile, sequence) items, by clusters / by chunks in us:
-//   1 x 50,000 x 64 f32 (2 items)           forward 102 / 32   gradient 214 / 39
-//   39 packed, 1,997,736 rows x 33 (39)               692 / 307          1406 / 588
-//   1 x 50,021 x 1,000 f32 (32)                       163 / 197           292 / 236
-//   2 packed, 20,106 x 59 f32 (4)                      34 / 32             65 / 42
-//   100 packed, 2,000,000 x 30, per channel (100)     465 / 169           972 / 372
-//   120 packed, 2,400,000 x 20 f32 (120)              391 / 292           793 / 529
-//   3 packed, 30,000 x 2,000 bf16 (96)                132 / 150           243 / 277
-//   1 x 2,000 x 512 bf16 (8)                           12 / 26             18 / 32
+//   1 x 50,000 x 64 f32 (2 items)           forward 105 / 32   gradient 225 / 41
+//   39 packed, 1,997,736 rows x 33, per channel (39)  674 / 286          1279 / 594
+//   1 x 50,021 x 1,000 f32 (32)                       166 / 200           293 / 241
+//   2 packed, 20,106 x 59 f32 (4)                      35 / 30             64 / 42
+//   100 packed, 2,000,000 x 30, per channel (100)     296 / 157           610 / 369
+//   120 packed, 2,400,000 x 20 f32, per channel (120) 251 / 154           525 / 246
+//   3 packed, 30,000 x 2,000 bf16 (96)                132 / 142           238 / 308
+//   1 x 2,000 x 512 bf16 (8)                           12 / 24             18 / 32
 Plan plan_of(const snn_scan* d, bool grad) {
     const int width = 128 / snnb::elem_size(d->type), tile = grad ? Bwd::TT : Fwd::TT;
     Plan p;
@@ -229,6 +232,8 @@ Plan plan_of(const snn_scan* d, bool grad) {
     if (mean_steps(d) >= (grad ? 6144 : 12288) && items <= (d->offsets ? (p.ctiles <= 8 ? 160 : 48) : grad ? 36 : 16)) {
         const int64_t warps = SMS * (grad ? 8 : 12) * (d->flags & SNN_SCAN_CHANNEL ? 2 : 1);
         const int64_t c = (rows * p.ctiles + warps - 1) / warps;
+        // (at least 96 steps: 1 x 20,000 x 300 bf16 gradient 65 us by 128, 59 by 96,
+        // 59 by 64; 1 x 50,000 x 64 f32 forward 34, 33, 38)
         p.chunk = (int)std::max<int64_t>(96, (c + 15) / 16 * 16);
         p.n_chunks = rows / p.chunk + d->n_seq;
         p.workers = (int)std::min<int64_t>(p.n_chunks, std::max(32, 32 * SMS / p.ctiles));
@@ -238,10 +243,10 @@ Plan plan_of(const snn_scan* d, bool grad) {
     const int64_t wanted = (d->offsets ? 8 : 2) * SMS, ctas = (int64_t)p.ctiles * p.workers;
     while (p.cluster < MAX_CLUSTER && ctas * p.cluster < wanted && (int64_t)tile * p.cluster < mean_steps(d))
         p.cluster *= 2;
-    // Without clusters: 16 x 4,096 x 2,048 in bf16 (512 items) gradient 332 us by
-    // tiles, 299 by the smaller ones, 375 by single warps (forward 158 / - / 178);
-    // a raster of 1,000 x 55,000 (1,719 items) forward 69 / - / 49, gradient 134 /
-    // - / 79.
+    // Without clusters: 16 x 4,096 x 2,048 in bf16 (512 items) gradient 335 us by
+    // tiles, 273 by the smaller ones, 376 by single warps (forward 163 / - / 172);
+    // a raster of 1,000 x 55,000 (1,719 items) forward 55 / - / 47, gradient 132 /
+    // - / 81.
     p.shape = p.cluster > 1 || ctas < 3 * SMS ? 0 : ctas < 8 * SMS ? 1 : 2;
     return p;
 }
@@ -295,7 +300,7 @@ void zero_rows(const snn_scan* d, const ScanArgs& A, const Rows& r, cudaStream_t
 bool fits(const Rows& r, int size, int bytes) {
     return (uintptr_t)r.p % bytes == 0 && r.ss * size % bytes == 0 && r.st * size % bytes == 0;
 }
-// The words that rows are staged in (see stage_rows); written rows go in 4-byte
+// The words that rows are staged in (see Rower); written rows go in 4-byte
 // words, or in the third form an element at a time.
 int copy_words(const snn_scan* d, std::initializer_list<Rows> in, std::initializer_list<Rows> out) {
     const int size = snnb::elem_size(d->type);
