@@ -438,9 +438,10 @@ int snn_embed_grad(const void* tokens, int32_t tok_type, int64_t n, const void* 
  * Spans of steps (up to a whole sequence) are joined by the products of their
  * decays: where decays beyond 1 take such a product past f32, a state of 0 stays
  * what the steps make of it, any other may turn infinite or NaN even if step by
- * step it would not.  The same holds for the gradients.  A logit's 1 - a keeps
- * its relative precision along the sequence, also where the logit stays the same
- * (rounded to f32, a decay of 1 - s would be off by up to 2^-25 / s of the state).
+ * step it would not.  The same holds for the gradients.  1 - a keeps its relative
+ * precision along the sequence, also where the gate stays the same (a decay or a
+ * product of decays of 1 - s rounded to f32 would put the state off by up to
+ * 2^-25 / s).
  * Layout: dense (offsets NULL): n_seq sequences of n_steps steps; packed
  * (offsets set): n_steps rows in all, sequence s the rows
  * [offsets[s], offsets[s + 1]) of every tensor (int64[n_seq + 1] in device

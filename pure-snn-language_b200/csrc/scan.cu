@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(256) k_scan_gate_sum(const ScanArgs A, int row
 // The states (GRAD: r) that the chunks of a sequence start from, from their
 // maps; in place of map_h.  A warp per consecutive part of the chunks joins its
 // maps, the parts' maps give each its first state.
-template <bool GRAD, bool KEEP>
+template <bool GRAD, bool KEEP, bool OVER>
 __global__ void k_scan_join(const ScanArgs A) {
     __shared__ Vec<1> sa[32][32], sl[32][32], sh[32][32];
     const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, groups = blockDim.x >> 5;
@@ -102,7 +102,7 @@ __global__ void k_scan_join(const ScanArgs A) {
 #pragma unroll 8
             for (int p = lo; p < min(hi, n - 1); ++p) {
                 const Vec<1> ma = {A.map_a[at(p)]}, ml = {KEEP ? A.map_l[at(p)] : 0.0f}, mh = {A.map_h[at(p)]};
-                h = KEEP ? plain<KEEP>(ma, ml, h, mh) : mapped<KEEP>(ma, ml, h, mh);
+                h = OVER ? mapped<KEEP>(ma, ml, h, mh) : plain<KEEP>(ma, ml, h, mh);
                 if (KEEP) span_times(ma, ml, a, l);
                 else a = vmul(ma, a);
             }
@@ -112,14 +112,14 @@ __global__ void k_scan_join(const ScanArgs A) {
         __syncthreads();
         if (c < A.D) {
             h.v[0] = !GRAD && A.h0 ? A.h0[s * A.D + c] : 0.0f;
-            for (int k = 0; k < g; ++k) h = KEEP ? plain<KEEP>(sa[k][lane], sl[k][lane], h, sh[k][lane]) : mapped<KEEP>(sa[k][lane], sl[k][lane], h, sh[k][lane]);
+            for (int k = 0; k < g; ++k) h = OVER ? mapped<KEEP>(sa[k][lane], sl[k][lane], h, sh[k][lane]) : plain<KEEP>(sa[k][lane], sl[k][lane], h, sh[k][lane]);
 #pragma unroll 8
             for (int p = lo; p < hi; ++p) {
                 const bool map = p < n - 1;
                 const Vec<1> ma = {map ? A.map_a[at(p)] : 0.0f}, ml = {map && KEEP ? A.map_l[at(p)] : 0.0f};
                 const Vec<1> mh = {map ? A.map_h[at(p)] : 0.0f};
                 A.map_h[at(p)] = h.v[0];
-                h = KEEP ? plain<KEEP>(ma, ml, h, mh) : mapped<KEEP>(ma, ml, h, mh);
+                h = OVER ? mapped<KEEP>(ma, ml, h, mh) : plain<KEEP>(ma, ml, h, mh);
             }
         }
         __syncthreads();
@@ -279,8 +279,9 @@ void run_plan(const snn_scan* d, int words, const Plan& p, void* work, ScanArgs&
             int groups = 1;
             while (groups < 32 && groups * 4 < mean) groups *= 2;
             const dim3 grid((unsigned)((d->n_channels + 31) / 32), (unsigned)std::min<int64_t>(d->n_seq, 65535));
-            if (A.logit) k_scan_join<GRAD, true><<<grid, 32 * groups, 0, st>>>(A);
-            else k_scan_join<GRAD, false><<<grid, 32 * groups, 0, st>>>(A);
+            if (A.logit) k_scan_join<GRAD, true, false><<<grid, 32 * groups, 0, st>>>(A);
+            else if (gm == GATE_VALUE && sizeof(T) == 2) k_scan_join<GRAD, false, true><<<grid, 32 * groups, 0, st>>>(A);
+            else k_scan_join<GRAD, true, true><<<grid, 32 * groups, 0, st>>>(A);
             SNN_CUDA(cudaGetLastError());  // the launch after it does not report this one
         }
         launch_tiles<GRAD, T>(gm, raster, words, false, p, A, st);

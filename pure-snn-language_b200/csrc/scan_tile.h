@@ -194,6 +194,11 @@ struct Decay<V, true> {
 };
 template <typename T, int GM>
 constexpr bool keeps_lo = GM == GATE_CHANNEL_LOGIT || (GM == GATE_LOGIT && sizeof(T) == 4);
+// The maps of spans keep what the product of their decays is off by (span_lo),
+// but for given decays of 16 bits: those are 1 - 2^-11 at most, whose memory of
+// 2,048 steps adds less than 2^-16 up.
+template <typename T, int GM>
+constexpr bool keeps_span = is_logit<GM> || per_channel<GM> || sizeof(T) == 4;
 // 16-bit logits
 template <typename T, int GM>
 constexpr bool short_logit = GM == GATE_LOGIT && sizeof(T) == 2;
@@ -203,13 +208,14 @@ constexpr bool short_logit = GM == GATE_LOGIT && sizeof(T) == 2;
 // 1, and 1 - a is known better than a: as r = the sum over the steps of (1 -
 // decay) times the product before it, each 1 - decay with its own relative
 // precision.  So l = (1 - a) - r where 1 - a is exact; where a span halves the
-// state, roundings of its own add up over few spans only, and l is 0.  Kept for
-// logits (KEEP); decays that are given are multiplied as they are.
-template <int V>
+// state, roundings of its own add up over few spans only, and l is 0.  (OVER:
+// decays may be beyond 1.)
+template <bool OVER, int V>
 __device__ __forceinline__ Vec<V> span_lo(const Vec<V>& a, const Vec<V>& r) {
     Vec<V> l;
 #pragma unroll
-    for (int k = 0; k < V; ++k) l.v[k] = a.v[k] >= 0.5f ? (1.0f - a.v[k]) - r.v[k] : 0.0f;
+    for (int k = 0; k < V; ++k)
+        l.v[k] = a.v[k] >= 0.5f && (!OVER || a.v[k] <= 2.0f) ? (1.0f - a.v[k]) - r.v[k] : 0.0f;
     return l;
 }
 // decay a = 1 / (1 + exp(-z)) and its rest 1 - a, each with its own relative
@@ -258,7 +264,7 @@ template <typename T, int GM, int V, bool LO>
 __device__ __forceinline__ void decays(const Vec<V>& z, Decay<V, LO>& d, Vec<V>& rest) {
     if constexpr (short_logit<T, GM>) {
         logistic_fast(z, d.a, rest);
-        const Vec<V> lo = span_lo(d.a, rest);
+        const Vec<V> lo = span_lo<false>(d.a, rest);
 #pragma unroll
         for (int k = 0; k < V; ++k) d.set_lo(k, lo.v[k]);
     } else {
@@ -395,7 +401,7 @@ struct Shape {
 using Fwd = Shape<8, 16, 2, 2>;
 using Bwd = Shape<8, 8, 3, 2>;
 // Decays per channel leave the forward pass registers for a third CTA: 80 a
-// thread, of which 16-bit forms spill 8 - 24 bytes (the gradient spills more and
+// thread, of which 16-bit forms spill 8 - 32 bytes (the gradient spills more and
 // loses by one: documents 171 -> 187 us).
 using FwdChannel = Shape<8, 16, 2, 3>;
 // Without clusters the gradient takes smaller CTAs, twice as many on an SM.
@@ -497,13 +503,13 @@ template <int V, int W, bool LO>
 __device__ __forceinline__ bool powers(Powers<V, W>& P, const Decay<V, LO>& d, const Vec<V>& rest, int steps, int w, int lane) {
     Vec<V> a = splat<V>(1.0f), r = splat<V>(0.0f), pa = a, pl = r;
     for (int i = 0; i < steps; ++i) {
-        if (LO) r = vfma(rest, a, r);
+        r = vfma(rest, a, r);
         a = vmul(d.a, a);
     }
-    const Vec<V> l = LO ? span_lo(a, r) : r;
+    const Vec<V> l = span_lo<!LO>(a, r);
     if (w == 0) P.p[0][lane] = {pa, pl};
     for (int j = 0; j <= w; ++j) span_times(a, l, pa, pl);
-    P.p[w + 1][lane] = {pa, LO ? pl : r};
+    P.p[w + 1][lane] = {pa, pl};
     return __syncthreads_or(!LO && overflowed(a));
 }
 template <int V>
@@ -656,7 +662,7 @@ struct Stage {
 template <typename SH, typename T, int GM, bool RASTER, bool LEAKY, int COPY>
 __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanArgs A) {
     constexpr int W = SH::W, L = SH::L, TT = SH::TT, S = SH::S, V = lane_channels<T>;
-    constexpr bool LO = keeps_lo<T, GM>, PC = per_channel<GM>, KEEP = is_logit<GM>;
+    constexpr bool LO = keeps_lo<T, GM>, PC = per_channel<GM>, KEEP = keeps_span<T, GM>, OVER = !is_logit<GM>;
     using St = Stage<GM, RASTER, COPY, L, V, false>;
     static_assert(L * V <= 32, "a lane holds one raster word");
     extern __shared__ __align__(16) char rows[];
@@ -745,9 +751,11 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
             slot = slot + 1 == S ? 0 : slot + 1;
             Vec<V> h = carry;
             if constexpr (W > 1) {
-                // (a, h) and (l, 1 - a) of the warps' maps; h alone where the products are fixed
-                __shared__ Pair<V> maps[PC ? 1 : 2][PC ? 1 : W][32], prods[PC ? 1 : 2][PC ? 1 : W][32];
-                __shared__ Vec<V> ends[PC ? 2 : 1][PC ? W : 1][32];
+                // (a, h), l and 1 - a of the warps' maps; h alone where the products are fixed.  (Words of which
+                // only a half is read would lie in half of the banks.)
+                constexpr int P2 = PC ? 1 : 2, PW = PC ? 1 : W, K2 = KEEP ? P2 : 1, KW = KEEP ? PW : 1;
+                __shared__ Pair<V> maps[P2][PW][32];
+                __shared__ Vec<V> los[K2][KW][32], rests[K2][KW][32], ends[PC ? 2 : 1][PC ? W : 1][32];
                 __shared__ ClusterMaps<V> cm;
                 h = zero;
 #pragma unroll
@@ -761,8 +769,11 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
                     __syncthreads();
                 } else {
                     maps[par][w][lane] = {a, h};
-                    if (KEEP) prods[par][w][lane] = {span_lo(a, ar), ar};
-                    if (KEEP) __syncthreads();
+                    if constexpr (KEEP) {
+                        los[par][w][lane] = span_lo<OVER>(a, ar);
+                        rests[par][w][lane] = ar;
+                    }
+                    if (!OVER) __syncthreads();
                     else over = __syncthreads_or(overflowed(a));
                 }
                 auto map = [&](int j, Vec<V>& ja, Vec<V>& jl, Vec<V>& jh) {
@@ -773,14 +784,15 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
                     } else {
                         ja = maps[par][j][lane].a;
                         jh = maps[par][j][lane].b;
-                        jl = KEEP ? prods[par][j][lane].a : zero;
+                        jl = zero;
+                        if constexpr (KEEP) jl = los[par][j][lane];
                     }
                 };
                 if (CL > 1) {
                     // The warps before this one as one map: state from zero ht, product ta and 1 - it.  The last
                     // warp, whose own steps end the tile, sends the tile's map to all.
                     Vec<V> ht = zero, ta = one, tr = zero, tl = zero;
-                    if (!KEEP && over) {
+                    if (OVER && over) {
                         Vec<V> end = zero;
                         join_spans<KEEP>(W, w, end, ht, map);
                     }
@@ -789,9 +801,9 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
                         if (j == w) break;
                         Vec<V> ja, jl, jh;
                         map(j, ja, jl, jh);
-                        if (KEEP || !over) ht = plain<KEEP>(ja, jl, ht, jh);
+                        if (!OVER || !over) ht = plain<KEEP>(ja, jl, ht, jh);
                         if constexpr (!PC) {
-                            if (KEEP) tr = vfma(prods[par][j][lane].b, ta, tr);
+                            if constexpr (KEEP) tr = vfma(rests[par][j][lane], ta, tr);
                             ta = vmul(ja, ta);
                         }
                     }
@@ -799,16 +811,16 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
                         ta = pw_s.p[w][lane].a;
                         tl = pw_s.p[w][lane].b;
                     } else {
-                        if (KEEP) tl = span_lo(ta, tr);
+                        if (KEEP) tl = span_lo<OVER>(ta, tr);
                     }
                     if (w == W - 1) {
                         Vec<V> ja, jl, jh;
                         map(w, ja, jl, jh);
-                        jh = KEEP ? plain<KEEP>(ja, jl, ht, jh) : mapped<KEEP>(ja, jl, ht, jh);
+                        jh = OVER ? mapped<KEEP>(ja, jl, ht, jh) : plain<KEEP>(ja, jl, ht, jh);
                         if constexpr (!PC) {
                             if (KEEP) tr = vfma(ar, ta, tr);
                             ja = vmul(a, ta);
-                            jl = KEEP ? span_lo(ja, tr) : zero;
+                            jl = KEEP ? span_lo<OVER>(ja, tr) : zero;
                         }
                         for (int r = 0; r < CL; ++r) {
                             if (!PC) store_peer(&cm.p[par][rank][lane], r, Pair<V>{ja, jl});
@@ -832,12 +844,12 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
                         tile_map(r, ra, rl, rh);
                         carry = plain<KEEP>(ra, rl, carry, rh);
                     }
-                    if (!KEEP && any_nan(carry)) {
+                    if (OVER && any_nan(carry)) {
                         carry = was;
                         join_spans<KEEP>(CL, rank, carry, in, tile_map);
                     }
-                    h = KEEP ? plain<KEEP>(ta, tl, in, ht) : mapped<KEEP>(ta, tl, in, ht);
-                } else if (!KEEP && over) {  // the state before this warp (h) and behind the tile (carry)
+                    h = OVER ? mapped<KEEP>(ta, tl, in, ht) : plain<KEEP>(ta, tl, in, ht);
+                } else if (OVER && over) {  // the state before this warp (h) and behind the tile (carry)
                     join_spans<KEEP>(W, w, carry, h, map);
                 } else {
 #pragma unroll
@@ -854,7 +866,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
                 Vec<V> end = zero;
 #pragma unroll
                 for (int i = 0; i < L; ++i) end = d[i].step(end, u[i]);
-                carry = plain<KEEP>(a, span_lo(a, ar), carry, end);
+                carry = plain<KEEP>(a, span_lo<OVER>(a, ar), carry, end);
             }
             const int n = min(L, to_t - t0);
             if (nl > 0 && n > 0) {
@@ -885,7 +897,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
 template <typename SH, typename T, int GM, bool RASTER, bool LEAKY, int COPY>
 __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const ScanArgs A) {
     constexpr int W = SH::W, L = SH::L, TT = SH::TT, S = SH::S, V = lane_channels<T>;
-    constexpr bool LO = keeps_lo<T, GM>, PC = per_channel<GM>, KEEP = is_logit<GM>;
+    constexpr bool LO = keeps_lo<T, GM>, PC = per_channel<GM>, KEEP = keeps_span<T, GM>, OVER = !is_logit<GM>;
     using St = Stage<GM, RASTER, COPY, L, V, true>;
     extern __shared__ __align__(16) char rows[];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -996,10 +1008,11 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
             slot = slot + 1 == S ? 0 : slot + 1;
             Vec<V> h = h0, r = carry;
             if constexpr (W > 1) {
-                // (a, h), (r, l) and 1 - a of the warps' maps; h and r where the products are fixed
-                constexpr bool RESTS = !PC && KEEP && SH::clusters;
-                __shared__ Pair<V> maps[PC ? 1 : 2][PC ? 1 : W][32], back[2][W][32];
-                __shared__ Vec<V> ends[PC ? 2 : 1][PC ? W : 1][32], rests[RESTS ? 2 : 1][RESTS ? W : 1][32];
+                // (a, h), (r, l) and 1 - a of the warps' maps; h and r where that is all
+                constexpr bool PAIR = KEEP && !PC, RESTS = PAIR && SH::clusters;
+                __shared__ Pair<V> maps[PC ? 1 : 2][PC ? 1 : W][32], back[PAIR ? 2 : 1][PAIR ? W : 1][32];
+                __shared__ Vec<V> ends[PC ? 2 : 1][PC ? W : 1][32], rs[PAIR ? 1 : 2][PAIR ? 1 : W][32];
+                __shared__ Vec<V> rests[RESTS ? 2 : 1][RESTS ? W : 1][32];
                 h = r = zero;
 #pragma unroll
                 for (int i = 0; i < L; ++i) {
@@ -1012,13 +1025,14 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
                 }
                 if constexpr (PC) {
                     ends[par][w][lane] = h;
-                    back[par][w][lane].a = r;
+                    rs[par][w][lane] = r;
                     __syncthreads();
                 } else {
                     maps[par][w][lane] = {a, h};
-                    back[par][w][lane] = {r, KEEP ? span_lo(a, ar) : zero};
+                    if constexpr (PAIR) back[par][w][lane] = {r, span_lo<OVER>(a, ar)};
+                    else rs[par][w][lane] = r;
                     if constexpr (RESTS) rests[par][w][lane] = ar;
-                    if (KEEP) __syncthreads();
+                    if (!OVER) __syncthreads();
                     else over = __syncthreads_or(overflowed(a));
                 }
                 // The states start anew in every tile: they do without l.
@@ -1033,16 +1047,22 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
                     }
                 };
                 auto map_back = [&](int j, Vec<V>& ja, Vec<V>& jl, Vec<V>& jr) {
-                    jr = back[par][W - 1 - j][lane].a;
+                    const int k = W - 1 - j;
                     if constexpr (PC) {
                         ja = pw_s.p[1][lane].a;
                         jl = pw_s.p[1][lane].b;
                     } else {
-                        ja = maps[par][W - 1 - j][lane].a;
-                        jl = back[par][W - 1 - j][lane].b;
+                        ja = maps[par][k][lane].a;
+                    }
+                    if constexpr (PAIR) {
+                        jr = back[par][k][lane].a;
+                        jl = back[par][k][lane].b;
+                    } else {
+                        jr = rs[par][k][lane];
+                        if (!PC) jl = zero;
                     }
                 };
-                if (!KEEP && over) {
+                if (OVER && over) {
                     Vec<V> end = h0;
                     join_spans<KEEP>(W, w, end, h, map);
                 } else {
@@ -1060,7 +1080,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
                     __shared__ ClusterMaps<V> cm;
                     // as in the forward pass, from the last warp to the first
                     Vec<V> rt = zero, ta = one, tr = zero, tl = zero;
-                    if (!KEEP && over) {
+                    if (OVER && over) {
                         Vec<V> end = zero;
                         join_spans<KEEP>(W, W - 1 - w, end, rt, map_back);
                     }
@@ -1069,7 +1089,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
                         if (W - 1 - j == w) break;
                         Vec<V> ja, jl, jr;
                         map_back(j, ja, jl, jr);
-                        if (KEEP || !over) rt = plain<KEEP>(ja, jl, rt, jr);
+                        if (!OVER || !over) rt = plain<KEEP>(ja, jl, rt, jr);
                         if constexpr (!PC) {
                             if constexpr (RESTS) tr = vfma(rests[par][W - 1 - j][lane], ta, tr);
                             ta = vmul(ja, ta);
@@ -1079,16 +1099,16 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
                         ta = pw_s.p[W - 1 - w][lane].a;
                         tl = pw_s.p[W - 1 - w][lane].b;
                     } else {
-                        if (KEEP) tl = span_lo(ta, tr);
+                        if (KEEP) tl = span_lo<OVER>(ta, tr);
                     }
                     if (w == 0) {
                         Vec<V> ja, jl, jr;
                         map_back(W - 1, ja, jl, jr);
-                        jr = KEEP ? plain<KEEP>(ja, jl, rt, jr) : mapped<KEEP>(ja, jl, rt, jr);
+                        jr = OVER ? mapped<KEEP>(ja, jl, rt, jr) : plain<KEEP>(ja, jl, rt, jr);
                         if constexpr (!PC) {
                             if (KEEP) tr = vfma(ar, ta, tr);
                             ja = vmul(a, ta);
-                            jl = KEEP ? span_lo(ja, tr) : zero;
+                            jl = KEEP ? span_lo<OVER>(ja, tr) : zero;
                         }
                         for (int q = 0; q < CL; ++q) {
                             if (!PC) store_peer(&cm.p[par][rank][lane], q, Pair<V>{ja, jl});
@@ -1112,15 +1132,15 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
                         tile_map(q, qa, ql, qr);
                         carry = plain<KEEP>(qa, ql, carry, qr);
                     }
-                    if (!KEEP && any_nan(carry)) {
+                    if (OVER && any_nan(carry)) {
                         carry = was;
                         join_spans<KEEP>(CL, rank, carry, in, tile_map);
                     }
-                    r = KEEP ? plain<KEEP>(ta, tl, in, rt) : mapped<KEEP>(ta, tl, in, rt);
+                    r = OVER ? mapped<KEEP>(ta, tl, in, rt) : plain<KEEP>(ta, tl, in, rt);
                     joined = true;
                 }
                 if (joined) {
-                } else if (!KEEP && over) {  // r behind this warp's steps (r) and before the tile's (carry)
+                } else if (OVER && over) {  // r behind this warp's steps (r) and before the tile's (carry)
                     join_spans<KEEP>(W, W - 1 - w, carry, r, map_back);
                 } else {
 #pragma unroll
@@ -1137,7 +1157,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
                 Vec<V> end = zero;
 #pragma unroll
                 for (int i = L - 1; i >= 0; --i) end = d[i].times(vadd(o[i], end));
-                carry = plain<KEEP>(a, span_lo(a, ar), carry, end);
+                carry = plain<KEEP>(a, span_lo<OVER>(a, ar), carry, end);
             }
             if (nl > 0 && some) {
                 // x becomes the derivative of h_t in a_t: h_{t-1}, or h_{t-1} - x_t
@@ -1199,7 +1219,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
 template <typename SH, typename T, int GM, bool RASTER, bool LEAKY, int COPY, bool GRAD>
 __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_map(const ScanArgs A) {
     constexpr int L = SH::L, S = SH::S, V = lane_channels<T>;
-    constexpr bool LO = keeps_lo<T, GM>, PC = per_channel<GM>, KEEP = is_logit<GM>;
+    constexpr bool LO = keeps_lo<T, GM>, PC = per_channel<GM>, KEEP = keeps_span<T, GM>, OVER = !is_logit<GM>;
     using St = Stage<GM, RASTER, COPY, L, V, false>;  // its x is dy for the gradient
     static_assert(SH::W == 1, "a warp by itself");
     extern __shared__ __align__(16) char rows[];
@@ -1288,7 +1308,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_map(const ScanAr
                     product(n, ra, rr);
                 }
             }
-            if (KEEP) span_times(ra, span_lo(ra, rr), a, l);
+            if (KEEP) span_times(ra, span_lo<OVER>(ra, rr), a, l);
             else a = vmul(ra, a);
             const Vec<V> before = h;
             if (short_logit<T, GM>) h = zero;
@@ -1307,7 +1327,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_map(const ScanAr
                 for (int i = 0; i < L; ++i)
                     if (i < n) h = d[PC ? 0 : i].step(h, u[i]);
             }
-            if (short_logit<T, GM>) h = plain<KEEP>(ra, span_lo(ra, rr), before, h);
+            if (short_logit<T, GM>) h = plain<KEEP>(ra, span_lo<OVER>(ra, rr), before, h);
         }
         copy_wait<0>();
         __syncwarp();

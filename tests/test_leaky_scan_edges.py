@@ -90,6 +90,32 @@ def test_constant_logits_keep_their_memory(fwd, bwd, b, t, d, kind, z):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fwd,bwd,b,t,d", KEPT)
+@pytest.mark.parametrize("kind,logit,channel", [("f32", False, False), ("f32", False, True), ("f32", True, True),
+                                                ("bf16", False, True), ("bf16", True, True)])
+@pytest.mark.parametrize("s", [7.1e-4, 1.3e-4, 1.7e-5])
+def test_constant_decays_keep_their_memory(fwd, bwd, b, t, d, kind, logit, channel, s):
+    """The same of decays 1 - s given in f32, exact or as logits, per step or per channel: with the same bound (a
+    given decay has no error of its own, one from a logit in f32 a smaller one)."""
+    import torch
+    assert (plan(b, t, d, kind, False), plan(b, t, d, kind, True)) == (fwd, bwd)
+    value = np.float32(np.log(1 / s - 1) if logit else 1 - s)
+    log_a = -np.log1p(np.exp(-np.float64(value))) if logit else np.log(np.float64(value))
+    bound = ref.U * (2 * np.sqrt(2 * t * np.log(2e12) / (b * d)) + 50 * s * t + 64)
+    rng = np.random.default_rng(int(1 / s))
+    first = torch.from_numpy(rng.uniform(1, 2, (b, d)).astype(np.float32)).cuda()
+    gate = torch.full((d,), float(value), device="cuda")
+    x = torch.zeros((d,), dtype=dt(kind), device="cuda").expand(b, t, d)
+    if not channel:
+        gate = gate.expand(b, t, d)
+    want = host(first) * np.exp(t * log_a)
+    y, h, saved = snn.leaky_scan(gate, x, first, logit=logit, leaky=True, save=True)
+    assert abs((host(h) / want - 1).mean()) <= bound
+    _, _, dh0 = snn.leaky_scan_grad(gate, x, None, saved, dh=first, logit=logit, leaky=True, need_gate=False, need_x=False)
+    assert abs((host(dh0) / want - 1).mean()) <= bound
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
 def test_constant_logits_step_by_step(kind):
     """The same a step a call, the state carried in place; 4,096 channels, 3,000 calls."""
