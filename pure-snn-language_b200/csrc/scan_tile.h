@@ -844,7 +844,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_tile(const ScanA
                         tile_map(r, ra, rl, rh);
                         carry = plain<KEEP>(ra, rl, carry, rh);
                     }
-                    if (OVER && any_nan(carry)) {
+                    if (OVER && __any_sync(~0u, any_nan(carry))) {
                         carry = was;
                         join_spans<KEEP>(CL, rank, carry, in, tile_map);
                     }
@@ -1132,7 +1132,7 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_grad_tile(const 
                         tile_map(q, qa, ql, qr);
                         carry = plain<KEEP>(qa, ql, carry, qr);
                     }
-                    if (OVER && any_nan(carry)) {
+                    if (OVER && __any_sync(~0u, any_nan(carry))) {
                         carry = was;
                         join_spans<KEEP>(CL, rank, carry, in, tile_map);
                     }

@@ -4,7 +4,7 @@ import pytest
 
 import leaky_ref as ref
 import snn_b200 as snn
-from test_leaky_scan import check, dt, gate_of, host, make, test_packed as packed_case
+from test_leaky_scan import check, dt, gate_of, host, make, same, test_packed as packed_case
 
 SMS = 148
 
@@ -271,3 +271,31 @@ def test_holding_resetting_and_nan_logits(fwd, bwd, b, t, d, kind):
     assert spoilt[b - 1, :at + 1, 3].all() and spoilt.sum() == at + 1
     spoilt = torch.isnan(dh0)
     assert spoilt[b - 1, 3] and spoilt.sum() == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("b,t,d", [(2, 400, 1100), (2, 150, 45), (500, 130, 33), (1, 13000, 33)])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("logit", [False, True])
+@pytest.mark.parametrize("channel", [False, True])
+def test_equal_calls_give_equal_bits(b, t, d, kind, logit, channel):
+    """Whatever other kernels left in shared memory, where the last tile's rows are not staged; decays below -1 among
+    them, whose states overflow."""
+    import torch
+    rng = np.random.default_rng(d)
+    gate = gate_of(rng, (d,) if channel else (b, t, d), "f32" if channel else kind, logit)
+    if not logit:
+        gate[..., 3] = -1.4375
+    x, dy = make(rng, (b, t, d), kind), make(rng, (b, t, d), kind)
+    how = dict(logit=logit, leaky=True)
+    junk, ends = torch.full((1024, 1024), float("nan"), device="cuda"), torch.tensor([0, 300, 1024], device="cuda")
+    first = None
+    for k in range(25):
+        if k % 5 == 0:
+            junk @ junk
+        else:
+            snn.leaky_scan(junk[:, :37], junk[:, :37], offsets=ends, logit=True)
+        y, h, saved = snn.leaky_scan(gate, x, save=True, **how)
+        got = (y, h) + snn.leaky_scan_grad(gate, x, dy, saved, **how)
+        first = first or got
+        assert all(same(p, q) for p, q in zip(got, first))
