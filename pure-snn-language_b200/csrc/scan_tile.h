@@ -1275,31 +1275,47 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_map(const ScanAr
         int slot = 0, t0 = t1;
         for (int b = 0; b < tiles; ++b, t0 += step) {
             Decay<V, LO> d[PC ? 1 : L];
-            Vec<V> u[L], ra = one, rr = zero;  // these steps' product of decays and 1 - it
+            Vec<V> u[L], f[PC ? 1 : L], ra = one, rr = zero;  // these steps' product of decays and 1 - it
+            f[0] = factor;
             copy_wait<S - 1>();
             __syncwarp();
             const char* from = rows + slot * St::bytes;
-            const int n = min(L, to_t - t0);
 #pragma unroll
             for (int i = 0; i < L; ++i) {
-                Vec<V> f = factor;
                 if constexpr (!PC) {
                     const Vec<V> z = Unpack<T>::get(staged<COPY>(from + St::gate, i, lane, i & 1 ? g1 : g0));
-                    decays<T, GM>(z, d[i], f);
+                    decays<T, GM>(z, d[i], f[i]);
                 }
                 if constexpr (RASTER) u[i] = raster_values<V>(from + St::x, i, lane);
                 else u[i] = Unpack<T>::get(staged<COPY>(from + St::x, i, lane, i & 1 ? x1 : x0));
                 if (!in.p) u[i] = zero;
-                if (LEAKY && !GRAD) u[i] = vmul(f, u[i]);
-                if (!PC && i < n) {
-                    if (KEEP) rr = vfma(f, ra, rr);
-                    ra = vmul(d[PC ? 0 : i].a, ra);
-                }
+                if (LEAKY && !GRAD) u[i] = vmul(f[PC ? 0 : i], u[i]);
             }
             if (PC) d[0] = fixed;
             __syncwarp();
             fetch(t0 + S * step, slot);
             slot = slot + 1 == S ? 0 : slot + 1;
+            const int n = min(L, to_t - t0);
+            const Vec<V> before = h;
+            if (short_logit<T, GM>) h = zero;
+            if (GRAD && A.dh && t0 + n == sp.len) {
+                const Vec<V> dh = load_n<V>(A.dh + s * A.D + c, nl);
+#pragma unroll
+                for (int i = 0; i < L; ++i)
+                    if (i == n - 1) u[i] = vadd(u[i], dh);
+            }
+#pragma unroll
+            for (int k = 0; k < L; ++k) {
+                const int i = GRAD ? L - 1 - k : k;
+                if (i < n) {
+                    if (GRAD) h = d[PC ? 0 : i].times(vadd(u[i], h));
+                    else h = d[PC ? 0 : i].step(h, u[i]);
+                    if constexpr (!PC) {
+                        if (KEEP) rr = vfma(f[i], ra, rr);
+                        ra = vmul(d[i].a, ra);
+                    }
+                }
+            }
             if (PC) {
                 if (n == L) {
                     ra = all_a;
@@ -1310,23 +1326,6 @@ __global__ void __launch_bounds__(SH::threads, SH::CTAS) k_scan_map(const ScanAr
             }
             if (KEEP) span_times(ra, span_lo<OVER>(ra, rr), a, l);
             else a = vmul(ra, a);
-            const Vec<V> before = h;
-            if (short_logit<T, GM>) h = zero;
-            if (GRAD) {
-                if (A.dh && t0 + n == sp.len) {
-                    const Vec<V> dh = load_n<V>(A.dh + s * A.D + c, nl);
-#pragma unroll
-                    for (int i = 0; i < L; ++i)
-                        if (i == n - 1) u[i] = vadd(u[i], dh);
-                }
-#pragma unroll
-                for (int i = L - 1; i >= 0; --i)
-                    if (i < n) h = d[PC ? 0 : i].times(vadd(u[i], h));
-            } else {
-#pragma unroll
-                for (int i = 0; i < L; ++i)
-                    if (i < n) h = d[PC ? 0 : i].step(h, u[i]);
-            }
             if (short_logit<T, GM>) h = plain<KEEP>(ra, span_lo<OVER>(ra, rr), before, h);
         }
         copy_wait<0>();
