@@ -203,23 +203,23 @@ int64_t mean_steps(const snn_scan* d) { return d->offsets ? d->n_steps / std::ma
 // sequences may differ in length and end at different times: four times the
 // CTAs, so that the longest is split too (24 sequences of 40,003 rows by 1,001
 // channels, us by 2 / 4 / 8 CTAs an SM: forward 117 / 101 / 88, gradient 249 /
-// 177 / 160 before the last changes of the joins; by 8 now 87 / 156).  The mean
+// 177 / 160, by 8 with the present joins 87 / 156).  The mean
 // length stands for the longest: one sequence of 30,000 rows beside 255 of one
 // row, by 2,048 channels in bf16, goes to single warps and takes 1.2 ms forward,
 // where 16 of equal lengths take 0.14.
 // Where even clusters leave most SMs empty for long, the sequences are cut into
 // chunks: a first kernel reads them for their maps, a second joins the maps,
 // and the chunks run as sequences of their own.  That reads the inputs twice and
-// costs 20 us (gradient 27) however little there is, so it takes long
+// costs 20 us (gradient 25) however little there is, so it takes long
 // sequences of few (tile, sequence) items, by clusters / by chunks in us:
-//   1 x 50,000 x 64 f32 (2 items)           forward 105 / 32   gradient 225 / 41
-//   39 packed, 1,997,736 rows x 33, per channel (39)  674 / 286          1279 / 594
-//   1 x 50,021 x 1,000 f32 (32)                       166 / 200           293 / 241
-//   2 packed, 20,106 x 59 f32 (4)                      35 / 30             64 / 42
-//   100 packed, 2,000,000 x 30, per channel (100)     296 / 157           610 / 369
-//   120 packed, 2,400,000 x 20 f32, per channel (120) 251 / 154           525 / 246
-//   3 packed, 30,000 x 2,000 bf16 (96)                132 / 142           238 / 308
-//   1 x 2,000 x 512 bf16 (8)                           12 / 24             18 / 32
+//   1 x 50,000 x 64 f32 (2 items)           forward 102 / 31   gradient 221 / 39
+//   39 packed, 1,997,736 rows x 33, per channel (39)  670 / 284          1267 / 592
+//   1 x 50,021 x 1,000 f32 (32)                       162 / 198           292 / 234
+//   2 packed, 20,106 x 59 f32 (4)                      33 / 29             61 / 39
+//   100 packed, 2,000,000 x 30, per channel (100)     285 / 162           605 / 373
+//   120 packed, 2,400,000 x 20 f32, per channel (120) 246 / 151           518 / 242
+//   3 packed, 30,000 x 2,000 bf16 (96)                131 / 141           238 / 280
+//   1 x 2,000 x 512 bf16 (8)                           12 / 23             16 / 29
 Plan plan_of(const snn_scan* d, bool grad) {
     const int width = 128 / snnb::elem_size(d->type), tile = grad ? Bwd::TT : Fwd::TT;
     Plan p;
