@@ -504,6 +504,88 @@ int snn_leaky_scan_grad(const snn_scan* desc, const snn_rows* gate, const snn_ro
                         const snn_rows* dgate, const snn_rows* dx, float* dh0, void* work,
                         int64_t work_bytes, void* stream);
 
+/* ---- norms of queries and keys, with the position rotation ----------------
+ * For every head x of a row (dim elements of queries or keys):
+ *   y = turn(x r w),   r = 1 / sqrt(mean x^2 + eps), with SNN_QK_UNIT the sum in
+ * place of the mean (rows of unit length, what snn_delta_scan wants of keys);
+ * turn rotates pairs of the first rot elements by positions[row] * freqs[pair]:
+ * pair j is (j, j + rot / 2), with SNN_QK_ADJACENT (2 j, 2 j + 1).  Angles are
+ * products in 64 bits; sums f32; y is rounded once.  Rows are n_seq x n_steps,
+ * positions (pos_type SNN_I32 or SNN_I64) [n_seq * n_steps] contiguous, freqs f32
+ * [rot / 2] in radians a position; both may be NULL where rot is 0.  w (f32 [dim],
+ * one for queries, one for keys) may be NULL: ones.  Heads of one row share its
+ * position.  q_heads or k_heads may be 0: that tensor is then not looked at.
+ * dim <= 512, rot even and <= dim.  Strides are any of which heads that are written
+ * do not overlap; outputs may be their own inputs (same data and strides), and
+ * must not overlap anything else. */
+#define SNN_QK_UNIT 1
+#define SNN_QK_ADJACENT 2
+typedef struct snn_qk {
+    int32_t type;            /* SNN_F32 / SNN_BF16 / SNN_F16                     */
+    int32_t flags;           /* SNN_QK_*                                         */
+    int64_t n_seq, n_steps;
+    int64_t q_heads, k_heads;
+    int64_t dim, rot;
+    int32_t pos_type;
+    float eps;
+} snn_qk;
+typedef struct snn_heads {   /* one tensor of rows of heads, unit element stride */
+    void* data;
+    int64_t seq_stride;      /* elements between sequences (dense)               */
+    int64_t step_stride;     /* elements between steps (rows)                    */
+    int64_t head_stride;     /* elements between heads                           */
+} snn_heads;
+int snn_qk_norm(const snn_qk* desc, const snn_heads* q, const snn_heads* k, const float* q_weight,
+                const float* k_weight, const void* positions, const float* freqs,
+                const snn_heads* yq, const snn_heads* yk, void* stream);
+
+/* Gradients of snn_qk_norm from those of its results: with z = turn^-1(dy),
+ * n = x r:  dw = sum over rows and heads of z n,
+ *           dx = r (z w - n sum(z w n) / dim)   (SNN_QK_UNIT: 1 for dim).
+ * dq, dk as q, k (they may be dyq, dyk or q, k themselves); dq_weight, dk_weight
+ * (f32 [dim], nullable) are summed in an order that depends on the sizes and
+ * alignment alone.  work: as for snn_embed_grad, of the size that
+ * snn_qk_norm_grad_workspace says; not needed without gradients of weights. */
+int snn_qk_norm_grad_workspace(const snn_qk* desc, int64_t* bytes);
+int snn_qk_norm_grad(const snn_qk* desc, const snn_heads* q, const snn_heads* k,
+                     const float* q_weight, const float* k_weight, const void* positions,
+                     const float* freqs, const snn_heads* dyq, const snn_heads* dyk,
+                     const snn_heads* dq, const snn_heads* dk, float* dq_weight, float* dk_weight,
+                     void* work, int64_t work_bytes, void* stream);
+
+/* ---- AdamW -------------------------------------------------------------------
+ * One step over many tensors, each of n elements in device memory (contiguous):
+ *   g' = grad_scale g,   m = beta1 m + (1 - beta1) g',   v = beta2 v + (1 - beta2) g'^2,
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps)
+ * in f32, one rounding an operation.  Parameters are f32; copy (nullable) takes them
+ * rounded to copy_type.  Gradients are of any element type; a tensor whose g is NULL or
+ * whose n is 0 is left alone.  bits = 32: m, v are f32.  bits = 8: m and the root
+ * of v are held as e4m3 values (a byte each) with f32 scales [ceil(n / 256)] for every 256
+ * elements, the largest magnitude / 448; a root above zero is held as 2^-9 of its
+ * scale at least.  step is counted from 1; with step_device (int64 in device memory)
+ * it is read there, so that a captured step counts on.  Tensors of a call must not
+ * overlap.  `tensors` is host memory, read before the call returns; the call is
+ * asynchronous, allocates nothing on the device and may be captured (a graph
+ * keeps the pointers and the other settings). */
+typedef struct snn_adamw_tensor {
+    float* p;
+    const void* g;
+    void* m;
+    void* v;
+    float* m_scale;
+    float* v_scale;
+    void* copy;
+    int64_t n;
+    int32_t g_type, copy_type;
+} snn_adamw_tensor;
+typedef struct snn_adamw_rule {
+    double lr, beta1, beta2, eps, weight_decay, grad_scale;
+    int64_t step;
+    const int64_t* step_device;
+} snn_adamw_rule;
+int snn_adamw(const snn_adamw_tensor* tensors, int64_t count, int32_t bits,
+              const snn_adamw_rule* rule, void* stream);
+
 /* Seeded synthetic UTF-8 byte stream: a fraction p_cjk of characters are
  * CJK code points U+4E00..U+9FFF drawn Zipf(zipf_s) by rank (rank -> code
  * point through a seeded permutation), 3 bytes each; the rest are ASCII

@@ -456,4 +456,34 @@ int snn_leaky_scan_grad(const snn_scan* desc, const snn_rows* gate, const snn_ro
     });
 }
 
+int snn_qk_norm(const snn_qk* desc, const snn_heads* q, const snn_heads* k, const float* q_weight,
+                const float* k_weight, const void* positions, const float* freqs, const snn_heads* yq,
+                const snn_heads* yk, void* stream) {
+    return guard_op([&] {
+        snnb::qk_norm(desc, q, k, q_weight, k_weight, positions, freqs, yq, yk, (cudaStream_t)stream);
+    });
+}
+
+int snn_qk_norm_grad_workspace(const snn_qk* desc, int64_t* bytes) {
+    return guard_op([&] {
+        SNN_REQUIRE(bytes, SNN_ERR_ARG, "null result");
+        *bytes = snnb::qk_norm_grad_workspace(desc);
+    });
+}
+
+int snn_qk_norm_grad(const snn_qk* desc, const snn_heads* q, const snn_heads* k, const float* q_weight,
+                     const float* k_weight, const void* positions, const float* freqs, const snn_heads* dyq,
+                     const snn_heads* dyk, const snn_heads* dq, const snn_heads* dk, float* dq_weight,
+                     float* dk_weight, void* work, int64_t work_bytes, void* stream) {
+    return guard_op([&] {
+        snnb::qk_norm_grad(desc, q, k, q_weight, k_weight, positions, freqs, dyq, dyk, dq, dk, dq_weight, dk_weight,
+                           work, work_bytes, (cudaStream_t)stream);
+    });
+}
+
+int snn_adamw(const snn_adamw_tensor* tensors, int64_t count, int32_t bits, const snn_adamw_rule* rule,
+              void* stream) {
+    return guard_op([&] { snnb::adamw(tensors, count, bits, rule, (cudaStream_t)stream); });
+}
+
 }  // extern "C"

@@ -128,4 +128,13 @@ void leaky_scan_grad(const snn_scan* desc, const snn_rows* gate, const snn_rows*
                      const snn_rows* dy, const float* dh, const snn_rows* dgate, const snn_rows* dx, float* dh0,
                      void* work, int64_t work_bytes, cudaStream_t stream);
 
+void qk_norm(const snn_qk* desc, const snn_heads* q, const snn_heads* k, const float* wq, const float* wk,
+             const void* positions, const float* freqs, const snn_heads* yq, const snn_heads* yk, cudaStream_t st);
+int64_t qk_norm_grad_workspace(const snn_qk* desc);
+void qk_norm_grad(const snn_qk* desc, const snn_heads* q, const snn_heads* k, const float* wq, const float* wk,
+                  const void* positions, const float* freqs, const snn_heads* dyq, const snn_heads* dyk,
+                  const snn_heads* dq, const snn_heads* dk, float* dwq, float* dwk, void* work, int64_t work_bytes,
+                  cudaStream_t st);
+void adamw(const snn_adamw_tensor* tensors, int64_t count, int32_t bits, const snn_adamw_rule* rule, cudaStream_t st);
+
 }  // namespace snnb

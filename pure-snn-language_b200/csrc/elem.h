@@ -1,7 +1,10 @@
 // elem.h - element types of the device-tensor operators: loads widened to f32,
 // stores rounded once (to nearest even).
 #pragma once
+#include <algorithm>
 #include <atomic>
+#include <utility>
+#include <vector>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "common.h"
@@ -26,6 +29,18 @@ void with_elem(int32_t type, F&& f) {
     else if (type == SNN_BF16) f(__nv_bfloat16());
     else if (type == SNN_F16) f(__half());
     else throw Error(SNN_ERR_ARG, "element type must be SNN_F32, SNN_BF16 or SNN_F16");
+}
+
+// Whether runs of `width` elements, one for each index of dimensions {count, stride},
+// lie apart (each stride clears what the smaller ones span)
+inline bool apart(std::vector<std::pair<int64_t, int64_t>> dims, int64_t width) {
+    std::sort(dims.begin(), dims.end(), [](auto& a, auto& b) { return a.second < b.second; });
+    for (const auto& [count, stride] : dims) {
+        if (count <= 1) continue;
+        if (stride < width) return false;
+        width += (count - 1) * stride;
+    }
+    return true;
 }
 
 // the current device's multiprocessors (looked up once per device)

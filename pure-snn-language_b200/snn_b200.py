@@ -31,6 +31,7 @@ MODEL_STAGE2E, MODEL_STAGE0, MODEL_PROP = 0, 1, 2
 PROP_PLAIN, PROP_STDP, PROP_STP = 0, 1, 2
 PRESET_REF, PRESET_BASELINE = 0, 1
 CORPUS_TEXT_FILTER = 1
+QK_UNIT, QK_ADJACENT = 1, 2
 SCAN_LOGIT, SCAN_LEAKY, SCAN_CHANNEL, SCAN_RASTER, SCAN_ZERO = 1, 2, 4, 8, 32
 FMT_NATIVE, FMT_SNN2_V1, FMT_SCKP_V2, FMT_RAW_F32 = 0, 1, 2, 3
 
@@ -128,7 +129,8 @@ EXPORTS = ["snn_config_init", "snn_topology_init", "snn_create", "snn_destroy",
            "snn_nccl_unique_id", "snn_set_shard", "snn_shard_plan", "snn_semantic_eval",
            "snn_set_corpus_ex", "snn_load_text_corpus", "snn_byte_classes", "snn_embed",
            "snn_embed_grad", "snn_embed_grad_workspace", "snn_leaky_scan", "snn_leaky_scan_saved", "snn_leaky_scan_workspace",
-           "snn_leaky_scan_grad", "snn_leaky_scan_grad_workspace"]
+           "snn_leaky_scan_grad", "snn_leaky_scan_grad_workspace", "snn_qk_norm", "snn_qk_norm_grad",
+           "snn_qk_norm_grad_workspace", "snn_adamw"]
 
 _lib = None
 _lib_refmath = None
@@ -194,6 +196,10 @@ def _load(path):
     L.snn_leaky_scan_workspace.argtypes = [ps, vp]
     L.snn_leaky_scan_grad_workspace.argtypes = [ps, vp]
     L.snn_leaky_scan_grad.argtypes = [ps, pr, pr, vp, pr, vp, pr, pr, vp, vp, i64, vp]
+    L.snn_qk_norm.argtypes = [ps, pr, pr, vp, vp, vp, vp, pr, pr, vp]
+    L.snn_qk_norm_grad_workspace.argtypes = [ps, vp]
+    L.snn_qk_norm_grad.argtypes = [ps, pr, pr, vp, vp, vp, vp, pr, pr, pr, pr, vp, vp, vp, i64, vp]
+    L.snn_adamw.argtypes = [vp, i64, i32, ps, vp]
     L.snn_shard_plan.argtypes = [C.POINTER(TopologySpec), C.c_int32, C.c_int32, vp, C.c_int32]
     return L
 
@@ -544,6 +550,213 @@ def leaky_scan_grad(gate, x, dy, saved, dh=None, logit=False, leaky=False, offse
     _call(lib().snn_leaky_scan_grad, dev, stream, desc, g, xr, saved.data_ptr(), dyr,
           None if dh is None else _state(dh, "dh", state, dev), dgr, dxr, hp, wp, sizes[2])
     return dgate, dx, dh0
+
+
+_QK = struct.Struct("=iiqqqqqqif")  # snn_qk
+_HEADS = struct.Struct("=Qqqq")     # snn_heads
+
+
+def _heads(t, name, shape, dtype):
+    """snn_heads of a tensor [rows, heads, dim] or [sequences, steps, heads, dim]."""
+    if t.shape != shape or t.dtype != dtype:
+        raise SnnError(1, f"{name} must be {tuple(shape)} in {dtype}, not {tuple(t.shape)} in {t.dtype}")
+    st = t.stride()
+    if st[-1] != 1 and shape[-1] != 1:
+        raise SnnError(1, f"{name} wants unit stride in its last dimension")
+    return _HEADS.pack(t.data_ptr(), st[0], st[-3], st[-2])
+
+
+def _new_heads(dev, stream, shape, dtype):
+    """(a new tensor of heads, its snn_heads)"""
+    t, n = _new(dev, stream, tuple(shape), dtype), shape[-2] * shape[-1]
+    return t, _HEADS.pack(t.data_ptr(), shape[-3] * n, n, shape[-1])
+
+
+def _qk_args(q, k, wq, wk, positions, freqs, eps, unit, adjacent):
+    """(device, snn_qk, [rows of q, of k], [address of the weights, ..], address of positions, of freqs)"""
+    if _T is None:
+        _torch()
+    some = q if q is not None else k
+    _require(some is not None, "neither q nor k is given")
+    dev, shape = some.device, some.shape
+    if dev.type != "cuda":
+        raise SnnError(1, "q and k must be CUDA tensors")
+    _require(len(shape) in (3, 4) and shape[-1] >= 1,
+             "q and k must be [rows, heads, dim] or [sequences, steps, heads, dim]")
+    dim, lead, kind = shape[-1], shape[:-2], _elem(some.dtype)
+    n_seq, n_steps = lead if len(lead) == 2 else (1, lead[0])
+    rows, weights, heads = [None, None], [None, None], [0, 0]
+    for i, (x, w, name) in enumerate(((q, wq, "q"), (k, wk, "k"))):
+        if x is None:
+            continue
+        _cuda(x, name, dev)
+        heads[i] = x.shape[-2] if x.dim() == len(shape) else 0
+        rows[i] = _heads(x, name, (*lead, heads[i], dim), some.dtype)
+        if w is not None:
+            _cuda(w, name + "_weight", dev)
+            _require(w.shape == (dim,) and w.dtype == _T.float32 and w.is_contiguous(),
+                     f"{name}_weight must be contiguous float32 [dim]")
+            weights[i] = w.data_ptr()
+    rot, pos_type, pp, fp = 0, 9, None, None
+    _require((positions is None) == (freqs is None), "positions and freqs are given together")
+    if freqs is not None:
+        _cuda(freqs, "freqs", dev)
+        _cuda(positions, "positions", dev)
+        _require(freqs.dim() == 1 and freqs.dtype == _T.float32 and freqs.is_contiguous() and 2 * freqs.numel() <= dim,
+                 "freqs must be contiguous float32 of at most dim / 2 elements")
+        _require(positions.shape == lead and positions.dtype in (_T.int32, _T.int64) and positions.is_contiguous(),
+                 "positions must be contiguous int32 or int64, one for each row")
+        rot, pos_type, pp, fp = 2 * freqs.numel(), _TOKEN[positions.dtype], positions.data_ptr(), freqs.data_ptr()
+    desc = _QK.pack(kind, (QK_UNIT if unit else 0) | (QK_ADJACENT if adjacent else 0), n_seq, n_steps, *heads, dim, rot,
+                    pos_type, eps)
+    return dev, desc, rows, weights, pp, fp
+
+
+def _qk_results(dev, stream, q, k, out):
+    """(the results for q and k, new or those of out; their snn_heads)"""
+    res, to = [None, None], [None, None]
+    for i, x in enumerate((q, k)):
+        if x is None:
+            continue
+        if out[i] is None:
+            res[i], to[i] = _new_heads(dev, stream, x.shape, x.dtype)
+        else:
+            _cuda(out[i], "out", dev)
+            res[i], to[i] = out[i], _heads(out[i], "out", x.shape, x.dtype)
+    return res, to
+
+
+def qk_norm(q, k, q_weight=None, k_weight=None, positions=None, freqs=None, eps=1e-6, unit=False,
+            adjacent=False, out=(None, None), stream=None):
+    """Norms of queries and keys for each head, then the position rotation
+    (snn_qk_norm): y = turn(x / sqrt(mean x^2 + eps) * weight); unit=True takes
+    the sum in place of the mean (rows of unit length).
+
+    q, k: [rows, heads, dim] or [sequences, steps, heads, dim] in float32 / bfloat16
+    / float16, any strides but a unit one of dim; the heads may differ in number,
+    either may be None.  Weights: float32 [dim].  positions: int32 / int64, one for each row,
+    and freqs: float32, the angle a position of each rotated pair (at most dim / 2 pairs; the
+    elements behind them are not rotated); pairs lie half of the rotated elements
+    apart, with adjacent=True beside one another.  Returns (yq, yk), new
+    tensors or `out`, which may be (q, k).  autograd does not see this call:
+    qk_norm_grad is the gradient."""
+    dev, desc, rows, weights, pp, fp = _qk_args(q, k, q_weight, k_weight, positions, freqs, eps, unit, adjacent)
+    res, to = _qk_results(dev, stream, q, k, out)
+    _call(lib().snn_qk_norm, dev, stream, desc, *rows, *weights, pp, fp, *to)
+    return tuple(res)
+
+
+@functools.lru_cache(maxsize=1024)
+def _qk_work(desc):
+    size = C.c_int64()
+    _check(lib().snn_qk_norm_grad_workspace(desc, C.byref(size)))
+    return size.value
+
+
+def qk_norm_grad(q, k, dyq, dyk, q_weight=None, k_weight=None, positions=None, freqs=None, eps=1e-6,
+                 unit=False, adjacent=False, out=(None, None), stream=None):
+    """Gradients of qk_norm (snn_qk_norm_grad) from those of its results: (dq, dk,
+    dq_weight, dk_weight), the last two float32 [dim], None without that weight.
+    Arguments as for qk_norm; `out` takes (dq, dk) and may be (dyq, dyk)."""
+    dev, desc, rows, weights, pp, fp = _qk_args(q, k, q_weight, k_weight, positions, freqs, eps, unit, adjacent)
+    dy, dw, dwp = [None, None], [None, None], [None, None]
+    for i, (x, g, name) in enumerate(((q, dyq, "dyq"), (k, dyk, "dyk"))):
+        if x is None:
+            continue
+        _require(g is not None, f"{name} is missing")
+        _cuda(g, name, dev)
+        dy[i] = _heads(g, name, x.shape, x.dtype)
+        if weights[i] is not None:
+            dw[i] = _new(dev, stream, (x.shape[-1],), _T.float32)
+            dwp[i] = dw[i].data_ptr()
+    res, to = _qk_results(dev, stream, q, k, out)
+    size, wp = 0, None
+    if dwp != [None, None]:
+        size = _qk_work(desc)
+        work = _new(dev, stream, (size,), _T.uint8)
+        wp = work.data_ptr()
+    _call(lib().snn_qk_norm_grad, dev, stream, desc, *rows, *weights, pp, fp, *dy, *to, *dwp, wp, size)
+    return (*res, *dw)
+
+
+_ADAMW_TENSOR = np.dtype([(i, np.uint64) for i in ("p", "g", "m", "v", "ms", "vs", "copy")] + [
+    ("n", np.int64), ("g_type", np.int32), ("copy_type", np.int32)])  # snn_adamw_tensor
+_ADAMW_RULE = struct.Struct("=ddddddqQ")                              # snn_adamw_rule
+
+
+class AdamW:
+    """AdamW over a list of parameters (snn_adamw), a launch for up to 400 tensors.
+
+    params: contiguous float32 CUDA tensors of one device, no two of which overlap.
+    bits: how the moments are held, 32, or 8 (e4m3 values with a float32 scale
+    for every 256 elements; of second moments the root).  copies: None, or
+    for each parameter a bfloat16 or float16 tensor that takes its rounded
+    values (entries may be None).  The moments are the lists m and v (with
+    8 bits float8_e4m3fn, their scales in m_scale and v_scale), zeros at
+    first; moments=(m, v, m_scale, v_scale) takes those of an earlier run over."""
+
+    def __init__(self, params, bits=32, copies=None, moments=None):
+        T = _torch()
+        self.params, self.bits = list(params), bits
+        _require(bits in (32, 8), "moments have 32 or 8 bits")
+        _require(len(self.params) > 0, "no parameters")
+        self.device = dev = self.params[0].device
+        kind = T.float32 if bits == 32 else T.float8_e4m3fn
+        n = len(self.params)
+        blocks = [0 if bits == 32 else (p.numel() + 255) // 256 for p in self.params]
+        if moments is None:
+            moments = tuple([T.zeros(p.shape, device=dev).to(kind) for p in self.params] for _ in range(2)) + tuple(
+                [T.zeros(b, device=dev) for b in blocks] for _ in range(2))
+        self.m, self.v, self.m_scale, self.v_scale = (list(x) for x in moments)
+        self.copies = [None] * n if copies is None else list(copies)
+        _require(all(len(x) == n for x in (self.m, self.v, self.m_scale, self.v_scale, self.copies)),
+                 "moments, scales and copies are as many as the parameters")
+        self._table, used = np.zeros(n, _ADAMW_TENSOR), []
+        for i, p in enumerate(self.params):
+            held = [("p", p, p.shape, T.float32), ("m", self.m[i], p.shape, kind), ("v", self.v[i], p.shape, kind)]
+            if bits == 8:
+                held += [("ms", self.m_scale[i], (blocks[i],), T.float32), ("vs", self.v_scale[i], (blocks[i],), T.float32)]
+            if self.copies[i] is not None:
+                c = self.copies[i]
+                _require(c.dtype in (T.bfloat16, T.float16), "copies are bfloat16 or float16")
+                held.append(("copy", c, p.shape, c.dtype))
+                self._table["copy_type"][i] = _ELEM[c.dtype]
+            for name, t, shape, dtype in held:
+                _require(t.is_cuda and t.device == dev and t.shape == shape and t.dtype == dtype and t.is_contiguous(),
+                         f"{name} of parameter {i} must be a contiguous CUDA tensor {tuple(shape)} in {dtype} on {dev}")
+                self._table[name][i] = t.data_ptr()
+                if t.numel():
+                    used.append((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()))
+            self._table["n"][i] = p.numel()
+        used.sort()
+        _require(all(a[1] <= b[0] for a, b in zip(used, used[1:])), "parameters, moments, scales or copies overlap")
+        self._shapes = [p.shape for p in self.params]
+
+    def step(self, grads, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, grad_scale=1.0, stream=None):
+        """One step, in place: grads, one for each parameter (contiguous, float32 / bfloat16
+        / float16, its shape; None leaves a parameter and its moments alone); step, counted from 1, a
+        number or an int64 CUDA tensor of one element, which is read when the step
+        runs (for captured steps)."""
+        dev, table = self.device, self._table.copy()
+        _require(len(grads) == len(self._shapes), "grads are as many as the parameters")
+        at, kinds = [], []
+        for g, shape in zip(grads, self._shapes):
+            if g is None:
+                at.append(0)
+                kinds.append(0)
+                continue
+            if g.shape != shape or g.device != dev or not g.is_contiguous():
+                raise SnnError(1, f"grads must be contiguous tensors of the parameters' shapes on {dev}")
+            at.append(g.data_ptr())
+            kinds.append(_elem(g.dtype))
+        table["g"], table["g_type"] = at, kinds
+        there = 0
+        if isinstance(step, _T.Tensor):
+            _cuda(step, "step", dev)
+            _require(step.dtype == _T.int64 and step.numel() == 1, "step must be a number or one int64")
+            there, step = step.data_ptr(), 0
+        rule = _ADAMW_RULE.pack(lr, *betas, eps, weight_decay, grad_scale, step, there)
+        _call(lib().snn_adamw, dev, stream, table.ctypes.data, len(table), self.bits, rule)
 
 
 def nccl_unique_id():
