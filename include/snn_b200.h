@@ -553,6 +553,70 @@ int snn_qk_norm_grad(const snn_qk* desc, const snn_heads* q, const snn_heads* k,
                      const snn_heads* dq, const snn_heads* dk, float* dq_weight, float* dk_weight,
                      void* work, int64_t work_bytes, void* stream);
 
+/* ---- delta-rule scan -------------------------------------------------------------
+ * A leaky scan whose state is a matrix S [k_dim, v_dim] of fast synapses for each
+ * head.  Every step decays them, reads them with its key, corrects them by the
+ * error of what was read, and answers its query:
+ *   S' = a_t S_{t-1},   u_t = b_t (v_t - S'^T k_t),   S_t = S' + k_t u_t^T,
+ *   y_t = scale S_t^T q_t
+ * with a = exp(gate), b = beta, or with SNN_SCAN_LOGIT a = 1 / (1 + exp(-gate)),
+ * b = 1 / (1 + exp(-beta)).  gate is a logarithm, so that decays near 1 keep their
+ * memory; minus infinity forgets everything.  Keys of unit length and rates in
+ * [0, 2] keep S bounded (snn_qk_norm with SNN_QK_UNIT); any are taken.
+ * q, k: rows of k_heads x k_dim, v, y: of heads x v_dim, gate, beta: of heads;
+ * head h reads key head h / (heads / k_heads).  All have element type `type`, unit
+ * stride of their last dimension; dense or packed as in snn_leaky_scan, with SNN_SCAN_ZERO
+ * for the rows of no sequence.  k_dim <= 128, v_dim <= 1024.
+ * States are f32 [n_seq, heads, k_dim, v_dim]; h0 (nullable: zeros) and h (nullable)
+ * may be the same.  Sums are f32, y is rounded once.  Long sequences are
+ * taken 64 steps at a time, the recurrence's sum in another order: a NaN or an
+ * infinity in a row may then make the other rows of its 64 steps NaN too.  The same
+ * holds for the gradients.
+ * Where sequences have 8 steps or fewer in the mean the steps are taken one by one,
+ * without a workspace. */
+typedef struct snn_delta {
+    int32_t type;            /* SNN_F32 / SNN_BF16 / SNN_F16                     */
+    int32_t flags;           /* SNN_SCAN_LOGIT, SNN_SCAN_ZERO                    */
+    int64_t n_seq;
+    int64_t n_steps;         /* dense: steps of a sequence; packed: rows in all  */
+    int64_t k_heads, heads;
+    int64_t k_dim, v_dim;
+    const int64_t* offsets;  /* NULL = dense                                     */
+    float scale;
+    int32_t reserved;
+} snn_delta;
+
+/* saved (nullable): saved_bytes bytes, 256-byte aligned, of the size that
+ * snn_delta_scan_saved says; it receives what snn_delta_scan_grad needs.  work: as
+ * for snn_embed_grad, of the size that snn_delta_scan_workspace says; not needed
+ * with saved. */
+int snn_delta_scan_saved(const snn_delta* desc, int64_t* bytes);
+int snn_delta_scan_workspace(const snn_delta* desc, int64_t* bytes);
+int snn_delta_scan(const snn_delta* desc, const snn_heads* q, const snn_heads* k,
+                   const snn_heads* v, const snn_rows* gate, const snn_rows* beta, const float* h0,
+                   const snn_heads* y, float* h, void* saved, int64_t saved_bytes, void* work,
+                   int64_t work_bytes, void* stream);
+
+/* Gradients of snn_delta_scan, from those of y (dy, nullable) and of the final
+ * states (dh, nullable; not both NULL).  With D_t the gradient of S_t, which is
+ * a_{t+1} (D_{t+1} - k_{t+1} (b_{t+1} k_{t+1}^T D_{t+1})) + scale q_t dy_t^T (the last
+ * step: dh + scale q_t dy_t^T), S' and u as above and e_t = b_t D_t^T k_t:
+ *   dq_t = scale S_t dy_t,   dv_t = e_t,   dk_t = D_t u_t - S'_t e_t,
+ *   db_t = (D_t^T k_t).(v_t - S'_t^T k_t),   da_t = <D_t - k_t e_t^T, S_{t-1}>,
+ *   dgate = a da, dbeta = db, or with SNN_SCAN_LOGIT a (1 - a) da and b (1 - b) db;
+ *   dh0 = the gradient of the first S_{t-1}.
+ * dq and dk are summed over the heads that read them, in order.  All results have
+ * their inputs' forms (dq, dk, dv, dgate, dbeta as q, k, v, gate, beta; dh0, nullable, f32
+ * states); rows of no sequence as in the forward call.  saved is what the
+ * forward call wrote.  work: of the size that snn_delta_scan_grad_workspace says. */
+int snn_delta_scan_grad_workspace(const snn_delta* desc, int64_t* bytes);
+int snn_delta_scan_grad(const snn_delta* desc, const snn_heads* q, const snn_heads* k,
+                        const snn_heads* v, const snn_rows* gate, const snn_rows* beta,
+                        const void* saved, int64_t saved_bytes, const snn_heads* dy, const float* dh,
+                        const snn_heads* dq, const snn_heads* dk, const snn_heads* dv,
+                        const snn_rows* dgate, const snn_rows* dbeta, float* dh0, void* work,
+                        int64_t work_bytes, void* stream);
+
 /* ---- AdamW -------------------------------------------------------------------
  * One step over many tensors, each of n elements in device memory (contiguous):
  *   g' = grad_scale g,   m = beta1 m + (1 - beta1) g',   v = beta2 v + (1 - beta2) g'^2,

@@ -481,6 +481,46 @@ int snn_qk_norm_grad(const snn_qk* desc, const snn_heads* q, const snn_heads* k,
     });
 }
 
+int snn_delta_scan_saved(const snn_delta* desc, int64_t* bytes) {
+    return guard_op([&] {
+        SNN_REQUIRE(bytes, SNN_ERR_ARG, "null result");
+        *bytes = snnb::delta_scan_saved(desc);
+    });
+}
+
+int snn_delta_scan_workspace(const snn_delta* desc, int64_t* bytes) {
+    return guard_op([&] {
+        SNN_REQUIRE(bytes, SNN_ERR_ARG, "null result");
+        *bytes = snnb::delta_scan_workspace(desc);
+    });
+}
+
+int snn_delta_scan(const snn_delta* desc, const snn_heads* q, const snn_heads* k, const snn_heads* v,
+                   const snn_rows* gate, const snn_rows* beta, const float* h0, const snn_heads* y, float* h,
+                   void* saved, int64_t saved_bytes, void* work, int64_t work_bytes, void* stream) {
+    return guard_op([&] {
+        snnb::delta_scan(desc, q, k, v, gate, beta, h0, y, h, saved, saved_bytes, work, work_bytes, (cudaStream_t)stream);
+    });
+}
+
+int snn_delta_scan_grad_workspace(const snn_delta* desc, int64_t* bytes) {
+    return guard_op([&] {
+        SNN_REQUIRE(bytes, SNN_ERR_ARG, "null result");
+        *bytes = snnb::delta_scan_grad_workspace(desc);
+    });
+}
+
+int snn_delta_scan_grad(const snn_delta* desc, const snn_heads* q, const snn_heads* k, const snn_heads* v,
+                        const snn_rows* gate, const snn_rows* beta, const void* saved, int64_t saved_bytes,
+                        const snn_heads* dy, const float* dh, const snn_heads* dq, const snn_heads* dk,
+                        const snn_heads* dv, const snn_rows* dgate, const snn_rows* dbeta, float* dh0, void* work,
+                        int64_t work_bytes, void* stream) {
+    return guard_op([&] {
+        snnb::delta_scan_grad(desc, q, k, v, gate, beta, saved, saved_bytes, dy, dh, dq, dk, dv, dgate, dbeta, dh0, work,
+                              work_bytes, (cudaStream_t)stream);
+    });
+}
+
 int snn_adamw(const snn_adamw_tensor* tensors, int64_t count, int32_t bits, const snn_adamw_rule* rule,
               void* stream) {
     return guard_op([&] { snnb::adamw(tensors, count, bits, rule, (cudaStream_t)stream); });

@@ -135,6 +135,17 @@ void qk_norm_grad(const snn_qk* desc, const snn_heads* q, const snn_heads* k, co
                   const void* positions, const float* freqs, const snn_heads* dyq, const snn_heads* dyk,
                   const snn_heads* dq, const snn_heads* dk, float* dwq, float* dwk, void* work, int64_t work_bytes,
                   cudaStream_t st);
+int64_t delta_scan_saved(const snn_delta* desc);
+int64_t delta_scan_workspace(const snn_delta* desc);
+void delta_scan(const snn_delta* desc, const snn_heads* q, const snn_heads* k, const snn_heads* v, const snn_rows* gate,
+                const snn_rows* beta, const float* h0, const snn_heads* y, float* h, void* saved, int64_t saved_bytes,
+                void* work, int64_t work_bytes, cudaStream_t st);
+int64_t delta_scan_grad_workspace(const snn_delta* desc);
+void delta_scan_grad(const snn_delta* desc, const snn_heads* q, const snn_heads* k, const snn_heads* v,
+                     const snn_rows* gate, const snn_rows* beta, const void* saved, int64_t saved_bytes,
+                     const snn_heads* dy, const float* dh, const snn_heads* dq, const snn_heads* dk, const snn_heads* dv,
+                     const snn_rows* dgate, const snn_rows* dbeta, float* dh0, void* work, int64_t work_bytes,
+                     cudaStream_t st);
 void adamw(const snn_adamw_tensor* tensors, int64_t count, int32_t bits, const snn_adamw_rule* rule, cudaStream_t st);
 
 }  // namespace snnb

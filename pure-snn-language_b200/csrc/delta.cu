@@ -1,0 +1,301 @@
+// delta.cu - the delta-rule scan (snn_delta_scan): arguments, the choice of kernels,
+// and the kernel for single steps.
+#include "delta_tile.h"
+
+namespace snnb_delta {
+template <> DeltaSizes delta_sizes<float>();
+template <> DeltaSizes delta_sizes<__nv_bfloat16>();
+template <> DeltaSizes delta_sizes<__half>();
+template <> void launch_prep<float>(const DeltaArgs&, cudaStream_t);
+template <> void launch_prep<__nv_bfloat16>(const DeltaArgs&, cudaStream_t);
+template <> void launch_prep<__half>(const DeltaArgs&, cudaStream_t);
+template <> void launch_scan<float>(const DeltaArgs&, int, cudaStream_t);
+template <> void launch_scan<__nv_bfloat16>(const DeltaArgs&, int, cudaStream_t);
+template <> void launch_scan<__half>(const DeltaArgs&, int, cudaStream_t);
+}  // namespace snnb_delta
+
+namespace {
+using namespace snnb_delta;
+constexpr int MAX_K = 128;
+
+// ---- few steps: the recurrence itself ------------------------------------------------
+// A CTA takes 32 V columns of a head's state, a warp every eighth row of it, in registers
+// from the first step to the last.  Bound by the state's way from memory and back.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) k_delta_steps(const __grid_constant__ DeltaArgs A) {
+    constexpr int R = MAX_K / 8;  // rows of a warp
+    __shared__ float key[MAX_K], query[MAX_K], part[8][2][32 * V];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int head = blockIdx.y, col = ((int)blockIdx.z * 32 + lane) * V, kh = head / A.group;
+    const bool on = col < A.vdim;
+    struct alignas(4 * V) F {
+        float v[V];
+    };
+    for (long long s = blockIdx.x; s < A.n_seq; s += gridDim.x) {
+        const Span sp = span_of(A, s);
+        const long long at = (s * A.heads + head) * (long long)A.kdim * A.vdim + col;
+        F S[R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int d = i * 8 + warp;
+            if (A.h0 && on && d < A.kdim) S[i] = *reinterpret_cast<const F*>(A.h0 + at + (long long)d * A.vdim);
+            else
+#pragma unroll
+                for (int j = 0; j < V; ++j) S[i].v[j] = 0.0f;
+        }
+        for (int t = 0; t < sp.len; ++t) {
+            if (tid < MAX_K) {
+                key[tid] = tid < A.kdim ? to_f32(((const T*)A.k.p)[row_at(A, A.k, s, sp, t) + kh * A.k.hs + tid]) : 0.0f;
+            } else {
+                const int d = tid - MAX_K;
+                query[d] = d < A.kdim ? to_f32(((const T*)A.q.p)[row_at(A, A.q, s, sp, t) + kh * A.q.hs + d]) : 0.0f;
+            }
+            float v[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                v[j] = on ? to_f32(((const T*)A.v.p)[row_at(A, A.v, s, sp, t) + head * A.v.hs + col + j]) : 0.0f;
+            const float l = log_decay(A, ((const T*)A.gate.p)[row_at(A, A.gate, s, sp, t) + head * A.gate.hs]);
+            const float rate = rate_of(A, ((const T*)A.beta.p)[row_at(A, A.beta, s, sp, t) + head * A.beta.hs]);
+            const float lost = -expm1f(l);  // 1 - a, which keeps its bits where a is near 1
+            __syncthreads();
+            float k[R], dk[V] = {}, dq[V] = {}, kq = 0.0f;
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                k[i] = key[i * 8 + warp];
+                const float q = query[i * 8 + warp];
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    S[i].v[j] = fmaf(-lost, S[i].v[j], S[i].v[j]);
+                    dk[j] = fmaf(k[i], S[i].v[j], dk[j]);
+                    dq[j] = fmaf(q, S[i].v[j], dq[j]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < MAX_K / 32; ++i) kq = fmaf(key[i * 32 + lane], query[i * 32 + lane], kq);
+#pragma unroll
+            for (int o = 16; o; o >>= 1) kq += __shfl_xor_sync(~0u, kq, o);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                part[warp][0][lane * V + j] = dk[j];
+                part[warp][1][lane * V + j] = dq[j];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                float sk = 0.0f, sq = 0.0f;
+#pragma unroll
+                for (int w = 0; w < 8; ++w) {
+                    sk += part[w][0][lane * V + j];
+                    sq += part[w][1][lane * V + j];
+                }
+                const float u = rate * (v[j] - sk);
+#pragma unroll
+                for (int i = 0; i < R; ++i) S[i].v[j] = fmaf(k[i], u, S[i].v[j]);
+                if (warp == 0 && on)
+                    ((T*)A.y.p)[row_at(A, A.y, s, sp, t) + head * A.y.hs + col + j] = from_f32<T>(A.scale * fmaf(kq, u, sq));
+            }
+        }
+        if (A.h && on)
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (i * 8 + warp < A.kdim) *reinterpret_cast<F*>(A.h + at + (long long)(i * 8 + warp) * A.vdim) = S[i];
+    }
+    if (A.zero) zero_rest<T>(A, A.y, A.heads, A.vdim, ((long long)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x,
+                             (long long)gridDim.x * gridDim.y * gridDim.z);
+}
+
+// the rows of no sequence where there is no sequence at all
+template <typename T>
+__global__ void __launch_bounds__(256) k_delta_zero(const __grid_constant__ DeltaArgs A, Heads r, int heads, int width) {
+    zero_rest<T>(A, r, heads, width, blockIdx.x, gridDim.x);
+}
+
+void check_desc(const snn_delta* d) {
+    SNN_REQUIRE(d, SNN_ERR_ARG, "delta: null description");
+    SNN_REQUIRE(snnb::elem_type_ok(d->type), SNN_ERR_ARG, "delta: type must be SNN_F32, SNN_BF16 or SNN_F16");
+    SNN_REQUIRE((d->flags & ~(SNN_SCAN_LOGIT | SNN_SCAN_ZERO)) == 0, SNN_ERR_ARG, "delta: unknown flags");
+    SNN_REQUIRE(d->n_seq >= 0 && d->n_seq <= (1ll << 30), SNN_ERR_ARG, "delta: n_seq must lie in [0, 2^30]");
+    SNN_REQUIRE(d->n_steps >= 0 && d->n_steps <= (1ll << 30), SNN_ERR_ARG, "delta: n_steps must lie in [0, 2^30]");
+    SNN_REQUIRE(d->k_heads >= 1 && d->heads >= d->k_heads && d->heads <= 65535 && d->heads % d->k_heads == 0, SNN_ERR_ARG,
+                "delta: heads must be a multiple of k_heads, at most 65535");
+    SNN_REQUIRE(d->k_dim >= 1 && d->k_dim <= MAX_K, SNN_ERR_ARG, "delta: k_dim must lie in [1, 128]");
+    SNN_REQUIRE(d->v_dim >= 1 && d->v_dim <= 1024, SNN_ERR_ARG, "delta: v_dim must lie in [1, 1024]");
+    const int64_t slots = d->offsets ? d->n_steps / C + d->n_seq : d->n_seq * ((d->n_steps + C - 1) / C);
+    SNN_REQUIRE(slots < (1ll << 31) && (slots + d->n_seq) <= (1ll << 46) / (d->heads * d->v_dim * 128 * 4), SNN_ERR_ARG,
+                "delta: more than 2^46 bytes of states");
+}
+int64_t slots_of(const snn_delta* d) {
+    return d->offsets ? d->n_steps / C + d->n_seq : d->n_seq * ((d->n_steps + C - 1) / C);
+}
+int64_t mean_steps(const snn_delta* d) { return d->offsets ? d->n_steps / std::max<int64_t>(d->n_seq, 1) : d->n_steps; }
+
+Heads heads_of(const snn_delta* d, const snn_heads* h, int64_t heads, int64_t width, const char* name, bool written = false) {
+    const int size = snnb::elem_size(d->type);
+    SNN_REQUIRE(h && (h->data || d->n_steps == 0), SNN_ERR_ARG, std::string("delta: null ") + name);
+    SNN_REQUIRE((uintptr_t)h->data % size == 0, SNN_ERR_ARG, std::string("delta: misaligned ") + name);
+    const int64_t seqs = d->offsets ? 1 : d->n_seq, most = 1ll << 46;
+    const int64_t ss = seqs > 1 ? h->seq_stride : 0, st = d->n_steps > 1 ? h->step_stride : 0, hs = heads > 1 ? h->head_stride : 0;
+    SNN_REQUIRE(ss >= 0 && st >= 0 && hs >= 0 && ss <= most / std::max<int64_t>(seqs, 1) &&
+                    st <= most / std::max<int64_t>(d->n_steps, 1) && hs <= most / heads,
+                SNN_ERR_ARG, std::string("delta: bad strides of ") + name);
+    if (written)
+        SNN_REQUIRE(snnb::apart({{seqs, ss}, {d->n_steps, st}, {heads, hs}}, width), SNN_ERR_ARG,
+                    std::string("delta: rows overlap in ") + name);
+    const int v = 16 / size;
+    const bool vec = (uintptr_t)h->data % 16 == 0 && ss % v == 0 && st % v == 0 && hs % v == 0 && width % v == 0;
+    return {h->data, ss, st, hs, vec};
+}
+// a gate's or rate's rows: a head beside the other
+Heads gates_of(const snn_delta* d, const snn_rows* r, const char* name, bool written = false) {
+    SNN_REQUIRE(r, SNN_ERR_ARG, std::string("delta: null ") + name);
+    const snn_heads h = {r->data, r->seq_stride, r->step_stride, 1};
+    Heads o = heads_of(d, &h, d->heads, 1, name, written);
+    o.hs = 1;
+    return o;
+}
+void check_states(std::initializer_list<const void*> p) {
+    for (const void* q : p) SNN_REQUIRE((uintptr_t)q % 4 == 0, SNN_ERR_ARG, "delta: misaligned states");
+}
+
+DeltaSizes sizes_of(const snn_delta* d) {
+    DeltaSizes z{};
+    snnb::with_elem(d->type, [&](auto t) { z = delta_sizes<decltype(t)>(); });
+    return z;
+}
+int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
+// T, P and factors, then (kept for the gradient) states and U
+struct Layout {
+    int64_t factors, states, u, all, kept_all;
+};
+Layout layout_of(const snn_delta* d) {
+    const DeltaSizes z = sizes_of(d);
+    const int64_t units = slots_of(d) * d->heads, kd = d->k_dim <= 64 ? 64 : 128;
+    Layout l;
+    l.factors = round256(units * z.squares);
+    l.all = l.states = l.factors + round256(units * SC * 4);
+    l.u = l.states + round256(units * d->v_dim * kd * z.kept);
+    l.kept_all = l.u + round256(units * C * d->v_dim * z.kept);
+    return l;
+}
+bool by_steps(const snn_delta* d) { return mean_steps(d) <= 8; }
+
+DeltaArgs base_args(const snn_delta* d, const snn_heads* q, const snn_heads* k, const snn_heads* v, const snn_rows* gate,
+                    const snn_rows* beta) {
+    SNN_REQUIRE((uintptr_t)d->offsets % 8 == 0, SNN_ERR_ARG, "delta: misaligned offsets");
+    DeltaArgs A;
+    memset(&A, 0, sizeof(A));
+    A.q = heads_of(d, q, d->k_heads, d->k_dim, "q");
+    A.k = heads_of(d, k, d->k_heads, d->k_dim, "k");
+    A.v = heads_of(d, v, d->heads, d->v_dim, "v");
+    A.gate = gates_of(d, gate, "gate");
+    A.beta = gates_of(d, beta, "beta");
+    A.off = d->offsets;
+    A.n_seq = d->n_seq;
+    A.slots = slots_of(d);
+    A.n_steps = (int)d->n_steps;
+    A.hk = (int)d->k_heads;
+    A.heads = (int)d->heads;
+    A.group = (int)(d->heads / d->k_heads);
+    A.kdim = (int)d->k_dim;
+    A.vdim = (int)d->v_dim;
+    A.logit = (d->flags & SNN_SCAN_LOGIT) != 0;
+    A.zero = d->offsets && (d->flags & SNN_SCAN_ZERO) != 0;
+    A.scale = d->scale;
+    return A;
+}
+void zero_rows(const snn_delta* d, const DeltaArgs& A, const Heads& r, int heads, int width, cudaStream_t st) {
+    if (!A.zero || !r.p || d->n_steps == 0) return;
+    snnb::with_elem(d->type, [&](auto t) { k_delta_zero<decltype(t)><<<4 * SMS, 256, 0, st>>>(A, r, heads, width); });
+    SNN_CUDA(cudaGetLastError());
+}
+
+// Warps of a CTA.  A chunk's K, Q, T and P fill a CTA's shared memory (one CTA an SM), and
+// serve its warps, each with 16 columns of the state.  Up to four warps have a tensor core
+// each; eight share them (1.8 times the time for twice the work), but CTAs that do
+// not fit on the SMs at once are a second round.
+int warps_of(const snn_delta* d) {
+    int best = 1;
+    double least = 1e300;
+    for (int nw = 1; nw <= 8; nw *= 2) {
+        const int64_t ctas = d->n_seq * d->heads * ((d->v_dim + 16 * nw - 1) / (16 * nw));
+        const double cost = (double)((ctas + SMS - 1) / SMS) * (nw == 8 ? 1.8 : 1.0);
+        if (nw > 1 && 16 * nw >= 2 * d->v_dim) break;  // no warp without columns where fewer do
+        if (cost <= least) {
+            least = cost;
+            best = nw;
+        }
+    }
+    return best;
+}
+
+void check_work(const void* work, int64_t bytes, int64_t needed, const char* name) {
+    SNN_REQUIRE(needed == 0 || (work && (uintptr_t)work % 256 == 0 && bytes >= needed), SNN_ERR_ARG,
+                std::string("delta: ") + name + " null, misaligned or too small");
+}
+
+}  // namespace
+
+namespace snnb {
+
+int64_t delta_scan_saved(const snn_delta* d) {
+    check_desc(d);
+    return layout_of(d).kept_all;
+}
+int64_t delta_scan_workspace(const snn_delta* d) {
+    check_desc(d);
+    return by_steps(d) ? 0 : layout_of(d).all;
+}
+
+void delta_scan(const snn_delta* d, const snn_heads* q, const snn_heads* k, const snn_heads* v, const snn_rows* gate,
+                const snn_rows* beta, const float* h0, const snn_heads* y, float* h, void* saved, int64_t saved_bytes,
+                void* work, int64_t work_bytes, cudaStream_t st) {
+    check_desc(d);
+    DeltaArgs A = base_args(d, q, k, v, gate, beta);
+    A.y = heads_of(d, y, d->heads, d->v_dim, "y", true);
+    check_states({h0, h});
+    A.h0 = h0;
+    A.h = h;
+    if (d->n_seq == 0) return zero_rows(d, A, A.y, A.heads, A.vdim, st);
+    const Layout l = layout_of(d);
+    if (!saved && by_steps(d)) {
+        const bool wide = d->v_dim % 4 == 0 && (uintptr_t)h0 % 16 == 0 && (uintptr_t)h % 16 == 0 && d->v_dim > 32;
+        with_elem(d->type, [&](auto t) {
+            using T = decltype(t);
+            const int cols = wide ? 128 : 32;
+            const dim3 grid((unsigned)d->n_seq, (unsigned)d->heads, (unsigned)((d->v_dim + cols - 1) / cols));
+            if (wide) k_delta_steps<T, 4><<<grid, 256, 0, st>>>(A);
+            else k_delta_steps<T, 1><<<grid, 256, 0, st>>>(A);
+        });
+        SNN_CUDA(cudaGetLastError());
+        return;
+    }
+    char* base = (char*)(saved ? saved : work);
+    if (saved) check_work(saved, saved_bytes, l.kept_all, "saved");
+    else check_work(work, work_bytes, l.all, "workspace");
+    A.squares = base;
+    A.factors = (float*)(base + l.factors);
+    if (saved) {
+        A.states = base + l.states;
+        A.u = base + l.u;
+    }
+    with_elem(d->type, [&](auto t) {
+        using T = decltype(t);
+        if (A.slots) launch_prep<T>(A, st);
+        launch_scan<T>(A, warps_of(d), st);
+    });
+}
+
+}  // namespace snnb
+
+namespace snnb {
+int64_t delta_scan_grad_workspace(const snn_delta* d) {
+    check_desc(d);
+    return 0;
+}
+void delta_scan_grad(const snn_delta*, const snn_heads*, const snn_heads*, const snn_heads*, const snn_rows*,
+                     const snn_rows*, const void*, int64_t, const snn_heads*, const float*, const snn_heads*,
+                     const snn_heads*, const snn_heads*, const snn_rows*, const snn_rows*, float*, void*, int64_t,
+                     cudaStream_t) {
+    throw Error(SNN_ERR_UNSUPPORTED, "delta: no gradient yet");
+}
+}  // namespace snnb

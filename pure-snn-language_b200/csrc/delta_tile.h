@@ -1,0 +1,839 @@
+// delta_tile.h - kernels of the delta-rule scan (snn_delta_scan) over chunks of 64
+// steps, included by one file per element type.
+//
+// With S the state [dk, dv] before a chunk, a_t the decays, G_ij = a_{j+1} .. a_i,
+// since_i = a_1 .. a_i and until_j = a_{j+1} .. a_64 (steps counted in the chunk):
+//   A_ij = b_i G_ij k_i.k_j (j < i),   T = (1 + A)^-1,   P_ij = G_ij q_i.k_j (j <= i)
+//   U = T b (V - since K S),   Y = scale (since Q S + P U),   S <- since_64 S + (until K)^T U
+// which is the recurrence's own sum, reordered (the chunked form of the gated delta
+// rule).  T and P do not depend on the state: k_delta_prep makes them for all chunks at
+// once.  k_delta_scan then runs along the sequence.  Columns of the state are
+// independent, so a warp takes 16 of them, alone: it holds S^T [16, dk] in registers
+// as accumulators of the matrix instruction, whose layout (a thread has columns 2t,
+// 2t+1 of rows g, g+8) is that of the instruction's first operand again.  So
+// every product takes its first operand from the accumulators of the one before it and the
+// second (K, Q, T, P; by rows or transposed) from shared memory, and the state never leaves
+// the registers.  Tensor memory would hold a state per SM only and pay a round trip
+// through shared memory for each of the three products that follow one another in a
+// chunk; warps that need not wait for one another hide each other's latency.
+//
+// Numbers: states, U and sums are f32.  The matrix instruction takes 16-bit (or tf32)
+// operands, so an f32 operand is split into pieces that are summed: three of bf16 (24
+// bits), two of f16 times a power of two (22 bits), two of tf32 (22 bits).  K and Q are exact
+// in one piece but for f32 tensors.  What only reaches Y takes two pieces.
+#pragma once
+#include <algorithm>
+#include <cfloat>
+#include <type_traits>
+#include "elem.h"
+
+namespace snnb_delta {
+using snnb::from_f32;
+using snnb::to_f32;
+constexpr int C = 64;         // steps of a chunk
+constexpr int MS = C + 8;     // row stride of T and P in shared memory and the workspace
+constexpr int PAD = 8;        // elements behind a row in shared memory: eight rows lie in different banks
+constexpr int SC = 3 * C + 8; // floats of a chunk's factors: since, until, rate, then those of Factor
+enum Factor { LOST = 3 * C, T_SCALE, P_SCALE };
+constexpr int SMS = 148;
+
+struct Heads {                // rows of heads: strides in elements
+    void* p;
+    long long ss, st, hs;
+    int vec;                  // rows and heads are words of 16 bytes
+};
+struct DeltaArgs {
+    Heads q, k, v, y, dy, dq, dk, dv;
+    Heads gate, beta, dgate, dbeta;
+    const float *h0, *dh;
+    float *h, *dh0;
+    const int64_t* off;
+    long long n_seq, slots;   // chunks in all (packed: at most)
+    int n_steps, hk, heads, group, kdim, vdim;
+    int logit, zero;
+    float scale;
+    char* squares;            // [slots, heads] of Path::SQUARES bytes
+    float* factors;           // [slots, heads, SC]
+    char *states, *u;         // saved: [slots, heads, vdim, KD], [slots, heads, C, vdim] of Path::Kept
+    char *dstates, *dr;       // gradients' workspace: the same forms
+};
+
+struct Span {
+    long long start;          // first row (packed)
+    int len;
+    long long chunk;          // first chunk
+};
+__device__ __forceinline__ Span span_of(const DeltaArgs& A, long long s) {
+    if (!A.off) return {0, A.n_steps, s * ((A.n_steps + C - 1) / C)};
+    const long long n = A.n_steps, b = min(max((long long)A.off[s], 0ll), n), e = min(max((long long)A.off[s + 1], b), n);
+    return {b, (int)(e - b), b / C + s};
+}
+__device__ __forceinline__ long long row_at(const DeltaArgs& A, const Heads& h, long long s, const Span& sp, int t) {
+    return A.off ? (sp.start + t) * h.st : s * h.ss + t * h.st;
+}
+
+// decay's logarithm and rate of a step
+template <typename T>
+__device__ __forceinline__ float log_decay(const DeltaArgs& A, T g) {
+    const float z = to_f32(g);
+    if (!A.logit) return z;
+    return z > 0.0f ? -log1pf(expf(-z)) : z - log1pf(expf(z));
+}
+template <typename T>
+__device__ __forceinline__ float rate_of(const DeltaArgs& A, T b) {
+    const float z = to_f32(b);
+    return A.logit ? 1.0f / (1.0f + expf(-z)) : z;
+}
+
+// ---- copies to shared memory --------------------------------------------------
+__device__ __forceinline__ void copy16(void* to, const void* from, bool there) {
+    const unsigned a = (unsigned)__cvta_generic_to_shared(to);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(a), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// C rows of W columns, n and w of them there, zeros in the others; rows `to` of stride W + PAD
+template <typename T, int W>
+__device__ __forceinline__ void load_rows(T* to, const T* from, long long st, int n, int w, bool vec, int tid, int threads) {
+    if (vec) {
+        constexpr int V = 16 / (int)sizeof(T), N = W / V;
+        for (int i = tid; i < C * N; i += threads) {
+            const int r = i / N, c = (i - r * N) * V;
+            const bool there = r < n && c < w;
+            copy16(to + r * (W + PAD) + c, there ? from + r * st + c : from, there);
+        }
+    } else {
+        for (int i = tid; i < C * W; i += threads) {
+            const int r = i / W, c = i - r * W;
+            to[r * (W + PAD) + c] = r < n && c < w ? from[r * st + c] : from_f32<T>(0.0f);
+        }
+    }
+}
+__device__ __forceinline__ void load_words(void* to, const void* from, int bytes, int tid, int threads) {
+    for (int i = tid * 16; i < bytes; i += threads * 16) copy16((char*)to + i, (const char*)from + i, true);
+}
+
+// ---- products -------------------------------------------------------------------
+// A fragment of the first operand [16, 16] comes from two accumulator tiles [16, 8].
+__device__ __forceinline__ void ldsm4(unsigned (&r)[4], const void* p) {
+    const unsigned a = (unsigned)__cvta_generic_to_shared(p);
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(unsigned (&r)[4], const void* p) {
+    const unsigned a = (unsigned)__cvta_generic_to_shared(p);
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16(float (&d)[4], const unsigned (&a)[4], const unsigned (&b)[2]) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+__device__ __forceinline__ void mma8(float (&d)[4], const unsigned* a, const unsigned* b) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+
+// two f32 as a pair of 16-bit values (the first one low), and what that leaves of them
+template <typename T>
+__device__ __forceinline__ unsigned pair_of(float x, float y) {
+    unsigned w;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(y), "f"(x));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(y), "f"(x));
+    return w;
+}
+template <typename T>
+__device__ __forceinline__ float2 of_pair(unsigned w) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    } else {
+        __half2 h;
+        memcpy(&h, &w, 4);
+        return __half22float2(h);
+    }
+}
+template <typename T>
+__device__ __forceinline__ unsigned piece(float& x, float& y) {
+    const unsigned w = pair_of<T>(x, y);
+    const float2 f = of_pair<T>(w);
+    x -= f.x;
+    y -= f.y;
+    return w;
+}
+
+// 16-bit elements: N pieces of the state's side
+template <typename T_, int N_>
+struct Path16 {
+    using T = T_;
+    static constexpr int N = N_;
+    static constexpr bool SCALED = std::is_same<T, __half>::value;  // pieces keep their bits near 1 only
+    static constexpr int T_PLANES = N, P_PLANES = 2, STAGES = 2;
+    using Sq = T;             // elements of T's and P's planes
+    static constexpr int PLANE = C * MS, SQUARES = (T_PLANES + P_PLANES) * PLANE * 2;
+    struct A {
+        unsigned v[N][4];
+    };
+    struct B {
+        unsigned v[2];
+    };
+    static __device__ __forceinline__ A split(const float (&x)[4], const float (&y)[4], float s) {
+        A a;
+        float c[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        if constexpr (SCALED)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) c[i] *= s;
+#pragma unroll
+        for (int p = 0; p < N; ++p)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a.v[p][i] = p < N - 1 ? piece<T>(c[2 * i], c[2 * i + 1]) : pair_of<T>(c[2 * i], c[2 * i + 1]);
+        return a;
+    }
+    // B [16, 2 x 8] with B[k][n] = m[n][k] (rows of m are n), or m[k][n]
+    static __device__ __forceinline__ void by_rows(B (&b)[2], const T* m, int st) {
+        const int l = threadIdx.x & 31;
+        unsigned r[4];
+        ldsm4(r, m + ((l & 7) + (l >> 4) * 8) * st + ((l >> 3) & 1) * 8);
+        b[0] = {{r[0], r[1]}};
+        b[1] = {{r[2], r[3]}};
+    }
+    static __device__ __forceinline__ void by_columns(B (&b)[2], const T* m, int st) {
+        const int l = threadIdx.x & 31;
+        unsigned r[4];
+        ldsm4t(r, m + ((l & 7) + ((l >> 3) & 1) * 8) * st + (l >> 4) * 8);
+        b[0] = {{r[0], r[1]}};
+        b[1] = {{r[2], r[3]}};
+    }
+    // d += a b: all pieces (what a state is made of), or what reaches a rounded result
+    static __device__ __forceinline__ void full(float (&d0)[4], float (&d1)[4], const A& a, const B (&b)[2]) {
+#pragma unroll
+        for (int p = N - 1; p >= 0; --p) {
+            mma16<T>(d0, a.v[p], b[0].v);
+            mma16<T>(d1, a.v[p], b[1].v);
+        }
+    }
+    static __device__ __forceinline__ void out(float (&d0)[4], float (&d1)[4], const A& a, const B (&b)[2]) {
+#pragma unroll
+        for (int p = 1; p >= 0; --p) {
+            mma16<T>(d0, a.v[p], b[0].v);
+            mma16<T>(d1, a.v[p], b[1].v);
+        }
+    }
+    // the same with a matrix in PLANES pieces: the products of pieces i, j with i + j < N
+    template <int PLANES, bool ROWS>
+    static __device__ __forceinline__ void square(float (&d0)[4], float (&d1)[4], const A& a, const T* m) {
+#pragma unroll
+        for (int j = PLANES - 1; j >= 0; --j) {
+            B b[2];
+            if (ROWS) by_rows(b, m + j * PLANE, MS);
+            else by_columns(b, m + j * PLANE, MS);
+#pragma unroll
+            for (int p = N - 1; p >= 0; --p)
+                if (p + j < PLANES) {
+                    mma16<T>(d0, a.v[p], b[0].v);
+                    mma16<T>(d1, a.v[p], b[1].v);
+                }
+        }
+    }
+    // elements (i, j), (i, j + 1) of a matrix into its planes
+    template <int PLANES>
+    static __device__ __forceinline__ void put(T* m, int i, int j, float x, float y, float s) {
+        if constexpr (SCALED) {
+            x *= s;
+            y *= s;
+        }
+#pragma unroll
+        for (int p = 0; p < PLANES; ++p) *reinterpret_cast<unsigned*>(m + p * PLANE + i * MS + j) = piece<T>(x, y);
+    }
+    // d0, d1 += x y^T for rows of T in shared memory: 16 rows of x, 2 x 8 of y, 16 columns
+    static __device__ __forceinline__ void gram(float (&d0)[4], float (&d1)[4], const T* x, const T* y, int st) {
+        const int l = threadIdx.x & 31;
+        unsigned a[4];
+        ldsm4(a, x + (l & 15) * st + (l >> 4) * 8);
+        B b[2];
+        by_rows(b, y, st);
+        mma16<T>(d0, a, b[0].v);
+        mma16<T>(d1, a, b[1].v);
+    }
+};
+
+__device__ __forceinline__ unsigned tf32_of(float x) {
+    unsigned w;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(w) : "f"(x));
+    return w;
+}
+__device__ __forceinline__ void tf32_split(float x, unsigned& h, unsigned& l) {
+    h = tf32_of(x);
+    l = tf32_of(x - __uint_as_float(h));
+}
+// f32 elements: two tf32 pieces on both sides.  The k index of an 8-deep product is
+// permuted (0, 2, 4, 6, 1, 3, 5, 7), which makes accumulators its first operand.
+struct Path32 {
+    using T = float;
+    static constexpr bool SCALED = false;
+    static constexpr int T_PLANES = 1, P_PLANES = 1, STAGES = 1;
+    using Sq = float;
+    static constexpr int PLANE = C * MS, SQUARES = 2 * PLANE * 4;
+    struct A {
+        unsigned h[8], l[8];
+    };
+    struct B {
+        unsigned h[4], l[4];
+    };
+    static __device__ __forceinline__ A split(const float (&x)[4], const float (&y)[4], float) {
+        A a;
+        const float c[8] = {x[0], x[2], x[1], x[3], y[0], y[2], y[1], y[3]};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) tf32_split(c[i], a.h[i], a.l[i]);
+        return a;
+    }
+    static __device__ __forceinline__ void by_rows(B (&b)[2], const float* m, int st) {
+        const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const float2 v = *reinterpret_cast<const float2*>(m + (n * 8 + g) * st + k * 8 + 2 * t);
+                tf32_split(v.x, b[n].h[2 * k], b[n].l[2 * k]);
+                tf32_split(v.y, b[n].h[2 * k + 1], b[n].l[2 * k + 1]);
+            }
+    }
+    static __device__ __forceinline__ void by_columns(B (&b)[2], const float* m, int st) {
+        const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    tf32_split(m[(k * 8 + 2 * t + i) * st + n * 8 + g], b[n].h[2 * k + i], b[n].l[2 * k + i]);
+    }
+    static __device__ __forceinline__ void full(float (&d0)[4], float (&d1)[4], const A& a, const B (&b)[2]) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            mma8(d0, a.l + 4 * k, b[0].h + 2 * k);
+            mma8(d1, a.l + 4 * k, b[1].h + 2 * k);
+            mma8(d0, a.h + 4 * k, b[0].l + 2 * k);
+            mma8(d1, a.h + 4 * k, b[1].l + 2 * k);
+            mma8(d0, a.h + 4 * k, b[0].h + 2 * k);
+            mma8(d1, a.h + 4 * k, b[1].h + 2 * k);
+        }
+    }
+    static __device__ __forceinline__ void out(float (&d0)[4], float (&d1)[4], const A& a, const B (&b)[2]) { full(d0, d1, a, b); }
+    template <int PLANES, bool ROWS>
+    static __device__ __forceinline__ void square(float (&d0)[4], float (&d1)[4], const A& a, const float* m) {
+        B b[2];
+        if (ROWS) by_rows(b, m, MS);
+        else by_columns(b, m, MS);
+        full(d0, d1, a, b);
+    }
+    template <int PLANES>
+    static __device__ __forceinline__ void put(float* m, int i, int j, float x, float y, float) {
+        *reinterpret_cast<float2*>(m + i * MS + j) = make_float2(x, y);
+    }
+    static __device__ __forceinline__ void gram(float (&d0)[4], float (&d1)[4], const float* x, const float* y, int st) {
+        const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+        float c[2][4];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float2 v = *reinterpret_cast<const float2*>(x + (i * 8 + g) * st + k * 8 + 2 * t);
+                c[k][2 * i] = v.x;
+                c[k][2 * i + 1] = v.y;
+            }
+        B b[2];
+        by_rows(b, y, st);
+        full(d0, d1, split(c[0], c[1], 1.0f), b);
+    }
+};
+template <typename T> struct PathOf;
+template <> struct PathOf<__nv_bfloat16> { using P = Path16<__nv_bfloat16, 3>; };
+template <> struct PathOf<__half> { using P = Path16<__half, 2>; };
+template <> struct PathOf<float> { using P = Path32; };
+
+// A power of two that brings the largest magnitude to 2^13 .. 2^14, near f16's largest
+// values, so that smaller ones keep 24 bits down to 2^-17 of it; held to 2^-40 .. 2^40,
+// so that what it multiplies stays finite
+__device__ __forceinline__ float scale_for(float top) {
+    const int e = min(max(140 + 127 - (int)(__float_as_uint(top) >> 23) , 127 - 40), 127 + 40);
+    return __uint_as_float((unsigned)e << 23);
+}
+__device__ __forceinline__ float inverse_of(float s) {  // of a power of two
+    return __uint_as_float((254u << 23) - __float_as_uint(s));
+}
+template <int N>
+__device__ __forceinline__ float warp_scale(const float (&x)[N][4]) {
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(x[i][j]));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+    return scale_for(top);
+}
+
+// ---- T, P and the factors of every chunk ------------------------------------------
+constexpr int PREP = 128;
+template <class P, int KD>
+constexpr int prep_smem() {
+    return 2 * C * (KD + PAD) * (int)sizeof(typename P::T) + C * (C + 4) * 4;
+}
+template <class P, int KD>
+__global__ void __launch_bounds__(PREP) k_delta_prep(const __grid_constant__ DeltaArgs A) {
+    using T = typename P::T;
+    extern __shared__ __align__(16) char smem[];
+    T *K = reinterpret_cast<T*>(smem), *Q = K + C * (KD + PAD);
+    float* M = reinterpret_cast<float*>(Q + C * (KD + PAD));  // [C][C + 4]: A, then T
+    __shared__ double up[C];   // sums of the logarithms of the decays but for those that are 0
+    __shared__ int cut[C];     // how many are
+    __shared__ float rate[C], top[2][4];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, head = blockIdx.y;
+    const long long slot = blockIdx.x;
+    // the sequence of this chunk
+    long long s = 0;
+    if (A.off) {
+        long long lo = 0, hi = A.n_seq - 1;
+        while (lo < hi) {
+            const long long mid = (lo + hi + 1) / 2;
+            if (span_of(A, mid).chunk <= slot) lo = mid;
+            else hi = mid - 1;
+        }
+        s = lo;
+    } else {
+        s = slot / ((A.n_steps + C - 1) / C);
+    }
+    const Span sp = span_of(A, s);
+    const long long t0 = (slot - sp.chunk) * C;
+    if (t0 < 0 || t0 >= sp.len) return;
+    const int n = (int)min((long long)C, sp.len - t0), kh = head / A.group;
+    load_rows<T, KD>(K, (const T*)A.k.p + row_at(A, A.k, s, sp, (int)t0) + kh * A.k.hs, A.k.st, n, A.kdim, A.k.vec, tid, PREP);
+    load_rows<T, KD>(Q, (const T*)A.q.p + row_at(A, A.q, s, sp, (int)t0) + kh * A.q.hs, A.q.st, n, A.kdim, A.q.vec, tid, PREP);
+    copies_end();
+    if (warp == 0) {
+        double l[2];
+        int z[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int t = 2 * lane + i;
+            float lg = 0.0f, r = 0.0f;
+            if (t < n) {
+                lg = log_decay(A, ((const T*)A.gate.p)[row_at(A, A.gate, s, sp, (int)t0 + t) + head * A.gate.hs]);
+                r = rate_of(A, ((const T*)A.beta.p)[row_at(A, A.beta, s, sp, (int)t0 + t) + head * A.beta.hs]);
+            }
+            z[i] = lg == -INFINITY;
+            l[i] = z[i] ? 0.0 : (double)lg;
+            rate[t] = r;
+        }
+        double sum = l[0] + l[1];
+        int cuts = z[0] + z[1];
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const double d = __shfl_up_sync(~0u, sum, o);
+            const int c = __shfl_up_sync(~0u, cuts, o);
+            if (lane >= o) {
+                sum += d;
+                cuts += c;
+            }
+        }
+        up[2 * lane] = sum - l[1];
+        up[2 * lane + 1] = sum;
+        cut[2 * lane] = cuts - z[1];
+        cut[2 * lane + 1] = cuts;
+    }
+    copies_wait<0>();
+    __syncthreads();
+    const long long unit = slot * A.heads + head;
+    float* F = A.factors + unit * SC;
+    typename P::Sq *Tm = reinterpret_cast<typename P::Sq*>(A.squares + unit * P::SQUARES), *Pm = Tm + P::T_PLANES * P::PLANE;
+    if (tid < C) {
+        F[tid] = cut[tid] ? 0.0f : expf((float)up[tid]);
+        F[C + tid] = cut[tid] == cut[C - 1] ? expf((float)(up[C - 1] - up[tid])) : 0.0f;
+        F[2 * C + tid] = rate[tid];
+        if (tid == 0) F[LOST] = cut[C - 1] ? 1.0f : -expm1f((float)up[C - 1]);
+    }
+    // rows 16 warp .. of the products of keys, and of queries with keys
+    const int g = lane >> 2, t4 = lane & 3;
+    float kk[8][4] = {}, qk[8][4] = {};
+#pragma unroll
+    for (int np = 0; np < 4; ++np) {
+        if (np > warp) break;  // above the diagonal
+#pragma unroll 2
+        for (int d = 0; d < KD; d += 16) {
+            P::gram(kk[2 * np], kk[2 * np + 1], K + warp * 16 * (KD + PAD) + d, K + np * 16 * (KD + PAD) + d, KD + PAD);
+            P::gram(qk[2 * np], qk[2 * np + 1], Q + warp * 16 * (KD + PAD) + d, K + np * 16 * (KD + PAD) + d, KD + PAD);
+        }
+    }
+    float most = 0.0f;
+#pragma unroll
+    for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int i = warp * 16 + g + (e >> 1) * 8, j = nt * 8 + 2 * t4 + (e & 1);
+            const float G = j <= i && cut[i] == cut[j] ? expf((float)(up[i] - up[j])) : 0.0f;
+            // (a factor of 0 takes all: what lies above the diagonal may be anything)
+            qk[nt][e] = j <= i && G != 0.0f ? G * qk[nt][e] : 0.0f;
+            const float a = rate[i] * G;
+            M[i * (C + 4) + j] = j < i && a != 0.0f ? a * kk[nt][e] : 0.0f;
+            most = fmaxf(most, fabsf(qk[nt][e]));
+        }
+    if constexpr (P::SCALED) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, o));
+        if (lane == 0) top[0][warp] = most;
+    }
+    __syncthreads();
+    float p_scale = 1.0f, t_scale = 1.0f;
+    if constexpr (P::SCALED) p_scale = scale_for(fmaxf(fmaxf(top[0][0], top[0][1]), fmaxf(top[0][2], top[0][3])));
+#pragma unroll
+    for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            P::template put<P::P_PLANES>(Pm, warp * 16 + g + h * 8, nt * 8 + 2 * t4, qk[nt][2 * h], qk[nt][2 * h + 1], p_scale);
+    // T by forward substitution, a column to a thread
+    float x[C];
+    if (tid < C) {
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            float a0 = 0.0f, a1 = 0.0f, a2 = 0.0f, a3 = 0.0f;
+#pragma unroll
+            for (int m = 0; m < (i + 3) / 4; ++m) {
+                const float4 r = *reinterpret_cast<const float4*>(M + i * (C + 4) + 4 * m);
+                a0 = fmaf(r.x, x[4 * m], a0);
+                if (4 * m + 1 < i) a1 = fmaf(r.y, x[4 * m + 1], a1);
+                if (4 * m + 2 < i) a2 = fmaf(r.z, x[4 * m + 2], a2);
+                if (4 * m + 3 < i) a3 = fmaf(r.w, x[4 * m + 3], a3);
+            }
+            x[i] = i < tid ? 0.0f : (i == tid ? 1.0f : 0.0f) - ((a0 + a1) + (a2 + a3));
+        }
+    }
+    __syncthreads();
+    if (tid < C) {
+        float big = 0.0f;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            M[i * (C + 4) + tid] = x[i];
+            big = fmaxf(big, fabsf(x[i]));
+        }
+        if constexpr (P::SCALED) {
+#pragma unroll
+            for (int o = 16; o; o >>= 1) big = fmaxf(big, __shfl_xor_sync(~0u, big, o));
+            if (lane == 0) top[1][warp] = big;
+        }
+    }
+    __syncthreads();
+    if constexpr (P::SCALED) t_scale = scale_for(fmaxf(top[1][0], top[1][1]));
+    for (int i = tid; i < C * C / 2; i += PREP) {
+        const int r = i / (C / 2), c = 2 * (i % (C / 2));
+        P::template put<P::T_PLANES>(Tm, r, c, M[r * (C + 4) + c], M[r * (C + 4) + c + 1], t_scale);
+    }
+    if (tid == 0) {
+        F[T_SCALE] = t_scale;
+        F[P_SCALE] = p_scale;
+    }
+}
+
+// ---- along the sequences ------------------------------------------------------------
+template <class P, int KD, int NW>
+struct Stage {
+    using T = typename P::T;
+    static constexpr int VW = 16 * NW;
+    static constexpr int KEYS = C * (KD + PAD) * (int)sizeof(T), VALUES = C * (VW + PAD) * (int)sizeof(T);
+    static constexpr int BYTES = 2 * KEYS + VALUES + P::SQUARES + SC * 4;
+    static constexpr int STAGES = P::STAGES * BYTES <= 227 * 1024 - 1024 ? P::STAGES : 1;
+    T *k, *q, *v;
+    typename P::Sq *t, *p;
+    float* f;
+    __device__ __forceinline__ explicit Stage(char* m) {
+        k = reinterpret_cast<T*>(m);
+        q = reinterpret_cast<T*>(m + KEYS);
+        v = reinterpret_cast<T*>(m + 2 * KEYS);
+        t = reinterpret_cast<typename P::Sq*>(m + 2 * KEYS + VALUES);
+        p = t + P::T_PLANES * P::PLANE;
+        f = reinterpret_cast<float*>(m + 2 * KEYS + VALUES + P::SQUARES);
+    }
+    // chunk c of sequence s; v: the values' rows or, backward, those of dy
+    __device__ __forceinline__ void load(const DeltaArgs& A, const Heads& vals, long long s, const Span& sp, int c, int head,
+                                         int col0, int tid) {
+        const int n = min(C, sp.len - c * C), kh = head / A.group;
+        const long long unit = (sp.chunk + c) * A.heads + head;
+        load_rows<T, KD>(k, (const T*)A.k.p + row_at(A, A.k, s, sp, c * C) + kh * A.k.hs, A.k.st, n, A.kdim, A.k.vec, tid, NW * 32);
+        load_rows<T, KD>(q, (const T*)A.q.p + row_at(A, A.q, s, sp, c * C) + kh * A.q.hs, A.q.st, n, A.kdim, A.q.vec, tid, NW * 32);
+        load_rows<T, VW>(v, (const T*)vals.p + row_at(A, vals, s, sp, c * C) + head * vals.hs + col0, vals.st, n,
+                         A.vdim - col0, vals.vec, tid, NW * 32);
+        load_words(t, A.squares + unit * P::SQUARES, P::SQUARES, tid, NW * 32);
+        load_words(f, A.factors + unit * SC, SC * 4, tid, NW * 32);
+    }
+};
+
+// a warp's tile [16 columns, C steps] (accumulators) as rows of T: into its columns of
+// `stage` [C][VW + PAD], from there to memory
+template <typename T, int ST>
+__device__ __forceinline__ void store_tile(const float (&o)[8][4], T* stage, T* to, long long st, int n, int w, bool vec) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) stage[(i * 8 + 2 * t4 + (e & 1)) * ST + g + (e >> 1) * 8] = from_f32<T>(o[i][e]);
+    __syncwarp();
+    if (vec && w >= 16) {
+        constexpr int V = 16 / (int)sizeof(T), N = 16 / V;
+        for (int i = lane; i < n * N; i += 32) {
+            const int r = i / N, c = i % N * V;
+            *reinterpret_cast<uint4*>(to + r * st + c) = *reinterpret_cast<const uint4*>(stage + r * ST + c);
+        }
+    } else {
+        for (int i = lane; i < n * 16; i += 32) {
+            const int r = i >> 4, c = i & 15;
+            if (c < w) to[r * st + c] = stage[r * ST + c];
+        }
+    }
+    __syncwarp();
+}
+
+// S^T [16 columns, KD] of a warp as it is kept for the gradient: rows of KD elements
+template <typename T, int NT>
+__device__ __forceinline__ void keep_state(const float (&S)[NT][4], T* to, int w) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+    constexpr int KD = NT * 8;
+#pragma unroll
+    for (int i = 0; i < NT; i += 2)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            // lanes of even t take four elements of tile i, of odd t of tile i + 1: 16 elements of a row in a store
+            const bool odd = t4 & 1;
+            const float x = odd ? S[i][2 * h] : S[i + 1][2 * h], y = odd ? S[i][2 * h + 1] : S[i + 1][2 * h + 1];
+            const float px = __shfl_xor_sync(~0u, x, 1), py = __shfl_xor_sync(~0u, y, 1);
+            const float mx = odd ? S[i + 1][2 * h] : S[i][2 * h], my = odd ? S[i + 1][2 * h + 1] : S[i][2 * h + 1];
+            const int row = g + 8 * h, col = (i + odd) * 8 + (t4 >> 1) * 4;
+            if (row < w) {
+                if constexpr (sizeof(T) == 4) {
+                    *reinterpret_cast<float4*>(to + row * KD + col) = odd ? make_float4(px, py, mx, my) : make_float4(mx, my, px, py);
+                } else {
+                    const unsigned a = pair_of<T>(mx, my), b = pair_of<T>(px, py);
+                    *reinterpret_cast<uint2*>(to + row * KD + col) = odd ? make_uint2(b, a) : make_uint2(a, b);
+                }
+            }
+        }
+}
+// f32 states [kdim, vdim] from and to a warp's columns
+template <int NT>
+__device__ __forceinline__ void read_state(float (&S)[NT][4], const float* h, const DeltaArgs& A, int col) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int c = col + g + (e >> 1) * 8, d = i * 8 + 2 * t4 + (e & 1);
+            S[i][e] = h && c < A.vdim && d < A.kdim ? h[(long long)d * A.vdim + c] : 0.0f;
+        }
+}
+template <int NT>
+__device__ __forceinline__ void write_state(const float (&S)[NT][4], float* h, const DeltaArgs& A, int col) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int c = col + g + (e >> 1) * 8, d = i * 8 + 2 * t4 + (e & 1);
+            if (c < A.vdim && d < A.kdim) h[(long long)d * A.vdim + c] = S[i][e];
+        }
+}
+
+// what the gradient needs of states and U in which type: bf16 gradients are rounded to
+// 8 bits themselves
+template <typename T> struct Kept { using K = float; };
+template <> struct Kept<__nv_bfloat16> { using K = __nv_bfloat16; };
+
+// rows of no sequence become zero in y-like tensors
+template <typename T>
+__device__ void zero_rest(const DeltaArgs& A, const Heads& r, int heads, int width, long long cta, long long ctas) {
+    if (!r.p) return;
+    const long long n = A.n_steps;
+    const long long first = A.n_seq ? min(max((long long)A.off[0], 0ll), n) : n, last = A.n_seq ? min(max((long long)A.off[A.n_seq], first), n) : n;
+    const long long rows = first + (n - last), per = (long long)heads * width;
+    for (long long i = cta * blockDim.x + threadIdx.x; i < rows * per; i += ctas * blockDim.x) {
+        const long long k = i / per, e = i - k * per, row = k < first ? k : last + (k - first);
+        ((T*)r.p)[row * r.st + e / width * r.hs + e % width] = from_f32<T>(0.0f);
+    }
+}
+
+template <class P, int KD, int NW>
+__global__ void __launch_bounds__(NW * 32, 1) k_delta_scan(const __grid_constant__ DeltaArgs A) {
+    using T = typename P::T;
+    using St = Stage<P, KD, NW>;
+    using K = typename Kept<T>::K;
+    constexpr int NT = KD / 8, KS = KD + PAD, VS = St::VW + PAD;
+    extern __shared__ __align__(16) char smem[];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+    const int head = blockIdx.y, col0 = (int)blockIdx.z * St::VW, col = col0 + warp * 16;
+    const int w = A.vdim - col;  // this warp's columns (16 and more: all; none: it only loads)
+    for (long long s = blockIdx.x; s < A.n_seq; s += gridDim.x) {
+        const Span sp = span_of(A, s);
+        const int chunks = (sp.len + C - 1) / C;
+        float S[NT][4];
+        read_state<NT>(S, A.h0 ? A.h0 + (s * A.heads + head) * A.kdim * A.vdim : nullptr, A, col);
+        if (St::STAGES == 2 && chunks) St(smem).load(A, A.v, s, sp, 0, head, col0, tid);
+        copies_end();
+        for (int c = 0; c < chunks; ++c) {
+            const St st(smem + (St::STAGES == 2 ? (c & 1) * St::BYTES : 0));
+            if (St::STAGES == 1) St(smem).load(A, A.v, s, sp, c, head, col0, tid);
+            else if (c + 1 < chunks) St(smem + ((c + 1) & 1) * St::BYTES).load(A, A.v, s, sp, c + 1, head, col0, tid);
+            copies_end();
+            copies_wait<St::STAGES - 1>();
+            __syncthreads();
+            if (w > 0) {
+                const int n = min(C, sp.len - c * C);
+                const long long unit = (sp.chunk + c) * A.heads + head;
+                if (A.states) keep_state<K, NT>(S, (K*)A.states + (unit * A.vdim + col) * KD, w);
+                float r[8][4] = {}, o[8][4] = {};
+                float ss = 1.0f, back = 1.0f;
+                if constexpr (P::SCALED) {
+                    ss = warp_scale(S);
+                    back = inverse_of(ss);
+                }
+#pragma unroll
+                for (int d = 0; d < KD / 16; ++d) {
+                    const typename P::A a = P::split(S[2 * d], S[2 * d + 1], ss);
+#pragma unroll
+                    for (int np = 0; np < 4; ++np) {
+                        typename P::B b[2], e[2];
+                        P::by_rows(b, st.k + np * 16 * KS + d * 16, KS);
+                        P::by_rows(e, st.q + np * 16 * KS + d * 16, KS);
+                        P::full(r[2 * np], r[2 * np + 1], a, b);
+                        P::out(o[2 * np], o[2 * np + 1], a, e);
+                    }
+                }
+                // r = b (v - since r), o = since o
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float2 since = *reinterpret_cast<const float2*>(st.f + i * 8 + 2 * t4);
+                    const float2 rate = *reinterpret_cast<const float2*>(st.f + 2 * C + i * 8 + 2 * t4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float f = (e & 1 ? since.y : since.x) * back;
+                        const float v = to_f32(st.v[(i * 8 + 2 * t4 + (e & 1)) * VS + warp * 16 + g + (e >> 1) * 8]);
+                        r[i][e] = (e & 1 ? rate.y : rate.x) * fmaf(-f, r[i][e], v);
+                        o[i][e] *= f;
+                    }
+                }
+                // U = T r
+                float u[8][4] = {};
+                if constexpr (P::SCALED) ss = warp_scale(r);
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const typename P::A a = P::split(r[2 * d], r[2 * d + 1], ss);
+#pragma unroll
+                    for (int np = 0; np < 4; ++np)
+                        if (np >= d)
+                            P::template square<P::T_PLANES, true>(u[2 * np], u[2 * np + 1], a, st.t + np * 16 * MS + d * 16);
+                }
+                if constexpr (P::SCALED) {
+                    const float f = inverse_of(ss) * inverse_of(st.f[T_SCALE]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) u[i][e] *= f;
+                    ss = warp_scale(u);
+                    const float up = ss * st.f[P_SCALE];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[i][e] *= up;
+                    back = inverse_of(ss) * inverse_of(st.f[P_SCALE]);
+                }
+                // o += P U
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const typename P::A a = P::split(u[2 * d], u[2 * d + 1], ss);
+#pragma unroll
+                    for (int np = 0; np < 4; ++np)
+                        if (np >= d)
+                            P::template square<P::P_PLANES, true>(o[2 * np], o[2 * np + 1], a, st.p + np * 16 * MS + d * 16);
+                }
+                const float f = P::SCALED ? A.scale * back : A.scale;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[i][e] *= f;
+                store_tile<T, VS>(o, st.v + warp * 16, (T*)A.y.p + row_at(A, A.y, s, sp, c * C) + head * A.y.hs + col, A.y.st, n, w, A.y.vec);
+                if (A.u) {
+                    K* to = (K*)A.u + unit * C * A.vdim + col;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int t = i * 8 + 2 * t4 + (e & 1), cc = g + (e >> 1) * 8;
+                            if (cc < w) to[(long long)t * A.vdim + cc] = from_f32<K>(u[i][e]);
+                        }
+                }
+                // S = since_64 S + (until U)^T K; 1 - since_64 keeps its bits where decays are near 1
+                const float lost = st.f[LOST];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float2 until = *reinterpret_cast<const float2*>(st.f + C + i * 8 + 2 * t4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) u[i][e] *= e & 1 ? until.y : until.x;
+                }
+                if constexpr (P::SCALED) {
+                    ss = warp_scale(u);
+                    back = inverse_of(ss);
+                }
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        S[i][e] = fmaf(-lost, S[i][e], S[i][e]);
+                        if constexpr (P::SCALED) S[i][e] *= ss;
+                    }
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const typename P::A a = P::split(u[2 * d], u[2 * d + 1], ss);
+#pragma unroll
+                    for (int np = 0; np < KD / 16; ++np) {
+                        typename P::B b[2];
+                        P::by_columns(b, st.k + d * 16 * KS + np * 16, KS);
+                        P::full(S[2 * np], S[2 * np + 1], a, b);
+                    }
+                }
+                if constexpr (P::SCALED)
+#pragma unroll
+                    for (int i = 0; i < NT; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) S[i][e] *= back;
+            }
+            __syncthreads();
+        }
+        if (A.h && w > 0) write_state<NT>(S, A.h + (s * A.heads + head) * A.kdim * A.vdim, A, col);
+        copies_wait<0>();
+        __syncthreads();
+    }
+    if (A.zero) zero_rest<T>(A, A.y, A.heads, A.vdim, ((long long)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x,
+                             (long long)gridDim.x * gridDim.y * gridDim.z);
+}
+
+// ---- launches, one file per type -----------------------------------------------------
+struct DeltaSizes {
+    int squares, kept;   // bytes of T and P of a chunk; of an element kept for the gradient
+};
+template <typename T> DeltaSizes delta_sizes();
+template <typename T> void launch_prep(const DeltaArgs& A, cudaStream_t st);
+template <typename T> void launch_scan(const DeltaArgs& A, int warps, cudaStream_t st);
+
+template <typename F>
+void set_smem(F* kernel, int bytes) {
+    SNN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+}
+}  // namespace snnb_delta

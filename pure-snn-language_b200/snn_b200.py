@@ -130,7 +130,8 @@ EXPORTS = ["snn_config_init", "snn_topology_init", "snn_create", "snn_destroy",
            "snn_set_corpus_ex", "snn_load_text_corpus", "snn_byte_classes", "snn_embed",
            "snn_embed_grad", "snn_embed_grad_workspace", "snn_leaky_scan", "snn_leaky_scan_saved", "snn_leaky_scan_workspace",
            "snn_leaky_scan_grad", "snn_leaky_scan_grad_workspace", "snn_qk_norm", "snn_qk_norm_grad",
-           "snn_qk_norm_grad_workspace", "snn_adamw"]
+           "snn_qk_norm_grad_workspace", "snn_adamw", "snn_delta_scan", "snn_delta_scan_saved",
+           "snn_delta_scan_workspace", "snn_delta_scan_grad", "snn_delta_scan_grad_workspace"]
 
 _lib = None
 _lib_refmath = None
@@ -199,6 +200,11 @@ def _load(path):
     L.snn_qk_norm.argtypes = [ps, pr, pr, vp, vp, vp, vp, pr, pr, vp]
     L.snn_qk_norm_grad_workspace.argtypes = [ps, vp]
     L.snn_qk_norm_grad.argtypes = [ps, pr, pr, vp, vp, vp, vp, pr, pr, pr, pr, vp, vp, vp, i64, vp]
+    L.snn_delta_scan_saved.argtypes = [ps, vp]
+    L.snn_delta_scan_workspace.argtypes = [ps, vp]
+    L.snn_delta_scan_grad_workspace.argtypes = [ps, vp]
+    L.snn_delta_scan.argtypes = [ps, pr, pr, pr, pr, pr, vp, pr, vp, vp, i64, vp, i64, vp]
+    L.snn_delta_scan_grad.argtypes = [ps, pr, pr, pr, pr, pr, vp, i64, pr, vp, pr, pr, pr, pr, pr, vp, vp, i64, vp]
     L.snn_adamw.argtypes = [vp, i64, i32, ps, vp]
     L.snn_shard_plan.argtypes = [C.POINTER(TopologySpec), C.c_int32, C.c_int32, vp, C.c_int32]
     return L
@@ -677,6 +683,126 @@ def qk_norm_grad(q, k, dyq, dyk, q_weight=None, k_weight=None, positions=None, f
         wp = work.data_ptr()
     _call(lib().snn_qk_norm_grad, dev, stream, desc, *rows, *weights, pp, fp, *dy, *to, *dwp, wp, size)
     return (*res, *dw)
+
+
+_DELTA = struct.Struct("=iiqqqqqqQfi")  # snn_delta
+
+
+def _delta_args(q, k, v, gate, beta, scale, logit, offsets, zero):
+    """(snn_delta, (snn_heads of q, k, v, snn_rows of gate, beta), the states' shape, _delta_sizes)"""
+    if _T is None:
+        _torch()
+    dev, dtype, shape, qs = v.device, v.dtype, v.shape, q.shape
+    if dev.type != "cuda":
+        raise SnnError(1, "v must be a CUDA tensor")
+    for t, name in ((q, "q"), (k, "k"), (gate, "gate"), (beta, "beta")):
+        if t.device != dev:
+            _cuda(t, name, dev)
+    if len(shape) != (4 if offsets is None else 3) or len(qs) != len(shape):
+        raise SnnError(1, "q, k and v must be [sequences, steps, heads, dim], or [rows, heads, dim] with offsets")
+    lead, heads, dv, hk, dk = shape[:-2], shape[-2], shape[-1], qs[-2], qs[-1]
+    if not (hk and dk and dv and heads and heads % hk == 0):
+        raise SnnError(1, "the heads of v must be a multiple of those of q and k, no dimension of heads empty")
+    rows = (_heads(q, "q", (*lead, hk, dk), dtype), _heads(k, "k", (*lead, hk, dk), dtype), _heads(v, "v", shape, dtype),
+            _scan_rows(gate, "gate", (*lead, heads), dtype), _scan_rows(beta, "beta", (*lead, heads), dtype))
+    flags = SCAN_LOGIT if logit else 0
+    if offsets is None:
+        n_seq, off = shape[0], 0
+    else:
+        _cuda(offsets, "offsets", dev)
+        _require(offsets.dtype == _T.int64 and offsets.dim() == 1 and offsets.is_contiguous()
+                 and offsets.numel() >= 1, "offsets must be contiguous int64 [sequences + 1]")
+        n_seq, off = offsets.numel() - 1, offsets.data_ptr()
+        if zero:
+            flags |= SCAN_ZERO
+    kind, n = _elem(dtype), shape[-3]
+    return (_DELTA.pack(kind, flags, n_seq, n, hk, heads, dk, dv, off, scale, 0), rows, (n_seq, heads, dk, dv),
+            _delta_sizes(kind, n_seq, n, hk, heads, dk, dv, offsets is not None))
+
+
+@functools.lru_cache(maxsize=1024)
+def _delta_sizes(kind, n_seq, n, hk, heads, dk, dv, packed):
+    """(bytes of saved, workspace bytes forward, gradient) of a delta-rule scan's sizes."""
+    desc, size, L, out = _DELTA.pack(kind, 0, n_seq, n, hk, heads, dk, dv, 8 if packed else 0, 1.0, 0), C.c_int64(), lib(), []
+    for fn in (L.snn_delta_scan_saved, L.snn_delta_scan_workspace, L.snn_delta_scan_grad_workspace):
+        _check(fn(desc, C.byref(size)))
+        out.append(size.value)
+    return tuple(out)
+
+
+def delta_scan(q, k, v, gate, beta, h0=None, scale=1.0, logit=False, offsets=None, out=None, h_out=None,
+               save=False, stream=None):
+    """Delta-rule scan along whole sequences (snn_delta_scan): a state matrix S of
+    fast synapses for each head, S' = a_t S, u = b_t (v_t - S'^T k_t), S = S' + k_t u^T,
+    y_t = scale S^T q_t with a = exp(gate), b = beta, or both logistic (logit).
+
+    q, k: [sequences, steps, key heads, dk] or, with offsets (int64 [sequences
+    + 1]), packed [rows, key heads, dk]; v likewise with `heads`, a multiple of the key
+    heads, and dv; gate, beta: [.., heads]; all float32, bfloat16 or float16 alike, of any
+    strides but a unit last one; dk <= 128, dv <= 1024.  Keys are wanted of unit length
+    (qk_norm with unit=True).  h0: float32 [sequences, heads, dk, dv] (default
+    zeros).  Returns (y, h), h the float32 states after the last steps; with
+    save=True also what delta_scan_grad needs.  `out` takes y; `h_out` takes h and
+    may be h0, so that a stream of single steps keeps its state in place.  Rows of no
+    sequence are zero in a new y and not written in `out`.  autograd does not see this
+    call: delta_scan_grad is the gradient."""
+    desc, rows, state, sizes = _delta_args(q, k, v, gate, beta, scale, logit, offsets, out is None)
+    dev = v.device
+    if out is None:
+        out, yr = _new_heads(dev, stream, v.shape, v.dtype)
+    else:
+        _cuda(out, "out", dev)
+        yr = _heads(out, "out", v.shape, v.dtype)
+    if h_out is None:
+        h_out = _new(dev, stream, state, _T.float32)
+        hp = h_out.data_ptr()
+    else:
+        hp = _state(h_out, "h_out", state, dev)
+    saved = sp = wp = None
+    if save:
+        saved = _new(dev, stream, (sizes[0],), _T.uint8)
+        sp = saved.data_ptr()
+    elif sizes[1]:
+        work = _new(dev, stream, (sizes[1],), _T.uint8)
+        wp = work.data_ptr()
+    _call(lib().snn_delta_scan, dev, stream, desc, *rows, None if h0 is None else _state(h0, "h0", state, dev), yr, hp,
+          sp, sizes[0], wp, sizes[1])
+    return (out, h_out, saved) if save else (out, h_out)
+
+
+def delta_scan_grad(q, k, v, gate, beta, dy, saved, dh=None, scale=1.0, logit=False, offsets=None, need_h0=True,
+                    stream=None):
+    """Gradients of delta_scan (snn_delta_scan_grad) from those of y (dy, None for
+    none) and of the final states (dh): (dq, dk, dv, dgate, dbeta, dh0) of the forms of their
+    inputs, dh0 None where it is not needed.  The other arguments as in the forward call
+    with save=True, `saved` its result.  Rows of no sequence have the gradient 0."""
+    desc, rows, state, sizes = _delta_args(q, k, v, gate, beta, scale, logit, offsets, True)
+    dev, dtype = v.device, v.dtype
+    if dy is None and dh is None:
+        raise SnnError(1, "neither dy nor dh is given")
+    _cuda(saved, "saved", dev)
+    if saved.dtype != _T.uint8 or saved.numel() != sizes[0] or not saved.is_contiguous():
+        raise SnnError(1, "saved is not what the forward call of these sizes gives")
+    dyr = None
+    if dy is not None:
+        _cuda(dy, "dy", dev)
+        dyr = _heads(dy, "dy", v.shape, dtype)
+    dq, dqr = _new_heads(dev, stream, q.shape, dtype)
+    dk, dkr = _new_heads(dev, stream, k.shape, dtype)
+    dv, dvr = _new_heads(dev, stream, v.shape, dtype)
+    dgate, dbeta = _new(dev, stream, gate.shape, dtype), _new(dev, stream, gate.shape, dtype)
+    n = gate.shape[-1]
+    gr, br = (_ROWS.pack(t.data_ptr(), gate.shape[-2] * n, n) for t in (dgate, dbeta))
+    dh0 = hp = wp = None
+    if need_h0:
+        dh0 = _new(dev, stream, state, _T.float32)
+        hp = dh0.data_ptr()
+    if sizes[2]:
+        work = _new(dev, stream, (sizes[2],), _T.uint8)
+        wp = work.data_ptr()
+    _call(lib().snn_delta_scan_grad, dev, stream, desc, *rows, saved.data_ptr(), sizes[0], dyr,
+          None if dh is None else _state(dh, "dh", state, dev), dqr, dkr, dvr, gr, br, hp, wp, sizes[2])
+    return dq, dk, dv, dgate, dbeta, dh0
 
 
 _ADAMW_TENSOR = np.dtype([(i, np.uint64) for i in ("p", "g", "m", "v", "ms", "vs", "copy")] + [
