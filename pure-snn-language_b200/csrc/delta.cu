@@ -12,6 +12,9 @@ template <> void launch_prep<__half>(const DeltaArgs&, cudaStream_t);
 template <> void launch_scan<float>(const DeltaArgs&, int, cudaStream_t);
 template <> void launch_scan<__nv_bfloat16>(const DeltaArgs&, int, cudaStream_t);
 template <> void launch_scan<__half>(const DeltaArgs&, int, cudaStream_t);
+template <> void launch_grads<float>(const DeltaArgs&, int, cudaStream_t);
+template <> void launch_grads<__nv_bfloat16>(const DeltaArgs&, int, cudaStream_t);
+template <> void launch_grads<__half>(const DeltaArgs&, int, cudaStream_t);
 }  // namespace snnb_delta
 
 namespace {
@@ -288,14 +291,47 @@ void delta_scan(const snn_delta* d, const snn_heads* q, const snn_heads* k, cons
 }  // namespace snnb
 
 namespace snnb {
+
 int64_t delta_scan_grad_workspace(const snn_delta* d) {
     check_desc(d);
-    return 0;
+    const Layout l = layout_of(d);
+    return l.kept_all - l.states;
 }
-void delta_scan_grad(const snn_delta*, const snn_heads*, const snn_heads*, const snn_heads*, const snn_rows*,
-                     const snn_rows*, const void*, int64_t, const snn_heads*, const float*, const snn_heads*,
-                     const snn_heads*, const snn_heads*, const snn_rows*, const snn_rows*, float*, void*, int64_t,
-                     cudaStream_t) {
-    throw Error(SNN_ERR_UNSUPPORTED, "delta: no gradient yet");
+
+void delta_scan_grad(const snn_delta* d, const snn_heads* q, const snn_heads* k, const snn_heads* v, const snn_rows* gate,
+                     const snn_rows* beta, const void* saved, int64_t saved_bytes, const snn_heads* dy, const float* dh,
+                     const snn_heads* dq, const snn_heads* dk, const snn_heads* dv, const snn_rows* dgate,
+                     const snn_rows* dbeta, float* dh0, void* work, int64_t work_bytes, cudaStream_t st) {
+    check_desc(d);
+    SNN_REQUIRE(dy || dh, SNN_ERR_ARG, "delta: neither dy nor dh");
+    DeltaArgs A = base_args(d, q, k, v, gate, beta);
+    if (dy) A.dy = heads_of(d, dy, d->heads, d->v_dim, "dy");
+    else A.dy.vec = 1;
+    A.dq = heads_of(d, dq, d->k_heads, d->k_dim, "dq", true);
+    A.dk = heads_of(d, dk, d->k_heads, d->k_dim, "dk", true);
+    A.dv = heads_of(d, dv, d->heads, d->v_dim, "dv", true);
+    A.dgate = gates_of(d, dgate, "dgate", true);
+    A.dbeta = gates_of(d, dbeta, "dbeta", true);
+    check_states({dh, dh0});
+    A.dh = dh;
+    A.dh0 = dh0;
+    zero_rows(d, A, A.dq, A.hk, A.kdim, st);
+    zero_rows(d, A, A.dk, A.hk, A.kdim, st);
+    zero_rows(d, A, A.dv, A.heads, A.vdim, st);
+    zero_rows(d, A, A.dgate, A.heads, 1, st);
+    zero_rows(d, A, A.dbeta, A.heads, 1, st);
+    if (d->n_seq == 0) return;
+    const Layout l = layout_of(d);
+    check_work(saved, saved_bytes, l.kept_all, "saved");
+    check_work(work, work_bytes, l.kept_all - l.states, "workspace");
+    char* base = (char*)saved;
+    A.squares = base;
+    A.factors = (float*)(base + l.factors);
+    A.states = base + l.states;
+    A.u = base + l.u;
+    A.dstates = (char*)work;
+    A.dr = (char*)work + (l.u - l.states);
+    with_elem(d->type, [&](auto t) { launch_grads<decltype(t)>(A, warps_of(d), st); });
 }
+
 }  // namespace snnb

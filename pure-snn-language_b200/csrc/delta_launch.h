@@ -42,6 +42,28 @@ void launch_scan_of(const DeltaArgs& A, int warps, cudaStream_t st) {
     });
     SNN_CUDA(cudaGetLastError());
 }
+template <typename T>
+void launch_grads_of(const DeltaArgs& A, int warps, cudaStream_t st) {
+    using P = typename PathOf<T>::P;
+    by_dim<T>(A.kdim, [&](auto kd) {
+        constexpr int KD = decltype(kd)::value;
+        by_warps(warps, [&](auto nw) {
+            constexpr int NW = decltype(nw)::value;
+            using S = Stage<P, KD, NW>;
+            auto* kernel = k_delta_back<P, KD, NW>;
+            set_smem(kernel, S::STAGES * S::BYTES);
+            const dim3 grid((unsigned)std::min<long long>(A.n_seq, 1 << 30), (unsigned)A.heads,
+                            (unsigned)((A.vdim + S::VW - 1) / S::VW));
+            kernel<<<grid, NW * 32, S::STAGES * S::BYTES, st>>>(A);
+            SNN_CUDA(cudaGetLastError());
+        });
+        if (!A.slots) return;
+        auto* kernel = k_delta_grads<T, KD>;
+        set_smem(kernel, GradTile<T, KD>::BYTES);
+        kernel<<<dim3((unsigned)A.slots, (unsigned)A.hk), GRADS, GradTile<T, KD>::BYTES, st>>>(A);
+        SNN_CUDA(cudaGetLastError());
+    });
+}
 }  // namespace snnb_delta
 
 #define SNN_DELTA_LAUNCHES(T)                                                                        \
@@ -49,4 +71,5 @@ void launch_scan_of(const DeltaArgs& A, int warps, cudaStream_t st) {
         return {PathOf<T>::P::SQUARES, (int)sizeof(Kept<T>::K)};                                     \
     }                                                                                                \
     template <> void launch_prep<T>(const DeltaArgs& A, cudaStream_t st) { launch_prep_of<T>(A, st); } \
-    template <> void launch_scan<T>(const DeltaArgs& A, int warps, cudaStream_t st) { launch_scan_of<T>(A, warps, st); }
+    template <> void launch_scan<T>(const DeltaArgs& A, int warps, cudaStream_t st) { launch_scan_of<T>(A, warps, st); } \
+    template <> void launch_grads<T>(const DeltaArgs& A, int warps, cudaStream_t st) { launch_grads_of<T>(A, warps, st); }

@@ -178,7 +178,7 @@ struct Path16 {
     using T = T_;
     static constexpr int N = N_;
     static constexpr bool SCALED = std::is_same<T, __half>::value;  // pieces keep their bits near 1 only
-    static constexpr int T_PLANES = N, P_PLANES = 2, STAGES = 2;
+    static constexpr int T_PLANES = N, P_PLANES = N, STAGES = 2;
     using Sq = T;             // elements of T's and P's planes
     static constexpr int PLANE = C * MS, SQUARES = (T_PLANES + P_PLANES) * PLANE * 2;
     struct A {
@@ -384,6 +384,56 @@ __device__ __forceinline__ float warp_scale(const float (&x)[N][4]) {
     return scale_for(top);
 }
 
+// By one warp: sums of the logarithms of a chunk's decays (64 bits: differences of them
+// are what counts) but for those of decays of 0, which are counted apart, and the rates
+template <typename T>
+__device__ __forceinline__ void chunk_decays(const DeltaArgs& A, long long s, const Span& sp, int t0, int n, int head, int lane,
+                                             double* up, int* cut, float* rate) {
+    double l[2];
+    int z[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int t = 2 * lane + i;
+        float lg = 0.0f, r = 0.0f;
+        if (t < n) {
+            lg = log_decay(A, ((const T*)A.gate.p)[row_at(A, A.gate, s, sp, t0 + t) + head * A.gate.hs]);
+            r = rate_of(A, ((const T*)A.beta.p)[row_at(A, A.beta, s, sp, t0 + t) + head * A.beta.hs]);
+        }
+        z[i] = lg == -INFINITY;
+        l[i] = z[i] ? 0.0 : (double)lg;
+        rate[t] = r;
+    }
+    double sum = l[0] + l[1];
+    int cuts = z[0] + z[1];
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const double d = __shfl_up_sync(~0u, sum, o);
+        const int c = __shfl_up_sync(~0u, cuts, o);
+        if (lane >= o) {
+            sum += d;
+            cuts += c;
+        }
+    }
+    up[2 * lane] = sum - l[1];
+    up[2 * lane + 1] = sum;
+    cut[2 * lane] = cuts - z[1];
+    cut[2 * lane + 1] = cuts;
+}
+__device__ __forceinline__ float decay_between(const double* up, const int* cut, int i, int j) {
+    return cut[i] == cut[j] ? expf((float)(up[i] - up[j])) : 0.0f;
+}
+// the sequence that chunk `slot` belongs to, the last that does not begin behind it
+__device__ __forceinline__ long long sequence_of(const DeltaArgs& A, long long slot) {
+    if (!A.off) return slot / ((A.n_steps + C - 1) / C);
+    long long lo = 0, hi = A.n_seq - 1;
+    while (lo < hi) {
+        const long long mid = (lo + hi + 1) / 2;
+        if (span_of(A, mid).chunk <= slot) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
 // ---- T, P and the factors of every chunk ------------------------------------------
 constexpr int PREP = 128;
 template <class P, int KD>
@@ -396,24 +446,12 @@ __global__ void __launch_bounds__(PREP) k_delta_prep(const __grid_constant__ Del
     extern __shared__ __align__(16) char smem[];
     T *K = reinterpret_cast<T*>(smem), *Q = K + C * (KD + PAD);
     float* M = reinterpret_cast<float*>(Q + C * (KD + PAD));  // [C][C + 4]: A, then T
-    __shared__ double up[C];   // sums of the logarithms of the decays but for those that are 0
-    __shared__ int cut[C];     // how many are
+    __shared__ double up[C];
+    __shared__ int cut[C];
     __shared__ float rate[C], top[2][4];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, head = blockIdx.y;
     const long long slot = blockIdx.x;
-    // the sequence of this chunk
-    long long s = 0;
-    if (A.off) {
-        long long lo = 0, hi = A.n_seq - 1;
-        while (lo < hi) {
-            const long long mid = (lo + hi + 1) / 2;
-            if (span_of(A, mid).chunk <= slot) lo = mid;
-            else hi = mid - 1;
-        }
-        s = lo;
-    } else {
-        s = slot / ((A.n_steps + C - 1) / C);
-    }
+    const long long s = sequence_of(A, slot);
     const Span sp = span_of(A, s);
     const long long t0 = (slot - sp.chunk) * C;
     if (t0 < 0 || t0 >= sp.len) return;
@@ -421,37 +459,7 @@ __global__ void __launch_bounds__(PREP) k_delta_prep(const __grid_constant__ Del
     load_rows<T, KD>(K, (const T*)A.k.p + row_at(A, A.k, s, sp, (int)t0) + kh * A.k.hs, A.k.st, n, A.kdim, A.k.vec, tid, PREP);
     load_rows<T, KD>(Q, (const T*)A.q.p + row_at(A, A.q, s, sp, (int)t0) + kh * A.q.hs, A.q.st, n, A.kdim, A.q.vec, tid, PREP);
     copies_end();
-    if (warp == 0) {
-        double l[2];
-        int z[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int t = 2 * lane + i;
-            float lg = 0.0f, r = 0.0f;
-            if (t < n) {
-                lg = log_decay(A, ((const T*)A.gate.p)[row_at(A, A.gate, s, sp, (int)t0 + t) + head * A.gate.hs]);
-                r = rate_of(A, ((const T*)A.beta.p)[row_at(A, A.beta, s, sp, (int)t0 + t) + head * A.beta.hs]);
-            }
-            z[i] = lg == -INFINITY;
-            l[i] = z[i] ? 0.0 : (double)lg;
-            rate[t] = r;
-        }
-        double sum = l[0] + l[1];
-        int cuts = z[0] + z[1];
-#pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-            const double d = __shfl_up_sync(~0u, sum, o);
-            const int c = __shfl_up_sync(~0u, cuts, o);
-            if (lane >= o) {
-                sum += d;
-                cuts += c;
-            }
-        }
-        up[2 * lane] = sum - l[1];
-        up[2 * lane + 1] = sum;
-        cut[2 * lane] = cuts - z[1];
-        cut[2 * lane + 1] = cuts;
-    }
+    if (warp == 0) chunk_decays<T>(A, s, sp, (int)t0, n, head, lane, up, cut, rate);
     copies_wait<0>();
     __syncthreads();
     const long long unit = slot * A.heads + head;
@@ -459,7 +467,7 @@ __global__ void __launch_bounds__(PREP) k_delta_prep(const __grid_constant__ Del
     typename P::Sq *Tm = reinterpret_cast<typename P::Sq*>(A.squares + unit * P::SQUARES), *Pm = Tm + P::T_PLANES * P::PLANE;
     if (tid < C) {
         F[tid] = cut[tid] ? 0.0f : expf((float)up[tid]);
-        F[C + tid] = cut[tid] == cut[C - 1] ? expf((float)(up[C - 1] - up[tid])) : 0.0f;
+        F[C + tid] = decay_between(up, cut, C - 1, tid);
         F[2 * C + tid] = rate[tid];
         if (tid == 0) F[LOST] = cut[C - 1] ? 1.0f : -expm1f((float)up[C - 1]);
     }
@@ -481,7 +489,7 @@ __global__ void __launch_bounds__(PREP) k_delta_prep(const __grid_constant__ Del
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int i = warp * 16 + g + (e >> 1) * 8, j = nt * 8 + 2 * t4 + (e & 1);
-            const float G = j <= i && cut[i] == cut[j] ? expf((float)(up[i] - up[j])) : 0.0f;
+            const float G = j <= i ? decay_between(up, cut, i, j) : 0.0f;
             // (a factor of 0 takes all: what lies above the diagonal may be anything)
             qk[nt][e] = j <= i && G != 0.0f ? G * qk[nt][e] : 0.0f;
             const float a = rate[i] * G;
@@ -564,15 +572,15 @@ struct Stage {
         f = reinterpret_cast<float*>(m + 2 * KEYS + VALUES + P::SQUARES);
     }
     // chunk c of sequence s; v: the values' rows or, backward, those of dy
-    __device__ __forceinline__ void load(const DeltaArgs& A, const Heads& vals, long long s, const Span& sp, int c, int head,
-                                         int col0, int tid) {
+    __device__ __forceinline__ void load(const DeltaArgs& A, const Heads& vals, int squares, long long s, const Span& sp, int c,
+                                         int head, int col0, int tid) {
         const int n = min(C, sp.len - c * C), kh = head / A.group;
         const long long unit = (sp.chunk + c) * A.heads + head;
         load_rows<T, KD>(k, (const T*)A.k.p + row_at(A, A.k, s, sp, c * C) + kh * A.k.hs, A.k.st, n, A.kdim, A.k.vec, tid, NW * 32);
         load_rows<T, KD>(q, (const T*)A.q.p + row_at(A, A.q, s, sp, c * C) + kh * A.q.hs, A.q.st, n, A.kdim, A.q.vec, tid, NW * 32);
-        load_rows<T, VW>(v, (const T*)vals.p + row_at(A, vals, s, sp, c * C) + head * vals.hs + col0, vals.st, n,
-                         A.vdim - col0, vals.vec, tid, NW * 32);
-        load_words(t, A.squares + unit * P::SQUARES, P::SQUARES, tid, NW * 32);
+        load_rows<T, VW>(v, (const T*)vals.p + row_at(A, vals, s, sp, c * C) + head * vals.hs + col0, vals.st,
+                         vals.p ? n : 0, A.vdim - col0, vals.vec, tid, NW * 32);
+        load_words(t, A.squares + unit * P::SQUARES, squares, tid, NW * 32);
         load_words(f, A.factors + unit * SC, SC * 4, tid, NW * 32);
     }
 };
@@ -676,6 +684,8 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_scan(const __grid_constant
     using St = Stage<P, KD, NW>;
     using K = typename Kept<T>::K;
     constexpr int NT = KD / 8, KS = KD + PAD, VS = St::VW + PAD;
+    constexpr int OUT = P::P_PLANES < 2 ? 1 : 2;  // pieces of P that reach a rounded result
+    constexpr int SQUARES = (P::T_PLANES + OUT) * P::PLANE * (int)sizeof(typename P::Sq);
     extern __shared__ __align__(16) char smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
     const int head = blockIdx.y, col0 = (int)blockIdx.z * St::VW, col = col0 + warp * 16;
@@ -685,12 +695,12 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_scan(const __grid_constant
         const int chunks = (sp.len + C - 1) / C;
         float S[NT][4];
         read_state<NT>(S, A.h0 ? A.h0 + (s * A.heads + head) * A.kdim * A.vdim : nullptr, A, col);
-        if (St::STAGES == 2 && chunks) St(smem).load(A, A.v, s, sp, 0, head, col0, tid);
+        if (St::STAGES == 2 && chunks) St(smem).load(A, A.v, SQUARES, s, sp, 0, head, col0, tid);
         copies_end();
         for (int c = 0; c < chunks; ++c) {
             const St st(smem + (St::STAGES == 2 ? (c & 1) * St::BYTES : 0));
-            if (St::STAGES == 1) St(smem).load(A, A.v, s, sp, c, head, col0, tid);
-            else if (c + 1 < chunks) St(smem + ((c + 1) & 1) * St::BYTES).load(A, A.v, s, sp, c + 1, head, col0, tid);
+            if (St::STAGES == 1) St(smem).load(A, A.v, SQUARES, s, sp, c, head, col0, tid);
+            else if (c + 1 < chunks) St(smem + ((c + 1) & 1) * St::BYTES).load(A, A.v, SQUARES, s, sp, c + 1, head, col0, tid);
             copies_end();
             copies_wait<St::STAGES - 1>();
             __syncthreads();
@@ -761,7 +771,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_scan(const __grid_constant
 #pragma unroll
                     for (int np = 0; np < 4; ++np)
                         if (np >= d)
-                            P::template square<P::P_PLANES, true>(o[2 * np], o[2 * np + 1], a, st.p + np * 16 * MS + d * 16);
+                            P::template square<OUT, true>(o[2 * np], o[2 * np + 1], a, st.p + np * 16 * MS + d * 16);
                 }
                 const float f = P::SCALED ? A.scale * back : A.scale;
 #pragma unroll
@@ -824,6 +834,534 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_scan(const __grid_constant
                              (long long)gridDim.x * gridDim.y * gridDim.z);
 }
 
+// ---- gradients: the states' along the sequences, from the last chunk ------------------
+// With D the gradient of the state behind a chunk, Z = scale dy:
+//   dU = P^T Z + until K D,   R = T^T dU,   dV = b R,
+//   D <- since_64 D + (since Z)^T Q - (since b R)^T K   (the transposed scan, in the same layout)
+template <class P, int KD, int NW>
+__global__ void __launch_bounds__(NW * 32, 1) k_delta_back(const __grid_constant__ DeltaArgs A) {
+    using T = typename P::T;
+    using St = Stage<P, KD, NW>;
+    using K = typename Kept<T>::K;
+    constexpr int NT = KD / 8, KS = KD + PAD, VS = St::VW + PAD;
+    extern __shared__ __align__(16) char smem[];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+    const int head = blockIdx.y, col0 = (int)blockIdx.z * St::VW, col = col0 + warp * 16;
+    const int w = A.vdim - col;
+    for (long long s = blockIdx.x; s < A.n_seq; s += gridDim.x) {
+        const Span sp = span_of(A, s);
+        const int chunks = (sp.len + C - 1) / C;
+        float D[NT][4];
+        read_state<NT>(D, A.dh ? A.dh + (s * A.heads + head) * A.kdim * A.vdim : nullptr, A, col);
+        if (St::STAGES == 2 && chunks) St(smem).load(A, A.dy, P::SQUARES, s, sp, chunks - 1, head, col0, tid);
+        copies_end();
+        for (int i = 0; i < chunks; ++i) {
+            const int c = chunks - 1 - i;
+            const St st(smem + (St::STAGES == 2 ? (i & 1) * St::BYTES : 0));
+            if (St::STAGES == 1) St(smem).load(A, A.dy, P::SQUARES, s, sp, c, head, col0, tid);
+            else if (c > 0) St(smem + ((i + 1) & 1) * St::BYTES).load(A, A.dy, P::SQUARES, s, sp, c - 1, head, col0, tid);
+            copies_end();
+            copies_wait<St::STAGES - 1>();
+            __syncthreads();
+            if (w > 0) {
+                const int n = min(C, sp.len - c * C);
+                const long long unit = (sp.chunk + c) * A.heads + head;
+                keep_state<K, NT>(D, (K*)A.dstates + (unit * A.vdim + col) * KD, w);
+                float u[8][4] = {}, r[8][4] = {}, z[8][4];
+                float ss = 1.0f, back = 1.0f;
+                if constexpr (P::SCALED) {
+                    ss = warp_scale(D);
+                    back = inverse_of(ss);
+                }
+#pragma unroll
+                for (int d = 0; d < KD / 16; ++d) {
+                    const typename P::A a = P::split(D[2 * d], D[2 * d + 1], ss);
+#pragma unroll
+                    for (int np = 0; np < 4; ++np) {
+                        typename P::B b[2];
+                        P::by_rows(b, st.k + np * 16 * KS + d * 16, KS);
+                        P::full(u[2 * np], u[2 * np + 1], a, b);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float2 until = *reinterpret_cast<const float2*>(st.f + C + j * 8 + 2 * t4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        u[j][e] *= (e & 1 ? until.y : until.x) * back;
+                        z[j][e] = A.scale * to_f32(st.v[(j * 8 + 2 * t4 + (e & 1)) * VS + warp * 16 + g + (e >> 1) * 8]);
+                    }
+                }
+                if constexpr (P::SCALED) {
+                    ss = warp_scale(z);
+                    const float f = ss * st.f[P_SCALE];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) u[j][e] *= f;
+                }
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const typename P::A a = P::split(z[2 * d], z[2 * d + 1], ss);
+#pragma unroll
+                    for (int np = 0; np < 4; ++np)
+                        if (np <= d)
+                            P::template square<P::P_PLANES, false>(u[2 * np], u[2 * np + 1], a, st.p + d * 16 * MS + np * 16);
+                }
+                if constexpr (P::SCALED) {
+                    back = inverse_of(ss) * inverse_of(st.f[P_SCALE]);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) u[j][e] *= back;
+                    ss = warp_scale(u);
+                }
+                // R = T^T dU
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const typename P::A a = P::split(u[2 * d], u[2 * d + 1], ss);
+#pragma unroll
+                    for (int np = 0; np < 4; ++np)
+                        if (np <= d)
+                            P::template square<P::T_PLANES, false>(r[2 * np], r[2 * np + 1], a, st.t + d * 16 * MS + np * 16);
+                }
+                const float f = P::SCALED ? inverse_of(ss) * inverse_of(st.f[T_SCALE]) : 1.0f;
+                K* to = (K*)A.dr + unit * C * A.vdim + col;
+                // u <- -since b R, z <- since Z
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float2 since = *reinterpret_cast<const float2*>(st.f + j * 8 + 2 * t4);
+                    const float2 rate = *reinterpret_cast<const float2*>(st.f + 2 * C + j * 8 + 2 * t4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int t = j * 8 + 2 * t4 + (e & 1), cc = g + (e >> 1) * 8;
+                        if constexpr (P::SCALED) r[j][e] *= f;
+                        if (cc < w) to[(long long)t * A.vdim + cc] = from_f32<K>(r[j][e]);
+                        const float si = e & 1 ? since.y : since.x;
+                        r[j][e] *= e & 1 ? rate.y : rate.x;
+                        u[j][e] = -si * r[j][e];
+                        z[j][e] *= si;
+                    }
+                }
+                const float lost = st.f[LOST];
+                if constexpr (P::SCALED) {
+                    ss = fminf(warp_scale(u), warp_scale(z));
+                    back = inverse_of(ss);
+                }
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        D[j][e] = fmaf(-lost, D[j][e], D[j][e]);
+                        if constexpr (P::SCALED) D[j][e] *= ss;
+                    }
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const typename P::A a = P::split(z[2 * d], z[2 * d + 1], ss), m = P::split(u[2 * d], u[2 * d + 1], ss);
+#pragma unroll
+                    for (int np = 0; np < KD / 16; ++np) {
+                        typename P::B b[2];
+                        P::by_columns(b, st.q + d * 16 * KS + np * 16, KS);
+                        P::full(D[2 * np], D[2 * np + 1], a, b);
+                        P::by_columns(b, st.k + d * 16 * KS + np * 16, KS);
+                        P::full(D[2 * np], D[2 * np + 1], m, b);
+                    }
+                }
+                if constexpr (P::SCALED)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) D[j][e] *= back;
+                store_tile<T, VS>(r, st.v + warp * 16, (T*)A.dv.p + row_at(A, A.dv, s, sp, c * C) + head * A.dv.hs + col, A.dv.st, n, w, A.dv.vec);
+            }
+            __syncthreads();
+        }
+        if (A.dh0 && w > 0) write_state<NT>(D, A.dh0 + (s * A.heads + head) * A.kdim * A.vdim, A, col);
+        copies_wait<0>();
+        __syncthreads();
+    }
+}
+
+// ---- gradients: what is left, for all chunks at once -------------------------------------
+// With S before a chunk, D behind it, U and R as above, G the decays between steps:
+//   p = G (Z U^T) (j <= i),   x = -b G (R U^T) (j < i)
+//   dQ = since Z S^T + p K,   dK = -since b R S^T + until U D^T + x K + x^T K + p^T Q
+//   db_i = R_i.V_i - since_i k_i.(S R_i) + sum_j x_ij k_i.k_j / b_i
+// and for the logarithm of a decay all terms that it is a factor of: their sum over
+// i >= t > j, as sums over rows less sums over columns from t on.
+// Operands are bf16 for bf16 tensors (the results are rounded to that), otherwise f32 in
+// two tf32 pieces.  16 warps: 16 rows and a quarter of the columns each.
+template <typename T> struct GradOps;
+template <> struct GradOps<__nv_bfloat16> {
+    using E = __nv_bfloat16;
+    struct A {
+        unsigned v[4];
+    };
+    using P = Path16<__nv_bfloat16, 3>;
+    using B = P::B;
+    static __device__ __forceinline__ A by_rows(const E* m, int st) {  // A[m][k] = x[m][k]
+        const int l = threadIdx.x & 31;
+        A a;
+        ldsm4(a.v, m + (l & 15) * st + (l >> 4) * 8);
+        return a;
+    }
+    static __device__ __forceinline__ A by_columns(const E* m, int st) {  // A[m][k] = x[k][m]
+        const int l = threadIdx.x & 31;
+        A a;
+        ldsm4t(a.v, m + ((l >> 4) * 8 + (l & 7)) * st + ((l >> 3) & 1) * 8);
+        return a;
+    }
+    static __device__ __forceinline__ void mma(float (&d0)[4], float (&d1)[4], const A& a, const B (&b)[2]) {
+        mma16<E>(d0, a.v, b[0].v);
+        mma16<E>(d1, a.v, b[1].v);
+    }
+    static __device__ __forceinline__ void put(E* m, float x, float y) { *reinterpret_cast<unsigned*>(m) = pair_of<E>(x, y); }
+};
+template <> struct GradOps<float> {
+    using E = float;
+    using A = Path32::A;
+    using P = Path32;
+    using B = P::B;
+    static __device__ __forceinline__ A by_rows(const float* m, int st) {
+        const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+        A a;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float2 v = *reinterpret_cast<const float2*>(m + (i * 8 + g) * st + k * 8 + 2 * t);
+                tf32_split(v.x, a.h[4 * k + i], a.l[4 * k + i]);
+                tf32_split(v.y, a.h[4 * k + 2 + i], a.l[4 * k + 2 + i]);
+            }
+        return a;
+    }
+    static __device__ __forceinline__ A by_columns(const float* m, int st) {
+        const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+        A a;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    tf32_split(m[(k * 8 + 2 * t + j) * st + i * 8 + g], a.h[4 * k + 2 * j + i], a.l[4 * k + 2 * j + i]);
+        return a;
+    }
+    static __device__ __forceinline__ void mma(float (&d0)[4], float (&d1)[4], const A& a, const B (&b)[2]) { P::full(d0, d1, a, b); }
+    static __device__ __forceinline__ void put(float* m, float x, float y) { *reinterpret_cast<float2*>(m) = make_float2(x, y); }
+};
+template <> struct GradOps<__half> : GradOps<float> {};
+
+// R rows of W columns of F as E, r and w of them there, zeros in the others
+template <typename E, int R, int W, typename F>
+__device__ __forceinline__ void load_as(E* to, const F* from, long long st, int r, int w, bool vec, int tid, int threads) {
+    if constexpr (std::is_same<E, F>::value)
+        if (vec) {
+            constexpr int V = 16 / (int)sizeof(E), N = W / V;
+            for (int i = tid; i < R * N; i += threads) {
+                const int a = i / N, c = (i - a * N) * V;
+                const bool there = a < r && c < w;
+                copy16(to + a * (W + PAD) + c, there ? from + a * st + c : from, there);
+            }
+            return;
+        }
+    for (int i = tid; i < R * W; i += threads) {
+        const int a = i / W, c = i - a * W;
+        to[a * (W + PAD) + c] = from_f32<E>(a < r && c < w ? to_f32(from[a * st + c]) : 0.0f);
+    }
+}
+
+constexpr int GRADS = 512, GW = 32;  // threads; columns of the values taken at a time
+template <typename T, int KD>
+struct GradTile {
+    using E = typename GradOps<T>::E;
+    static constexpr int KEYS = C * (KD + PAD), ROWS = C * (GW + PAD), STATE = GW * (KD + PAD);
+    static constexpr int BLOCK = 4 * ROWS + 2 * STATE, SQ = C * MS;
+    static constexpr int STAGES = sizeof(E) == 2 ? 2 : 1;
+    // the squares take the blocks' place, or what they are short of it
+    static constexpr int ELEMS = 2 * KEYS + (STAGES * BLOCK > 2 * SQ ? STAGES * BLOCK : 2 * SQ);
+    static constexpr int BYTES = ELEMS * (int)sizeof(E);
+};
+
+template <typename T, int KD>
+__global__ void __launch_bounds__(GRADS, 1) k_delta_grads(const __grid_constant__ DeltaArgs A) {
+    using Op = GradOps<T>;
+    using G = GradTile<T, KD>;
+    using E = typename G::E;
+    using K = typename Kept<T>::K;
+    static_assert(std::is_same<E, K>::value, "what is kept is an operand");
+    constexpr int KS = KD + PAD, RS = GW + PAD, NQ = KD / 32;  // NQ: tiles of 8 columns of a warp
+    extern __shared__ __align__(16) char smem[];
+    E *Ks = reinterpret_cast<E*>(smem), *Qs = Ks + G::KEYS, *blocks = Qs + G::KEYS;
+    E *Ps = blocks, *Xs = blocks + G::SQ;
+    __shared__ double up[C];
+    __shared__ int cut[C];
+    __shared__ float rate[C], since[C], until[C], rows[4][4][C], cols[4][C], more[GRADS / 32], dots[C];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+    const int wr = warp & 3, wc = warp >> 2, kh = blockIdx.y;
+    const long long slot = blockIdx.x, s = sequence_of(A, slot);
+    const Span sp = span_of(A, s);
+    const long long first = (slot - sp.chunk) * C;
+    if (first < 0 || first >= sp.len) return;
+    const int t0 = (int)first, n = min(C, sp.len - t0);
+    load_as<E, C, KD>(Ks, (const T*)A.k.p + row_at(A, A.k, s, sp, t0) + kh * A.k.hs, A.k.st, n, A.kdim, A.k.vec, tid, GRADS);
+    load_as<E, C, KD>(Qs, (const T*)A.q.p + row_at(A, A.q, s, sp, t0) + kh * A.q.hs, A.q.st, n, A.kdim, A.q.vec, tid, GRADS);
+    float tq[NQ][4] = {}, tk[NQ][4] = {};
+#pragma unroll 1
+    for (int gi = 0; gi < A.group; ++gi) {
+        const int head = kh * A.group + gi;
+        const long long unit = slot * A.heads + head;
+        const bool kvec = A.vdim % (16 / (int)sizeof(K)) == 0;
+        auto load = [&](int b) {
+            E* m = blocks + (G::STAGES == 2 ? (b & 1) * G::BLOCK : 0);
+            const int c0 = b * GW, w = A.vdim - c0;
+            load_as<E, C, GW>(m, (const T*)A.dy.p + row_at(A, A.dy, s, sp, t0) + head * A.dy.hs + c0, A.dy.st, A.dy.p ? n : 0, w, A.dy.vec, tid, GRADS);
+            load_as<E, C, GW>(m + G::ROWS, (const K*)A.u + unit * C * A.vdim + c0, A.vdim, C, w, kvec, tid, GRADS);
+            load_as<E, C, GW>(m + 2 * G::ROWS, (const K*)A.dr + unit * C * A.vdim + c0, A.vdim, C, w, kvec, tid, GRADS);
+            load_as<E, C, GW>(m + 3 * G::ROWS, (const T*)A.v.p + row_at(A, A.v, s, sp, t0) + head * A.v.hs + c0, A.v.st, n, w, A.v.vec, tid, GRADS);
+            load_as<E, GW, KD>(m + 4 * G::ROWS, (const K*)A.states + (unit * A.vdim + c0) * KD, KD, w, KD, true, tid, GRADS);
+            load_as<E, GW, KD>(m + 4 * G::ROWS + G::STATE, (const K*)A.dstates + (unit * A.vdim + c0) * KD, KD, w, KD, true, tid, GRADS);
+        };
+        const int n_blocks = (A.vdim + GW - 1) / GW;
+        if (G::STAGES == 2) load(0);
+        copies_end();
+        if (warp == 0) chunk_decays<T>(A, s, sp, t0, n, head, lane, up, cut, rate);
+        __syncthreads();
+        if (tid < C) {
+            since[tid] = cut[tid] ? 0.0f : expf((float)up[tid]);
+            until[tid] = decay_between(up, cut, C - 1, tid);
+        }
+        float zq[NQ][4] = {}, zk[NQ][4] = {}, zm[NQ][4] = {}, p[2][4] = {}, x[2][4] = {};
+        float inner = 0.0f, rv = 0.0f;  // <S, D>; R_i.V_i of row tid / 8
+#pragma unroll 1
+        for (int b = 0; b < n_blocks; ++b) {
+            if (G::STAGES == 1) load(b);
+            else if (b + 1 < n_blocks) load(b + 1);
+            copies_end();
+            copies_wait<G::STAGES - 1>();
+            __syncthreads();
+            const E* m = blocks + (G::STAGES == 2 ? (b & 1) * G::BLOCK : 0);
+            const E *Z = m, *U = m + G::ROWS, *R = m + 2 * G::ROWS, *V = m + 3 * G::ROWS, *S = m + 4 * G::ROWS, *D = S + G::STATE;
+#pragma unroll
+            for (int k = 0; k < GW; k += 16) {
+                const typename Op::A az = Op::by_rows(Z + wr * 16 * RS + k, RS), ar = Op::by_rows(R + wr * 16 * RS + k, RS);
+                const typename Op::A au = Op::by_rows(U + wr * 16 * RS + k, RS);
+                typename Op::B bb[2];
+#pragma unroll
+                for (int j = 0; j < NQ; j += 2) {
+                    Op::P::by_columns(bb, S + k * KS + wc * (KD / 4) + j * 8, KS);
+                    Op::mma(zq[j], zq[j + 1], az, bb);
+                    Op::mma(zk[j], zk[j + 1], ar, bb);
+                    Op::P::by_columns(bb, D + k * KS + wc * (KD / 4) + j * 8, KS);
+                    Op::mma(zm[j], zm[j + 1], au, bb);
+                }
+                if (wc <= wr) {
+                    Op::P::by_rows(bb, U + wc * 16 * RS + k, RS);
+                    Op::mma(p[0], p[1], az, bb);
+                    Op::mma(x[0], x[1], ar, bb);
+                }
+            }
+            const int row = tid >> 3, e0 = (tid & 7) * (GW / 8);
+#pragma unroll
+            for (int e = 0; e < GW / 8; ++e) rv = fmaf(to_f32(R[row * RS + e0 + e]), to_f32(V[row * RS + e0 + e]), rv);
+            for (int e = tid; e < GW * KD; e += GRADS) {
+                const int at = e / KD * KS + e % KD;
+                inner = fmaf(to_f32(S[at]), to_f32(D[at]), inner);
+            }
+            __syncthreads();
+        }
+        copies_wait<0>();
+        // the products' sums of rows and columns, for the decays and rates
+        float kk[2][4] = {}, qk[2][4] = {};
+        if (wc <= wr) {
+#pragma unroll 2
+            for (int d = 0; d < KD; d += 16) {
+                typename Op::B bb[2];
+                Op::P::by_rows(bb, Ks + wc * 16 * KS + d, KS);
+                Op::mma(kk[0], kk[1], Op::by_rows(Ks + wr * 16 * KS + d, KS), bb);
+                Op::mma(qk[0], qk[1], Op::by_rows(Qs + wr * 16 * KS + d, KS), bb);
+            }
+        }
+        float by_row[4][2] = {}, by_col[2][2] = {};  // q.dQ + b k.., k..until, R part of db, sum of x k.k / b; columns
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = wr * 16 + g + (e >> 1) * 8, jj = wc * 16 + j * 8 + 2 * t4 + (e & 1);
+                const float d = jj <= i ? decay_between(up, cut, i, jj) : 0.0f;
+                const float pv = d != 0.0f ? A.scale * d * p[j][e] : 0.0f, xv = d != 0.0f && jj < i ? -d * x[j][e] : 0.0f;
+                const float xr = xv * kk[j][e], mp = pv * qk[j][e], both = fmaf(rate[i], xr, mp);
+                by_row[0][e >> 1] += both;
+                by_row[3][e >> 1] += xr;
+                by_col[j][e & 1] += both;
+                p[j][e] = pv;
+                x[j][e] = rate[i] * xv;
+            }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int at = (wr * 16 + g + h * 8) * MS + wc * 16 + j * 8 + 2 * t4;
+                Op::put(Ps + at, p[j][2 * h], p[j][2 * h + 1]);
+                Op::put(Xs + at, x[j][2 * h], x[j][2 * h + 1]);
+            }
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = wr * 16 + g + (e >> 1) * 8, c = wc * (KD / 4) + j * 8 + 2 * t4 + (e & 1);
+                const float kv = to_f32(Ks[i * KS + c]), qv = to_f32(Qs[i * KS + c]);
+                zq[j][e] *= A.scale * since[i];
+                zk[j][e] *= -since[i];
+                zm[j][e] *= until[i];
+                by_row[0][e >> 1] = fmaf(qv, zq[j][e], by_row[0][e >> 1]);
+                by_row[2][e >> 1] = fmaf(kv, zk[j][e], by_row[2][e >> 1]);
+                by_row[1][e >> 1] = fmaf(kv, zm[j][e], by_row[1][e >> 1]);
+                zk[j][e] = fmaf(rate[i], zk[j][e], zm[j][e]);
+            }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float v = by_row[q][h];
+                v += __shfl_xor_sync(~0u, v, 1);
+                v += __shfl_xor_sync(~0u, v, 2);
+                if (t4 == 0) rows[q][wc][wr * 16 + g + h * 8] = v;
+            }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float v = by_col[j][h];
+                v += __shfl_xor_sync(~0u, v, 4);
+                v += __shfl_xor_sync(~0u, v, 8);
+                v += __shfl_xor_sync(~0u, v, 16);
+                if (g == 0) cols[wr][wc * 16 + j * 8 + 2 * t4 + h] = v;
+            }
+#pragma unroll
+        for (int o = 1; o < 8; o *= 2) rv += __shfl_xor_sync(~0u, rv, o);
+        if ((tid & 7) == 0) dots[tid >> 3] = rv;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) inner += __shfl_xor_sync(~0u, inner, o);
+        if (lane == 0) more[warp] = inner;
+        __syncthreads();
+        // dQ += p K, dK += x K + x^T K + p^T Q
+#pragma unroll 1
+        for (int d = 0; d < 4; ++d) {
+            typename Op::B bk[2], bq[2];
+            const bool low = d <= wr, high = d >= wr;
+            typename Op::A ap, ax, pt, xt;
+            if (low) {
+                ap = Op::by_rows(Ps + wr * 16 * MS + d * 16, MS);
+                ax = Op::by_rows(Xs + wr * 16 * MS + d * 16, MS);
+            }
+            if (high) {
+                pt = Op::by_columns(Ps + d * 16 * MS + wr * 16, MS);
+                xt = Op::by_columns(Xs + d * 16 * MS + wr * 16, MS);
+            }
+#pragma unroll
+            for (int j = 0; j < NQ; j += 2) {
+                Op::P::by_columns(bk, Ks + d * 16 * KS + wc * (KD / 4) + j * 8, KS);
+                if (low) {
+                    Op::mma(zq[j], zq[j + 1], ap, bk);
+                    Op::mma(zk[j], zk[j + 1], ax, bk);
+                }
+                if (high) {
+                    Op::P::by_columns(bq, Qs + d * 16 * KS + wc * (KD / 4) + j * 8, KS);
+                    Op::mma(zk[j], zk[j + 1], xt, bk);
+                    Op::mma(zk[j], zk[j + 1], pt, bq);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                tq[j][e] += zq[j][e];
+                tk[j][e] += zk[j][e];
+            }
+        if (warp == 0) {
+            // rows 2 lane, 2 lane + 1: what each adds to the decays up to it
+            float d[2], whole = 0.0f, edge = 0.0f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int i = 2 * lane + h;
+                float a = 0.0f, m = 0.0f, r = 0.0f, xs = 0.0f, c = 0.0f;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    a += rows[0][q][i];
+                    m += rows[1][q][i];
+                    r += rows[2][q][i];
+                    xs += rows[3][q][i];
+                    c += cols[q][i];
+                }
+                d[h] = a + rate[i] * r - m - c;
+                edge += m;
+                if (i < n) {
+                    float db = dots[i] + r + xs;
+                    if (A.logit) db *= rate[i] * (1.0f - rate[i]);
+                    ((T*)A.dbeta.p)[row_at(A, A.dbeta, s, sp, t0 + i) + head * A.dbeta.hs] = from_f32<T>(db);
+                }
+            }
+            if (lane < GRADS / 32) whole = more[lane];
+            // (since at the chunk's end is 0 where a decay is)
+            whole *= since[C - 1];
+#pragma unroll
+            for (int o = 16; o; o >>= 1) {
+                whole += __shfl_xor_sync(~0u, whole, o);
+                edge += __shfl_xor_sync(~0u, edge, o);
+            }
+            float sum = d[0] + d[1];
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const float v = __shfl_down_sync(~0u, sum, o);
+                if (lane + o < 32) sum += v;
+            }
+            whole += edge;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int i = 2 * lane + h;
+                float dg = whole + sum - (h ? d[0] : 0.0f);
+                if (i < n) {
+                    const T gate = ((const T*)A.gate.p)[row_at(A, A.gate, s, sp, t0 + i) + head * A.gate.hs];
+                    if (A.logit) dg *= 1.0f / (1.0f + expf(to_f32(gate)));
+                    else if (to_f32(gate) == -INFINITY) dg = 0.0f;
+                    ((T*)A.dgate.p)[row_at(A, A.dgate, s, sp, t0 + i) + head * A.dgate.hs] = from_f32<T>(dg);
+                }
+            }
+        }
+        __syncthreads();
+    }
+    // dQ, dK as rows of T, through the keys' and queries' place
+    T *oq = reinterpret_cast<T*>(Qs), *ok = reinterpret_cast<T*>(Ks);
+#pragma unroll
+    for (int j = 0; j < NQ; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int at = (wr * 16 + g + (e >> 1) * 8) * KS + wc * (KD / 4) + j * 8 + 2 * t4 + (e & 1);
+            oq[at] = from_f32<T>(tq[j][e]);
+            ok[at] = from_f32<T>(tk[j][e]);
+        }
+    __syncthreads();
+    auto store = [&](const Heads& h, const T* from) {
+        T* to = (T*)h.p + row_at(A, h, s, sp, t0) + kh * h.hs;
+        if (h.vec) {
+            constexpr int V = 16 / (int)sizeof(T), N = KD / V;
+            for (int i = tid; i < n * N; i += GRADS) {
+                const int r = i / N, c = i % N * V;
+                if (c < A.kdim) *reinterpret_cast<uint4*>(to + r * h.st + c) = *reinterpret_cast<const uint4*>(from + r * KS + c);
+            }
+        } else {
+            for (int i = tid; i < n * KD; i += GRADS) {
+                const int r = i / KD, c = i % KD;
+                if (c < A.kdim) to[r * h.st + c] = from[r * KS + c];
+            }
+        }
+    };
+    store(A.dq, oq);
+    store(A.dk, ok);
+}
+
 // ---- launches, one file per type -----------------------------------------------------
 struct DeltaSizes {
     int squares, kept;   // bytes of T and P of a chunk; of an element kept for the gradient
@@ -831,6 +1369,7 @@ struct DeltaSizes {
 template <typename T> DeltaSizes delta_sizes();
 template <typename T> void launch_prep(const DeltaArgs& A, cudaStream_t st);
 template <typename T> void launch_scan(const DeltaArgs& A, int warps, cudaStream_t st);
+template <typename T> void launch_grads(const DeltaArgs& A, int warps, cudaStream_t st);
 
 template <typename F>
 void set_smem(F* kernel, int bytes) {
