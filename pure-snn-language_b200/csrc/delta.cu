@@ -144,9 +144,10 @@ Heads heads_of(const snn_delta* d, const snn_heads* h, int64_t heads, int64_t wi
     if (written)
         SNN_REQUIRE(snnb::apart({{seqs, ss}, {d->n_steps, st}, {heads, hs}}, width), SNN_ERR_ARG,
                     std::string("delta: rows overlap in ") + name);
-    const int v = 16 / size;
-    const bool vec = (uintptr_t)h->data % 16 == 0 && ss % v == 0 && st % v == 0 && hs % v == 0 && width % v == 0;
-    return {h->data, ss, st, hs, vec};
+    int word = 16;  // bytes
+    while (word > size && ((uintptr_t)h->data % word || ss * size % word || st * size % word || hs * size % word || width * size % word))
+        word /= 2;
+    return {h->data, ss, st, hs, word};
 }
 // a gate's or rate's rows: a head beside the other
 Heads gates_of(const snn_delta* d, const snn_rows* r, const char* name, bool written = false) {
@@ -166,15 +167,16 @@ DeltaSizes sizes_of(const snn_delta* d) {
     return z;
 }
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
-// T, P and factors, then (kept for the gradient) states and U
+// T and P, keys, factors, then (kept for the gradient) states and U
 struct Layout {
-    int64_t factors, states, u, all, kept_all;
+    int64_t keys, factors, states, u, all, kept_all;
 };
 Layout layout_of(const snn_delta* d) {
     const DeltaSizes z = sizes_of(d);
     const int64_t units = slots_of(d) * d->heads, kd = d->k_dim <= 64 ? 64 : 128;
     Layout l;
-    l.factors = round256(units * z.squares);
+    l.keys = round256(units * z.squares);
+    l.factors = l.keys + round256(slots_of(d) * d->k_heads * 2 * C * kd * z.key);
     l.all = l.states = l.factors + round256(units * SC * 4);
     l.u = l.states + round256(units * d->v_dim * kd * z.kept);
     l.kept_all = l.u + round256(units * C * d->v_dim * z.kept);
@@ -276,6 +278,7 @@ void delta_scan(const snn_delta* d, const snn_heads* q, const snn_heads* k, cons
     if (saved) check_work(saved, saved_bytes, l.kept_all, "saved");
     else check_work(work, work_bytes, l.all, "workspace");
     A.squares = base;
+    A.keys = base + l.keys;
     A.factors = (float*)(base + l.factors);
     if (saved) {
         A.states = base + l.states;
@@ -306,7 +309,7 @@ void delta_scan_grad(const snn_delta* d, const snn_heads* q, const snn_heads* k,
     SNN_REQUIRE(dy || dh, SNN_ERR_ARG, "delta: neither dy nor dh");
     DeltaArgs A = base_args(d, q, k, v, gate, beta);
     if (dy) A.dy = heads_of(d, dy, d->heads, d->v_dim, "dy");
-    else A.dy.vec = 1;
+    else A.dy.word = 16;
     A.dq = heads_of(d, dq, d->k_heads, d->k_dim, "dq", true);
     A.dk = heads_of(d, dk, d->k_heads, d->k_dim, "dk", true);
     A.dv = heads_of(d, dv, d->heads, d->v_dim, "dv", true);
@@ -326,6 +329,7 @@ void delta_scan_grad(const snn_delta* d, const snn_heads* q, const snn_heads* k,
     check_work(work, work_bytes, l.kept_all - l.states, "workspace");
     char* base = (char*)saved;
     A.squares = base;
+    A.keys = base + l.keys;
     A.factors = (float*)(base + l.factors);
     A.states = base + l.states;
     A.u = base + l.u;

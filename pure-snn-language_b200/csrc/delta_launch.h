@@ -32,7 +32,7 @@ void launch_scan_of(const DeltaArgs& A, int warps, cudaStream_t st) {
     by_dim<T>(A.kdim, [&](auto kd) {
         by_warps(warps, [&](auto nw) {
             constexpr int KD = decltype(kd)::value, NW = decltype(nw)::value;
-            using S = Stage<P, KD, NW>;
+            using S = Stage<P, KD, NW, P::OUT>;
             auto* kernel = k_delta_scan<P, KD, NW>;
             set_smem(kernel, S::STAGES * S::BYTES);
             const dim3 grid((unsigned)std::min<long long>(A.n_seq, 1 << 30), (unsigned)A.heads,
@@ -49,7 +49,7 @@ void launch_grads_of(const DeltaArgs& A, int warps, cudaStream_t st) {
         constexpr int KD = decltype(kd)::value;
         by_warps(warps, [&](auto nw) {
             constexpr int NW = decltype(nw)::value;
-            using S = Stage<P, KD, NW>;
+            using S = Stage<P, KD, NW, P::PLANES>;
             auto* kernel = k_delta_back<P, KD, NW>;
             set_smem(kernel, S::STAGES * S::BYTES);
             const dim3 grid((unsigned)std::min<long long>(A.n_seq, 1 << 30), (unsigned)A.heads,
@@ -68,7 +68,7 @@ void launch_grads_of(const DeltaArgs& A, int warps, cudaStream_t st) {
 
 #define SNN_DELTA_LAUNCHES(T)                                                                        \
     template <> DeltaSizes delta_sizes<T>() {                                                        \
-        return {PathOf<T>::P::SQUARES, (int)sizeof(Kept<T>::K)};                                     \
+        return {PathOf<T>::P::SQUARES, (int)sizeof(PathOf<T>::P::KE), (int)sizeof(Kept<T>::K)};                                   \
     }                                                                                                \
     template <> void launch_prep<T>(const DeltaArgs& A, cudaStream_t st) { launch_prep_of<T>(A, st); } \
     template <> void launch_scan<T>(const DeltaArgs& A, int warps, cudaStream_t st) { launch_scan_of<T>(A, warps, st); } \
