@@ -167,6 +167,7 @@ DeltaSizes sizes_of(const snn_delta* d) {
     return z;
 }
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
+int64_t vpad_of(const snn_delta* d) { return (d->v_dim + 7) / 8 * 8; }
 // T and P, keys, factors, then (kept for the gradient) states and U
 struct Layout {
     int64_t keys, factors, states, u, all, kept_all;
@@ -176,10 +177,10 @@ Layout layout_of(const snn_delta* d) {
     const int64_t units = slots_of(d) * d->heads, kd = d->k_dim <= 64 ? 64 : 128;
     Layout l;
     l.keys = round256(units * z.squares);
-    l.factors = l.keys + round256(slots_of(d) * d->k_heads * 2 * C * kd * z.key);
+    l.factors = l.keys + round256(slots_of(d) * d->k_heads * 2 * C * (kd + PAD) * z.key);
     l.all = l.states = l.factors + round256(units * SC * 4);
     l.u = l.states + round256(units * d->v_dim * kd * z.kept);
-    l.kept_all = l.u + round256(units * C * d->v_dim * z.kept);
+    l.kept_all = l.u + round256(units * C * vpad_of(d) * z.kept);
     return l;
 }
 bool by_steps(const snn_delta* d) { return mean_steps(d) <= 8; }
@@ -203,6 +204,7 @@ DeltaArgs base_args(const snn_delta* d, const snn_heads* q, const snn_heads* k, 
     A.group = (int)(d->heads / d->k_heads);
     A.kdim = (int)d->k_dim;
     A.vdim = (int)d->v_dim;
+    A.vpad = (int)vpad_of(d);
     A.logit = (d->flags & SNN_SCAN_LOGIT) != 0;
     A.zero = d->offsets && (d->flags & SNN_SCAN_ZERO) != 0;
     A.scale = d->scale;

@@ -1,6 +1,8 @@
 // delta_launch.h - the launches of one element type (included by a file for each)
 #pragma once
-#include "delta_tile.h"
+#include "delta_grads.h"
+#include "delta_prep.h"
+#include "delta_scan.h"
 
 namespace snnb_delta {
 template <typename T, typename F>
@@ -49,7 +51,7 @@ void launch_grads_of(const DeltaArgs& A, int warps, cudaStream_t st) {
         constexpr int KD = decltype(kd)::value;
         by_warps(warps, [&](auto nw) {
             constexpr int NW = decltype(nw)::value;
-            using S = Stage<P, KD, NW, P::PLANES>;
+            using S = Stage<P, KD, NW, P::PIECES>;
             auto* kernel = k_delta_back<P, KD, NW>;
             set_smem(kernel, S::STAGES * S::BYTES);
             const dim3 grid((unsigned)std::min<long long>(A.n_seq, 1 << 30), (unsigned)A.heads,

@@ -1,0 +1,474 @@
+// delta_scan.h - a delta-rule scan along the sequences, forward (k_delta_scan) and, for
+// the states' gradients, back (k_delta_back).
+#pragma once
+#include "delta_tile.h"
+
+namespace snnb_delta {
+// A chunk in shared memory: K, Q, T and the first PP planes of P, the factors and the
+// columns of V (or dy), two chunks where they fit.  All but the last are copied as they
+// lie in the workspace.
+template <class P, int KD, int NW, int PP>
+struct Stage {
+    using T = typename P::T;
+    using KE = typename P::KE;
+    static constexpr int VW = 16 * NW;
+    static constexpr int KEYS = C * (KD + PAD) * (int)sizeof(KE), VALUES = C * (VW + PAD) * (int)sizeof(T);
+    static constexpr int SQUARES = (P::PIECES + PP) * LOW * (int)sizeof(KE);
+    static constexpr int BYTES = 2 * KEYS + VALUES + SQUARES + SCAN_FACTORS * 4;
+    static constexpr int STAGES = 2 * BYTES <= 227 * 1024 - 1024 ? 2 : 1;
+    KE *k, *q, *t, *p;
+    T* v;
+    float* f;
+    __device__ __forceinline__ explicit Stage(char* m) {
+        k = reinterpret_cast<KE*>(m);
+        q = reinterpret_cast<KE*>(m + KEYS);
+        v = reinterpret_cast<T*>(m + 2 * KEYS);
+        t = reinterpret_cast<KE*>(m + 2 * KEYS + VALUES);
+        p = t + P::PIECES * LOW;
+        f = reinterpret_cast<float*>(m + 2 * KEYS + VALUES + SQUARES);
+    }
+    // chunk c of sequence s; vals: the values' rows or, backward, those of dy (or none)
+    __device__ __forceinline__ void load(const DeltaArgs& A, const Heads& vals, long long s, const Span& sp, int c, int head,
+                                         int col0, int tid) {
+        const int n = min(C, sp.len - c * C);
+        const long long slot = sp.chunk + c, unit = slot * A.heads + head;
+        load_words(k, A.keys + (slot * A.hk + head / A.group) * 2 * KEYS, 2 * KEYS, tid, NW * 32);
+        load_rows<T, C, VW>(v, (const T*)vals.p + row_at(A, vals, s, sp, c * C) + head * vals.hs + col0, vals.st,
+                            vals.p ? n : 0, A.vdim - col0, vals.word, tid, NW * 32);
+        load_words(t, A.squares + unit * P::SQUARES, SQUARES, tid, NW * 32);
+        load_words(f, A.factors + unit * SC, SCAN_FACTORS * 4, tid, NW * 32);
+    }
+};
+
+// a warp's columns of the values' tile [C][ST] as accumulators [16 columns, C steps]
+template <typename T, int ST>
+__device__ __forceinline__ void values_of(float (&o)[8][4], const T* v) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            unsigned r[4];
+            ldsm4t(r, v + (i * 8 + (lane >> 4) * 8 + (lane & 7)) * ST + ((lane >> 3) & 1) * 8);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 f = of_pair<T>(r[k]);
+                o[i + (k >> 1)][2 * (k & 1)] = f.x;
+                o[i + (k >> 1)][2 * (k & 1) + 1] = f.y;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][e] = v[(i * 8 + 2 * t4 + (e & 1)) * ST + g + (e >> 1) * 8];
+    }
+}
+// accumulators [16 columns, C steps] as n rows of T, the first w columns: through the warp's columns
+// of `stage` [C][ST]
+template <typename T, int ST>
+__device__ __forceinline__ void store_tile(const float (&o)[8][4], T* stage, T* to, long long st, int n, int w, int word) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+    __syncwarp();
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2)
+            stsm4t(stage + (i * 8 + (lane >> 4) * 8 + (lane & 7)) * ST + ((lane >> 3) & 1) * 8, pair_of<T>(o[i][0], o[i][1]),
+                   pair_of<T>(o[i][2], o[i][3]), pair_of<T>(o[i + 1][0], o[i + 1][1]), pair_of<T>(o[i + 1][2], o[i + 1][3]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) stage[(i * 8 + 2 * t4 + (e & 1)) * ST + g + (e >> 1) * 8] = o[i][e];
+    }
+    __syncwarp();
+    auto words = [&](auto z) {
+        using W = decltype(z);
+        constexpr int V = (int)(sizeof(W) / sizeof(T)), N = 16 / V;
+        const int c = lane % N * V;
+        if (c < w)
+#pragma unroll 4
+            for (int r = lane / N; r < n; r += 32 / N)
+                *reinterpret_cast<W*>(to + r * st + c) = *reinterpret_cast<const W*>(stage + r * ST + c);
+    };
+    if (word == 16) words(uint4());
+    else if (word == 8) words(uint2());
+    else if (word == 4) words(unsigned());
+    else {
+        for (int i = lane; i < n * 16; i += 32) {
+            const int r = i >> 4, c = i & 15;
+            if (c < w) to[r * st + c] = stage[r * ST + c];
+        }
+    }
+    __syncwarp();
+}
+// accumulators as C rows of what is kept, w columns (whole words of 16 bytes)
+template <typename T, typename K, int ST>
+__device__ __forceinline__ void keep_tile(const float (&o)[8][4], T* stage, K* to, long long st, int w) {
+    if constexpr (std::is_same<T, K>::value) {
+        store_tile<T, ST>(o, stage, to, st, C, w, 16);
+    } else {  // f32 of f16 tensors
+        const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int c = g + (e >> 1) * 8;
+                if (c < w) to[(long long)(i * 8 + 2 * t4 + (e & 1)) * st + c] = from_f32<K>(o[i][e]);
+            }
+    }
+}
+// S^T [16 columns, KD] of a warp, divided by its scale, as w rows of KD elements
+template <typename K, int NT>
+__device__ __forceinline__ void keep_state(const float (&S)[NT][4], float back, K* to, int w) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        if (g + 8 * h < w)
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                K* p = to + (g + 8 * h) * NT * 8 + i * 8 + 2 * t4;
+                const float x = S[i][2 * h] * back, y = S[i][2 * h + 1] * back;
+                if constexpr (sizeof(K) == 4) *reinterpret_cast<float2*>(p) = make_float2(x, y);
+                else *reinterpret_cast<unsigned*>(p) = pair_of<K>(x, y);
+            }
+}
+// f32 states [kdim, vdim] from and to a warp's columns
+template <int NT>
+__device__ __forceinline__ void read_state(float (&S)[NT][4], const float* h, const DeltaArgs& A, int col) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int c = col + g + (e >> 1) * 8, d = i * 8 + 2 * t4 + (e & 1);
+            S[i][e] = h && c < A.vdim && d < A.kdim ? h[(long long)d * A.vdim + c] : 0.0f;
+        }
+}
+template <int NT>
+__device__ __forceinline__ void write_state(const float (&S)[NT][4], float back, float* h, const DeltaArgs& A, int col) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int c = col + g + (e >> 1) * 8, d = i * 8 + 2 * t4 + (e & 1);
+            if (c < A.vdim && d < A.kdim) h[(long long)d * A.vdim + c] = S[i][e] * back;
+        }
+}
+
+
+// Accumulators that are the first operand of products as they are, in pieces: times a
+// power of two that keeps their largest magnitude in 2^6 .. 2^15, changed only where it
+// leaves that.  The scale is returned.
+template <int NT>
+__device__ __forceinline__ float recentre(float (&S)[NT][4], float scale) {
+    const float top = warp_top(S);
+    if (top >= 0x1p15f || (top < 0x1p6f && top > 0.0f && scale < 0x1p60f)) {
+        const float f = fminf(scale_for(top), 0x1p60f * inverse_of(scale));
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) S[i][e] *= f;
+        scale *= f;
+    }
+    return scale;
+}
+// the same for a state to which products of x and y (already times its scale, to be pieces)
+// are to be added
+template <int NT>
+__device__ __forceinline__ float make_room(float (&S)[NT][4], float (&x)[8][4], float (&y)[8][4], float scale) {
+    const float top = fmaxf(warp_top(x), warp_top(y));
+    if (top >= 0x1p15f) {
+        const float f = scale_for(top);
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) S[i][e] *= f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[i][e] *= f;
+                if (&x != &y) y[i][e] *= f;
+            }
+        scale *= f;
+    }
+    return scale;
+}
+// acc [16, 64] += x m^T (ROWS; m lower triangular: steps k <= n) or x m (k >= n), in N pieces
+template <class P, int N, bool ROWS, typename F>
+__device__ __forceinline__ void times_square(float (&acc)[8][4], const float (&x)[8][4], F scale, const typename P::KE* m) {
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        const typename P::A a = P::split(x[2 * d], x[2 * d + 1], scale(d));
+        auto plane = [&](auto jj) {
+            constexpr int j = decltype(jj)::value;
+            typename P::B b[4][2];
+#pragma unroll
+            for (int np = 0; np < 4; ++np) {
+                if (ROWS && np >= d) P::by_rows(b[np], m + j * LOW + low_at(np) + 16 * d, low_stride(np));
+                if (!ROWS && np <= d) P::by_columns(b[np], m + j * LOW + low_at(d) + 16 * np, low_stride(d));
+            }
+            if constexpr (N - 1 - j >= 1)
+#pragma unroll
+                for (int np = 0; np < 4; ++np)
+                    if (ROWS ? np >= d : np <= d) P::template mma<1>(acc[2 * np], acc[2 * np + 1], a, b[np]);
+#pragma unroll
+            for (int np = 0; np < 4; ++np)
+                if (ROWS ? np >= d : np <= d) P::template mma<0>(acc[2 * np], acc[2 * np + 1], a, b[np]);
+        };
+        if constexpr (N == 2) plane(std::integral_constant<int, 1>());
+        plane(std::integral_constant<int, 0>());
+    }
+}
+// S^T [16, KD] += x [16, 64] m [64, KD], x in all pieces
+template <class P, int KD>
+__device__ __forceinline__ void add_outer(float (&S)[KD / 8][4], const float (&x)[8][4], const typename P::KE* m) {
+    constexpr int KS = KD + PAD;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        const typename P::A a = P::split(x[2 * d], x[2 * d + 1], 1.0f);
+#pragma unroll
+        for (int h = 0; h < KD / 64; ++h) {
+            typename P::B b[4][2];
+#pragma unroll
+            for (int np = 0; np < 4; ++np) P::by_columns(b[np], m + d * 16 * KS + (h * 4 + np) * 16, KS);
+            if constexpr (P::PIECES == 2)
+#pragma unroll
+                for (int np = 0; np < 4; ++np) P::template mma<1>(S[2 * (h * 4 + np)], S[2 * (h * 4 + np) + 1], a, b[np]);
+#pragma unroll
+            for (int np = 0; np < 4; ++np) P::template mma<0>(S[2 * (h * 4 + np)], S[2 * (h * 4 + np) + 1], a, b[np]);
+        }
+    }
+}
+// acc [16, 64] += S^T [16, KD] m^T for m [64, KD], piece d of 16 of the depth
+template <class P, int N, int KD>
+__device__ __forceinline__ void read_with(float (&acc)[8][4], const typename P::A& a, const typename P::KE* m, int d) {
+    constexpr int KS = KD + PAD;
+    typename P::B b[4][2];
+#pragma unroll
+    for (int np = 0; np < 4; ++np) P::by_rows(b[np], m + np * 16 * KS + d * 16, KS);
+    if constexpr (N == 2)
+#pragma unroll
+        for (int np = 0; np < 4; ++np) P::template mma<1>(acc[2 * np], acc[2 * np + 1], a, b[np]);
+#pragma unroll
+    for (int np = 0; np < 4; ++np) P::template mma<0>(acc[2 * np], acc[2 * np + 1], a, b[np]);
+}
+__device__ __forceinline__ float2 pair_at(const float* f, int i) {  // of an accumulator tile's two steps
+    return *reinterpret_cast<const float2*>(f + i * 8 + 2 * (threadIdx.x & 3));
+}
+
+template <class P, int KD, int NW>
+__global__ void __launch_bounds__(NW * 32, 1) k_delta_scan(const __grid_constant__ DeltaArgs A) {
+    using T = typename P::T;
+    using St = Stage<P, KD, NW, P::OUT>;
+    using K = typename Kept<T>::K;
+    constexpr int NT = KD / 8, VS = St::VW + PAD;
+    extern __shared__ __align__(16) char smem[];
+    const int tid = threadIdx.x, warp = tid >> 5;
+    const int head = blockIdx.y, col0 = (int)blockIdx.z * St::VW, col = col0 + warp * 16;
+    const int w = A.vdim - col;  // this warp's columns (16 and more: all; none: it only loads)
+    for (long long s = blockIdx.x; s < A.n_seq; s += gridDim.x) {
+        const Span sp = span_of(A, s);
+        const int chunks = (sp.len + C - 1) / C;
+        float S[NT][4], sigma = 1.0f;  // S times sigma
+        read_state<NT>(S, A.h0 ? A.h0 + (s * A.heads + head) * A.kdim * A.vdim : nullptr, A, col);
+        if (St::STAGES == 2 && chunks) St(smem).load(A, A.v, s, sp, 0, head, col0, tid);
+        copies_end();
+        for (int c = 0; c < chunks; ++c) {
+            const St st(smem + (St::STAGES == 2 ? (c & 1) * St::BYTES : 0));
+            if (St::STAGES == 1) St(smem).load(A, A.v, s, sp, c, head, col0, tid);
+            else if (c + 1 < chunks) St(smem + ((c + 1) & 1) * St::BYTES).load(A, A.v, s, sp, c + 1, head, col0, tid);
+            copies_end();
+            copies_wait<St::STAGES - 1>();
+            __syncthreads();
+            if (w > 0) {
+                const int n = min(C, sp.len - c * C);
+                const long long unit = (sp.chunk + c) * A.heads + head;
+                if constexpr (P::SCALED) sigma = recentre(S, sigma);
+                float back = inverse_of(sigma), ik = 1.0f, iq = 1.0f;
+                if constexpr (P::SCALED) {
+                    ik = inverse_of(st.f[K_SCALE]);
+                    iq = inverse_of(st.f[Q_SCALE]);
+                }
+                if (A.states) keep_state<K, NT>(S, back, (K*)A.states + (unit * A.vdim + col) * KD, w);
+                float r[8][4] = {}, o[8][4] = {}, u[8][4];
+#pragma unroll
+                for (int d = 0; d < KD / 16; ++d) {
+                    const typename P::A a = P::split(S[2 * d], S[2 * d + 1], 1.0f);
+                    read_with<P, P::PIECES, KD>(r, a, st.k, d);
+                    read_with<P, P::OUT, KD>(o, a, st.q, d);
+                }
+                // r = b (v - since K S)
+                values_of<T, VS>(u, st.v + warp * 16);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float2 since = pair_at(st.f, i), rate = pair_at(st.f + 2 * C, i);
+                    const float f0 = -since.x * back * ik, f1 = -since.y * back * ik;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        r[i][e] = (e & 1 ? rate.y : rate.x) * fmaf(e & 1 ? f1 : f0, r[i][e], u[i][e]);
+                        u[i][e] = 0.0f;
+                    }
+                }
+                // u = T r
+                float ss = 1.0f;
+                if constexpr (P::SCALED) ss = warp_scale(r);
+                times_square<P, P::PIECES, true>(u, r, [&](int) { return ss; }, st.t);
+                if constexpr (P::SCALED) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float f = inverse_of(ss) * inverse_of(st.f[T_SCALE + i / 2]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) u[i][e] *= f;
+                    }
+                    ss = warp_scale(u);
+                }
+                // o = since Q S + P u, times the pieces' scales
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float2 since = pair_at(st.f, i);
+                    const float f = P::SCALED ? ss * st.f[P_SCALE + i / 2] : 1.0f, f0 = since.x * back * iq, f1 = since.y * back * iq;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[i][e] = o[i][e] * (e & 1 ? f1 : f0) * f;
+                }
+                times_square<P, P::OUT, true>(o, u, [&](int) { return ss; }, st.p);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float f = P::SCALED ? A.scale * (inverse_of(ss) * inverse_of(st.f[P_SCALE + i / 2])) : A.scale;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[i][e] *= f;
+                }
+                store_tile<T, VS>(o, st.v + warp * 16, (T*)A.y.p + row_at(A, A.y, s, sp, c * C) + head * A.y.hs + col, A.y.st, n, w, A.y.word);
+                if (A.u) keep_tile<T, K, VS>(u, st.v + warp * 16, (K*)A.u + unit * C * A.vpad + col, A.vpad, A.vpad - col);
+                // S = since_64 S + (until u)^T K; 1 - since_64 keeps its bits where decays are near 1
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float2 until = pair_at(st.f + C, i);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) u[i][e] *= (e & 1 ? until.y : until.x) * sigma * ik;
+                }
+                if constexpr (P::SCALED) sigma = make_room(S, u, u, sigma);
+                const float lost = st.f[LOST];
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) S[i][e] = fmaf(-lost, S[i][e], S[i][e]);
+                add_outer<P, KD>(S, u, st.k);
+            }
+            __syncthreads();
+        }
+        if (A.h && w > 0) write_state<NT>(S, inverse_of(sigma), A.h + (s * A.heads + head) * A.kdim * A.vdim, A, col);
+        copies_wait<0>();
+        __syncthreads();
+    }
+    if (A.zero) zero_rest<T>(A, A.y, A.heads, A.vdim, ((long long)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x,
+                             (long long)gridDim.x * gridDim.y * gridDim.z);
+}
+
+// The states' gradients, from the last chunk.  With D the gradient of the state behind a
+// chunk, Z = scale dy:
+//   dU = P^T Z + until K D,   R = T^T dU,   dV = b R,
+//   D <- since_64 D + (since Z)^T Q - (since b R)^T K   (the transposed scan, in the same layout)
+template <class P, int KD, int NW>
+__global__ void __launch_bounds__(NW * 32, 1) k_delta_back(const __grid_constant__ DeltaArgs A) {
+    using T = typename P::T;
+    using St = Stage<P, KD, NW, P::PIECES>;
+    using K = typename Kept<T>::K;
+    constexpr int NT = KD / 8, VS = St::VW + PAD;
+    extern __shared__ __align__(16) char smem[];
+    const int tid = threadIdx.x, warp = tid >> 5;
+    const int head = blockIdx.y, col0 = (int)blockIdx.z * St::VW, col = col0 + warp * 16;
+    const int w = A.vdim - col;
+    for (long long s = blockIdx.x; s < A.n_seq; s += gridDim.x) {
+        const Span sp = span_of(A, s);
+        const int chunks = (sp.len + C - 1) / C;
+        float D[NT][4], sigma = 1.0f;
+        read_state<NT>(D, A.dh ? A.dh + (s * A.heads + head) * A.kdim * A.vdim : nullptr, A, col);
+        if (St::STAGES == 2 && chunks) St(smem).load(A, A.dy, s, sp, chunks - 1, head, col0, tid);
+        copies_end();
+        for (int i = 0; i < chunks; ++i) {
+            const int c = chunks - 1 - i;
+            const St st(smem + (St::STAGES == 2 ? (i & 1) * St::BYTES : 0));
+            if (St::STAGES == 1) St(smem).load(A, A.dy, s, sp, c, head, col0, tid);
+            else if (c > 0) St(smem + ((i + 1) & 1) * St::BYTES).load(A, A.dy, s, sp, c - 1, head, col0, tid);
+            copies_end();
+            copies_wait<St::STAGES - 1>();
+            __syncthreads();
+            if (w > 0) {
+                const int n = min(C, sp.len - c * C);
+                const long long unit = (sp.chunk + c) * A.heads + head;
+                if constexpr (P::SCALED) sigma = recentre(D, sigma);
+                float back = inverse_of(sigma), ik = 1.0f, iq = 1.0f;
+                if constexpr (P::SCALED) {
+                    ik = inverse_of(st.f[K_SCALE]);
+                    iq = inverse_of(st.f[Q_SCALE]);
+                }
+                keep_state<K, NT>(D, back, (K*)A.dstates + (unit * A.vdim + col) * KD, w);
+                float u[8][4] = {}, r[8][4] = {}, z[8][4];
+#pragma unroll
+                for (int d = 0; d < KD / 16; ++d) {
+                    const typename P::A a = P::split(D[2 * d], D[2 * d + 1], 1.0f);
+                    read_with<P, P::PIECES, KD>(u, a, st.k, d);
+                }
+                values_of<T, VS>(z, st.v + warp * 16);
+                // u = P^T Z + until K D, times c; the scales of row blocks are made up for in Z, R's in u
+                float c1 = 1.0f, c2 = 1.0f;
+                if constexpr (P::SCALED)
+                    c1 = scale_for(fabsf(A.scale) * warp_top(z)) *
+                         fminf(fminf(st.f[P_SCALE], st.f[P_SCALE + 1]), fminf(st.f[P_SCALE + 2], st.f[P_SCALE + 3]));
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float2 until = pair_at(st.f + C, j);
+                    const float f0 = until.x * back * ik, f1 = until.y * back * ik;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        u[j][e] = u[j][e] * (e & 1 ? f1 : f0) * c1;
+                        z[j][e] *= A.scale;
+                    }
+                }
+                times_square<P, P::PIECES, false>(u, z, [&](int d) { return P::SCALED ? c1 * inverse_of(st.f[P_SCALE + d]) : 1.0f; }, st.p);
+                if constexpr (P::SCALED)
+                    c2 = warp_scale(u) * fminf(fminf(st.f[T_SCALE], st.f[T_SCALE + 1]), fminf(st.f[T_SCALE + 2], st.f[T_SCALE + 3]));
+                times_square<P, P::PIECES, false>(r, u, [&](int d) { return P::SCALED ? c2 * inverse_of(st.f[T_SCALE + d]) : 1.0f; }, st.t);
+                if constexpr (P::SCALED) {
+                    const float f1 = inverse_of(c1), f2 = inverse_of(c2);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) r[j][e] = r[j][e] * f2 * f1;
+                }
+                // (dy's tile is not read any more)
+                keep_tile<T, K, VS>(r, st.v + warp * 16, (K*)A.dr + unit * C * A.vpad + col, A.vpad, A.vpad - col);
+                // r = b R, u = -since b R, z = since Z, the last two times sigma / ks, sigma / qs
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float2 since = pair_at(st.f, j), rate = pair_at(st.f + 2 * C, j);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float si = (e & 1 ? since.y : since.x) * sigma;
+                        r[j][e] *= e & 1 ? rate.y : rate.x;
+                        u[j][e] = r[j][e] * (-si * ik);
+                        z[j][e] *= si * iq;
+                    }
+                }
+                store_tile<T, VS>(r, st.v + warp * 16, (T*)A.dv.p + row_at(A, A.dv, s, sp, c * C) + head * A.dv.hs + col, A.dv.st, n, w, A.dv.word);
+                if constexpr (P::SCALED) {
+                    sigma = make_room(D, u, z, sigma);
+                }
+                const float lost = st.f[LOST];
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) D[j][e] = fmaf(-lost, D[j][e], D[j][e]);
+                add_outer<P, KD>(D, z, st.q);
+                add_outer<P, KD>(D, u, st.k);
+            }
+            __syncthreads();
+        }
+        if (A.dh0 && w > 0) write_state<NT>(D, inverse_of(sigma), A.dh0 + (s * A.heads + head) * A.kdim * A.vdim, A, col);
+        copies_wait<0>();
+        __syncthreads();
+    }
+}
+}  // namespace snnb_delta
