@@ -59,7 +59,8 @@ __global__ void __launch_bounds__(256) k_delta_steps(const __grid_constant__ Del
                 v[j] = on ? to_f32(((const T*)A.v.p)[row_at(A, A.v, s, sp, t) + head * A.v.hs + col + j]) : 0.0f;
             const float l = log_decay(A, ((const T*)A.gate.p)[row_at(A, A.gate, s, sp, t) + head * A.gate.hs]);
             const float rate = rate_of(A, ((const T*)A.beta.p)[row_at(A, A.beta, s, sp, t) + head * A.beta.hs]);
-            const float lost = -expm1f(l);  // 1 - a, which keeps its bits where a is near 1
+            const float lost = -expm1f(l), kept = expf(l);  // 1 - a keeps its bits where a is near 1
+            const bool little = lost < 0.5f;
             __syncthreads();
             float k[R], dk[V] = {}, dq[V] = {}, kq = 0.0f;
 #pragma unroll
@@ -68,7 +69,7 @@ __global__ void __launch_bounds__(256) k_delta_steps(const __grid_constant__ Del
                 const float q = query[i * 8 + warp];
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    S[i].v[j] = fmaf(-lost, S[i].v[j], S[i].v[j]);
+                    S[i].v[j] = little ? fmaf(-lost, S[i].v[j], S[i].v[j]) : kept * S[i].v[j];
                     dk[j] = fmaf(k[i], S[i].v[j], dk[j]);
                     dq[j] = fmaf(q, S[i].v[j], dq[j]);
                 }

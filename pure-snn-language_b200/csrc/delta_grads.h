@@ -311,9 +311,9 @@ __global__ void __launch_bounds__(GRADS, 1) k_delta_grads(const __grid_constant_
                 tp = fmaxf(tp, top[0][i]);
                 tx = fmaxf(tx, top[1][i]);
             }
-            fk = fminf(scale_for(tx) * ks, scale_for(tp) * qs);  // x K and p^T Q meet in dK
-            xs = fk * ik;
-            ps = fk * iq;
+            xs = scale_for(tx);
+            ps = scale_for(tp);
+            fk = xs * ks;
             fq = ps * ks;
 #pragma unroll
             for (int j = 0; j < NQ; ++j)
@@ -333,35 +333,49 @@ __global__ void __launch_bounds__(GRADS, 1) k_delta_grads(const __grid_constant_
                     KOp::template put<PIECES>(Xs + at, x[j][2 * h] * xs, x[j][2 * h + 1] * xs);
                 }
         __syncthreads();
-        // dQ += p K, dK += x K + x^T K + p^T Q
+        // dQ += p K, dK += x K + x^T K, then p^T Q in its own scale
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
-            typename KOp::B bk[NQ], bq[NQ];
+            typename KOp::B bk[NQ / 2][2];
 #pragma unroll
-            for (int j = 0; j < NQ; j += 2) {
-                KOp::by_columns(reinterpret_cast<typename KOp::B(&)[2]>(bk[j]), Ks + d * 16 * KS + wc * (KD / 4) + j * 8, KS);
-                KOp::by_columns(reinterpret_cast<typename KOp::B(&)[2]>(bq[j]), Qs + d * 16 * KS + wc * (KD / 4) + j * 8, KS);
-            }
+            for (int j = 0; j < NQ / 2; ++j) KOp::by_columns(bk[j], Ks + d * 16 * KS + wc * (KD / 4) + j * 16, KS);
 #pragma unroll
             for (int i = PIECES - 1; i >= 0; --i) {
                 if (d <= wr) {
                     const typename KOp::A ap = KOp::rows_of(Ps + i * C * MS + wr * 16 * MS + d * 16, MS);
                     const typename KOp::A ax = KOp::rows_of(Xs + i * C * MS + wr * 16 * MS + d * 16, MS);
 #pragma unroll
-                    for (int j = 0; j < NQ; j += 2) {
-                        KOp::mma(zq[j], zq[j + 1], ap, reinterpret_cast<typename KOp::B(&)[2]>(bk[j]));
-                        KOp::mma(zk[j], zk[j + 1], ax, reinterpret_cast<typename KOp::B(&)[2]>(bk[j]));
+                    for (int j = 0; j < NQ / 2; ++j) {
+                        KOp::mma(zq[2 * j], zq[2 * j + 1], ap, bk[j]);
+                        KOp::mma(zk[2 * j], zk[2 * j + 1], ax, bk[j]);
                     }
                 }
                 if (d >= wr) {
-                    const typename KOp::A pt = KOp::columns_of(Ps + i * C * MS + d * 16 * MS + wr * 16, MS);
                     const typename KOp::A xt = KOp::columns_of(Xs + i * C * MS + d * 16 * MS + wr * 16, MS);
 #pragma unroll
-                    for (int j = 0; j < NQ; j += 2) {
-                        KOp::mma(zk[j], zk[j + 1], xt, reinterpret_cast<typename KOp::B(&)[2]>(bk[j]));
-                        KOp::mma(zk[j], zk[j + 1], pt, reinterpret_cast<typename KOp::B(&)[2]>(bq[j]));
-                    }
+                    for (int j = 0; j < NQ / 2; ++j) KOp::mma(zk[2 * j], zk[2 * j + 1], xt, bk[j]);
                 }
+            }
+        }
+        if constexpr (SCALED) {
+            const float to = inverse_of(fk), next = ps * qs;
+            fk = next;
+#pragma unroll
+            for (int j = 0; j < NQ; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) zk[j][e] = zk[j][e] * to * next;
+        }
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            if (d < wr) continue;
+            typename KOp::B bq[NQ / 2][2];
+#pragma unroll
+            for (int j = 0; j < NQ / 2; ++j) KOp::by_columns(bq[j], Qs + d * 16 * KS + wc * (KD / 4) + j * 16, KS);
+#pragma unroll
+            for (int i = PIECES - 1; i >= 0; --i) {
+                const typename KOp::A pt = KOp::columns_of(Ps + i * C * MS + d * 16 * MS + wr * 16, MS);
+#pragma unroll
+                for (int j = 0; j < NQ / 2; ++j) KOp::mma(zk[2 * j], zk[2 * j + 1], pt, bq[j]);
             }
         }
         const float bq1 = inverse_of(fq), bk1 = inverse_of(fk);

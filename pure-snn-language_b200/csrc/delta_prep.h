@@ -14,6 +14,9 @@ constexpr int prep_smem() {
     const int keys = 2 * C * (KD + PAD) * (int)sizeof(typename P::KE), m = C * MS * 4;
     return keys > m ? keys : m;  // A and T take the place of K and Q
 }
+// Scale of a chunk's keys or queries.  At most 2^40, and that where all are zero: what
+// they are multiplied with shares the scale of the product and must not lose bits to nothing.
+__device__ __forceinline__ float key_scale(float top) { return top == 0.0f ? 0x1p40f : fminf(scale_for(top), 0x1p40f); }
 // rows of keys or queries into registers, words of V elements; their largest magnitude
 template <typename T, int KD, int N>
 __device__ __forceinline__ float read_keys(uint4 (&w)[N], const T* from, long long st, int n, const DeltaArgs& A, int word) {
@@ -93,8 +96,8 @@ __global__ void __launch_bounds__(PREP, 4) k_delta_prep(const __grid_constant__ 
                 top[1][warp] = b;
             }
             __syncthreads();
-            ks = scale_for(fmaxf(fmaxf(top[0][0], top[0][1]), fmaxf(top[0][2], top[0][3])));
-            qs = scale_for(fmaxf(fmaxf(top[1][0], top[1][1]), fmaxf(top[1][2], top[1][3])));
+            ks = key_scale(fmaxf(fmaxf(top[0][0], top[0][1]), fmaxf(top[0][2], top[0][3])));
+            qs = key_scale(fmaxf(fmaxf(top[1][0], top[1][1]), fmaxf(top[1][2], top[1][3])));
         }
         KE* copy = head % A.group == 0 ? (KE*)A.keys + (slot * A.hk + kh) * 2 * C * KS : nullptr;
         write_keys<T, KE, KD>(wk, K, copy, ks);
@@ -106,14 +109,14 @@ __global__ void __launch_bounds__(PREP, 4) k_delta_prep(const __grid_constant__ 
     KE *Tm = reinterpret_cast<KE*>(A.squares + unit * P::SQUARES) + low_at(warp), *Pm = Tm + P::PIECES * LOW;
     const int st = low_stride(warp);
     if (tid < C) {
-        F[tid] = cut[tid] ? 0.0f : expf(up[tid]);
+        F[tid] = cut[tid] ? 0.0f : expf(up[tid]) * (1.0f + low[tid]);
         F[C + tid] = decay_between(up, low, cut, C - 1, tid);
         F[2 * C + tid] = rate[tid];
         F[UP + tid] = up[tid];
         F[UP_LOW + tid] = low[tid];
         reinterpret_cast<int*>(F + CUT)[tid] = cut[tid];
         if (tid == 0) {
-            F[LOST] = cut[C - 1] ? 1.0f : -expm1f(up[C - 1]);
+            F[LOST] = cut[C - 1] ? 1.0f : fmaf(-low[C - 1], expf(up[C - 1]), -expm1f(up[C - 1]));
             F[K_SCALE] = ks;
             F[Q_SCALE] = qs;
         }

@@ -158,11 +158,11 @@ __device__ __forceinline__ void write_state(const float (&S)[NT][4], float back,
 
 
 // Accumulators that are the first operand of products as they are, in pieces: times a
-// power of two that keeps their largest magnitude in 2^6 .. 2^15, changed only where it
-// leaves that.  The scale is returned.
+// power of two (scale) that keeps their largest magnitude (top) in 2^6 .. 2^15, changed
+// only where it leaves that.
 template <int NT>
-__device__ __forceinline__ float recentre(float (&S)[NT][4], float scale) {
-    const float top = warp_top(S);
+__device__ __forceinline__ void recentre(float (&S)[NT][4], float& scale, float& top) {
+    top = warp_top(S);
     if (top >= 0x1p15f || (top < 0x1p6f && top > 0.0f && scale < 0x1p60f)) {
         const float f = fminf(scale_for(top), 0x1p60f * inverse_of(scale));
 #pragma unroll
@@ -170,16 +170,17 @@ __device__ __forceinline__ float recentre(float (&S)[NT][4], float scale) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) S[i][e] *= f;
         scale *= f;
+        top *= f;
     }
-    return scale;
 }
-// the same for a state to which products of x and y (already times its scale, to be pieces)
-// are to be added
+// The same before products of x and y, which are already times their part of the scale to be
+// pieces, are added to what a chunk leaves of S (at most top): neither is too large for
+// a piece, nor all of them so small that pieces lose bits.
 template <int NT>
-__device__ __forceinline__ float make_room(float (&S)[NT][4], float (&x)[8][4], float (&y)[8][4], float scale) {
-    const float top = fmaxf(warp_top(x), warp_top(y));
-    if (top >= 0x1p15f) {
-        const float f = scale_for(top);
+__device__ __forceinline__ void make_room(float (&S)[NT][4], float (&x)[8][4], float (&y)[8][4], float& scale, float top) {
+    const float both = fmaxf(warp_top(x), &x != &y ? warp_top(y) : 0.0f), all = fmaxf(both, top);
+    if (both >= 0x1p15f || (all < 0x1p6f && all > 0.0f && scale < 0x1p60f)) {
+        const float f = fminf(scale_for(both >= 0x1p15f ? both : all), 0x1p60f * inverse_of(scale));
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -193,7 +194,22 @@ __device__ __forceinline__ float make_room(float (&S)[NT][4], float (&x)[8][4], 
             }
         scale *= f;
     }
-    return scale;
+}
+// S times the decays of a chunk: by what they take off where that is little, since 1 - lost keeps its
+// bits there (and S those that it has)
+template <int NT>
+__device__ __forceinline__ void decay_state(float (&S)[NT][4], float lost, float kept) {
+    if (lost < 0.5f) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) S[i][e] = fmaf(-lost, S[i][e], S[i][e]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) S[i][e] *= kept;
+    }
 }
 // acc [16, 64] += x m^T (ROWS; m lower triangular: steps k <= n) or x m (k >= n), in N pieces
 template <class P, int N, bool ROWS, typename F>
@@ -285,7 +301,8 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_scan(const __grid_constant
             if (w > 0) {
                 const int n = min(C, sp.len - c * C);
                 const long long unit = (sp.chunk + c) * A.heads + head;
-                if constexpr (P::SCALED) sigma = recentre(S, sigma);
+                float top = 0.0f;
+                if constexpr (P::SCALED) recentre(S, sigma, top);
                 float back = inverse_of(sigma), ik = 1.0f, iq = 1.0f;
                 if constexpr (P::SCALED) {
                     ik = inverse_of(st.f[K_SCALE]);
@@ -348,12 +365,8 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_scan(const __grid_constant
 #pragma unroll
                     for (int e = 0; e < 4; ++e) u[i][e] *= (e & 1 ? until.y : until.x) * sigma * ik;
                 }
-                if constexpr (P::SCALED) sigma = make_room(S, u, u, sigma);
-                const float lost = st.f[LOST];
-#pragma unroll
-                for (int i = 0; i < NT; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) S[i][e] = fmaf(-lost, S[i][e], S[i][e]);
+                if constexpr (P::SCALED) make_room(S, u, u, sigma, top * st.f[C - 1]);
+                decay_state(S, st.f[LOST], st.f[C - 1]);
                 add_outer<P, KD>(S, u, st.k);
             }
             __syncthreads();
@@ -398,7 +411,8 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_back(const __grid_constant
             if (w > 0) {
                 const int n = min(C, sp.len - c * C);
                 const long long unit = (sp.chunk + c) * A.heads + head;
-                if constexpr (P::SCALED) sigma = recentre(D, sigma);
+                float top = 0.0f;
+                if constexpr (P::SCALED) recentre(D, sigma, top);
                 float back = inverse_of(sigma), ik = 1.0f, iq = 1.0f;
                 if constexpr (P::SCALED) {
                     ik = inverse_of(st.f[K_SCALE]);
@@ -453,14 +467,8 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_back(const __grid_constant
                     }
                 }
                 store_tile<T, VS>(r, st.v + warp * 16, (T*)A.dv.p + row_at(A, A.dv, s, sp, c * C) + head * A.dv.hs + col, A.dv.st, n, w, A.dv.word);
-                if constexpr (P::SCALED) {
-                    sigma = make_room(D, u, z, sigma);
-                }
-                const float lost = st.f[LOST];
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) D[j][e] = fmaf(-lost, D[j][e], D[j][e]);
+                if constexpr (P::SCALED) make_room(D, u, z, sigma, top * st.f[C - 1]);
+                decay_state(D, st.f[LOST], st.f[C - 1]);
                 add_outer<P, KD>(D, z, st.q);
                 add_outer<P, KD>(D, u, st.k);
             }

@@ -34,6 +34,8 @@ void with_elem(int32_t type, F&& f) {
 // Whether runs of `width` elements, one for each index of dimensions {count, stride},
 // lie apart (each stride clears what the smaller ones span)
 inline bool apart(std::vector<std::pair<int64_t, int64_t>> dims, int64_t width) {
+    for (const auto& d : dims)
+        if (d.first == 0) return true;
     std::sort(dims.begin(), dims.end(), [](auto& a, auto& b) { return a.second < b.second; });
     for (const auto& [count, stride] : dims) {
         if (count <= 1) continue;

@@ -568,6 +568,8 @@ def _heads(t, name, shape, dtype):
         raise SnnError(1, f"{name} must be {tuple(shape)} in {dtype}, not {tuple(t.shape)} in {t.dtype}")
     st = t.stride()
     if st[-1] != 1 and shape[-1] != 1:
+        if t.numel() == 0:  # (torch gives these any strides)
+            return _HEADS.pack(0, 0, 0, 0)
         raise SnnError(1, f"{name} wants unit stride in its last dimension")
     return _HEADS.pack(t.data_ptr(), st[0], st[-3], st[-2])
 
@@ -688,6 +690,13 @@ def qk_norm_grad(q, k, dyq, dyk, q_weight=None, k_weight=None, positions=None, f
 _DELTA = struct.Struct("=iiqqqqqqQfi")  # snn_delta
 
 
+def _gate_rows(t, name, shape, dtype):
+    """_scan_rows, of tensors without elements too (torch gives these any strides)"""
+    if t.shape == shape and t.dtype == dtype and t.numel() == 0:
+        return _ROWS.pack(0, 0, 0)
+    return _scan_rows(t, name, shape, dtype)
+
+
 def _delta_args(q, k, v, gate, beta, scale, logit, offsets, zero):
     """(snn_delta, (snn_heads of q, k, v, snn_rows of gate, beta), the states' shape, _delta_sizes)"""
     if _T is None:
@@ -704,7 +713,7 @@ def _delta_args(q, k, v, gate, beta, scale, logit, offsets, zero):
     if not (hk and dk and dv and heads and heads % hk == 0):
         raise SnnError(1, "the heads of v must be a multiple of those of q and k, no dimension of heads empty")
     rows = (_heads(q, "q", (*lead, hk, dk), dtype), _heads(k, "k", (*lead, hk, dk), dtype), _heads(v, "v", shape, dtype),
-            _scan_rows(gate, "gate", (*lead, heads), dtype), _scan_rows(beta, "beta", (*lead, heads), dtype))
+            _gate_rows(gate, "gate", (*lead, heads), dtype), _gate_rows(beta, "beta", (*lead, heads), dtype))
     flags = SCAN_LOGIT if logit else 0
     if offsets is None:
         n_seq, off = shape[0], 0
