@@ -56,12 +56,33 @@ __device__ __forceinline__ Moments moments(const Rule& r, float g, float m, floa
 __device__ __forceinline__ float updated(const Rule& r, float size, float root, float p, Moments x) {
     return p * r.decay - x.m / (sqrtf(x.v) * root + r.eps) * size;
 }
-__device__ __forceinline__ float from_e4m3(unsigned char c) {
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+// Four e4m3 values in a word
+__device__ __forceinline__ void from_e4m3(unsigned w, float* o) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const __half2 h = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (16 * i)), __NV_E4M3));
+        const float2 f = __half22float2(h);
+        o[2 * i] = f.x;
+        o[2 * i + 1] = f.y;
+    }
 }
-__device__ __forceinline__ unsigned char to_e4m3(float v) {
-    return (unsigned char)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+__device__ __forceinline__ unsigned to_e4m3(const float* v) {
+    return (unsigned)__nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E4M3) |
+           (unsigned)__nv_cvt_float2_to_fp8x2(make_float2(v[2], v[3]), __NV_SATFINITE, __NV_E4M3) << 16;
 }
+// Quotients by one divisor, rounded as a division is: from the rounded reciprocal, a product and
+// one correction by the remainder, which a fused product has exactly (Markstein 1990).  The remainder
+// must not be lost below the smallest numbers: divisors outside 2^-80 .. 2^80 are divided by.
+struct Divisor {
+    float d, inv;
+    bool plain;
+    __device__ __forceinline__ explicit Divisor(float v) : d(v), inv(1.0f / v), plain(!(v > 0x1p-80f && v < 0x1p80f)) {}
+    __device__ __forceinline__ float under(float a) const {
+        if (plain) return a / d;
+        const float q = a * inv;
+        return fmaf(fmaf(-q, d, a), inv, q);
+    }
+};
 
 template <typename T, int V>
 struct alignas(sizeof(T) * V > 16 ? 16 : sizeof(T) * V) Word {
@@ -90,6 +111,28 @@ __device__ __forceinline__ void store(T* p, int n, bool wide, const T (&o)[V]) {
 #pragma unroll
         for (int i = 0; i < V; ++i)
             if (i < n) p[i] = o[i];
+    }
+}
+// eight bytes
+__device__ __forceinline__ void load8(const unsigned char* p, int n, bool wide, unsigned (&o)[2]) {
+    if (wide && n == 8) {
+        const uint2 w = *reinterpret_cast<const uint2*>(p);
+        o[0] = w.x;
+        o[1] = w.y;
+    } else {
+        o[0] = o[1] = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) o[i / 4] |= (unsigned)p[i] << (8 * (i % 4));
+    }
+}
+__device__ __forceinline__ void store8(unsigned char* p, int n, bool wide, const unsigned (&o)[2]) {
+    if (wide && n == 8) {
+        *reinterpret_cast<uint2*>(p) = make_uint2(o[0], o[1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) p[i] = (unsigned char)(o[i / 4] >> (8 * (i % 4)));
     }
 }
 template <int V>
@@ -141,20 +184,25 @@ __device__ __forceinline__ void chunk(const Rule& r, const Tensor& t, int64_t be
             const int n = (int)max((int64_t)0, min((int64_t)V, end - at));
             G g[V];
             float p[V], m[V], v[V];
-            unsigned char m8[V], v8[V];
+            unsigned m8[2], v8[2];
             load<V>(reinterpret_cast<const G*>(t.g) + at, n, t.wide, g);
             load<V>(t.p + at, n, t.wide, p);
-            load<V>(reinterpret_cast<const unsigned char*>(t.m) + at, n, t.wide, m8);
-            load<V>(reinterpret_cast<const unsigned char*>(t.v) + at, n, t.wide, v8);
+            load8(reinterpret_cast<const unsigned char*>(t.m) + at, n, t.wide, m8);
+            load8(reinterpret_cast<const unsigned char*>(t.v) + at, n, t.wide, v8);
+            float om[V], ov[V];
+            from_e4m3(m8[0], om);
+            from_e4m3(m8[1], om + 4);
+            from_e4m3(v8[0], ov);
+            from_e4m3(v8[1], ov + 4);
             float ms = t.ms[b / BLOCK], vs = t.vs[b / BLOCK], top_m = 0.0f, top_v = 0.0f;
             bool nan_m = false, nan_v = false;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float root_v = from_e4m3(v8[i]) * vs;
-                const Moments x = moments(r, to_f32(g[i]), from_e4m3(m8[i]) * ms, root_v * root_v);
-                p[i] = updated(r, size, root, p[i], x);
-                m[i] = x.m;
+                const float root_v = ov[i] * vs;
+                const Moments x = moments(r, to_f32(g[i]), om[i] * ms, root_v * root_v);
                 v[i] = sqrtf(x.v);
+                p[i] = p[i] * r.decay - x.m / (v[i] * root + r.eps) * size;
+                m[i] = x.m;
                 if (i < n) {
                     top_m = fmaxf(top_m, fabsf(m[i]));
                     top_v = fmaxf(top_v, v[i]);
@@ -172,15 +220,20 @@ __device__ __forceinline__ void chunk(const Rule& r, const Tensor& t, int64_t be
             // a block that holds a NaN becomes NaN as a whole, and says so
             ms = __any_sync(~0u, nan_m) ? NAN : top_m * (1.0f / 448.0f);
             vs = __any_sync(~0u, nan_v) ? NAN : top_v * (1.0f / 448.0f);
+            const Divisor dm(ms), dv(vs);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                m8[i] = to_e4m3(ms > 0.0f ? m[i] / ms : ms);
-                float z = vs > 0.0f ? v[i] / vs : vs;
-                if (v[i] > 0.0f) z = fmaxf(z, 0x1p-9f);
-                v8[i] = to_e4m3(z);
+                m[i] = ms > 0.0f ? dm.under(m[i]) : ms;
+                const float z = vs > 0.0f ? dv.under(v[i]) : vs;
+                v[i] = v[i] > 0.0f ? fmaxf(z, 0x1p-9f) : z;
             }
-            store<V>(reinterpret_cast<unsigned char*>(t.m) + at, n, t.wide, m8);
-            store<V>(reinterpret_cast<unsigned char*>(t.v) + at, n, t.wide, v8);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                m8[i] = to_e4m3(m + 4 * i);
+                v8[i] = to_e4m3(v + 4 * i);
+            }
+            store8(reinterpret_cast<unsigned char*>(t.m) + at, n, t.wide, m8);
+            store8(reinterpret_cast<unsigned char*>(t.v) + at, n, t.wide, v8);
             if (lane == 0) {
                 t.ms[b / BLOCK] = ms;
                 t.vs[b / BLOCK] = vs;

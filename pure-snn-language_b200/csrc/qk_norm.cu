@@ -6,16 +6,17 @@
 // Bound by memory: every element is read once and written once.  A group of G
 // lanes takes a head, a lane whole words of up to 16 bytes of it such that both
 // elements of a rotated pair are its own, so that nothing but the sum of squares
-// crosses lanes.  Cosines and sines of a row are made once for all of its heads,
-// in shared memory; angles are products in 64 bits (a position of 1e5 has an angle
-// whose f32 would be off by 4e-3), reduced to a turn before the f32 sine.
+// crosses lanes.  Cosines and sines of a row are made once for all of its heads of both
+// sides, in shared memory, where the weights lie too (in registers, both cost two of five
+// CTAs an SM, and more time than the reads).  Angles are products in 64 bits (a position
+// of 1e5 has an angle whose f32 would be off by 4e-3), reduced to a turn before the f32 sine.
 #include <algorithm>
 #include "elem.h"
 
 namespace {
 using snnb::from_f32;
 using snnb::to_f32;
-constexpr int SMS = 148, THREADS = 256, MAX_DIM = 512, MAX_ROWS = 8;
+constexpr int SMS = 148, THREADS = 256, MAX_DIM = 512, MAX_ROWS = 16;
 
 struct Heads {
     void* p;
@@ -32,7 +33,7 @@ struct NormArgs {
     const void* pos;
     const float* freqs;
     long long rows, steps;
-    int dim, rot, per_tile, pos64, adjacent;
+    int dim, rot, per_tile, places, pos64, adjacent;  // places: of a row's cosines and sines
     float eps, inv_count;
 };
 
@@ -57,37 +58,62 @@ __device__ __forceinline__ void words_of(const NormArgs& A, int s, int& a, int& 
         b = s + P;
     }
 }
-// The pairs of words a, b of slot s turned (BACK: the other way).  IN: pairs lie
-// inside a word.
+// Cosine and sine of pair j, and weight j, lie at place_of<V>(j): lanes read theirs side by side
+template <int V>
+__device__ __forceinline__ int place_of(int j, int n) { return j % V * ((n + V - 1) / V) + j / V; }
+// The pairs of the two words of slot s turned (BACK: the other way), its pairs being s V .. s V +
+// V - 1.  IN: they lie inside a word.
 template <int V, bool IN, bool BACK>
-__device__ __forceinline__ void turn(const NormArgs& A, const float2* cs, int s, float (&a)[V], float (&b)[V]) {
-    auto pair = [&](float& u, float& v, int j) {
-        const float2 c = cs[j];
+__device__ __forceinline__ void turn(int half, const float2* cs, int s, float (&a)[V], float (&b)[V]) {
+    if (s * V >= half) return;
+    const int step = (half + V - 1) / V;
+    auto pair = [&](float& u, float& v, int i) {
+        const float2 c = cs[i * step + s];
         const float si = BACK ? -c.y : c.y, x = u, y = v;
-        u = x * c.x - y * si;
-        v = x * si + y * c.x;
+        u = fmaf(x, c.x, -(y * si));
+        v = fmaf(x, si, y * c.x);
     };
-    const int half = A.rot / 2;
-    if constexpr (IN) {
-        if constexpr (V > 1) {
+    if constexpr (IN && V > 1) {
 #pragma unroll
-            for (int i = 0; i < V / 2; ++i) {
-                const int j = s * V + i;
-                if (j < half) pair(a[2 * i], a[2 * i + 1], j);
-                if (j + V / 2 < half) pair(b[2 * i], b[2 * i + 1], j + V / 2);
+        for (int i = 0; i < V / 2; ++i) {
+            if (s * V + i < half) pair(a[2 * i], a[2 * i + 1], i);
+            if (s * V + i + V / 2 < half) pair(b[2 * i], b[2 * i + 1], i + V / 2);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) pair(a[i], b[i], i);
+    }
+}
+template <typename T, int V>
+__device__ __forceinline__ Word<T, V> word_of(const float (&o)[V]) {
+    Word<T, V> x;
+    if constexpr (sizeof(T) == 2 && V > 1) {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+            if constexpr (std::is_same<T, __half>::value) {
+                const __half2 h = __floats2half2_rn(o[i], o[i + 1]);
+                x.v[i] = __low2half(h);
+                x.v[i + 1] = __high2half(h);
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(o[i], o[i + 1]);
+                x.v[i] = __low2bfloat16(h);
+                x.v[i + 1] = __high2bfloat16(h);
             }
         }
-    } else if (s * V < half) {
+    } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) pair(a[i], b[i], s * V + i);
+        for (int i = 0; i < V; ++i) x.v[i] = from_f32<T>(o[i]);
     }
+    return x;
 }
 
 // V elements a word, SL slots of two words a lane, G lanes a head
+// CTAs that an SM has registers for
+__host__ __device__ constexpr int resident(int v, int sl, bool grad) { return v * sl > 8 ? 2 : grad ? (v == 8 ? 2 : 3) : 4; }
 template <typename T, int V, int SL, bool IN, bool GRAD>
-__global__ void __launch_bounds__(THREADS) k_qk_norm(const __grid_constant__ NormArgs A, int G) {
-    extern __shared__ float2 cs[];  // [rows of a tile][rot / 2]
-    __shared__ float sum[GRAD ? MAX_DIM : 1];
+__global__ void __launch_bounds__(THREADS, resident(V, SL, GRAD)) k_qk_norm(const __grid_constant__ NormArgs A, int G) {
+    extern __shared__ float2 tables[];  // [2][rows of a tile][places]
+    __shared__ float weight[2][MAX_DIM], sum[GRAD ? MAX_DIM : 1];
     using W = Word<T, V>;
     const int lane = threadIdx.x & (G - 1), group = threadIdx.x / G, groups = THREADS / G, half = A.rot / 2;
     const int words = A.dim / V;
@@ -99,133 +125,153 @@ __global__ void __launch_bounds__(THREADS) k_qk_norm(const __grid_constant__ Nor
     int wa[SL], wb[SL];
 #pragma unroll
     for (int i = 0; i < SL; ++i) words_of<V, IN>(A, lane + i * G, wa[i], wb[i]);
+    for (int i = threadIdx.x; i < A.dim; i += THREADS) {
+        weight[0][place_of<V>(i, A.dim)] = A.side[0].w ? A.side[0].w[i] : 1.0f;
+        weight[1][place_of<V>(i, A.dim)] = A.side[1].w ? A.side[1].w[i] : 1.0f;
+    }
     auto load = [&](const T* p, int w, float (&o)[V]) {
-        if (w < words) {
-            const W x = *reinterpret_cast<const W*>(p + w * V);
+        W x = {};
+        if (w < words) x = *reinterpret_cast<const W*>(p + w * V);
 #pragma unroll
-            for (int i = 0; i < V; ++i) o[i] = to_f32(x.v[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) o[i] = 0.0f;
-        }
+        for (int i = 0; i < V; ++i) o[i] = to_f32(x.v[i]);
     };
     auto store = [&](T* p, int w, const float (&o)[V]) {
-        if (w >= words) return;
-        W x;
-#pragma unroll
-        for (int i = 0; i < V; ++i) x.v[i] = from_f32<T>(o[i]);
-        *reinterpret_cast<W*>(p + w * V) = x;
+        if (w < words) *reinterpret_cast<W*>(p + w * V) = word_of<T, V>(o);
     };
-#pragma unroll 1
-    for (int which = 0; which < 2; ++which) {
+    // o times the weights of word w
+    auto weigh = [&](const float* wt, int w, float (&o)[V]) {
+        if (w >= words) return;
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] *= wt[i * words + w];
+    };
+    float da[2][GRAD ? SL : 1][V] = {}, db[2][GRAD ? SL : 1][V] = {};
+    const int per_row = groups / A.per_tile, r = group / per_row;  // groups that take a row's heads in turn
+    auto heads = [&](auto which_, const float2* c, long long row) {
+        constexpr int which = decltype(which_)::value;
         const Side& S = A.side[which];
-        if (!S.x.p) continue;
-        float ga[SL][V], gb[SL][V], da[GRAD ? SL : 1][V], db[GRAD ? SL : 1][V];
-#pragma unroll
-        for (int i = 0; i < SL; ++i)
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                ga[i][j] = S.w && wa[i] < words ? S.w[wa[i] * V + j] : 1.0f;
-                gb[i][j] = S.w && wb[i] < words ? S.w[wb[i] * V + j] : 1.0f;
-                if (GRAD) da[i][j] = db[i][j] = 0.0f;
-            }
+        int head = group - r * per_row;
+        if (head >= S.heads) return;
+        const T* x = reinterpret_cast<const T*>(S.x.p) + row_at(S.x, A, row) + head * S.x.hs;
+        T* y = reinterpret_cast<T*>(S.y.p) + row_at(S.y, A, row) + head * S.y.hs;
+        T* dx = GRAD ? reinterpret_cast<T*>(S.dx.p) + row_at(S.dx, A, row) + head * S.dx.hs : nullptr;
+        // (the loop's end is the same for all lanes of a group: they shuffle among themselves)
 #pragma unroll 1
-        for (long long tile = (long long)blockIdx.x * A.per_tile; tile < A.rows; tile += (long long)gridDim.x * A.per_tile) {
-            const int n = (int)min((long long)A.per_tile, A.rows - tile);
-            __syncthreads();
-            for (int i = threadIdx.x; i < n * half; i += THREADS) {
-                const int r = i / half;
-                const long long at = tile + r;
-                const double pos = A.pos64 ? (double)reinterpret_cast<const long long*>(A.pos)[at]
-                                           : (double)reinterpret_cast<const int*>(A.pos)[at];
-                const double turns = pos * (double)A.freqs[i - r * half] * 0.15915494309189533577;  // 1 / (2 pi)
-                float s, c;
-                sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-                cs[i] = make_float2(c, s);
+        for (; head < S.heads; head += per_row, x += per_row * S.x.hs, y += per_row * S.y.hs, dx += GRAD ? per_row * S.dx.hs : 0) {
+            float a[SL][V], b[SL][V];
+            [[maybe_unused]] float za[GRAD ? SL : 1][V], zb[GRAD ? SL : 1][V];
+#pragma unroll
+            for (int i = 0; i < SL; ++i) {
+                load(x, wa[i], a[i]);
+                load(x, wb[i], b[i]);
+                if constexpr (GRAD) {
+                    load(y, wa[i], za[i]);
+                    load(y, wb[i], zb[i]);
+                }
             }
-            __syncthreads();
-            for (int e = group; e < n * S.heads; e += groups) {
-                const int r = e / S.heads, head = e - r * S.heads;
-                const long long row = tile + r;
-                const float2* c = cs + r * half;
-                const T* x = reinterpret_cast<const T*>(S.x.p) + row_at(S.x, A, row) + head * S.x.hs;
-                T* y = reinterpret_cast<T*>(S.y.p) + row_at(S.y, A, row) + head * S.y.hs;
-                float a[SL][V], b[SL][V], za[GRAD ? SL : 1][V], zb[GRAD ? SL : 1][V];
+            float sq = 0.0f;
+#pragma unroll
+            for (int i = 0; i < SL; ++i)
+#pragma unroll
+                for (int j = 0; j < V; ++j) sq = fmaf(a[i][j], a[i][j], fmaf(b[i][j], b[i][j], sq));
+            const float inv = rsqrtf(fmaf(all(sq), A.inv_count, A.eps));
+#pragma unroll
+            for (int i = 0; i < SL; ++i)
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    a[i][j] *= inv;
+                    b[i][j] *= inv;
+                }
+            if constexpr (!GRAD) {
 #pragma unroll
                 for (int i = 0; i < SL; ++i) {
-                    load(x, wa[i], a[i]);
-                    load(x, wb[i], b[i]);
-                    if constexpr (GRAD) {
-                        load(y, wa[i], za[i]);
-                        load(y, wb[i], zb[i]);
+                    if (S.w) {
+                        weigh(weight[which], wa[i], a[i]);
+                        weigh(weight[which], wb[i], b[i]);
                     }
+                    turn<V, IN, false>(half, c, lane + i * G, a[i], b[i]);
+                    store(y, wa[i], a[i]);
+                    store(y, wb[i], b[i]);
                 }
-                float sq = 0.0f;
+            } else {
+                float dot = 0.0f;
 #pragma unroll
-                for (int i = 0; i < SL; ++i)
-#pragma unroll
-                    for (int j = 0; j < V; ++j) sq = fmaf(a[i][j], a[i][j], fmaf(b[i][j], b[i][j], sq));
-                const float inv = 1.0f / sqrtf(fmaf(all(sq), A.inv_count, A.eps));
-                if constexpr (!GRAD) {
-#pragma unroll
-                    for (int i = 0; i < SL; ++i) {
+                for (int i = 0; i < SL; ++i) {
+                    turn<V, IN, true>(half, c, lane + i * G, za[i], zb[i]);
+                    if (S.w) {
 #pragma unroll
                         for (int j = 0; j < V; ++j) {
-                            a[i][j] = a[i][j] * inv * ga[i][j];
-                            b[i][j] = b[i][j] * inv * gb[i][j];
+                            da[which][i][j] = fmaf(za[i][j], a[i][j], da[which][i][j]);
+                            db[which][i][j] = fmaf(zb[i][j], b[i][j], db[which][i][j]);
                         }
-                        turn<V, IN, false>(A, c, lane + i * G, a[i], b[i]);
-                        store(y, wa[i], a[i]);
-                        store(y, wb[i], b[i]);
+                        weigh(weight[which], wa[i], za[i]);
+                        weigh(weight[which], wb[i], zb[i]);
                     }
-                } else {
-                    float dot = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < SL; ++i) {
-                        turn<V, IN, true>(A, c, lane + i * G, za[i], zb[i]);
+                    for (int j = 0; j < V; ++j) dot = fmaf(za[i][j], a[i][j], fmaf(zb[i][j], b[i][j], dot));
+                }
+                dot = all(dot) * A.inv_count;
 #pragma unroll
-                        for (int j = 0; j < V; ++j) {
-                            a[i][j] *= inv;
-                            b[i][j] *= inv;
-                            da[i][j] = fmaf(za[i][j], a[i][j], da[i][j]);
-                            db[i][j] = fmaf(zb[i][j], b[i][j], db[i][j]);
-                            za[i][j] *= ga[i][j];
-                            zb[i][j] *= gb[i][j];
-                            dot = fmaf(za[i][j], a[i][j], fmaf(zb[i][j], b[i][j], dot));
-                        }
+                for (int i = 0; i < SL; ++i) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        a[i][j] = inv * fmaf(-a[i][j], dot, za[i][j]);
+                        b[i][j] = inv * fmaf(-b[i][j], dot, zb[i][j]);
                     }
-                    dot = all(dot) * A.inv_count;
-                    T* dx = reinterpret_cast<T*>(S.dx.p) + row_at(S.dx, A, row) + head * S.dx.hs;
-#pragma unroll
-                    for (int i = 0; i < SL; ++i) {
-#pragma unroll
-                        for (int j = 0; j < V; ++j) {
-                            a[i][j] = inv * fmaf(-a[i][j], dot, za[i][j]);
-                            b[i][j] = inv * fmaf(-b[i][j], dot, zb[i][j]);
-                        }
-                        store(dx, wa[i], a[i]);
-                        store(dx, wb[i], b[i]);
-                    }
+                    store(dx, wa[i], a[i]);
+                    store(dx, wb[i], b[i]);
                 }
             }
         }
-        if constexpr (GRAD) {  // the groups' sums, one group after the other
-            if (!S.part) continue;
+    };
+    auto table = [&](long long tile, float2* cs) {
+        const int n = (int)min((long long)A.per_tile, A.rows - tile);
+        for (int i = threadIdx.x; i < n * half; i += THREADS) {
+            const int k = i / half;
+            const long long at = tile + k;
+            const double pos = A.pos64 ? (double)reinterpret_cast<const long long*>(A.pos)[at]
+                                       : (double)reinterpret_cast<const int*>(A.pos)[at];
+            const double turns = pos * (double)A.freqs[i - k * half] * 0.15915494309189533577;  // 1 / (2 pi)
+            float s, c;
+            sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
+            cs[k * A.places + place_of<V>(i - k * half, half)] = make_float2(c, s);
+        }
+    };
+    const long long step = (long long)gridDim.x * A.per_tile;
+    long long tile = (long long)blockIdx.x * A.per_tile;
+    float2 *now = tables, *next = tables + A.per_tile * A.places;
+    if (tile < A.rows) table(tile, now);
 #pragma unroll 1
-            for (int g = 0; g < groups; ++g) {
+    for (; tile < A.rows; tile += step) {
+        __syncthreads();  // this tile's table is there, the other one's is no longer read
+        if (tile + step < A.rows) table(tile + step, next);
+        if (tile + r < A.rows) {
+            heads(std::integral_constant<int, 0>(), now + r * A.places, tile + r);
+            heads(std::integral_constant<int, 1>(), now + r * A.places, tile + r);
+        }
+        float2* t = now;
+        now = next;
+        next = t;
+    }
+    if constexpr (GRAD) {  // the groups' sums, one group after the other
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            float* part = A.side[which].part;
+            if (!part) continue;
+#pragma unroll 1
+            for (int k = 0; k < groups; ++k) {
                 __syncthreads();
-                if (group == g)
+                if (group == k)
 #pragma unroll
                     for (int i = 0; i < SL; ++i)
 #pragma unroll
                         for (int j = 0; j < V; ++j) {
                             const int ea = wa[i] * V + j, eb = wb[i] * V + j;
-                            if (wa[i] < words) sum[ea] = g ? sum[ea] + da[i][j] : da[i][j];
-                            if (wb[i] < words) sum[eb] = g ? sum[eb] + db[i][j] : db[i][j];
+                            if (wa[i] < words) sum[ea] = k ? sum[ea] + da[which][i][j] : da[which][i][j];
+                            if (wb[i] < words) sum[eb] = k ? sum[eb] + db[which][i][j] : db[which][i][j];
                         }
             }
             __syncthreads();
-            for (int i = threadIdx.x; i < A.dim; i += THREADS) S.part[(long long)blockIdx.x * A.dim + i] = sum[i];
+            for (int i = threadIdx.x; i < A.dim; i += THREADS) part[(long long)blockIdx.x * A.dim + i] = sum[i];
         }
     }
 }
@@ -238,6 +284,7 @@ __global__ void __launch_bounds__(1024) k_qk_norm_sum(const __grid_constant__ No
     const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, c = (int)blockIdx.x * 32 + lane;
     float v = 0.0f;
     if (c < A.dim)
+#pragma unroll 8
         for (int i = g; i < ctas; i += 32) v += S.part[(long long)i * A.dim + c];
     s[g][lane] = v;
     __syncthreads();
@@ -280,64 +327,75 @@ Heads heads_of(const snn_qk* d, const snn_heads* h, int64_t heads, const char* n
     return {h->data, ss, st, hs};
 }
 
-struct Plan {
-    int per_tile, ctas;
-};
-// Rows of a tile: up to 8, as far as that leaves eight CTAs an SM.  With gradients of
-// weights each CTA leaves a row of sums, so they are at most four an SM.
-Plan plan_of(const snn_qk* d, bool grad) {
-    Plan p;
-    const int64_t n = rows_of(d);
-    p.per_tile = (int)std::min<int64_t>(MAX_ROWS, std::max<int64_t>(1, n / (8 * SMS)));
-    const int64_t tiles = (n + p.per_tile - 1) / p.per_tile;
-    p.ctas = (int)std::min<int64_t>(tiles, grad ? 4 * SMS : 64 * SMS);
-    return p;
-}
-
-template <typename T, int V, int SL, bool IN, bool GRAD>
-void launch(const NormArgs& A, int ctas, int G, cudaStream_t st) {
-    k_qk_norm<T, V, SL, IN, GRAD><<<ctas, THREADS, (size_t)A.per_tile * (A.rot / 2) * 8, st>>>(A, G);
-    SNN_CUDA(cudaGetLastError());
-}
-template <typename T, int V, bool GRAD>
-void by_slots(const NormArgs& A, int ctas, cudaStream_t st) {
-    const int words = A.dim / V, slots = (words + 1) / 2;
-    int G = 1;
-    while (G < 32 && G < slots) G *= 2;
-    const int per = (slots + G - 1) / G;
-    const bool in = V > 1 && A.adjacent;
-    constexpr int MOST = MAX_DIM / V / 64;  // slots a lane may have
-    if constexpr (MOST >= 2)
-        if (per > 1) {
-            if (in) launch<T, V, MOST, V != 1, GRAD>(A, ctas, G, st);
-            else launch<T, V, MOST, false, GRAD>(A, ctas, G, st);
-            return;
-        }
-    if (in) launch<T, V, 1, V != 1, GRAD>(A, ctas, G, st);
-    else launch<T, V, 1, false, GRAD>(A, ctas, G, st);
-}
-
-template <bool GRAD>
-void run(const snn_qk* d, NormArgs& A, cudaStream_t st) {
-    const Plan p = plan_of(d, GRAD);
-    A.per_tile = p.per_tile;
+// The widest word that rows, heads and (pairs of halves) the halves consist of
+int width_of(const snn_qk* d, const NormArgs& A) {
     const int size = snnb::elem_size(d->type);
-    // The widest word that rows, heads and (pairs of halves) the halves consist of
-    auto fits = [&](int v) {
+    int v = 16 / size;
+    auto fits = [&] {
         if (d->dim % v || (!A.adjacent && A.rot % (2 * v))) return false;
         for (const Side& S : A.side)
             for (const Heads& h : {S.x, S.y, S.dx})
                 if (h.p && ((uintptr_t)h.p % (v * size) || h.ss % v || h.st % v || h.hs % v)) return false;
         return true;
     };
-    snnb::with_elem(d->type, [&](auto t) {
+    while (v > 1 && !fits()) v /= 2;
+    return v;
+}
+int lanes_of(const snn_qk* d, int v) {  // of a head
+    const int slots = ((int)d->dim / v + 1) / 2;
+    int G = 1;
+    while (G < 32 && G < slots) G *= 2;
+    return G;
+}
+// Rows of a tile: a power of two up to 16 and the groups of a CTA, as far as that leaves eight CTAs an SM.
+int rows_of_tile(const snn_qk* d, int v) {
+    int r = 1;
+    while (r < MAX_ROWS && r < THREADS / lanes_of(d, v) && rows_of(d) >= 2ll * r * 8 * SMS) r *= 2;
+    return r;
+}
+// CTAs of a gradient at most: each leaves a row of sums
+int most_ctas(const snn_qk* d) { return (int)std::min<int64_t>(std::max<int64_t>(1, rows_of(d)), 3 * SMS); }
+
+template <typename T, int V, int SL, bool IN, bool GRAD>
+int launch(const NormArgs& A, int tiles, int G, cudaStream_t st) {
+    // with sums of weights' gradients, and where it fills the SMs, one round of CTAs
+    const int ctas = std::min(tiles, (GRAD ? 1 : 4) * resident(V, SL, GRAD) * SMS);
+    auto* kernel = k_qk_norm<T, V, SL, IN, GRAD>;
+    const size_t smem = (size_t)2 * A.per_tile * A.places * 8;
+    if (smem > 40 * 1024) SNN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    kernel<<<ctas, THREADS, smem, st>>>(A, G);
+    SNN_CUDA(cudaGetLastError());
+    return ctas;
+}
+// the number of CTAs
+template <bool GRAD>
+int run(const snn_qk* d, NormArgs& A, cudaStream_t st) {
+    const int v = width_of(d, A), G = lanes_of(d, v), slots = ((int)d->dim / v + 1) / 2;
+    A.per_tile = rows_of_tile(d, v);
+    A.places = (A.rot / 2 + v - 1) / v * v;
+    const int tiles = (int)std::min<int64_t>(1 << 30, (rows_of(d) + A.per_tile - 1) / A.per_tile);
+    int ctas = 0;
+    auto by_slots = [&](auto t, auto vv) {
         using T = decltype(t);
-        constexpr int W = 16 / (int)sizeof(T);
-        if (fits(W)) by_slots<T, W, GRAD>(A, p.ctas, st);
-        else if (sizeof(T) == 2 && fits(4)) by_slots<T, 4, GRAD>(A, p.ctas, st);
-        else if (fits(2)) by_slots<T, 2, GRAD>(A, p.ctas, st);
-        else by_slots<T, 1, GRAD>(A, p.ctas, st);
+        constexpr int V = decltype(vv)::value, MOST = MAX_DIM / V / 64;  // slots that a lane may have
+        const bool in = V > 1 && A.adjacent;
+        if constexpr (MOST >= 2)
+            if (slots > G) {
+                if (in) ctas = launch<T, V, MOST, V != 1, GRAD>(A, tiles, G, st);
+                else ctas = launch<T, V, MOST, false, GRAD>(A, tiles, G, st);
+                return;
+            }
+        if (in) ctas = launch<T, V, 1, V != 1, GRAD>(A, tiles, G, st);
+        else ctas = launch<T, V, 1, false, GRAD>(A, tiles, G, st);
+    };
+    snnb::with_elem(d->type, [&](auto t) {
+        constexpr int W = 16 / (int)sizeof(t);
+        if (v == W) by_slots(t, std::integral_constant<int, W>());
+        else if (v == 4) by_slots(t, std::integral_constant<int, 4>());
+        else if (v == 2) by_slots(t, std::integral_constant<int, 2>());
+        else by_slots(t, std::integral_constant<int, 1>());
     });
+    return ctas;
 }
 
 NormArgs base_args(const snn_qk* d, const void* positions, const float* freqs) {
@@ -390,7 +448,7 @@ void qk_norm(const snn_qk* d, const snn_heads* q, const snn_heads* k, const floa
 
 int64_t qk_norm_grad_workspace(const snn_qk* d) {
     check_desc(d);
-    return (int64_t)plan_of(d, true).ctas * 2 * d->dim * 4;
+    return (int64_t)most_ctas(d) * 2 * d->dim * 4;
 }
 
 void qk_norm_grad(const snn_qk* d, const snn_heads* q, const snn_heads* k, const float* wq, const float* wk,
@@ -420,14 +478,14 @@ void qk_norm_grad(const snn_qk* d, const snn_heads* q, const snn_heads* k, const
             const int64_t need = qk_norm_grad_workspace(d);
             SNN_REQUIRE(work && (uintptr_t)work % 256 == 0 && work_bytes >= need, SNN_ERR_ARG,
                         "qk_norm: workspace null, misaligned or too small");
-            S.part = (float*)work + (i ? (int64_t)plan_of(d, true).ctas * d->dim : 0);
+            S.part = (float*)work + (i ? (int64_t)most_ctas(d) * d->dim : 0);
             sums = true;
         }
     }
     if (!A.side[0].x.p && !A.side[1].x.p) return;
-    run<true>(d, A, st);
+    const int ctas = run<true>(d, A, st);
     if (sums) {
-        k_qk_norm_sum<<<dim3((unsigned)((d->dim + 31) / 32), 2), 1024, 0, st>>>(A, plan_of(d, true).ctas);
+        k_qk_norm_sum<<<dim3((unsigned)((d->dim + 31) / 32), 2), 1024, 0, st>>>(A, ctas);
         SNN_CUDA(cudaGetLastError());
     }
 }
