@@ -30,6 +30,7 @@ constexpr int STEP_WARPS = 16;
 template <typename T, int V>
 __global__ void __launch_bounds__(32 * STEP_WARPS, 2) k_delta_steps(const __grid_constant__ DeltaArgs A) {
     constexpr int R = MAX_K / STEP_WARPS;  // rows of a warp
+    __shared__ float factor[3];  // what a decay takes off, what it leaves, the rate
     __shared__ __align__(16) float key[MAX_K], query[MAX_K], part[STEP_WARPS][2][32 * V];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int head = blockIdx.y, col = ((int)blockIdx.z * 32 + lane) * V, kh = head / A.group;
@@ -56,15 +57,25 @@ __global__ void __launch_bounds__(32 * STEP_WARPS, 2) k_delta_steps(const __grid
                 const int d = tid - MAX_K;
                 query[d] = d < A.kdim ? to_f32(((const T*)A.q.p)[row_at(A, A.q, s, sp, t) + kh * A.q.hs + d]) : 0.0f;
             }
-            float v[V];
+            if (tid == 2 * MAX_K) {
+                const float l = log_decay(A, ((const T*)A.gate.p)[row_at(A, A.gate, s, sp, t) + head * A.gate.hs]);
+                factor[0] = -expm1f(l);  // 1 - a keeps its bits where a is near 1
+                factor[1] = expf(l);
+                factor[2] = rate_of(A, ((const T*)A.beta.p)[row_at(A, A.beta, s, sp, t) + head * A.beta.hs]);
+            }
+            struct alignas(sizeof(T) * V) E {
+                T v[V];
+            } vt;
+            const T* vp = (const T*)A.v.p + row_at(A, A.v, s, sp, t) + head * A.v.hs + col;
+            if (on && A.v.word >= (int)sizeof(E)) {
+                vt = *reinterpret_cast<const E*>(vp);
+            } else {
 #pragma unroll
-            for (int j = 0; j < V; ++j)
-                v[j] = on ? to_f32(((const T*)A.v.p)[row_at(A, A.v, s, sp, t) + head * A.v.hs + col + j]) : 0.0f;
-            const float l = log_decay(A, ((const T*)A.gate.p)[row_at(A, A.gate, s, sp, t) + head * A.gate.hs]);
-            const float rate = rate_of(A, ((const T*)A.beta.p)[row_at(A, A.beta, s, sp, t) + head * A.beta.hs]);
-            const float lost = -expm1f(l), kept = expf(l);  // 1 - a keeps its bits where a is near 1
-            const bool little = lost < 0.5f;
+                for (int j = 0; j < V; ++j) vt.v[j] = on ? vp[j] : from_f32<T>(0.0f);
+            }
             __syncthreads();
+            const float lost = factor[0], kept = factor[1], rate = factor[2];
+            const bool little = lost < 0.5f;
             float k[R], dk[V] = {}, dq[V] = {}, kq = 0.0f;
 #pragma unroll
             for (int i = 0; i < R; ++i) {
@@ -104,13 +115,22 @@ __global__ void __launch_bounds__(32 * STEP_WARPS, 2) k_delta_steps(const __grid
 #pragma unroll
                     for (int j = 0; j < V; ++j) sq[j] += f.v[j];
                 }
+            E yt;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float u = rate * (v[j] - sk[j]);
+                const float u = rate * (to_f32(vt.v[j]) - sk[j]);
 #pragma unroll
                 for (int i = 0; i < R; ++i) S[i].v[j] = fmaf(k[i], u, S[i].v[j]);
-                if (warp == 0 && on)
-                    ((T*)A.y.p)[row_at(A, A.y, s, sp, t) + head * A.y.hs + col + j] = from_f32<T>(A.scale * fmaf(kq, u, sq[j]));
+                yt.v[j] = from_f32<T>(A.scale * fmaf(kq, u, sq[j]));
+            }
+            if (warp == 0 && on) {
+                T* yp = (T*)A.y.p + row_at(A, A.y, s, sp, t) + head * A.y.hs + col;
+                if (A.y.word >= (int)sizeof(E)) {
+                    *reinterpret_cast<E*>(yp) = yt;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) yp[j] = yt.v[j];
+                }
             }
         }
         if (A.h && on)

@@ -17,63 +17,48 @@ constexpr int prep_smem() {
 // Scale of a chunk's keys or queries.  At most 2^40, and that where all are zero: what
 // they are multiplied with shares the scale of the product and must not lose bits to nothing.
 __device__ __forceinline__ float key_scale(float top) { return top == 0.0f ? 0x1p40f : fminf(scale_for(top), 0x1p40f); }
-// rows of keys or queries into registers, words of V elements; their largest magnitude
-template <typename T, int KD, int N>
-__device__ __forceinline__ float read_keys(uint4 (&w)[N], const T* from, long long st, int n, const DeltaArgs& A, int word) {
+// The largest magnitude of this thread's words of a [C, KD] tile (stride KD + PAD), and the tile
+// times s as KE in its place and, unless null, in memory
+template <typename T, int KD>
+__device__ __forceinline__ float top_of_tile(const T* m) {
     constexpr int V = 16 / (int)sizeof(T), L = KD / V;
-    float top = 0.0f;
+    unsigned top = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int k = threadIdx.x + i * PREP, r = k / L, c = (k - r * L) * V;
-        w[i] = make_uint4(0, 0, 0, 0);
-        if (r >= n || c >= A.kdim) continue;
-        const T* p = from + r * st + c;
-        if (word == 16) {
-            w[i] = *reinterpret_cast<const uint4*>(p);
-        } else {
-            T e[V];
-#pragma unroll
-            for (int j = 0; j < V; ++j) e[j] = c + j < A.kdim ? p[j] : from_f32<T>(0.0f);
-            memcpy(&w[i], e, 16);
-        }
+    for (int i = threadIdx.x; i < C * L; i += PREP) {
+        const uint4 w = *reinterpret_cast<const uint4*>(m + i / L * (KD + PAD) + i % L * V);
+        // (magnitudes of 16 bits order as their bits)
+        top = __vmaxu2(__vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)), top);
     }
-    if constexpr (sizeof(T) == 2)
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 f = of_pair<T>((&w[i].x)[j]);
-                top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-            }
-    return top;
+    const float2 f = of_pair<T>(top);
+    return fmaxf(f.x, f.y);
 }
-// the same times s as KE, rows of stride KD + PAD, to shared memory and, unless null, to memory
-template <typename T, typename KE, int KD, int N>
-__device__ __forceinline__ void write_keys(const uint4 (&w)[N], KE* sm, KE* copy, float s) {
+template <typename T, typename KE, int KD>
+__device__ __forceinline__ void scale_tile(KE* m, KE* copy, float s) {
     constexpr int V = 16 / (int)sizeof(T), L = KD / V;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int k = threadIdx.x + i * PREP, r = k / L, c = (k - r * L) * V;
-        uint4 o = w[i];
-        if constexpr (sizeof(T) == 2)
+#pragma unroll 4
+    for (int i = threadIdx.x; i < C * L; i += PREP) {
+        const int at = i / L * (KD + PAD) + i % L * V;
+        uint4 w = *reinterpret_cast<const uint4*>(m + at);
+        if constexpr (sizeof(T) == 2) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float2 f = of_pair<T>((&w[i].x)[j]);
-                (&o.x)[j] = pair_of<KE>(f.x * s, f.y * s);
+                const float2 f = of_pair<T>((&w.x)[j]);
+                (&w.x)[j] = pair_of<KE>(f.x * s, f.y * s);
             }
-        *reinterpret_cast<uint4*>(sm + r * (KD + PAD) + c) = o;
-        if (copy) *reinterpret_cast<uint4*>(copy + r * (KD + PAD) + c) = o;
+            *reinterpret_cast<uint4*>(m + at) = w;
+        }
+        if (copy) *reinterpret_cast<uint4*>(copy + at) = w;
     }
 }
 template <class P, int KD>
-__global__ void __launch_bounds__(PREP, 4) k_delta_prep(const __grid_constant__ DeltaArgs A) {
+__global__ void __launch_bounds__(PREP, 5) k_delta_prep(const __grid_constant__ DeltaArgs A) {
     using T = typename P::T;
     using KE = typename P::KE;
-    constexpr int KS = KD + PAD, WORDS = C * KD * (int)sizeof(T) / 16 / PREP;
+    constexpr int KS = KD + PAD;
     extern __shared__ __align__(16) char smem[];
     KE *K = reinterpret_cast<KE*>(smem), *Q = K + C * KS;
     float* M = reinterpret_cast<float*>(smem);  // [C][MS]
-    __shared__ float up[C], low[C], rate[C], top[2][4];
+    __shared__ __align__(16) float up[C], low[C], rate[C], top[2][4];
     __shared__ int cut[C];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, head = blockIdx.y, kh = head / A.group;
     const int g = lane >> 2, t4 = lane & 3;
@@ -83,25 +68,28 @@ __global__ void __launch_bounds__(PREP, 4) k_delta_prep(const __grid_constant__ 
     if (first < 0 || first >= sp.len) return;
     const int t0 = (int)first, n = min(C, sp.len - t0);
     float ks = 1.0f, qs = 1.0f;
-    {
-        uint4 wk[WORDS], wq[WORDS];
-        float a = read_keys<T, KD>(wk, (const T*)A.k.p + row_at(A, A.k, s, sp, t0) + kh * A.k.hs, A.k.st, n, A, A.k.word);
-        float b = read_keys<T, KD>(wq, (const T*)A.q.p + row_at(A, A.q, s, sp, t0) + kh * A.q.hs, A.q.st, n, A, A.q.word);
-        if (warp == 0) chunk_decays<T>(A, s, sp, t0, n, head, lane, up, low, cut, rate);
-        if constexpr (P::SCALED) {
-            a = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(a)));
-            b = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(b)));
-            if (lane == 0) {
-                top[0][warp] = a;
-                top[1][warp] = b;
-            }
-            __syncthreads();
-            ks = key_scale(fmaxf(fmaxf(top[0][0], top[0][1]), fmaxf(top[0][2], top[0][3])));
-            qs = key_scale(fmaxf(fmaxf(top[1][0], top[1][1]), fmaxf(top[1][2], top[1][3])));
+    float lost = 0.0f;
+    load_rows<T, C, KD>(reinterpret_cast<T*>(K), (const T*)A.k.p + row_at(A, A.k, s, sp, t0) + kh * A.k.hs, A.k.st, n, A.kdim, A.k.word, tid, PREP);
+    load_rows<T, C, KD>(reinterpret_cast<T*>(Q), (const T*)A.q.p + row_at(A, A.q, s, sp, t0) + kh * A.q.hs, A.q.st, n, A.kdim, A.q.word, tid, PREP);
+    copies_end();
+    if (warp == 0) chunk_decays<T>(A, s, sp, t0, n, head, lane, up, low, cut, rate, lost);
+    copies_wait<0>();
+    __syncthreads();
+    if constexpr (P::SCALED) {
+        const float a = top_of_tile<T, KD>(reinterpret_cast<T*>(K)), b = top_of_tile<T, KD>(reinterpret_cast<T*>(Q));
+        const unsigned ka = __reduce_max_sync(~0u, __float_as_uint(a)), qa = __reduce_max_sync(~0u, __float_as_uint(b));
+        if (lane == 0) {
+            top[0][warp] = __uint_as_float(ka);
+            top[1][warp] = __uint_as_float(qa);
         }
-        KE* copy = head % A.group == 0 ? (KE*)A.keys + (slot * A.hk + kh) * 2 * C * KS : nullptr;
-        write_keys<T, KE, KD>(wk, K, copy, ks);
-        write_keys<T, KE, KD>(wq, Q, copy ? copy + C * KS : nullptr, qs);
+        __syncthreads();
+        ks = key_scale(fmaxf(fmaxf(top[0][0], top[0][1]), fmaxf(top[0][2], top[0][3])));
+        qs = key_scale(fmaxf(fmaxf(top[1][0], top[1][1]), fmaxf(top[1][2], top[1][3])));
+    }
+    KE* copy = head % A.group == 0 ? (KE*)A.keys + (slot * A.hk + kh) * 2 * C * KS : nullptr;
+    if (P::SCALED || copy) {
+        scale_tile<T, KE, KD>(K, copy, ks);
+        scale_tile<T, KE, KD>(Q, copy ? copy + C * KS : nullptr, qs);
     }
     __syncthreads();
     const long long unit = slot * A.heads + head;
@@ -109,14 +97,14 @@ __global__ void __launch_bounds__(PREP, 4) k_delta_prep(const __grid_constant__ 
     KE *Tm = reinterpret_cast<KE*>(A.squares + unit * P::SQUARES) + low_at(warp), *Pm = Tm + P::PIECES * LOW;
     const int st = low_stride(warp);
     if (tid < C) {
-        F[tid] = cut[tid] ? 0.0f : expf(up[tid]) * (1.0f + low[tid]);
+        F[tid] = cut[tid] ? 0.0f : power_of_2(up[tid] + low[tid]);
         F[C + tid] = decay_between(up, low, cut, C - 1, tid);
         F[2 * C + tid] = rate[tid];
         F[UP + tid] = up[tid];
         F[UP_LOW + tid] = low[tid];
         reinterpret_cast<int*>(F + CUT)[tid] = cut[tid];
-        if (tid == 0) {
-            F[LOST] = cut[C - 1] ? 1.0f : fmaf(-low[C - 1], expf(up[C - 1]), -expm1f(up[C - 1]));
+        if (tid == 31) {  // (the last lane of the warp that summed)
+            F[LOST] = lost;
             F[K_SCALE] = ks;
             F[Q_SCALE] = qs;
         }
@@ -135,15 +123,29 @@ __global__ void __launch_bounds__(PREP, 4) k_delta_prep(const __grid_constant__ 
         }
     }
     float most = 0.0f;
+    const bool cuts = cut[C - 1] != 0;
+    const float iqk = P::SCALED ? ik * iq : 1.0f;
+    float upi[2], lowi[2], ri[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int i = warp * 16 + g + 8 * h;
+        upi[h] = up[i];
+        lowi[h] = low[i];
+        ri[h] = rate[i];
+    }
 #pragma unroll
     for (int nt = 0; nt < 8; ++nt) {
         if (nt / 2 > warp) break;
+        const float2 upj = *reinterpret_cast<const float2*>(up + nt * 8 + 2 * t4), lowj = *reinterpret_cast<const float2*>(low + nt * 8 + 2 * t4);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int i = warp * 16 + g + (e >> 1) * 8, j = nt * 8 + 2 * t4 + (e & 1);
-            const float G = j <= i ? decay_between(up, low, cut, i, j) : 0.0f, a = rate[i] * G;
-            p2[nt][e] = G != 0.0f ? G * (p2[nt][e] * ik * iq) : 0.0f;
-            x2[nt][e] = j < i && a != 0.0f ? a * (x2[nt][e] * ik * ik) : 0.0f;
+            const int h = e >> 1, i = warp * 16 + g + h * 8, j = nt * 8 + 2 * t4 + (e & 1);
+            float G = power_of_2((upi[h] - (e & 1 ? upj.y : upj.x)) + (lowi[h] - (e & 1 ? lowj.y : lowj.x)));
+            if (nt / 2 == warp && j > i) G = 0.0f;
+            if (cuts && cut[i] != cut[j]) G = 0.0f;
+            const float a = ri[h] * G;
+            p2[nt][e] = G != 0.0f ? G * (p2[nt][e] * iqk) : 0.0f;
+            x2[nt][e] = a != 0.0f && (nt / 2 < warp || j < i) ? a * (x2[nt][e] * ik * ik) : 0.0f;
             most = fmaxf(most, fabsf(p2[nt][e]));
         }
     }

@@ -385,12 +385,12 @@ __device__ __forceinline__ float warp_top(const float (&x)[N][4]) {
 template <int N>
 __device__ __forceinline__ float warp_scale(const float (&x)[N][4]) { return scale_for(warp_top(x)); }
 
-// By one warp: sums of the logarithms of a chunk's decays (64 bits, kept as two f32:
-// differences of them are what counts) but for those of decays of 0, which are counted
-// apart, and the rates
+// By one warp: sums of the logarithms of a chunk's decays (64 bits, kept as two f32 of
+// their binary logarithms: differences of them are what counts) but for those of decays of
+// 0, which are counted apart, and the rates.  In the last lane's `lost` 1 - the chunk's decay.
 template <typename T>
 __device__ __forceinline__ void chunk_decays(const DeltaArgs& A, long long s, const Span& sp, int t0, int n, int head, int lane,
-                                             float* up, float* low, int* cut, float* rate) {
+                                             float* up, float* low, int* cut, float* rate, float& lost) {
     double l[2];
     int z[2];
 #pragma unroll
@@ -416,16 +416,24 @@ __device__ __forceinline__ void chunk_decays(const DeltaArgs& A, long long s, co
             cuts += c;
         }
     }
-    const double v[2] = {sum - l[1], sum};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        up[2 * lane + i] = (float)v[i];
-        low[2 * lane + i] = (float)(v[i] - (double)(float)v[i]);
+        const double v = (i ? sum : sum - l[1]) * 1.4426950408889634074;
+        up[2 * lane + i] = (float)v;
+        low[2 * lane + i] = (float)(v - (double)(float)v);
         cut[2 * lane + i] = cuts - (i ? 0 : z[1]);
     }
+    const float whole = (float)sum, rest = (float)(sum - (double)whole);
+    lost = cuts ? 1.0f : fmaf(-rest, expf(whole), -expm1f(whole));
+}
+// 2^x by the exponential unit: off by 2^-22 of the value, as expf
+__device__ __forceinline__ float power_of_2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 __device__ __forceinline__ float decay_between(const float* up, const float* low, const int* cut, int i, int j) {
-    return cut[i] == cut[j] ? expf((up[i] - up[j]) + (low[i] - low[j])) : 0.0f;
+    return cut[i] == cut[j] ? power_of_2((up[i] - up[j]) + (low[i] - low[j])) : 0.0f;
 }
 // the sequence that chunk `slot` belongs to, the last that does not begin behind it
 __device__ __forceinline__ long long sequence_of(const DeltaArgs& A, long long slot) {

@@ -576,48 +576,66 @@ def _heads(t, name, shape, dtype):
 
 def _new_heads(dev, stream, shape, dtype):
     """(a new tensor of heads, its snn_heads)"""
-    t, n = _new(dev, stream, tuple(shape), dtype), shape[-2] * shape[-1]
-    return t, _HEADS.pack(t.data_ptr(), shape[-3] * n, n, shape[-1])
+    d = shape[-1]
+    n = shape[-2] * d
+    if stream is not None:
+        t = _new(dev, stream, tuple(shape), dtype)
+    elif len(shape) == 4:  # (as in _new)
+        t = _T.empty_strided(shape, (shape[1] * n, n, d, 1), dtype=dtype, device=dev)
+    else:
+        t = _T.empty_strided(shape, (n, d, 1), dtype=dtype, device=dev)
+    return t, _HEADS.pack(t.data_ptr(), shape[-3] * n, n, d)
 
 
 def _qk_args(q, k, wq, wk, positions, freqs, eps, unit, adjacent):
-    """(device, snn_qk, [rows of q, of k], [address of the weights, ..], address of positions, of freqs)"""
+    """(device, snn_qk, (rows of q, of k), (addresses of the weights), address of positions, of freqs)"""
     if _T is None:
         _torch()
     some = q if q is not None else k
     _require(some is not None, "neither q nor k is given")
-    dev, shape = some.device, some.shape
+    dev, shape, dtype = some.device, some.shape, some.dtype
     if dev.type != "cuda":
         raise SnnError(1, "q and k must be CUDA tensors")
-    _require(len(shape) in (3, 4) and shape[-1] >= 1,
-             "q and k must be [rows, heads, dim] or [sequences, steps, heads, dim]")
-    dim, lead, kind = shape[-1], shape[:-2], _elem(some.dtype)
-    n_seq, n_steps = lead if len(lead) == 2 else (1, lead[0])
-    rows, weights, heads = [None, None], [None, None], [0, 0]
-    for i, (x, w, name) in enumerate(((q, wq, "q"), (k, wk, "k"))):
-        if x is None:
-            continue
-        _cuda(x, name, dev)
-        heads[i] = x.shape[-2] if x.dim() == len(shape) else 0
-        rows[i] = _heads(x, name, (*lead, heads[i], dim), some.dtype)
-        if w is not None:
-            _cuda(w, name + "_weight", dev)
-            _require(w.shape == (dim,) and w.dtype == _T.float32 and w.is_contiguous(),
-                     f"{name}_weight must be contiguous float32 [dim]")
-            weights[i] = w.data_ptr()
-    rot, pos_type, pp, fp = 0, 9, None, None
-    _require((positions is None) == (freqs is None), "positions and freqs are given together")
+    if len(shape) not in (3, 4) or shape[-1] < 1:
+        raise SnnError(1, "q and k must be [rows, heads, dim] or [sequences, steps, heads, dim]")
+    dim, lead = shape[-1], shape[:-2]
+    hq = hk = 0
+    rq = rk = pq = pk = pp = fp = None
+    if q is not None:
+        hq = shape[-2]
+        rq, pq = _heads(q, "q", shape, dtype), _qk_weight(wq, "q_weight", dim, dev)
+    if k is not None:
+        if k.device != dev:
+            _cuda(k, "k", dev)
+        hk = k.shape[-2] if k.dim() == len(shape) else 0
+        rk, pk = _heads(k, "k", (*lead, hk, dim), dtype), _qk_weight(wk, "k_weight", dim, dev)
+    rot, pos_type = 0, 9
+    if (positions is None) != (freqs is None):
+        raise SnnError(1, "positions and freqs are given together")
     if freqs is not None:
-        _cuda(freqs, "freqs", dev)
-        _cuda(positions, "positions", dev)
-        _require(freqs.dim() == 1 and freqs.dtype == _T.float32 and freqs.is_contiguous() and 2 * freqs.numel() <= dim,
-                 "freqs must be contiguous float32 of at most dim / 2 elements")
-        _require(positions.shape == lead and positions.dtype in (_T.int32, _T.int64) and positions.is_contiguous(),
-                 "positions must be contiguous int32 or int64, one for each row")
-        rot, pos_type, pp, fp = 2 * freqs.numel(), _TOKEN[positions.dtype], positions.data_ptr(), freqs.data_ptr()
-    desc = _QK.pack(kind, (QK_UNIT if unit else 0) | (QK_ADJACENT if adjacent else 0), n_seq, n_steps, *heads, dim, rot,
+        if freqs.device != dev or positions.device != dev:
+            _cuda(freqs, "freqs", dev)
+            _cuda(positions, "positions", dev)
+        rot, pos_type = 2 * freqs.numel(), _TOKEN.get(positions.dtype)
+        if freqs.dim() != 1 or freqs.dtype != _T.float32 or not freqs.is_contiguous() or rot > dim:
+            raise SnnError(1, "freqs must be contiguous float32 of at most dim / 2 elements")
+        if positions.shape != lead or pos_type not in (9, 10) or not positions.is_contiguous():
+            raise SnnError(1, "positions must be contiguous int32 or int64, one for each row")
+        pp, fp = positions.data_ptr(), freqs.data_ptr()
+    n_seq, n_steps = lead if len(lead) == 2 else (1, lead[0])
+    desc = _QK.pack(_elem(dtype), (QK_UNIT if unit else 0) | (QK_ADJACENT if adjacent else 0), n_seq, n_steps, hq, hk, dim, rot,
                     pos_type, eps)
-    return dev, desc, rows, weights, pp, fp
+    return dev, desc, (rq, rk), (pq, pk), pp, fp
+
+
+def _qk_weight(w, name, dim, dev):
+    """Address of a side's weights, or None."""
+    if w is None:
+        return None
+    _cuda(w, name, dev)
+    if w.shape != (dim,) or w.dtype != _T.float32 or not w.is_contiguous():
+        raise SnnError(1, f"{name} must be contiguous float32 [dim]")
+    return w.data_ptr()
 
 
 def _qk_results(dev, stream, q, k, out):
@@ -763,7 +781,7 @@ def delta_scan(q, k, v, gate, beta, h0=None, scale=1.0, logit=False, offsets=Non
         _cuda(out, "out", dev)
         yr = _heads(out, "out", v.shape, v.dtype)
     if h_out is None:
-        h_out = _new(dev, stream, state, _T.float32)
+        h_out = _new_heads(dev, stream, state, _T.float32)[0]
         hp = h_out.data_ptr()
     else:
         hp = _state(h_out, "h_out", state, dev)
