@@ -214,7 +214,7 @@ Layout layout_of(const snn_delta* d) {
     l.keys = round256(units * z.squares);
     l.factors = l.keys + round256(slots_of(d) * d->k_heads * 2 * C * (kd + PAD) * z.key);
     l.all = l.states = l.factors + round256(units * SC * 4);
-    l.u = l.states + round256(units * d->v_dim * kd * z.kept);
+    l.u = l.states + round256(units * d->v_dim * (kd + PAD) * z.kept);
     l.kept_all = l.u + round256(units * C * vpad_of(d) * z.kept);
     return l;
 }

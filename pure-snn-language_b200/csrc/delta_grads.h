@@ -158,8 +158,8 @@ __global__ void __launch_bounds__(GRADS, 1) k_delta_grads(const __grid_constant_
             load_tile<E, C, GW>(m + G::ROWS, (const E*)A.u + unit * C * A.vpad + c0, A.vpad, C, A.vpad - c0, 16);
             load_tile<E, C, GW>(m + 2 * G::ROWS, (const E*)A.dr + unit * C * A.vpad + c0, A.vpad, C, A.vpad - c0, 16);
             load_tile<E, C, GW>(m + 3 * G::ROWS, (const T*)A.v.p + row_at(A, A.v, s, sp, t0) + head * A.v.hs + c0, A.v.st, n, w, A.v.word);
-            load_tile<E, GW, KD>(m + 4 * G::ROWS, (const E*)A.states + (unit * A.vdim + c0) * KD, KD, w, KD, 16);
-            load_tile<E, GW, KD>(m + 4 * G::ROWS + G::STATE, (const E*)A.dstates + (unit * A.vdim + c0) * KD, KD, w, KD, 16);
+            load_tile<E, GW, KD>(m + 4 * G::ROWS, (const E*)A.states + (unit * A.vdim + c0) * KS, KS, w, KD, 16);
+            load_tile<E, GW, KD>(m + 4 * G::ROWS + G::STATE, (const E*)A.dstates + (unit * A.vdim + c0) * KS, KS, w, KD, 16);
         };
         if (gi == 0) load_words(Ks, keys, 2 * G::KEYS * (int)sizeof(KE), tid, GRADS);
         load_words(F, A.factors + unit * SC, SC * 4, tid, GRADS);

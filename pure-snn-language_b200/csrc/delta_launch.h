@@ -36,10 +36,10 @@ void launch_scan_of(const DeltaArgs& A, int warps, cudaStream_t st) {
             constexpr int KD = decltype(kd)::value, NW = decltype(nw)::value;
             using S = Stage<P, KD, NW, P::OUT>;
             auto* kernel = k_delta_scan<P, KD, NW>;
-            set_smem(kernel, S::STAGES * S::BYTES);
+            set_smem(kernel, S::SMEM);
             const dim3 grid((unsigned)std::min<long long>(A.n_seq, 1 << 30), (unsigned)A.heads,
                             (unsigned)((A.vdim + S::VW - 1) / S::VW));
-            kernel<<<grid, NW * 32, S::STAGES * S::BYTES, st>>>(A);
+            kernel<<<grid, NW * 32, S::SMEM, st>>>(A);
         });
     });
     SNN_CUDA(cudaGetLastError());
@@ -53,10 +53,10 @@ void launch_grads_of(const DeltaArgs& A, int warps, cudaStream_t st) {
             constexpr int NW = decltype(nw)::value;
             using S = Stage<P, KD, NW, P::PIECES>;
             auto* kernel = k_delta_back<P, KD, NW>;
-            set_smem(kernel, S::STAGES * S::BYTES);
+            set_smem(kernel, S::SMEM);
             const dim3 grid((unsigned)std::min<long long>(A.n_seq, 1 << 30), (unsigned)A.heads,
                             (unsigned)((A.vdim + S::VW - 1) / S::VW));
-            kernel<<<grid, NW * 32, S::STAGES * S::BYTES, st>>>(A);
+            kernel<<<grid, NW * 32, S::SMEM, st>>>(A);
             SNN_CUDA(cudaGetLastError());
         });
         if (!A.slots) return;

@@ -51,7 +51,7 @@ __device__ __forceinline__ void scale_tile(KE* m, KE* copy, float s) {
     }
 }
 template <class P, int KD>
-__global__ void __launch_bounds__(PREP, 5) k_delta_prep(const __grid_constant__ DeltaArgs A) {
+__global__ void __launch_bounds__(PREP, 4) k_delta_prep(const __grid_constant__ DeltaArgs A) {
     using T = typename P::T;
     using KE = typename P::KE;
     constexpr int KS = KD + PAD;

@@ -15,7 +15,11 @@ struct Stage {
     static constexpr int KEYS = C * (KD + PAD) * (int)sizeof(KE), VALUES = C * (VW + PAD) * (int)sizeof(T);
     static constexpr int SQUARES = (P::PIECES + PP) * LOW * (int)sizeof(KE);
     static constexpr int BYTES = 2 * KEYS + VALUES + SQUARES + SCAN_FACTORS * 4;
-    static constexpr int STAGES = 2 * BYTES <= 227 * 1024 - 1024 ? 2 : 1;
+    using K = typename Kept<T>::K;
+    static constexpr int KEEP = sizeof(K) == 2 ? 16 * (KD + PAD) * 2 : 0;  // a warp's stage of its state
+    static constexpr int STAGES = 2 * BYTES + NW * KEEP <= 227 * 1024 - 1024 ? 2 : 1;
+    static constexpr int SMEM = STAGES * BYTES + NW * KEEP;
+    static __device__ __forceinline__ K* keep(char* m, int warp) { return reinterpret_cast<K*>(m + STAGES * BYTES + warp * KEEP); }
     KE *k, *q, *t, *p;
     T* v;
     float* f;
@@ -117,20 +121,32 @@ __device__ __forceinline__ void keep_tile(const float (&o)[8][4], T* stage, K* t
             }
     }
 }
-// S^T [16 columns, KD] of a warp, divided by its scale, as w rows of KD elements
+// S^T [16 columns, KD] of a warp, divided by its scale, as w rows of KD elements (stride KD +
+// PAD).  bf16: through the warp's `stage` [16][KD + PAD], from where it is copied while the
+// warp goes on (stores from registers, of 16 bytes to a row, took 2 us of 9.5 a chunk).
 template <typename K, int NT>
-__device__ __forceinline__ void keep_state(const float (&S)[NT][4], float back, K* to, int w) {
+__device__ __forceinline__ void keep_state(const float (&S)[NT][4], float back, K* stage, K* to, int w) {
+    constexpr int KS = NT * 8 + PAD;
     const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+    if constexpr (sizeof(K) == 2) {
+        if (lane == 0) store_read();  // what was kept before has left the stage
+        __syncwarp();
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-        if (g + 8 * h < w)
+        for (int i = 0; i < NT; i += 2)
+            stsm4(stage + ((lane & 7) + ((lane >> 3) & 1) * 8) * KS + (i + (lane >> 4)) * 8, pair_of<K>(S[i][0] * back, S[i][1] * back),
+                  pair_of<K>(S[i][2] * back, S[i][3] * back), pair_of<K>(S[i + 1][0] * back, S[i + 1][1] * back),
+                  pair_of<K>(S[i + 1][2] * back, S[i + 1][3] * back));
+        store_fence();
+        __syncwarp();
+        if (lane == 0) store_bulk(to, stage, min(w, 16) * KS * 2);
+    } else {
 #pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                K* p = to + (g + 8 * h) * NT * 8 + i * 8 + 2 * t4;
-                const float x = S[i][2 * h] * back, y = S[i][2 * h + 1] * back;
-                if constexpr (sizeof(K) == 4) *reinterpret_cast<float2*>(p) = make_float2(x, y);
-                else *reinterpret_cast<unsigned*>(p) = pair_of<K>(x, y);
-            }
+        for (int h = 0; h < 2; ++h)
+            if (g + 8 * h < w)
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+                    *reinterpret_cast<float2*>(to + (g + 8 * h) * KS + i * 8 + 2 * t4) = make_float2(S[i][2 * h] * back, S[i][2 * h + 1] * back);
+    }
 }
 // f32 states [kdim, vdim] from and to a warp's columns
 template <int NT>
@@ -308,7 +324,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_scan(const __grid_constant
                     ik = inverse_of(st.f[K_SCALE]);
                     iq = inverse_of(st.f[Q_SCALE]);
                 }
-                if (A.states) keep_state<K, NT>(S, back, (K*)A.states + (unit * A.vdim + col) * KD, w);
+                if (A.states) keep_state<K, NT>(S, back, St::keep(smem, warp), (K*)A.states + (unit * A.vdim + col) * (KD + PAD), w);
                 float r[8][4] = {}, o[8][4] = {}, u[8][4];
 #pragma unroll
                 for (int d = 0; d < KD / 16; ++d) {
@@ -375,6 +391,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_scan(const __grid_constant
         copies_wait<0>();
         __syncthreads();
     }
+    store_done();
     if (A.zero) zero_rest<T>(A, A.y, A.heads, A.vdim, ((long long)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x,
                              (long long)gridDim.x * gridDim.y * gridDim.z);
 }
@@ -418,7 +435,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_back(const __grid_constant
                     ik = inverse_of(st.f[K_SCALE]);
                     iq = inverse_of(st.f[Q_SCALE]);
                 }
-                keep_state<K, NT>(D, back, (K*)A.dstates + (unit * A.vdim + col) * KD, w);
+                keep_state<K, NT>(D, back, St::keep(smem, warp), (K*)A.dstates + (unit * A.vdim + col) * (KD + PAD), w);
                 float u[8][4] = {}, r[8][4] = {}, z[8][4];
 #pragma unroll
                 for (int d = 0; d < KD / 16; ++d) {
@@ -478,5 +495,6 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_back(const __grid_constant
         copies_wait<0>();
         __syncthreads();
     }
+    store_done();
 }
 }  // namespace snnb_delta

@@ -63,7 +63,7 @@ struct DeltaArgs {
     char* keys;               // [slots, hk, 2, C, KD + PAD] of Path::KE: K and Q times their scales
     char* squares;            // [slots, heads] of Path::SQUARES bytes: planes of T, of P
     float* factors;           // [slots, heads, SC]
-    char *states, *u;         // saved: [slots, heads, vdim, KD], [slots, heads, C, vpad] of Kept
+    char *states, *u;         // saved: [slots, heads, vdim, KD + PAD], [slots, heads, C, vpad] of Kept
     char *dstates, *dr;       // gradients' workspace: the same forms
 };
 
@@ -147,6 +147,20 @@ __device__ __forceinline__ void ldsm4t(unsigned (&r)[4], const void* p) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
+__device__ __forceinline__ void stsm4(void* p, unsigned a, unsigned b, unsigned c, unsigned d) {
+    const unsigned at = (unsigned)__cvta_generic_to_shared(p);
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// bytes (a multiple of 16, as the addresses) of shared memory to memory, by one thread, behind a fence of
+// those that wrote them; the shared memory is read when store_read returns, all is done when store_done does
+__device__ __forceinline__ void store_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void store_bulk(void* to, const void* from, int bytes) {
+    const unsigned at = (unsigned)__cvta_generic_to_shared(from);
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(at), "r"(bytes) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void store_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void stsm4t(void* p, unsigned a, unsigned b, unsigned c, unsigned d) {
     const unsigned at = (unsigned)__cvta_generic_to_shared(p);
     asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
