@@ -88,6 +88,10 @@ __device__ __forceinline__ void load_tile(E* to, const F* from, long long st, in
             copy16(to + a * (W + PAD), there ? p + a * st : from, there);
         }
     } else {
+        if constexpr (std::is_same<E, F>::value) {
+            if (word == 8) return load_by<E, R, W, 8>(to, from, st, r, w, threadIdx.x, GRADS);
+            if (word == 4) return load_by<E, R, W, 4>(to, from, st, r, w, threadIdx.x, GRADS);
+        }
         for (int i = threadIdx.x; i < R * W; i += GRADS) {
             const int a = i / W, c = i - a * W;
             to[a * (W + PAD) + c] = from_f32<E>(a < r && c < w ? to_f32(from[a * st + c]) : 0.0f);

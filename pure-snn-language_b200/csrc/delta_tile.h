@@ -324,15 +324,26 @@ struct Path32 {
                 for (int i = 0; i < 2; ++i)
                     tf32_split(m[(k * 8 + 2 * t + i) * st + n * 8 + g], b[n].h[2 * k + i], b[n].l[2 * k + i]);
     }
+    // (The instruction cuts the bits that its sum has no room for, always towards zero, which adds
+    // up over a long sum: it sums a depth of 16, and rounded additions those sums.)
     static __device__ __forceinline__ void full(float (&d0)[4], float (&d1)[4], const A& a, const B (&b)[2]) {
+        float t0[4] = {}, t1[4] = {};
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            mma8(d0, a.l + 4 * k, b[0].h + 2 * k);
-            mma8(d1, a.l + 4 * k, b[1].h + 2 * k);
-            mma8(d0, a.h + 4 * k, b[0].l + 2 * k);
-            mma8(d1, a.h + 4 * k, b[1].l + 2 * k);
-            mma8(d0, a.h + 4 * k, b[0].h + 2 * k);
-            mma8(d1, a.h + 4 * k, b[1].h + 2 * k);
+            mma8(t0, a.l + 4 * k, b[0].h + 2 * k);
+            mma8(t1, a.l + 4 * k, b[1].h + 2 * k);
+            mma8(t0, a.h + 4 * k, b[0].l + 2 * k);
+            mma8(t1, a.h + 4 * k, b[1].l + 2 * k);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            mma8(t0, a.h + 4 * k, b[0].h + 2 * k);
+            mma8(t1, a.h + 4 * k, b[1].h + 2 * k);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            d0[e] += t0[e];
+            d1[e] += t1[e];
         }
     }
     template <int p>
