@@ -588,10 +588,10 @@ typedef struct snn_delta {
 
 /* saved (nullable): saved_bytes bytes, 256-byte aligned, of the size that
  * snn_delta_scan_saved says; it receives what snn_delta_scan_grad needs.  work: as
- * for snn_embed_grad, of the size that snn_delta_scan_workspace says; not needed
- * with saved. */
+ * for snn_embed_grad, of the size that snn_delta_scan_workspace says for a call with or without
+ * saved (it may be 0). */
 int snn_delta_scan_saved(const snn_delta* desc, int64_t* bytes);
-int snn_delta_scan_workspace(const snn_delta* desc, int64_t* bytes);
+int snn_delta_scan_workspace(const snn_delta* desc, int32_t with_saved, int64_t* bytes);
 int snn_delta_scan(const snn_delta* desc, const snn_heads* q, const snn_heads* k,
                    const snn_heads* v, const snn_rows* gate, const snn_rows* beta, const float* h0,
                    const snn_heads* y, float* h, void* saved, int64_t saved_bytes, void* work,

@@ -488,10 +488,10 @@ int snn_delta_scan_saved(const snn_delta* desc, int64_t* bytes) {
     });
 }
 
-int snn_delta_scan_workspace(const snn_delta* desc, int64_t* bytes) {
+int snn_delta_scan_workspace(const snn_delta* desc, int32_t with_saved, int64_t* bytes) {
     return guard_op([&] {
         SNN_REQUIRE(bytes, SNN_ERR_ARG, "null result");
-        *bytes = snnb::delta_scan_workspace(desc);
+        *bytes = snnb::delta_scan_workspace(desc, with_saved != 0);
     });
 }
 

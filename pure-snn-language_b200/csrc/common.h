@@ -136,7 +136,7 @@ void qk_norm_grad(const snn_qk* desc, const snn_heads* q, const snn_heads* k, co
                   const snn_heads* dq, const snn_heads* dk, float* dwq, float* dwk, void* work, int64_t work_bytes,
                   cudaStream_t st);
 int64_t delta_scan_saved(const snn_delta* desc);
-int64_t delta_scan_workspace(const snn_delta* desc);
+int64_t delta_scan_workspace(const snn_delta* desc, bool with_saved);
 void delta_scan(const snn_delta* desc, const snn_heads* q, const snn_heads* k, const snn_heads* v, const snn_rows* gate,
                 const snn_rows* beta, const float* h0, const snn_heads* y, float* h, void* saved, int64_t saved_bytes,
                 void* work, int64_t work_bytes, cudaStream_t st);

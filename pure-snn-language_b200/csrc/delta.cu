@@ -142,6 +142,78 @@ __global__ void __launch_bounds__(32 * STEP_WARPS, 2) k_delta_steps(const __grid
                              (long long)gridDim.x * gridDim.y * gridDim.z);
 }
 
+// Where the segments start from: starts[g + 1], which holds what segment g makes of nothing, gains its
+// steps' product times starts[g], one segment after the other.  A CTA takes 16 columns of a
+// head, in shared memory from one segment to the next; the next product is on its way
+// meanwhile.  A thread has 8 columns of a row.  (6 products of 16 heads of 128 x 128: 40 us.)
+constexpr int JOIN_COLS = 16, JOIN_ROW = MAX_K + 4, JOIN_SMEM = (2 * MAX_K * JOIN_ROW + MAX_K * JOIN_COLS) * 4;
+__global__ void __launch_bounds__(256) k_delta_join(const __grid_constant__ DeltaArgs A) {
+    extern __shared__ __align__(16) float join[];  // two products [MAX_K][JOIN_ROW], a state [MAX_K][JOIN_COLS]
+    float* S = join + 2 * MAX_K * JOIN_ROW;
+    const int tid = threadIdx.x, head = blockIdx.y, c0 = (int)blockIdx.z * JOIN_COLS;
+    const int d = tid >> 1, c = (tid & 1) * 8, kdim = A.kdim, kpad = (kdim + 3) / 4 * 4;
+    const long long s = blockIdx.x, size = (long long)kdim * A.vdim;
+    const int all = (span_of(A, s).len + C - 1) / C, last = (all + A.seg - 1) / A.seg - 1;
+    auto unit = [&](int g) { return (s * A.segs + g) * A.heads + head; };
+    auto load = [&](int g) {
+        const float* M = A.maps + unit(g) * kdim * kdim;
+        float* to = join + (g & 1) * MAX_K * JOIN_ROW;
+        if (kdim == kpad) {
+            for (int i = tid; i < kdim * (kdim / 4); i += 256) {
+                const int r = i / (kdim / 4), k = i % (kdim / 4) * 4;
+                copy16(to + r * JOIN_ROW + k, M + r * kdim + k, true);
+            }
+        } else {
+            for (int i = tid; i < kdim * kpad; i += 256) {
+                const int r = i / kpad, k = i % kpad;
+                to[r * JOIN_ROW + k] = k < kdim ? M[r * kdim + k] : 0.0f;
+            }
+        }
+        copies_end();
+    };
+    if (last < 2) return;
+    load(1);
+    for (int i = tid; i < MAX_K * JOIN_COLS; i += 256) {
+        const int r = i / JOIN_COLS, cc = c0 + i % JOIN_COLS;
+        S[i] = r < kdim && cc < A.vdim ? A.starts[unit(1) * size + (long long)r * A.vdim + cc] : 0.0f;
+    }
+    for (int g = 1; g < last; ++g) {
+        if (g + 1 < last) load(g + 1);
+        else copies_end();
+        float* to = A.starts + unit(g + 1) * size + (long long)d * A.vdim + c0 + c;
+        float sum[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[j] = d < kdim && c0 + c + j < A.vdim ? to[j] : 0.0f;
+        copies_wait<1>();
+        __syncthreads();
+        const float* M = join + (g & 1) * MAX_K * JOIN_ROW + d * JOIN_ROW;
+        if (d < kdim)
+#pragma unroll 2
+            for (int k = 0; k < kpad; k += 4) {
+                const float4 m = *reinterpret_cast<const float4*>(M + k);
+                const float mk[4] = {m.x, m.y, m.z, m.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int j = 0; j < 8; j += 4) {
+                        const float4 v = *reinterpret_cast<const float4*>(S + (k + e) * JOIN_COLS + c + j);
+                        sum[j] = fmaf(mk[e], v.x, sum[j]);
+                        sum[j + 1] = fmaf(mk[e], v.y, sum[j + 1]);
+                        sum[j + 2] = fmaf(mk[e], v.z, sum[j + 2]);
+                        sum[j + 3] = fmaf(mk[e], v.w, sum[j + 3]);
+                    }
+            }
+        __syncthreads();  // S and the product are no longer read
+        if (d < kdim)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                S[d * JOIN_COLS + c + j] = sum[j];
+                if (c0 + c + j < A.vdim) to[j] = sum[j];
+            }
+    }
+    copies_wait<0>();
+}
+
 // the rows of no sequence where there is no sequence at all
 template <typename T>
 __global__ void __launch_bounds__(256) k_delta_zero(const __grid_constant__ DeltaArgs A, Heads r, int heads, int width) {
@@ -206,7 +278,25 @@ int64_t vpad_of(const snn_delta* d) { return (d->v_dim + 7) / 8 * 8; }
 // T and P, keys, factors, then (kept for the gradient) states and U
 struct Layout {
     int64_t keys, factors, states, u, all, kept_all;
+    int64_t starts, maps, cut;  // of a workspace for segments: their offsets in it, its size
 };
+// Chunks of a segment, and how many segments a sequence has at most (1: whole).  Few heads leave
+// most SMs empty for long: then sequences are cut, a first run makes what each segment makes of no
+// state and the product of its steps (twice the columns, no results), those are joined, and all segments
+// run at once.  That is 2.7 times the work (about), so it takes four segments and more, as many as
+// give every SM eight warps; a segment has at least 8 chunks.  1 x 16,384 steps x 16 heads of 128 x 128 f16: whole
+// 1,300 us, by 8 segments 361 + 40 + 281.  Packed sequences may be of any lengths: segments are of the mean's
+// size, and a sequence has as many as all rows would fill.
+void segments_of(const snn_delta* d, int& seg, int& segs) {
+    seg = 0;
+    segs = 1;
+    const int64_t chunks = (mean_steps(d) + C - 1) / C, warps = d->n_seq * d->heads * ((d->v_dim + 15) / 16);
+    int64_t g = 1;
+    while (g < 16 && warps * g * 2 <= 8 * SMS && chunks >= 16 * g) g *= 2;
+    if (g < 4 || d->n_seq > 64) return;
+    seg = (int)((chunks + g - 1) / g);
+    segs = (int)(d->offsets ? (d->n_steps / C + 1) / seg + 1 : (chunks + seg - 1) / seg);
+}
 Layout layout_of(const snn_delta* d) {
     const DeltaSizes z = sizes_of(d);
     const int64_t units = slots_of(d) * d->heads, kd = d->k_dim <= 64 ? 64 : 128;
@@ -216,6 +306,11 @@ Layout layout_of(const snn_delta* d) {
     l.all = l.states = l.factors + round256(units * SC * 4);
     l.u = l.states + round256(units * d->v_dim * (kd + PAD) * z.kept);
     l.kept_all = l.u + round256(units * C * vpad_of(d) * z.kept);
+    int seg, segs;
+    segments_of(d, seg, segs);
+    l.starts = 0;
+    l.maps = segs > 1 ? round256(d->n_seq * segs * d->heads * d->k_dim * d->v_dim * 4) : 0;
+    l.cut = segs > 1 ? l.maps + round256(d->n_seq * segs * d->heads * d->k_dim * d->k_dim * 4) : 0;
     return l;
 }
 bool by_steps(const snn_delta* d) { return mean_steps(d) <= 8; }
@@ -243,6 +338,7 @@ DeltaArgs base_args(const snn_delta* d, const snn_heads* q, const snn_heads* k, 
     A.logit = (d->flags & SNN_SCAN_LOGIT) != 0;
     A.zero = d->offsets && (d->flags & SNN_SCAN_ZERO) != 0;
     A.scale = d->scale;
+    A.segs = 1;
     return A;
 }
 void zero_rows(const snn_delta* d, const DeltaArgs& A, const Heads& r, int heads, int width, cudaStream_t st) {
@@ -255,11 +351,11 @@ void zero_rows(const snn_delta* d, const DeltaArgs& A, const Heads& r, int heads
 // serve its warps, each with 16 columns of the state.  Up to four warps have a tensor core
 // each; eight share them (1.8 times the time for twice the work), but CTAs that do
 // not fit on the SMs at once are a second round.
-int warps_of(const snn_delta* d) {
+int warps_of(const snn_delta* d, int64_t segs) {
     int best = 1;
     double least = 1e300;
     for (int nw = 1; nw <= 8; nw *= 2) {
-        const int64_t ctas = d->n_seq * d->heads * ((d->v_dim + 16 * nw - 1) / (16 * nw));
+        const int64_t ctas = d->n_seq * segs * d->heads * ((d->v_dim + 16 * nw - 1) / (16 * nw));
         const double cost = (double)((ctas + SMS - 1) / SMS) * (nw == 8 ? 1.8 : 1.0);
         if (nw > 1 && 16 * nw >= 2 * d->v_dim) break;  // no warp without columns where fewer do
         if (cost <= least) {
@@ -283,9 +379,10 @@ int64_t delta_scan_saved(const snn_delta* d) {
     check_desc(d);
     return layout_of(d).kept_all;
 }
-int64_t delta_scan_workspace(const snn_delta* d) {
+int64_t delta_scan_workspace(const snn_delta* d, bool with_saved) {
     check_desc(d);
-    return by_steps(d) ? 0 : layout_of(d).all;
+    const Layout l = layout_of(d);
+    return with_saved ? l.cut : by_steps(d) ? 0 : l.cut + l.all;
 }
 
 void delta_scan(const snn_delta* d, const snn_heads* q, const snn_heads* k, const snn_heads* v, const snn_rows* gate,
@@ -311,9 +408,11 @@ void delta_scan(const snn_delta* d, const snn_heads* q, const snn_heads* k, cons
         SNN_CUDA(cudaGetLastError());
         return;
     }
-    char* base = (char*)(saved ? saved : work);
+    // the workspace: what cut sequences want, then, without saved, what it would hold of the chunks
+    char* base = (char*)saved;
     if (saved) check_work(saved, saved_bytes, l.kept_all, "saved");
-    else check_work(work, work_bytes, l.all, "workspace");
+    check_work(work, work_bytes, saved ? l.cut : l.cut + l.all, "workspace");
+    if (!saved) base = (char*)work + l.cut;
     A.squares = base;
     A.keys = base + l.keys;
     A.factors = (float*)(base + l.factors);
@@ -321,10 +420,22 @@ void delta_scan(const snn_delta* d, const snn_heads* q, const snn_heads* k, cons
         A.states = base + l.states;
         A.u = base + l.u;
     }
+    segments_of(d, A.seg, A.segs);
+    A.starts = (float*)work;
+    A.maps = (float*)((char*)work + l.maps);
     with_elem(d->type, [&](auto t) {
         using T = decltype(t);
         if (A.slots) launch_prep<T>(A, st);
-        launch_scan<T>(A, warps_of(d), st);
+        if (A.segs > 1) {
+            A.only = 1;
+            launch_scan<T>(A, 8, st);
+            A.only = 0;
+            set_smem(k_delta_join, JOIN_SMEM);
+            const dim3 grid((unsigned)d->n_seq, (unsigned)d->heads, (unsigned)((d->v_dim + JOIN_COLS - 1) / JOIN_COLS));
+            k_delta_join<<<grid, 256, JOIN_SMEM, st>>>(A);
+            SNN_CUDA(cudaGetLastError());
+        }
+        launch_scan<T>(A, warps_of(d, A.segs), st);
     });
 }
 
@@ -372,7 +483,7 @@ void delta_scan_grad(const snn_delta* d, const snn_heads* q, const snn_heads* k,
     A.u = base + l.u;
     A.dstates = (char*)work;
     A.dr = (char*)work + (l.u - l.states);
-    with_elem(d->type, [&](auto t) { launch_grads<decltype(t)>(A, warps_of(d), st); });
+    with_elem(d->type, [&](auto t) { launch_grads<decltype(t)>(A, warps_of(d, 1), st); });
 }
 
 }  // namespace snnb

@@ -37,9 +37,12 @@ void launch_scan_of(const DeltaArgs& A, int warps, cudaStream_t st) {
             using S = Stage<P, KD, NW, P::OUT>;
             auto* kernel = k_delta_scan<P, KD, NW>;
             set_smem(kernel, S::SMEM);
-            const dim3 grid((unsigned)std::min<long long>(A.n_seq, 1 << 30), (unsigned)A.heads,
-                            (unsigned)((A.vdim + S::VW - 1) / S::VW));
-            kernel<<<grid, NW * 32, S::SMEM, st>>>(A);
+            const int tiles = (A.vdim + S::VW - 1) / S::VW;
+            DeltaArgs B = A;
+            B.tiles = tiles;
+            const dim3 grid((unsigned)std::min<long long>(A.n_seq * A.segs, 1 << 30), (unsigned)A.heads,
+                            (unsigned)(A.only ? tiles + (A.kdim + S::VW - 1) / S::VW : tiles));
+            kernel<<<grid, NW * 32, S::SMEM, st>>>(B);
         });
     });
     SNN_CUDA(cudaGetLastError());

@@ -33,12 +33,12 @@ struct Stage {
     }
     // chunk c of sequence s; vals: the values' rows or, backward, those of dy (or none)
     __device__ __forceinline__ void load(const DeltaArgs& A, const Heads& vals, long long s, const Span& sp, int c, int head,
-                                         int col0, int tid) {
+                                         int col0, int vdim, int tid) {
         const int n = min(C, sp.len - c * C);
         const long long slot = sp.chunk + c, unit = slot * A.heads + head;
         load_words(k, A.keys + (slot * A.hk + head / A.group) * 2 * KEYS, 2 * KEYS, tid, NW * 32);
         load_rows<T, C, VW>(v, (const T*)vals.p + row_at(A, vals, s, sp, c * C) + head * vals.hs + col0, vals.st,
-                            vals.p ? n : 0, A.vdim - col0, vals.word, tid, NW * 32);
+                            vals.p ? n : 0, vdim - col0, vals.p ? vals.word : 16, tid, NW * 32);
         load_words(t, A.squares + unit * P::SQUARES, SQUARES, tid, NW * 32);
         load_words(f, A.factors + unit * SC, SCAN_FACTORS * 4, tid, NW * 32);
     }
@@ -150,25 +150,25 @@ __device__ __forceinline__ void keep_state(const float (&S)[NT][4], float back, 
 }
 // f32 states [kdim, vdim] from and to a warp's columns
 template <int NT>
-__device__ __forceinline__ void read_state(float (&S)[NT][4], const float* h, const DeltaArgs& A, int col) {
+__device__ __forceinline__ void read_state(float (&S)[NT][4], const float* h, const DeltaArgs& A, int col, int vdim) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int c = col + g + (e >> 1) * 8, d = i * 8 + 2 * t4 + (e & 1);
-            S[i][e] = h && c < A.vdim && d < A.kdim ? h[(long long)d * A.vdim + c] : 0.0f;
+            S[i][e] = h && c < vdim && d < A.kdim ? h[(long long)d * vdim + c] : 0.0f;
         }
 }
 template <int NT>
-__device__ __forceinline__ void write_state(const float (&S)[NT][4], float back, float* h, const DeltaArgs& A, int col) {
+__device__ __forceinline__ void write_state(const float (&S)[NT][4], float back, float* h, const DeltaArgs& A, int col, int vdim) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int c = col + g + (e >> 1) * 8, d = i * 8 + 2 * t4 + (e & 1);
-            if (c < A.vdim && d < A.kdim) h[(long long)d * A.vdim + c] = S[i][e] * back;
+            if (c < vdim && d < A.kdim) h[(long long)d * vdim + c] = S[i][e] * back;
         }
 }
 
@@ -298,19 +298,39 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_scan(const __grid_constant
     constexpr int NT = KD / 8, VS = St::VW + PAD;
     extern __shared__ __align__(16) char smem[];
     const int tid = threadIdx.x, warp = tid >> 5;
-    const int head = blockIdx.y, col0 = (int)blockIdx.z * St::VW, col = col0 + warp * 16;
-    const int w = A.vdim - col;  // this warp's columns (16 and more: all; none: it only loads)
-    for (long long s = blockIdx.x; s < A.n_seq; s += gridDim.x) {
+    // (of the runs that make the segments' starts, those behind the values' columns take the unit matrix along, with
+    // no values: what comes out is the product of the steps)
+    const bool unit_run = A.only && (int)blockIdx.z >= A.tiles;
+    const int head = blockIdx.y, col0 = ((int)blockIdx.z - (unit_run ? A.tiles : 0)) * St::VW, col = col0 + warp * 16;
+    const int vdim = unit_run ? A.kdim : A.vdim, w = vdim - col;  // w: this warp's columns (16 and more: all; none: it only loads)
+    Heads values = A.v;
+    if (unit_run) values.p = nullptr;
+    for (long long item = blockIdx.x; item < A.n_seq * A.segs; item += gridDim.x) {
+        const long long s = item / A.segs;
+        const int segment = (int)(item - s * A.segs);
         const Span sp = span_of(A, s);
-        const int chunks = (sp.len + C - 1) / C;
+        const int all = (sp.len + C - 1) / C, first = segment * A.seg;
+        const int chunks = A.seg ? min(all, first + A.seg) : all;  // the first one that is not this segment's
+        const bool last = segment == (A.seg ? max(0, (all + A.seg - 1) / A.seg - 1) : 0);
+        if ((!last && chunks <= first) || (A.only && (last || (unit_run && segment == 0)))) continue;
         float S[NT][4], sigma = 1.0f;  // S times sigma
-        read_state<NT>(S, A.h0 ? A.h0 + (s * A.heads + head) * A.kdim * A.vdim : nullptr, A, col);
-        if (St::STAGES == 2 && chunks) St(smem).load(A, A.v, s, sp, 0, head, col0, tid);
+        const long long size = (long long)A.kdim * A.vdim;
+        if (unit_run) {
+            const int lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) S[i][e] = col + g + (e >> 1) * 8 == i * 8 + 2 * t4 + (e & 1) ? 1.0f : 0.0f;
+        } else {
+            read_state<NT>(S, segment == 0 ? (A.h0 ? A.h0 + (s * A.heads + head) * size : nullptr)
+                                           : (A.only ? nullptr : A.starts + (item * A.heads + head) * size), A, col, vdim);
+        }
+        if (St::STAGES == 2 && chunks > first) St(smem + (first & 1) * St::BYTES).load(A, values, s, sp, first, head, col0, vdim, tid);
         copies_end();
-        for (int c = 0; c < chunks; ++c) {
+        for (int c = first; c < chunks; ++c) {
             const St st(smem + (St::STAGES == 2 ? (c & 1) * St::BYTES : 0));
-            if (St::STAGES == 1) St(smem).load(A, A.v, s, sp, c, head, col0, tid);
-            else if (c + 1 < chunks) St(smem + ((c + 1) & 1) * St::BYTES).load(A, A.v, s, sp, c + 1, head, col0, tid);
+            if (St::STAGES == 1) St(smem).load(A, values, s, sp, c, head, col0, vdim, tid);
+            else if (c + 1 < chunks) St(smem + ((c + 1) & 1) * St::BYTES).load(A, values, s, sp, c + 1, head, col0, vdim, tid);
             copies_end();
             copies_wait<St::STAGES - 1>();
             __syncthreads();
@@ -324,13 +344,13 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_scan(const __grid_constant
                     ik = inverse_of(st.f[K_SCALE]);
                     iq = inverse_of(st.f[Q_SCALE]);
                 }
-                if (A.states) keep_state<K, NT>(S, back, St::keep(smem, warp), (K*)A.states + (unit * A.vdim + col) * (KD + PAD), w);
+                if (A.states && !A.only) keep_state<K, NT>(S, back, St::keep(smem, warp), (K*)A.states + (unit * A.vdim + col) * (KD + PAD), w);
                 float r[8][4] = {}, o[8][4] = {}, u[8][4];
 #pragma unroll
                 for (int d = 0; d < KD / 16; ++d) {
                     const typename P::A a = P::split(S[2 * d], S[2 * d + 1], 1.0f);
                     read_with<P, P::PIECES, KD>(r, a, st.k, d);
-                    read_with<P, P::OUT, KD>(o, a, st.q, d);
+                    if (!A.only) read_with<P, P::OUT, KD>(o, a, st.q, d);
                 }
                 // r = b (v - since K S)
                 values_of<T, VS>(u, st.v + warp * 16);
@@ -357,6 +377,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_scan(const __grid_constant
                     }
                     ss = warp_scale(u);
                 }
+                if (!A.only) {
                 // o = since Q S + P u, times the pieces' scales
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -373,7 +394,8 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_scan(const __grid_constant
                     for (int e = 0; e < 4; ++e) o[i][e] *= f;
                 }
                 store_tile<T, VS>(o, st.v + warp * 16, (T*)A.y.p + row_at(A, A.y, s, sp, c * C) + head * A.y.hs + col, A.y.st, n, w, A.y.word);
-                if (A.u) keep_tile<T, K, VS>(u, st.v + warp * 16, (K*)A.u + unit * C * A.vpad + col, A.vpad, A.vpad - col);
+                }
+                if (A.u && !A.only) keep_tile<T, K, VS>(u, st.v + warp * 16, (K*)A.u + unit * C * A.vpad + col, A.vpad, A.vpad - col);
                 // S = since_64 S + (until u)^T K; 1 - since_64 keeps its bits where decays are near 1
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -387,12 +409,14 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_scan(const __grid_constant
             }
             __syncthreads();
         }
-        if (A.h && w > 0) write_state<NT>(S, inverse_of(sigma), A.h + (s * A.heads + head) * A.kdim * A.vdim, A, col);
+        float* to = unit_run ? A.maps + (item * A.heads + head) * A.kdim * A.kdim
+                             : A.only ? A.starts + ((item + 1) * A.heads + head) * size : A.h && last ? A.h + (s * A.heads + head) * size : nullptr;
+        if (to && w > 0) write_state<NT>(S, inverse_of(sigma), to, A, col, vdim);
         copies_wait<0>();
         __syncthreads();
     }
     store_done();
-    if (A.zero) zero_rest<T>(A, A.y, A.heads, A.vdim, ((long long)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x,
+    if (A.zero && !A.only) zero_rest<T>(A, A.y, A.heads, A.vdim, ((long long)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x,
                              (long long)gridDim.x * gridDim.y * gridDim.z);
 }
 
@@ -414,14 +438,14 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_back(const __grid_constant
         const Span sp = span_of(A, s);
         const int chunks = (sp.len + C - 1) / C;
         float D[NT][4], sigma = 1.0f;
-        read_state<NT>(D, A.dh ? A.dh + (s * A.heads + head) * A.kdim * A.vdim : nullptr, A, col);
-        if (St::STAGES == 2 && chunks) St(smem).load(A, A.dy, s, sp, chunks - 1, head, col0, tid);
+        read_state<NT>(D, A.dh ? A.dh + (s * A.heads + head) * A.kdim * A.vdim : nullptr, A, col, A.vdim);
+        if (St::STAGES == 2 && chunks) St(smem).load(A, A.dy, s, sp, chunks - 1, head, col0, A.vdim, tid);
         copies_end();
         for (int i = 0; i < chunks; ++i) {
             const int c = chunks - 1 - i;
             const St st(smem + (St::STAGES == 2 ? (i & 1) * St::BYTES : 0));
-            if (St::STAGES == 1) St(smem).load(A, A.dy, s, sp, c, head, col0, tid);
-            else if (c > 0) St(smem + ((i + 1) & 1) * St::BYTES).load(A, A.dy, s, sp, c - 1, head, col0, tid);
+            if (St::STAGES == 1) St(smem).load(A, A.dy, s, sp, c, head, col0, A.vdim, tid);
+            else if (c > 0) St(smem + ((i + 1) & 1) * St::BYTES).load(A, A.dy, s, sp, c - 1, head, col0, A.vdim, tid);
             copies_end();
             copies_wait<St::STAGES - 1>();
             __syncthreads();
@@ -491,7 +515,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_back(const __grid_constant
             }
             __syncthreads();
         }
-        if (A.dh0 && w > 0) write_state<NT>(D, inverse_of(sigma), A.dh0 + (s * A.heads + head) * A.kdim * A.vdim, A, col);
+        if (A.dh0 && w > 0) write_state<NT>(D, inverse_of(sigma), A.dh0 + (s * A.heads + head) * A.kdim * A.vdim, A, col, A.vdim);
         copies_wait<0>();
         __syncthreads();
     }

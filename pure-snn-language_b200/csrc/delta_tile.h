@@ -65,6 +65,10 @@ struct DeltaArgs {
     float* factors;           // [slots, heads, SC]
     char *states, *u;         // saved: [slots, heads, vdim, KD + PAD], [slots, heads, C, vpad] of Kept
     char *dstates, *dr;       // gradients' workspace: the same forms
+    // sequences cut into `segs` segments of `seg` chunks (0: whole): where each starts from [n_seq, segs, heads, kdim,
+    // vdim] (`only`: the run that makes them, and of those between the products of their steps [.., kdim, kdim])
+    int seg, segs, only, tiles;  // tiles: CTAs along the values' columns
+    float *starts, *maps;
 };
 
 struct Span {

@@ -201,7 +201,7 @@ def _load(path):
     L.snn_qk_norm_grad_workspace.argtypes = [ps, vp]
     L.snn_qk_norm_grad.argtypes = [ps, pr, pr, vp, vp, vp, vp, pr, pr, pr, pr, vp, vp, vp, i64, vp]
     L.snn_delta_scan_saved.argtypes = [ps, vp]
-    L.snn_delta_scan_workspace.argtypes = [ps, vp]
+    L.snn_delta_scan_workspace.argtypes = [ps, i32, vp]
     L.snn_delta_scan_grad_workspace.argtypes = [ps, vp]
     L.snn_delta_scan.argtypes = [ps, pr, pr, pr, pr, pr, vp, pr, vp, vp, i64, vp, i64, vp]
     L.snn_delta_scan_grad.argtypes = [ps, pr, pr, pr, pr, pr, vp, i64, pr, vp, pr, pr, pr, pr, pr, vp, vp, i64, vp]
@@ -749,10 +749,11 @@ def _delta_args(q, k, v, gate, beta, scale, logit, offsets, zero):
 
 @functools.lru_cache(maxsize=1024)
 def _delta_sizes(kind, n_seq, n, hk, heads, dk, dv, packed):
-    """(bytes of saved, workspace bytes forward, gradient) of a delta-rule scan's sizes."""
+    """(bytes of saved, workspace bytes forward, with saved, gradient) of a delta-rule scan's sizes."""
     desc, size, L, out = _DELTA.pack(kind, 0, n_seq, n, hk, heads, dk, dv, 8 if packed else 0, 1.0, 0), C.c_int64(), lib(), []
-    for fn in (L.snn_delta_scan_saved, L.snn_delta_scan_workspace, L.snn_delta_scan_grad_workspace):
-        _check(fn(desc, C.byref(size)))
+    for fn, how in ((L.snn_delta_scan_saved, ()), (L.snn_delta_scan_workspace, (0,)), (L.snn_delta_scan_workspace, (1,)),
+                    (L.snn_delta_scan_grad_workspace, ())):
+        _check(fn(desc, *how, C.byref(size)))
         out.append(size.value)
     return tuple(out)
 
@@ -789,11 +790,12 @@ def delta_scan(q, k, v, gate, beta, h0=None, scale=1.0, logit=False, offsets=Non
     if save:
         saved = _new(dev, stream, (sizes[0],), _T.uint8)
         sp = saved.data_ptr()
-    elif sizes[1]:
-        work = _new(dev, stream, (sizes[1],), _T.uint8)
+    size = sizes[2] if save else sizes[1]
+    if size:
+        work = _new(dev, stream, (size,), _T.uint8)
         wp = work.data_ptr()
     _call(lib().snn_delta_scan, dev, stream, desc, *rows, None if h0 is None else _state(h0, "h0", state, dev), yr, hp,
-          sp, sizes[0], wp, sizes[1])
+          sp, sizes[0], wp, size)
     return (out, h_out, saved) if save else (out, h_out)
 
 
@@ -824,11 +826,11 @@ def delta_scan_grad(q, k, v, gate, beta, dy, saved, dh=None, scale=1.0, logit=Fa
     if need_h0:
         dh0 = _new(dev, stream, state, _T.float32)
         hp = dh0.data_ptr()
-    if sizes[2]:
-        work = _new(dev, stream, (sizes[2],), _T.uint8)
+    if sizes[3]:
+        work = _new(dev, stream, (sizes[3],), _T.uint8)
         wp = work.data_ptr()
     _call(lib().snn_delta_scan_grad, dev, stream, desc, *rows, saved.data_ptr(), sizes[0], dyr,
-          None if dh is None else _state(dh, "dh", state, dev), dqr, dkr, dvr, gr, br, hp, wp, sizes[2])
+          None if dh is None else _state(dh, "dh", state, dev), dqr, dkr, dvr, gr, br, hp, wp, sizes[3])
     return dq, dk, dv, dgate, dbeta, dh0
 
 

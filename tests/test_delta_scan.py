@@ -114,13 +114,13 @@ def test_grad_refuses(over):
 
 def test_null_descriptions_and_sizes():
     n, L = C.c_int64(), snn.lib()
-    for fn in (L.snn_delta_scan_saved, L.snn_delta_scan_workspace, L.snn_delta_scan_grad_workspace):
-        assert fn(None, C.byref(n)) == 1
+    for fn, how in ((L.snn_delta_scan_saved, ()), (L.snn_delta_scan_workspace, (0,)), (L.snn_delta_scan_grad_workspace, ())):
+        assert fn(None, *how, C.byref(n)) == 1
     d = snn._DELTA.pack(1, 0, 3, 100, 2, 4, 128, 100, 0, 1.0, 0)
     assert L.snn_delta_scan_saved(d, None) == 1
     assert L.snn_delta_scan_saved(d, C.byref(n)) == 0 and n.value >= 3 * 2 * 4 * 100 * 128 * 2  # a state a chunk
     d = snn._DELTA.pack(1, 0, 3, 8, 2, 4, 128, 100, 0, 1.0, 0)  # single steps want no workspace
-    assert L.snn_delta_scan_workspace(d, C.byref(n)) == 0 and n.value == 0
+    assert L.snn_delta_scan_workspace(d, 0, C.byref(n)) == 0 and n.value == 0
 
 
 # ---- GPU ------------------------------------------------------------------------------
@@ -212,6 +212,31 @@ def test_packed(kind, lengths, before, behind):
     ref.close(host(y2[before:rows - behind]), (want["y"][0][before:rows - behind], want["y"][1]), kind, "y")
     ref.close(host(h2), want["h"], kind, "h")
     assert (out[:before] == 7).all() and (out[rows - behind:] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("logit", [False, True])
+def test_segments(kind, logit):
+    """Long sequences of few heads are cut into segments that run at once."""
+    check(kind, 1, 2500, 1, 2, 40, 24, logit=logit, scale=0.2, grads=kind == "f32")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("lengths", [[4000, 0, 100], [64 * 40, 64 * 25 + 1, 3]])
+def test_segments_packed(kind, lengths):
+    import torch
+    off = np.concatenate([[2], 2 + np.cumsum(lengths)])
+    x, s0, _, _ = make(13, (int(off[-1]) + 3,), 1, 1, 20, 36, kind, n_seq=len(lengths))
+    want = ref.run(*map(host, x), host(s0), offsets=off.tolist(), kind=kind)
+    y, h = snn.delta_scan(*x, s0, offsets=torch.tensor(off, device="cuda"))
+    ref.close(host(y), want["y"], kind, "y")
+    ref.close(host(h), want["h"], kind, "h")
+    y, h, _ = snn.delta_scan(*x, offsets=torch.tensor(off, device="cuda"), save=True)
+    want = ref.run(*map(host, x), 0 * host(s0), offsets=off.tolist(), kind=kind)
+    ref.close(host(y), want["y"], kind, "y")
+    ref.close(host(h), want["h"], kind, "h")
 
 
 @pytest.mark.gpu
