@@ -570,8 +570,9 @@ int snn_qk_norm_grad(const snn_qk* desc, const snn_heads* q, const snn_heads* k,
  * States are f32 [n_seq, heads, k_dim, v_dim]; h0 (nullable: zeros) and h (nullable)
  * may be the same.  Sums are f32, y is rounded once.  Long sequences are
  * taken 64 steps at a time, the recurrence's sum in another order: a NaN or an
- * infinity in a row may then make the other rows of its 64 steps NaN too.  The same
- * holds for the gradients.
+ * infinity in a key, value, gate or rate may then make earlier rows of its 64 steps
+ * NaN too (of a value, in its column).  The same holds for the gradients, in both
+ * directions.
  * Where sequences have 8 steps or fewer in the mean the steps are taken one by one,
  * without a workspace. */
 typedef struct snn_delta {
@@ -626,7 +627,7 @@ int snn_delta_scan_grad(const snn_delta* desc, const snn_heads* q, const snn_hea
  * whose n is 0 is left alone.  bits = 32: m, v are f32.  bits = 8: m and the root
  * of v are held as e4m3 values (a byte each) with f32 scales [ceil(n / 256)] for every 256
  * elements, the largest magnitude / 448; a root above zero is held as 2^-9 of its
- * scale at least.  step is counted from 1; with step_device (int64 in device memory)
+ * scale at least; a block that has come to hold a NaN is NaN as a whole.  step is counted from 1; with step_device (int64 in device memory)
  * it is read there, so that a captured step counts on.  Tensors of a call must not
  * overlap.  `tensors` is host memory, read before the call returns; the call is
  * asynchronous, allocates nothing on the device and may be captured (a graph

@@ -430,7 +430,7 @@ void delta_scan(const snn_delta* d, const snn_heads* q, const snn_heads* k, cons
             A.only = 1;
             launch_scan<T>(A, 8, st);
             A.only = 0;
-            set_smem(k_delta_join, JOIN_SMEM);
+            set_smem<k_delta_join>(JOIN_SMEM);
             const dim3 grid((unsigned)d->n_seq, (unsigned)d->heads, (unsigned)((d->v_dim + JOIN_COLS - 1) / JOIN_COLS));
             k_delta_join<<<grid, 256, JOIN_SMEM, st>>>(A);
             SNN_CUDA(cudaGetLastError());

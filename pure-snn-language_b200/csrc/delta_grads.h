@@ -242,8 +242,8 @@ __global__ void __launch_bounds__(GRADS, 1) k_delta_grads(const __grid_constant_
                     by_col[j][e & 1] += both;
                     p[j][e] = pv;
                     x[j][e] = rate[i] * xv;
-                    tp = fmaxf(tp, fabsf(p[j][e]));
-                    tx = fmaxf(tx, fabsf(x[j][e]));
+                    tp = fmaxf(tp, finite_size(p[j][e]));
+                    tx = fmaxf(tx, finite_size(x[j][e]));
                 }
 #pragma unroll
         for (int j = 0; j < NQ; ++j)
@@ -435,7 +435,7 @@ __global__ void __launch_bounds__(GRADS, 1) k_delta_grads(const __grid_constant_
                 if (i < n) {
                     const T gate = ((const T*)A.gate.p)[row_at(A, A.gate, s, sp, t0 + i) + head * A.gate.hs];
                     if (A.logit) dg *= 1.0f / (1.0f + expf(to_f32(gate)));
-                    else if (to_f32(gate) == -INFINITY) dg = 0.0f;
+                    if (to_f32(gate) == -INFINITY) dg = 0.0f;
                     ((T*)A.dgate.p)[row_at(A, A.dgate, s, sp, t0 + i) + head * A.dgate.hs] = from_f32<T>(dg);
                 }
             }

@@ -22,8 +22,8 @@ void launch_prep_of(const DeltaArgs& A, cudaStream_t st) {
     using P = typename PathOf<T>::P;
     by_dim<T>(A.kdim, [&](auto kd) {
         constexpr int KD = decltype(kd)::value;
-        auto* kernel = k_delta_prep<P, KD>;
-        set_smem(kernel, prep_smem<P, KD>());
+        constexpr auto* kernel = k_delta_prep<P, KD>;
+        set_smem<kernel>(prep_smem<P, KD>());
         kernel<<<dim3((unsigned)A.slots, (unsigned)A.heads), PREP, prep_smem<P, KD>(), st>>>(A);
     });
     SNN_CUDA(cudaGetLastError());
@@ -35,8 +35,8 @@ void launch_scan_of(const DeltaArgs& A, int warps, cudaStream_t st) {
         by_warps(warps, [&](auto nw) {
             constexpr int KD = decltype(kd)::value, NW = decltype(nw)::value;
             using S = Stage<P, KD, NW, P::OUT>;
-            auto* kernel = k_delta_scan<P, KD, NW>;
-            set_smem(kernel, S::SMEM);
+            constexpr auto* kernel = k_delta_scan<P, KD, NW>;
+            set_smem<kernel>(S::SMEM);
             const int tiles = (A.vdim + S::VW - 1) / S::VW;
             DeltaArgs B = A;
             B.tiles = tiles;
@@ -55,16 +55,16 @@ void launch_grads_of(const DeltaArgs& A, int warps, cudaStream_t st) {
         by_warps(warps, [&](auto nw) {
             constexpr int NW = decltype(nw)::value;
             using S = Stage<P, KD, NW, P::PIECES>;
-            auto* kernel = k_delta_back<P, KD, NW>;
-            set_smem(kernel, S::SMEM);
+            constexpr auto* kernel = k_delta_back<P, KD, NW>;
+            set_smem<kernel>(S::SMEM);
             const dim3 grid((unsigned)std::min<long long>(A.n_seq, 1 << 30), (unsigned)A.heads,
                             (unsigned)((A.vdim + S::VW - 1) / S::VW));
             kernel<<<grid, NW * 32, S::SMEM, st>>>(A);
             SNN_CUDA(cudaGetLastError());
         });
         if (!A.slots) return;
-        auto* kernel = k_delta_grads<T, KD>;
-        set_smem(kernel, GradTile<T, KD>::BYTES);
+        constexpr auto* kernel = k_delta_grads<T, KD>;
+        set_smem<kernel>(GradTile<T, KD>::BYTES);
         kernel<<<dim3((unsigned)A.slots, (unsigned)A.hk), GRADS, GradTile<T, KD>::BYTES, st>>>(A);
         SNN_CUDA(cudaGetLastError());
     });

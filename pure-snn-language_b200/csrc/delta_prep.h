@@ -22,12 +22,18 @@ __device__ __forceinline__ float key_scale(float top) { return top == 0.0f ? 0x1
 template <typename T, int KD>
 __device__ __forceinline__ float top_of_tile(const T* m) {
     constexpr int V = 16 / (int)sizeof(T), L = KD / V;
+    // (infinities and NaN do not set the scale of the others)
+    constexpr unsigned INFINITE = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
     unsigned top = 0;
 #pragma unroll
     for (int i = threadIdx.x; i < C * L; i += PREP) {
         const uint4 w = *reinterpret_cast<const uint4*>(m + i / L * (KD + PAD) + i % L * V);
         // (magnitudes of 16 bits order as their bits)
-        top = __vmaxu2(__vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)), top);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const unsigned size = (&w.x)[j] & 0x7fff7fffu;
+            top = __vmaxu2(top, size & __vcmpltu2(size, INFINITE));
+        }
     }
     const float2 f = of_pair<T>(top);
     return fmaxf(f.x, f.y);
@@ -146,7 +152,7 @@ __global__ void __launch_bounds__(PREP, 4) k_delta_prep(const __grid_constant__ 
             const float a = ri[h] * G;
             p2[nt][e] = G != 0.0f ? G * (p2[nt][e] * iqk) : 0.0f;
             x2[nt][e] = a != 0.0f && (nt / 2 < warp || j < i) ? a * (x2[nt][e] * ik * ik) : 0.0f;
-            most = fmaxf(most, fabsf(p2[nt][e]));
+            most = fmaxf(most, finite_size(p2[nt][e]));
         }
     }
     float scale = 1.0f;
@@ -242,7 +248,7 @@ __global__ void __launch_bounds__(PREP, 4) k_delta_prep(const __grid_constant__ 
     for (int i = 0; i < 16; ++i)  // row i, a lane a pair of columns
         if (2 * lane < 16 * (warp + 1)) {
             v[i] = *reinterpret_cast<const float2*>(rows + i * MS + 2 * lane);
-            big = fmaxf(big, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
+            big = fmaxf(big, fmaxf(finite_size(v[i].x), finite_size(v[i].y)));
         }
     scale = 1.0f;
     if constexpr (P::SCALED) {

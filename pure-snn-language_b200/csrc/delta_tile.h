@@ -400,6 +400,7 @@ __device__ __forceinline__ float scale_for(float top) {
 __device__ __forceinline__ float inverse_of(float s) {  // of a power of two
     return __uint_as_float((254u << 23) - __float_as_uint(s));
 }
+__device__ __forceinline__ float finite_size(float x) { return fabsf(x) <= FLT_MAX ? fabsf(x) : 0.0f; }
 template <int N>
 __device__ __forceinline__ float warp_top(const float (&x)[N][4]) {
     float a = 0.0f, b = 0.0f;
@@ -408,8 +409,17 @@ __device__ __forceinline__ float warp_top(const float (&x)[N][4]) {
         a = fmaxf(a, fmaxf(fabsf(x[i][0]), fabsf(x[i][1])));
         b = fmaxf(b, fmaxf(fabsf(x[i][2]), fabsf(x[i][3])));
     }
-    // (magnitudes order as their bits; a NaN is the largest and gives the smallest scale)
-    return __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(fmaxf(a, b))));
+    // (magnitudes order as their bits; fmaxf passes NaN over)
+    float top = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(fmaxf(a, b))));
+    if (top > FLT_MAX) {  // an infinity does not set the scale of its neighbours
+        a = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a = fmaxf(a, finite_size(x[i][j]));
+        top = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(a)));
+    }
+    return top;
 }
 template <int N>
 __device__ __forceinline__ float warp_scale(const float (&x)[N][4]) { return scale_for(warp_top(x)); }
@@ -503,8 +513,15 @@ template <typename T> void launch_prep(const DeltaArgs& A, cudaStream_t st);
 template <typename T> void launch_scan(const DeltaArgs& A, int warps, cudaStream_t st);
 template <typename T> void launch_grads(const DeltaArgs& A, int warps, cudaStream_t st);
 
-template <typename F>
-void set_smem(F* kernel, int bytes) {
-    SNN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+// a kernel's dynamic shared memory, set once for a device
+template <auto* KERNEL>
+void set_smem(int bytes) {
+    static std::atomic<unsigned long long> done;
+    int dev = 0;
+    SNN_CUDA(cudaGetDevice(&dev));
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (dev < 64 && (done & bit)) return;
+    SNN_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done |= bit;
 }
 }  // namespace snnb_delta

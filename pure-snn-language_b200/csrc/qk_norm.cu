@@ -197,12 +197,14 @@ __global__ void __launch_bounds__(THREADS, resident(V, SL, GRAD)) k_qk_norm(cons
 #pragma unroll
                 for (int i = 0; i < SL; ++i) {
                     turn<V, IN, true>(half, c, lane + i * G, za[i], zb[i]);
-                    if (S.w) {
+                    if (S.part) {
 #pragma unroll
                         for (int j = 0; j < V; ++j) {
                             da[which][i][j] = fmaf(za[i][j], a[i][j], da[which][i][j]);
                             db[which][i][j] = fmaf(zb[i][j], b[i][j], db[which][i][j]);
                         }
+                    }
+                    if (S.w) {
                         weigh(weight[which], wa[i], za[i]);
                         weigh(weight[which], wb[i], zb[i]);
                     }

@@ -885,7 +885,7 @@ class AdamW:
             self._table["n"][i] = p.numel()
         used.sort()
         _require(all(a[1] <= b[0] for a, b in zip(used, used[1:])), "parameters, moments, scales or copies overlap")
-        self._shapes = [p.shape for p in self.params]
+        self._shapes, self._at = [p.shape for p in self.params], [p.data_ptr() for p in self.params]
 
     def step(self, grads, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, grad_scale=1.0, stream=None):
         """One step, in place: grads, one for each parameter (contiguous, float32 / bfloat16
@@ -894,6 +894,8 @@ class AdamW:
         runs (for captured steps)."""
         dev, table = self.device, self._table.copy()
         _require(len(grads) == len(self._shapes), "grads are as many as the parameters")
+        if [p.data_ptr() for p in self.params] != self._at:
+            raise SnnError(1, "a parameter's memory is not what it was when this was made")
         at, kinds = [], []
         for g, shape in zip(grads, self._shapes):
             if g is None:

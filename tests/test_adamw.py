@@ -200,7 +200,9 @@ def test_binding_refuses():
         with pytest.raises(snn.SnnError):
             bad()
     opt = snn.AdamW(p)
-    for bad in (lambda: opt.step([p[0]], 1), lambda: opt.step([p[0], p[0]], 1), lambda: opt.step([p[0].cpu(), p[1]], 1),
+    moved = snn.AdamW([torch.zeros(3, device="cuda")])
+    moved.params[0].data = torch.ones(3, device="cuda")
+    for bad in (lambda: moved.step([torch.ones(3, device="cuda")], 1), lambda: opt.step([p[0]], 1), lambda: opt.step([p[0], p[0]], 1), lambda: opt.step([p[0].cpu(), p[1]], 1),
                 lambda: opt.step([p[0], p[1].t()[:2]], 1), lambda: opt.step([p[0].double(), p[1]], 1), lambda: opt.step(p, 0),
                 lambda: opt.step(p, torch.ones(1, device="cuda"))):
         with pytest.raises(snn.SnnError):

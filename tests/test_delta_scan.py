@@ -161,7 +161,7 @@ def test_lengths(kind, t):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", list(KINDS))
-@pytest.mark.parametrize("dk,dv", [(1, 1), (7, 5), (16, 16), (50, 60), (64, 128), (65, 17), (128, 100), (100, 256), (128, 33)])
+@pytest.mark.parametrize("dk,dv", [(1, 1), (7, 5), (16, 16), (50, 60), (64, 128), (65, 17), (128, 100), (100, 256), (128, 33), (8, 1000)])
 @pytest.mark.parametrize("logit", [False, True])
 def test_dims(kind, dk, dv, logit):
     check(kind, 1, 100, 1, 1, dk, dv, logit=logit, scale=dk ** -0.5)
@@ -264,6 +264,7 @@ def test_forgetting_all(kind, t):
     import torch
     x, s0, dy, dh = make(2, (1, t), 1, 1, 16, 16, kind)
     x[3][:, t // 2] = -float("inf")
+    assert snn.delta_scan_grad(*x, dy, snn.delta_scan(*x, s0, logit=True, save=True)[2], dh=dh, logit=True)[3][0, t // 2].item() == 0
     want = ref.run(*map(host, x), host(s0), dy=host(dy), dh=host(dh), kind=kind)
     y, h, saved = snn.delta_scan(*x, s0, save=True)
     ref.close(host(y), want["y"], kind, "y")
@@ -293,6 +294,34 @@ def test_magnitudes(kind, size):
     ref.close(host(h), want["h"], kind, "h")
     for name, g in zip(("dq", "dk", "dv", "dgate", "dbeta", "dh0"), snn.delta_scan_grad(*x, dy, saved, dh=dh)):
         ref.close(host(g), want[name], kind, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(KINDS))
+def test_infinities_stay_where_they_belong(kind):
+    """An infinity in one column of a value reaches that column alone, one in a query its own answer alone."""
+    import torch
+    x, s0, dy, dh = make(8, (1, 200), 1, 1, 32, 48, kind)
+    want = ref.run(*map(host, x), host(s0), dy=host(dy), dh=host(dh), kind=kind)
+    v = x[2].clone()
+    v[0, 100, 0, 20] = float("inf")
+    y, h = snn.delta_scan(*x[:2], v, *x[3:], s0)
+    others = [c for c in range(48) if c != 20]
+    ref.close(host(y)[..., others], (want["y"][0][..., others], want["y"][1]), kind, "y")
+    ref.close(host(h)[..., others], (want["h"][0][..., others], want["h"][1]), kind, "h")
+    ref.close(host(y)[:, :64], (want["y"][0][:, :64], want["y"][1]), kind, "y")
+    assert not torch.isfinite(y[0, 100, 0, 20]) and not torch.isfinite(h[..., 20]).all()
+    q = x[0].clone()
+    q[0, 70, 0, 3] = float("inf")
+    y, h = snn.delta_scan(q, *x[1:], s0)
+    rows = [t for t in range(200) if t != 70]
+    ref.close(host(y)[:, rows], (want["y"][0][:, rows], want["y"][1]), kind, "y")
+    ref.close(host(h), want["h"], kind, "h")
+    _, _, saved = snn.delta_scan(*x, s0, save=True)
+    d = dy.clone()
+    d[0, 100, 0, 20] = float("inf")
+    dv = snn.delta_scan_grad(*x, d, saved, dh=dh)[2]
+    ref.close(host(dv)[..., others], (want["dv"][0][..., others], want["dv"][1]), kind, "dv")
 
 
 @pytest.mark.gpu

@@ -222,6 +222,20 @@ def test_in_place_streams_and_graphs(kind):
 
 
 @pytest.mark.gpu
+def test_gradient_of_weights_that_are_ones():
+    """In C a weight may be NULL and have a gradient all the same."""
+    import torch
+    q, dy = torch.randn(40, 3, 24, device="cuda"), torch.randn(40, 3, 24, device="cuda")
+    dx, dw, work = torch.empty_like(q), torch.empty(24, device="cuda"), torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+    desc = snn._QK.pack(0, 0, 1, 40, 3, 0, 24, 0, 9, 1e-6)
+    rows = [snn._HEADS.pack(t.data_ptr(), 0, 72, 24) for t in (q, dy, dx)]
+    assert snn.lib().snn_qk_norm_grad(desc, rows[0], None, None, None, None, None, rows[1], None, rows[2], None, dw.data_ptr(), None,
+                                      work.data_ptr(), work.numel(), torch.cuda.current_stream().cuda_stream) == 0
+    want = snn.qk_norm_grad(q, None, dy, None, torch.ones(24, device="cuda"))
+    assert torch.equal(dx, want[0]) and torch.equal(dw, want[2])
+
+
+@pytest.mark.gpu
 def test_binding_refuses():
     import torch
     q, k = torch.randn(6, 4, 8, device="cuda"), torch.randn(6, 2, 8, device="cuda")
