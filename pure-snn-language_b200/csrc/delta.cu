@@ -25,7 +25,7 @@ constexpr int MAX_K = 128;
 // A CTA takes 32 V columns of a head's state, a warp every sixteenth row of it, in registers
 // from the first step to the last.  Bound by the state's way from memory and back: 16
 // warps of 64 registers, two CTAs an SM, have 128 kB of it in flight (64 streams x 8 heads
-// x 128 x 128: 8 warps of 215 registers 22.8 us, these 14.5).
+// x 128 x 128 bf16: 8 warps of 215 registers 22.8 us, these 18, of 10.4 at the copy rate).
 constexpr int STEP_WARPS = 16;
 template <typename T, int V>
 __global__ void __launch_bounds__(32 * STEP_WARPS, 2) k_delta_steps(const __grid_constant__ DeltaArgs A) {
@@ -349,14 +349,14 @@ void zero_rows(const snn_delta* d, const DeltaArgs& A, const Heads& r, int heads
 
 // Warps of a CTA.  A chunk's K, Q, T and P fill a CTA's shared memory (one CTA an SM), and
 // serve its warps, each with 16 columns of the state.  Up to four warps have a tensor core
-// each; eight share them (1.8 times the time for twice the work), but CTAs that do
-// not fit on the SMs at once are a second round.
+// each (5.1 us a chunk of 128 x 16, f16); eight share them (7.3), but CTAs that do not fit on
+// the SMs at once are a second round.
 int warps_of(const snn_delta* d, int64_t segs) {
     int best = 1;
     double least = 1e300;
     for (int nw = 1; nw <= 8; nw *= 2) {
         const int64_t ctas = d->n_seq * segs * d->heads * ((d->v_dim + 16 * nw - 1) / (16 * nw));
-        const double cost = (double)((ctas + SMS - 1) / SMS) * (nw == 8 ? 1.8 : 1.0);
+        const double cost = (double)((ctas + SMS - 1) / SMS) * (nw == 8 ? 1.45 : 1.0);
         if (nw > 1 && 16 * nw >= 2 * d->v_dim) break;  // no warp without columns where fewer do
         if (cost <= least) {
             least = cost;

@@ -12,7 +12,9 @@ namespace snnb_delta {
 // Products over the values' columns have bf16 operands for bf16 tensors (as the results
 // are rounded), otherwise f32 in two tf32 pieces; those over steps the keys' type, p and x in
 // one piece of f16 for bf16 tensors, two for f16.  16 warps: 16 rows and a quarter
-// of the columns each; half of the registers are accumulators.
+// of the columns each; half of an SM's registers are accumulators, so that S, D, U, R and dy are
+// read once.  That leaves one CTA an SM, whose phases wait for one another: 8,192 chunks of 128 x 128
+// bf16 800 us (40 % of the issue slots, 22 % of the tensor pipe; 240 at the copy rate).
 struct Ops16 {                 // one piece of a 16-bit type E
     template <typename E>
     static __device__ __forceinline__ void rows_of(unsigned (&a)[4], const E* m, int st) {  // A[i][k] = m[i][k]
