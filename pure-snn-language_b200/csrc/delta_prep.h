@@ -25,16 +25,20 @@ __device__ __forceinline__ float key_scale(float top) { return top == 0.0f ? 0x1
 template <typename T, int KD>
 __device__ __forceinline__ float top_of_tile(const T* m) {
     constexpr int V = 16 / (int)sizeof(T), L = KD / V;
-    // (infinities and NaN do not set the scale of the others)
+    // (magnitudes of 16 bits order as their bits)
     constexpr unsigned INFINITE = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
     unsigned top = 0;
 #pragma unroll
     for (int i = threadIdx.x; i < C * L; i += PREP) {
         const uint4 w = *reinterpret_cast<const uint4*>(m + i / L * (KD + PAD) + i % L * V);
-        // (magnitudes of 16 bits order as their bits)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const unsigned size = (&w.x)[j] & 0x7fff7fffu;
+        top = __vmaxu2(__vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)), top);
+    }
+    if (__vcmpgeu2(top, INFINITE)) {  // infinities and NaN do not set the scale of the others
+        top = 0;
+#pragma unroll 1
+        for (int i = threadIdx.x; i < C * L * 4; i += PREP) {  // the same words, a quarter at a time
+            const int k = threadIdx.x + i / (4 * PREP) * PREP, q = (i / PREP) % 4;
+            const unsigned size = *reinterpret_cast<const unsigned*>(m + k / L * (KD + PAD) + k % L * V + q * (V / 4)) & 0x7fff7fffu;
             top = __vmaxu2(top, size & __vcmpltu2(size, INFINITE));
         }
     }

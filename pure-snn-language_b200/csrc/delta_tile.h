@@ -409,17 +409,9 @@ __device__ __forceinline__ float warp_top(const float (&x)[N][4]) {
         a = fmaxf(a, fmaxf(fabsf(x[i][0]), fabsf(x[i][1])));
         b = fmaxf(b, fmaxf(fabsf(x[i][2]), fabsf(x[i][3])));
     }
-    // (magnitudes order as their bits; fmaxf passes NaN over)
-    float top = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(fmaxf(a, b))));
-    if (top > FLT_MAX) {  // an infinity does not set the scale of its neighbours
-        a = 0.0f;
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) a = fmaxf(a, finite_size(x[i][j]));
-        top = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(a)));
-    }
-    return top;
+    // (magnitudes order as their bits; fmaxf passes NaN over.  A column with an infinity is lost
+    // and does not set the scale of its neighbours.)
+    return __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(fmaxf(finite_size(a), finite_size(b)))));
 }
 template <int N>
 __device__ __forceinline__ float warp_scale(const float (&x)[N][4]) { return scale_for(warp_top(x)); }
