@@ -305,7 +305,7 @@ Layout layout_of(const snn_delta* d) {
     l.factors = l.keys + round256(slots_of(d) * d->k_heads * 2 * C * (kd + PAD) * z.key);
     l.all = l.states = l.factors + round256(units * SC * 4);
     l.u = l.states + round256(units * d->v_dim * (kd + PAD) * z.kept);
-    l.kept_all = l.u + round256(units * C * vpad_of(d) * z.kept);
+    l.kept_all = l.u + round256(units * z.planes * C * vpad_of(d) * z.kept);
     int seg, segs;
     segments_of(d, seg, segs);
     l.starts = 0;
@@ -313,6 +313,7 @@ Layout layout_of(const snn_delta* d) {
     l.cut = segs > 1 ? l.maps + round256(d->n_seq * segs * d->heads * d->k_dim * d->k_dim * 4) : 0;
     return l;
 }
+// Up to 8 steps one by one (64 x 8 heads of 128 x 128 bf16, us by 4 and 8 steps: 32, 55; as a chunk 74)
 bool by_steps(const snn_delta* d) { return mean_steps(d) <= 8; }
 
 DeltaArgs base_args(const snn_delta* d, const snn_heads* q, const snn_heads* k, const snn_heads* v, const snn_rows* gate,

@@ -122,7 +122,8 @@ struct GradTile {
     static constexpr int GW = sizeof(E) == 2 ? 64 : 32;  // columns of the values taken at a time
     static constexpr int STAGES = sizeof(E) == 2 ? 2 : 1, PIECES = sizeof(E) == 4 && sizeof(KE) == 2 ? 2 : 1;
     static constexpr int KEYS = C * (KD + PAD), ROWS = C * (GW + PAD), STATE = GW * (KD + PAD);
-    static constexpr int BLOCK = 4 * ROWS + 2 * STATE, SQ = PIECES * C * MS;
+    static constexpr int PLANES = Kept<T>::PLANES;            // of U and R
+    static constexpr int BLOCK = (2 + 2 * PLANES) * ROWS + 2 * STATE, SQ = PIECES * C * MS;
     // p and x take the blocks' place
     static constexpr int BLOCKS = STAGES * BLOCK * (int)sizeof(E), SQUARES = 2 * SQ * (int)sizeof(KE);
     static constexpr int BYTES = 2 * KEYS * (int)sizeof(KE) + SC * 4 + (BLOCKS > SQUARES ? BLOCKS : SQUARES);
@@ -161,8 +162,13 @@ __global__ void __launch_bounds__(GRADS, 1) k_delta_grads(const __grid_constant_
             E* m = blocks + (G::STAGES == 2 ? (b & 1) * G::BLOCK : 0);
             const int c0 = b * GW, w = A.vdim - c0;
             load_tile<E, C, GW>(m, (const T*)A.dy.p + row_at(A, A.dy, s, sp, t0) + head * A.dy.hs + c0, A.dy.st, A.dy.p ? n : 0, w, A.dy.word);
-            load_tile<E, C, GW>(m + G::ROWS, (const E*)A.u + unit * C * A.vpad + c0, A.vpad, C, A.vpad - c0, 16);
-            load_tile<E, C, GW>(m + 2 * G::ROWS, (const E*)A.dr + unit * C * A.vpad + c0, A.vpad, C, A.vpad - c0, 16);
+            load_tile<E, C, GW>(m + G::ROWS, (const E*)A.u + unit * G::PLANES * C * A.vpad + c0, A.vpad, C, A.vpad - c0, 16);
+            load_tile<E, C, GW>(m + 2 * G::ROWS, (const E*)A.dr + unit * G::PLANES * C * A.vpad + c0, A.vpad, C, A.vpad - c0, 16);
+            if constexpr (G::PLANES == 2) {
+                E* rest = m + 4 * G::ROWS + 2 * G::STATE;
+                load_tile<E, C, GW>(rest, (const E*)A.u + (unit * 2 + 1) * C * A.vpad + c0, A.vpad, C, A.vpad - c0, 16);
+                load_tile<E, C, GW>(rest + G::ROWS, (const E*)A.dr + (unit * 2 + 1) * C * A.vpad + c0, A.vpad, C, A.vpad - c0, 16);
+            }
             load_tile<E, C, GW>(m + 3 * G::ROWS, (const T*)A.v.p + row_at(A, A.v, s, sp, t0) + head * A.v.hs + c0, A.v.st, n, w, A.v.word);
             load_tile<E, GW, KD>(m + 4 * G::ROWS, (const E*)A.states + (unit * A.vdim + c0) * KS, KS, w, KD, 16);
             load_tile<E, GW, KD>(m + 4 * G::ROWS + G::STATE, (const E*)A.dstates + (unit * A.vdim + c0) * KS, KS, w, KD, 16);
@@ -181,22 +187,36 @@ __global__ void __launch_bounds__(GRADS, 1) k_delta_grads(const __grid_constant_
             __syncthreads();
             const E* m = blocks + (G::STAGES == 2 ? (b & 1) * G::BLOCK : 0);
             const E *Z = m, *U = m + G::ROWS, *R = m + 2 * G::ROWS, *V = m + 3 * G::ROWS, *S = m + 4 * G::ROWS, *D = S + G::STATE;
+            [[maybe_unused]] const E *UL = D + G::STATE, *RL = UL + G::ROWS;  // the second pieces
 #pragma unroll
             for (int k = 0; k < GW; k += 16) {
                 const typename Op::A az = Op::rows_of(Z + wr * 16 * RS + k, RS), ar = Op::rows_of(R + wr * 16 * RS + k, RS);
                 const typename Op::A au = Op::rows_of(U + wr * 16 * RS + k, RS);
+                typename Op::A rl, ul;
+                if constexpr (G::PLANES == 2) {
+                    rl = Op::rows_of(RL + wr * 16 * RS + k, RS);
+                    ul = Op::rows_of(UL + wr * 16 * RS + k, RS);
+                }
                 typename Op::B bb[2];
 #pragma unroll
                 for (int j = 0; j < NQ; j += 2) {
                     Op::by_columns(bb, S + k * KS + wc * (KD / 4) + j * 8, KS);
                     Op::mma(zq[j], zq[j + 1], az, bb);
+                    if constexpr (G::PLANES == 2) Op::mma(zk[j], zk[j + 1], rl, bb);
                     Op::mma(zk[j], zk[j + 1], ar, bb);
                     Op::by_columns(bb, D + k * KS + wc * (KD / 4) + j * 8, KS);
+                    if constexpr (G::PLANES == 2) Op::mma(zm[j], zm[j + 1], ul, bb);
                     Op::mma(zm[j], zm[j + 1], au, bb);
                 }
                 if (wc <= wr) {
+                    if constexpr (G::PLANES == 2) {
+                        Op::by_rows(bb, UL + wc * 16 * RS + k, RS);
+                        Op::mma(p[0], p[1], az, bb);
+                        Op::mma(x[0], x[1], ar, bb);
+                    }
                     Op::by_rows(bb, U + wc * 16 * RS + k, RS);
                     Op::mma(p[0], p[1], az, bb);
+                    if constexpr (G::PLANES == 2) Op::mma(x[0], x[1], rl, bb);
                     Op::mma(x[0], x[1], ar, bb);
                 }
             }
@@ -204,6 +224,7 @@ __global__ void __launch_bounds__(GRADS, 1) k_delta_grads(const __grid_constant_
             static_assert(C * GW / V4 == GRADS, "a word of R and V to a thread");
             const int at = (tid >> 3) * RS + (tid & 7) * V4;
             rv = word_dot(R + at, V + at, rv);
+            if constexpr (G::PLANES == 2) rv = word_dot(RL + at, V + at, rv);
 #pragma unroll
             for (int i = tid; i < GW * KD / V4; i += GRADS) {
                 const int e = i / (KD / V4) * KS + i % (KD / V4) * V4;

@@ -73,7 +73,7 @@ void launch_grads_of(const DeltaArgs& A, int warps, cudaStream_t st) {
 
 #define SNN_DELTA_LAUNCHES(T)                                                                        \
     template <> DeltaSizes delta_sizes<T>() {                                                        \
-        return {PathOf<T>::P::SQUARES, (int)sizeof(PathOf<T>::P::KE), (int)sizeof(Kept<T>::K)};                                   \
+        return {PathOf<T>::P::SQUARES, (int)sizeof(PathOf<T>::P::KE), (int)sizeof(Kept<T>::K), Kept<T>::PLANES};                                   \
     }                                                                                                \
     template <> void launch_prep<T>(const DeltaArgs& A, cudaStream_t st) { launch_prep_of<T>(A, st); } \
     template <> void launch_scan<T>(const DeltaArgs& A, int warps, cudaStream_t st) { launch_scan_of<T>(A, warps, st); } \

@@ -74,15 +74,19 @@ __device__ __forceinline__ void values_of(float (&o)[8][4], const T* v) {
 }
 // accumulators [16 columns, C steps] as n rows of T, the first w columns: through the warp's columns
 // of `stage` [C][ST]
-template <typename T, int ST>
+template <typename T, int ST, bool REST = false>  // REST: what rounding to T leaves of them
 __device__ __forceinline__ void store_tile(const float (&o)[8][4], T* stage, T* to, long long st, int n, int w, int word) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+    auto pair = [](float x, float y) {
+        if constexpr (REST) piece<T>(x, y);
+        return pair_of<T>(x, y);
+    };
     __syncwarp();
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
         for (int i = 0; i < 8; i += 2)
-            stsm4t(stage + (i * 8 + (lane >> 4) * 8 + (lane & 7)) * ST + ((lane >> 3) & 1) * 8, pair_of<T>(o[i][0], o[i][1]),
-                   pair_of<T>(o[i][2], o[i][3]), pair_of<T>(o[i + 1][0], o[i + 1][1]), pair_of<T>(o[i + 1][2], o[i + 1][3]));
+            stsm4t(stage + (i * 8 + (lane >> 4) * 8 + (lane & 7)) * ST + ((lane >> 3) & 1) * 8, pair(o[i][0], o[i][1]),
+                   pair(o[i][2], o[i][3]), pair(o[i + 1][0], o[i + 1][1]), pair(o[i + 1][2], o[i + 1][3]));
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -115,6 +119,7 @@ template <typename T, typename K, int ST>
 __device__ __forceinline__ void keep_tile(const float (&o)[8][4], T* stage, K* to, long long st, int w) {
     if constexpr (std::is_same<T, K>::value) {
         store_tile<T, ST>(o, stage, to, st, C, w, 16);
+        if constexpr (Kept<T>::PLANES == 2) store_tile<T, ST, true>(o, stage, to + C * st, st, C, w, 16);
     } else {  // f32 of f16 tensors
         const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
 #pragma unroll
@@ -400,7 +405,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_scan(const __grid_constant
                 }
                 store_tile<T, VS>(o, st.v + warp * 16, (T*)A.y.p + row_at(A, A.y, s, sp, c * C) + head * A.y.hs + col, A.y.st, n, w, A.y.word);
                 }
-                if (A.u && !A.only) keep_tile<T, K, VS>(u, st.v + warp * 16, (K*)A.u + unit * C * A.vpad + col, A.vpad, A.vpad - col);
+                if (A.u && !A.only) keep_tile<T, K, VS>(u, st.v + warp * 16, (K*)A.u + unit * Kept<T>::PLANES * C * A.vpad + col, A.vpad, A.vpad - col);
                 // S = since_64 S + (until u)^T K; 1 - since_64 keeps its bits where decays are near 1
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -499,7 +504,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_back(const __grid_constant
                         for (int e = 0; e < 4; ++e) r[j][e] = r[j][e] * f2 * f1;
                 }
                 // (dy's tile is not read any more)
-                keep_tile<T, K, VS>(r, st.v + warp * 16, (K*)A.dr + unit * C * A.vpad + col, A.vpad, A.vpad - col);
+                keep_tile<T, K, VS>(r, st.v + warp * 16, (K*)A.dr + unit * Kept<T>::PLANES * C * A.vpad + col, A.vpad, A.vpad - col);
                 // r = b R, u = -since b R, z = since Z, the last two times sigma / ks, sigma / qs
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {

@@ -63,7 +63,7 @@ struct DeltaArgs {
     char* keys;               // [slots, hk, 2, C, KD + PAD] of Path::KE: K and Q times their scales
     char* squares;            // [slots, heads] of Path::SQUARES bytes: planes of T, of P
     float* factors;           // [slots, heads, SC]
-    char *states, *u;         // saved: [slots, heads, vdim, KD + PAD], [slots, heads, C, vpad] of Kept
+    char *states, *u;         // saved: [slots, heads, vdim, KD + PAD], [slots, heads, PLANES, C, vpad] of Kept
     char *dstates, *dr;       // gradients' workspace: the same forms
     // sequences cut into `segs` segments of `seg` chunks (0: whole): where each starts from [n_seq, segs, heads, kdim,
     // vdim] (`only`: the run that makes them, and of those between the products of their steps [.., kdim, kdim])
@@ -480,8 +480,15 @@ __device__ __forceinline__ long long sequence_of(const DeltaArgs& A, long long s
 
 // what the gradient needs of states and U in which type: bf16 gradients are rounded to
 // 8 bits themselves
-template <typename T> struct Kept { using K = float; };
-template <> struct Kept<__nv_bfloat16> { using K = __nv_bfloat16; };
+// (U and R in two pieces there: they meet states that are rounded)
+template <typename T> struct Kept {
+    using K = float;
+    static constexpr int PLANES = 1;
+};
+template <> struct Kept<__nv_bfloat16> {
+    using K = __nv_bfloat16;
+    static constexpr int PLANES = 2;
+};
 
 // rows of no sequence become zero in y-like tensors
 template <typename T>
@@ -498,7 +505,7 @@ __device__ void zero_rest(const DeltaArgs& A, const Heads& r, int heads, int wid
 
 // ---- launches, one file per type -----------------------------------------------------
 struct DeltaSizes {
-    int squares, key, kept;   // bytes of T and P of a chunk, of an element of keys, of one kept for the gradient
+    int squares, key, kept, planes;  // bytes of T and P of a chunk, of an element of keys, of one kept for the gradient; planes of U
 };
 template <typename T> DeltaSizes delta_sizes();
 template <typename T> void launch_prep(const DeltaArgs& A, cudaStream_t st);
