@@ -14,7 +14,8 @@ namespace snnb_delta {
 // one piece of f16 for bf16 tensors, two for f16.  16 warps: 16 rows and a quarter
 // of the columns each; half of an SM's registers are accumulators, so that S, D, U, R and dy are
 // read once.  That leaves one CTA an SM, whose phases wait for one another: 8,192 chunks of 128 x 128
-// bf16 800 us (40 % of the issue slots, 22 % of the tensor pipe; 240 at the copy rate).
+// bf16 945 us (280 at the copy rate; 800 with U and R in one piece, whose gradients are off by
+// 2.5e-3 of their norm where these are by 1.9e-3 and the rounding alone makes 1.7e-3).
 struct Ops16 {                 // one piece of a 16-bit type E
     template <typename E>
     static __device__ __forceinline__ void rows_of(unsigned (&a)[4], const E* m, int st) {  // A[i][k] = m[i][k]
