@@ -36,9 +36,10 @@ constexpr int C = 64;         // steps of a chunk
 constexpr int MS = C + 8;     // row stride of [C, C] matrices in shared memory
 constexpr int PAD = 8;        // elements behind a row in shared memory: eight rows lie in different banks
 // T and P are lower triangular: row block b of 16 keeps its 16 (b + 1) columns and PAD
-constexpr int LOW = 3072;     // elements of such a matrix
+constexpr int LOW = C * (C + 16) / 2 + C * PAD;  // elements of such a matrix
 __host__ __device__ constexpr int low_at(int b) { return 128 * b * (b + 2); }
 __host__ __device__ constexpr int low_stride(int b) { return 16 * b + 16 + PAD; }
+static_assert(low_at(4) == LOW, "row blocks fill it");
 // floats of a chunk's factors: since, until, rate, those of Factor (scales of T and P by row
 // blocks); for the gradients the logarithms' sums in two parts and the counts of decays of 0
 enum Factor { LOST = 3 * C, K_SCALE, Q_SCALE, T_SCALE = LOST + 4, P_SCALE = LOST + 8, SCAN_FACTORS = LOST + 12,
