@@ -561,7 +561,8 @@ int snn_qk_norm_grad(const snn_qk* desc, const snn_heads* q, const snn_heads* k,
  *   y_t = scale S_t^T q_t
  * with a = exp(gate), b = beta, or with SNN_SCAN_LOGIT a = 1 / (1 + exp(-gate)),
  * b = 1 / (1 + exp(-beta)).  gate is a logarithm, so that decays near 1 keep their
- * memory; minus infinity forgets everything.  Keys of unit length and rates in
+ * memory; below -104 (minus infinity, the type's lowest value) the decay is 0 in f32: the
+ * step forgets every finite state and its gate has the gradient 0.  Keys of unit length and rates in
  * [0, 2] keep S bounded (snn_qk_norm with SNN_QK_UNIT); any are taken.
  * q, k: rows of k_heads x k_dim, v, y: of heads x v_dim, gate, beta: of heads;
  * head h reads key head h / (heads / k_heads).  All have element type `type`, unit

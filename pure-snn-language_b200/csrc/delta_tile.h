@@ -417,6 +417,10 @@ __device__ __forceinline__ float warp_top(const float (&x)[N][4]) {
 template <int N>
 __device__ __forceinline__ float warp_scale(const float (&x)[N][4]) { return scale_for(warp_top(x)); }
 
+// A decay whose logarithm lies below this is 0 in f32 (half of the smallest f32 is exp(-103.97)): the
+// step forgets everything.  Such logarithms may be as low as the type goes and stay out of all sums.
+constexpr float FORGETS = -104.0f;
+
 // By one warp: sums of the logarithms of a chunk's decays (64 bits, kept as two f32 of
 // their binary logarithms: differences of them are what counts) but for those of decays of
 // 0, which are counted apart, and the rates.  In the last lane's `lost` 1 - the chunk's decay.
@@ -433,7 +437,7 @@ __device__ __forceinline__ void chunk_decays(const DeltaArgs& A, long long s, co
             lg = log_decay(A, ((const T*)A.gate.p)[row_at(A, A.gate, s, sp, t0 + t) + head * A.gate.hs]);
             r = rate_of(A, ((const T*)A.beta.p)[row_at(A, A.beta, s, sp, t0 + t) + head * A.beta.hs]);
         }
-        z[i] = lg == -INFINITY;
+        z[i] = lg < FORGETS;
         l[i] = z[i] ? 0.0 : (double)lg;
         rate[t] = r;
     }

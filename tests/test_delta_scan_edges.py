@@ -1,0 +1,38 @@
+"""snn_delta_scan and snn_delta_scan_grad at the borders of what their chunks take: gates that forget everything,
+sequences cut into segments, workspaces.  64-bit forms and bounds in delta_ref."""
+import numpy as np
+import pytest
+
+import delta_ref as ref
+import snn_b200 as snn
+from test_delta_scan import KINDS, host, make
+
+GRADS = ("dq", "dk", "dv", "dgate", "dbeta", "dh0")
+
+
+# ---- gates that forget -----------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("t", [5, 9, 150])
+@pytest.mark.parametrize("logit", [False, True])
+@pytest.mark.parametrize("low", [-1e2, -103.9, -104.5, -1e4, -1e13, -1e15, -1e30, "lowest"])
+def test_finite_gates_that_forget(kind, t, logit, low):
+    """A gate far below zero, down to the type's lowest value, is a decay of 0 and nothing else: what comes after it
+    decays by its own gates, and it gets no gradient."""
+    import torch
+    x, s0, dy, dh = make(21, (2, t), 1, 2, 24, 20, kind, logit)
+    lowest = torch.finfo(x[3].dtype).min
+    at = [0, 3, 4] if t < 64 else [0, 3, 4, 40, 63, 64, 100, 149]
+    for i in at:
+        x[3][0, i] = lowest if low == "lowest" else max(low, lowest)
+    want = ref.run(*map(host, x), host(s0), dy=host(dy), dh=host(dh), kind=kind, logit=logit)
+    y, h = snn.delta_scan(*x, s0, logit=logit)
+    ref.close(host(y), want["y"], kind, "y")
+    ref.close(host(h), want["h"], kind, "h")
+    y, h, saved = snn.delta_scan(*x, s0, logit=logit, save=True)
+    ref.close(host(y), want["y"], kind, "y")
+    ref.close(host(h), want["h"], kind, "h")
+    for name, g in zip(GRADS, snn.delta_scan_grad(*x, dy, saved, dh=dh, logit=logit)):
+        ref.close(host(g), want[name], kind, name)
+        if name == "dgate" and low not in (-1e2, -103.9):
+            assert (g[0, at] == 0).all()
