@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_scan(const __grid_constant
     const int head = blockIdx.y, col0 = ((int)blockIdx.z - (unit_run ? A.tiles : 0)) * St::VW, col = col0 + warp * 16;
     const int vdim = unit_run ? A.kdim : A.vdim, w = vdim - col;  // w: this warp's columns (16 and more: all; none: it only loads)
     Heads values = A.v;
-    if (unit_run) values.p = nullptr;
+    if (unit_run) values = {nullptr, 0, 0, 0, 16};  // (copies of nothing have an aligned address all the same)
     for (long long item = blockIdx.x; item < A.n_seq * A.segs; item += gridDim.x) {
         const long long s = item / A.segs;
         const int segment = (int)(item - s * A.segs);

@@ -36,3 +36,25 @@ def test_finite_gates_that_forget(kind, t, logit, low):
         ref.close(host(g), want[name], kind, name)
         if name == "dgate" and low not in (-1e2, -103.9):
             assert (g[0, at] == 0).all()
+
+
+# ---- sequences cut into segments ---------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("dk,dv", [(40, 33), (64, 100), (100, 7)])
+@pytest.mark.parametrize("packed", [False, True])
+def test_segments_of_odd_rows(kind, dk, dv, packed):
+    """Values whose rows and heads lie at addresses of any alignment, packed sequences that begin at odd rows."""
+    import torch
+    lengths = [2101, 2499]
+    if packed:
+        off = np.concatenate([[1], 1 + np.cumsum(lengths)])
+        x, s0, _, _ = make(31, (int(off[-1]) + 2,), 1, 2, dk, dv, kind, n_seq=2)
+    else:
+        off = None
+        x, s0, _, _ = make(32, (2, 2101), 1, 2, dk, dv, kind)
+    how = dict(scale=0.3)
+    want = ref.run(*map(host, x), host(s0), offsets=None if off is None else off.tolist(), kind=kind, **how)
+    y, h = snn.delta_scan(*x, s0, offsets=None if off is None else torch.tensor(off, device="cuda"), **how)
+    ref.close(host(y), want["y"], kind, "y")
+    ref.close(host(h), want["h"], kind, "h")
