@@ -332,8 +332,12 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_scan(const __grid_constant
 #pragma unroll
                 for (int e = 0; e < 4; ++e) S[i][e] = col + g + (e >> 1) * 8 == i * 8 + 2 * t4 + (e & 1) ? 1.0f : 0.0f;
         } else {
-            read_state<NT>(S, segment == 0 ? (A.h0 ? A.h0 + (s * A.heads + head) * size : nullptr)
-                                           : (A.only ? nullptr : A.starts + (item * A.heads + head) * size), A, col, vdim);
+            // (h may be h0: where another CTA writes h, that is, behind other segments, segment 0 takes what the first run left
+            // of h0 for it)
+            float* start = A.segs > 1 ? A.starts + (item * A.heads + head) * size : nullptr;
+            const bool from_h0 = segment == 0 && (A.only || last);
+            read_state<NT>(S, from_h0 ? (A.h0 ? A.h0 + (s * A.heads + head) * size : nullptr) : (A.only ? nullptr : start), A, col, vdim);
+            if (A.only && segment == 0 && w > 0) write_state<NT>(S, 1.0f, start, A, col, vdim);
         }
         if (St::STAGES == 2 && chunks > first) St(smem + (first & 1) * St::BYTES).load(A, values, s, sp, first, head, col0, vdim, tid);
         copies_end();

@@ -58,3 +58,26 @@ def test_segments_of_odd_rows(kind, dk, dv, packed):
     y, h = snn.delta_scan(*x, s0, offsets=None if off is None else torch.tensor(off, device="cuda"), **how)
     ref.close(host(y), want["y"], kind, "y")
     ref.close(host(h), want["h"], kind, "h")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("lengths", [[2500], [64 * 36 + 1] * 3, [9000, 0, 3, 64 * 40, 64 * 23]])
+def test_segments_with_the_state_in_place(kind, lengths):
+    """h_out may be h0: the same bits as with another h, where sequences are cut, short ones and ones whose
+    last segment is one chunk among them."""
+    import torch
+    off = torch.tensor(np.concatenate([[0], np.cumsum(lengths)]), device="cuda")
+    x, s0, _, _ = make(33, (sum(lengths),), 1, 2, 64, 128, kind, n_seq=len(lengths))
+    if lengths[:1] == lengths[-1:]:  # equal ones as a dense batch too
+        dense = [v.unflatten(0, (len(lengths), -1)) for v in x]
+        y, h = snn.delta_scan(*dense, s0)
+        for _ in range(3):
+            state = s0.clone()
+            y2, h2 = snn.delta_scan(*dense, state, h_out=state)
+            assert h2 is state and torch.equal(y2, y) and torch.equal(state, h)
+    y, h = snn.delta_scan(*x, s0, offsets=off)
+    for _ in range(3):
+        state = s0.clone()
+        y2, _ = snn.delta_scan(*x, state, offsets=off, h_out=state)
+        assert torch.equal(y2, y) and torch.equal(state, h)
