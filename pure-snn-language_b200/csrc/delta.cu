@@ -153,8 +153,10 @@ __global__ void __launch_bounds__(256) k_delta_join(const __grid_constant__ Delt
     const int tid = threadIdx.x, head = blockIdx.y, c0 = (int)blockIdx.z * JOIN_COLS;
     const int d = tid >> 1, c = (tid & 1) * 8, kdim = A.kdim, kpad = (kdim + 3) / 4 * 4;
     const long long s = blockIdx.x, size = (long long)kdim * A.vdim;
-    const int all = (span_of(A, s).len + C - 1) / C, last = (all + A.seg - 1) / A.seg - 1;
-    auto unit = [&](int g) { return (s * A.segs + g) * A.heads + head; };
+    const Span sp = span_of(A, s);
+    const long long first = item_at(A, s, sp);
+    const int all = (sp.len + C - 1) / C, last = (all + A.seg - 1) / A.seg - 1;
+    auto unit = [&](int g) { return (first + g) * A.heads + head; };
     auto load = [&](int g) {
         const float* M = A.maps + unit(g) * kdim * kdim;
         float* to = join + (g & 1) * MAX_K * JOIN_ROW;
@@ -280,22 +282,24 @@ struct Layout {
     int64_t keys, factors, states, u, all, kept_all;
     int64_t starts, maps, cut;  // of a workspace for segments: their offsets in it, its size
 };
-// Chunks of a segment, and how many segments a sequence has at most (1: whole).  Few heads leave
+// Chunks of a segment (0: sequences stay whole) and how many segments there are (packed: at most).  Few heads leave
 // most SMs empty for long: then sequences are cut, a first run makes what each segment makes of no
 // state and the product of its steps (twice the columns, no results), those are joined, and all segments
 // run at once.  That is 2.7 times the work (about), so it takes four segments and more, as many as
 // give every SM eight warps; a segment has at least 8 chunks.  1 x 16,384 steps x 16 heads of 128 x 128 f16: whole
 // 1,300 us, by 8 segments 361 + 40 + 281.  Packed sequences may be of any lengths: segments are of the mean's
-// size, and a sequence has as many as all rows would fill.
-void segments_of(const snn_delta* d, int& seg, int& segs) {
-    seg = 0;
-    segs = 1;
+// size, and numbered as their chunks are, by their rows' place.
+struct Cut {
+    int seg;
+    int64_t items;
+};
+Cut segments_of(const snn_delta* d) {
     const int64_t chunks = (mean_steps(d) + C - 1) / C, warps = d->n_seq * d->heads * ((d->v_dim + 15) / 16);
     int64_t g = 1;
     while (g < 16 && warps * g * 2 <= 8 * SMS && chunks >= 16 * g) g *= 2;
-    if (g < 4 || d->n_seq > 64) return;
-    seg = (int)((chunks + g - 1) / g);
-    segs = (int)(d->offsets ? (d->n_steps / C + 1) / seg + 1 : (chunks + seg - 1) / seg);
+    if (g < 4 || d->n_seq > 64) return {0, d->n_seq};
+    const int64_t seg = (chunks + g - 1) / g;
+    return {(int)seg, d->offsets ? d->n_steps / (seg * C) + d->n_seq : d->n_seq * ((chunks + seg - 1) / seg)};
 }
 Layout layout_of(const snn_delta* d) {
     const DeltaSizes z = sizes_of(d);
@@ -306,11 +310,10 @@ Layout layout_of(const snn_delta* d) {
     l.all = l.states = l.factors + round256(units * SC * 4);
     l.u = l.states + round256(units * d->v_dim * (kd + PAD) * z.kept);
     l.kept_all = l.u + round256(units * z.planes * C * vpad_of(d) * z.kept);
-    int seg, segs;
-    segments_of(d, seg, segs);
+    const Cut cut = segments_of(d);
     l.starts = 0;
-    l.maps = segs > 1 ? round256(d->n_seq * segs * d->heads * d->k_dim * d->v_dim * 4) : 0;
-    l.cut = segs > 1 ? l.maps + round256(d->n_seq * segs * d->heads * d->k_dim * d->k_dim * 4) : 0;
+    l.maps = cut.seg ? round256(cut.items * d->heads * d->k_dim * d->v_dim * 4) : 0;
+    l.cut = cut.seg ? l.maps + round256(cut.items * d->heads * d->k_dim * d->k_dim * 4) : 0;
     return l;
 }
 // Up to 8 steps one by one (64 x 8 heads of 128 x 128 bf16, us by 4 and 8 steps: 32, 55; as a chunk 74)
@@ -339,7 +342,7 @@ DeltaArgs base_args(const snn_delta* d, const snn_heads* q, const snn_heads* k, 
     A.logit = (d->flags & SNN_SCAN_LOGIT) != 0;
     A.zero = d->offsets && (d->flags & SNN_SCAN_ZERO) != 0;
     A.scale = d->scale;
-    A.segs = 1;
+    A.items = d->n_seq;
     return A;
 }
 void zero_rows(const snn_delta* d, const DeltaArgs& A, const Heads& r, int heads, int width, cudaStream_t st) {
@@ -352,11 +355,11 @@ void zero_rows(const snn_delta* d, const DeltaArgs& A, const Heads& r, int heads
 // serve its warps, each with 16 columns of the state.  Up to four warps have a tensor core
 // each (5.1 us a chunk of 128 x 16, f16); eight share them (7.3), but CTAs that do not fit on
 // the SMs at once are a second round.
-int warps_of(const snn_delta* d, int64_t segs) {
+int warps_of(const snn_delta* d, int64_t items) {
     int best = 1;
     double least = 1e300;
     for (int nw = 1; nw <= 8; nw *= 2) {
-        const int64_t ctas = d->n_seq * segs * d->heads * ((d->v_dim + 16 * nw - 1) / (16 * nw));
+        const int64_t ctas = items * d->heads * ((d->v_dim + 16 * nw - 1) / (16 * nw));
         const double cost = (double)((ctas + SMS - 1) / SMS) * (nw == 8 ? 1.45 : 1.0);
         if (nw > 1 && 16 * nw >= 2 * d->v_dim) break;  // no warp without columns where fewer do
         if (cost <= least) {
@@ -421,13 +424,15 @@ void delta_scan(const snn_delta* d, const snn_heads* q, const snn_heads* k, cons
         A.states = base + l.states;
         A.u = base + l.u;
     }
-    segments_of(d, A.seg, A.segs);
+    const Cut cut = segments_of(d);
+    A.seg = cut.seg;
+    A.items = cut.items;
     A.starts = (float*)work;
     A.maps = (float*)((char*)work + l.maps);
     with_elem(d->type, [&](auto t) {
         using T = decltype(t);
         if (A.slots) launch_prep<T>(A, st);
-        if (A.segs > 1) {
+        if (A.seg) {
             A.only = 1;
             launch_scan<T>(A, 8, st);
             A.only = 0;
@@ -436,7 +441,7 @@ void delta_scan(const snn_delta* d, const snn_heads* q, const snn_heads* k, cons
             k_delta_join<<<grid, 256, JOIN_SMEM, st>>>(A);
             SNN_CUDA(cudaGetLastError());
         }
-        launch_scan<T>(A, warps_of(d, A.segs), st);
+        launch_scan<T>(A, warps_of(d, A.items), st);
     });
 }
 
@@ -484,7 +489,7 @@ void delta_scan_grad(const snn_delta* d, const snn_heads* q, const snn_heads* k,
     A.u = base + l.u;
     A.dstates = (char*)work;
     A.dr = (char*)work + (l.u - l.states);
-    with_elem(d->type, [&](auto t) { launch_grads<decltype(t)>(A, warps_of(d, 1), st); });
+    with_elem(d->type, [&](auto t) { launch_grads<decltype(t)>(A, warps_of(d, d->n_seq), st); });
 }
 
 }  // namespace snnb

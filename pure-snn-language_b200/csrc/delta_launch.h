@@ -40,7 +40,7 @@ void launch_scan_of(const DeltaArgs& A, int warps, cudaStream_t st) {
             const int tiles = (A.vdim + S::VW - 1) / S::VW;
             DeltaArgs B = A;
             B.tiles = tiles;
-            const dim3 grid((unsigned)std::min<long long>(A.n_seq * A.segs, 1 << 30), (unsigned)A.heads,
+            const dim3 grid((unsigned)std::min<long long>(A.items, 1 << 30), (unsigned)A.heads,
                             (unsigned)(A.only ? tiles + (A.kdim + S::VW - 1) / S::VW : tiles));
             kernel<<<grid, NW * 32, S::SMEM, st>>>(B);
         });

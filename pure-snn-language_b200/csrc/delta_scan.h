@@ -315,10 +315,11 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_scan(const __grid_constant
     const int vdim = unit_run ? A.kdim : A.vdim, w = vdim - col;  // w: this warp's columns (16 and more: all; none: it only loads)
     Heads values = A.v;
     if (unit_run) values = {nullptr, 0, 0, 0, 16};  // (copies of nothing have an aligned address all the same)
-    for (long long item = blockIdx.x; item < A.n_seq * A.segs; item += gridDim.x) {
-        const long long s = item / A.segs;
-        const int segment = (int)(item - s * A.segs);
+    for (long long item = blockIdx.x; item < A.items; item += gridDim.x) {
+        const long long s = sequence_of_item(A, item);
         const Span sp = span_of(A, s);
+        const int segment = (int)(item - item_at(A, s, sp));
+        if (segment < 0) continue;  // of no sequence
         const int all = (sp.len + C - 1) / C, first = segment * A.seg;
         const int chunks = A.seg ? min(all, first + A.seg) : all;  // the first one that is not this segment's
         const bool last = segment == (A.seg ? max(0, (all + A.seg - 1) / A.seg - 1) : 0);
@@ -334,7 +335,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_scan(const __grid_constant
         } else {
             // (h may be h0: where another CTA writes h, that is, behind other segments, segment 0 takes what the first run left
             // of h0 for it)
-            float* start = A.segs > 1 ? A.starts + (item * A.heads + head) * size : nullptr;
+            float* start = A.seg ? A.starts + (item * A.heads + head) * size : nullptr;
             const bool from_h0 = segment == 0 && (A.only || last);
             read_state<NT>(S, from_h0 ? (A.h0 ? A.h0 + (s * A.heads + head) * size : nullptr) : (A.only ? nullptr : start), A, col, vdim);
             if (A.only && segment == 0 && w > 0) write_state<NT>(S, 1.0f, start, A, col, vdim);

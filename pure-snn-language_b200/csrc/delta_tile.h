@@ -66,9 +66,11 @@ struct DeltaArgs {
     float* factors;           // [slots, heads, SC]
     char *states, *u;         // saved: [slots, heads, vdim, KD + PAD], [slots, heads, PLANES, C, vpad] of Kept
     char *dstates, *dr;       // gradients' workspace: the same forms
-    // sequences cut into `segs` segments of `seg` chunks (0: whole): where each starts from [n_seq, segs, heads, kdim,
-    // vdim] (`only`: the run that makes them, and of those between the products of their steps [.., kdim, kdim])
-    int seg, segs, only, tiles;  // tiles: CTAs along the values' columns
+    // sequences cut into segments of `seg` chunks (0: whole), `items` in all (packed: at most): where each starts from
+    // [items, heads, kdim, vdim] (`only`: the run that makes them, and of those between the products of their steps [..,
+    // kdim, kdim])
+    int seg, only, tiles;     // tiles: CTAs along the values' columns
+    long long items;
     float *starts, *maps;
 };
 
@@ -81,6 +83,22 @@ __device__ __forceinline__ Span span_of(const DeltaArgs& A, long long s) {
     if (!A.off) return {0, A.n_steps, s * ((A.n_steps + C - 1) / C)};
     const long long n = A.n_steps, b = min(max((long long)A.off[s], 0ll), n), e = min(max((long long)A.off[s + 1], b), n);
     return {b, (int)(e - b), b / C + s};
+}
+// the first item of sequence s, which has one at least
+__device__ __forceinline__ long long item_at(const DeltaArgs& A, long long s, const Span& sp) {
+    if (!A.seg) return s;
+    return A.off ? sp.start / (A.seg * (long long)C) + s : s * (((A.n_steps + C - 1) / C + A.seg - 1) / A.seg);
+}
+// the sequence that an item belongs to: the last one whose first item is not behind it (by a whole warp)
+__device__ __forceinline__ long long sequence_of_item(const DeltaArgs& A, long long item) {
+    if (!A.seg) return item;
+    if (!A.off) return item / (((A.n_steps + C - 1) / C + A.seg - 1) / A.seg);
+    long long before = 0;
+    for (long long base = 0; base < A.n_seq; base += 32) {
+        const long long s = base + (threadIdx.x & 31);
+        before += __popc(__ballot_sync(~0u, s < A.n_seq && item_at(A, s, span_of(A, s)) <= item));
+    }
+    return max(before - 1, 0ll);
 }
 __device__ __forceinline__ long long row_at(const DeltaArgs& A, const Heads& h, long long s, const Span& sp, int t) {
     return A.off ? (sp.start + t) * h.st : s * h.ss + t * h.st;

@@ -1,5 +1,7 @@
 """snn_delta_scan and snn_delta_scan_grad at the borders of what their chunks take: gates that forget everything,
 sequences cut into segments, workspaces.  64-bit forms and bounds in delta_ref."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -39,6 +41,26 @@ def test_finite_gates_that_forget(kind, t, logit, low):
 
 
 # ---- sequences cut into segments ---------------------------------------------------------
+
+def sizes(packed, n_seq, n_steps, heads, dk, dv, saved):
+    desc, n = snn._DELTA.pack(1, 0, n_seq, n_steps, heads, heads, dk, dv, 8 if packed else 0, 1.0, 0), C.c_int64()
+    assert snn.lib().snn_delta_scan_workspace(desc, saved, C.byref(n)) == 0
+    return n.value
+
+
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("n_seq,mean,heads,dk,dv", [(64, 8192, 1, 128, 16), (1, 16384, 16, 128, 128), (3, 2500, 1, 20, 36),
+                                                   (50, 5000, 1, 128, 8), (12, 20000, 2, 96, 100), (64, 16400, 1, 64, 1)])
+def test_workspace_of_segments(packed, n_seq, mean, heads, dk, dv):
+    """A segment is 8 chunks of 64 steps at least, and a sequence has one that is not full at most: a state and the
+    product of its steps each, whether the sequences are packed or not."""
+    n_steps = mean * n_seq if packed else mean
+    cut = sizes(packed, n_seq, n_steps, heads, dk, dv, 1)
+    assert 0 < cut <= (mean * n_seq // 512 + n_seq) * heads * dk * (dv + dk) * 4 + 512
+    # no more beside it than what is kept of all chunks (keys and queries, T and P: 40 kB and 1 kB of factors at most)
+    assert sizes(packed, n_seq, n_steps, heads, dk, dv, 0) - cut <= (mean * n_seq // 64 + n_seq) * heads * 90000
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", list(KINDS))
 @pytest.mark.parametrize("dk,dv", [(40, 33), (64, 100), (100, 7)])
@@ -81,3 +103,25 @@ def test_segments_with_the_state_in_place(kind, lengths):
         state = s0.clone()
         y2, _ = snn.delta_scan(*x, state, offsets=off, h_out=state)
         assert torch.equal(y2, y) and torch.equal(state, h)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lengths", [[2100 + 37 * i for i in range(40)], [0] * 20 + [70000] + [1] * 10, [64 * 700, 1, 640, 639, 641, 0]])
+def test_segments_of_many_packed_sequences(lengths):
+    """Many sequences, and very unequal ones, cut by their rows' place: the same as each sequence alone."""
+    import torch
+    off = np.concatenate([[700], 700 + np.cumsum(lengths)])
+    x, s0, _, _ = make(34, (int(off[-1]) + 1000,), 1, 1, 32, 16, "f32", n_seq=len(lengths))
+    y, h = snn.delta_scan(*x, s0, offsets=torch.tensor(off, device="cuda"))
+    assert (y[:700] == 0).all() and (y[off[-1]:] == 0).all()
+    _, h1, _ = snn.delta_scan(*x, s0, offsets=torch.tensor(off, device="cuda"), save=True)
+    assert torch.equal(h1, h)
+    for i, n in enumerate(lengths):
+        if n == 0:
+            assert torch.equal(h[i], s0[i])
+            continue
+        want = ref.run(*(host(v[off[i]:off[i + 1]][-300:]) for v in x), np.zeros((1, 1, 32, 16)), offsets=[0, min(n, 300)])
+        alone = snn.delta_scan(*(v[off[i]:off[i + 1]][None] for v in x), s0[i:i + 1])
+        # two ways of cutting: each is off the 64-bit form by what `far` says of its last 300 steps, which forget the rest
+        far = max(want["h"][1], want["y"][1])
+        assert (y[off[i]:off[i + 1]] - alone[0][0]).abs().max() <= 8 * far and (h[i] - alone[1][0]).abs().max() <= 8 * far
