@@ -848,7 +848,9 @@ class AdamW:
     for each parameter a bfloat16 or float16 tensor that takes its rounded
     values (entries may be None).  The moments are the lists m and v (with
     8 bits float8_e4m3fn, their scales in m_scale and v_scale), zeros at
-    first; moments=(m, v, m_scale, v_scale) takes those of an earlier run over."""
+    first; moments=(m, v, m_scale, v_scale) takes those of an earlier run over.
+    All these tensors stay where they are: a step refuses one that has been replaced
+    or has moved (m[i].copy_(..) restores a moment)."""
 
     def __init__(self, params, bits=32, copies=None, moments=None):
         T = _torch()
@@ -866,7 +868,7 @@ class AdamW:
         self.copies = [None] * n if copies is None else list(copies)
         _require(all(len(x) == n for x in (self.m, self.v, self.m_scale, self.v_scale, self.copies)),
                  "moments, scales and copies are as many as the parameters")
-        self._table, used = np.zeros(n, _ADAMW_TENSOR), []
+        self._table, used, self._held = np.zeros(n, _ADAMW_TENSOR), [], []
         for i, p in enumerate(self.params):
             held = [("p", p, p.shape, T.float32), ("m", self.m[i], p.shape, kind), ("v", self.v[i], p.shape, kind)]
             if bits == 8:
@@ -880,22 +882,33 @@ class AdamW:
                 _require(t.is_cuda and t.device == dev and t.shape == shape and t.dtype == dtype and t.is_contiguous(),
                          f"{name} of parameter {i} must be a contiguous CUDA tensor {tuple(shape)} in {dtype} on {dev}")
                 self._table[name][i] = t.data_ptr()
+                self._held.append(t.detach())  # (while this holds it, its memory becomes nothing else's)
                 if t.numel():
                     used.append((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()))
             self._table["n"][i] = p.numel()
         used.sort()
         _require(all(a[1] <= b[0] for a, b in zip(used, used[1:])), "parameters, moments, scales or copies overlap")
-        self._shapes, self._at = [p.shape for p in self.params], [p.data_ptr() for p in self.params]
+        self._shapes, self._at, self._table_at = [p.shape for p in self.params], self._addresses(), self._table.ctypes.data
+
+    def _addresses(self):
+        """Where all that a step writes lies now."""
+        try:
+            held = self.params + self.m + self.v
+            if self.bits == 8:
+                held += self.m_scale + self.v_scale
+            return list(map(_T.Tensor.data_ptr, held)) + [0 if t is None else t.data_ptr() for t in self.copies]
+        except (AttributeError, TypeError):  # something else than a tensor
+            return None
 
     def step(self, grads, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, grad_scale=1.0, stream=None):
         """One step, in place: grads, one for each parameter (contiguous, float32 / bfloat16
         / float16, its shape; None leaves a parameter and its moments alone); step, counted from 1, a
         number or an int64 CUDA tensor of one element, which is read when the step
         runs (for captured steps)."""
-        dev, table = self.device, self._table.copy()
+        dev, table = self.device, self._table  # (the call reads it before it returns)
         _require(len(grads) == len(self._shapes), "grads are as many as the parameters")
-        if [p.data_ptr() for p in self.params] != self._at:
-            raise SnnError(1, "a parameter's memory is not what it was when this was made")
+        if self._addresses() != self._at:
+            raise SnnError(1, "a parameter's, moment's, scale's or copy's memory is not what it was when this was made")
         at, kinds = [], []
         for g, shape in zip(grads, self._shapes):
             if g is None:
@@ -913,7 +926,7 @@ class AdamW:
             _require(step.dtype == _T.int64 and step.numel() == 1, "step must be a number or one int64")
             there, step = step.data_ptr(), 0
         rule = _ADAMW_RULE.pack(lr, *betas, eps, weight_decay, grad_scale, step, there)
-        _call(lib().snn_adamw, dev, stream, table.ctypes.data, len(table), self.bits, rule)
+        _call(lib().snn_adamw, dev, stream, self._table_at, len(at), self.bits, rule)
 
 
 def nccl_unique_id():

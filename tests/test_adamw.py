@@ -207,3 +207,42 @@ def test_binding_refuses():
                 lambda: opt.step(p, torch.ones(1, device="cuda"))):
         with pytest.raises(snn.SnnError):
             bad()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_what_has_been_replaced_or_moved_is_refused(bits):
+    """A step writes parameters, moments, scales and copies: none of them through an address that is no longer theirs."""
+    import torch
+    p = [torch.ones(300, device="cuda"), torch.ones(7, 5, device="cuda")]
+    opt = snn.AdamW(p, bits=bits, copies=[None, torch.zeros(7, 5, device="cuda").half()])
+    g = [torch.ones(300, device="cuda"), torch.ones(7, 5, device="cuda")]
+    opt.step(g, 1)
+    for name in ("m", "v", "copies", "params") + (("m_scale", "v_scale") if bits == 8 else ()):
+        entries = getattr(opt, name)
+        for change in ("entry", "memory", "list", "none", "length"):
+            before, t = [x.clone() for x in p], entries[1]
+            was = t.data
+            if change == "entry":
+                entries[1] = t.clone()
+            elif change == "memory":
+                t.data = t.clone()
+            elif change == "list":
+                setattr(opt, name, [None if x is None else x.clone() for x in entries])
+            elif change == "none":
+                entries[1] = None
+            else:
+                entries.append(t)
+            with pytest.raises(snn.SnnError):
+                opt.step(g, 2)
+            assert all(torch.equal(a, b) for a, b in zip(before, p))
+            t.data = was
+            entries[1:] = [t]
+            setattr(opt, name, entries)
+    opt.copies[:] = opt.copies[::-1]
+    with pytest.raises(snn.SnnError):
+        opt.step(g, 2)
+    opt.copies[:] = opt.copies[::-1]
+    opt.m[1].copy_(opt.m[1].clone())
+    opt.step(g, 2)
+    assert (p[1] != 1).all()
