@@ -243,7 +243,8 @@ int64_t mean_steps(const snn_delta* d) { return d->offsets ? d->n_steps / std::m
 
 Heads heads_of(const snn_delta* d, const snn_heads* h, int64_t heads, int64_t width, const char* name, bool written = false) {
     const int size = snnb::elem_size(d->type);
-    SNN_REQUIRE(h && (h->data || d->n_steps == 0), SNN_ERR_ARG, std::string("delta: null ") + name);
+    const bool rows = d->n_steps > 0 && (d->offsets || d->n_seq > 0);
+    SNN_REQUIRE(h && (h->data || !rows), SNN_ERR_ARG, std::string("delta: null ") + name);
     SNN_REQUIRE((uintptr_t)h->data % size == 0, SNN_ERR_ARG, std::string("delta: misaligned ") + name);
     const int64_t seqs = d->offsets ? 1 : d->n_seq, most = 1ll << 46;
     const int64_t ss = seqs > 1 ? h->seq_stride : 0, st = d->n_steps > 1 ? h->step_stride : 0, hs = heads > 1 ? h->head_stride : 0;
@@ -460,7 +461,7 @@ void delta_scan_grad(const snn_delta* d, const snn_heads* q, const snn_heads* k,
                      const snn_heads* dq, const snn_heads* dk, const snn_heads* dv, const snn_rows* dgate,
                      const snn_rows* dbeta, float* dh0, void* work, int64_t work_bytes, cudaStream_t st) {
     check_desc(d);
-    SNN_REQUIRE(dy || dh, SNN_ERR_ARG, "delta: neither dy nor dh");
+    SNN_REQUIRE(dy || dh || d->n_seq == 0, SNN_ERR_ARG, "delta: neither dy nor dh");
     DeltaArgs A = base_args(d, q, k, v, gate, beta);
     if (dy) A.dy = heads_of(d, dy, d->heads, d->v_dim, "dy");
     else A.dy.word = 16;

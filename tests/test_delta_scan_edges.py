@@ -7,7 +7,7 @@ import pytest
 
 import delta_ref as ref
 import snn_b200 as snn
-from test_delta_scan import KINDS, host, make
+from test_delta_scan import KINDS, call, host, make
 
 GRADS = ("dq", "dk", "dv", "dgate", "dbeta", "dh0")
 
@@ -125,3 +125,30 @@ def test_segments_of_many_packed_sequences(lengths):
         # two ways of cutting: each is off the 64-bit form by what `far` says of its last 300 steps, which forget the rest
         far = max(want["h"][1], want["y"][1])
         assert (y[off[i]:off[i + 1]] - alone[0][0]).abs().max() <= 8 * far and (h[i] - alone[1][0]).abs().max() <= 8 * far
+
+
+# ---- no sequence ---------------------------------------------------------------------------
+NOTHING = {n: None for n in ("h0", "h", "dh", "dh0", "saved", "work")} | {n: (None, 0, 16, 8) for n in ("q", "k", "v", "y", "dy", "dq", "dk", "dv")}
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_a_batch_of_no_sequence(grad):
+    """Tensors without elements have no address: a dense batch of no sequence is nothing to do."""
+    over = NOTHING | {n: (None, 400, 4) for n in ("gate", "beta", "dgate", "dbeta")}
+    assert call(grad=grad, desc=dict(n_seq=0), bytes=0, sbytes=0, **over) == 0
+    assert call(grad=grad, desc=dict(n_seq=1), bytes=0, sbytes=0, **over) == 1
+    if grad:  # (gradients of the final states of none)
+        assert call(grad=True, desc=dict(n_seq=0), bytes=0, sbytes=0, **(over | dict(dy=None))) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [1, 20])
+def test_a_batch_of_no_sequence_through_the_binding(t):
+    import torch
+    x, s0, dy, dh = make(1, (0, t), 2, 4, 8, 12, "bf16")
+    y, h, saved = snn.delta_scan(*x, s0, save=True)
+    assert y.shape == (0, t, 4, 12) and h.shape == (0, 4, 8, 12)
+    assert [tuple(g.shape) for g in snn.delta_scan_grad(*x, dy, saved, dh=dh)] == [
+        (0, t, 2, 8), (0, t, 2, 8), (0, t, 4, 12), (0, t, 4), (0, t, 4), (0, 4, 8, 12)]
+    assert snn.delta_scan_grad(*x, None, saved, dh=dh)[5].shape == s0.shape
+    assert snn.delta_scan(*x)[0].shape == (0, t, 4, 12)
