@@ -152,3 +152,10 @@ def test_a_batch_of_no_sequence_through_the_binding(t):
         (0, t, 2, 8), (0, t, 2, 8), (0, t, 4, 12), (0, t, 4), (0, t, 4), (0, 4, 8, 12)]
     assert snn.delta_scan_grad(*x, None, saved, dh=dh)[5].shape == s0.shape
     assert snn.delta_scan(*x)[0].shape == (0, t, 4, 12)
+
+
+@pytest.mark.parametrize("over", [dict(saved=None), dict(saved=(1 << 30) + 8), dict(sbytes=64), dict(work=None), dict(bytes=64)])
+def test_grad_refuses_before_it_writes(over):
+    """Nothing has been launched, not even the zeros of rows of no sequence, when an argument is refused (without a GPU
+    any launch would be another error)."""
+    assert call(grad=True, desc=dict(off=4096, flags=snn.SCAN_ZERO, n_seq=3), **over) == 1
