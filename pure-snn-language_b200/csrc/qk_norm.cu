@@ -469,7 +469,6 @@ void qk_norm_grad(const snn_qk* d, const snn_heads* q, const snn_heads* k, const
     for (int i = 0; i < 2; ++i) {
         check_weight(w[i]);
         check_weight(dw[i]);
-        if (dw[i] && (A.rows == 0 || heads[i] == 0)) SNN_CUDA(cudaMemsetAsync(dw[i], 0, (size_t)d->dim * 4, st));
         if (A.rows == 0 || heads[i] == 0) continue;
         Side& S = A.side[i];
         S.x = heads_of(d, x[i], heads[i], i ? "k" : "q", false);
@@ -486,6 +485,8 @@ void qk_norm_grad(const snn_qk* d, const snn_heads* q, const snn_heads* k, const
             sums = true;
         }
     }
+    for (int i = 0; i < 2; ++i)  // (all has been looked at)
+        if (dw[i] && !A.side[i].x.p) SNN_CUDA(cudaMemsetAsync(dw[i], 0, (size_t)d->dim * 4, st));
     if (!A.side[0].x.p && !A.side[1].x.p) return;
     const int ctas = run<true>(d, A, st);
     if (sums) {

@@ -249,3 +249,10 @@ def test_binding_refuses():
                 lambda: snn.qk_norm_grad(q, k, q, None), lambda: snn.qk_norm_grad(q, k, q.half(), k)):
         with pytest.raises(snn.SnnError):
             bad()
+
+
+@pytest.mark.parametrize("over", [dict(k=None), dict(dyk=None), dict(wk=2), dict(dwk=2), dict(work=None), dict(bytes=8)])
+def test_grad_refuses_before_it_writes(over):
+    """No weight's gradient is written, of queries that are not there either, when an argument is refused (without a GPU
+    any launch would be another error)."""
+    assert call(grad=True, desc=dict(hq=0), **over) == 1
