@@ -473,9 +473,11 @@ void delta_scan_grad(const snn_delta* d, const snn_heads* q, const snn_heads* k,
     check_states({dh, dh0});
     A.dh = dh;
     A.dh0 = dh0;
-    const Layout l = layout_of(d);  // (of no sequence: of no size)
-    check_work(saved, saved_bytes, l.kept_all, "saved");
-    check_work(work, work_bytes, l.kept_all - l.states, "workspace");
+    const Layout l = layout_of(d);
+    if (d->n_seq) {
+        check_work(saved, saved_bytes, l.kept_all, "saved");
+        check_work(work, work_bytes, l.kept_all - l.states, "workspace");
+    }
     zero_rows(d, A, A.dq, A.hk, A.kdim, st);
     zero_rows(d, A, A.dk, A.hk, A.kdim, st);
     zero_rows(d, A, A.dv, A.heads, A.vdim, st);

@@ -137,6 +137,8 @@ def test_a_batch_of_no_sequence(grad):
     over = NOTHING | {n: (None, 400, 4) for n in ("gate", "beta", "dgate", "dbeta")}
     assert call(grad=grad, desc=dict(n_seq=0), bytes=0, sbytes=0, **over) == 0
     assert call(grad=grad, desc=dict(n_seq=1), bytes=0, sbytes=0, **over) == 1
+    # rows of no sequence want neither saved nor a workspace
+    assert call(grad=grad, desc=dict(n_seq=0, n_steps=500, off=4096), bytes=0, sbytes=0, saved=None, work=None) == 0
     if grad:  # (gradients of the final states of none)
         assert call(grad=True, desc=dict(n_seq=0), bytes=0, sbytes=0, **(over | dict(dy=None))) == 0
 
