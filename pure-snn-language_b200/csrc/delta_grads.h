@@ -282,17 +282,18 @@ __global__ void __launch_bounds__(GRADS, 1) k_delta_grads(const __grid_constant_
                     kv = *reinterpret_cast<const float2*>(Ks + i * KS + c);
                     qv = *reinterpret_cast<const float2*>(Qs + i * KS + c);
                 }
-                const float si = since[i], un = until[i], ra = rate[i];
+                // (divided by the scales of the keys and queries that they meet here)
+                const float fq1 = A.scale * since[i] * iq, fk1 = -since[i] * ik, fm1 = until[i] * ik, ra = rate[i];
                 float *q2 = zq[j] + 2 * h, *k2 = zk[j] + 2 * h, *m2 = zm[j] + 2 * h;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    q2[e] *= A.scale * si;
-                    k2[e] *= -si;
-                    m2[e] *= un;
+                    q2[e] *= fq1;
+                    k2[e] *= fk1;
+                    m2[e] *= fm1;
                 }
-                by_row[0][h] = fmaf(iq, fmaf(qv.x, q2[0], qv.y * q2[1]), by_row[0][h]);
-                by_row[2][h] = fmaf(ik, fmaf(kv.x, k2[0], kv.y * k2[1]), by_row[2][h]);
-                by_row[1][h] = fmaf(ik, fmaf(kv.x, m2[0], kv.y * m2[1]), by_row[1][h]);
+                by_row[0][h] += fmaf(qv.x, q2[0], qv.y * q2[1]);
+                by_row[2][h] += fmaf(kv.x, k2[0], kv.y * k2[1]);
+                by_row[1][h] += fmaf(kv.x, m2[0], kv.y * m2[1]);
                 k2[0] = fmaf(ra, k2[0], m2[0]);
                 k2[1] = fmaf(ra, k2[1], m2[1]);
             }
@@ -339,16 +340,17 @@ __global__ void __launch_bounds__(GRADS, 1) k_delta_grads(const __grid_constant_
                 tp = fmaxf(tp, top[0][i]);
                 tx = fmaxf(tx, top[1][i]);
             }
-            xs = scale_for(tx);
-            ps = scale_for(tp);
-            fk = xs * ks;
-            fq = ps * ks;
+            // (held so that a product with both keys' scales is below 2^120)
+            xs = fminf(scale_for(tx), 0x1p120f * ik * ik);
+            ps = fminf(scale_for(tp), 0x1p120f * ik * iq);
+            fk = scale_of_both(xs, ks);
+            fq = scale_of_both(ps, ks);
 #pragma unroll
             for (int j = 0; j < NQ; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    zq[j][e] *= fq;
-                    zk[j][e] *= fk;
+                    zq[j][e] *= fq * qs;
+                    zk[j][e] *= fk * ks;
                 }
         }
         if (wc <= wr)
@@ -386,7 +388,7 @@ __global__ void __launch_bounds__(GRADS, 1) k_delta_grads(const __grid_constant_
             }
         }
         if constexpr (SCALED) {
-            const float to = inverse_of(fk), next = ps * qs;
+            const float to = inverse_of(fk), next = scale_of_both(ps, qs);
             fk = next;
 #pragma unroll
             for (int j = 0; j < NQ; ++j)

@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(PREP, 4) k_delta_prep(const __grid_constant__ 
     }
     float scale = 1.0f;
     if constexpr (P::SCALED) {
-        scale = scale_for(__uint_as_float(__reduce_max_sync(~0u, __float_as_uint(most))));
+        scale = fminf(scale_for(__uint_as_float(__reduce_max_sync(~0u, __float_as_uint(most)))), 0x1p40f);
         if (lane == 0) F[P_SCALE + warp] = scale;
     }
 #pragma unroll

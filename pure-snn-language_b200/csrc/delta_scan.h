@@ -189,8 +189,8 @@ __device__ __forceinline__ void write_state(const float (&S)[NT][4], float back,
 template <int NT>
 __device__ __forceinline__ void recentre(float (&S)[NT][4], float& scale, float& top) {
     top = warp_top(S);
-    if (top >= 0x1p15f || (top < 0x1p6f && top > 0.0f && scale < 0x1p60f)) {
-        const float f = fminf(scale_for(top), 0x1p60f * inverse_of(scale));
+    if (top >= 0x1p15f || (top < 0x1p6f && top > 0.0f && scale < MOST_SCALE)) {
+        const float f = fminf(scale_for(top), MOST_SCALE * inverse_of(scale));
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -205,8 +205,8 @@ __device__ __forceinline__ void recentre(float (&S)[NT][4], float& scale, float&
 template <int NT>
 __device__ __forceinline__ void make_room(float (&S)[NT][4], float (&x)[8][4], float (&y)[8][4], float& scale, float top) {
     const float both = fmaxf(warp_top(x), &x != &y ? warp_top(y) : 0.0f), all = fmaxf(both, top);
-    if (both >= 0x1p15f || (all < 0x1p6f && all > 0.0f && scale < 0x1p60f)) {
-        const float f = fminf(scale_for(both >= 0x1p15f ? both : all), 0x1p60f * inverse_of(scale));
+    if (both >= 0x1p15f || (all < 0x1p6f && all > 0.0f && scale < MOST_SCALE)) {
+        const float f = fminf(scale_for(both >= 0x1p15f ? both : all), MOST_SCALE * inverse_of(scale));
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -485,8 +485,8 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_back(const __grid_constant
                 // u = P^T Z + until K D, times c; the scales of row blocks are made up for in Z, R's in u
                 float c1 = 1.0f, c2 = 1.0f;
                 if constexpr (P::SCALED)
-                    c1 = scale_for(fabsf(A.scale) * warp_top(z)) *
-                         fminf(fminf(st.f[P_SCALE], st.f[P_SCALE + 1]), fminf(st.f[P_SCALE + 2], st.f[P_SCALE + 3]));
+                    c1 = scale_of_both(scale_for(fabsf(A.scale) * warp_top(z)),
+                                       fminf(fminf(st.f[P_SCALE], st.f[P_SCALE + 1]), fminf(st.f[P_SCALE + 2], st.f[P_SCALE + 3])));
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const float2 until = pair_at(st.f + C, j);
@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_back(const __grid_constant
                 }
                 times_square<P, P::PIECES, false>(u, z, [&](int d) { return P::SCALED ? c1 * inverse_of(st.f[P_SCALE + d]) : 1.0f; }, st.p);
                 if constexpr (P::SCALED)
-                    c2 = warp_scale(u) * fminf(fminf(st.f[T_SCALE], st.f[T_SCALE + 1]), fminf(st.f[T_SCALE + 2], st.f[T_SCALE + 3]));
+                    c2 = scale_of_both(warp_scale(u), fminf(fminf(st.f[T_SCALE], st.f[T_SCALE + 1]), fminf(st.f[T_SCALE + 2], st.f[T_SCALE + 3])));
                 times_square<P, P::PIECES, false>(r, u, [&](int d) { return P::SCALED ? c2 * inverse_of(st.f[T_SCALE + d]) : 1.0f; }, st.t);
                 if constexpr (P::SCALED) {
                     const float f1 = inverse_of(c1), f2 = inverse_of(c2);

@@ -410,15 +410,20 @@ template <> struct PathOf<__half> { using P = Path16<__half>; };
 template <> struct PathOf<float> { using P = Path32; };
 
 // A power of two that brings the largest magnitude to 2^13 .. 2^14, near f16's largest
-// values, so that smaller ones keep 22 bits down to 2^-16 of it; held to 2^-60 .. 2^60,
-// so that what it multiplies stays finite.  1 where all is zero.
+// values, so that smaller ones keep 22 bits down to 2^-16 of it; 2^-113 at least (f32's largest values
+// then lie below 2^15) and 2^80 at most (of a top below 2^-67 fewer bits are kept; those of keys, queries
+// and P are held to 2^40, so that products with these have an inverse).  1 where all is zero.
+constexpr float MOST_SCALE = 0x1p80f;
 __device__ __forceinline__ float scale_for(float top) {
-    const int b = (int)(__float_as_uint(top) >> 23), e = min(max(13 + 127 + 127 - b, 127 - 60), 127 + 60);
+    const int b = (int)(__float_as_uint(top) >> 23), e = min(max(13 + 127 + 127 - b, 127 - 113), 127 + 80);
     return __uint_as_float((unsigned)(b ? e : 127) << 23);
 }
 __device__ __forceinline__ float inverse_of(float s) {  // of a power of two
     return __uint_as_float((254u << 23) - __float_as_uint(s));
 }
+// The product of two scales.  Where it is below 2^-126 it has no inverse, and what they scale has a product beyond
+// f32, which is not to pass for a number.
+__device__ __forceinline__ float scale_of_both(float a, float b) { return a * b < 0x1p-126f ? NAN : a * b; }
 __device__ __forceinline__ float finite_size(float x) { return fabsf(x) <= FLT_MAX ? fabsf(x) : 0.0f; }
 template <int N>
 __device__ __forceinline__ float warp_top(const float (&x)[N][4]) {

@@ -161,3 +161,32 @@ def test_grad_refuses_before_it_writes(over):
     """Nothing has been launched, not even the zeros of rows of no sequence, when an argument is refused (without a GPU
     any launch would be another error)."""
     assert call(grad=True, desc=dict(off=4096, flags=snn.SCAN_ZERO, n_seq=3), **over) == 1
+
+
+# ---- magnitudes ----------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("values,gradients", [(2.0 ** 80, 1.0), (2.0 ** 112, 1.0), (1.0, 2.0 ** 80), (1.0, 2.0 ** 112), (2.0 ** 55, 2.0 ** 50),
+                                              (2.0 ** -40, 2.0 ** -40)])
+def test_magnitudes_of_the_types(kind, values, gradients):
+    """Values, states and gradients up to the magnitudes that bf16 and f32 have."""
+    x, s0, dy, dh = make(41, (2, 150), 1, 2, 40, 36, kind)
+    x[2], s0, dy, dh = x[2] * values, s0 * values, dy * gradients, dh * gradients
+    x[0] = x[0] / 8
+    want = ref.run(*map(host, x), host(s0), dy=host(dy), dh=host(dh), kind=kind)
+    y, h, saved = snn.delta_scan(*x, s0, save=True)
+    ref.close(host(y), want["y"], kind, "y")
+    ref.close(host(h), want["h"], kind, "h")
+    for name, g in zip(GRADS, snn.delta_scan_grad(*x, dy, saved, dh=dh)):
+        ref.close(host(g), want[name], kind, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [2.0 ** 20, 2.0 ** 90])
+def test_states_beyond_f16(size):
+    """States are f32 beside f16 tensors too; answers that are too large for f16 are infinite."""
+    x, s0, _, _ = make(42, (2, 150), 1, 2, 40, 36, "f16")
+    want = ref.run(*map(host, x), host(s0 * size), kind="f16")
+    y, h = snn.delta_scan(*x, s0 * size)
+    ref.close(host(h), want["h"], "f16", "h")
+    assert not np.isnan(host(y)).any()
