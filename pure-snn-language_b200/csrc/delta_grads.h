@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(GRADS, 1) k_delta_grads(const __grid_constant_
                 if (i < n) {
                     const T gate = ((const T*)A.gate.p)[row_at(A, A.gate, s, sp, t0 + i) + head * A.gate.hs];
                     if (A.logit) dg *= 1.0f / (1.0f + expf(to_f32(gate)));
-                    if (log_decay(A, gate) < FORGETS) dg = 0.0f;  // a decay of 0
+                    if (cut[i] != (i ? cut[i - 1] : 0)) dg = 0.0f;  // a decay of 0
                     ((T*)A.dgate.p)[row_at(A, A.dgate, s, sp, t0 + i) + head * A.dgate.hs] = from_f32<T>(dg);
                 }
             }
