@@ -515,8 +515,10 @@ int snn_leaky_scan_grad(const snn_scan* desc, const snn_rows* gate, const snn_ro
  * [rot / 2] in radians a position; both may be NULL where rot is 0.  w (f32 [dim],
  * one for queries, one for keys) may be NULL: ones.  Heads of one row share its
  * position.  q_heads or k_heads may be 0: that tensor is then not looked at.
- * dim <= 512, rot even and <= dim.  Strides are any of which heads that are written
- * do not overlap; outputs may be their own inputs (same data and strides), and
+ * dim <= 512, rot even and <= dim.  Sums of squares are f32 (elements below 2^59).
+ * Words of 16 bytes are taken where dim, strides and, unless SNN_QK_ADJACENT, rot / 2
+ * are whole words; otherwise shorter ones, down to single elements, at a lower rate.
+ * Strides are any of which heads that are written do not overlap; outputs may be their own inputs (same data and strides), and
  * must not overlap anything else. */
 #define SNN_QK_UNIT 1
 #define SNN_QK_ADJACENT 2
@@ -561,21 +563,26 @@ int snn_qk_norm_grad(const snn_qk* desc, const snn_heads* q, const snn_heads* k,
  *   y_t = scale S_t^T q_t
  * with a = exp(gate), b = beta, or with SNN_SCAN_LOGIT a = 1 / (1 + exp(-gate)),
  * b = 1 / (1 + exp(-beta)).  gate is a logarithm, so that decays near 1 keep their
- * memory; below -104 (minus infinity, the type's lowest value) the decay is 0 in f32: the
- * step forgets every finite state and its gate has the gradient 0.  Keys of unit length and rates in
- * [0, 2] keep S bounded (snn_qk_norm with SNN_QK_UNIT); any are taken.
+ * memory; below -104 (minus infinity, the type's lowest value) the decay is 0 in f32:
+ * the step forgets every finite state and its gate has the gradient 0.  Keys of unit
+ * length and rates in [0, 2] keep S bounded (snn_qk_norm with SNN_QK_UNIT); any are taken.
  * q, k: rows of k_heads x k_dim, v, y: of heads x v_dim, gate, beta: of heads;
  * head h reads key head h / (heads / k_heads).  All have element type `type`, unit
  * stride of their last dimension; dense or packed as in snn_leaky_scan, with SNN_SCAN_ZERO
  * for the rows of no sequence.  k_dim <= 128, v_dim <= 1024.
  * States are f32 [n_seq, heads, k_dim, v_dim]; h0 (nullable: zeros) and h (nullable)
- * may be the same.  Sums are f32, y is rounded once.  Long sequences are
- * taken 64 steps at a time, the recurrence's sum in another order: a NaN or an
- * infinity in a key, value, gate or rate may then make earlier rows of its 64 steps
- * NaN too (of a value, in its column).  The same holds for the gradients, in both
- * directions.
+ * may be the same.  States and sums are f32, y is rounded once.  Long sequences are
+ * taken 64 steps at a time, the recurrence's sum in another order, by matrix
+ * instructions whose operands have fewer bits: f32 ones are taken in two pieces of 11 bits
+ * (f16 times a power of two, tf32 of f32 tensors), of what only reaches a bf16 y in one.
+ * With 16-bit tensors 16 columns of a state share a power of two: what lies below 2^-16 of
+ * the largest finite one of them keeps fewer bits, below 2^-38 none; so does all that is below
+ * 2^-67 (keys, queries 2^-27).  A NaN or an infinity in a key, value, gate or rate
+ * may make earlier rows of its 64 steps NaN too (of a value, in its column).  The same
+ * holds for the gradients, in both directions.
  * Where sequences have 8 steps or fewer in the mean the steps are taken one by one,
- * without a workspace. */
+ * without a workspace, in a long sequence among many single steps too: such a batch
+ * is faster as two calls. */
 typedef struct snn_delta {
     int32_t type;            /* SNN_F32 / SNN_BF16 / SNN_F16                     */
     int32_t flags;           /* SNN_SCAN_LOGIT, SNN_SCAN_ZERO                    */
@@ -607,7 +614,11 @@ int snn_delta_scan(const snn_delta* desc, const snn_heads* q, const snn_heads* k
  *   db_t = (D_t^T k_t).(v_t - S'_t^T k_t),   da_t = <D_t - k_t e_t^T, S_{t-1}>,
  *   dgate = a da, dbeta = db, or with SNN_SCAN_LOGIT a (1 - a) da and b (1 - b) db;
  *   dh0 = the gradient of the first S_{t-1}.
- * dq and dk are summed over the heads that read them, in order.  All results have
+ * dq and dk are summed over the heads that read them, in order.  Sums are f32, results
+ * rounded once.  Of bf16 tensors S and D are kept and multiplied as bf16, u and e in two
+ * pieces of it, and products of 64 steps with keys and queries take one piece of 11 bits:
+ * the gradients are off by about 1.1 times what their rounding to bf16 alone makes (2-norm
+ * 1.9e-3 and 1.7e-3).  Otherwise operands are as in the forward call.  All results have
  * their inputs' forms (dq, dk, dv, dgate, dbeta as q, k, v, gate, beta; dh0, nullable, f32
  * states); rows of no sequence as in the forward call.  saved is what the
  * forward call wrote.  work: of the size that snn_delta_scan_grad_workspace says. */

@@ -4,8 +4,8 @@
 // Bound by memory: 28 bytes an element with f32 moments and f32 gradients (p, m, v
 // read and written, g read), 16 with 8-bit ones.  Descriptions of the tensors travel
 // as kernel parameters, so a step over up to 400 tensors is one launch and needs
-// no table on the device.  69 M parameters, 16-bit gradients and copies: 347 us, 297 at the
-// copy rate; 8-bit moments 306 of 169, bound by the instructions (120 an element).  Roundings are those of the formula taken one operation
+// no table on the device.  69 M parameters, 16-bit gradients and copies: a step 353 us, 297 at the
+// copy rate; 8-bit moments 307 of 169, bound by the instructions (120 an element).  Roundings are those of the formula taken one operation
 // at a time (this file is compiled without contraction).
 //
 // 8-bit moments: e4m3 values (half a step is 2^-4 of a value) with an f32 scale for

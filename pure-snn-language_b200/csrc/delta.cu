@@ -25,7 +25,7 @@ constexpr int MAX_K = 128;
 // A CTA takes 32 V columns of a head's state, a warp every sixteenth row of it, in registers
 // from the first step to the last.  Bound by the state's way from memory and back: 16
 // warps of 64 registers, two CTAs an SM, have 128 kB of it in flight (64 streams x 8 heads
-// x 128 x 128 bf16: 8 warps of 215 registers 22.8 us, these 18, of 10.4 at the copy rate).
+// x 128 x 128 bf16: kernel with 8 warps of 215 registers 22.8 us, this one 18, of 10.4 at the copy rate).
 constexpr int STEP_WARPS = 16;
 template <typename T, int V>
 __global__ void __launch_bounds__(32 * STEP_WARPS, 2) k_delta_steps(const __grid_constant__ DeltaArgs A) {
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(32 * STEP_WARPS, 2) k_delta_steps(const __grid
 // Where the segments start from: starts[g + 1], which holds what segment g makes of nothing, gains its
 // steps' product times starts[g], one segment after the other.  A CTA takes 16 columns of a
 // head, in shared memory from one segment to the next; the next product is on its way
-// meanwhile.  A thread has 8 columns of a row.  (6 products of 16 heads of 128 x 128: 40 us.)
+// meanwhile.  A thread has 8 columns of a row.  (6 products of 16 heads of 128 x 128: kernel 40 us.)
 constexpr int JOIN_COLS = 16, JOIN_ROW = MAX_K + 4, JOIN_SMEM = (2 * MAX_K * JOIN_ROW + MAX_K * JOIN_COLS) * 4;
 __global__ void __launch_bounds__(256) k_delta_join(const __grid_constant__ DeltaArgs A) {
     extern __shared__ __align__(16) float join[];  // two products [MAX_K][JOIN_ROW], a state [MAX_K][JOIN_COLS]
@@ -288,7 +288,7 @@ struct Layout {
 // state and the product of its steps (twice the columns, no results), those are joined, and all segments
 // run at once.  That is 2.7 times the work (about), so it takes four segments and more, as many as
 // give every SM eight warps; a segment has at least 8 chunks.  1 x 16,384 steps x 16 heads of 128 x 128 f16: whole
-// 1,300 us, by 8 segments 361 + 40 + 281.  Packed sequences may be of any lengths: segments are of the mean's
+// 1,300 us, by 8 segments 626 for both runs, 40 to join.  Packed sequences may be of any lengths: segments are of the mean's
 // size, and numbered as their chunks are, by their rows' place.
 struct Cut {
     int seg;
@@ -317,7 +317,9 @@ Layout layout_of(const snn_delta* d) {
     l.cut = cut.seg ? l.maps + round256(cut.items * d->heads * d->k_dim * d->k_dim * 4) : 0;
     return l;
 }
-// Up to 8 steps one by one (64 x 8 heads of 128 x 128 bf16, us by 4 and 8 steps: 32, 55; as a chunk 74)
+// Up to 8 steps one by one (64 x 8 heads of 128 x 128 bf16, us by 4 and 8 steps: 32, 55; as a chunk 74).  The
+// mean decides for all: packed lengths lie on the device.  A long sequence among single steps is then slow: 63
+// of one step and one of 400, 8 heads, 811 us (141 as chunks, 77 as two calls).
 bool by_steps(const snn_delta* d) { return mean_steps(d) <= 8; }
 
 DeltaArgs base_args(const snn_delta* d, const snn_heads* q, const snn_heads* k, const snn_heads* v, const snn_rows* gate,

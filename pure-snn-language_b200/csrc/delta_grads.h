@@ -3,7 +3,7 @@
 #include "delta_tile.h"
 
 namespace snnb_delta {
-// For all chunks at once.  // With S before a chunk, D behind it, U and R as above, G the decays between steps:
+// For all chunks at once.  With S before a chunk, D behind it, U and R as above, G the decays between steps:
 //   p = G (Z U^T) (j <= i),   x = -b G (R U^T) (j < i)
 //   dQ = since Z S^T + p K,   dK = -since b R S^T + until U D^T + x K + x^T K + p^T Q
 //   db_i = R_i.V_i - since_i k_i.(S R_i) + sum_j x_ij k_i.k_j / b_i
@@ -14,7 +14,7 @@ namespace snnb_delta {
 // one piece of f16 for bf16 tensors, two for f16.  16 warps: 16 rows and a quarter
 // of the columns each; half of an SM's registers are accumulators, so that S, D, U, R and dy are
 // read once.  That leaves one CTA an SM, whose phases wait for one another: 8,192 chunks of 128 x 128
-// bf16 945 us (280 at the copy rate; 800 with U and R in one piece, whose gradients are off by
+// bf16: kernel 911 us (280 at the copy rate; 800 with U and R in one piece, whose gradients are off by
 // 2.5e-3 of their norm where these are by 1.9e-3 and the rounding alone makes 1.7e-3).
 struct Ops16 {                 // one piece of a 16-bit type E
     template <typename E>

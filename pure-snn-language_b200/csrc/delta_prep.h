@@ -5,7 +5,7 @@
 // with N = -T_ii A_im:  T_ij = sum of N_im T_mj, one row of blocks after the other, in f32
 // by two tf32 pieces.  Bound by latency (half of it loads, scaling and
 // decays, half products and the inversion), which four CTAs on an SM hide in part: 8,192 chunks
-// of 128 bf16 275 us, 117 at the copy rate.  Five CTAs of 96 registers: 290; eight warps,
+// of 128 bf16: kernel 277 us, 117 at the copy rate.  Five CTAs of 96 registers: 290; eight warps,
 // queries and keys apart: 322.
 #pragma once
 #include "delta_tile.h"
