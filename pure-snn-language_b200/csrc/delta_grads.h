@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(GRADS, 1) k_delta_grads(const __grid_constant_
     float* F = reinterpret_cast<float*>(Qs + G::KEYS);
     E* blocks = reinterpret_cast<E*>(F + SC);
     KE *Ps = reinterpret_cast<KE*>(blocks), *Xs = Ps + G::SQ;
-    __shared__ float rows[4][4][C], cols[4][C], more[GRADS / 32], dots[C], top[2][GRADS / 32];
+    __shared__ float rows[4][4][C], cols[4][C], more[GRADS / 32], dots[C], top[4][GRADS / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
     const int wr = warp & 3, wc = warp >> 2, kh = blockIdx.y;
     const long long slot = blockIdx.x, s = sequence_of(A, slot);
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(GRADS, 1) k_delta_grads(const __grid_constant_
             }
         }
         float by_row[4][2] = {}, by_col[2][2] = {};  // q.dQ + b k.., k..until, R part of db, sum of x k.k / b; columns
-        float tp = 0.0f, tx = 0.0f;
+        float tp = 0.0f, tx = 0.0f, tq1 = 0.0f, tk1 = 0.0f;  // the largest of p, x, zq and zk
         if (wc <= wr)
 #pragma unroll
             for (int j = 0; j < 2; ++j)
@@ -296,6 +296,10 @@ __global__ void __launch_bounds__(GRADS, 1) k_delta_grads(const __grid_constant_
                 by_row[1][h] += fmaf(kv.x, m2[0], kv.y * m2[1]);
                 k2[0] = fmaf(ra, k2[0], m2[0]);
                 k2[1] = fmaf(ra, k2[1], m2[1]);
+                if constexpr (SCALED) {
+                    tq1 = fmaxf(tq1, fmaxf(fabsf(q2[0]), fabsf(q2[1])));
+                    tk1 = fmaxf(tk1, fmaxf(fabsf(k2[0]), fabsf(k2[1])));
+                }
             }
 #pragma unroll
         for (int q = 0; q < 4; ++q)
@@ -320,29 +324,31 @@ __global__ void __launch_bounds__(GRADS, 1) k_delta_grads(const __grid_constant_
         for (int o = 1; o < 8; o *= 2) rv += __shfl_xor_sync(~0u, rv, o);
         if ((tid & 7) == 0) dots[tid >> 3] = rv;
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            inner += __shfl_xor_sync(~0u, inner, o);
-            if constexpr (SCALED) {
-                tp = fmaxf(tp, __shfl_xor_sync(~0u, tp, o));
-                tx = fmaxf(tx, __shfl_xor_sync(~0u, tx, o));
-            }
+        for (int o = 16; o; o >>= 1) inner += __shfl_xor_sync(~0u, inner, o);
+        auto most = [](float v) { return __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(v))); };
+        if constexpr (SCALED) {
+            tp = most(tp);
+            tx = most(tx);
+            tq1 = most(finite_size(tq1));
+            tk1 = most(finite_size(tk1));
         }
         if (lane == 0) {
             more[warp] = inner;
             top[0][warp] = tp;
             top[1][warp] = tx;
+            top[2][warp] = tq1;
+            top[3][warp] = tk1;
         }
         float ps = 1.0f, xs = 1.0f, fq = 1.0f, fk = 1.0f;  // scales of p, x and of what they are added to
         if constexpr (SCALED) {
             __syncthreads();
-#pragma unroll
-            for (int i = 0; i < GRADS / 32; ++i) {
-                tp = fmaxf(tp, top[0][i]);
-                tx = fmaxf(tx, top[1][i]);
-            }
-            // (held so that a product with both keys' scales is below 2^120)
-            xs = fminf(scale_for(tx), 0x1p120f * ik * ik);
-            ps = fminf(scale_for(tp), 0x1p120f * ik * iq);
+            tp = most(top[0][lane % (GRADS / 32)]);
+            tx = most(top[1][lane % (GRADS / 32)]);
+            tq1 = most(top[2][lane % (GRADS / 32)]);
+            tk1 = most(top[3][lane % (GRADS / 32)]);
+            // (held so that a product with both keys' scales is finite, and so are zq and zk times these)
+            xs = scale_within(scale_for(tx), fminf(0x1p100f * scale_for(tk1), 0x1p120f) * ik * ik);
+            ps = scale_within(scale_for(tp), fminf(0x1p100f * scale_for(tq1), 0x1p120f) * ik * iq);
             fk = scale_of_both(xs, ks);
             fq = scale_of_both(ps, ks);
 #pragma unroll
@@ -363,7 +369,7 @@ __global__ void __launch_bounds__(GRADS, 1) k_delta_grads(const __grid_constant_
                     KOp::template put<PIECES>(Xs + at, x[j][2 * h] * xs, x[j][2 * h + 1] * xs);
                 }
         __syncthreads();
-        // dQ += p K, dK += x K + x^T K, then p^T Q in its own scale
+        // dQ += p K, dK += x K + x^T K, then p^T Q, which has a scale of its own
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
             typename KOp::B bk[NQ / 2][2];
@@ -387,14 +393,15 @@ __global__ void __launch_bounds__(GRADS, 1) k_delta_grads(const __grid_constant_
                 }
             }
         }
-        if constexpr (SCALED) {
-            const float to = inverse_of(fk), next = scale_of_both(ps, qs);
-            fk = next;
+        const float bq1 = inverse_of(fq), bk1 = inverse_of(fk), bp1 = inverse_of(SCALED ? scale_of_both(ps, qs) : 1.0f);
 #pragma unroll
-            for (int j = 0; j < NQ; ++j)
+        for (int j = 0; j < NQ; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) zk[j][e] = zk[j][e] * to * next;
-        }
+            for (int e = 0; e < 4; ++e) {
+                tq[j][e] = fmaf(zq[j][e], bq1, tq[j][e]);
+                tk[j][e] = fmaf(zk[j][e], bk1, tk[j][e]);
+                zq[j][e] = 0.0f;
+            }
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
             if (d < wr) continue;
@@ -405,17 +412,13 @@ __global__ void __launch_bounds__(GRADS, 1) k_delta_grads(const __grid_constant_
             for (int i = PIECES - 1; i >= 0; --i) {
                 const typename KOp::A pt = KOp::columns_of(Ps + i * C * MS + d * 16 * MS + wr * 16, MS);
 #pragma unroll
-                for (int j = 0; j < NQ / 2; ++j) KOp::mma(zk[2 * j], zk[2 * j + 1], pt, bq[j]);
+                for (int j = 0; j < NQ / 2; ++j) KOp::mma(zq[2 * j], zq[2 * j + 1], pt, bq[j]);
             }
         }
-        const float bq1 = inverse_of(fq), bk1 = inverse_of(fk);
 #pragma unroll
         for (int j = 0; j < NQ; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                tq[j][e] = fmaf(zq[j][e], bq1, tq[j][e]);
-                tk[j][e] = fmaf(zk[j][e], bk1, tk[j][e]);
-            }
+            for (int e = 0; e < 4; ++e) tk[j][e] = fmaf(zq[j][e], bp1, tk[j][e]);
         if (warp == 0) {
             // rows 2 lane, 2 lane + 1: what each adds to the decays up to it
             float d[2], whole = 0.0f, edge = 0.0f;

@@ -201,16 +201,17 @@ __device__ __forceinline__ void recentre(float (&S)[NT][4], float& scale, float&
 }
 // The same before products of x and y, which are already times their part of the scale to be
 // pieces, are added to what a chunk leaves of S (at most top): neither is too large for
-// a piece, nor all of them so small that pieces lose bits.
+// a piece, nor all of them so small that pieces lose bits.  `held` is the scale as x and y have it: less than S's
+// where they would not be finite otherwise.
 template <int NT>
-__device__ __forceinline__ void make_room(float (&S)[NT][4], float (&x)[8][4], float (&y)[8][4], float& scale, float top) {
-    const float both = fmaxf(warp_top(x), &x != &y ? warp_top(y) : 0.0f), all = fmaxf(both, top);
-    if (both >= 0x1p15f || (all < 0x1p6f && all > 0.0f && scale < MOST_SCALE)) {
-        const float f = fminf(scale_for(both >= 0x1p15f ? both : all), MOST_SCALE * inverse_of(scale));
+__device__ __forceinline__ void make_room(float (&S)[NT][4], float (&x)[8][4], float (&y)[8][4], float& scale, float held, float top) {
+    const float part = held * inverse_of(scale), both = fmaxf(warp_top(x), &x != &y ? warp_top(y) : 0.0f), all = fmaxf(both, top * part);
+    if (held < scale || both >= 0x1p15f || (all < 0x1p6f && all > 0.0f && scale < MOST_SCALE)) {
+        const float f = fminf(scale_for(both >= 0x1p15f ? both : all), MOST_SCALE * inverse_of(held)), fs = part * f;
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) S[i][e] *= f;
+            for (int e = 0; e < 4; ++e) S[i][e] *= fs;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -218,7 +219,7 @@ __device__ __forceinline__ void make_room(float (&S)[NT][4], float (&x)[8][4], f
                 x[i][e] *= f;
                 if (&x != &y) y[i][e] *= f;
             }
-        scale *= f;
+        scale = held * f;
     }
 }
 // S times the decays of a chunk: by what they take off where that is little, since 1 - lost keeps its
@@ -380,7 +381,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_scan(const __grid_constant
                     }
                 }
                 // u = T r
-                float ss = 1.0f;
+                float ss = 1.0f, held = sigma;
                 if constexpr (P::SCALED) ss = warp_scale(r);
                 times_square<P, P::PIECES, true>(u, r, [&](int) { return ss; }, st.t);
                 if constexpr (P::SCALED) {
@@ -390,7 +391,11 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_scan(const __grid_constant
 #pragma unroll
                         for (int e = 0; e < 4; ++e) u[i][e] *= f;
                     }
+                    // (times the state's scale u is 2^74 at most; the answers' sum of state and queries, 2^35 / (their scales)
+                    // at most, is taken times ss and P's scale, which is 2^40 at most)
                     ss = warp_scale(u);
+                    held = scale_within(sigma, 0x1p60f * ss * st.f[K_SCALE]);
+                    ss = scale_within(ss, 0x1p45f * sigma * st.f[Q_SCALE]);
                 }
                 if (!A.only) {
                 // o = since Q S + P u, times the pieces' scales
@@ -416,9 +421,9 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_scan(const __grid_constant
                 for (int i = 0; i < 8; ++i) {
                     const float2 until = pair_at(st.f + C, i);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) u[i][e] *= (e & 1 ? until.y : until.x) * sigma * ik;
+                    for (int e = 0; e < 4; ++e) u[i][e] *= (e & 1 ? until.y : until.x) * held * ik;
                 }
-                if constexpr (P::SCALED) make_room(S, u, u, sigma, top * st.f[C - 1]);
+                if constexpr (P::SCALED) make_room(S, u, u, sigma, held, top * st.f[C - 1]);
                 decay_state(S, st.f[LOST], st.f[C - 1]);
                 add_outer<P, KD>(S, u, st.k);
             }
@@ -483,10 +488,13 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_back(const __grid_constant
                 }
                 values_of<T, VS>(z, st.v + warp * 16);
                 // u = P^T Z + until K D, times c; the scales of row blocks are made up for in Z, R's in u
-                float c1 = 1.0f, c2 = 1.0f;
-                if constexpr (P::SCALED)
-                    c1 = scale_of_both(scale_for(fabsf(A.scale) * warp_top(z)),
-                                       fminf(fminf(st.f[P_SCALE], st.f[P_SCALE + 1]), fminf(st.f[P_SCALE + 2], st.f[P_SCALE + 3])));
+                float c1 = 1.0f, c2 = 1.0f, cz = 1.0f, held = sigma;
+                if constexpr (P::SCALED) {
+                    const float least_p = fminf(fminf(st.f[P_SCALE], st.f[P_SCALE + 1]), fminf(st.f[P_SCALE + 2], st.f[P_SCALE + 3]));
+                    cz = scale_for(fabsf(A.scale) * warp_top(z));
+                    // (K D, 2^35 / (their scales) at most, is taken times c1)
+                    c1 = scale_of_both(scale_within(cz, 0x1p85f * sigma * st.f[K_SCALE] * inverse_of(least_p)), least_p);
+                }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const float2 until = pair_at(st.f + C, j);
@@ -502,6 +510,8 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_back(const __grid_constant
                     c2 = scale_of_both(warp_scale(u), fminf(fminf(st.f[T_SCALE], st.f[T_SCALE + 1]), fminf(st.f[T_SCALE + 2], st.f[T_SCALE + 3])));
                 times_square<P, P::PIECES, false>(r, u, [&](int d) { return P::SCALED ? c2 * inverse_of(st.f[T_SCALE + d]) : 1.0f; }, st.t);
                 if constexpr (P::SCALED) {
+                    // (R is 2^35 / (c1 c2) at most, Z 2^14 / cz: times D's scale they are finite)
+                    held = scale_within(sigma, 0x1p60f * cz * st.f[Q_SCALE], 0x1p70f * c1 * c2 * st.f[K_SCALE]);
                     const float f1 = inverse_of(c1), f2 = inverse_of(c2);
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
@@ -516,14 +526,14 @@ __global__ void __launch_bounds__(NW * 32, 1) k_delta_back(const __grid_constant
                     const float2 since = pair_at(st.f, j), rate = pair_at(st.f + 2 * C, j);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float si = (e & 1 ? since.y : since.x) * sigma;
+                        const float si = (e & 1 ? since.y : since.x) * held;
                         r[j][e] *= e & 1 ? rate.y : rate.x;
                         u[j][e] = r[j][e] * (-si * ik);
                         z[j][e] *= si * iq;
                     }
                 }
                 store_tile<T, VS>(r, st.v + warp * 16, (T*)A.dv.p + row_at(A, A.dv, s, sp, c * C) + head * A.dv.hs + col, A.dv.st, n, w, A.dv.word);
-                if constexpr (P::SCALED) make_room(D, u, z, sigma, top * st.f[C - 1]);
+                if constexpr (P::SCALED) make_room(D, u, z, sigma, held, top * st.f[C - 1]);
                 decay_state(D, st.f[LOST], st.f[C - 1]);
                 add_outer<P, KD>(D, z, st.q);
                 add_outer<P, KD>(D, u, st.k);

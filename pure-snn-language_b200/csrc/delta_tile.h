@@ -424,6 +424,9 @@ __device__ __forceinline__ float inverse_of(float s) {  // of a power of two
 // The product of two scales.  Where it is below 2^-126 it has no inverse, and what they scale has a product beyond
 // f32, which is not to pass for a number.
 __device__ __forceinline__ float scale_of_both(float a, float b) { return a * b < 0x1p-126f ? NAN : a * b; }
+// The least of three powers of two, 2^-113 at least: a scale for what has a scale of its own and meets sums of other
+// sizes, which must stay finite times it
+__device__ __forceinline__ float scale_within(float own, float a, float b = INFINITY) { return fmaxf(fminf(own, fminf(a, b)), 0x1p-113f); }
 __device__ __forceinline__ float finite_size(float x) { return fabsf(x) <= FLT_MAX ? fabsf(x) : 0.0f; }
 template <int N>
 __device__ __forceinline__ float warp_top(const float (&x)[N][4]) {

@@ -226,3 +226,37 @@ def test_pieces_of_bf16_gradients(monkeypatch):
             assert err <= 1.05 * off[2][name]
         else:
             assert off[1][name] > 1.2 * off[2][name] and err < (off[1][name] * off[2][name]) ** 0.5, (name, err, off)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("v,h0,dy,dh,q,late", [
+    (2.0 ** 100, 2.0 ** -75, 1.0, 1.0, 1.0, 0.0),     # large values meet a state that is next to nothing
+    (2.0 ** 100, 2.0 ** -75, 2.0 ** -30, 1.0, 1.0, 70),  # .. after some chunks without values
+    (1.0, 1.0, 2.0 ** 90, 2.0 ** -80, 1.0, 0.0),      # and backwards
+    (1.0, 1.0, 2.0 ** -70, 2.0 ** 60, 2.0 ** -20, 0.0),  # small gradients of answers beside large ones of states
+    (1.0, 2.0 ** 60, 2.0 ** -60, 1.0, 1.0, 140)])
+def test_magnitudes_far_apart(kind, v, h0, dy, dh, q, late):
+    """A scale that brings out what is small does not lose what is large beside it."""
+    x, s0, g, d1 = make(43, (1, 200), 1, 1, 40, 36, kind)
+    x[2], s0, g, d1, x[0] = x[2] * v, s0 * h0, g * dy, d1 * dh, x[0] * q
+    if late:
+        x[2][:, :int(late)] = 0
+    want = ref.run(*map(host, x), host(s0), dy=host(g), dh=host(d1), kind=kind)
+    y, h, saved = snn.delta_scan(*x, s0, save=True)
+    ref.close(host(y), want["y"], kind, "y")
+    ref.close(host(h), want["h"], kind, "h")
+    for name, grad in zip(GRADS, snn.delta_scan_grad(*x, g, saved, dh=d1)):
+        ref.close(host(grad), want[name], kind, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rate", [-60.0, -80.0])
+def test_large_states_and_rates_next_to_nothing(rate):
+    x, s0, _, _ = make(44, (1, 200), 1, 1, 40, 36, "bf16", logit=True)
+    x[4][:] = rate
+    s0 = s0 * 2.0 ** 60
+    want = ref.run(*map(host, x), host(s0), kind="bf16", logit=True)
+    y, h = snn.delta_scan(*x, s0, logit=True)
+    ref.close(host(y), want["y"], "bf16", "y")
+    ref.close(host(h), want["h"], "bf16", "h")
