@@ -288,7 +288,7 @@ struct Layout {
 // state and the product of its steps (twice the columns, no results), those are joined, and all segments
 // run at once.  That is 2.7 times the work (about), so it takes four segments and more, as many as
 // give every SM eight warps; a segment has at least 8 chunks.  1 x 16,384 steps x 16 heads of 128 x 128 f16: whole
-// 1,300 us, by 8 segments 626 for both runs, 40 to join.  Packed sequences may be of any lengths: segments are of the mean's
+// 1,300 us, by 8 segments 630 for both runs, 40 to join.  Packed sequences may be of any lengths: segments are of the mean's
 // size, and numbered as their chunks are, by their rows' place.
 struct Cut {
     int seg;

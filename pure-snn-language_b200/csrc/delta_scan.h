@@ -2,7 +2,7 @@
 // the states' gradients, back (k_delta_back).  Bound by the chain of products of a chunk: a warp
 // has 400 (back 504) matrix instructions and 2,500 others for its 16 columns of 64 steps,
 // and a scheduler two warps at most, since a warp takes 250 registers.  8 x 4,096 steps x 16 heads of
-// 128 x 128 bf16: kernel 560 us, 480 without what the gradient wants, back 620; tensor pipe 39 %, issue
+// 128 x 128 bf16: kernel 560 us, 480 without what the gradient wants, back 615; tensor pipe 39 %, issue
 // 30 %.  Columns could not be cut finer (16 is the instruction's height), and a second warp for the same
 // columns would have to exchange half of K S, of the answers and of U in every chunk.
 #pragma once
